@@ -12,6 +12,11 @@ _LIB = None
 _NATIVE = None
 
 
+# What the training operators call, in the order that the native module expects.
+_TRAIN = ("b2_last_error", "b2_pack8", "b2_unpack8", "b2_gelu8_forward", "b2_gelu8_backward", "b2_weight_grad8_workspace", "b2_weight_grad8",
+          "b2_rotate_heads", "b2_rotate_heads_backward")
+
+
 class B2Config(ctypes.Structure):
     _fields_ = [
         ("transport", ctypes.c_int),
@@ -99,7 +104,7 @@ def check(code):
 
 
 def load_native_calls():
-    """The module with the collective calls (src/python/torch_binding.cc), bound to the library that
+    """The module with the collective calls and the training operators (src/python/torch_binding.cc, torch_ops.cc), bound to the library that
     load() returns. Like the library it is built in-tree, and nothing stands in for it."""
     global _NATIVE
     if _NATIVE is None:
@@ -122,5 +127,6 @@ def load_native_calls():
         lib = load()
         address = [ctypes.cast(f, ctypes.c_void_p).value for f in (lib.b2_collective, lib.b2_last_error)]
         module.bind(address[0], address[1], B200CclError)
+        module.bind_train(B200CclError, tuple(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in _TRAIN))
         _NATIVE = module
     return _NATIVE

@@ -1,0 +1,127 @@
+"""Activations kept in 8 bits for the backward pass.
+
+What a training step keeps between forward and backward bounds the batch of a GPU, and with it the tokens that
+one gradient all-reduce pays for. Here an activation is kept as blocks of 32 neighbouring elements of its last
+axis: a power of two for the block and 8 bits for each element, 33 bytes instead of 64. With the block's largest
+magnitude in ``[2^a, 2^(a+1))`` the step is ``2^q``, ``q = max(a - 6, -126)`` (-24 for fp16), and an element becomes
+
+    x^ = sign(x) * min(round(|x| / 2^q), 127) * 2^q        (ties to even)
+
+which is exact in the activation's own type. Forward results are made from the activation itself and do not change; gradients are
+exactly those of the formula at ``x^``. A block that holds an infinity or NaN reads back as NaN, so that a loss scaler sees it.
+
+The kernels are this library's own (CUDA tensors of float32, float16 or bfloat16); calls run on the current stream of the tensors' device.
+A step captured into a CUDA graph is captured with its backward pass and on one stream, after eager steps of the same parameters have
+been run and their graphs dropped, as for any torch module.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .._lib import load_native_calls
+
+_APPROXIMATIONS = {"none": False, "tanh": True}
+
+
+class Packed8:
+    """An activation in 8 bits, from :func:`pack8`: ``data`` (bytes: the codes, rows padded to whole blocks, then one scale for each
+    block), and the ``shape`` and ``dtype`` that it reads back as."""
+
+    __slots__ = ("data", "shape", "dtype")
+
+    def __init__(self, data, shape, dtype):
+        self.data, self.shape, self.dtype = data, tuple(shape), dtype
+
+    @property
+    def nbytes(self):
+        return self.data.numel()
+
+    def __repr__(self):
+        return f"Packed8(shape={self.shape}, dtype={self.dtype}, nbytes={self.nbytes})"
+
+
+def _packed(what, p):
+    if not isinstance(p, Packed8):
+        raise ValueError(f"{what} must be a Packed8, as pack8() returns it")
+
+
+def pack8(x):
+    """``x`` (any shape with at least one axis, any strides) in 8 bits. No gradient flows through it."""
+    return Packed8(load_native_calls().pack8(x), x.shape, x.dtype)
+
+
+def unpack8(packed):
+    """What :func:`pack8` kept, as a new tensor without gaps."""
+    _packed("unpack8's argument", packed)
+    return load_native_calls().unpack8(packed.data, packed.shape, packed.dtype)
+
+
+class _Gelu8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, tanh):
+        y, kept = load_native_calls().gelu8_forward(x, tanh, True)
+        ctx.save_for_backward(kept)
+        ctx.tanh = tanh
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (kept,) = ctx.saved_tensors
+        return load_native_calls().gelu8_backward(dy, kept, ctx.tanh), None
+
+
+def gelu8(x, approximate="none"):
+    """``torch.nn.functional.gelu(x, approximate)``; the backward pass reads ``x`` in 8 bits, written in the same pass as the result."""
+    if approximate not in _APPROXIMATIONS:
+        raise ValueError(f"unknown approximation '{approximate}'")
+    tanh = _APPROXIMATIONS[approximate]
+    if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
+        return _Gelu8.apply(x, tanh)
+    return load_native_calls().gelu8_forward(x, tanh, False)[0]
+
+
+def weight_grad8(dy, packed, bias=False):
+    """Gradients of a projection ``y = x @ w.T + b`` whose input was kept: ``(dw, db)``, ``db`` None unless ``bias``.
+
+    ``dy``: [..., outputs], ``packed``: of [..., inputs] with the same leading axes and the same dtype. Sums over all leading axes are held in
+    32 bits and rounded once to that dtype (float32: products of full 24-bit numbers). Results do not depend on timing."""
+    _packed("packed", packed)
+    if isinstance(dy, torch.Tensor):
+        if dy.dtype != packed.dtype:
+            raise ValueError(f"dy has dtype {dy.dtype}, the packed input {packed.dtype}")
+        if dy.shape[:-1] != packed.shape[:-1]:
+            raise ValueError(f"dy of shape {tuple(dy.shape)} does not belong to an input of shape {packed.shape}")
+    return load_native_calls().weight_grad8(dy, packed.data, packed.shape[-1], bias)
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        kept = load_native_calls().pack8(x) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else None
+        ctx.save_for_backward(weight, kept)
+        return torch.nn.functional.linear(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        weight, kept = ctx.saved_tensors
+        need_x, need_weight, need_bias = ctx.needs_input_grad
+        dx = dy @ weight if need_x else None
+        dw = db = None
+        if kept is not None:
+            dw, db = load_native_calls().weight_grad8(dy, kept, weight.shape[1], need_bias)
+        return dx, dw if need_weight else None, db
+
+
+def linear8(x, weight, bias=None):
+    """``torch.nn.functional.linear(x, weight, bias)``; the weight's gradient reads ``x`` in 8 bits (:func:`weight_grad8`)."""
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype)
+        with torch.autocast("cuda", enabled=False):
+            return linear8(x, weight, bias)
+    if x.dim() < 2 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear8: an input of shape {tuple(x.shape)} does not go into a weight of shape {tuple(weight.shape)}")
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise ValueError("linear8: x, weight and bias must share one dtype")
+    return _Linear8.apply(x, weight, bias)

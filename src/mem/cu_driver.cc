@@ -46,6 +46,7 @@ Api load() {
     ok &= resolve("cuMemImportFromShareableHandle", &a.MemImportFromShareableHandle);
     a.vmm_ok = ok;
     if (!ok) a.why = "driver does not export the cuMem* virtual memory API";
+    resolve("cuTensorMapEncodeTiled", &a.TensorMapEncodeTiled);
     bool mc = ok;
     mc &= resolve("cuMulticastCreate", &a.MulticastCreate);
     mc &= resolve("cuMulticastAddDevice", &a.MulticastAddDevice);

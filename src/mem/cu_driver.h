@@ -35,6 +35,9 @@ struct Api {
     CUresult (*MulticastUnbind)(CUmemGenericAllocationHandle, CUdevice, size_t, size_t) = nullptr;
     CUresult (*MulticastGetGranularity)(size_t*, const CUmulticastObjectProp*,
                                         CUmulticastGranularity_flags) = nullptr;
+    CUresult (*TensorMapEncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill) = nullptr;
     bool vmm_ok = false;        // every cuMem* pointer above resolved
     bool multicast_ok = false;  // every cuMulticast* pointer resolved
     std::string why;            // reason when vmm_ok is false

@@ -17,6 +17,7 @@
 #include <torch/version.h>
 
 #include "b200ccl/types.h"
+#include "torch_ops.h"
 
 #include <cstdint>
 #include <exception>
@@ -291,7 +292,16 @@ PyObject* bind(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
-PyMethodDef module_methods[] = {{"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+// bind_train(exception class, addresses of the training operators): torch_ops.h
+PyObject* bind_train(PyObject*, PyObject* args) {
+    PyObject *cls = nullptr, *addresses = nullptr;
+    if (!PyArg_ParseTuple(args, "OO!", &cls, &PyTuple_Type, &addresses)) return nullptr;
+    if (!b200ccl::python::bind_train(cls, addresses)) return nullptr;
+    Py_RETURN_NONE;
+}
+
+PyMethodDef module_methods[] = {
+    {"bind", bind, METH_VARARGS, nullptr}, {"bind_train", bind_train, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_b200ccl_torch", nullptr, -1, module_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -299,6 +309,10 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_b200ccl_torch", nullptr, -1, 
 PyMODINIT_FUNC PyInit__b200ccl_torch() {
     PyObject* m = PyModule_Create(&module_def);
     if (m == nullptr) return nullptr;
+    if (PyModule_AddFunctions(m, b200ccl::python::train_methods) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
     PyObject* type = PyType_FromSpec(&caller_spec);
     if (type == nullptr || PyModule_AddObject(m, "Caller", type) < 0) {
         Py_XDECREF(type);
