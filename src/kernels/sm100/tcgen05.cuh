@@ -18,33 +18,44 @@ __device__ __forceinline__ unsigned cluster_rank() {
 }
 // Barrier of all threads of the cluster; what they stored before it is visible after it.
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // ---- barriers -------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mbar_arrive(unsigned bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The barrier at the same place in CTA `rank` of the cluster; release at cluster scope.
+// The barrier at the same place in CTA `rank` of the cluster. What this thread's CTA stored to its shared memory, and this thread has seen, is visible to
+// who waits there; nothing else is ordered, because a release of everything at cluster scope waits for this thread's accesses to global memory too.
 __device__ __forceinline__ void mbar_arrive_at(unsigned bar, unsigned rank) {
     asm volatile(
-        "{\n .reg .b32 remote;\n mapa.shared::cluster.u32 remote, %0, %1;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n}\n" ::"r"(bar),
+        "{\n .reg .b32 remote;\n mapa.shared::cluster.u32 remote, %0, %1;\n fence.release.sync_restrict::shared::cta.cluster;\n"
+        " mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [remote];\n}\n" ::"r"(bar),
         "r"(rank)
         : "memory");
 }
+// kCluster: threads of the other CTA arrive at the barrier too (mbar_arrive_at); otherwise this CTA's threads, its copies and products.
+template <bool kCluster>
 __device__ __forceinline__ bool phase_over(unsigned bar, unsigned parity) {
     unsigned done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 1000;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if constexpr (kCluster) {
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, 1000;\n selp.u32 %0, 1, 0, p;\n"
+            " fence.acquire.sync_restrict::shared::cluster.cluster;\n}\n"
+            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    } else {
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    }
     return done != 0u;
 }
 // Waits for the phase of parity `parity`, for two seconds at most; false then, and in every later wait of the CTA (`failed`, shared).
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_phase(unsigned bar, unsigned parity, volatile unsigned* failed) {
-    if (phase_over(bar, parity)) return true;
+    if (phase_over<kCluster>(bar, parity)) return true;
     unsigned long long t0 = 0;
     for (unsigned polls = 1;; ++polls) {
-        if (phase_over(bar, parity)) return true;
+        if (phase_over<kCluster>(bar, parity)) return true;
         if ((polls & 63u) != 0u) continue;
         const unsigned long long now = global_timer_ns();
         if (t0 == 0) t0 = now;

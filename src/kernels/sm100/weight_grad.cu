@@ -6,16 +6,20 @@
 // next is summed. A pair halves what a tile reads: alone, a CTA with 128 x 256 would draw 80 bytes per cycle from L2 (32 KiB of dY
 // and 8 KiB of codes every 512 cycles, which a step takes), the pair 48 per SM.
 //
-// Roles of a CTA's 16 warps: one thread copies dY by TMA; one thread of the first CTA issues the products, and its counterpart in the second tells it that
+// Roles of a CTA's 16 warps: one thread copies dY and codes by TMA; one thread of the first CTA issues the products, and its counterpart in the second tells it that
 // its dY has come; eight warps widen codes to 16-bit numbers, exactly (block8.cuh), straight into the swizzled operand (per 4 codes: 5 byte
 // permutes and 4 two-wide operations, about a third of the issue slots of a step); four warps write finished tiles; two sum columns of dY
 // for the bias out of shared memory, each tile of features for its own share of the steps, so that every step of dY is summed once.
 //
-// Work is cut evenly, not by tiles: the steps of all tiles stand in one row, and pair i of P takes steps [i S / P, (i+1) S / P). A tile that is
+// P pairs take P whole tiles at a time, as long as there are so many: they are at the same tokens then, and read them from L2 once one of them has.
+// What is left is cut evenly, not by tiles: its steps stand in one row, and pair i takes steps [i S / P, (i+1) S / P). A tile that is
 // cut is summed in pieces, in 32 bits in the workspace, and finish_kernel adds them in the order of tokens: the result does not depend on timing.
+// (All tiles in one row: pairs are at different tokens, and 16384 x 4096 x 4096 draws 3.2 GB from HBM.)
 //
 // fp32: X^ is a bf16 number in any case, and dY is the exact sum of three (its 24 bits cut into eights), so three products of bf16 numbers
-// with 32-bit accumulators give it in full; the three parts follow one another along the summed axis.
+// with 32-bit accumulators give it in full. The tensor cores cut what an addition leaves below 24 bits, so their sums are added to those in
+// memory, rounded, after every 512 tokens: the error does not grow with the number of tokens as it would (8192 tokens: 7.5e-6 of the
+// result's norm without).
 //
 // dY that TMA cannot read (rows or address not at a multiple of 16 bytes) is copied first.
 #include "kernels/sm100/weight_grad.h"
@@ -44,20 +48,24 @@ using u64 = unsigned long long;
 constexpr unsigned kTile = 256;       // features and outputs of a pair's tile
 constexpr unsigned kHalf = 128;       // of one CTA
 constexpr unsigned kStep = 64;        // tokens
-constexpr unsigned kStages = 6;       // steps in shared memory
+constexpr unsigned kStages = 6;       // steps whose dY and codes are in shared memory or on the way
 constexpr unsigned kBlockBytes = kStep * 128;         // 64 elements of every token of a step
 constexpr unsigned kOperandBytes = 2 * kBlockBytes;   // a CTA's half of an operand
-constexpr unsigned kStageBytes = 2 * kOperandBytes;
+constexpr unsigned kCodeBytes = kStep * kHalf;
 constexpr unsigned kThreads = 512;
-constexpr unsigned kTransformWarps = 8, kFirstTransformWarp = 4, kFirstEpilogueWarp = 12;
-constexpr unsigned kAhead = 3;        // steps whose codes are on the way
+constexpr unsigned kFirstTransformWarp = 4, kFirstEpilogueWarp = 12;
+constexpr unsigned kGroups = 4, kGroupWarps = 2;  // of transform warps: a group widens every fourth step, into an operand of its own
+constexpr unsigned kChunkSteps = 8;   // fp32: steps of each part between two additions to the sums in memory
 constexpr unsigned kMaxPairs = 74;    // 148 SMs
 constexpr unsigned kFinishRows = 16;  // outputs of a tile that a CTA of finish_kernel adds up
-constexpr unsigned kShared = kStages * kStageBytes + 1024 /* to the next multiple of 1024 */ + 512;
+// Shared memory, from a multiple of 1024 bytes on: dY of the stages, X^ of the groups, codes of the stages, barriers.
+constexpr unsigned kAtX = kStages * kOperandBytes, kAtCodes = kAtX + kGroups * kOperandBytes, kAtBarriers = kAtCodes + kStages * kCodeBytes;
+constexpr unsigned kShared = kAtBarriers + 512 + 1024;
+static_assert(kShared <= 227 * 1024);
 
 struct alignas(64) WeightGradArgs {
-    CUtensorMap dy;  // [parts][tokens][outputs]
-    const unsigned char* codes;
+    CUtensorMap dy;     // [parts][tokens][outputs]
+    CUtensorMap codes;  // [1][tokens][pitch]
     const unsigned char* scales;
     void* out;
     float* pieces;     // [2 * pairs][256 outputs][256 features]
@@ -65,7 +73,9 @@ struct alignas(64) WeightGradArgs {
     unsigned* status;  // host memory
     u64 pitch;         // bytes of a token's codes
     unsigned tokens, inputs, outputs;
-    unsigned feature_tiles, steps_of_part, steps_of_tile, steps, pairs;
+    unsigned feature_tiles, parts, steps_of_part, steps_of_tile;
+    unsigned pairs, waves;  // of whole tiles
+    unsigned steps;         // of the tiles that are left
 };
 
 struct FinishArgs {
@@ -74,6 +84,7 @@ struct FinishArgs {
     const float* pieces;
     const float* bias;
     unsigned inputs, outputs, feature_tiles, steps_of_tile, steps, pairs;
+    unsigned whole_tiles;  // that come before those that are cut
     unsigned piece_ctas;  // CTAs that add pieces; the others make the bias's gradient
 };
 
@@ -83,8 +94,10 @@ __host__ __device__ inline unsigned first_step(unsigned pair, unsigned steps, un
 struct Barriers {
     u64 dy[kStages];       // this CTA's dY of a stage has come
     u64 dy_other[kStages]; // first CTA: the other's has
-    u64 x[kStages];        // first CTA: both CTAs' X^ is written
+    u64 codes[kStages];    // this CTA's codes of a stage have come
     u64 empty[kStages];    // the stage has been read
+    u64 x[kGroups];        // first CTA: both CTAs' X^ of a group is written
+    u64 x_empty[kGroups];  // it has been read
     u64 sums[2];           // accumulators are complete
     u64 sums_free[2];      // first CTA: both CTAs have written theirs out
     u64 drained;           // first CTA, after a failure
@@ -123,23 +136,80 @@ __device__ __forceinline__ unsigned step_pair(unsigned scale) {
 __device__ __forceinline__ void store_shared16(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ uint4 load_shared16(unsigned at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ unsigned load_shared4(unsigned at) {
     unsigned v;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return v;
 }
 
-// The pieces of a pair: steps of one tile each.
-struct Piece {
-    unsigned tile, from, to, at;  // steps of the tile; `at` in the row of all steps
+// What a pair does, in order: `waves` whole tiles, then its steps of the tiles that are left.
+struct Share {
+    unsigned pair, begin, end;  // in the row of steps that are left
+    unsigned whole, all;        // steps of its whole tiles, of everything
 };
-__device__ __forceinline__ Piece piece_at(const WeightGradArgs& a, unsigned at, unsigned end) {
+__device__ __forceinline__ Share share_of(const WeightGradArgs& a, unsigned pair) {
+    Share s;
+    s.pair = pair;
+    s.begin = first_step(pair, a.steps, a.pairs);
+    s.end = first_step(pair + 1, a.steps, a.pairs);
+    s.whole = a.waves * a.steps_of_tile;
+    s.all = s.whole + (s.end - s.begin);
+    return s;
+}
+// Its n-th step.
+struct Where {
+    unsigned tile, k;
+};
+__device__ __forceinline__ Where where_is(const WeightGradArgs& a, const Share& s, unsigned n) {
+    const bool whole = n < s.whole;
+    const unsigned at = whole ? n : s.begin + (n - s.whole), row = at / a.steps_of_tile;
+    return {whole ? row * a.pairs + s.pair : a.waves * a.pairs + row, at - row * a.steps_of_tile};
+}
+// A run of steps of one tile, from its n-th step on.
+struct Piece {
+    unsigned tile, from, to;  // steps of the tile
+    bool whole;               // this pair sums all of the tile
+    bool later;               // not the pair's first step of the tile
+    unsigned slot;            // of the sums in memory, where it is not whole
+};
+__device__ __forceinline__ Piece piece_at(const WeightGradArgs& a, const Share& s, unsigned n) {
+    const Where w = where_is(a, s, n);
     Piece p;
-    p.at = at;
-    p.tile = at / a.steps_of_tile;
-    p.from = at - p.tile * a.steps_of_tile;
-    p.to = min(a.steps_of_tile, p.from + (end - at));
+    p.tile = w.tile;
+    p.from = w.k;
+    p.to = min(a.steps_of_tile, w.k + (s.all - n));
+    if (n < s.whole) {
+        p.whole = true;
+        p.later = w.k != 0;
+        p.slot = 0;
+    } else {
+        const unsigned tile_at = s.begin + (n - s.whole) - w.k;  // in the row of steps
+        p.whole = tile_at >= s.begin && tile_at + a.steps_of_tile <= s.end;
+        p.later = w.k != 0 && n != s.whole;
+        p.slot = 2u * s.pair + (tile_at <= s.begin ? 0u : 1u);
+    }
     return p;
+}
+// The part of a piece that is summed on the tensor cores alone: all of it, or (fp32) eight steps of each part of dY.
+__device__ __forceinline__ Piece segment_at(const WeightGradArgs& a, const Share& s, unsigned n) {
+    Piece p = piece_at(a, s, n);
+    if (a.parts > 1) p.to = min(p.to, (p.from / (a.parts * kChunkSteps) + 1u) * (a.parts * kChunkSteps));
+    return p;
+}
+// Which part of dY, and which 64 tokens, step k of a tile takes: eight steps of one part, the same eight of the next, and so on.
+struct Spot {
+    unsigned part, step;
+};
+__device__ __forceinline__ Spot spot_of(const WeightGradArgs& a, unsigned k) {
+    if (a.parts == 1) return {0u, k};
+    const unsigned chunk = k / (a.parts * kChunkSteps), in_chunk = k - chunk * (a.parts * kChunkSteps);
+    const unsigned length = min(kChunkSteps, a.steps_of_part - chunk * kChunkSteps), part = in_chunk / length;
+    return {part, chunk * kChunkSteps + in_chunk - part * length};
 }
 
 // T: type of dY and the gradients. kBias: also columns of dY.
@@ -149,19 +219,23 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
     extern __shared__ unsigned char raw[];
     // Swizzled operands start at multiples of 1024 bytes; the same place in both CTAs.
     unsigned char* shared = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
-    Barriers& bars = *reinterpret_cast<Barriers*>(shared + kStages * kStageBytes);
+    Barriers& bars = *reinterpret_cast<Barriers*>(shared + kAtBarriers);
     volatile unsigned* failed = &bars.failed;
     const unsigned base = smem_addr(shared);
     const unsigned warp = threadIdx.x / 32u, lane = threadIdx.x & 31u;
-    const unsigned rank = cluster_rank(), pair = blockIdx.x / 2u;
-    const unsigned begin = first_step(pair, a.steps, a.pairs), end = first_step(pair + 1, a.steps, a.pairs);
+    const unsigned rank = cluster_rank();
+    const Share share = share_of(a, blockIdx.x / 2u);
 
     if (warp == 0 && lane == 0) {
         for (unsigned s = 0; s < kStages; ++s) {
             mbar_init(&bars.dy[s], 1);
             mbar_init(&bars.dy_other[s], 1);
-            mbar_init(&bars.x[s], 2 * kTransformWarps);
-            mbar_init(&bars.empty[s], kBias ? 3 : 1);
+            mbar_init(&bars.codes[s], 1);
+            mbar_init(&bars.empty[s], 1 + kGroupWarps + (kBias ? 2 : 0));
+        }
+        for (unsigned i = 0; i < kGroups; ++i) {
+            mbar_init(&bars.x[i], 2 * kGroupWarps);
+            mbar_init(&bars.x_empty[i], 1);
         }
         for (unsigned i = 0; i < 2; ++i) {
             mbar_init(&bars.sums[i], 1);
@@ -171,7 +245,9 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         bars.failed = 0;
         mbar_fence_init();
         tma_prefetch_map(&a.dy);
+        tma_prefetch_map(&a.codes);
     }
+    __syncwarp();
     if (warp == 1) tmem_alloc_pair(smem_addr(&bars.tmem), 2 * kTile);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tcgen05_fence_before();
@@ -185,28 +261,30 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         if (lane == 0) {
             unsigned n = 0;  // steps so far
             bool ok = true;
-            for (unsigned at = begin; at < end && ok;) {
-                const Piece p = piece_at(a, at, end);
+            while (n < share.all && ok) {
+                const Piece p = piece_at(a, share, n);
                 const int output = (int)((p.tile / a.feature_tiles) * kTile + rank * kHalf);
-                unsigned part = p.from / a.steps_of_part, step = p.from - part * a.steps_of_part;
+                const int feature = (int)((p.tile % a.feature_tiles) * kTile + rank * kHalf);
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
                     const unsigned s = n % kStages;
+                    const Spot spot = spot_of(a, k);
                     ok = wait_phase(bar(bars.empty[s]), ((n / kStages) & 1u) ^ 1u, failed);
                     if (!ok) break;
+                    mbar_arrive_expect_tx(&bars.codes[s], kCodeBytes);
+                    tma_load_box(base + kAtCodes + s * kCodeBytes, &a.codes, feature, (int)(spot.step * kStep), 0, bar(bars.codes[s]));
                     mbar_arrive_expect_tx(&bars.dy[s], kOperandBytes);
-                    const unsigned dst = base + s * kStageBytes + kOperandBytes;
-                    tma_load_box(dst, &a.dy, output, (int)(step * kStep), (int)part, bar(bars.dy[s]));
-                    tma_load_box(dst + kBlockBytes, &a.dy, output + 64, (int)(step * kStep), (int)part, bar(bars.dy[s]));
-                    if (++step == a.steps_of_part) { step = 0; ++part; }
+                    const unsigned dst = base + s * kOperandBytes;
+                    tma_load_box(dst, &a.dy, output, (int)(spot.step * kStep), (int)spot.part, bar(bars.dy[s]));
+                    tma_load_box(dst + kBlockBytes, &a.dy, output + 64, (int)(spot.step * kStep), (int)spot.part, bar(bars.dy[s]));
                 }
-                at += p.to - p.from;
             }
             // Copies have landed and stages been given back before the CTA ends, after a failure too.
             if (ok) {
                 for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i) wait_phase(bar(bars.empty[i % kStages]), (i / kStages) & 1u, failed);
             } else {
                 for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i)
-                    for (unsigned polls = 0; polls < 1000u && !phase_over(bar(bars.dy[i % kStages]), (i / kStages) & 1u); ++polls) {}
+                    for (unsigned polls = 0; polls < 1000u && !(phase_over<false>(bar(bars.dy[i % kStages]), (i / kStages) & 1u) &&
+                                                                 phase_over<false>(bar(bars.codes[i % kStages]), (i / kStages) & 1u)); ++polls) {}
             }
         }
     } else if (warp == 1) {
@@ -214,35 +292,35 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             const unsigned shape = product_by_rows(kTile, kTile, kBf16);
             unsigned n = 0, pieces = 0;
             bool ok = true;
-            for (unsigned at = begin; at < end && ok; ++pieces) {
-                const Piece p = piece_at(a, at, end);
+            for (; n < share.all && ok; ++pieces) {
+                const Piece p = segment_at(a, share, n);
                 const unsigned buffer = pieces & 1u;
-                ok = wait_phase(bar(bars.sums_free[buffer]), ((pieces >> 1) & 1u) ^ 1u, failed);
+                ok = wait_phase<true>(bar(bars.sums_free[buffer]), ((pieces >> 1) & 1u) ^ 1u, failed);
                 if (!ok) break;
                 tcgen05_fence_after();
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
-                    const unsigned s = n % kStages, parity = (n / kStages) & 1u;
-                    ok = wait_phase(bar(bars.dy[s]), parity, failed) && wait_phase(bar(bars.dy_other[s]), parity, failed) &&
-                         wait_phase(bar(bars.x[s]), parity, failed);
+                    const unsigned s = n % kStages, parity = (n / kStages) & 1u, group = n % kGroups;
+                    ok = wait_phase(bar(bars.dy[s]), parity, failed) && wait_phase<true>(bar(bars.dy_other[s]), parity, failed) &&
+                         wait_phase<true>(bar(bars.x[group]), (n / kGroups) & 1u, failed);
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const std::uint64_t x = operand_by_rows(base + s * kStageBytes, kBlockBytes);
-                    const std::uint64_t dy = operand_by_rows(base + s * kStageBytes + kOperandBytes, kBlockBytes);
+                    const std::uint64_t x = operand_by_rows(base + kAtX + group * kOperandBytes, kBlockBytes);
+                    const std::uint64_t dy = operand_by_rows(base + s * kOperandBytes, kBlockBytes);
 #pragma unroll
                     for (unsigned i = 0; i < kStep / 16; ++i)  // 16 tokens are 2048 bytes
                         mma_pair(tmem + buffer * kTile, x + i * (2048 >> 4), dy + i * (2048 >> 4), shape, k > p.from || i > 0);
+                    commit_pair(bar(bars.x_empty[group]));
                     commit_pair(bar(bars.empty[s]));
                 }
                 if (!ok) break;
                 commit_pair(bar(bars.sums[buffer]));
-                at += p.to - p.from;
             }
             if (!ok) {  // products under way read shared memory of both CTAs
                 commit_pair(bar(bars.drained));
-                for (unsigned polls = 0; polls < 1000u && !phase_over(bar(bars.drained), 0); ++polls) {}
+                for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
             }
         } else if (lane == 0) {
-            for (unsigned n = 0; n < end - begin; ++n) {
+            for (unsigned n = 0; n < share.all; ++n) {
                 if (!wait_phase(bar(bars.dy[n % kStages]), (n / kStages) & 1u, failed)) break;
                 mbar_arrive_at(bar(bars.dy_other[n % kStages]), 0);
             }
@@ -252,16 +330,16 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             const unsigned column = (warp - 2u) * 64u + lane * 2u;  // of this CTA's 128 outputs
             unsigned n = 0;
             bool ok = true;
-            for (unsigned at = begin; at < end && ok;) {
-                const Piece p = piece_at(a, at, end);
-                const unsigned share = p.tile % a.feature_tiles;
+            while (n < share.all && ok) {
+                const Piece p = piece_at(a, share, n);
+                const unsigned turn = p.tile % a.feature_tiles;
                 float x = 0.0f, y = 0.0f;
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
                     const unsigned s = n % kStages;
                     ok = __all_sync(0xffffffffu, wait_phase(bar(bars.dy[s]), (n / kStages) & 1u, failed));
                     if (!ok) break;
-                    if (k % a.feature_tiles == share) {
-                        const unsigned from = base + s * kStageBytes + kOperandBytes + (warp - 2u) * kBlockBytes;
+                    if (k % a.feature_tiles == turn) {
+                        const unsigned from = base + s * kOperandBytes + (warp - 2u) * kBlockBytes;
 #pragma unroll 16
                         for (unsigned t = 0; t < kStep; ++t) {
                             const unsigned w = load_shared4(from + t * 128u + (((lane / 4u) ^ (t & 7u)) * 16u) + (lane & 3u) * 4u);
@@ -274,98 +352,95 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                     if (lane == 0) mbar_arrive(bar(bars.empty[s]));
                 }
                 if (!ok) break;
-                float* to = a.bias + (u64)(p.from == 0 ? p.tile : a.feature_tiles * ((a.outputs + kTile - 1) / kTile) + pair) * kTile;
+                float* to = a.bias + (u64)(p.from == 0 ? p.tile : a.feature_tiles * ((a.outputs + kTile - 1) / kTile) + share.pair) * kTile;
                 *reinterpret_cast<float2*>(to + rank * kHalf + column) = make_float2(x, y);
-                at += p.to - p.from;
             }
         }
     } else if (warp < kFirstEpilogueWarp) {
-        const unsigned tid = threadIdx.x - kFirstTransformWarp * 32u;
-        const unsigned chunk = tid & 7u, row = tid >> 3;  // 16 features of a token; the tokens row and row + 32 of a step
-        uint4 code[kAhead][2];
-        unsigned scale[kAhead][2];
-        // Where the next codes are read.
-        unsigned next = begin, tile = begin / a.steps_of_tile, k = begin - tile * a.steps_of_tile;
-        unsigned step = k % a.steps_of_part;
-        unsigned feature = (tile % a.feature_tiles) * kTile + rank * kHalf + chunk * 16u;
-        const auto load = [&](uint4(&c)[2], unsigned(&sc)[2]) {
+        const unsigned group = (warp - kFirstTransformWarp) / kGroupWarps;
+        const unsigned tid = threadIdx.x & (kGroupWarps * 32u - 1u);
+        const unsigned chunk = tid & 7u, row = tid >> 3;  // 16 features of the tokens row, row + 8, ... of a step
+        // Scales are read a turn of the group ahead, straight from memory (a step's are 4 bytes of each of 64 tokens).
+        unsigned scale[8];
+        const auto load_scales = [&](unsigned n) {
+            const Where w = where_is(a, share, n);
+            const u64 token = (u64)spot_of(a, w.k).step * kStep + row;
+            const unsigned feature = (w.tile % a.feature_tiles) * kTile + rank * kHalf + chunk * 16u;
+            const unsigned char* from = a.scales + (token * a.pitch + feature) / kBlock8;
 #pragma unroll
-            for (unsigned u = 0; u < 2; ++u) {
-                const u64 token = (u64)step * kStep + row + u * 32u;
-                const bool there = token < a.tokens && feature < a.pitch;
-                c[u] = there ? *reinterpret_cast<const uint4*>(a.codes + token * a.pitch + feature) : make_uint4(0u, 0u, 0u, 0u);
-                sc[u] = there ? a.scales[(token * a.pitch + feature) / kBlock8] : 127u;
-            }
-            ++next;
-            if (++step == a.steps_of_part) step = 0;
-            if (++k == a.steps_of_tile) {
-                k = 0;
-                ++tile;
-                feature = (tile % a.feature_tiles) * kTile + rank * kHalf + chunk * 16u;
-            }
+            for (unsigned u = 0; u < 8; ++u)
+                scale[u] = token + 8u * u < a.tokens && feature < a.pitch ? from[8u * u * (a.pitch / kBlock8)] : 127u;
         };
+        if (group < share.all) load_scales(group);
+        // A chunk's two halves go to columns of 16 bytes, the odd one first for the second block of 64 features: eight lanes then write to eight
+        // different columns of the shared memory's banks. (Eight tokens are 1024 bytes, so the swizzle is the same for all of a lane's.)
+        const unsigned odd = chunk >> 2, column = (chunk & 3u) * 2u;
+        const unsigned block = base + kAtX + group * kOperandBytes + odd * kBlockBytes + row * 128u;
+        const unsigned first = block + (((column + odd) ^ row) * 16u), second = block + (((column + (odd ^ 1u)) ^ row) * 16u);
+        const unsigned codes = base + kAtCodes + row * kHalf + chunk * 16u;
+        unsigned n = group;
+        for (; n < share.all; n += kGroups) {
+            const unsigned s = n % kStages;
+            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.codes[s]), (n / kStages) & 1u, failed) &&
+                                             wait_phase(bar(bars.x_empty[group]), ((n / kGroups) & 1u) ^ 1u, failed)))
+                break;
 #pragma unroll
-        for (unsigned i = 0; i < kAhead; ++i)
-            if (next < end) load(code[i], scale[i]);
-        // The two halves of a chunk go out in turn, odd ones first for the second block of 64 features: eight lanes then write to eight
-        // different 16-byte columns of the shared memory's banks.
-        const unsigned block = base + (chunk >> 2) * kBlockBytes, odd = chunk >> 2;
-        const unsigned column0 = ((chunk & 3u) * 2u + odd), column1 = ((chunk & 3u) * 2u + (odd ^ 1u));
-        unsigned n = 0;
-        bool ok = true;
-        for (unsigned at = begin; at < end && ok; at += kAhead) {
-#pragma unroll
-            for (unsigned i = 0; i < kAhead; ++i) {
-                if (at + i < end && ok) {
-                    const unsigned s = n % kStages;
-                    ok = __all_sync(0xffffffffu, wait_phase(bar(bars.empty[s]), ((n / kStages) & 1u) ^ 1u, failed));
-                    if (!ok) break;
-#pragma unroll
-                    for (unsigned u = 0; u < 2; ++u) {
-                        const unsigned t = row + u * 32u;
-                        const unsigned s2 = step_pair<kBf16>(scale[i][u]);
-                        const uint2 w0 = widen4<kBf16>(code[i][u].x, s2), w1 = widen4<kBf16>(code[i][u].y, s2);
-                        const uint2 w2 = widen4<kBf16>(code[i][u].z, s2), w3 = widen4<kBf16>(code[i][u].w, s2);
-                        const unsigned to = block + s * kStageBytes + t * 128u;
-                        const unsigned c0 = to + ((column0 ^ (t & 7u)) * 16u), c1 = to + ((column1 ^ (t & 7u)) * 16u);
-                        if (odd) {
-                            store_shared16(c0, w2.x, w2.y, w3.x, w3.y);
-                            store_shared16(c1, w0.x, w0.y, w1.x, w1.y);
-                        } else {
-                            store_shared16(c0, w0.x, w0.y, w1.x, w1.y);
-                            store_shared16(c1, w2.x, w2.y, w3.x, w3.y);
-                        }
-                    }
-                    fence_shared_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_at(bar(bars.x[s]), 0);
-                    if (next < end) load(code[i], scale[i]);
-                    ++n;
-                }
+            for (unsigned u = 0; u < 8; ++u) {
+                const uint4 c = load_shared16(codes + s * kCodeBytes + u * (8u * kHalf));
+                const unsigned s2 = step_pair<kBf16>(scale[u]);
+                const uint2 w0 = widen4<kBf16>(odd ? c.z : c.x, s2), w1 = widen4<kBf16>(odd ? c.w : c.y, s2);
+                const uint2 w2 = widen4<kBf16>(odd ? c.x : c.z, s2), w3 = widen4<kBf16>(odd ? c.y : c.w, s2);
+                store_shared16(first + u * 1024u, w0.x, w0.y, w1.x, w1.y);
+                store_shared16(second + u * 1024u, w2.x, w2.y, w3.x, w3.y);
             }
+            fence_shared_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive_at(bar(bars.x[group]), 0);
+                mbar_arrive(bar(bars.empty[s]));
+            }
+            if (n + kGroups < share.all) load_scales(n + kGroups);  // (before the fence, the fence would wait for them)
         }
+        // The arrival that gives the operand back comes before the CTA ends.
+        if (n >= share.all && n != group) wait_phase(bar(bars.x_empty[group]), (n / kGroups - 1u) & 1u, failed);
     } else {
         const unsigned quarter = warp & 3u;  // lanes of tensor memory that this warp reaches
         const unsigned in_tile = rank * kHalf + quarter * 32u + lane;
-        unsigned pieces = 0;
-        for (unsigned at = begin; at < end; ++pieces) {
-            const Piece p = piece_at(a, at, end);
+        unsigned pieces = 0, n = 0;
+        for (; n < share.all; ++pieces) {
+            const Piece p = segment_at(a, share, n);
             const unsigned buffer = pieces & 1u;
             if (!__all_sync(0xffffffffu, wait_phase(bar(bars.sums[buffer]), (pieces >> 1) & 1u, failed))) break;
             tcgen05_fence_after();
-            const bool whole = p.from == 0 && p.to == a.steps_of_tile;
             const unsigned feature = (p.tile % a.feature_tiles) * kTile + in_tile;
             const unsigned output0 = (p.tile / a.feature_tiles) * kTile;
-            float* piece = a.pieces + (u64)(2u * pair + (p.at == begin ? 0u : 1u)) * (kTile * kTile) + in_tile;
+            float* piece = a.pieces + (u64)p.slot * (kTile * kTile) + in_tile;
             for (unsigned c = 0; c < kTile; c += 32u) {
                 float f[32];
+                __syncwarp();
                 tmem_load32(tmem + buffer * kTile + c + (quarter * 32u << 16), f);
-                if (whole) {
-                    T* out = static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature;
+                if (p.whole) {
+                    if (feature < a.inputs) {
+                        T* out = static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature;
+                        const unsigned there = output0 + c < a.outputs ? min(32u, a.outputs - (output0 + c)) : 0u;
+                        if constexpr (sizeof(T) == 4) {
+                            if (p.later) {
 #pragma unroll
-                    for (unsigned j = 0; j < 32; ++j)
-                        if (feature < a.inputs && output0 + c + j < a.outputs) out[(u64)j * a.inputs] = Elem<T>::from_f(f[j]);
+                                for (unsigned j = 0; j < 32; ++j)
+                                    if (j < there) f[j] += out[(u64)j * a.inputs];
+                            }
+                        }
+#pragma unroll
+                        for (unsigned j = 0; j < 32; ++j)
+                            if (j < there) out[(u64)j * a.inputs] = Elem<T>::from_f(f[j]);
+                    }
                 } else {
+                    if constexpr (sizeof(T) == 4) {
+                        if (p.later) {
+#pragma unroll
+                            for (unsigned j = 0; j < 32; ++j) f[j] += piece[(u64)(c + j) * kTile];
+                        }
+                    }
 #pragma unroll
                     for (unsigned j = 0; j < 32; ++j) piece[(u64)(c + j) * kTile] = f[j];
                 }
@@ -373,14 +448,16 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_at(bar(bars.sums_free[buffer]), 0);
-            at += p.to - p.from;
+            n += p.to - p.from;
         }
     }
     __syncthreads();
     if (threadIdx.x == 0 && *failed != 0u) *static_cast<volatile unsigned*>(a.status) = 1u;
+    __syncwarp();
     tcgen05_fence_before();
     cluster_sync();  // nothing of this CTA is read or arrived at by the other any more
     tcgen05_fence_after();
+    __syncwarp();
     if (warp == 1) tmem_free_pair(tmem, 2 * kTile);
 }
 
@@ -394,7 +471,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         constexpr unsigned kParts = kTile / kFinishRows;
         const unsigned border = blockIdx.x / kParts + 1u, part = blockIdx.x % kParts;
         const unsigned at = first_step(border, a.steps, a.pairs);
-        const unsigned tile = at / a.steps_of_tile, from = tile * a.steps_of_tile;
+        const unsigned row = at / a.steps_of_tile, from = row * a.steps_of_tile, tile = a.whole_tiles + row;
         const unsigned before = first_step(border - 1u, a.steps, a.pairs);
         if (at == from || before > from) return;
         const unsigned output0 = (tile / a.feature_tiles) * kTile + part * kFinishRows, feature0 = (tile % a.feature_tiles) * kTile;
@@ -405,6 +482,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
             const auto read = [&](unsigned slot) { return *reinterpret_cast<const float4*>(a.pieces + (u64)slot * (kTile * kTile) + in_piece); };
             float4 sum = read(2u * (border - 1u) + (before == from ? 0u : 1u));
             for (unsigned p = border; p < a.pairs && first_step(p, a.steps, a.pairs) < to; ++p) {
+                if (first_step(p, a.steps, a.pairs) == first_step(p + 1u, a.steps, a.pairs)) continue;  // it has no step
                 const float4 v = read(2u * p);
                 sum.x += v.x;
                 sum.y += v.y;
@@ -421,16 +499,26 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         }
         return;
     }
-    const unsigned output_tile = blockIdx.x - a.piece_ctas, output = output_tile * kTile + threadIdx.x;
+    // 32 outputs of a tile per CTA, eight threads for each.
+    const unsigned index = blockIdx.x - a.piece_ctas, output_tile = index / (kTile / 32u), column = (index % (kTile / 32u)) * 32u + (threadIdx.x & 31u);
     const unsigned tiles = a.feature_tiles * ((a.outputs + kTile - 1) / kTile);
     float sum = 0.0f;
-    for (unsigned m = 0; m < a.feature_tiles; ++m) {
-        const unsigned tile = output_tile * a.feature_tiles + m, from = tile * a.steps_of_tile, to = from + a.steps_of_tile;
-        sum += a.bias[(u64)tile * kTile + threadIdx.x];
+    for (unsigned m = threadIdx.x / 32u; m < a.feature_tiles; m += 8u) {
+        const unsigned tile = output_tile * a.feature_tiles + m;
+        sum += a.bias[(u64)tile * kTile + column];
+        if (tile < a.whole_tiles) continue;
+        const unsigned from = (tile - a.whole_tiles) * a.steps_of_tile, to = from + a.steps_of_tile;
         unsigned p = (unsigned)((u64)from * a.pairs / a.steps);
         while (p < a.pairs && first_step(p, a.steps, a.pairs) <= from) ++p;
-        for (; p < a.pairs && first_step(p, a.steps, a.pairs) < to; ++p) sum += a.bias[(u64)(tiles + p) * kTile + threadIdx.x];
+        for (; p < a.pairs && first_step(p, a.steps, a.pairs) < to; ++p)
+            if (first_step(p, a.steps, a.pairs) != first_step(p + 1u, a.steps, a.pairs)) sum += a.bias[(u64)(tiles + p) * kTile + column];
     }
+    __shared__ float sums[8][32];
+    sums[threadIdx.x / 32u][threadIdx.x & 31u] = sum;
+    __syncthreads();
+    if (threadIdx.x >= 32u) return;
+    for (unsigned i = 1; i < 8; ++i) sum += sums[i][threadIdx.x];
+    const unsigned output = output_tile * kTile + column;
     if (output < a.outputs) static_cast<T*>(a.bias_out)[output] = Elem<T>::from_f(sum);
 }
 
@@ -475,7 +563,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ La
 }
 
 struct Plan {
-    unsigned parts = 1, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0;
+    unsigned parts = 1, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0;
     bool copied = false;
     std::size_t pieces_at = 0, bias_at = 0, bytes = 0;
 };
@@ -534,11 +622,12 @@ Plan plan_of(const WeightGradCall& c) {
                "weight_grad8: too many tokens, inputs and outputs for one call");
     p.steps_of_part = (unsigned)steps_of_part;
     p.steps_of_tile = p.steps_of_part * p.parts;
-    p.steps = p.steps_of_tile * (unsigned)tiles;
     const int device = current_device();
     prepare_device(device);
     // Four steps of a pair at least: less, and the pieces cost more than the sums (a piece is 256 KiB to write and read again).
-    p.pairs = std::max(1u, std::min(pairs_of_device(device), p.steps / 4u));
+    p.pairs = (unsigned)std::max<u64>(1, std::min<u64>(pairs_of_device(device), tiles * p.steps_of_tile / 4));
+    p.waves = (unsigned)tiles / p.pairs;
+    p.steps = ((unsigned)tiles - p.waves * p.pairs) * p.steps_of_tile;
     const std::size_t copy = p.copied ? (std::size_t)p.parts * c.tokens * p.pitch * 2 : 0;
     p.pieces_at = (copy + 255) / 256 * 256;
     p.bias_at = p.pieces_at + (std::size_t)2 * p.pairs * kTile * kTile * sizeof(float);
@@ -584,28 +673,32 @@ void launch(const WeightGradCall& c, const Plan& p) {
     WeightGradArgs a;
     const auto encode = cu::api().TensorMapEncodeTiled;
     if (encode == nullptr) throw std::runtime_error("weight_grad8: the driver does not export cuTensorMapEncodeTiled");
-    const cuuint64_t extent[3] = {c.outputs, c.tokens, p.parts};
-    const cuuint64_t strides[2] = {row_bytes, row_bytes * c.tokens};
-    const cuuint32_t box[3] = {64, kStep, 1}, element_strides[3] = {1, 1, 1};
-    cu::check(encode(&a.dy, sizeof(T) == 2 && std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                     const_cast<void*>(dy), extent, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
-              "weight_grad8: tensor map of dy");
-    a.codes = c.codes;
+    const auto map = [&](CUtensorMap* m, CUtensorMapDataType type, const void* data, u64 columns, u64 rows, u64 planes, u64 bytes, cuuint32_t box_columns,
+                         CUtensorMapSwizzle swizzle, const char* what) {
+        const cuuint64_t extent[3] = {columns, rows, planes}, strides[2] = {bytes, bytes * rows};
+        const cuuint32_t box[3] = {box_columns, kStep, 1}, element_strides[3] = {1, 1, 1};
+        cu::check(encode(m, type, 3, const_cast<void*>(data), extent, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE), what);
+    };
+    map(&a.dy, std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, c.outputs, c.tokens, p.parts, row_bytes, 64,
+        CU_TENSOR_MAP_SWIZZLE_128B, "weight_grad8: tensor map of dy");
+    a.pitch = (c.inputs + kBlock8 - 1) / kBlock8 * kBlock8;
+    map(&a.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.codes, a.pitch, c.tokens, 1, a.pitch, kHalf, CU_TENSOR_MAP_SWIZZLE_NONE, "weight_grad8: tensor map of the codes");
     a.scales = c.scales;
     a.out = c.weight_grad;
     a.pieces = reinterpret_cast<float*>(workspace + p.pieces_at);
     a.bias = c.bias_grad != nullptr ? reinterpret_cast<float*>(workspace + p.bias_at) : nullptr;
     a.status = status_word();
-    a.pitch = (c.inputs + kBlock8 - 1) / kBlock8 * kBlock8;
     a.tokens = (unsigned)c.tokens;
     a.inputs = (unsigned)c.inputs;
     a.outputs = (unsigned)c.outputs;
     a.feature_tiles = p.feature_tiles;
+    a.parts = p.parts;
     a.steps_of_part = p.steps_of_part;
     a.steps_of_tile = p.steps_of_tile;
     a.steps = p.steps;
     a.pairs = p.pairs;
+    a.waves = p.waves;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(2 * p.pairs);
     config.blockDim = dim3(kThreads);
@@ -634,8 +727,9 @@ void launch(const WeightGradCall& c, const Plan& p) {
     f.steps_of_tile = p.steps_of_tile;
     f.steps = p.steps;
     f.pairs = p.pairs;
+    f.whole_tiles = p.waves * p.pairs;
     f.piece_ctas = cut ? (p.pairs - 1) * (kTile / kFinishRows) : 0;
-    const unsigned grid = f.piece_ctas + (c.bias_grad != nullptr ? p.output_tiles : 0);
+    const unsigned grid = f.piece_ctas + (c.bias_grad != nullptr ? p.output_tiles * (kTile / 32) : 0);
     B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<T>, dim3(grid), 256, 0, c.stream, f));
 }
 
