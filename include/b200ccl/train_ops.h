@@ -65,7 +65,7 @@ typedef struct b2_heads {
     void* weight_grad;      /* backward: [dim] */
     void* partial;          /* backward: B2_HEAD_GRAD_PARTIALS * dim floats of scratch */
 } b2_heads;
-#define B2_HEAD_GRAD_PARTIALS 592
+#define B2_HEAD_GRAD_PARTIALS 296
 typedef struct b2_rotation {
     int dtype;
     long long batch, tokens;

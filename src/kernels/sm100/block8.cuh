@@ -6,12 +6,15 @@
 // smallest subnormal): a kept value is the same number wherever it is read, in matrix products too. |x^ - x| <= 2^(q-1), for the few
 // elements above 127.5 steps 2^q: at most 2^-6 of the block's largest magnitude, 2^-7 where nothing is clamped.
 //
-// A code is sign << 7 | m and not two's complement because 0x4300 | m is the bf16 number 128 + m: a code widens without a
-// conversion instruction. The scale byte is q + 127, so that it is the exponent field of the step; 255 marks a block that held an
+// A code is sign << 7 | m and not two's complement, so that a code widens without a conversion instruction: as a bf16 number, sign << 15 | m is
+// +-m 2^-133, exactly. And rounding needs none either: |x| 2^-q + 128 in bf16 (+ 1024 in fp16) is rounded to a whole number by its own
+// last bit, ties to even. Both work on two elements at once. The scale byte is q + 127, so that it is the exponent field of the step; 255 marks a block that held an
 // infinity or NaN: its codes are 0 and 0 * inf = NaN, so that every gradient made from the block says so.
 #pragma once
 
 #include "kernels/sm100/vec.cuh"
+
+#include <type_traits>
 
 namespace b200ccl::dev {
 
@@ -56,6 +59,74 @@ __device__ __forceinline__ unsigned encode8x4(const float* f, float inverse) {
 }
 // A block that is not finite: x * 0 would be NaN, whose low bits are anything.
 __device__ __forceinline__ unsigned finite8(unsigned word, unsigned scale) { return scale == 255u ? 0u : word; }
+
+// ---- 16-bit types, two elements in a word ----------------------------------------------------------------
+__device__ __forceinline__ __nv_bfloat162 as_b2(unsigned w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+__device__ __forceinline__ __half2 as_h2(unsigned w) { return *reinterpret_cast<__half2*>(&w); }
+__device__ __forceinline__ unsigned bits_of(__nv_bfloat162 v) { return *reinterpret_cast<unsigned*>(&v); }
+__device__ __forceinline__ unsigned bits_of(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
+
+// The larger magnitude of each half so far, and of both at the end, as fp32.
+__device__ __forceinline__ unsigned larger_magnitudes(unsigned so_far, unsigned word) { return __vmaxu2(so_far, word & 0x7fff7fffu); }
+template <typename T>
+__device__ __forceinline__ unsigned magnitude_of_pair(unsigned pair) {
+    const unsigned m = max(pair & 0xffffu, pair >> 16);
+    if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+    return m << 16;
+}
+
+// 2^-q for words of T: bf16 in one factor; fp16, which does not reach 2^24, in two.
+template <typename T>
+struct Inverse16 {
+    unsigned a, b;
+    __device__ __forceinline__ explicit Inverse16(unsigned scale) {
+        if constexpr (std::is_same_v<T, __half>) {
+            const int e = 127 - (int)scale, first = e >> 1, second = e - first;  // e from -9 to 24
+            a = scale == 255u ? 0u : (unsigned)(15 + first) * 0x04000400u;
+            b = scale == 255u ? 0u : (unsigned)(15 + second) * 0x04000400u;
+        } else {
+            a = scale == 255u ? 0u : (254u - scale) * 0x00800080u;
+            b = 0u;
+        }
+    }
+};
+// Codes of the four elements of two words (of a block that is finite).
+template <typename T>
+__device__ __forceinline__ unsigned encode8x4(unsigned x, unsigned y, const Inverse16<T>& inverse) {
+    unsigned mx, my;
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 top = as_h2(0x647f647fu), magic = as_h2(0x64006400u);  // 1024 + 127, 1024
+        mx = bits_of(__hmin2(__hfma2(__hmul2(__habs2(as_h2(x)), as_h2(inverse.a)), as_h2(inverse.b), magic), top));
+        my = bits_of(__hmin2(__hfma2(__hmul2(__habs2(as_h2(y)), as_h2(inverse.a)), as_h2(inverse.b), magic), top));
+    } else {
+        const __nv_bfloat162 top = as_b2(0x437f437fu), magic = as_b2(0x43004300u);  // 128 + 127, 128
+        mx = bits_of(__hmin2(__hfma2(__habs2(as_b2(x)), as_b2(inverse.a), magic), top));
+        my = bits_of(__hmin2(__hfma2(__habs2(as_b2(y)), as_b2(inverse.a), magic), top));
+    }
+    return __byte_perm(mx, my, 0x6420) | (__byte_perm(x, y, 0x7531) & 0x80808080u);
+}
+// What widens codes to words of T. bf16: 2^(q + 6), behind a factor 2^127. fp16: 2^q.
+template <typename T>
+__device__ __forceinline__ unsigned step16(unsigned scale) {
+    if constexpr (std::is_same_v<T, __half>) return bits_of(__float2half2_rn(step8(scale)));
+    return min(scale + 6u, 255u) * 0x00800080u;
+}
+// Four codes as two words of T.
+template <typename T>
+__device__ __forceinline__ uint2 widen8x4(unsigned word, unsigned step) {
+    const unsigned m = word & 0x7f7f7f7fu, sign = word & 0x80808080u;
+    if constexpr (std::is_same_v<T, __half>) {
+        // 1024 + m, less 1024, times the step: fp16 has no exponents left for the other way.
+        const __half2 off = as_h2(0x64006400u);
+        const unsigned a = bits_of(__hmul2(__hsub2(as_h2(__byte_perm(m, 0x64646464u, 0x4140)), off), as_h2(step)));
+        const unsigned b = bits_of(__hmul2(__hsub2(as_h2(__byte_perm(m, 0x64646464u, 0x4342)), off), as_h2(step)));
+        return make_uint2(a | __byte_perm(sign, 0u, 0x1404), b | __byte_perm(sign, 0u, 0x3424));
+    } else {
+        const __nv_bfloat162 far = as_b2(0x7f007f00u);  // 2^127
+        return make_uint2(bits_of(__hmul2(__hmul2(as_b2(__byte_perm(m, sign, 0x5140)), far), as_b2(step))),
+                          bits_of(__hmul2(__hmul2(as_b2(__byte_perm(m, sign, 0x7362)), far), as_b2(step))));
+    }
+}
 
 __device__ __forceinline__ unsigned magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 

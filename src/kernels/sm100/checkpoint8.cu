@@ -11,8 +11,10 @@
 
 #include "kernels/sm100/block8.cuh"
 #include "kernels/sm100/launch.h"
+#include "kernels/sm100/pair32.cuh"
 
 #include <cstdint>
+#include <type_traits>
 
 namespace b200ccl::kernels {
 
@@ -34,85 +36,169 @@ struct Kept8Args {
     unsigned items;            // half blocks (flat) or blocks (ragged) of all rows
 };
 
-// exp(-x^2/2) and 1 - Phi(|x|).
-__device__ __forceinline__ void normal_tail(float x, float* density, float* tail) {
-    const float t = __fdividef(1.0f, fmaf(fabsf(x), 0.28f, 1.0f));
-    float p = 0.02585814922f;
-    p = fmaf(p, t, -0.09804277882f);
-    p = fmaf(p, t, 0.09953258518f);
-    p = fmaf(p, t, -0.01241061024f);
-    p = fmaf(p, t, 0.07559080114f);
-    p = fmaf(p, t, 0.08288812189f);
-    p = fmaf(p, t, 0.1031858347f);
-    p = fmaf(p, t, 0.1116940188f);
-    p = fmaf(p, t, 0.1117039230f);
-    *density = __expf(-0.5f * x * x);
-    *tail = *density * p * t;
+// exp(-x^2/2) and 1 - Phi(|x|) of two numbers.
+struct Tail {
+    Pair32 density, tail;
+};
+__device__ __forceinline__ Tail normal_tail(float2 x) {
+    const Pair32 d = fma2(pair32(fabsf(x.x), fabsf(x.y)), both32(0.28f), both32(1.0f));
+    const float2 f = apart(d);
+    const Pair32 t = pair32(reciprocal_fast(f.x), reciprocal_fast(f.y));
+    Pair32 p = both32(0.02585814922f);
+    p = fma2(p, t, both32(-0.09804277882f));
+    p = fma2(p, t, both32(0.09953258518f));
+    p = fma2(p, t, both32(-0.01241061024f));
+    p = fma2(p, t, both32(0.07559080114f));
+    p = fma2(p, t, both32(0.08288812189f));
+    p = fma2(p, t, both32(0.1031858347f));
+    p = fma2(p, t, both32(0.1116940188f));
+    p = fma2(p, t, both32(0.1117039230f));
+    const Pair32 v = pair32(x.x, x.y);
+    const float2 e = apart(mul2(v, mul2(v, both32(-0.7213475204f))));  // -x^2 / 2 * log2(e)
+    Tail r;
+    r.density = pair32(exp2_fast(e.x), exp2_fast(e.y));
+    r.tail = mul2(r.density, mul2(p, t));
+    return r;
 }
 
 constexpr float kTanhSlope = 0.7978845608f, kTanhCube = 0.044715f;  // tanh(sqrt(2/pi) (x + 0.044715 x^3))
 
+// e = exp(-2|u|) and s = 1 / (1 + e) of two numbers: (1 + tanh u) / 2 is s for u >= 0, e s below. u grows without bound, e ends at 0.
+struct Logistic {
+    float2 e, s;
+    Pair32 square;
+};
+__device__ __forceinline__ Logistic logistic(float2 x) {
+    Logistic r;
+    const Pair32 v = pair32(x.x, x.y);
+    r.square = mul2(v, v);
+    const float2 u = apart(mul2(v, fma2(r.square, both32(kTanhCube), both32(1.0f))));
+    constexpr float kSlope = -2.0f * kTanhSlope * 1.442695041f;
+    r.e = make_float2(exp2_fast(kSlope * fabsf(u.x)), exp2_fast(kSlope * fabsf(u.y)));
+    r.s = make_float2(reciprocal_fast(1.0f + r.e.x), reciprocal_fast(1.0f + r.e.y));
+    return r;
+}
+
 template <Activation kAct>
-__device__ __forceinline__ float activate(float x) {
+__device__ __forceinline__ float2 activate(float2 x) {
+    const Pair32 v = pair32(x.x, x.y);
     if constexpr (kAct == Activation::Gelu) {
-        float density, tail;
-        normal_tail(x, &density, &tail);
-        return x * (x >= 0.0f ? 1.0f - tail : tail);
+        const Pair32 tail = normal_tail(x).tail;
+        const float2 low = apart(tail), high = apart(fma2(tail, both32(-1.0f), both32(1.0f)));
+        return apart(mul2(v, pair32(x.x >= 0.0f ? high.x : low.x, x.y >= 0.0f ? high.y : low.y)));
     } else if constexpr (kAct == Activation::GeluTanh) {
-        // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
-        const float u = kTanhSlope * fmaf(kTanhCube * x * x, x, x);
-        const float e = __expf(-2.0f * fabsf(u)), s = __fdividef(1.0f, 1.0f + e);
-        return x * (x >= 0.0f ? s : e * s);
+        const Logistic l = logistic(x);
+        const float2 low = apart(mul2(pair32(l.e.x, l.e.y), pair32(l.s.x, l.s.y)));
+        return apart(mul2(v, pair32(x.x >= 0.0f ? l.s.x : low.x, x.y >= 0.0f ? l.s.y : low.y)));
     } else {
         return x;
     }
 }
 
-// The derivative at a kept value: finite, or NaN (which min and max without .NaN would lose).
+// dy times the derivative at kept values: finite, or NaN (which min and max without .NaN would lose).
 template <Activation kAct>
-__device__ __forceinline__ float slope(float x) {
+__device__ __forceinline__ float2 through(float2 x, float2 dy) {
+    const Pair32 g = pair32(dy.x, dy.y);
     if constexpr (kAct == Activation::Gelu) {
-        float density, tail;
-        normal_tail(x, &density, &tail);
-        return fmaf(x * 0.3989422804f, density, x >= 0.0f ? 1.0f - tail : tail);
+        // Phi + x phi: for x >= 0, 1 - (tail - |x| phi)
+        const Tail t = normal_tail(x);
+        const Pair32 below = fma2(mul2(pair32(fabsf(x.x), fabsf(x.y)), both32(-0.3989422804f)), t.density, t.tail);
+        const float2 low = apart(below), high = apart(fma2(below, both32(-1.0f), both32(1.0f)));
+        return apart(mul2(g, pair32(x.x >= 0.0f ? high.x : low.x, x.y >= 0.0f ? high.y : low.y)));
     } else if constexpr (kAct == Activation::GeluTanh) {
         // Beyond 64 the slope is 1 or 0 in 32 bits, and x^2 would overflow further out.
-        x = OpMin::apply(OpMax::apply(x, -64.0f), 64.0f);
-        const float square = x * x;
-        const float u = kTanhSlope * fmaf(kTanhCube * square, x, x);
-        const float e = __expf(-2.0f * fabsf(u)), s = __fdividef(1.0f, 1.0f + e);
+        x = make_float2(OpMin::apply(OpMax::apply(x.x, -64.0f), 64.0f), OpMin::apply(OpMax::apply(x.y, -64.0f), 64.0f));
+        const Logistic l = logistic(x);
+        const Pair32 s = pair32(l.s.x, l.s.y), es = mul2(pair32(l.e.x, l.e.y), s);
+        const float2 low = apart(es);
         // s(u) s(-u) = e s^2 for either sign: no difference of numbers near one
-        return fmaf(x * (2.0f * kTanhSlope) * fmaf(3.0f * kTanhCube, square, 1.0f), e * s * s, x >= 0.0f ? s : e * s);
+        const Pair32 du = mul2(mul2(pair32(x.x, x.y), both32(2.0f * kTanhSlope)), fma2(l.square, both32(3.0f * kTanhCube), both32(1.0f)));
+        return apart(mul2(g, fma2(du, mul2(es, s), pair32(x.x >= 0.0f ? l.s.x : low.x, x.y >= 0.0f ? l.s.y : low.y))));
     } else {
-        return 1.0f;
+        return x;
     }
 }
 
 // 16 elements of one row.
 template <typename T>
 struct Sixteen {
-    static constexpr int kPacks = 16 * sizeof(T) / 32;
-    Raw32 raw[kPacks];
+    static constexpr int kWords = 16 * sizeof(T) / 4;
+    unsigned w[kWords];
     __device__ __forceinline__ void load(const char* p) {
 #pragma unroll
-        for (int i = 0; i < kPacks; ++i) raw[i] = ld32_stream(p + 32 * i);
+        for (int i = 0; i < kWords / 8; ++i) put(i, ld32_stream(p + 32 * i));
     }
-    __device__ __forceinline__ void widen(float (&f)[16]) const {
+    __device__ __forceinline__ void put(int i, const Raw32& r) {
+        w[8 * i] = r.lo.x; w[8 * i + 1] = r.lo.y; w[8 * i + 2] = r.lo.z; w[8 * i + 3] = r.lo.w;
+        w[8 * i + 4] = r.hi.x; w[8 * i + 5] = r.hi.y; w[8 * i + 6] = r.hi.z; w[8 * i + 7] = r.hi.w;
+    }
+    __device__ __forceinline__ void store(char* p) const {
 #pragma unroll
-        for (int i = 0; i < kPacks; ++i) {
-            float g[16 / kPacks];
-            Wide32<T>::unpack(raw[i], g);
-#pragma unroll
-            for (int e = 0; e < 16 / kPacks; ++e) f[i * (16 / kPacks) + e] = g[e];
+        for (int i = 0; i < kWords / 8; ++i) {
+            Raw32 r;
+            r.lo = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
+            r.hi = make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+            st32(p + 32 * i, r);
         }
     }
-    static __device__ __forceinline__ void store(char* p, const float (&f)[16]) {
+    // Elements 2i and 2i + 1.
+    __device__ __forceinline__ float2 pair(int i) const {
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else if constexpr (std::is_same_v<T, __half>) return h2_to_f2(w[i]);
+        else return b2_to_f2(w[i]);
+    }
+    __device__ __forceinline__ void set(int i, float2 f) {
+        if constexpr (sizeof(T) == 4) { w[2 * i] = __float_as_uint(f.x); w[2 * i + 1] = __float_as_uint(f.y); }
+        else if constexpr (std::is_same_v<T, __half>) w[i] = f2_to_h2(f.x, f.y);
+        else w[i] = f2_to_b2(f.x, f.y);
+    }
+    __device__ __forceinline__ unsigned amax() const {
+        unsigned m = 0;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < kPacks; ++i) {
-            float g[16 / kPacks];
+            for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
+            return m;
+        } else {
 #pragma unroll
-            for (int e = 0; e < 16 / kPacks; ++e) g[e] = f[i * (16 / kPacks) + e];
-            st32(p + 32 * i, Wide32<T>::pack(g));
+            for (int i = 0; i < kWords; ++i) m = larger_magnitudes(m, w[i]);
+            return magnitude_of_pair<T>(m);
+        }
+    }
+    __device__ __forceinline__ uint4 codes(unsigned scale) const {
+        unsigned c[4];
+        if constexpr (sizeof(T) == 4) {
+            const float inverse = inverse_step8(scale);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f[4] = {__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]), __uint_as_float(w[4 * i + 2]), __uint_as_float(w[4 * i + 3])};
+                c[i] = finite8(encode8x4(f, inverse), scale);
+            }
+        } else {
+            const Inverse16<T> inverse(scale);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = finite8(encode8x4(w[2 * i], w[2 * i + 1], inverse), scale);
+        }
+        return make_uint4(c[0], c[1], c[2], c[3]);
+    }
+    __device__ __forceinline__ void widen(const uint4& codes, unsigned scale) {
+        const unsigned c[4] = {codes.x, codes.y, codes.z, codes.w};
+        if constexpr (sizeof(T) == 4) {
+            const float step = step8(scale);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float f[4];
+                decode8x4(c[i], step, f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * i + e] = __float_as_uint(f[e]);
+            }
+        } else {
+            const unsigned step = step16<T>(scale);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint2 v = widen8x4<T>(c[i], step);
+                w[2 * i] = v.x;
+                w[2 * i + 1] = v.y;
+            }
         }
     }
 };
@@ -140,30 +226,18 @@ __global__ void __launch_bounds__(kThreads) keep8_kernel(const Kept8Args a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const unsigned i = first + u * kThreads;
-        float f[16];
-        unsigned amax = 0;
-        if (i < a.items) {
-            x[u].widen(f);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) amax = max(amax, magnitude_bits(f[e]));
-        }
+        unsigned amax = i < a.items ? x[u].amax() : 0u;
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         if (i < a.items) {
             if (kAct == Activation::None || a.codes != nullptr) {
                 const unsigned scale = scale8<T>(amax);
-                const float inverse = inverse_step8(scale);
-                uint4 c;
-                c.x = finite8(encode8x4(f, inverse), scale);
-                c.y = finite8(encode8x4(f + 4, inverse), scale);
-                c.z = finite8(encode8x4(f + 8, inverse), scale);
-                c.w = finite8(encode8x4(f + 12, inverse), scale);
-                st16(reinterpret_cast<uint4*>(a.codes) + i, c);
+                st16(reinterpret_cast<uint4*>(a.codes) + i, x[u].codes(scale));
                 if ((i & 1u) == 0) a.scales[i >> 1] = (unsigned char)scale;
             }
             if constexpr (kAct != Activation::None) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) f[e] = activate<kAct>(f[e]);
-                Sixteen<T>::store(a.out + (u64)i * (16 * sizeof(T)), f);
+                for (int e = 0; e < 8; ++e) x[u].set(e, activate<kAct>(x[u].pair(e)));
+                x[u].store(a.out + (u64)i * (16 * sizeof(T)));
             }
         }
     }
@@ -194,19 +268,13 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const Kept8Args a) {
     for (int u = 0; u < U; ++u) {
         const unsigned i = first + u * kThreads;
         if (i < a.items) {
-            const float step = step8(scale[u]);
-            float f[16];
-            decode8x4(c[u].x, step, f);
-            decode8x4(c[u].y, step, f + 4);
-            decode8x4(c[u].z, step, f + 8);
-            decode8x4(c[u].w, step, f + 12);
+            Sixteen<T> x;
+            x.widen(c[u], scale[u]);
             if constexpr (kAct != Activation::None) {
-                float g[16];
-                dy[u].widen(g);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) f[e] = g[e] * slope<kAct>(f[e]);
+                for (int e = 0; e < 8; ++e) x.set(e, through<kAct>(x.pair(e), dy[u].pair(e)));
             }
-            Sixteen<T>::store(a.out + (u64)i * (16 * sizeof(T)), f);
+            x.store(a.out + (u64)i * (16 * sizeof(T)));
         }
     }
 }
@@ -241,7 +309,7 @@ __global__ void __launch_bounds__(kThreads) keep8_ragged_kernel(const Kept8Args 
                 if (lane == 0) a.scales[i] = (unsigned char)scale;
             }
             if constexpr (kAct != Activation::None)
-                if (at[u] != ~0ull) reinterpret_cast<T*>(a.out)[at[u]] = Elem<T>::from_f(activate<kAct>(f[u]));
+                if (at[u] != ~0ull) reinterpret_cast<T*>(a.out)[at[u]] = Elem<T>::from_f(activate<kAct>(make_float2(f[u], 0.0f)).x);
         }
     }
 }
@@ -270,7 +338,7 @@ __global__ void __launch_bounds__(kThreads) read8_ragged_kernel(const Kept8Args 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         float f = decode8<0>(code[u], step8(scale[u]));
-        if constexpr (kAct != Activation::None) f = dy[u] * slope<kAct>(f);
+        if constexpr (kAct != Activation::None) f = through<kAct>(make_float2(f, 0.0f), make_float2(dy[u], 0.0f)).x;
         if (at[u] != ~0ull) reinterpret_cast<T*>(a.out)[at[u]] = Elem<T>::from_f(f);
     }
 }

@@ -6,7 +6,8 @@
 //
 // Bound by HBM: every head is read once and written once. Angles are made where they are used: position * frequency as
 // turns in 64 bits, less its whole turns, then one sincospi in 32 bits (error 2e-7 at any position; in 32 bits the product alone is off by
-// 0.06 at a million). A CTA makes them once for its tokens, in shared memory, and all heads of a token share them.
+// 0.06 at a million). A warp makes them once for its tokens, in shared memory of its own, and all heads of a token, of queries and
+// keys, share them. Warps meet nowhere but at the end of the backward pass.
 //
 // A group of lanes holds a head: each lane V pairs at V neighbouring places of either half (interleaved: 2V neighbouring elements), so
 // both elements of a pair are in one lane and no exchange is needed but the sums over a head. Elements that do not turn are
@@ -21,6 +22,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 namespace b200ccl::kernels {
 
@@ -33,11 +35,24 @@ using i64 = long long;
 
 constexpr unsigned kThreads = 256;
 constexpr unsigned kWarps = kThreads / 32;
+constexpr unsigned kMaxTileTokens = 8;  // of a warp's table
+constexpr u64 kSms = 148;
 
 struct View {
     const char* data;
     i64 batch, token, head;  // bytes
 };
+
+// n / d for n below 2^31, as a product.
+struct Divisor {
+    unsigned d, factor, shift;
+    __device__ __forceinline__ unsigned divide(unsigned n) const { return (unsigned)(((u64)n * factor) >> shift); }
+};
+Divisor divisor_of(unsigned d) {
+    unsigned bits = 0;
+    while ((1ull << bits) < d) ++bits;
+    return {d, (unsigned)((1ull << (31 + bits)) / d + 1), 31 + bits};
+}
 
 struct Side {
     View x, grad;
@@ -47,10 +62,7 @@ struct Side {
     unsigned char* scales;
     char* weight_grad;
     float* partial;
-    unsigned heads;
-    unsigned tile;   // tokens of a tile
-    unsigned tiles;
-    unsigned ctas;
+    Divisor heads;  // d = 0: none
 };
 
 struct RotationArgs {
@@ -58,61 +70,73 @@ struct RotationArgs {
     const char* positions;
     i64 position_batch, position_token;  // elements
     const double* frequencies;
-    u64 all;  // tokens of all sequences
-    u64 tokens;
+    unsigned all;     // tokens of all sequences
+    Divisor tokens;   // of one
     unsigned dim, rotated, pitch;
     unsigned items;  // lanes' worth of pairs in a head
     unsigned group;  // lanes that hold a head, a power of two
+    unsigned tile;   // tokens of a warp's tile
+    unsigned split;  // warps that share a tile, each for some of its heads
+    unsigned tiles;  // times split
+    unsigned ctas;
     float magnitude, sine;  // what cosines and sines are multiplied with
     float eps;
     bool positions64;
 };
 
-// V neighbouring elements of T.
+// V neighbouring elements of T, as they lie in memory.
 template <typename T, int V>
-__device__ __forceinline__ void load_some(const char* p, float (&f)[V]) {
-    if constexpr (V * sizeof(T) == 16) {
-        Wide<T>::unpack(ld16_stream(reinterpret_cast<const uint4*>(p)), f);
-    } else if constexpr (V * sizeof(T) == 8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        float2 a, b;
-        if constexpr (sizeof(T) == 2) {
-            if constexpr (std::is_same_v<T, __half>) { a = h2_to_f2(w.x); b = h2_to_f2(w.y); }
-            else { a = b2_to_f2(w.x); b = b2_to_f2(w.y); }
+struct Some {
+    static constexpr int kBytes = V * sizeof(T);
+    using Word = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, T>>;
+    static_assert(kBytes == 16 || kBytes == 8 || V == 1);
+    Word w;
+    __device__ __forceinline__ void clear() { w = Word(); }
+    __device__ __forceinline__ void load(const char* p) {
+        if constexpr (kBytes == 16) w = ld16_stream(reinterpret_cast<const uint4*>(p));
+        else w = *reinterpret_cast<const Word*>(p);
+    }
+    __device__ __forceinline__ void widen(float (&f)[V]) const {
+        if constexpr (kBytes == 16) {
+            Wide<T>::unpack(w, f);
+        } else if constexpr (V > 1) {
+            const float2 a = std::is_same_v<T, __half> ? h2_to_f2(w.x) : b2_to_f2(w.x), b = std::is_same_v<T, __half> ? h2_to_f2(w.y) : b2_to_f2(w.y);
             f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+        } else {
+            f[0] = Elem<T>::to_f(w);
         }
-    } else {
-        static_assert(V == 1);
-        f[0] = Elem<T>::to_f(*reinterpret_cast<const T*>(p));
     }
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_some(char* p, const float (&f)[V]) {
-    if constexpr (V * sizeof(T) == 16) {
-        st16(reinterpret_cast<uint4*>(p), Wide<T>::pack(f));
-    } else if constexpr (V * sizeof(T) == 8) {
-        uint2 w;
-        if constexpr (std::is_same_v<T, __half>) { w.x = f2_to_h2(f[0], f[1]); w.y = f2_to_h2(f[2], f[3]); }
-        else { w.x = f2_to_b2(f[0], f[1]); w.y = f2_to_b2(f[2], f[3]); }
-        *reinterpret_cast<uint2*>(p) = w;
-    } else {
-        static_assert(V == 1);
-        *reinterpret_cast<T*>(p) = Elem<T>::from_f(f[0]);
+    static __device__ __forceinline__ void store(char* p, const float (&f)[V]) {
+        if constexpr (kBytes == 16) {
+            st16(reinterpret_cast<uint4*>(p), Wide<T>::pack(f));
+        } else if constexpr (V > 1) {
+            uint2 w;
+            if constexpr (std::is_same_v<T, __half>) { w.x = f2_to_h2(f[0], f[1]); w.y = f2_to_h2(f[2], f[3]); }
+            else { w.x = f2_to_b2(f[0], f[1]); w.y = f2_to_b2(f[2], f[3]); }
+            *reinterpret_cast<uint2*>(p) = w;
+        } else {
+            *reinterpret_cast<T*>(p) = Elem<T>::from_f(f[0]);
+        }
     }
-}
+};
 // V neighbouring codes.
 template <int V>
-__device__ __forceinline__ void load_codes(const unsigned char* p, float step, float (&f)[V]) {
-    if constexpr (V == 8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        decode8x4(w.x, step, f);
-        decode8x4(w.y, step, f + 4);
-    } else if constexpr (V == 4) {
-        decode8x4(*reinterpret_cast<const unsigned*>(p), step, f);
-    } else {
-        f[0] = decode8<0>(*p, step);
+struct Codes {
+    using Word = std::conditional_t<V == 8, uint2, std::conditional_t<V == 4, unsigned, unsigned char>>;
+    Word w;
+    __device__ __forceinline__ void clear() { w = Word(); }
+    __device__ __forceinline__ void load(const unsigned char* p) { w = *reinterpret_cast<const Word*>(p); }
+    __device__ __forceinline__ void widen(float step, float (&f)[V]) const {
+        if constexpr (V == 8) {
+            decode8x4(w.x, step, f);
+            decode8x4(w.y, step, f + 4);
+        } else if constexpr (V == 4) {
+            decode8x4(w, step, f);
+        } else {
+            f[0] = decode8<0>(w, step);
+        }
     }
-}
+};
 template <int V>
 __device__ __forceinline__ void store_codes(unsigned char* p, unsigned scale, const float (&f)[V]) {
     const float inverse = inverse_step8(scale);
@@ -157,15 +181,18 @@ __device__ __forceinline__ void join(float (&u)[V], float (&v)[V]) {
 }
 template <typename T, int V, bool kInterleaved>
 __device__ __forceinline__ void load_pairs(const char* head, const Place& at, float (&u)[V], float (&v)[V]) {
-    load_some<T, V>(head + at.first * sizeof(T), u);
-    load_some<T, V>(head + at.second * sizeof(T), v);
+    Some<T, V> a, b;
+    a.load(head + at.first * sizeof(T));
+    b.load(head + at.second * sizeof(T));
+    a.widen(u);
+    b.widen(v);
     if constexpr (kInterleaved && V > 1) part(u, v);
 }
 template <typename T, int V, bool kInterleaved>
 __device__ __forceinline__ void store_pairs(char* head, const Place& at, float (&u)[V], float (&v)[V]) {
     if constexpr (kInterleaved && V > 1) join(u, v);
-    store_some<T, V>(head + at.first * sizeof(T), u);
-    store_some<T, V>(head + at.second * sizeof(T), v);
+    Some<T, V>::store(head + at.first * sizeof(T), u);
+    Some<T, V>::store(head + at.second * sizeof(T), v);
 }
 
 __device__ __forceinline__ float group_sum(float v, unsigned group) {
@@ -177,252 +204,343 @@ __device__ __forceinline__ unsigned group_max(unsigned v, unsigned group) {
     return v;
 }
 
-// Cosine and sine of every pair of a tile's tokens, and the place of each token's first head in x and grad (bytes).
-__device__ __forceinline__ void make_table(const RotationArgs& a, const Side& s, u64 token0, unsigned tokens, float2* table, i64* x_at,
-                                           i64* grad_at) {
-    const unsigned pairs = a.rotated / 2;
-    for (unsigned i = threadIdx.x; i < tokens * pairs; i += kThreads) {
-        const unsigned t = i / pairs, p = i - t * pairs;
-        const u64 n = token0 + t, b = n / a.tokens;
-        const i64 at = (i64)b * a.position_batch + (i64)(n - b * a.tokens) * a.position_token;
+// A warp's share of the work: some tokens, and of their heads one part in `split`.
+struct Tile {
+    unsigned token, tokens, part;
+};
+__device__ __forceinline__ Tile tile_at(const RotationArgs& a, unsigned index) {
+    const unsigned t = a.split == 1u ? index : index / a.split;
+    return {t * a.tile, min(a.tile, a.all - t * a.tile), index - t * a.split};
+}
+// Its rows (heads of tokens, in order) of one side.
+struct Rows {
+    unsigned from, to;
+};
+__device__ __forceinline__ Rows rows_of(const RotationArgs& a, const Side& s, const Tile& t) {
+    const unsigned rows = t.tokens * s.heads.d;
+    if (a.split == 1u) return {0u, rows};
+    const unsigned each = (rows + a.split - 1u) / a.split;
+    return {min(rows, t.part * each), min(rows, (t.part + 1u) * each)};
+}
+
+// Cosine and sine of every pair of a tile's tokens, in a warp's own shared memory: pair item * V + i of token t at (t * V + i) * turning items
+// + item, so that neighbouring lanes read neighbouring words.
+template <int V>
+__device__ __forceinline__ void make_table(const RotationArgs& a, const Tile& tile, float2* table) {
+    const unsigned pairs = a.rotated / 2, items = pairs / V, lane = threadIdx.x & 31u;
+    for (unsigned t = 0; t < tile.tokens; ++t) {
+        const unsigned n = tile.token + t, b = a.tokens.divide(n);
+        const i64 at = (i64)b * a.position_batch + (i64)(n - b * a.tokens.d) * a.position_token;
         const double position = a.positions64 ? (double)*(reinterpret_cast<const i64*>(a.positions) + at)
                                               : (double)*(reinterpret_cast<const int*>(a.positions) + at);
-        double turns = position * (a.frequencies[p] * 0.15915494309189535);  // 1 / (2 pi)
-        turns -= rint(turns);
-        float sine, cosine;
-        sincospif((float)(2.0 * turns), &sine, &cosine);
-        table[i] = make_float2(a.magnitude * cosine, a.sine * sine);
-    }
-    for (unsigned t = threadIdx.x; t < tokens; t += kThreads) {
-        const u64 n = token0 + t, b = n / a.tokens;
-        const i64 in = (i64)(n - b * a.tokens);
-        x_at[t] = (i64)b * s.x.batch + in * s.x.token;
-        grad_at[t] = (i64)b * s.grad.batch + in * s.grad.token;
+        for (unsigned p = lane; p < pairs; p += 32u) {
+            double turns = position * (a.frequencies[p] * 0.15915494309189535);  // 1 / (2 pi)
+            turns -= rint(turns);
+            float sine, cosine;
+            sincospif((float)(2.0 * turns), &sine, &cosine);
+            table[t * pairs + (p % V) * items + p / V] = make_float2(a.magnitude * cosine, a.sine * sine);
+        }
     }
 }
 
 template <int V>
 __device__ __forceinline__ void turn(const float2* angles, const Place& at, unsigned pairs, float (&u)[V], float (&v)[V]) {
     if (at.pair >= pairs) return;
+    const unsigned items = pairs / V, item = at.pair / V;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float2 cs = angles[at.pair + i];
+        const float2 cs = angles[i * items + item];
         const float x = u[i], y = v[i];
         u[i] = fmaf(x, cs.x, -y * cs.y);
         v[i] = fmaf(x, cs.y, y * cs.x);
     }
 }
 
-// K: items of a lane.
+// One row of one side: which token of the tile it belongs to, and where its head lies in a view.
+struct Row {
+    bool there;
+    unsigned token;  // of the tile
+    unsigned n, b, h;
+};
+__device__ __forceinline__ Row row_at(const RotationArgs& a, const Side& s, const Tile& tile, unsigned r, unsigned to) {
+    Row w;
+    w.there = r < to;
+    w.token = w.there ? s.heads.divide(r) : 0u;
+    w.h = w.there ? r - w.token * s.heads.d : 0u;
+    w.n = tile.token + w.token;
+    w.b = a.tokens.divide(w.n);
+    return w;
+}
+__device__ __forceinline__ const char* head_in(const RotationArgs& a, const View& v, const Row& w) {
+    return v.data + (i64)w.b * v.batch + (i64)(w.n - w.b * a.tokens.d) * v.token + (i64)w.h * v.head;
+}
+
+// K: items of a lane. U: rows of a group in flight.
 template <typename T, int V, int K, bool kInterleaved, bool kNorm, int U>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant__ RotationArgs a) {
     extern __shared__ __align__(16) unsigned char shared[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const bool second = blockIdx.x >= a.side[0].ctas;
-    const Side& s = a.side[second ? 1 : 0];
-    const unsigned tile = blockIdx.x - (second ? a.side[0].ctas : 0u);
-    const u64 token0 = (u64)tile * s.tile;
-    const unsigned tokens = (unsigned)min((u64)s.tile, a.all - token0);
-    i64* x_at = reinterpret_cast<i64*>(shared);
-    i64* grad_at = x_at + s.tile;
-    float2* table = reinterpret_cast<float2*>(grad_at + s.tile);
-    make_table(a, s, token0, tokens, table, x_at, grad_at);
-    __syncthreads();
-    const unsigned lane = threadIdx.x & (a.group - 1u), pairs = a.rotated / 2;
+    const unsigned warp = threadIdx.x / 32u, index = blockIdx.x * kWarps + warp;
+    if (index >= a.tiles) return;
+    const Tile tile = tile_at(a, index);
+    const unsigned pairs = a.rotated / 2, lane = threadIdx.x & (a.group - 1u), groups = 32u / a.group, group = (threadIdx.x & 31u) / a.group;
+    float2* table = reinterpret_cast<float2*>(shared) + warp * a.tile * pairs;
     Place at[K];
     bool mine[K];
-    float wu[kNorm ? K : 1][V], wv[kNorm ? K : 1][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const unsigned item = lane + k * 32u;
         mine[k] = item < a.items;
         at[k] = place_of<V, kInterleaved>(a, mine[k] ? item : 0u);
-        if constexpr (kNorm) load_pairs<T, V, kInterleaved>(s.weight, at[k], wu[k], wv[k]);
     }
-    const unsigned rows = tokens * s.heads, step = kThreads / a.group;
-    // (All lanes of a warp stay to the end of a pass: they exchange sums.)
-    for (unsigned r0 = 0; r0 < rows; r0 += step * U) {
-        float u[U][K][V], v[U][K][V];
-        unsigned token[U];
-        bool there[U];
+    bool made = false;
+    for (int i = 0; i < 2; ++i) {
+        const Side& s = a.side[i];
+        if (s.heads.d == 0u) continue;
+        const Rows rows = rows_of(a, s, tile);
+        float wu[kNorm ? K : 1][V], wv[kNorm ? K : 1][V];
+        if constexpr (kNorm) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const unsigned r = r0 + j * step + threadIdx.x / a.group;
-            there[j] = r < rows;
-            token[j] = there[j] ? r / s.heads : 0u;
-            const char* head = s.x.data + x_at[token[j]] + (i64)(there[j] ? r - token[j] * s.heads : 0u) * s.x.head;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (there[j] && mine[k]) {
-                    load_pairs<T, V, kInterleaved>(head, at[k], u[j][k], v[j][k]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) u[j][k][i] = v[j][k][i] = 0.0f;
-                }
-            }
+            for (int k = 0; k < K; ++k) load_pairs<T, V, kInterleaved>(s.weight, at[k], wu[k], wv[k]);
         }
+        // (All lanes of a warp stay to the end of a pass: they exchange sums.)
+        for (unsigned r0 = rows.from; r0 < rows.to; r0 += groups * U) {
+            Some<T, V> first[U][K], second[U][K];
+            Row row[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const unsigned r = r0 + j * step + threadIdx.x / a.group;
-            const u64 row = token0 * s.heads + r;
-            if constexpr (kNorm) {
-                float squares = 0.0f;
-                unsigned amax = 0;
+            for (int j = 0; j < U; ++j) {
+                row[j] = row_at(a, s, tile, r0 + j * groups + group, rows.to);
+                const char* head = head_in(a, s.x, row[j]);
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        squares = fmaf(u[j][k][i], u[j][k][i], fmaf(v[j][k][i], v[j][k][i], squares));
-                        amax = max(amax, max(magnitude_bits(u[j][k][i]), magnitude_bits(v[j][k][i])));
+                    if (row[j].there && mine[k]) {
+                        first[j][k].load(head + at[k].first * sizeof(T));
+                        second[j][k].load(head + at[k].second * sizeof(T));
+                    } else {
+                        first[j][k].clear();
+                        second[j][k].clear();
                     }
                 }
-                if (s.codes != nullptr) {
-                    const unsigned scale = scale8<T>(group_max(amax, a.group));
+            }
+            if (!made) {  // while the first rows are on the way
+                make_table<V>(a, tile, table);
+                __syncwarp();
+                made = true;
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                float u[K][V], v[K][V];
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    first[j][k].widen(u[k]);
+                    second[j][k].widen(v[k]);
+                }
+                const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
+                if constexpr (kNorm) {
+                    float squares = 0.0f;
+                    unsigned amax = 0;
 #pragma unroll
                     for (int k = 0; k < K; ++k) {
-                        if (there[j] && mine[k]) {
-                            float c[V], d[V];
 #pragma unroll
-                            for (int i = 0; i < V; ++i) { c[i] = u[j][k][i]; d[i] = v[j][k][i]; }
-                            if constexpr (kInterleaved && V > 1) join(c, d);
-                            store_codes<V>(s.codes + row * a.pitch + at[k].first, scale, c);
-                            store_codes<V>(s.codes + row * a.pitch + at[k].second, scale, d);
+                        for (int e = 0; e < V; ++e) {
+                            squares = fmaf(u[k][e], u[k][e], fmaf(v[k][e], v[k][e], squares));
+                            amax = max(amax, max(magnitude_bits(u[k][e]), magnitude_bits(v[k][e])));
                         }
                     }
-                    if (there[j] && lane == 0) s.scales[row] = (unsigned char)scale;
+                    if (s.codes != nullptr) {
+                        const unsigned scale = scale8<T>(group_max(amax, a.group));
+#pragma unroll
+                        for (int k = 0; k < K; ++k) {
+                            if (row[j].there && mine[k]) {
+                                store_codes<V>(s.codes + r * a.pitch + at[k].first, scale, u[k]);
+                                store_codes<V>(s.codes + r * a.pitch + at[k].second, scale, v[k]);
+                            }
+                        }
+                        if (row[j].there && lane == 0) s.scales[r] = (unsigned char)scale;
+                    }
+                    const float rstd = rsqrtf(group_sum(squares, a.group) / (float)a.dim + a.eps);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        if constexpr (kInterleaved && V > 1) part(u[k], v[k]);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            u[k][e] *= rstd * wu[k][e];
+                            v[k][e] *= rstd * wv[k][e];
+                        }
+                    }
+                } else if constexpr (kInterleaved && V > 1) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) part(u[k], v[k]);
                 }
-                const float rstd = rsqrtf(group_sum(squares, a.group) / (float)a.dim + a.eps);
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        u[j][k][i] *= rstd * wu[k][i];
-                        v[j][k][i] *= rstd * wv[k][i];
+                    if (row[j].there && mine[k]) {
+                        turn(table + row[j].token * pairs, at[k], pairs, u[k], v[k]);
+                        store_pairs<T, V, kInterleaved>(s.out + r * a.dim * sizeof(T), at[k], u[k], v[k]);
                     }
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (there[j] && mine[k]) {
-                    turn(table + token[j] * pairs, at[k], pairs, u[j][k], v[j][k]);
-                    store_pairs<T, V, kInterleaved>(s.out + row * a.dim * sizeof(T), at[k], u[j][k], v[j][k]);
                 }
             }
         }
     }
 }
 
-// Gradients of the norm and rotation. A CTA takes tile after tile, so that its share of the weight's gradient stays in registers; the shares go to
-// `partial` and sum_kernel adds them in order, so that results do not depend on which CTA ends first.
-template <typename T, int V, int K, bool kInterleaved, bool kCodes>
-__global__ void __launch_bounds__(kThreads) rotate_norm_backward_kernel(const __grid_constant__ RotationArgs a) {
+// One side of a tile in the backward pass: gradients of the inputs, and this lane's share of the weight's.
+template <typename T, int V, int K, bool kInterleaved, bool kCodes, int U>
+__device__ __forceinline__ void backward_side(const RotationArgs& a, const Side& s, const Tile& tile, const Place (&at)[K], const bool (&mine)[K],
+                                              float2* table, bool* made, float (&du)[K][V], float (&dv)[K][V]) {
+    const unsigned pairs = a.rotated / 2, groups = 32u / a.group, group = (threadIdx.x & 31u) / a.group;
+    const Rows rows = rows_of(a, s, tile);
+    float wu[K][V], wv[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) load_pairs<T, V, kInterleaved>(s.weight, at[k], wu[k], wv[k]);
+    for (unsigned r0 = rows.from; r0 < rows.to; r0 += groups * U) {
+        Some<T, V> g1[U][K], g2[U][K];
+        std::conditional_t<kCodes, Codes<V>, Some<T, V>> x1[U][K], x2[U][K];
+        unsigned scale[U];
+        Row row[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            row[j] = row_at(a, s, tile, r0 + j * groups + group, rows.to);
+            const char* grad = head_in(a, s.grad, row[j]);
+            const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
+            scale[j] = kCodes ? s.scales[r] : 0u;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (row[j].there && mine[k]) {
+                    g1[j][k].load(grad + at[k].first * sizeof(T));
+                    g2[j][k].load(grad + at[k].second * sizeof(T));
+                    if constexpr (kCodes) {
+                        x1[j][k].load(s.codes + r * a.pitch + at[k].first);
+                        x2[j][k].load(s.codes + r * a.pitch + at[k].second);
+                    } else {
+                        const char* x = head_in(a, s.x, row[j]);
+                        x1[j][k].load(x + at[k].first * sizeof(T));
+                        x2[j][k].load(x + at[k].second * sizeof(T));
+                    }
+                } else {
+                    g1[j][k].clear();
+                    g2[j][k].clear();
+                    x1[j][k].clear();
+                    x2[j][k].clear();
+                }
+            }
+        }
+        if (!*made) {
+            __syncwarp();  // the table of the tile before has been read
+            make_table<V>(a, tile, table);
+            __syncwarp();
+            *made = true;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            float gu[K][V], gv[K][V], u[K][V], v[K][V];
+            float squares = 0.0f, dot = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                g1[j][k].widen(gu[k]);
+                g2[j][k].widen(gv[k]);
+                if constexpr (kCodes) {
+                    const float step = step8(scale[j]);
+                    x1[j][k].widen(step, u[k]);
+                    x2[j][k].widen(step, v[k]);
+                } else {
+                    x1[j][k].widen(u[k]);
+                    x2[j][k].widen(v[k]);
+                }
+                if constexpr (kInterleaved && V > 1) {
+                    part(gu[k], gv[k]);
+                    part(u[k], v[k]);
+                }
+                if (!mine[k]) {  // (its codes are zeros, but zero times the step of a head that is not finite is not)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) u[k][e] = v[k][e] = 0.0f;
+                }
+                turn(table + row[j].token * pairs, at[k], pairs, gu[k], gv[k]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    squares = fmaf(u[k][e], u[k][e], fmaf(v[k][e], v[k][e], squares));
+                    dot = fmaf(gu[k][e] * wu[k][e], u[k][e], fmaf(gv[k][e] * wv[k][e], v[k][e], dot));
+                }
+            }
+            squares = group_sum(squares, a.group);
+            dot = group_sum(dot, a.group);
+            if (!row[j].there) continue;
+            const float rstd = rsqrtf(squares / (float)a.dim + a.eps);
+            const float back = dot / (float)a.dim * rstd * rstd;
+            const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    du[k][e] = fmaf(gu[k][e] * rstd, u[k][e], du[k][e]);
+                    dv[k][e] = fmaf(gv[k][e] * rstd, v[k][e], dv[k][e]);
+                    u[k][e] = rstd * fmaf(-u[k][e], back, gu[k][e] * wu[k][e]);
+                    v[k][e] = rstd * fmaf(-v[k][e], back, gv[k][e] * wv[k][e]);
+                }
+                if (mine[k]) store_pairs<T, V, kInterleaved>(s.out + r * a.dim * sizeof(T), at[k], u[k], v[k]);
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// Gradients of the norm and rotation. A warp takes tile after tile, so that its share of the weights' gradients stays in registers; the shares
+// of a CTA go to `partial` and sum_kernel adds them in order, so that results do not depend on which CTA ends first.
+template <typename T, int V, int K, bool kInterleaved, bool kCodes, int U>
+__global__ void __launch_bounds__(kThreads, 2) rotate_norm_backward_kernel(const __grid_constant__ RotationArgs a) {
     extern __shared__ __align__(16) unsigned char shared[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const bool second = blockIdx.x >= a.side[0].ctas;
-    const Side& s = a.side[second ? 1 : 0];
-    const unsigned cta = blockIdx.x - (second ? a.side[0].ctas : 0u);
-    i64* x_at = reinterpret_cast<i64*>(shared);
-    i64* grad_at = x_at + s.tile;
-    float2* table = reinterpret_cast<float2*>(grad_at + s.tile);
-    const unsigned lane = threadIdx.x & (a.group - 1u), pairs = a.rotated / 2;
-    const unsigned step = kThreads / a.group;
+    const unsigned warp = threadIdx.x / 32u, in_warp = threadIdx.x & 31u, lane = threadIdx.x & (a.group - 1u);
+    float2* table = reinterpret_cast<float2*>(shared) + warp * a.tile * (a.rotated / 2);
     Place at[K];
     bool mine[K];
-    float wu[K][V], wv[K][V], du[K][V], dv[K][V];
+    float du[2][K][V], dv[2][K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const unsigned item = lane + k * 32u;
         mine[k] = item < a.items;
         at[k] = place_of<V, kInterleaved>(a, mine[k] ? item : 0u);
-        load_pairs<T, V, kInterleaved>(s.weight, at[k], wu[k], wv[k]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) du[k][i] = dv[k][i] = 0.0f;
+        for (int i = 0; i < V; ++i) du[0][k][i] = dv[0][k][i] = du[1][k][i] = dv[1][k][i] = 0.0f;
     }
-    for (unsigned tile = cta; tile < s.tiles; tile += s.ctas) {
-        const u64 token0 = (u64)tile * s.tile;
-        const unsigned tokens = (unsigned)min((u64)s.tile, a.all - token0);
-        __syncthreads();  // the table of the tile before has been read
-        make_table(a, s, token0, tokens, table, x_at, grad_at);
-        __syncthreads();
-        const unsigned rows = tokens * s.heads;
-        for (unsigned r0 = 0; r0 < rows; r0 += step) {
-            const unsigned r = r0 + threadIdx.x / a.group;
-            const bool there = r < rows;
-            const unsigned token = there ? r / s.heads : 0u;
-            const unsigned h = there ? r - token * s.heads : 0u;
-            const u64 row = token0 * s.heads + (there ? r : 0u);
-            const char* grad = s.grad.data + grad_at[token] + (i64)h * s.grad.head;
-            float gu[K][V], gv[K][V], u[K][V], v[K][V];
-            float step8_ = 0.0f;
-            if constexpr (kCodes) step8_ = step8(s.scales[row]);
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (there && mine[k]) {
-                    load_pairs<T, V, kInterleaved>(grad, at[k], gu[k], gv[k]);
-                    if constexpr (kCodes) {
-                        load_codes<V>(s.codes + row * a.pitch + at[k].first, step8_, u[k]);
-                        load_codes<V>(s.codes + row * a.pitch + at[k].second, step8_, v[k]);
-                        if constexpr (kInterleaved && V > 1) part(u[k], v[k]);
-                    } else {
-                        load_pairs<T, V, kInterleaved>(s.x.data + x_at[token] + (i64)h * s.x.head, at[k], u[k], v[k]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) gu[k][i] = gv[k][i] = u[k][i] = v[k][i] = 0.0f;
-                }
-            }
-            float squares = 0.0f, dot = 0.0f;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                turn(table + token * pairs, at[k], pairs, gu[k], gv[k]);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    squares = fmaf(u[k][i], u[k][i], fmaf(v[k][i], v[k][i], squares));
-                    dot = fmaf(gu[k][i] * wu[k][i], u[k][i], fmaf(gv[k][i] * wv[k][i], v[k][i], dot));
-                }
-            }
-            squares = group_sum(squares, a.group);
-            dot = group_sum(dot, a.group);
-            const float rstd = there ? rsqrtf(squares / (float)a.dim + a.eps) : 0.0f;
-            const float back = dot / (float)a.dim * rstd * rstd;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    du[k][i] = fmaf(gu[k][i] * rstd, u[k][i], du[k][i]);
-                    dv[k][i] = fmaf(gv[k][i] * rstd, v[k][i], dv[k][i]);
-                    u[k][i] = rstd * fmaf(-u[k][i], back, gu[k][i] * wu[k][i]);
-                    v[k][i] = rstd * fmaf(-v[k][i], back, gv[k][i] * wv[k][i]);
-                }
-                if (there && mine[k]) store_pairs<T, V, kInterleaved>(s.out + row * a.dim * sizeof(T), at[k], u[k], v[k]);
-            }
-        }
+    for (unsigned index = blockIdx.x * kWarps + warp; index < a.tiles; index += a.ctas * kWarps) {
+        const Tile tile = tile_at(a, index);
+        bool made = false;
+        if (a.side[0].heads.d != 0u)
+            backward_side<T, V, K, kInterleaved, kCodes, U>(a, a.side[0], tile, at, mine, table, &made, du[0], dv[0]);
+        if (a.side[1].heads.d != 0u)
+            backward_side<T, V, K, kInterleaved, kCodes, U>(a, a.side[1], tile, at, mine, table, &made, du[1], dv[1]);
     }
     // The groups of a warp, then the warps.
     __syncthreads();
     float* sums = reinterpret_cast<float*>(shared);
-    const unsigned warp = threadIdx.x / 32u, in_warp = threadIdx.x & 31u;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+    for (int side = 0; side < 2; ++side) {
+        const Side& s = a.side[side];
+        if (s.heads.d == 0u) continue;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            for (unsigned o = a.group; o < 32u; o <<= 1) {
-                du[k][i] += __shfl_xor_sync(0xffffffffu, du[k][i], o);
-                dv[k][i] += __shfl_xor_sync(0xffffffffu, dv[k][i], o);
-            }
-            if (in_warp < a.group && mine[k]) {
-                sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i : at[k].first + i)] = du[k][i];
-                sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i + 1 : at[k].second + i)] = dv[k][i];
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                for (unsigned o = a.group; o < 32u; o <<= 1) {
+                    du[side][k][i] += __shfl_xor_sync(0xffffffffu, du[side][k][i], o);
+                    dv[side][k][i] += __shfl_xor_sync(0xffffffffu, dv[side][k][i], o);
+                }
+                if (in_warp < a.group && mine[k]) {
+                    sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i : at[k].first + i)] = du[side][k][i];
+                    sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i + 1 : at[k].second + i)] = dv[side][k][i];
+                }
             }
         }
-    }
-    __syncthreads();
-    for (unsigned d = threadIdx.x; d < a.dim; d += kThreads) {
-        float sum = 0.0f;
-        for (unsigned w = 0; w < kWarps; ++w) sum += sums[w * a.dim + d];
-        s.partial[(u64)cta * a.dim + d] = sum;
+        __syncthreads();
+        for (unsigned d = threadIdx.x; d < a.dim; d += kThreads) {
+            float sum = 0.0f;
+            for (unsigned w = 0; w < kWarps; ++w) sum += sums[w * a.dim + d];
+            s.partial[(u64)blockIdx.x * a.dim + d] = sum;
+        }
+        __syncthreads();
     }
 }
 
@@ -434,15 +552,16 @@ __global__ void __launch_bounds__(1024) sum_kernel(const __grid_constant__ Rotat
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Side& s = a.side[blockIdx.y];
     const unsigned column = blockIdx.x * 32u + (threadIdx.x & 31u), part = threadIdx.x >> 5;
+    if (s.weight_grad == nullptr) return;
     float sum = 0.0f;
     if (column < a.dim)
-        for (unsigned c = part; c < s.ctas; c += 32u) sum += s.partial[(u64)c * a.dim + column];
+        for (unsigned c = part; c < a.ctas; c += 32u) sum += s.partial[(u64)c * a.dim + column];
     sums[part][threadIdx.x & 31u] = sum;
     __syncthreads();
     sum = sums[threadIdx.x & 31u][part];  // warp `part` adds column `part`
     for (unsigned o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const unsigned d = blockIdx.x * 32u + part;
-    if ((threadIdx.x & 31u) == 0 && d < a.dim && s.weight_grad != nullptr) reinterpret_cast<T*>(s.weight_grad)[d] = Elem<T>::from_f(sum);
+    if ((threadIdx.x & 31u) == 0 && d < a.dim) reinterpret_cast<T*>(s.weight_grad)[d] = Elem<T>::from_f(sum);
 }
 
 struct Shape {
@@ -485,8 +604,8 @@ RotationArgs args_of(const RotationCall& c, const Shape& shape, unsigned bytes) 
     a.position_token = c.position_token;
     a.positions64 = c.positions64;
     a.frequencies = c.frequencies;
-    a.all = (u64)c.batch * (u64)c.tokens;
-    a.tokens = (u64)c.tokens;
+    a.all = (unsigned)(c.batch * c.tokens);
+    a.tokens = divisor_of((unsigned)std::max(1ll, c.tokens));
     a.dim = (unsigned)c.dim;
     a.rotated = (unsigned)c.rotated;
     a.pitch = (a.dim + 15u) / 16u * 16u;
@@ -506,54 +625,53 @@ RotationArgs args_of(const RotationCall& c, const Shape& shape, unsigned bytes) 
         t.scales = s.scales;
         t.weight_grad = static_cast<char*>(s.weight_grad);
         t.partial = s.partial;
-        t.heads = (unsigned)s.heads;
+        if (s.heads != 0) t.heads = divisor_of((unsigned)s.heads);
     }
     return a;
 }
 
-// Tokens of a tile: as many as give every group `passes` heads.
-void cut(RotationArgs& a, unsigned passes) {
-    for (Side& s : a.side) {
-        if (s.heads == 0) continue;
-        const unsigned want = passes * (kThreads / a.group);
-        s.tile = (unsigned)std::min<u64>(std::max(1u, want / s.heads), a.all);
-        s.tiles = (unsigned)((a.all + s.tile - 1) / s.tile);
+// A warp's tile: as many tokens as give it `passes` rounds of rows of the side with fewer heads. Where that makes too few warps for the device, several
+// share a tile, down to one round of the side with more heads.
+void cut(RotationArgs& a, unsigned passes, u64 warps) {
+    unsigned fewest = 0, most = 0;
+    for (const Side& s : a.side) {
+        if (s.heads.d == 0) continue;
+        fewest = fewest == 0 ? s.heads.d : std::min(fewest, s.heads.d);
+        most = std::max(most, s.heads.d);
     }
+    const unsigned round = 32 / a.group * passes;
+    a.tile = std::min({kMaxTileTokens, std::max(1u, round / fewest), a.all});
+    while (a.tile > 1 && (a.all + a.tile - 1) / a.tile < warps) a.tile = (a.tile + 1) / 2;
+    const unsigned tiles = (a.all + a.tile - 1) / a.tile, rounds = (a.tile * most + round - 1) / round;
+    a.split = (unsigned)std::max<u64>(1, std::min<u64>(rounds, warps / tiles));
+    a.tiles = tiles * a.split;
 }
 
-std::size_t table_bytes(const RotationArgs& a) {
-    std::size_t most = 0;
-    for (const Side& s : a.side) most = std::max<std::size_t>(most, s.tile * (16 + (std::size_t)a.rotated / 2 * 8));
-    return most;
-}
+std::size_t table_bytes(const RotationArgs& a) { return (std::size_t)kWarps * a.tile * (a.rotated / 2) * sizeof(float2); }
 
 template <typename T, int V, int K, bool kInterleaved>
 cudaError_t forward(const RotationCall& c, RotationArgs& a) {
     constexpr int U = 2;
-    cut(a, U);
-    for (Side& s : a.side) s.ctas = s.heads == 0 ? 0u : s.tiles;
-    const unsigned grid = a.side[0].ctas + a.side[1].ctas;
+    cut(a, U, kSms * 4);
     return launch_dependent<RotationArgs>(c.norm ? rotate_kernel<T, V, K, kInterleaved, true, U> : rotate_kernel<T, V, K, kInterleaved, false, U>,
-                                          grid, kThreads, table_bytes(a), c.stream, a);
+                                          (a.tiles + kWarps - 1) / kWarps, kThreads, table_bytes(a), c.stream, a);
 }
 
 template <typename T, int V, int K, bool kInterleaved>
 cudaError_t backward(const RotationCall& c, RotationArgs& a) {
-    if (a.all == 0) return launch_dependent<RotationArgs>(sum_kernel<T>, dim3((a.dim + 31) / 32, 2), 1024, 0, c.stream, a);  // of nothing
-    cut(a, 2);
-    const unsigned heads = a.side[0].heads + a.side[1].heads;
+    constexpr int U = 1;
+    const dim3 columns((a.dim + 31) / 32, 2);
+    if (a.all == 0) return launch_dependent<RotationArgs>(sum_kernel<T>, columns, 1024, 0, c.stream, a);  // of nothing
+    cut(a, U, kSms * 4);
+    a.ctas = std::min(kHeadGradCtas, (a.tiles + kWarps - 1) / kWarps);
     bool codes = false;
-    for (Side& s : a.side) {
-        if (s.heads == 0) continue;
-        codes = s.codes != nullptr;
-        s.ctas = std::min(s.tiles, std::max(1u, kHeadGradCtas * s.heads / heads));
-    }
+    for (const Side& s : a.side) codes |= s.codes != nullptr;
     const std::size_t shared = std::max<std::size_t>(table_bytes(a), kWarps * a.dim * sizeof(float));
     const cudaError_t st = launch_dependent<RotationArgs>(
-        codes ? rotate_norm_backward_kernel<T, V, K, kInterleaved, true> : rotate_norm_backward_kernel<T, V, K, kInterleaved, false>,
-        a.side[0].ctas + a.side[1].ctas, kThreads, shared, c.stream, a);
+        codes ? rotate_norm_backward_kernel<T, V, K, kInterleaved, true, U> : rotate_norm_backward_kernel<T, V, K, kInterleaved, false, U>,
+        a.ctas, kThreads, shared, c.stream, a);
     if (st != cudaSuccess) return st;
-    return launch_dependent<RotationArgs>(sum_kernel<T>, dim3((a.dim + 31) / 32, 2), 1024, 0, c.stream, a);
+    return launch_dependent<RotationArgs>(sum_kernel<T>, columns, 1024, 0, c.stream, a);
 }
 
 template <typename T, int V, int K>

@@ -10,7 +10,7 @@
 namespace b200ccl::kernels {
 
 constexpr int kMaxHeadDim = 256;
-constexpr unsigned kHeadGradCtas = 592;  // at most so many partial sums of a weight's gradient: four CTAs on each of 148 SMs
+constexpr unsigned kHeadGradCtas = 296;  // at most so many partial sums of a weight's gradient: two CTAs on each of 148 SMs
 
 // [batch, tokens, heads, dim]: elements from one to the next, the last axis without gaps.
 struct HeadsView {

@@ -7,8 +7,8 @@
 // and 8 KiB of codes every 512 cycles, which a step takes), the pair 48 per SM.
 //
 // Roles of a CTA's 16 warps: one thread copies dY and codes by TMA; one thread of the first CTA issues the products, and its counterpart in the second tells it that
-// its dY has come; eight warps widen codes to 16-bit numbers, exactly (block8.cuh), straight into the swizzled operand (per 4 codes: 5 byte
-// permutes and 4 two-wide operations, about a third of the issue slots of a step); four warps write finished tiles; two sum columns of dY
+// its dY has come; eight warps widen codes to 16-bit numbers, exactly (block8.cuh), straight into the swizzled operand (per 4 codes of bf16:
+// two masks, two byte permutes and four two-wide products); four warps write finished tiles; two sum columns of dY
 // for the bias out of shared memory, each tile of features for its own share of the steps, so that every step of dY is summed once.
 //
 // P pairs take P whole tiles at a time, as long as there are so many: they are at the same tokens then, and read them from L2 once one of them has.
@@ -105,34 +105,6 @@ struct Barriers {
     unsigned failed;
 };
 
-// Four codes as two pairs of 16-bit numbers: 128 + m (bf16) or 1024 + m (fp16) by placing bytes, less 128 or 1024, times the step.
-template <bool kBf16>
-__device__ __forceinline__ uint2 widen4(unsigned word, unsigned step2) {
-    const unsigned m = word & 0x7f7f7f7fu;
-    const unsigned high = kBf16 ? 0x43434343u : 0x64646464u;
-    unsigned a = __byte_perm(m, high, 0x4140), b = __byte_perm(m, high, 0x4342);
-    const unsigned sa = __byte_perm(word, 0u, 0x1404), sb = __byte_perm(word, 0u, 0x3424);
-    if constexpr (kBf16) {
-        const __nv_bfloat162 off = __floats2bfloat162_rn(128.0f, 128.0f), s = *reinterpret_cast<const __nv_bfloat162*>(&step2);
-        const __nv_bfloat162 va = __hmul2(__hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), off), s);
-        const __nv_bfloat162 vb = __hmul2(__hsub2(*reinterpret_cast<__nv_bfloat162*>(&b), off), s);
-        a = *reinterpret_cast<const unsigned*>(&va);
-        b = *reinterpret_cast<const unsigned*>(&vb);
-    } else {
-        const __half2 off = __floats2half2_rn(1024.0f, 1024.0f), s = *reinterpret_cast<const __half2*>(&step2);
-        const __half2 va = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&a), off), s);
-        const __half2 vb = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&b), off), s);
-        a = *reinterpret_cast<const unsigned*>(&va);
-        b = *reinterpret_cast<const unsigned*>(&vb);
-    }
-    return make_uint2(a | (sa & 0x80008000u), b | (sb & 0x80008000u));
-}
-template <bool kBf16>
-__device__ __forceinline__ unsigned step_pair(unsigned scale) {
-    if constexpr (kBf16) return scale << 7 | scale << 23;
-    const __half2 s = __float2half2_rn(step8(scale));
-    return *reinterpret_cast<const unsigned*>(&s);
-}
 __device__ __forceinline__ void store_shared16(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -216,6 +188,7 @@ __device__ __forceinline__ Spot spot_of(const WeightGradArgs& a, unsigned k) {
 template <typename T, bool kBias>
 __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_constant__ WeightGradArgs a) {
     constexpr bool kBf16 = !std::is_same_v<T, __half>;
+    using Operand = std::conditional_t<kBf16, __nv_bfloat16, __half>;
     extern __shared__ unsigned char raw[];
     // Swizzled operands start at multiples of 1024 bytes; the same place in both CTAs.
     unsigned char* shared = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
@@ -387,9 +360,9 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
 #pragma unroll
             for (unsigned u = 0; u < 8; ++u) {
                 const uint4 c = load_shared16(codes + s * kCodeBytes + u * (8u * kHalf));
-                const unsigned s2 = step_pair<kBf16>(scale[u]);
-                const uint2 w0 = widen4<kBf16>(odd ? c.z : c.x, s2), w1 = widen4<kBf16>(odd ? c.w : c.y, s2);
-                const uint2 w2 = widen4<kBf16>(odd ? c.x : c.z, s2), w3 = widen4<kBf16>(odd ? c.y : c.w, s2);
+                const unsigned s2 = step16<Operand>(scale[u]);
+                const uint2 w0 = widen8x4<Operand>(odd ? c.z : c.x, s2), w1 = widen8x4<Operand>(odd ? c.w : c.y, s2);
+                const uint2 w2 = widen8x4<Operand>(odd ? c.x : c.z, s2), w3 = widen8x4<Operand>(odd ? c.y : c.w, s2);
                 store_shared16(first + u * 1024u, w0.x, w0.y, w1.x, w1.y);
                 store_shared16(second + u * 1024u, w2.x, w2.y, w3.x, w3.y);
             }
