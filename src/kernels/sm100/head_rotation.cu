@@ -19,6 +19,7 @@
 
 #include "kernels/sm100/block8.cuh"
 #include "kernels/sm100/launch.h"
+#include "kernels/sm100/pair32.cuh"
 
 #include <algorithm>
 #include <cstdint>
@@ -54,6 +55,13 @@ Divisor divisor_of(unsigned d) {
     return {d, (unsigned)((1ull << (31 + bits)) / d + 1), 31 + bits};
 }
 
+// How tokens are dealt out: a tile of tokens to a warp, or to `split` warps, each for some of the heads.
+struct Cut {
+    unsigned tile, split;
+    unsigned tiles;  // times split
+    unsigned ctas;   // backward: CTAs that take them in turn
+};
+
 struct Side {
     View x, grad;
     char* out;
@@ -63,6 +71,7 @@ struct Side {
     char* weight_grad;
     float* partial;
     Divisor heads;  // d = 0: none
+    Cut cut;        // backward: a CTA works on one side
 };
 
 struct RotationArgs {
@@ -75,14 +84,15 @@ struct RotationArgs {
     unsigned dim, rotated, pitch;
     unsigned items;  // lanes' worth of pairs in a head
     unsigned group;  // lanes that hold a head, a power of two
-    unsigned tile;   // tokens of a warp's tile
-    unsigned split;  // warps that share a tile, each for some of its heads
-    unsigned tiles;  // times split
-    unsigned ctas;
+    Cut cut;  // forward: a warp works on both sides of its tokens
     float magnitude, sine;  // what cosines and sines are multiplied with
     float eps;
     bool positions64;
 };
+
+// Numbers go by twos: V of them are (V + 1) / 2 pairs; a single one has a zero beside it.
+template <int V>
+constexpr int kPairs = (V + 1) / 2;
 
 // V neighbouring elements of T, as they lie in memory.
 template <typename T, int V>
@@ -96,58 +106,102 @@ struct Some {
         if constexpr (kBytes == 16) w = ld16_stream(reinterpret_cast<const uint4*>(p));
         else w = *reinterpret_cast<const Word*>(p);
     }
-    __device__ __forceinline__ void widen(float (&f)[V]) const {
-        if constexpr (kBytes == 16) {
-            Wide<T>::unpack(w, f);
-        } else if constexpr (V > 1) {
-            const float2 a = std::is_same_v<T, __half> ? h2_to_f2(w.x) : b2_to_f2(w.x), b = std::is_same_v<T, __half> ? h2_to_f2(w.y) : b2_to_f2(w.y);
-            f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+    __device__ __forceinline__ unsigned word(int i) const {
+        if constexpr (kBytes == 16) return i == 0 ? w.x : (i == 1 ? w.y : (i == 2 ? w.z : w.w));
+        else return i == 0 ? w.x : w.y;
+    }
+    static __device__ __forceinline__ float2 two(unsigned word) {
+        if constexpr (std::is_same_v<T, __half>) return h2_to_f2(word);
+        else return b2_to_f2(word);
+    }
+    __device__ __forceinline__ void widen(Pair32 (&f)[kPairs<V>]) const {
+        if constexpr (V == 1) {
+            f[0] = pair32(Elem<T>::to_f(w), 0.0f);
         } else {
-            f[0] = Elem<T>::to_f(w);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    f[i] = pair32(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
+                } else {
+                    const float2 g = two(word(i));
+                    f[i] = pair32(g.x, g.y);
+                }
+            }
         }
     }
-    static __device__ __forceinline__ void store(char* p, const float (&f)[V]) {
-        if constexpr (kBytes == 16) {
-            st16(reinterpret_cast<uint4*>(p), Wide<T>::pack(f));
-        } else if constexpr (V > 1) {
-            uint2 w;
-            if constexpr (std::is_same_v<T, __half>) { w.x = f2_to_h2(f[0], f[1]); w.y = f2_to_h2(f[2], f[3]); }
-            else { w.x = f2_to_b2(f[0], f[1]); w.y = f2_to_b2(f[2], f[3]); }
-            *reinterpret_cast<uint2*>(p) = w;
+    static __device__ __forceinline__ void store(char* p, const Pair32 (&f)[kPairs<V>]) {
+        if constexpr (V == 1) {
+            *reinterpret_cast<T*>(p) = Elem<T>::from_f(apart(f[0]).x);
+        } else if constexpr (sizeof(T) == 4) {
+            const float2 a = apart(f[0]), b = apart(f[1]);
+            st16(reinterpret_cast<uint4*>(p), make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)));
         } else {
-            *reinterpret_cast<T*>(p) = Elem<T>::from_f(f[0]);
+            unsigned r[V / 2];
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 g = apart(f[i]);
+                r[i] = std::is_same_v<T, __half> ? f2_to_h2(g.x, g.y) : f2_to_b2(g.x, g.y);
+            }
+            if constexpr (V == 8) st16(reinterpret_cast<uint4*>(p), make_uint4(r[0], r[1], r[2], r[3]));
+            else *reinterpret_cast<uint2*>(p) = make_uint2(r[0], r[1]);
+        }
+    }
+    // The largest magnitude so far and of these: of 16-bit types as two halves, see larger_magnitudes().
+    __device__ __forceinline__ unsigned larger(unsigned so_far) const {
+        if constexpr (V == 1) {
+            return max(so_far, magnitude_bits(Elem<T>::to_f(w)));
+        } else if constexpr (sizeof(T) == 4) {
+            return max(max(so_far, max(w.x & 0x7fffffffu, w.y & 0x7fffffffu)), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) so_far = larger_magnitudes(so_far, word(i));
+            return so_far;
+        }
+    }
+    static __device__ __forceinline__ unsigned magnitude(unsigned larger) { return V > 1 && sizeof(T) == 2 ? magnitude_of_pair<T>(larger) : larger; }
+    // Its codes, to where they are kept.
+    __device__ __forceinline__ void keep(unsigned char* p, unsigned scale) const {
+        if constexpr (V == 1) {
+            *p = (unsigned char)finite8(encode8(Elem<T>::to_f(w), inverse_step8(scale)), scale);
+        } else if constexpr (sizeof(T) == 4) {
+            const float f[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
+            *reinterpret_cast<unsigned*>(p) = finite8(encode8x4(f, inverse_step8(scale)), scale);
+        } else {
+            const Inverse16<T> inverse(scale);
+            const unsigned a = finite8(encode8x4(word(0), word(1), inverse), scale);
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(a, finite8(encode8x4(word(2), word(3), inverse), scale));
+            else *reinterpret_cast<unsigned*>(p) = a;
         }
     }
 };
-// V neighbouring codes.
-template <int V>
+// V neighbouring codes. What they stand for is a bf16 number too where T is fp32.
+template <typename T, int V>
 struct Codes {
     using Word = std::conditional_t<V == 8, uint2, std::conditional_t<V == 4, unsigned, unsigned char>>;
+    using Narrow16 = std::conditional_t<std::is_same_v<T, __half>, __half, __nv_bfloat16>;
     Word w;
     __device__ __forceinline__ void clear() { w = Word(); }
     __device__ __forceinline__ void load(const unsigned char* p) { w = *reinterpret_cast<const Word*>(p); }
-    __device__ __forceinline__ void widen(float step, float (&f)[V]) const {
-        if constexpr (V == 8) {
-            decode8x4(w.x, step, f);
-            decode8x4(w.y, step, f + 4);
-        } else if constexpr (V == 4) {
-            decode8x4(w, step, f);
+    static __device__ __forceinline__ void four(unsigned word, unsigned step, Pair32* f) {
+        const uint2 v = widen8x4<Narrow16>(word, step);
+        const float2 a = Some<Narrow16, 4>::two(v.x), b = Some<Narrow16, 4>::two(v.y);
+        f[0] = pair32(a.x, a.y);
+        f[1] = pair32(b.x, b.y);
+    }
+    __device__ __forceinline__ void widen(unsigned scale, Pair32 (&f)[kPairs<V>]) const {
+        if constexpr (V == 1) {
+            f[0] = pair32(decode8<0>(w, step8(scale)), 0.0f);
         } else {
-            f[0] = decode8<0>(w, step);
+            const unsigned step = step16<Narrow16>(scale);
+            if constexpr (V == 8) {
+                four(w.x, step, f);
+                four(w.y, step, f + 2);
+            } else {
+                four(w, step, f);
+            }
         }
     }
 };
-template <int V>
-__device__ __forceinline__ void store_codes(unsigned char* p, unsigned scale, const float (&f)[V]) {
-    const float inverse = inverse_step8(scale);
-    if constexpr (V == 8) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(finite8(encode8x4(f, inverse), scale), finite8(encode8x4(f + 4, inverse), scale));
-    } else if constexpr (V == 4) {
-        *reinterpret_cast<unsigned*>(p) = finite8(encode8x4(f, inverse), scale);
-    } else {
-        *p = (unsigned char)finite8(encode8(f[0], inverse), scale);
-    }
-}
 
 // Where a lane's pairs lie in a head: first elements at `first`, second ones at `second` (interleaved: from `first` on, in turn).
 struct Place {
@@ -162,35 +216,43 @@ __device__ __forceinline__ Place place_of(const RotationArgs& a, unsigned item) 
     return {p, first, first + (a.dim - a.rotated) / 2};
 }
 
-// u[i], v[i]: the elements of pair i. Interleaved ones arrive as u0 v0 u1 v1 ...
+// u, v: the first and second elements of the lane's pairs, in order. Interleaved ones arrive as u0 v0 u1 v1 ...
 template <int V>
-__device__ __forceinline__ void part(float (&u)[V], float (&v)[V]) {
-    float f[2 * V];
+__device__ __forceinline__ void part(Pair32 (&u)[kPairs<V>], Pair32 (&v)[kPairs<V>]) {
+    if constexpr (V > 1) {
+        float2 f[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) { f[i] = u[i]; f[V + i] = v[i]; }
+        for (int i = 0; i < V / 2; ++i) { f[i] = apart(u[i]); f[V / 2 + i] = apart(v[i]); }
 #pragma unroll
-    for (int i = 0; i < V; ++i) { u[i] = f[2 * i]; v[i] = f[2 * i + 1]; }
+        for (int i = 0; i < V / 2; ++i) { u[i] = pair32(f[2 * i].x, f[2 * i + 1].x); v[i] = pair32(f[2 * i].y, f[2 * i + 1].y); }
+    }
 }
 template <int V>
-__device__ __forceinline__ void join(float (&u)[V], float (&v)[V]) {
-    float f[2 * V];
+__device__ __forceinline__ void join(Pair32 (&u)[kPairs<V>], Pair32 (&v)[kPairs<V>]) {
+    if constexpr (V > 1) {
+        float2 f[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) { f[2 * i] = u[i]; f[2 * i + 1] = v[i]; }
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 a = apart(u[i]), b = apart(v[i]);
+            f[2 * i] = make_float2(a.x, b.x);
+            f[2 * i + 1] = make_float2(a.y, b.y);
+        }
 #pragma unroll
-    for (int i = 0; i < V; ++i) { u[i] = f[i]; v[i] = f[V + i]; }
+        for (int i = 0; i < V / 2; ++i) { u[i] = pair32(f[i].x, f[i].y); v[i] = pair32(f[V / 2 + i].x, f[V / 2 + i].y); }
+    }
 }
 template <typename T, int V, bool kInterleaved>
-__device__ __forceinline__ void load_pairs(const char* head, const Place& at, float (&u)[V], float (&v)[V]) {
+__device__ __forceinline__ void load_pairs(const char* head, const Place& at, Pair32 (&u)[kPairs<V>], Pair32 (&v)[kPairs<V>]) {
     Some<T, V> a, b;
     a.load(head + at.first * sizeof(T));
     b.load(head + at.second * sizeof(T));
     a.widen(u);
     b.widen(v);
-    if constexpr (kInterleaved && V > 1) part(u, v);
+    if constexpr (kInterleaved) part<V>(u, v);
 }
 template <typename T, int V, bool kInterleaved>
-__device__ __forceinline__ void store_pairs(char* head, const Place& at, float (&u)[V], float (&v)[V]) {
-    if constexpr (kInterleaved && V > 1) join(u, v);
+__device__ __forceinline__ void store_pairs(char* head, const Place& at, Pair32 (&u)[kPairs<V>], Pair32 (&v)[kPairs<V>]) {
+    if constexpr (kInterleaved) join<V>(u, v);
     Some<T, V>::store(head + at.first * sizeof(T), u);
     Some<T, V>::store(head + at.second * sizeof(T), v);
 }
@@ -208,25 +270,29 @@ __device__ __forceinline__ unsigned group_max(unsigned v, unsigned group) {
 struct Tile {
     unsigned token, tokens, part;
 };
-__device__ __forceinline__ Tile tile_at(const RotationArgs& a, unsigned index) {
-    const unsigned t = a.split == 1u ? index : index / a.split;
-    return {t * a.tile, min(a.tile, a.all - t * a.tile), index - t * a.split};
+__device__ __forceinline__ Tile tile_at(const RotationArgs& a, const Cut& cut, unsigned index) {
+    const unsigned t = cut.split == 1u ? index : index / cut.split;
+    return {t * cut.tile, min(cut.tile, a.all - t * cut.tile), index - t * cut.split};
 }
 // Its rows (heads of tokens, in order) of one side.
 struct Rows {
     unsigned from, to;
 };
-__device__ __forceinline__ Rows rows_of(const RotationArgs& a, const Side& s, const Tile& t) {
+__device__ __forceinline__ Rows rows_of(const Cut& cut, const Side& s, const Tile& t) {
     const unsigned rows = t.tokens * s.heads.d;
-    if (a.split == 1u) return {0u, rows};
-    const unsigned each = (rows + a.split - 1u) / a.split;
+    if (cut.split == 1u) return {0u, rows};
+    const unsigned each = (rows + cut.split - 1u) / cut.split;
     return {min(rows, t.part * each), min(rows, (t.part + 1u) * each)};
 }
 
-// Cosine and sine of every pair of a tile's tokens, in a warp's own shared memory: pair item * V + i of token t at (t * V + i) * turning items
-// + item, so that neighbouring lanes read neighbouring words.
+// Cosines and sines of a tile's tokens, in a warp's own shared memory: (cos, cos, sin, sin) of two pairs (of one, with zeros: V = 1) of an item, those of
+// neighbouring items beside one another, so that lanes read neighbouring 16 bytes.
 template <int V>
-__device__ __forceinline__ void make_table(const RotationArgs& a, const Tile& tile, float2* table) {
+__device__ __forceinline__ unsigned table_entries(const RotationArgs& a) {
+    return a.rotated / 2 / V * kPairs<V>;
+}
+template <int V>
+__device__ __forceinline__ void make_table(const RotationArgs& a, const Tile& tile, float4* table) {
     const unsigned pairs = a.rotated / 2, items = pairs / V, lane = threadIdx.x & 31u;
     for (unsigned t = 0; t < tile.tokens; ++t) {
         const unsigned n = tile.token + t, b = a.tokens.divide(n);
@@ -238,21 +304,24 @@ __device__ __forceinline__ void make_table(const RotationArgs& a, const Tile& ti
             turns -= rint(turns);
             float sine, cosine;
             sincospif((float)(2.0 * turns), &sine, &cosine);
-            table[t * pairs + (p % V) * items + p / V] = make_float2(a.magnitude * cosine, a.sine * sine);
+            float* entry = reinterpret_cast<float*>(table + t * (items * kPairs<V>) + (p % V / 2) * items + p / V);
+            entry[p % V % 2] = a.magnitude * cosine;
+            entry[2 + p % V % 2] = a.sine * sine;
+            if constexpr (V == 1) entry[1] = entry[3] = 0.0f;
         }
     }
 }
 
 template <int V>
-__device__ __forceinline__ void turn(const float2* angles, const Place& at, unsigned pairs, float (&u)[V], float (&v)[V]) {
+__device__ __forceinline__ void turn(const float4* angles, const Place& at, unsigned pairs, Pair32 (&u)[kPairs<V>], Pair32 (&v)[kPairs<V>]) {
     if (at.pair >= pairs) return;
     const unsigned items = pairs / V, item = at.pair / V;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float2 cs = angles[i * items + item];
-        const float x = u[i], y = v[i];
-        u[i] = fmaf(x, cs.x, -y * cs.y);
-        v[i] = fmaf(x, cs.y, y * cs.x);
+    for (int i = 0; i < kPairs<V>; ++i) {
+        const float4 cs = angles[i * items + item];
+        const Pair32 c = pair32(cs.x, cs.y), s = pair32(cs.z, cs.w), x = u[i], y = v[i];
+        u[i] = fma2(mul2(y, s), both32(-1.0f), mul2(x, c));
+        v[i] = fma2(x, s, mul2(y, c));
     }
 }
 
@@ -277,15 +346,17 @@ __device__ __forceinline__ const char* head_in(const RotationArgs& a, const View
 
 // K: items of a lane. U: rows of a group in flight.
 template <typename T, int V, int K, bool kInterleaved, bool kNorm, int U>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant__ RotationArgs a) {
+__global__ void __launch_bounds__(kThreads, kNorm ? 3 : 4) rotate_kernel(const __grid_constant__ RotationArgs a) {
+    constexpr int P = kPairs<V>;
     extern __shared__ __align__(16) unsigned char shared[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned warp = threadIdx.x / 32u, index = blockIdx.x * kWarps + warp;
-    if (index >= a.tiles) return;
-    const Tile tile = tile_at(a, index);
+    if (index >= a.cut.tiles) return;
+    const Tile tile = tile_at(a, a.cut, index);
     const unsigned pairs = a.rotated / 2, lane = threadIdx.x & (a.group - 1u), groups = 32u / a.group, group = (threadIdx.x & 31u) / a.group;
-    float2* table = reinterpret_cast<float2*>(shared) + warp * a.tile * pairs;
+    const unsigned entries = table_entries<V>(a);
+    float4* table = reinterpret_cast<float4*>(shared) + warp * a.cut.tile * entries;
     Place at[K];
     bool mine[K];
 #pragma unroll
@@ -298,8 +369,8 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
     for (int i = 0; i < 2; ++i) {
         const Side& s = a.side[i];
         if (s.heads.d == 0u) continue;
-        const Rows rows = rows_of(a, s, tile);
-        float wu[kNorm ? K : 1][V], wv[kNorm ? K : 1][V];
+        const Rows rows = rows_of(a.cut, s, tile);
+        Pair32 wu[kNorm ? K : 1][P], wv[kNorm ? K : 1][P];
         if constexpr (kNorm) {
 #pragma unroll
             for (int k = 0; k < K; ++k) load_pairs<T, V, kInterleaved>(s.weight, at[k], wu[k], wv[k]);
@@ -330,53 +401,50 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
             }
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                float u[K][V], v[K][V];
+                const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
+                if (kNorm && s.codes != nullptr) {
+                    unsigned amax = 0;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) amax = second[j][k].larger(first[j][k].larger(amax));
+                    const unsigned scale = scale8<T>(group_max(Some<T, V>::magnitude(amax), a.group));
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        if (row[j].there && mine[k]) {
+                            first[j][k].keep(s.codes + r * a.pitch + at[k].first, scale);
+                            second[j][k].keep(s.codes + r * a.pitch + at[k].second, scale);
+                        }
+                    }
+                    if (row[j].there && lane == 0) s.scales[r] = (unsigned char)scale;
+                }
+                Pair32 u[K][P], v[K][P];
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     first[j][k].widen(u[k]);
                     second[j][k].widen(v[k]);
+                    if constexpr (kInterleaved) part<V>(u[k], v[k]);
                 }
-                const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
                 if constexpr (kNorm) {
-                    float squares = 0.0f;
-                    unsigned amax = 0;
+                    Pair32 sum = both32(0.0f);
 #pragma unroll
                     for (int k = 0; k < K; ++k) {
 #pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            squares = fmaf(u[k][e], u[k][e], fmaf(v[k][e], v[k][e], squares));
-                            amax = max(amax, max(magnitude_bits(u[k][e]), magnitude_bits(v[k][e])));
-                        }
+                        for (int e = 0; e < P; ++e) sum = fma2(u[k][e], u[k][e], fma2(v[k][e], v[k][e], sum));
                     }
-                    if (s.codes != nullptr) {
-                        const unsigned scale = scale8<T>(group_max(amax, a.group));
-#pragma unroll
-                        for (int k = 0; k < K; ++k) {
-                            if (row[j].there && mine[k]) {
-                                store_codes<V>(s.codes + r * a.pitch + at[k].first, scale, u[k]);
-                                store_codes<V>(s.codes + r * a.pitch + at[k].second, scale, v[k]);
-                            }
-                        }
-                        if (row[j].there && lane == 0) s.scales[r] = (unsigned char)scale;
-                    }
-                    const float rstd = rsqrtf(group_sum(squares, a.group) / (float)a.dim + a.eps);
+                    const float2 squares = apart(sum);
+                    const Pair32 rstd = both32(rsqrtf(group_sum(squares.x + squares.y, a.group) / (float)a.dim + a.eps));
 #pragma unroll
                     for (int k = 0; k < K; ++k) {
-                        if constexpr (kInterleaved && V > 1) part(u[k], v[k]);
 #pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            u[k][e] *= rstd * wu[k][e];
-                            v[k][e] *= rstd * wv[k][e];
+                        for (int e = 0; e < P; ++e) {
+                            u[k][e] = mul2(mul2(u[k][e], rstd), wu[k][e]);
+                            v[k][e] = mul2(mul2(v[k][e], rstd), wv[k][e]);
                         }
                     }
-                } else if constexpr (kInterleaved && V > 1) {
-#pragma unroll
-                    for (int k = 0; k < K; ++k) part(u[k], v[k]);
                 }
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     if (row[j].there && mine[k]) {
-                        turn(table + row[j].token * pairs, at[k], pairs, u[k], v[k]);
+                        turn<V>(table + row[j].token * entries, at[k], pairs, u[k], v[k]);
                         store_pairs<T, V, kInterleaved>(s.out + r * a.dim * sizeof(T), at[k], u[k], v[k]);
                     }
                 }
@@ -385,162 +453,144 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
     }
 }
 
-// One side of a tile in the backward pass: gradients of the inputs, and this lane's share of the weight's.
-template <typename T, int V, int K, bool kInterleaved, bool kCodes, int U>
-__device__ __forceinline__ void backward_side(const RotationArgs& a, const Side& s, const Tile& tile, const Place (&at)[K], const bool (&mine)[K],
-                                              float2* table, bool* made, float (&du)[K][V], float (&dv)[K][V]) {
-    const unsigned pairs = a.rotated / 2, groups = 32u / a.group, group = (threadIdx.x & 31u) / a.group;
-    const Rows rows = rows_of(a, s, tile);
-    float wu[K][V], wv[K][V];
-#pragma unroll
-    for (int k = 0; k < K; ++k) load_pairs<T, V, kInterleaved>(s.weight, at[k], wu[k], wv[k]);
-    for (unsigned r0 = rows.from; r0 < rows.to; r0 += groups * U) {
-        Some<T, V> g1[U][K], g2[U][K];
-        std::conditional_t<kCodes, Codes<V>, Some<T, V>> x1[U][K], x2[U][K];
-        unsigned scale[U];
-        Row row[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            row[j] = row_at(a, s, tile, r0 + j * groups + group, rows.to);
-            const char* grad = head_in(a, s.grad, row[j]);
-            const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
-            scale[j] = kCodes ? s.scales[r] : 0u;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (row[j].there && mine[k]) {
-                    g1[j][k].load(grad + at[k].first * sizeof(T));
-                    g2[j][k].load(grad + at[k].second * sizeof(T));
-                    if constexpr (kCodes) {
-                        x1[j][k].load(s.codes + r * a.pitch + at[k].first);
-                        x2[j][k].load(s.codes + r * a.pitch + at[k].second);
-                    } else {
-                        const char* x = head_in(a, s.x, row[j]);
-                        x1[j][k].load(x + at[k].first * sizeof(T));
-                        x2[j][k].load(x + at[k].second * sizeof(T));
-                    }
-                } else {
-                    g1[j][k].clear();
-                    g2[j][k].clear();
-                    x1[j][k].clear();
-                    x2[j][k].clear();
-                }
-            }
-        }
-        if (!*made) {
-            __syncwarp();  // the table of the tile before has been read
-            make_table<V>(a, tile, table);
-            __syncwarp();
-            *made = true;
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            float gu[K][V], gv[K][V], u[K][V], v[K][V];
-            float squares = 0.0f, dot = 0.0f;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                g1[j][k].widen(gu[k]);
-                g2[j][k].widen(gv[k]);
-                if constexpr (kCodes) {
-                    const float step = step8(scale[j]);
-                    x1[j][k].widen(step, u[k]);
-                    x2[j][k].widen(step, v[k]);
-                } else {
-                    x1[j][k].widen(u[k]);
-                    x2[j][k].widen(v[k]);
-                }
-                if constexpr (kInterleaved && V > 1) {
-                    part(gu[k], gv[k]);
-                    part(u[k], v[k]);
-                }
-                if (!mine[k]) {  // (its codes are zeros, but zero times the step of a head that is not finite is not)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) u[k][e] = v[k][e] = 0.0f;
-                }
-                turn(table + row[j].token * pairs, at[k], pairs, gu[k], gv[k]);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    squares = fmaf(u[k][e], u[k][e], fmaf(v[k][e], v[k][e], squares));
-                    dot = fmaf(gu[k][e] * wu[k][e], u[k][e], fmaf(gv[k][e] * wv[k][e], v[k][e], dot));
-                }
-            }
-            squares = group_sum(squares, a.group);
-            dot = group_sum(dot, a.group);
-            if (!row[j].there) continue;
-            const float rstd = rsqrtf(squares / (float)a.dim + a.eps);
-            const float back = dot / (float)a.dim * rstd * rstd;
-            const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    du[k][e] = fmaf(gu[k][e] * rstd, u[k][e], du[k][e]);
-                    dv[k][e] = fmaf(gv[k][e] * rstd, v[k][e], dv[k][e]);
-                    u[k][e] = rstd * fmaf(-u[k][e], back, gu[k][e] * wu[k][e]);
-                    v[k][e] = rstd * fmaf(-v[k][e], back, gv[k][e] * wv[k][e]);
-                }
-                if (mine[k]) store_pairs<T, V, kInterleaved>(s.out + r * a.dim * sizeof(T), at[k], u[k], v[k]);
-            }
-        }
-        __syncwarp();
-    }
-}
-
-// Gradients of the norm and rotation. A warp takes tile after tile, so that its share of the weights' gradients stays in registers; the shares
-// of a CTA go to `partial` and sum_kernel adds them in order, so that results do not depend on which CTA ends first.
+// Gradients of the norm and rotation. A CTA belongs to one side and its warps take tile after tile, so that a lane's share of the weight's gradient
+// stays in registers; the CTA's share goes to `partial` and sum_kernel adds them in order, so that results do not depend on which CTA ends first.
 template <typename T, int V, int K, bool kInterleaved, bool kCodes, int U>
 __global__ void __launch_bounds__(kThreads, 2) rotate_norm_backward_kernel(const __grid_constant__ RotationArgs a) {
+    constexpr int P = kPairs<V>;
     extern __shared__ __align__(16) unsigned char shared[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool keys = blockIdx.x >= a.side[0].cut.ctas;
+    const Side& s = a.side[keys ? 1 : 0];
+    const unsigned cta = blockIdx.x - (keys ? a.side[0].cut.ctas : 0u);
     const unsigned warp = threadIdx.x / 32u, in_warp = threadIdx.x & 31u, lane = threadIdx.x & (a.group - 1u);
-    float2* table = reinterpret_cast<float2*>(shared) + warp * a.tile * (a.rotated / 2);
+    const unsigned pairs = a.rotated / 2, groups = 32u / a.group, group = in_warp / a.group, entries = table_entries<V>(a);
+    float4* table = reinterpret_cast<float4*>(shared) + warp * s.cut.tile * entries;
     Place at[K];
     bool mine[K];
-    float du[2][K][V], dv[2][K][V];
+    Pair32 wu[K][P], wv[K][P], du[K][P], dv[K][P];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const unsigned item = lane + k * 32u;
         mine[k] = item < a.items;
         at[k] = place_of<V, kInterleaved>(a, mine[k] ? item : 0u);
+        load_pairs<T, V, kInterleaved>(s.weight, at[k], wu[k], wv[k]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) du[0][k][i] = dv[0][k][i] = du[1][k][i] = dv[1][k][i] = 0.0f;
+        for (int i = 0; i < P; ++i) du[k][i] = dv[k][i] = both32(0.0f);
     }
-    for (unsigned index = blockIdx.x * kWarps + warp; index < a.tiles; index += a.ctas * kWarps) {
-        const Tile tile = tile_at(a, index);
-        bool made = false;
-        if (a.side[0].heads.d != 0u)
-            backward_side<T, V, K, kInterleaved, kCodes, U>(a, a.side[0], tile, at, mine, table, &made, du[0], dv[0]);
-        if (a.side[1].heads.d != 0u)
-            backward_side<T, V, K, kInterleaved, kCodes, U>(a, a.side[1], tile, at, mine, table, &made, du[1], dv[1]);
+    for (unsigned index = cta * kWarps + warp; index < s.cut.tiles; index += s.cut.ctas * kWarps) {
+        const Tile tile = tile_at(a, s.cut, index);
+        const Rows rows = rows_of(s.cut, s, tile);
+        for (unsigned r0 = rows.from; r0 < rows.to; r0 += groups * U) {
+            Some<T, V> g1[U][K], g2[U][K];
+            std::conditional_t<kCodes, Codes<T, V>, Some<T, V>> x1[U][K], x2[U][K];
+            unsigned scale[U];
+            Row row[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                row[j] = row_at(a, s, tile, r0 + j * groups + group, rows.to);
+                const char* grad = head_in(a, s.grad, row[j]);
+                const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
+                scale[j] = kCodes ? s.scales[r] : 0u;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (row[j].there && mine[k]) {
+                        g1[j][k].load(grad + at[k].first * sizeof(T));
+                        g2[j][k].load(grad + at[k].second * sizeof(T));
+                        if constexpr (kCodes) {
+                            x1[j][k].load(s.codes + r * a.pitch + at[k].first);
+                            x2[j][k].load(s.codes + r * a.pitch + at[k].second);
+                        } else {
+                            const char* x = head_in(a, s.x, row[j]);
+                            x1[j][k].load(x + at[k].first * sizeof(T));
+                            x2[j][k].load(x + at[k].second * sizeof(T));
+                        }
+                    } else {
+                        g1[j][k].clear();
+                        g2[j][k].clear();
+                        x1[j][k].clear();
+                        x2[j][k].clear();
+                    }
+                }
+            }
+            if (r0 == rows.from) {  // while the first rows are on the way
+                __syncwarp();       // the table of the tile before has been read
+                make_table<V>(a, tile, table);
+                __syncwarp();
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                Pair32 gu[K][P], gv[K][P], u[K][P], v[K][P];
+                Pair32 sum = both32(0.0f), product = both32(0.0f);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    g1[j][k].widen(gu[k]);
+                    g2[j][k].widen(gv[k]);
+                    if constexpr (kCodes) {
+                        // (Zero times the step of a head that is not finite is not zero: lanes without elements take another step.)
+                        const unsigned step = mine[k] ? scale[j] : 127u;
+                        x1[j][k].widen(step, u[k]);
+                        x2[j][k].widen(step, v[k]);
+                    } else {
+                        x1[j][k].widen(u[k]);
+                        x2[j][k].widen(v[k]);
+                    }
+                    if constexpr (kInterleaved) {
+                        part<V>(gu[k], gv[k]);
+                        part<V>(u[k], v[k]);
+                    }
+                    turn<V>(table + row[j].token * entries, at[k], pairs, gu[k], gv[k]);
+#pragma unroll
+                    for (int e = 0; e < P; ++e) {
+                        sum = fma2(u[k][e], u[k][e], fma2(v[k][e], v[k][e], sum));
+                        product = fma2(mul2(gu[k][e], wu[k][e]), u[k][e], fma2(mul2(gv[k][e], wv[k][e]), v[k][e], product));
+                    }
+                }
+                const float2 squares = apart(sum), products = apart(product);
+                const float mean = group_sum(squares.x + squares.y, a.group) / (float)a.dim, dot = group_sum(products.x + products.y, a.group) / (float)a.dim;
+                if (!row[j].there) continue;
+                const float r1 = rsqrtf(mean + a.eps);
+                const Pair32 rstd = both32(r1), back = both32(-dot * r1 * r1);
+                const u64 r = (u64)row[j].n * s.heads.d + row[j].h;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+#pragma unroll
+                    for (int e = 0; e < P; ++e) {
+                        du[k][e] = fma2(mul2(gu[k][e], rstd), u[k][e], du[k][e]);
+                        dv[k][e] = fma2(mul2(gv[k][e], rstd), v[k][e], dv[k][e]);
+                        u[k][e] = mul2(rstd, fma2(u[k][e], back, mul2(gu[k][e], wu[k][e])));
+                        v[k][e] = mul2(rstd, fma2(v[k][e], back, mul2(gv[k][e], wv[k][e])));
+                    }
+                    if (mine[k]) store_pairs<T, V, kInterleaved>(s.out + r * a.dim * sizeof(T), at[k], u[k], v[k]);
+                }
+            }
+            __syncwarp();
+        }
     }
     // The groups of a warp, then the warps.
     __syncthreads();
     float* sums = reinterpret_cast<float*>(shared);
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-        const Side& s = a.side[side];
-        if (s.heads.d == 0u) continue;
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                for (unsigned o = a.group; o < 32u; o <<= 1) {
-                    du[side][k][i] += __shfl_xor_sync(0xffffffffu, du[side][k][i], o);
-                    dv[side][k][i] += __shfl_xor_sync(0xffffffffu, dv[side][k][i], o);
-                }
-                if (in_warp < a.group && mine[k]) {
-                    sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i : at[k].first + i)] = du[side][k][i];
-                    sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i + 1 : at[k].second + i)] = dv[side][k][i];
-                }
+        for (int i = 0; i < V; ++i) {
+            float x = i % 2 == 0 ? apart(du[k][i / 2]).x : apart(du[k][i / 2]).y, y = i % 2 == 0 ? apart(dv[k][i / 2]).x : apart(dv[k][i / 2]).y;
+            for (unsigned o = a.group; o < 32u; o <<= 1) {
+                x += __shfl_xor_sync(0xffffffffu, x, o);
+                y += __shfl_xor_sync(0xffffffffu, y, o);
+            }
+            if (in_warp < a.group && mine[k]) {
+                sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i : at[k].first + i)] = x;
+                sums[warp * a.dim + (kInterleaved ? at[k].first + 2 * i + 1 : at[k].second + i)] = y;
             }
         }
-        __syncthreads();
-        for (unsigned d = threadIdx.x; d < a.dim; d += kThreads) {
-            float sum = 0.0f;
-            for (unsigned w = 0; w < kWarps; ++w) sum += sums[w * a.dim + d];
-            s.partial[(u64)blockIdx.x * a.dim + d] = sum;
-        }
-        __syncthreads();
+    }
+    __syncthreads();
+    for (unsigned d = threadIdx.x; d < a.dim; d += kThreads) {
+        float sum = 0.0f;
+        for (unsigned w = 0; w < kWarps; ++w) sum += sums[w * a.dim + d];
+        s.partial[(u64)cta * a.dim + d] = sum;
     }
 }
 
@@ -555,7 +605,7 @@ __global__ void __launch_bounds__(1024) sum_kernel(const __grid_constant__ Rotat
     if (s.weight_grad == nullptr) return;
     float sum = 0.0f;
     if (column < a.dim)
-        for (unsigned c = part; c < a.ctas; c += 32u) sum += s.partial[(u64)c * a.dim + column];
+        for (unsigned c = part; c < s.cut.ctas; c += 32u) sum += s.partial[(u64)c * a.dim + column];
     sums[part][threadIdx.x & 31u] = sum;
     __syncthreads();
     sum = sums[threadIdx.x & 31u][part];  // warp `part` adds column `part`
@@ -630,46 +680,51 @@ RotationArgs args_of(const RotationCall& c, const Shape& shape, unsigned bytes) 
     return a;
 }
 
-// A warp's tile: as many tokens as give it `passes` rounds of rows of the side with fewer heads. Where that makes too few warps for the device, several
+// A warp's tile: as many tokens as give it a round of rows of the side with fewer heads. Where that makes too few warps for the device, several
 // share a tile, down to one round of the side with more heads.
-void cut(RotationArgs& a, unsigned passes, u64 warps) {
-    unsigned fewest = 0, most = 0;
-    for (const Side& s : a.side) {
-        if (s.heads.d == 0) continue;
-        fewest = fewest == 0 ? s.heads.d : std::min(fewest, s.heads.d);
-        most = std::max(most, s.heads.d);
-    }
-    const unsigned round = 32 / a.group * passes;
-    a.tile = std::min({kMaxTileTokens, std::max(1u, round / fewest), a.all});
-    while (a.tile > 1 && (a.all + a.tile - 1) / a.tile < warps) a.tile = (a.tile + 1) / 2;
-    const unsigned tiles = (a.all + a.tile - 1) / a.tile, rounds = (a.tile * most + round - 1) / round;
-    a.split = (unsigned)std::max<u64>(1, std::min<u64>(rounds, warps / tiles));
-    a.tiles = tiles * a.split;
+Cut cut(const RotationArgs& a, unsigned rows, unsigned fewest, unsigned most, u64 warps) {
+    Cut c = {};
+    const unsigned round = 32 / a.group * rows;
+    c.tile = std::min({kMaxTileTokens, std::max(1u, round / fewest), a.all});
+    while (c.tile > 1 && (a.all + c.tile - 1) / c.tile < warps) c.tile = (c.tile + 1) / 2;
+    const unsigned tiles = (a.all + c.tile - 1) / c.tile, rounds = (c.tile * most + round - 1) / round;
+    c.split = (unsigned)std::max<u64>(1, std::min<u64>(rounds, warps / tiles));
+    c.tiles = tiles * c.split;
+    return c;
 }
 
-std::size_t table_bytes(const RotationArgs& a) { return (std::size_t)kWarps * a.tile * (a.rotated / 2) * sizeof(float2); }
+template <int V>
+std::size_t table_bytes(const RotationArgs& a, const Cut& c) {
+    return (std::size_t)kWarps * c.tile * (a.rotated / 2 / V * kPairs<V>) * sizeof(float4);
+}
 
 template <typename T, int V, int K, bool kInterleaved>
 cudaError_t forward(const RotationCall& c, RotationArgs& a) {
     constexpr int U = 2;
-    cut(a, U, kSms * 4);
+    const unsigned q = a.side[0].heads.d, k = a.side[1].heads.d;
+    a.cut = cut(a, U, q == 0 || k == 0 ? q + k : std::min(q, k), std::max(q, k), kSms * 4);
     return launch_dependent<RotationArgs>(c.norm ? rotate_kernel<T, V, K, kInterleaved, true, U> : rotate_kernel<T, V, K, kInterleaved, false, U>,
-                                          (a.tiles + kWarps - 1) / kWarps, kThreads, table_bytes(a), c.stream, a);
+                                          (a.cut.tiles + kWarps - 1) / kWarps, kThreads, table_bytes<V>(a, a.cut), c.stream, a);
 }
 
 template <typename T, int V, int K, bool kInterleaved>
 cudaError_t backward(const RotationCall& c, RotationArgs& a) {
-    constexpr int U = 1;
+    constexpr int U = V == 8 ? 2 : 1;
     const dim3 columns((a.dim + 31) / 32, 2);
     if (a.all == 0) return launch_dependent<RotationArgs>(sum_kernel<T>, columns, 1024, 0, c.stream, a);  // of nothing
-    cut(a, U, kSms * 4);
-    a.ctas = std::min(kHeadGradCtas, (a.tiles + kWarps - 1) / kWarps);
+    const unsigned heads = a.side[0].heads.d + a.side[1].heads.d;
     bool codes = false;
-    for (const Side& s : a.side) codes |= s.codes != nullptr;
-    const std::size_t shared = std::max<std::size_t>(table_bytes(a), kWarps * a.dim * sizeof(float));
+    std::size_t shared = kWarps * a.dim * sizeof(float);
+    for (Side& s : a.side) {
+        if (s.heads.d == 0) continue;
+        codes |= s.codes != nullptr;
+        s.cut = cut(a, U, s.heads.d, s.heads.d, kSms * 8);
+        s.cut.ctas = std::min((s.cut.tiles + kWarps - 1) / kWarps, std::max(1u, kHeadGradCtas * s.heads.d / heads));
+        shared = std::max(shared, table_bytes<V>(a, s.cut));
+    }
     const cudaError_t st = launch_dependent<RotationArgs>(
         codes ? rotate_norm_backward_kernel<T, V, K, kInterleaved, true, U> : rotate_norm_backward_kernel<T, V, K, kInterleaved, false, U>,
-        a.ctas, kThreads, shared, c.stream, a);
+        a.side[0].cut.ctas + a.side[1].cut.ctas, kThreads, shared, c.stream, a);
     if (st != cudaSuccess) return st;
     return launch_dependent<RotationArgs>(sum_kernel<T>, columns, 1024, 0, c.stream, a);
 }
