@@ -86,7 +86,7 @@ struct RotationArgs {
     unsigned group;  // lanes that hold a head, a power of two
     Cut cut;  // forward: a warp works on both sides of its tokens
     float magnitude, sine;  // what cosines and sines are multiplied with
-    float eps;
+    float eps, over_dim;
     bool positions64;
 };
 
@@ -161,15 +161,18 @@ struct Some {
     static __device__ __forceinline__ unsigned magnitude(unsigned larger) { return V > 1 && sizeof(T) == 2 ? magnitude_of_pair<T>(larger) : larger; }
     // Its codes, to where they are kept.
     __device__ __forceinline__ void keep(unsigned char* p, unsigned scale) const {
-        if constexpr (V == 1) {
-            *p = (unsigned char)finite8(encode8(Elem<T>::to_f(w), inverse_step8(scale)), scale);
+        using Out = std::conditional_t<V == 8, uint2, std::conditional_t<V == 4, unsigned, unsigned char>>;
+        if (scale == 255u) {
+            *reinterpret_cast<Out*>(p) = Out();
+        } else if constexpr (V == 1) {
+            *p = (unsigned char)encode8(Elem<T>::to_f(w), inverse_step8(scale));
         } else if constexpr (sizeof(T) == 4) {
             const float f[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
-            *reinterpret_cast<unsigned*>(p) = finite8(encode8x4(f, inverse_step8(scale)), scale);
+            *reinterpret_cast<unsigned*>(p) = encode8x4(f, inverse_step8(scale));
         } else {
             const Inverse16<T> inverse(scale);
-            const unsigned a = finite8(encode8x4(word(0), word(1), inverse), scale);
-            if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(a, finite8(encode8x4(word(2), word(3), inverse), scale));
+            const unsigned a = encode8x4(word(0), word(1), inverse);
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(a, encode8x4(word(2), word(3), inverse));
             else *reinterpret_cast<unsigned*>(p) = a;
         }
     }
@@ -346,7 +349,7 @@ __device__ __forceinline__ const char* head_in(const RotationArgs& a, const View
 
 // K: items of a lane. U: rows of a group in flight.
 template <typename T, int V, int K, bool kInterleaved, bool kNorm, int U>
-__global__ void __launch_bounds__(kThreads, kNorm ? 3 : 4) rotate_kernel(const __grid_constant__ RotationArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) rotate_kernel(const __grid_constant__ RotationArgs a) {
     constexpr int P = kPairs<V>;
     extern __shared__ __align__(16) unsigned char shared[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -366,6 +369,8 @@ __global__ void __launch_bounds__(kThreads, kNorm ? 3 : 4) rotate_kernel(const _
         at[k] = place_of<V, kInterleaved>(a, mine[k] ? item : 0u);
     }
     bool made = false;
+    // (Each side in code of its own: which it is is then known to the compiler, and its arguments are operands instead of loads.)
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
         const Side& s = a.side[i];
         if (s.heads.d == 0u) continue;
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, kNorm ? 3 : 4) rotate_kernel(const _
                         for (int e = 0; e < P; ++e) sum = fma2(u[k][e], u[k][e], fma2(v[k][e], v[k][e], sum));
                     }
                     const float2 squares = apart(sum);
-                    const Pair32 rstd = both32(rsqrtf(group_sum(squares.x + squares.y, a.group) / (float)a.dim + a.eps));
+                    const Pair32 rstd = both32(rsqrtf(fmaf(group_sum(squares.x + squares.y, a.group), a.over_dim, a.eps)));
 #pragma unroll
                     for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -456,14 +461,8 @@ __global__ void __launch_bounds__(kThreads, kNorm ? 3 : 4) rotate_kernel(const _
 // Gradients of the norm and rotation. A CTA belongs to one side and its warps take tile after tile, so that a lane's share of the weight's gradient
 // stays in registers; the CTA's share goes to `partial` and sum_kernel adds them in order, so that results do not depend on which CTA ends first.
 template <typename T, int V, int K, bool kInterleaved, bool kCodes, int U>
-__global__ void __launch_bounds__(kThreads, 2) rotate_norm_backward_kernel(const __grid_constant__ RotationArgs a) {
+__device__ __forceinline__ void rotate_norm_backward(const RotationArgs& a, const Side& s, unsigned cta, unsigned char* shared) {
     constexpr int P = kPairs<V>;
-    extern __shared__ __align__(16) unsigned char shared[];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const bool keys = blockIdx.x >= a.side[0].cut.ctas;
-    const Side& s = a.side[keys ? 1 : 0];
-    const unsigned cta = blockIdx.x - (keys ? a.side[0].cut.ctas : 0u);
     const unsigned warp = threadIdx.x / 32u, in_warp = threadIdx.x & 31u, lane = threadIdx.x & (a.group - 1u);
     const unsigned pairs = a.rotated / 2, groups = 32u / a.group, group = in_warp / a.group, entries = table_entries<V>(a);
     float4* table = reinterpret_cast<float4*>(shared) + warp * s.cut.tile * entries;
@@ -548,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotate_norm_backward_kernel(const
                     }
                 }
                 const float2 squares = apart(sum), products = apart(product);
-                const float mean = group_sum(squares.x + squares.y, a.group) / (float)a.dim, dot = group_sum(products.x + products.y, a.group) / (float)a.dim;
+                const float mean = group_sum(squares.x + squares.y, a.group) * a.over_dim, dot = group_sum(products.x + products.y, a.group) * a.over_dim;
                 if (!row[j].there) continue;
                 const float r1 = rsqrtf(mean + a.eps);
                 const Pair32 rstd = both32(r1), back = both32(-dot * r1 * r1);
@@ -592,6 +591,16 @@ __global__ void __launch_bounds__(kThreads, 2) rotate_norm_backward_kernel(const
         for (unsigned w = 0; w < kWarps; ++w) sum += sums[w * a.dim + d];
         s.partial[(u64)cta * a.dim + d] = sum;
     }
+}
+
+template <typename T, int V, int K, bool kInterleaved, bool kCodes, int U>
+__global__ void __launch_bounds__(kThreads, 2) rotate_norm_backward_kernel(const __grid_constant__ RotationArgs a) {
+    extern __shared__ __align__(16) unsigned char shared[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned ctas = a.side[0].cut.ctas;
+    if (blockIdx.x < ctas) rotate_norm_backward<T, V, K, kInterleaved, kCodes, U>(a, a.side[0], blockIdx.x, shared);
+    else rotate_norm_backward<T, V, K, kInterleaved, kCodes, U>(a, a.side[1], blockIdx.x - ctas, shared);
 }
 
 // weight_grad[d] = sum of partial[cta][d]: 32 columns of one side per CTA.
@@ -664,6 +673,7 @@ RotationArgs args_of(const RotationCall& c, const Shape& shape, unsigned bytes) 
     a.magnitude = c.magnitude;
     a.sine = c.inverse ? -c.magnitude : c.magnitude;
     a.eps = c.eps;
+    a.over_dim = 1.0f / (float)c.dim;
     for (int i = 0; i < 2; ++i) {
         const HeadsSide& s = c.side[i];
         Side& t = a.side[i];
