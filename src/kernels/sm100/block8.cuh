@@ -66,8 +66,12 @@ __device__ __forceinline__ __half2 as_h2(unsigned w) { return *reinterpret_cast<
 __device__ __forceinline__ unsigned bits_of(__nv_bfloat162 v) { return *reinterpret_cast<unsigned*>(&v); }
 __device__ __forceinline__ unsigned bits_of(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
 
-// The larger magnitude of each half so far, and of both at the end, as fp32.
-__device__ __forceinline__ unsigned larger_magnitudes(unsigned so_far, unsigned word) { return __vmaxu2(so_far, word & 0x7fff7fffu); }
+// The larger magnitude of each half so far, NaN once there is one; and of both at the end, as fp32.
+template <typename T>
+__device__ __forceinline__ unsigned larger_magnitudes(unsigned so_far, unsigned word) {
+    if constexpr (std::is_same_v<T, __half>) return bits_of(__hmax2_nan(as_h2(so_far), __habs2(as_h2(word))));
+    else return bits_of(__hmax2_nan(as_b2(so_far), __habs2(as_b2(word))));
+}
 template <typename T>
 __device__ __forceinline__ unsigned magnitude_of_pair(unsigned pair) {
     const unsigned m = max(pair & 0xffffu, pair >> 16);

@@ -160,7 +160,7 @@ struct Sixteen {
             return m;
         } else {
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) m = larger_magnitudes(m, w[i]);
+            for (int i = 0; i < kWords; ++i) m = larger_magnitudes<T>(m, w[i]);
             return magnitude_of_pair<T>(m);
         }
     }
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const Kept8Args a) {
     for (int u = 0; u < U; ++u) {
         const unsigned i = first + u * kThreads;
         if (i < a.items) {
-            c[u] = ld16_stream(reinterpret_cast<const uint4*>(a.codes) + i);
+            c[u] = load16_once(reinterpret_cast<const uint4*>(a.codes) + i);
             scale[u] = a.scales[i >> 1];
             if constexpr (kAct != Activation::None) {
                 const unsigned row = i / (2u * a.blocks), half = i - row * (2u * a.blocks);

@@ -103,7 +103,7 @@ struct Some {
     Word w;
     __device__ __forceinline__ void clear() { w = Word(); }
     __device__ __forceinline__ void load(const char* p) {
-        if constexpr (kBytes == 16) w = ld16_stream(reinterpret_cast<const uint4*>(p));
+        if constexpr (kBytes == 16) w = load16_once(p);
         else w = *reinterpret_cast<const Word*>(p);
     }
     __device__ __forceinline__ unsigned word(int i) const {
@@ -134,7 +134,7 @@ struct Some {
             *reinterpret_cast<T*>(p) = Elem<T>::from_f(apart(f[0]).x);
         } else if constexpr (sizeof(T) == 4) {
             const float2 a = apart(f[0]), b = apart(f[1]);
-            st16(reinterpret_cast<uint4*>(p), make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)));
+            store16_once(p, make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)));
         } else {
             unsigned r[V / 2];
 #pragma unroll
@@ -142,11 +142,11 @@ struct Some {
                 const float2 g = apart(f[i]);
                 r[i] = std::is_same_v<T, __half> ? f2_to_h2(g.x, g.y) : f2_to_b2(g.x, g.y);
             }
-            if constexpr (V == 8) st16(reinterpret_cast<uint4*>(p), make_uint4(r[0], r[1], r[2], r[3]));
+            if constexpr (V == 8) store16_once(p, make_uint4(r[0], r[1], r[2], r[3]));
             else *reinterpret_cast<uint2*>(p) = make_uint2(r[0], r[1]);
         }
     }
-    // The largest magnitude so far and of these: of 16-bit types as two halves, see larger_magnitudes().
+    // The largest magnitude so far and of these: of 16-bit types as two halves, see larger_magnitudes<T>().
     __device__ __forceinline__ unsigned larger(unsigned so_far) const {
         if constexpr (V == 1) {
             return max(so_far, magnitude_bits(Elem<T>::to_f(w)));
@@ -154,7 +154,7 @@ struct Some {
             return max(max(so_far, max(w.x & 0x7fffffffu, w.y & 0x7fffffffu)), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
         } else {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) so_far = larger_magnitudes(so_far, word(i));
+            for (int i = 0; i < V / 2; ++i) so_far = larger_magnitudes<T>(so_far, word(i));
             return so_far;
         }
     }
@@ -261,11 +261,15 @@ __device__ __forceinline__ void store_pairs(char* head, const Place& at, Pair32 
 }
 
 __device__ __forceinline__ float group_sum(float v, unsigned group) {
-    for (unsigned o = group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+    for (unsigned o = 16; o > 0; o >>= 1)
+        if (o < group) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 __device__ __forceinline__ unsigned group_max(unsigned v, unsigned group) {
-    for (unsigned o = group >> 1; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+#pragma unroll
+    for (unsigned o = 16; o > 0; o >>= 1)
+        if (o < group) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
