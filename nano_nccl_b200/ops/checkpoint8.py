@@ -15,7 +15,6 @@ A step captured into a CUDA graph is captured with its backward pass and on one 
 been run and their graphs dropped, as for any torch module.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._lib import load_native_calls
 
@@ -55,29 +54,11 @@ def unpack8(packed):
     return load_native_calls().unpack8(packed.data, packed.shape, packed.dtype)
 
 
-class _Gelu8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, tanh):
-        y, kept = load_native_calls().gelu8_forward(x, tanh, True)
-        ctx.save_for_backward(kept)
-        ctx.tanh = tanh
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (kept,) = ctx.saved_tensors
-        return load_native_calls().gelu8_backward(dy, kept, ctx.tanh), None
-
-
 def gelu8(x, approximate="none"):
     """``torch.nn.functional.gelu(x, approximate)``; the backward pass reads ``x`` in 8 bits, written in the same pass as the result."""
     if approximate not in _APPROXIMATIONS:
         raise ValueError(f"unknown approximation '{approximate}'")
-    tanh = _APPROXIMATIONS[approximate]
-    if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
-        return _Gelu8.apply(x, tanh)
-    return load_native_calls().gelu8_forward(x, tanh, False)[0]
+    return load_native_calls().gelu8(x, _APPROXIMATIONS[approximate])
 
 
 def weight_grad8(dy, packed, bias=False):
@@ -94,25 +75,6 @@ def weight_grad8(dy, packed, bias=False):
     return load_native_calls().weight_grad8(dy, packed.data, packed.shape[-1], bias)
 
 
-class _Linear8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        kept = load_native_calls().pack8(x) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else None
-        ctx.save_for_backward(weight, kept)
-        return torch.nn.functional.linear(x, weight, bias)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        weight, kept = ctx.saved_tensors
-        need_x, need_weight, need_bias = ctx.needs_input_grad
-        dx = dy @ weight if need_x else None
-        dw = db = None
-        if kept is not None:
-            dw, db = load_native_calls().weight_grad8(dy, kept, weight.shape[1], need_bias)
-        return dx, dw if need_weight else None, db
-
-
 def linear8(x, weight, bias=None):
     """``torch.nn.functional.linear(x, weight, bias)``; the weight's gradient reads ``x`` in 8 bits (:func:`weight_grad8`)."""
     if torch.is_autocast_enabled("cuda"):
@@ -120,8 +82,4 @@ def linear8(x, weight, bias=None):
         x, weight, bias = x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype)
         with torch.autocast("cuda", enabled=False):
             return linear8(x, weight, bias)
-    if x.dim() < 2 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"linear8: an input of shape {tuple(x.shape)} does not go into a weight of shape {tuple(weight.shape)}")
-    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
-        raise ValueError("linear8: x, weight and bias must share one dtype")
-    return _Linear8.apply(x, weight, bias)
+    return load_native_calls().linear8(x, weight, bias)

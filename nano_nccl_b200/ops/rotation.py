@@ -9,7 +9,6 @@ joint projection costs no copy); their heads may differ in number, and either ma
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._lib import load_native_calls
 
@@ -60,54 +59,9 @@ def _interleaved(layout):
     return _LAYOUTS[layout]
 
 
-def _wants_gradient(*tensors):
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, frequencies, interleaved, magnitude):
-        ctx.save_for_backward(positions, frequencies)
-        ctx.rest = interleaved, magnitude
-        ctx.set_materialize_grads(False)
-        return load_native_calls().rotate(q, k, positions, frequencies, interleaved, magnitude, False)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        if dq is None and dk is None:
-            return None, None, None, None, None, None
-        positions, frequencies = ctx.saved_tensors
-        dq, dk = load_native_calls().rotate(dq, dk, positions, frequencies, *ctx.rest, True)
-        return dq, dk, None, None, None, None
-
-
 def rotary(q, k, positions, frequencies, layout="half", magnitude=1.0):
     """(q, k) turned by their positions: ``magnitude * (u cos - v sin, u sin + v cos)`` for every pair, one rounding at the end."""
-    interleaved = _interleaved(layout)
-    if _wants_gradient(q, k):
-        return _Rotary.apply(q, k, positions, frequencies, interleaved, magnitude)
-    return load_native_calls().rotate(q, k, positions, frequencies, interleaved, magnitude, False)
-
-
-class _NormRotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, keep8):
-        q_out, k_out, kept = load_native_calls().norm_rotate(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, keep8)
-        ctx.save_for_backward(None if keep8 else q, None if keep8 else k, kept, q_weight, k_weight, positions, frequencies)
-        ctx.heads = tuple(0 if t is None else t.shape[-2] for t in (q, k))
-        ctx.rest = interleaved, magnitude, eps
-        ctx.set_materialize_grads(False)
-        return q_out, k_out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        if dq is None and dk is None:
-            return (None,) * 10
-        q, k, kept, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
-        grads = load_native_calls().norm_rotate_backward(dq, dk, q, k, kept, *ctx.heads, q_weight, k_weight, positions, frequencies, *ctx.rest)
-        return (*grads, None, None, None, None, None, None)
+    return load_native_calls().rotary(q, k, positions, frequencies, _interleaved(layout), magnitude)
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, layout="half", magnitude=1.0, eps=1e-6, keep="int8"):
@@ -120,6 +74,4 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, layout="hal
         raise ValueError(f"unknown way to keep queries and keys '{keep}'")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    if _wants_gradient(q, k, q_weight, k_weight):
-        return _NormRotary.apply(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, keep == "int8")
-    return load_native_calls().norm_rotate(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, False)[:2]
+    return load_native_calls().qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, keep == "int8")

@@ -88,7 +88,11 @@ struct FinishArgs {
     unsigned piece_ctas;  // CTAs that add pieces; the others make the bias's gradient
 };
 
-__host__ __device__ inline unsigned first_step(unsigned pair, unsigned steps, unsigned pairs) { return (unsigned)((u64)pair * steps / pairs); }
+// pair * steps / pairs, in 32 bits: pairs are few.
+__host__ __device__ inline unsigned first_step(unsigned pair, unsigned steps, unsigned pairs) {
+    const unsigned each = steps / pairs;
+    return pair * each + pair * (steps - each * pairs) / pairs;
+}
 
 // Barriers of a CTA, in its shared memory.
 struct Barriers {
@@ -447,25 +451,45 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         const unsigned row = at / a.steps_of_tile, from = row * a.steps_of_tile, tile = a.whole_tiles + row;
         const unsigned before = first_step(border - 1u, a.steps, a.pairs);
         if (at == from || before > from) return;
-        const unsigned output0 = (tile / a.feature_tiles) * kTile + part * kFinishRows, feature0 = (tile % a.feature_tiles) * kTile;
-        const unsigned feature = feature0 + (threadIdx.x & 63u) * 4u;
-        const unsigned to = from + a.steps_of_tile;
-        for (unsigned r = threadIdx.x / 64u; r < kFinishRows; r += 4u) {
-            const unsigned in_piece = (part * kFinishRows + r) * kTile + (threadIdx.x & 63u) * 4u;
-            const auto read = [&](unsigned slot) { return *reinterpret_cast<const float4*>(a.pieces + (u64)slot * (kTile * kTile) + in_piece); };
-            float4 sum = read(2u * (border - 1u) + (before == from ? 0u : 1u));
-            for (unsigned p = border; p < a.pairs && first_step(p, a.steps, a.pairs) < to; ++p) {
-                if (first_step(p, a.steps, a.pairs) == first_step(p + 1u, a.steps, a.pairs)) continue;  // it has no step
-                const float4 v = read(2u * p);
-                sum.x += v.x;
-                sum.y += v.y;
-                sum.z += v.z;
-                sum.w += v.w;
+        __shared__ unsigned slots[kMaxPairs];
+        __shared__ unsigned count;
+        if (threadIdx.x == 0) {
+            unsigned n = 0;
+            slots[n++] = 2u * (border - 1u) + (before == from ? 0u : 1u);
+            unsigned begin = at;
+            for (unsigned p = border; p < a.pairs && begin < from + a.steps_of_tile; ++p) {
+                const unsigned end = first_step(p + 1u, a.steps, a.pairs);
+                if (end != begin) slots[n++] = 2u * p;  // (else it has no step)
+                begin = end;
             }
-            const unsigned output = output0 + r;
+            count = n;
+        }
+        __syncthreads();
+        constexpr unsigned kRows = kFinishRows / 4;  // of a thread, and four neighbouring features of each
+        const unsigned column = (threadIdx.x & 63u) * 4u, row0 = part * kFinishRows + threadIdx.x / 64u * kRows;
+        float4 sum[kRows];
+#pragma unroll
+        for (unsigned r = 0; r < kRows; ++r) sum[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (unsigned i = 0; i < count; ++i) {
+            const float* piece = a.pieces + (u64)slots[i] * (kTile * kTile) + row0 * kTile + column;
+            float4 v[kRows];
+#pragma unroll
+            for (unsigned r = 0; r < kRows; ++r) v[r] = *reinterpret_cast<const float4*>(piece + r * kTile);
+#pragma unroll
+            for (unsigned r = 0; r < kRows; ++r) {
+                sum[r].x += v[r].x;
+                sum[r].y += v[r].y;
+                sum[r].z += v[r].z;
+                sum[r].w += v[r].w;
+            }
+        }
+        const unsigned feature = (tile % a.feature_tiles) * kTile + column;
+#pragma unroll
+        for (unsigned r = 0; r < kRows; ++r) {
+            const unsigned output = (tile / a.feature_tiles) * kTile + row0 + r;
             if (output >= a.outputs) continue;
             T* out = static_cast<T*>(a.out) + (u64)output * a.inputs + feature;
-            const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+            const float f[4] = {sum[r].x, sum[r].y, sum[r].z, sum[r].w};
 #pragma unroll
             for (unsigned i = 0; i < 4; ++i)
                 if (feature + i < a.inputs) out[i] = Elem<T>::from_f(f[i]);
@@ -481,10 +505,12 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         sum += a.bias[(u64)tile * kTile + column];
         if (tile < a.whole_tiles) continue;
         const unsigned from = (tile - a.whole_tiles) * a.steps_of_tile, to = from + a.steps_of_tile;
-        unsigned p = (unsigned)((u64)from * a.pairs / a.steps);
-        while (p < a.pairs && first_step(p, a.steps, a.pairs) <= from) ++p;
-        for (; p < a.pairs && first_step(p, a.steps, a.pairs) < to; ++p)
-            if (first_step(p, a.steps, a.pairs) != first_step(p + 1u, a.steps, a.pairs)) sum += a.bias[(u64)(tiles + p) * kTile + column];
+        unsigned p = (unsigned)((u64)from * a.pairs / a.steps), begin = first_step(p, a.steps, a.pairs);
+        for (; p < a.pairs && begin < to; ++p) {
+            const unsigned end = first_step(p + 1u, a.steps, a.pairs);
+            if (begin > from && end != begin) sum += a.bias[(u64)(tiles + p) * kTile + column];
+            begin = end;
+        }
     }
     __shared__ float sums[8][32];
     sums[threadIdx.x / 32u][threadIdx.x & 31u] = sum;
@@ -500,38 +526,44 @@ struct LayOutArgs {
     const char* dy;
     long long stride;  // bytes
     char* out;
-    u64 tokens;
-    unsigned outputs, pitch;
+    unsigned tokens, outputs, pitch;
 };
 
+// A thread takes eight outputs of a token.
 template <typename T>
 __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ LayOutArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const u64 i = (u64)blockIdx.x * 256u + threadIdx.x;
-    const u64 token = i / a.pitch;
-    const unsigned n = (unsigned)(i - token * a.pitch);
+    const unsigned eights = a.pitch / 8u, i = blockIdx.x * 256u + threadIdx.x, token = i / eights, n = (i - token * eights) * 8u;
     if (token >= a.tokens) return;
-    const bool there = n < a.outputs;
     const T* from = reinterpret_cast<const T*>(a.dy + (long long)token * a.stride) + n;
-    if constexpr (sizeof(T) == 2) {
-        reinterpret_cast<T*>(a.out)[i] = there ? *from : Elem<T>::from_f(0.0f);
+    T x[8];
+    if (sizeof(T) == 4 && n + 8u <= a.outputs && reinterpret_cast<std::uintptr_t>(from) % 16 == 0) {
+        *reinterpret_cast<uint4*>(x) = ld16_stream(reinterpret_cast<const uint4*>(from));
+        *reinterpret_cast<uint4*>(x + 4) = ld16_stream(reinterpret_cast<const uint4*>(from) + 1);
     } else {
-        const float x = there ? *from : 0.0f;
-        unsigned part[3];
-        float rest = x;
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {  // the leading eight bits of what is left, cut off and not rounded: the rest is exact, and nothing overflows
-            part[p] = __float_as_uint(rest) >> 16;
-            rest -= __uint_as_float(part[p] << 16);
-        }
-        if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) {
-            part[0] = x != x ? 0x7fc0u : part[0];
-            part[1] = part[2] = 0u;
-        }
-        unsigned short* out = reinterpret_cast<unsigned short*>(a.out);
+        for (unsigned e = 0; e < 8; ++e) x[e] = n + e < a.outputs ? from[e] : Elem<T>::from_f(0.0f);
+    }
+    if constexpr (sizeof(T) == 2) {
+        *(reinterpret_cast<uint4*>(a.out) + i) = *reinterpret_cast<const uint4*>(x);
+    } else {
+        unsigned part[3][4] = {};
 #pragma unroll
-        for (int p = 0; p < 3; ++p) out[(u64)p * a.tokens * a.pitch + i] = (unsigned short)part[p];
+        for (unsigned e = 0; e < 8; ++e) {
+            float rest = x[e];
+            const bool finite = (__float_as_uint(x[e]) & 0x7f800000u) != 0x7f800000u;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {  // the leading eight bits of what is left, cut off and not rounded: the rest is exact, and nothing overflows
+                const unsigned cut = __float_as_uint(rest) >> 16;
+                rest -= __uint_as_float(cut << 16);
+                const unsigned put = finite ? cut : (p == 0 ? (x[e] != x[e] ? 0x7fc0u : cut) : 0u);
+                part[p][e / 2u] |= put << (16u * (e & 1u));
+            }
+        }
+        const u64 eight = (u64)a.tokens * eights;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *(reinterpret_cast<uint4*>(a.out) + p * eight + i) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
     }
 }
 
@@ -634,11 +666,11 @@ void launch(const WeightGradCall& c, const Plan& p) {
         l.dy = static_cast<const char*>(c.dy);
         l.stride = c.stride * (long long)sizeof(T);
         l.out = workspace;
-        l.tokens = c.tokens;
+        l.tokens = (unsigned)c.tokens;
         l.outputs = (unsigned)c.outputs;
         l.pitch = p.pitch;
-        const u64 ctas = ((u64)c.tokens * p.pitch + 255) / 256;
-        B2_REQUIRE(ctas < (1ull << 31), "weight_grad8: dy is too large for one call");
+        const u64 eights = (u64)c.tokens * (p.pitch / 8), ctas = (eights + 255) / 256;
+        B2_REQUIRE(eights < (1ull << 31), "weight_grad8: dy is too large for one call");
         B2_CUDA(launch_dependent<LayOutArgs>(lay_out_kernel<T>, dim3((unsigned)ctas), 256, 0, c.stream, l));
         dy = workspace;
         row_bytes = (u64)p.pitch * 2;

@@ -1,6 +1,9 @@
 // The training operators (include/b200ccl/train_ops.h) on torch tensors: what a raw pointer does not show is checked here, outputs and scratch come from
 // torch's allocator (on the current stream of the tensors' device, so a captured call's memory is its graph's), and the call goes to the
 // C interface by the addresses handed over in bind().
+//
+// The operators with a gradient are nodes of autograd here and not Python classes: a backward pass then takes the GIL nowhere. (GELU of 1237 x 1003
+// numbers, forward and backward: 67 us as a Python class, 52 us so; the rest is torch's own way to its backward thread and back.)
 #include "torch_ops.h"
 
 #include "b200ccl/train_ops.h"
@@ -11,11 +14,18 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
+#include <memory>
+#include <optional>
+#include <stdexcept>
 #include <string>
+#include <tuple>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -37,13 +47,17 @@ struct Functions {
     decltype(&b2_rotate_heads_backward) rotate_heads_backward = nullptr;
 } g;
 
+// What a call is refused for, and what it failed of. In a backward pass there is no Python frame to raise in: see in_backward().
+struct Refused : std::invalid_argument {
+    using std::invalid_argument::invalid_argument;
+};
+struct Failed : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
 // A Python error is set.
 struct Raised {};
 
-[[noreturn]] void refuse(const std::string& why) {
-    PyErr_SetString(PyExc_ValueError, why.c_str());
-    throw Raised{};
-}
+[[noreturn]] void refuse(const std::string& why) { throw Refused(why); }
 
 void need_arguments(Py_ssize_t got, Py_ssize_t want) {
     if (got == want) return;
@@ -60,12 +74,16 @@ int dtype_code(const char* what, const at::Tensor& t) {
     }
 }
 
-const at::Tensor& tensor_of(const char* what, PyObject* obj) {
-    if (!THPVariable_Check(obj)) refuse(std::string(what) + " must be a tensor");
-    const at::Tensor& t = THPVariable_Unpack(obj);
+const at::Tensor& on_gpu(const char* what, const at::Tensor& t) {
     if (!t.is_cuda() || t.layout() != at::kStrided) refuse(std::string(what) + " must be a dense CUDA tensor");
     return t;
 }
+const at::Tensor& tensor_of(const char* what, PyObject* obj) {
+    if (!THPVariable_Check(obj)) refuse(std::string(what) + " must be a tensor");
+    return on_gpu(what, THPVariable_Unpack(obj));
+}
+// An argument that may be None: not defined then.
+at::Tensor maybe_tensor(const char* what, PyObject* obj) { return obj == Py_None ? at::Tensor() : tensor_of(what, obj); }
 
 void same_place(const char* what, const at::Tensor& t, const at::Tensor& first) {
     if (t.get_device() != first.get_device())
@@ -90,16 +108,14 @@ bool truth(PyObject* obj) {
     return v != 0;
 }
 
+// The C interface, without the GIL where this thread has it.
 template <typename F>
 void call(F&& f) {
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = f();
-    Py_END_ALLOW_THREADS
-    if (rc != 0) {
-        PyErr_SetString(rc == 2 ? PyExc_ValueError : g_error_class, g.last_error());
-        throw Raised{};
-    }
+    PyThreadState* held = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
+    const int rc = f();
+    if (held != nullptr) PyEval_RestoreThread(held);
+    if (rc == 2) throw Refused(g.last_error());
+    if (rc != 0) throw Failed(g.last_error());
 }
 
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(t.get_device())).stream(); }
@@ -145,17 +161,14 @@ Kept kept_bytes(std::int64_t rows, std::int64_t columns) {
 at::Tensor new_bytes(const at::Tensor& like, std::int64_t n) { return at::empty({n}, like.options().dtype(at::kByte).requires_grad(false)); }
 unsigned char* bytes_at(const at::Tensor& t, std::int64_t at) { return static_cast<unsigned char*>(t.data_ptr()) + at; }
 
-const at::Tensor& kept_of(PyObject* obj, std::int64_t bytes) {
-    const at::Tensor& t = tensor_of("the 8-bit form", obj);
+const at::Tensor& kept_of(const at::Tensor& t, std::int64_t bytes) {
+    on_gpu("the 8-bit form", t);
     if (t.scalar_type() != at::kByte || !t.is_contiguous() || t.numel() != bytes)
         refuse("the 8-bit form has " + std::to_string(t.numel()) + " elements, expected " + std::to_string(bytes) + " bytes without gaps");
     return t;
 }
 
-// pack8(x) -> bytes
-PyObject* pack8(PyObject* const* args, Py_ssize_t nargs) {
-    need_arguments(nargs, 1);
-    const at::Tensor& x = tensor_of("x", args[0]);
+at::Tensor pack(const at::Tensor& x) {
     const int dtype = dtype_code("x", x);
     const c10::cuda::CUDAGuard guard(x.device());
     const Rows r = rows_of("x", x);
@@ -163,7 +176,13 @@ PyObject* pack8(PyObject* const* args, Py_ssize_t nargs) {
     at::Tensor out = new_bytes(x, k.codes + k.scales);
     void* stream = stream_of(x);
     call([&] { return g.pack8(r.t.data_ptr(), r.stride, r.rows, r.columns, dtype, bytes_at(out, 0), bytes_at(out, k.codes), stream); });
-    return THPVariable_Wrap(std::move(out));
+    return out;
+}
+
+// pack8(x) -> bytes
+PyObject* pack8(PyObject* const* args, Py_ssize_t nargs) {
+    need_arguments(nargs, 1);
+    return THPVariable_Wrap(pack(tensor_of("x", args[0])));
 }
 
 // unpack8(bytes, sizes, dtype) -> x^
@@ -183,7 +202,7 @@ PyObject* unpack8(PyObject* const* args, Py_ssize_t nargs) {
     if (sizes.back() == 0) rows = 0;
     if (!THPDtype_Check(args[2])) refuse("the dtype must be a torch.dtype");
     const Kept k = kept_bytes(rows, sizes.back());
-    const at::Tensor& kept = kept_of(args[0], k.codes + k.scales);
+    const at::Tensor& kept = kept_of(tensor_of("the 8-bit form", args[0]), k.codes + k.scales);
     const c10::cuda::CUDAGuard guard(kept.device());
     at::Tensor out = at::empty(sizes, kept.options().dtype(reinterpret_cast<THPDtype*>(args[2])->scalar_type));
     const int dtype = dtype_code("the 8-bit form", out);
@@ -201,14 +220,45 @@ PyObject* two(at::Tensor a, at::Tensor b) {
     return t;
 }
 
-at::Tensor new_like(const at::Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)); }
+at::Tensor new_like(const at::Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
 
-// gelu8_forward(x, tanh, keep) -> (y, bytes or None)
-PyObject* gelu8_forward(PyObject* const* args, Py_ssize_t nargs) {
-    need_arguments(nargs, 3);
-    const at::Tensor& x = tensor_of("x", args[0]);
-    const int dtype = dtype_code("x", x), tanh = truth(args[1]) ? 1 : 0;
-    const bool keep = truth(args[2]);
+// ---- nodes of autograd -----------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients, computed by `f`. What f refuses is a ValueError where the backward pass was called; its results have no graph, and say so to
+// whoever differentiates them again.
+template <typename F>
+variable_list in_backward(const char* what, F&& f) {
+    variable_list grads;
+    try {
+        grads = f();
+    } catch (const Refused& e) {
+        TORCH_CHECK_VALUE(false, e.what());
+    }
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list marked;
+    for (at::Tensor& t : grads)
+        if (t.defined()) marked.push_back(t.detach().requires_grad_());
+    if (marked.empty()) return grads;
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", static_cast<std::int64_t>(marked.size()));
+    marked = (*error)(std::move(marked));
+    std::size_t i = 0;
+    for (at::Tensor& t : grads)
+        if (t.defined()) t = marked[i++];
+    return grads;
+}
+
+bool wants_gradient(std::initializer_list<const at::Tensor*> tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor* t : tensors)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// (y, bytes where they are kept)
+std::pair<at::Tensor, at::Tensor> gelu_forward(const at::Tensor& x, bool tanh, bool keep) {
+    const int dtype = dtype_code("x", x);
     const c10::cuda::CUDAGuard guard(x.device());
     const Rows r = rows_of("x", x);
     const Kept k = kept_bytes(r.rows, r.columns);
@@ -216,46 +266,60 @@ PyObject* gelu8_forward(PyObject* const* args, Py_ssize_t nargs) {
     if (keep) kept = new_bytes(x, k.codes + k.scales);
     void* stream = stream_of(x);
     call([&] {
-        return g.gelu8_forward(r.t.data_ptr(), r.stride, r.rows, r.columns, dtype, tanh, y.data_ptr(), keep ? bytes_at(kept, 0) : nullptr,
+        return g.gelu8_forward(r.t.data_ptr(), r.stride, r.rows, r.columns, dtype, tanh ? 1 : 0, y.data_ptr(), keep ? bytes_at(kept, 0) : nullptr,
                                keep ? bytes_at(kept, k.codes) : nullptr, stream);
     });
-    return two(std::move(y), std::move(kept));
+    return {std::move(y), std::move(kept)};
 }
 
-// gelu8_backward(dy, bytes, tanh) -> dx
-PyObject* gelu8_backward(PyObject* const* args, Py_ssize_t nargs) {
-    need_arguments(nargs, 3);
-    const at::Tensor& dy = tensor_of("dy", args[0]);
-    const int dtype = dtype_code("dy", dy), tanh = truth(args[2]) ? 1 : 0;
-    const c10::cuda::CUDAGuard guard(dy.device());
-    const Rows r = rows_of("dy", dy);
-    const Kept k = kept_bytes(r.rows, r.columns);
-    const at::Tensor& kept = kept_of(args[1], k.codes + k.scales);
-    same_place("the 8-bit form", kept, dy);
-    at::Tensor dx = new_like(dy);
-    void* stream = stream_of(dy);
-    call([&] {
-        return g.gelu8_backward(r.t.data_ptr(), r.stride, bytes_at(kept, 0), bytes_at(kept, k.codes), r.rows, r.columns, dtype, tanh, dx.data_ptr(), stream);
-    });
-    return THPVariable_Wrap(std::move(dx));
+struct Gelu8 : torch::autograd::Function<Gelu8> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, bool tanh) {
+        auto [y, kept] = gelu_forward(x, tanh, true);
+        ctx->save_for_backward({kept});
+        ctx->saved_data["tanh"] = tanh;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward("gelu8", [&]() -> variable_list {
+            const bool tanh = ctx->saved_data["tanh"].toBool();
+            const at::Tensor& dy = on_gpu("dy", grads[0]);
+            const at::Tensor saved = ctx->get_saved_variables()[0];
+            const int dtype = dtype_code("dy", dy);
+            const c10::cuda::CUDAGuard guard(dy.device());
+            const Rows r = rows_of("dy", dy);
+            const Kept k = kept_bytes(r.rows, r.columns);
+            const at::Tensor& kept = kept_of(saved, k.codes + k.scales);
+            same_place("the 8-bit form", kept, dy);
+            at::Tensor dx = new_like(dy);
+            void* stream = stream_of(dy);
+            call([&] {
+                return g.gelu8_backward(r.t.data_ptr(), r.stride, bytes_at(kept, 0), bytes_at(kept, k.codes), r.rows, r.columns, dtype, tanh ? 1 : 0,
+                                        dx.data_ptr(), stream);
+            });
+            return {dx, at::Tensor()};
+        });
+    }
+};
+
+// gelu8(x, tanh) -> y
+PyObject* gelu8(PyObject* const* args, Py_ssize_t nargs) {
+    need_arguments(nargs, 2);
+    const at::Tensor& x = tensor_of("x", args[0]);
+    const bool tanh = truth(args[1]);
+    return THPVariable_Wrap(wants_gradient({&x}) ? Gelu8::apply(x, tanh) : gelu_forward(x, tanh, false).first);
 }
 
-// weight_grad8(dy, bytes, inputs, bias) -> (dw, db or None)
-PyObject* weight_grad8(PyObject* const* args, Py_ssize_t nargs) {
-    need_arguments(nargs, 4);
-    const at::Tensor& dy = tensor_of("dy", args[0]);
+// (dw, db where it is wanted)
+std::pair<at::Tensor, at::Tensor> weight_grad(const at::Tensor& dy, const at::Tensor& given, std::int64_t inputs, bool bias) {
     b2_weight_grad c = {};
     c.dtype = dtype_code("dy", dy);
-    const long long inputs = PyLong_AsLongLong(args[2]);
-    if (inputs == -1 && PyErr_Occurred()) throw Raised{};
     if (inputs < 1) refuse("a projection has at least one input");
-    const bool bias = truth(args[3]);
     const c10::cuda::CUDAGuard guard(dy.device());
     const Rows r = rows_of("dy", dy);
     // (Without outputs there are no rows to be counted by dy, and nothing to be made from them.)
-    std::int64_t rows = r.columns == 0 ? 0 : r.rows;
+    const std::int64_t rows = r.columns == 0 ? 0 : r.rows;
     const Kept k = kept_bytes(rows, inputs);
-    const at::Tensor& kept = r.columns == 0 ? tensor_of("the 8-bit form", args[1]) : kept_of(args[1], k.codes + k.scales);
+    const at::Tensor& kept = r.columns == 0 ? on_gpu("the 8-bit form", given) : kept_of(given, k.codes + k.scales);
     same_place("the 8-bit form", kept, dy);
     const auto options = dy.options().requires_grad(false);
     at::Tensor dw = at::empty({r.columns, inputs}, options), db;
@@ -278,7 +342,56 @@ PyObject* weight_grad8(PyObject* const* args, Py_ssize_t nargs) {
     }
     void* stream = stream_of(dy);
     call([&] { return g.weight_grad8(&c, stream); });
+    return {std::move(dw), std::move(db)};
+}
+
+// weight_grad8(dy, bytes, inputs, bias) -> (dw, db or None)
+PyObject* weight_grad8(PyObject* const* args, Py_ssize_t nargs) {
+    need_arguments(nargs, 4);
+    const long long inputs = PyLong_AsLongLong(args[2]);
+    if (inputs == -1 && PyErr_Occurred()) throw Raised{};
+    auto [dw, db] = weight_grad(tensor_of("dy", args[0]), tensor_of("the 8-bit form", args[1]), inputs, truth(args[3]));
     return two(std::move(dw), std::move(db));
+}
+
+struct Linear8 : torch::autograd::Function<Linear8> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias) {
+        const bool needs = weight.requires_grad() || (bias.has_value() && bias->defined() && bias->requires_grad());
+        ctx->save_for_backward({weight, needs ? pack(x) : at::Tensor()});
+        ctx->saved_data["bias"] = bias.has_value();
+        return at::linear(x, weight, bias);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward("linear8", [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const at::Tensor &dy = grads[0], &weight = saved[0], &kept = saved[1];
+            const at::NoGradGuard no_grad;
+            at::Tensor dx, dw, db;
+            if (ctx->needs_input_grad(0)) dx = at::matmul(dy, weight);
+            const bool bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+            if (kept.defined()) std::tie(dw, db) = weight_grad(on_gpu("dy", dy), kept, weight.size(1), bias);
+            if (!ctx->needs_input_grad(1)) dw = at::Tensor();
+            return {dx, dw, db};
+        });
+    }
+};
+
+// linear8(x, weight, bias or None) -> y
+PyObject* linear8(PyObject* const* args, Py_ssize_t nargs) {
+    need_arguments(nargs, 3);
+    const at::Tensor &x = tensor_of("x", args[0]), &weight = tensor_of("weight", args[1]);
+    const at::Tensor bias = maybe_tensor("bias", args[2]);
+    same_place("weight", weight, x);
+    same_dtype("weight", weight, x);
+    if (x.dim() < 2 || weight.dim() != 2 || x.size(-1) != weight.size(1)) refuse("the input does not go into the weight");
+    if (bias.defined()) {
+        same_place("bias", bias, x);
+        same_dtype("bias", bias, x);
+        if (bias.dim() != 1 || bias.size(0) != weight.size(0)) refuse("the bias does not belong to the weight");
+    }
+    dtype_code("x", x);
+    const std::optional<at::Tensor> b = bias.defined() ? std::optional<at::Tensor>(bias) : std::nullopt;
+    return THPVariable_Wrap(wants_gradient({&x, &weight, &bias}) ? Linear8::apply(x, weight, b) : at::linear(x, weight, b));
 }
 
 // ---- rotation --------------------------------------------------------------------------------------------
@@ -307,11 +420,17 @@ Heads heads_of(const char* what, const at::Tensor& given) {
     return h;
 }
 
+// How to turn: what queries and keys share.
+struct Turn {
+    at::Tensor positions, frequencies;
+    bool interleaved = false;
+    double magnitude = 1.0, eps = 0.0;
+};
+
 // The arguments that all rotations share; `first` gives place and type.
-void shared_arguments(b2_rotation* c, const Heads& first, PyObject* positions_obj, PyObject* frequencies_obj, PyObject* interleaved, PyObject* magnitude) {
+void shared_arguments(b2_rotation* c, const Heads& first, const Turn& turn) {
     c->dtype = dtype_code("queries or keys", first.t);
-    const at::Tensor& positions = tensor_of("positions", positions_obj);
-    const at::Tensor& frequencies = tensor_of("frequencies", frequencies_obj);
+    const at::Tensor &positions = turn.positions, &frequencies = turn.frequencies;
     same_place("positions", positions, first.t);
     same_place("frequencies", frequencies, first.t);
     if (positions.scalar_type() != at::kLong && positions.scalar_type() != at::kInt) refuse("positions must be int64 or int32");
@@ -328,8 +447,9 @@ void shared_arguments(b2_rotation* c, const Heads& first, PyObject* positions_ob
     c->tokens = first.tokens;
     c->dim = static_cast<int>(first.dim);
     c->rotated = static_cast<int>(2 * frequencies.numel());
-    c->interleaved = truth(interleaved) ? 1 : 0;
-    c->magnitude = static_cast<float>(number("magnitude", magnitude));
+    c->interleaved = turn.interleaved ? 1 : 0;
+    c->magnitude = static_cast<float>(turn.magnitude);
+    c->eps = static_cast<float>(turn.eps);
     c->positions = positions.data_ptr();
     c->position_bytes = positions.scalar_type() == at::kLong ? 8 : 4;
     c->position_strides[0] = n == 2 && first.batch > 1 ? positions.stride(0) : 0;
@@ -337,30 +457,31 @@ void shared_arguments(b2_rotation* c, const Heads& first, PyObject* positions_ob
     c->frequencies = static_cast<const double*>(frequencies.data_ptr());
 }
 
-// Queries and keys, either of which may be None.
+// Queries and keys, either of which may be left out.
 struct Both {
     const char* names[2];
     Heads heads[2];
     bool there[2] = {false, false};
     int first = -1;
+    const Heads& any() const { return heads[first]; }
 };
-Both both_of(const char* q_name, const char* k_name, PyObject* q, PyObject* k) {
+Both both_of(const char* q_name, const char* k_name, const at::Tensor& q, const at::Tensor& k) {
     Both b;
     b.names[0] = q_name;
     b.names[1] = k_name;
-    PyObject* objs[2] = {q, k};
+    const at::Tensor* given[2] = {&q, &k};
     for (int i = 0; i < 2; ++i) {
-        if (objs[i] == Py_None) continue;
-        const at::Tensor& t = tensor_of(b.names[i], objs[i]);
+        if (!given[i]->defined()) continue;
+        const at::Tensor& t = on_gpu(b.names[i], *given[i]);
         if (b.first >= 0) {
-            same_place(b.names[i], t, b.heads[b.first].t);
-            same_dtype(b.names[i], t, b.heads[b.first].t);
+            same_place(b.names[i], t, b.any().t);
+            same_dtype(b.names[i], t, b.any().t);
         }
         const c10::cuda::CUDAGuard guard(t.device());
         b.heads[i] = heads_of(b.names[i], t);
         b.there[i] = true;
         if (b.first < 0) b.first = i;
-        const Heads &x = b.heads[b.first], &y = b.heads[i];
+        const Heads &x = b.any(), &y = b.heads[i];
         if (x.t.dim() != y.t.dim() || x.batch != y.batch || x.tokens != y.tokens || x.dim != y.dim)
             refuse(std::string(b.names[0]) + " and " + b.names[1] + " must agree in all but their heads");
     }
@@ -368,23 +489,13 @@ Both both_of(const char* q_name, const char* k_name, PyObject* q, PyObject* k) {
     return b;
 }
 
-const at::Tensor& weight_of(const char* what, PyObject* obj, const Heads& h) {
-    const at::Tensor& w = tensor_of(what, obj);
-    same_place(what, w, h.t);
-    same_dtype(what, w, h.t);
-    if (w.dim() != 1 || w.size(0) != h.dim || !w.is_contiguous()) refuse(std::string(what) + " must be a vector of the head dimension without gaps");
-    return w;
-}
-
-// rotate(q, k, positions, frequencies, interleaved, magnitude, inverse) -> (q, k)
-PyObject* rotate(PyObject* const* args, Py_ssize_t nargs) {
-    need_arguments(nargs, 7);
-    const Both b = both_of("q", "k", args[0], args[1]);
-    const Heads& first = b.heads[b.first];
+// (q, k) turned; what is left out stays undefined.
+std::pair<at::Tensor, at::Tensor> rotate(const Both& b, const Turn& turn, bool inverse) {
+    const Heads& first = b.any();
     const c10::cuda::CUDAGuard guard(first.t.device());
     b2_rotation c = {};
-    shared_arguments(&c, first, args[2], args[3], args[4], args[5]);
-    c.inverse = truth(args[6]) ? 1 : 0;
+    shared_arguments(&c, first, turn);
+    c.inverse = inverse ? 1 : 0;
     at::Tensor out[2];
     for (int i = 0; i < 2; ++i) {
         if (!b.there[i]) continue;
@@ -397,7 +508,89 @@ PyObject* rotate(PyObject* const* args, Py_ssize_t nargs) {
     }
     void* stream = stream_of(first.t);
     call([&] { return g.rotate_heads(&c, stream); });
-    return two(std::move(out[0]), std::move(out[1]));
+    return {std::move(out[0]), std::move(out[1])};
+}
+
+// The outputs that are there, and the tuple that a caller gets of them.
+variable_list defined_of(std::initializer_list<at::Tensor> tensors) {
+    variable_list v;
+    for (const at::Tensor& t : tensors)
+        if (t.defined()) v.push_back(t);
+    return v;
+}
+PyObject* pair_of(variable_list out, bool q, bool k) {
+    at::Tensor first = q ? out.front() : at::Tensor(), second = k ? out.back() : at::Tensor();
+    return two(std::move(first), std::move(second));
+}
+std::optional<at::Tensor> optional_of(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+at::Tensor value_of(const std::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
+
+// The rest of an autograd node: its Turn, and which sides there are with how many heads.
+void save_turn(AutogradContext* ctx, const Turn& turn, std::int64_t q_heads, std::int64_t k_heads) {
+    ctx->saved_data["numbers"] = std::vector<double>{turn.magnitude, turn.eps};
+    ctx->saved_data["whole"] = std::vector<std::int64_t>{turn.interleaved ? 1 : 0, q_heads, k_heads};
+    ctx->set_materialize_grads(false);
+}
+struct SavedTurn {
+    Turn turn;
+    std::int64_t heads[2];
+    at::Tensor grad[2];  // undefined where an output was not used
+};
+SavedTurn saved_turn(AutogradContext* ctx, const variable_list& grads, const at::Tensor& positions, const at::Tensor& frequencies) {
+    SavedTurn s;
+    const std::vector<double> numbers = ctx->saved_data["numbers"].toDoubleVector();
+    const std::vector<std::int64_t> whole = ctx->saved_data["whole"].toIntVector();
+    s.turn = {positions, frequencies, whole[0] != 0, numbers[0], numbers[1]};
+    std::size_t at = 0;
+    for (int i = 0; i < 2; ++i) {
+        s.heads[i] = whole[1 + i];
+        if (s.heads[i] != 0) s.grad[i] = grads[at++];
+    }
+    return s;
+}
+std::int64_t heads_in(const at::Tensor& t) { return t.defined() && t.dim() >= 3 ? t.size(-2) : 0; }
+
+using MaybeTensor = std::optional<at::Tensor>;
+
+struct Rotary : torch::autograd::Function<Rotary> {
+    static variable_list forward(AutogradContext* ctx, const MaybeTensor& q, const MaybeTensor& k, const at::Tensor& positions, const at::Tensor& frequencies,
+                                 bool interleaved, double magnitude) {
+        const Turn turn{positions, frequencies, interleaved, magnitude, 0.0};
+        const at::Tensor q_ = value_of(q), k_ = value_of(k);
+        auto [q_out, k_out] = rotate(both_of("q", "k", q_, k_), turn, false);
+        ctx->save_for_backward({positions, frequencies});
+        save_turn(ctx, turn, heads_in(q_), heads_in(k_));
+        return defined_of({q_out, k_out});
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward("rotary", [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const SavedTurn s = saved_turn(ctx, grads, saved[0], saved[1]);
+            at::Tensor dq, dk;
+            if (s.grad[0].defined() || s.grad[1].defined()) std::tie(dq, dk) = rotate(both_of("dq", "dk", s.grad[0], s.grad[1]), s.turn, true);
+            return {dq, dk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        });
+    }
+};
+
+// rotary(q, k, positions, frequencies, interleaved, magnitude) -> (q, k)
+PyObject* rotary(PyObject* const* args, Py_ssize_t nargs) {
+    need_arguments(nargs, 6);
+    const at::Tensor q = maybe_tensor("q", args[0]), k = maybe_tensor("k", args[1]);
+    const Turn turn{tensor_of("positions", args[2]), tensor_of("frequencies", args[3]), truth(args[4]), number("magnitude", args[5]), 0.0};
+    if (wants_gradient({&q, &k}))
+        return pair_of(Rotary::apply(optional_of(q), optional_of(k), turn.positions, turn.frequencies, turn.interleaved, turn.magnitude), q.defined(), k.defined());
+    auto [q_out, k_out] = rotate(both_of("q", "k", q, k), turn, false);
+    return two(std::move(q_out), std::move(k_out));
+}
+
+const at::Tensor& weight_of(const char* what, const at::Tensor& w, const Heads& h) {
+    if (!w.defined()) refuse(std::string(what) + " is None");
+    on_gpu(what, w);
+    same_place(what, w, h.t);
+    same_dtype(what, w, h.t);
+    if (w.dim() != 1 || w.size(0) != h.dim || !w.is_contiguous()) refuse(std::string(what) + " must be a vector of the head dimension without gaps");
+    return w;
 }
 
 // Bytes of the 8-bit form of queries and keys: codes of both, then scales of both.
@@ -414,125 +607,139 @@ KeptHeads kept_heads(std::int64_t tokens, std::int64_t q_heads, std::int64_t k_h
     return h;
 }
 
-// norm_rotate(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, keep) -> (q, k, bytes or None)
-PyObject* norm_rotate(PyObject* const* args, Py_ssize_t nargs) {
-    need_arguments(nargs, 10);
-    const Both b = both_of("q", "k", args[0], args[1]);
-    const Heads& first = b.heads[b.first];
+constexpr const char* kWeightNames[2] = {"q_weight", "k_weight"};
+
+struct NormRotated {
+    at::Tensor out[2], kept;
+};
+NormRotated norm_rotate(const Both& b, const at::Tensor (&weights)[2], const Turn& turn, bool keep) {
+    const Heads& first = b.any();
     const c10::cuda::CUDAGuard guard(first.t.device());
     b2_rotation c = {};
-    shared_arguments(&c, first, args[4], args[5], args[6], args[7]);
+    shared_arguments(&c, first, turn);
     c.norm = 1;
-    c.eps = static_cast<float>(number("eps", args[8]));
-    const bool keep = truth(args[9]);
-    at::Tensor out[2], kept;
+    for (int i = 0; i < 2; ++i)
+        if (b.there[i]) c.side[i].weight = weight_of(kWeightNames[i], weights[i], b.heads[i]).data_ptr();
+    NormRotated r;
     KeptHeads k8;
     if (keep) {
-        k8 = kept_heads(first.batch * first.tokens, b.there[0] ? b.heads[0].heads : 0, b.there[1] ? b.heads[1].heads : 0, first.dim);
-        kept = new_bytes(first.t, k8.bytes);
+        k8 = kept_heads(first.batch * first.tokens, b.heads[0].heads, b.heads[1].heads, first.dim);
+        r.kept = new_bytes(first.t, k8.bytes);
     }
     for (int i = 0; i < 2; ++i) {
         if (!b.there[i]) continue;
         const Heads& h = b.heads[i];
-        out[i] = new_like(h.t);
+        r.out[i] = new_like(h.t);
         c.side[i].heads = static_cast<int>(h.heads);
         c.side[i].x = h.t.data_ptr();
         std::copy(h.strides, h.strides + 3, c.side[i].x_strides);
-        c.side[i].out = out[i].data_ptr();
-        c.side[i].weight = weight_of(i == 0 ? "q_weight" : "k_weight", args[2 + i], h).data_ptr();
+        c.side[i].out = r.out[i].data_ptr();
         if (keep) {
-            c.side[i].codes = bytes_at(kept, k8.codes[i]);
-            c.side[i].scales = bytes_at(kept, k8.scales[i]);
+            c.side[i].codes = bytes_at(r.kept, k8.codes[i]);
+            c.side[i].scales = bytes_at(r.kept, k8.scales[i]);
         }
     }
     void* stream = stream_of(first.t);
     call([&] { return g.rotate_heads(&c, stream); });
-    PyObject* pair = two(std::move(out[0]), std::move(out[1]));
-    if (pair == nullptr) return nullptr;
-    PyObject* third = keep ? THPVariable_Wrap(std::move(kept)) : Py_NewRef(Py_None);
-    PyObject* t = third != nullptr ? PyTuple_Pack(3, PyTuple_GET_ITEM(pair, 0), PyTuple_GET_ITEM(pair, 1), third) : nullptr;
-    Py_DECREF(pair);
-    Py_XDECREF(third);
-    return t;
+    return r;
 }
 
-// norm_rotate_backward(dq, dk, q, k, bytes, q_heads, k_heads, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps)
-//   -> (gradients of q, k, q_weight, k_weight). Where there are bytes, q and k are None, and q_heads and k_heads are those of the kept form
-//   (a side whose gradient is None is left out).
-PyObject* norm_rotate_backward(PyObject* const* args, Py_ssize_t nargs) {
-    need_arguments(nargs, 14);
-    const Both b = both_of("dq", "dk", args[0], args[1]);
-    const Heads& first = b.heads[b.first];
-    const c10::cuda::CUDAGuard guard(first.t.device());
-    b2_rotation c = {};
-    shared_arguments(&c, first, args[9], args[10], args[11], args[12]);
-    c.norm = 1;
-    c.eps = static_cast<float>(number("eps", args[13]));
-    std::int64_t kept_counts[2];
-    for (int i = 0; i < 2; ++i) {
-        kept_counts[i] = PyLong_AsLongLong(args[5 + i]);
-        if (kept_counts[i] == -1 && PyErr_Occurred()) throw Raised{};
-        if (b.there[i] && kept_counts[i] != b.heads[i].heads) refuse("the gradients have another number of heads than queries and keys");
+struct NormRotary : torch::autograd::Function<NormRotary> {
+    static variable_list forward(AutogradContext* ctx, const MaybeTensor& q, const MaybeTensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight,
+                                 const at::Tensor& positions, const at::Tensor& frequencies, bool interleaved, double magnitude, double eps, bool keep8) {
+        const Turn turn{positions, frequencies, interleaved, magnitude, eps};
+        const at::Tensor q_ = value_of(q), k_ = value_of(k), weights[2] = {value_of(q_weight), value_of(k_weight)};
+        const NormRotated r = norm_rotate(both_of("q", "k", q_, k_), weights, turn, keep8);
+        ctx->save_for_backward({keep8 ? at::Tensor() : q_, keep8 ? at::Tensor() : k_, r.kept, weights[0], weights[1], positions, frequencies});
+        save_turn(ctx, turn, heads_in(q_), heads_in(k_));
+        return defined_of({r.out[0], r.out[1]});
     }
-    const bool kept_form = args[4] != Py_None;
-    KeptHeads k8;
-    if (kept_form) {
-        k8 = kept_heads(first.batch * first.tokens, kept_counts[0], kept_counts[1], first.dim);
-        same_place("the 8-bit form", kept_of(args[4], k8.bytes), first.t);
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward("qk_norm_rotary", [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const SavedTurn s = saved_turn(ctx, grads, saved[5], saved[6]);
+            variable_list result(10);
+            if (!s.grad[0].defined() && !s.grad[1].defined()) return result;
+            const Both b = both_of("dq", "dk", s.grad[0], s.grad[1]);
+            const Heads& first = b.any();
+            const c10::cuda::CUDAGuard guard(first.t.device());
+            b2_rotation c = {};
+            shared_arguments(&c, first, s.turn);
+            c.norm = 1;
+            const at::Tensor& kept = saved[2];
+            KeptHeads k8;
+            if (kept.defined()) {
+                k8 = kept_heads(first.batch * first.tokens, s.heads[0], s.heads[1], first.dim);
+                same_place("the 8-bit form", kept_of(kept, k8.bytes), first.t);
+            }
+            Heads x[2];
+            at::Tensor partial[2];
+            const auto options = first.t.options().requires_grad(false);
+            for (int i = 0; i < 2; ++i) {
+                if (!b.there[i]) continue;
+                const Heads& h = b.heads[i];
+                if (h.heads != s.heads[i]) refuse("a gradient has another shape than its queries or keys");
+                b2_heads& side = c.side[i];
+                result[i] = new_like(h.t);
+                result[2 + i] = at::empty({h.dim}, options);
+                partial[i] = at::empty({B2_HEAD_GRAD_PARTIALS * h.dim}, options.dtype(at::kFloat));
+                side.heads = static_cast<int>(h.heads);
+                side.grad = h.t.data_ptr();
+                std::copy(h.strides, h.strides + 3, side.grad_strides);
+                side.out = result[i].data_ptr();
+                side.weight = weight_of(kWeightNames[i], saved[3 + i], h).data_ptr();
+                side.weight_grad = result[2 + i].data_ptr();
+                side.partial = partial[i].data_ptr();
+                if (kept.defined()) {
+                    side.codes = bytes_at(kept, k8.codes[i]);
+                    side.scales = bytes_at(kept, k8.scales[i]);
+                } else {
+                    if (saved[i].sizes() != h.t.sizes()) refuse("a gradient has another shape than its queries or keys");
+                    same_place("a gradient", h.t, saved[i]);
+                    same_dtype("a gradient", h.t, saved[i]);
+                    x[i] = heads_of(i == 0 ? "q" : "k", saved[i]);
+                    side.x = x[i].t.data_ptr();
+                    std::copy(x[i].strides, x[i].strides + 3, side.x_strides);
+                }
+            }
+            void* stream = stream_of(first.t);
+            call([&] { return g.rotate_heads_backward(&c, stream); });
+            return result;
+        });
     }
-    Heads x[2];
-    at::Tensor out[2], weight_grad[2], partial[2];
-    const auto options = first.t.options().requires_grad(false);
-    for (int i = 0; i < 2; ++i) {
-        if (!b.there[i]) continue;
-        const Heads& h = b.heads[i];
-        b2_heads& s = c.side[i];
-        out[i] = new_like(h.t);
-        weight_grad[i] = at::empty({h.dim}, options);
-        partial[i] = at::empty({B2_HEAD_GRAD_PARTIALS * h.dim}, options.dtype(at::kFloat));
-        s.heads = static_cast<int>(h.heads);
-        s.grad = h.t.data_ptr();
-        std::copy(h.strides, h.strides + 3, s.grad_strides);
-        s.out = out[i].data_ptr();
-        s.weight = weight_of(i == 0 ? "q_weight" : "k_weight", args[7 + i], h).data_ptr();
-        s.weight_grad = weight_grad[i].data_ptr();
-        s.partial = partial[i].data_ptr();
-        if (kept_form) {
-            const at::Tensor& kept = THPVariable_Unpack(args[4]);
-            s.codes = bytes_at(kept, k8.codes[i]);
-            s.scales = bytes_at(kept, k8.scales[i]);
-        } else {
-            const at::Tensor& t = tensor_of(i == 0 ? "q" : "k", args[2 + i]);
-            same_place(i == 0 ? "q" : "k", t, first.t);
-            same_dtype(i == 0 ? "q" : "k", t, first.t);
-            if (t.sizes() != h.t.sizes()) refuse("a gradient has another shape than its queries or keys");
-            x[i] = heads_of(i == 0 ? "q" : "k", t);
-            s.x = x[i].t.data_ptr();
-            std::copy(x[i].strides, x[i].strides + 3, s.x_strides);
-        }
-    }
-    void* stream = stream_of(first.t);
-    call([&] { return g.rotate_heads_backward(&c, stream); });
-    PyObject* heads = two(std::move(out[0]), std::move(out[1]));
-    PyObject* weights = heads != nullptr ? two(std::move(weight_grad[0]), std::move(weight_grad[1])) : nullptr;
-    PyObject* all = weights != nullptr ? PySequence_Concat(heads, weights) : nullptr;
-    Py_XDECREF(heads);
-    Py_XDECREF(weights);
-    return all;
+};
+
+// qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, keep8) -> (q, k)
+PyObject* qk_norm_rotary(PyObject* const* args, Py_ssize_t nargs) {
+    need_arguments(nargs, 10);
+    const at::Tensor q = maybe_tensor("q", args[0]), k = maybe_tensor("k", args[1]);
+    const at::Tensor weights[2] = {maybe_tensor(kWeightNames[0], args[2]), maybe_tensor(kWeightNames[1], args[3])};
+    const Turn turn{tensor_of("positions", args[4]), tensor_of("frequencies", args[5]), truth(args[6]), number("magnitude", args[7]), number("eps", args[8])};
+    const bool keep8 = truth(args[9]);
+    if (wants_gradient({&q, &k, &weights[0], &weights[1]}))
+        return pair_of(NormRotary::apply(optional_of(q), optional_of(k), optional_of(weights[0]), optional_of(weights[1]), turn.positions, turn.frequencies,
+                                         turn.interleaved, turn.magnitude, turn.eps, keep8),
+                       q.defined(), k.defined());
+    const NormRotated r = norm_rotate(both_of("q", "k", q, k), weights, turn, false);
+    return two(r.out[0], r.out[1]);
 }
 
 template <PyObject* (*kFunction)(PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS  // an allocation that fails raises torch's own error
     if (g.last_error == nullptr) {
-        PyErr_SetString(PyExc_RuntimeError, "bind() first");
+        PyErr_SetString(PyExc_RuntimeError, "bind_train() first");
         return nullptr;
     }
     try {
         return kFunction(args, nargs);
+    } catch (const Refused& e) {
+        PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (const Failed& e) {
+        PyErr_SetString(g_error_class, e.what());
     } catch (const Raised&) {
-        return nullptr;
     }
+    return nullptr;
     END_HANDLE_TH_ERRORS
 }
 
@@ -541,12 +748,11 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef train_methods[] = {
     {"pack8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<pack8>)), METH_FASTCALL, nullptr},
     {"unpack8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<unpack8>)), METH_FASTCALL, nullptr},
-    {"gelu8_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<gelu8_forward>)), METH_FASTCALL, nullptr},
-    {"gelu8_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<gelu8_backward>)), METH_FASTCALL, nullptr},
+    {"gelu8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<gelu8>)), METH_FASTCALL, nullptr},
     {"weight_grad8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<weight_grad8>)), METH_FASTCALL, nullptr},
-    {"rotate", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<rotate>)), METH_FASTCALL, nullptr},
-    {"norm_rotate", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<norm_rotate>)), METH_FASTCALL, nullptr},
-    {"norm_rotate_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<norm_rotate_backward>)), METH_FASTCALL, nullptr},
+    {"linear8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<linear8>)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<rotary>)), METH_FASTCALL, nullptr},
+    {"qk_norm_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<qk_norm_rotary>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 bool bind_train(PyObject* error_class, PyObject* addresses) {

@@ -276,6 +276,15 @@ def test_on_another_stream_and_in_graphs_that_live_together():
             assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_no_second_derivative():
+    x = torch.randn(8, 64, device="cuda", requires_grad=True)
+    w = torch.randn(16, 64, device="cuda", requires_grad=True)
+    for y, leaf in ((ops.gelu8(x), x), (ops.linear8(x, w), w)):
+        (g,) = torch.autograd.grad(y.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            g.sum().backward()
+
+
 def test_refusals():
     x = torch.ones(4, 64, device="cuda")
     p = ops.pack8(x)
