@@ -3,6 +3,8 @@ vocabulary 50257, context 1024) used as the gradient list of the bucketed all-re
 a tiny trainable module of the same structure for data-parallel smoke tests."""
 import torch
 
+from .. import ops
+
 
 def gpt2_small_shapes(hidden=768, layers=12, vocab=50257, context=1024):
     shapes = [(vocab, hidden), (context, hidden)]
@@ -17,31 +19,85 @@ def gpt2_small_shapes(hidden=768, layers=12, vocab=50257, context=1024):
     return shapes
 
 
-class _Block(torch.nn.Module):
-    def __init__(self, hidden, heads):
+class _Attention(torch.nn.Module):
+    """Self-attention whose queries and keys are turned by their positions (``rotary``), after a norm of each head where ``qk_norm`` says so.
+    Projections keep their inputs in 8 bits where ``checkpoints`` says so; so do the norms."""
+
+    def __init__(self, hidden, heads, rotary, qk_norm, checkpoints):
         super().__init__()
+        self.heads, self.rotary, self.checkpoints = heads, rotary, checkpoints
+        self.c_attn = torch.nn.Linear(hidden, 3 * hidden)
+        self.c_proj = torch.nn.Linear(hidden, hidden)
+        if qk_norm:
+            self.q_norm = torch.nn.Parameter(torch.ones(hidden // heads))
+            self.k_norm = torch.nn.Parameter(torch.ones(hidden // heads))
+        self.qk_norm = qk_norm
+        self._frequencies = None  # (not a buffer: it stays in 64 bits whatever type the module is cast to)
+
+    def frequencies(self, device):
+        if self._frequencies is None or self._frequencies.device != device:
+            rotated = self.c_proj.in_features // self.heads if self.rotary else 0
+            self._frequencies = ops.rotary_frequencies(rotated, device=device)[0] if rotated else torch.empty(0, dtype=torch.float64, device=device)
+        return self._frequencies
+
+    def forward(self, x):
+        b, t, hidden = x.shape
+        q, k, v = (p.view(b, t, self.heads, -1) for p in _linear(x, self.c_attn, self.checkpoints).split(hidden, -1))
+        positions = torch.arange(t, device=x.device)
+        if self.qk_norm:
+            q, k = ops.qk_norm_rotary(q, k, self.q_norm, self.k_norm, positions, self.frequencies(x.device), keep=self.checkpoints)
+        elif self.rotary:
+            q, k = ops.rotary(q, k, positions, self.frequencies(x.device))
+        y = torch.nn.functional.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
+        return _linear(y.transpose(1, 2).reshape(b, t, hidden), self.c_proj, self.checkpoints)
+
+
+def _linear(x, layer, checkpoints):
+    return layer(x) if checkpoints is None else ops.linear8(x, layer.weight, layer.bias)
+
+
+class _Block(torch.nn.Module):
+    def __init__(self, hidden, heads, rotary=False, qk_norm=False, checkpoints=None):
+        super().__init__()
+        self.checkpoints = checkpoints
+        self.plain_attention = not rotary and not qk_norm and checkpoints is None
         self.ln_1 = torch.nn.LayerNorm(hidden)
-        self.attn = torch.nn.MultiheadAttention(hidden, heads, batch_first=True)
+        self.attn = (torch.nn.MultiheadAttention(hidden, heads, batch_first=True) if self.plain_attention
+                     else _Attention(hidden, heads, rotary, qk_norm, checkpoints))
         self.ln_2 = torch.nn.LayerNorm(hidden)
         self.mlp = torch.nn.Sequential(torch.nn.Linear(hidden, 4 * hidden), torch.nn.GELU(), torch.nn.Linear(4 * hidden, hidden))
 
     def forward(self, x):
         h = self.ln_1(x)
-        x = x + self.attn(h, h, h, need_weights=False)[0]
-        return x + self.mlp(self.ln_2(x))
+        x = x + (self.attn(h, h, h, need_weights=False)[0] if self.plain_attention else self.attn(h))
+        h = self.ln_2(x)
+        if self.checkpoints is None:
+            return x + self.mlp(h)
+        return x + _linear(ops.gelu8(_linear(h, self.mlp[0], self.checkpoints)), self.mlp[2], self.checkpoints)
 
 
 class TinyGPT2(torch.nn.Module):
-    def __init__(self, vocab=512, context=64, hidden=64, layers=2, heads=4):
+    """``positions``: "learned" (an embedding) or "rotary" (queries and keys are turned). ``qk_norm``: a norm of each head of queries and keys.
+    ``checkpoints``: "int8" keeps the inputs of projections, activations and head norms in 8 bits for the backward pass, None keeps them as they
+    are. All but the defaults run on CUDA only (:mod:`nano_nccl_b200.ops`)."""
+
+    def __init__(self, vocab=512, context=64, hidden=64, layers=2, heads=4, positions="learned", qk_norm=False, checkpoints=None):
         super().__init__()
+        if positions not in ("learned", "rotary"):
+            raise ValueError(f"unknown kind of positions '{positions}'")
+        if checkpoints not in (None, "int8"):
+            raise ValueError(f"unknown kind of checkpoints '{checkpoints}'")
+        if (positions == "rotary" or qk_norm) and (hidden % heads or (hidden // heads) % 2 or hidden // heads > 256):
+            raise ValueError(f"{heads} heads of an even size up to 256 do not make {hidden}")
         self.wte = torch.nn.Embedding(vocab, hidden)
-        self.wpe = torch.nn.Embedding(context, hidden)
-        self.blocks = torch.nn.ModuleList([_Block(hidden, heads) for _ in range(layers)])
+        self.wpe = torch.nn.Embedding(context, hidden) if positions == "learned" else None
+        self.blocks = torch.nn.ModuleList([_Block(hidden, heads, positions == "rotary", qk_norm, checkpoints) for _ in range(layers)])
         self.ln_f = torch.nn.LayerNorm(hidden)
 
     def forward(self, tokens):
-        pos = torch.arange(tokens.shape[1], device=tokens.device)
-        x = self.wte(tokens) + self.wpe(pos)
+        x = self.wte(tokens)
+        if self.wpe is not None:
+            x = x + self.wpe(torch.arange(tokens.shape[1], device=tokens.device))
         for b in self.blocks:
             x = b(x)
         return self.ln_f(x) @ self.wte.weight.t()
