@@ -43,7 +43,7 @@ DType dtype_of(int code) {
 bool aligned(const void* p, std::size_t n) { return reinterpret_cast<std::uintptr_t>(p) % n == 0; }
 
 void check_kept(const void* codes, const void* scales, std::size_t rows, std::size_t columns, bool needed = true) {
-    B2_REQUIRE(columns < (1ull << 31) && rows < (1ull << 31), "more than 2^31 rows or columns");
+    B2_REQUIRE(columns <= (1ull << 30) && rows < (1ull << 31), "more than 2^31 rows or 2^30 columns");
     B2_REQUIRE(rows * ((columns + 31) / 32) < (1ull << 30), "more than 2^30 blocks of 32 elements");
     if (rows == 0 || columns == 0 || !needed) return;
     B2_REQUIRE(codes != nullptr && scales != nullptr, "codes and scales must be non-null");

@@ -32,8 +32,11 @@ struct Kept8Args {
     char* out;
     unsigned char* codes;
     unsigned char* scales;
-    unsigned columns, blocks;  // of a row
-    unsigned items;            // half blocks (flat) or blocks (ragged) of all rows
+    u64 elements;     // of all rows
+    unsigned columns;
+    Divisor halves;   // half blocks of a row
+    unsigned items;   // half blocks of all rows
+    Divisor by_columns;
 };
 
 // exp(-x^2/2) and 1 - Phi(|x|) of two numbers.
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) keep8_kernel(const Kept8Args a) {
     for (int u = 0; u < U; ++u) {
         const unsigned i = first + u * kThreads;
         if (i < a.items) {
-            const unsigned row = i / (2u * a.blocks), half = i - row * (2u * a.blocks);
+            const unsigned row = a.halves.divide(i), half = i - row * a.halves.d;
             x[u].load(a.in + (long long)row * a.stride + (u64)half * (16 * sizeof(T)));
         }
     }
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const Kept8Args a) {
             c[u] = load16_once(reinterpret_cast<const uint4*>(a.codes) + i);
             scale[u] = a.scales[i >> 1];
             if constexpr (kAct != Activation::None) {
-                const unsigned row = i / (2u * a.blocks), half = i - row * (2u * a.blocks);
+                const unsigned row = a.halves.divide(i), half = i - row * a.halves.d;
                 dy[u].load(a.in + (long long)row * a.stride + (u64)half * (16 * sizeof(T)));
             }
         }
@@ -279,67 +282,213 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const Kept8Args a) {
     }
 }
 
-// Any columns, strides and alignment: a warp takes a block, a lane an element, so that neighbouring lanes touch neighbouring bytes.
-constexpr int kRaggedBlocks = 4;  // blocks in flight per warp
+// ---- any columns, strides and alignment ------------------------------------------------------------------
+// Inputs are read as the aligned 16 bytes that they lie in, and shifted; only those that hold a wanted element are touched. What is written to rows without
+// gaps is cut where the memory is aligned, wherever rows and blocks begin: a thread makes 16 bytes of the output.
 
-template <typename T, Activation kAct>
-__global__ void __launch_bounds__(kThreads) keep8_ragged_kernel(const Kept8Args a) {
-    constexpr int U = kRaggedBlocks;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned lane = threadIdx.x & 31u;
-    const unsigned first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * U;
-    float f[U];
-    u64 at[U];  // of the element among rows without gaps
+// N neighbouring elements at p, of which `count` are there; the others are zeros.
+template <typename T, int N>
+__device__ __forceinline__ void load_any(const char* p, unsigned count, unsigned (&w)[N * sizeof(T) / 4]) {
+    constexpr unsigned W = N * sizeof(T) / 4, G = W / 4 + 1;
+    const unsigned shift = (unsigned)(reinterpret_cast<std::uintptr_t>(p) & 15u);
+    const char* base = p - shift;
+    unsigned r[4 * G];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned i = first + u;
-        const unsigned row = i / a.blocks, column = (i - row * a.blocks) * kBlock8 + lane;
-        const bool there = i < a.items && column < a.columns;
-        at[u] = there ? (u64)row * a.columns + column : ~0ull;
-        f[u] = there ? Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)row * a.stride) + column)) : 0.0f;
+    for (unsigned g = 0; g < G; ++g) {
+        const uint4 v = 16u * g < shift + count * (unsigned)sizeof(T) && count != 0u ? *reinterpret_cast<const uint4*>(base + 16 * g) : make_uint4(0u, 0u, 0u, 0u);
+        r[4 * g] = v.x;
+        r[4 * g + 1] = v.y;
+        r[4 * g + 2] = v.z;
+        r[4 * g + 3] = v.w;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned i = first + u;
-        if (i < a.items) {  // the same for the whole warp
-            if (kAct == Activation::None || a.codes != nullptr) {
-                const unsigned scale = scale8<T>(__reduce_max_sync(0xffffffffu, magnitude_bits(f[u])));
-                a.codes[(u64)i * kBlock8 + lane] = (unsigned char)finite8(encode8(f[u], inverse_step8(scale)), scale);
-                if (lane == 0) a.scales[i] = (unsigned char)scale;
-            }
-            if constexpr (kAct != Activation::None)
-                if (at[u] != ~0ull) reinterpret_cast<T*>(a.out)[at[u]] = Elem<T>::from_f(activate<kAct>(make_float2(f[u], 0.0f)).x);
+    for (unsigned i = 0; i < W + 2; ++i) r[i] = shift & 8u ? r[i + 2] : r[i];
+#pragma unroll
+    for (unsigned i = 0; i < W + 1; ++i) r[i] = shift & 4u ? r[i + 1] : r[i];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (unsigned i = 0; i < W; ++i) w[i] = shift & 2u ? __funnelshift_r(r[i], r[i + 1], 16) : r[i];
+    } else {
+#pragma unroll
+        for (unsigned i = 0; i < W; ++i) w[i] = r[i];
+    }
+    if (count < (unsigned)N) {
+#pragma unroll
+        for (unsigned i = 0; i < W; ++i) {
+            if constexpr (sizeof(T) == 2) w[i] = 2u * i + 1u < count ? w[i] : (2u * i < count ? w[i] & 0xffffu : 0u);
+            else w[i] = i < count ? w[i] : 0u;
         }
     }
 }
 
+template <typename T>
+constexpr int kGranule = 16 / sizeof(T);  // elements of 16 bytes
+
+template <typename T>
+__device__ __forceinline__ float2 pair_in(const unsigned* w, int i) {
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if constexpr (std::is_same_v<T, __half>) return h2_to_f2(w[i]);
+    else return b2_to_f2(w[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store_granule(char* p, const float2 (&f)[kGranule<T> / 2]) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < kGranule<T> / 2; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            w[2 * i] = __float_as_uint(f[i].x);
+            w[2 * i + 1] = __float_as_uint(f[i].y);
+        } else {
+            w[i] = std::is_same_v<T, __half> ? f2_to_h2(f[i].x, f[i].y) : f2_to_b2(f[i].x, f[i].y);
+        }
+    }
+    store16_once(p, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// Where element `from + offset` of all lies, `from` being element (row, column): offsets are small.
+struct Spot {
+    unsigned row, column;
+};
+__device__ __forceinline__ Spot spot_at(const Kept8Args& a, const Spot& from, unsigned offset) {
+    const unsigned in = from.column + offset, rows = a.by_columns.divide(in);
+    return {from.row + rows, in - rows * a.columns};
+}
+
+// One element of x^, or of dx.
 template <typename T, Activation kAct>
-__global__ void __launch_bounds__(kThreads) read8_ragged_kernel(const Kept8Args a) {
-    constexpr int U = kRaggedBlocks;
+__device__ __forceinline__ float read_one(const Kept8Args& a, const Spot& s) {
+    const u64 half = (u64)s.row * a.halves.d;
+    const float v = decode8<0>(a.codes[half * 16u + s.column], step8(a.scales[half / 2u + s.column / kBlock8]));
+    if constexpr (kAct == Activation::None) return v;
+    const float dy = Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)s.row * a.stride) + s.column));
+    return through<kAct>(make_float2(v, 0.0f), make_float2(dy, 0.0f)).x;
+}
+template <typename T, Activation kAct>
+__device__ __forceinline__ float activate_one(const Kept8Args& a, const Spot& s) {
+    return activate<kAct>(make_float2(Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)s.row * a.stride) + s.column)), 0.0f)).x;
+}
+// The elements of a granule that lies across rows, or not wholly in the output.
+template <typename T, typename F>
+__device__ __forceinline__ void one_by_one(const Kept8Args& a, u64 begin, u64 end, const Spot& from, u64 origin, F&& f) {
+    for (u64 e = begin; e < end; ++e) reinterpret_cast<T*>(a.out)[e] = Elem<T>::from_f(f(spot_at(a, from, (unsigned)(e - origin))));
+}
+
+// Elements by which the output lies behind a multiple of 16 bytes.
+template <typename T>
+__device__ __forceinline__ unsigned behind(const Kept8Args& a) {
+    return (unsigned)(reinterpret_cast<std::uintptr_t>(a.out) & 15u) / (unsigned)sizeof(T);
+}
+
+template <typename T, Activation kAct>
+__global__ void __launch_bounds__(kThreads) keep8_any_kernel(const Kept8Args a) {
+    constexpr int U = kInFlight<T>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned lane = threadIdx.x & 31u;
-    const unsigned first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * U;
-    unsigned code[U], scale[U];
-    float dy[U];
-    u64 at[U];
+    const unsigned begin = blockIdx.x * (kThreads * U);
+    if (kAct == Activation::None || a.codes != nullptr) {
+        Sixteen<T> x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned i = first + u;
-        const unsigned row = i / a.blocks, column = (i - row * a.blocks) * kBlock8 + lane;
-        const bool there = i < a.items && column < a.columns;
-        at[u] = there ? (u64)row * a.columns + column : ~0ull;
-        code[u] = there ? a.codes[(u64)i * kBlock8 + lane] : 0u;
-        scale[u] = there ? a.scales[i] : 1u;
-        if constexpr (kAct != Activation::None)
-            dy[u] = there ? Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)row * a.stride) + column)) : 0.0f;
+        for (int u = 0; u < U; ++u) {
+            const unsigned i = begin + threadIdx.x + u * kThreads;
+            const unsigned row = a.halves.divide(i), column = (i - row * a.halves.d) * 16u;
+            const unsigned count = i < a.items && column < a.columns ? min(16u, a.columns - column) : 0u;
+            load_any<T, 16>(a.in + (count == 0u ? 0ll : (long long)row * a.stride + (long long)(column * (unsigned)sizeof(T))), count, x[u].w);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned i = begin + threadIdx.x + u * kThreads;
+            unsigned amax = x[u].amax();
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            if (i < a.items) {
+                const unsigned scale = scale8<T>(amax);
+                store16_once(a.codes + (u64)i * 16u, x[u].codes(scale));
+                if ((i & 1u) == 0) a.scales[i >> 1] = (unsigned char)scale;
+            }
+        }
     }
+    if constexpr (kAct != Activation::None) {
+        // The elements of the same half blocks, by granules of the output that begin among them; they are in L1.
+        constexpr unsigned E = kGranule<T>;
+        const unsigned end = min(a.items, begin + kThreads * U), m = behind<T>(a);
+        const auto first_of = [&](unsigned i) {
+            const unsigned row = a.halves.divide(i);
+            return Spot{row, min(a.columns, (i - row * a.halves.d) * 16u)};
+        };
+        const Spot from = first_of(begin), to = first_of(end);
+        const u64 origin = (u64)from.row * a.columns + from.column, stop = end == a.items ? a.elements : (u64)to.row * a.columns + to.column;
+        const u64 k0 = origin == 0 ? 0 : (origin + m + E - 1) / E, k1 = (stop + m + E - 1) / E;
+        for (u64 k = k0 + threadIdx.x; k < k1; k += kThreads) {
+            const u64 e = k * E - m;  // before 0 for the first granule of an output that is not aligned
+            const Spot s = spot_at(a, from, k * E < m ? 0u : (unsigned)(e - origin));
+            if (k * E >= m && e + E <= a.elements && s.column + E <= a.columns) {
+                unsigned w[4];
+                load_any<T, E>(a.in + (long long)s.row * a.stride + (long long)(s.column * (unsigned)sizeof(T)), E, w);
+                float2 f[E / 2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        float f = decode8<0>(code[u], step8(scale[u]));
-        if constexpr (kAct != Activation::None) f = through<kAct>(make_float2(f, 0.0f), make_float2(dy[u], 0.0f)).x;
-        if (at[u] != ~0ull) reinterpret_cast<T*>(a.out)[at[u]] = Elem<T>::from_f(f);
+                for (unsigned i = 0; i < E / 2; ++i) f[i] = activate<kAct>(pair_in<T>(w, i));
+                store_granule<T>(a.out + e * sizeof(T), f);
+            } else {
+                one_by_one<T>(a, k * E < m ? 0 : e, min(a.elements, e + E), from, origin, [&](const Spot& t) { return activate_one<T, kAct>(a, t); });
+            }
+        }
+    }
+}
+
+constexpr unsigned kGranules = 2;  // of a thread
+
+template <typename T, Activation kAct>
+__global__ void __launch_bounds__(kThreads) read8_any_kernel(const Kept8Args a) {
+    constexpr unsigned E = kGranule<T>;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned m = behind<T>(a);
+    const u64 k0 = (u64)blockIdx.x * (kThreads * kGranules);
+    const u64 origin = k0 * E < m ? 0 : k0 * E - m;
+    __shared__ Spot first;
+    if (threadIdx.x == 0) {  // a division of 64 bits, once
+        const u64 row = origin / a.columns;
+        first = {(unsigned)row, (unsigned)(origin - row * a.columns)};
+    }
+    __syncthreads();
+    const Spot from = first;
+#pragma unroll
+    for (unsigned u = 0; u < kGranules; ++u) {
+        const u64 k = k0 + threadIdx.x + u * kThreads;
+        const bool before = k * E < m;
+        const u64 e = k * E - m;
+        if (!before && e >= a.elements) continue;
+        const Spot s = spot_at(a, from, before ? 0u : (unsigned)(e - origin));
+        if (before || e + E > a.elements || s.column + E > a.columns) {
+            one_by_one<T>(a, before ? 0 : e, min(a.elements, e + E), from, origin, [&](const Spot& t) { return read_one<T, kAct>(a, t); });
+            continue;
+        }
+        // E codes, at any address, and the steps of the one or two blocks that they belong to.
+        const u64 half = (u64)s.row * a.halves.d;
+        const unsigned char* codes = a.codes + half * 16u + s.column;
+        const unsigned shift = (unsigned)(reinterpret_cast<std::uintptr_t>(codes) & 3u) * 8u;
+        const unsigned* words = reinterpret_cast<const unsigned*>(codes - shift / 8u);
+        unsigned c[E / 4 + 1];
+#pragma unroll
+        for (unsigned i = 0; i < E / 4; ++i) c[i] = words[i];
+        c[E / 4] = shift != 0u ? words[E / 4] : 0u;
+        const unsigned char* scale = a.scales + half / 2u + s.column / kBlock8;
+        const unsigned in_block = s.column % kBlock8;
+        const float near = step8(scale[0]), far = in_block + E > kBlock8 ? step8(scale[1]) : near;
+        unsigned dy[4];
+        if constexpr (kAct != Activation::None)
+            load_any<T, E>(a.in + (long long)s.row * a.stride + (long long)(s.column * (unsigned)sizeof(T)), E, dy);
+        float2 f[E / 2];
+#pragma unroll
+        for (unsigned i = 0; i < E / 4; ++i) {
+            const unsigned w = __funnelshift_r(c[i], c[i + 1], shift);
+            f[2 * i] = make_float2(decode8<0>(w, in_block + 4u * i < kBlock8 ? near : far), decode8<1>(w, in_block + 4u * i + 1u < kBlock8 ? near : far));
+            f[2 * i + 1] = make_float2(decode8<2>(w, in_block + 4u * i + 2u < kBlock8 ? near : far), decode8<3>(w, in_block + 4u * i + 3u < kBlock8 ? near : far));
+        }
+        if constexpr (kAct != Activation::None) {
+#pragma unroll
+            for (unsigned i = 0; i < E / 2; ++i) f[i] = through<kAct>(f[i], pair_in<T>(dy, i));
+        }
+        store_granule<T>(a.out + e * sizeof(T), f);
     }
 }
 
@@ -352,19 +501,22 @@ cudaError_t start(const Kept8Call& c, bool keep) {
     a.out = static_cast<char*>(c.out);
     a.codes = c.codes;
     a.scales = c.scales;
+    const unsigned blocks = (unsigned)((c.columns + kBlock8 - 1) / kBlock8);
     a.columns = (unsigned)c.columns;
-    a.blocks = (unsigned)((c.columns + kBlock8 - 1) / kBlock8);
+    a.by_columns = Divisor(a.columns);
+    a.halves = Divisor(2u * blocks);
+    a.items = (unsigned)(c.rows * blocks * 2);
+    a.elements = (u64)c.rows * c.columns;
     const std::uintptr_t addresses = reinterpret_cast<std::uintptr_t>(c.in) | reinterpret_cast<std::uintptr_t>(c.out) |
                                      reinterpret_cast<std::uintptr_t>(c.codes) | (std::uintptr_t)(c.rows > 1 ? a.stride : 0);
-    if (c.columns % kBlock8 == 0 && addresses % 32 == 0) {
-        a.items = (unsigned)(c.rows * a.blocks * 2);
-        const unsigned grid = (a.items + kThreads * kInFlight<T> - 1) / (kThreads * kInFlight<T>);
-        return launch_dependent<Kept8Args>(keep ? keep8_kernel<T, kAct> : read8_kernel<T, kAct>, grid, kThreads, 0, c.stream, a);
-    }
-    a.items = (unsigned)(c.rows * a.blocks);
-    constexpr unsigned kPerCta = kThreads / 32 * kRaggedBlocks;
-    return launch_dependent<Kept8Args>(keep ? keep8_ragged_kernel<T, kAct> : read8_ragged_kernel<T, kAct>, (a.items + kPerCta - 1) / kPerCta,
-                                       kThreads, 0, c.stream, a);
+    constexpr unsigned kPerCta = kThreads * kInFlight<T>;
+    const unsigned ctas = (a.items + kPerCta - 1) / kPerCta;
+    if (c.columns % kBlock8 == 0 && addresses % 32 == 0)
+        return launch_dependent<Kept8Args>(keep ? keep8_kernel<T, kAct> : read8_kernel<T, kAct>, ctas, kThreads, 0, c.stream, a);
+    if (keep) return launch_dependent<Kept8Args>(keep8_any_kernel<T, kAct>, ctas, kThreads, 0, c.stream, a);
+    constexpr unsigned kElements = kThreads * kGranules * kGranule<T>;
+    const u64 granules = (a.elements + kGranule<T> + kElements - 1) / kElements;  // one more for an output that is not aligned
+    return launch_dependent<Kept8Args>(read8_any_kernel<T, kAct>, (unsigned)granules, kThreads, 0, c.stream, a);
 }
 
 template <typename T>

@@ -44,17 +44,6 @@ struct View {
     i64 batch, token, head;  // bytes
 };
 
-// n / d for n below 2^31, as a product.
-struct Divisor {
-    unsigned d, factor, shift;
-    __device__ __forceinline__ unsigned divide(unsigned n) const { return (unsigned)(((u64)n * factor) >> shift); }
-};
-Divisor divisor_of(unsigned d) {
-    unsigned bits = 0;
-    while ((1ull << bits) < d) ++bits;
-    return {d, (unsigned)((1ull << (31 + bits)) / d + 1), 31 + bits};
-}
-
 // How tokens are dealt out: a tile of tokens to a warp, or to `split` warps, each for some of the heads.
 struct Cut {
     unsigned tile, split;
@@ -668,7 +657,7 @@ RotationArgs args_of(const RotationCall& c, const Shape& shape, unsigned bytes) 
     a.positions64 = c.positions64;
     a.frequencies = c.frequencies;
     a.all = (unsigned)(c.batch * c.tokens);
-    a.tokens = divisor_of((unsigned)std::max(1ll, c.tokens));
+    a.tokens = Divisor((unsigned)std::max(1ll, c.tokens));
     a.dim = (unsigned)c.dim;
     a.rotated = (unsigned)c.rotated;
     a.pitch = (a.dim + 15u) / 16u * 16u;
@@ -689,7 +678,7 @@ RotationArgs args_of(const RotationCall& c, const Shape& shape, unsigned bytes) 
         t.scales = s.scales;
         t.weight_grad = static_cast<char*>(s.weight_grad);
         t.partial = s.partial;
-        if (s.heads != 0) t.heads = divisor_of((unsigned)s.heads);
+        if (s.heads != 0) t.heads = Divisor((unsigned)s.heads);
     }
     return a;
 }

@@ -5,6 +5,19 @@
 
 namespace b200ccl::kernels {
 
+// n / d for n below 2^31, as a product.
+struct Divisor {
+    unsigned d = 0, factor = 0, shift = 0;
+    Divisor() = default;
+    explicit Divisor(unsigned divisor) : d(divisor) {
+        unsigned bits = 0;
+        while ((1ull << bits) < d) ++bits;
+        shift = 31 + bits;
+        factor = (unsigned)((1ull << shift) / d + 1);
+    }
+    __device__ __forceinline__ unsigned divide(unsigned n) const { return (unsigned)(((unsigned long long)n * factor) >> shift); }
+};
+
 template <typename Args>
 cudaError_t launch_dependent(void (*kernel)(Args), dim3 grid, unsigned threads, std::size_t shared, cudaStream_t stream, const Args& args) {
     cudaLaunchConfig_t config = {};

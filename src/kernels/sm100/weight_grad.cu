@@ -58,8 +58,10 @@ constexpr unsigned kGroups = 4, kGroupWarps = 2;  // of transform warps: a group
 constexpr unsigned kChunkSteps = 8;   // fp32: steps of each part between two additions to the sums in memory
 constexpr unsigned kMaxPairs = 74;    // 148 SMs
 constexpr unsigned kFinishRows = 16;  // outputs of a tile that a CTA of finish_kernel adds up
-// Shared memory, from a multiple of 1024 bytes on: dY of the stages, X^ of the groups, codes of the stages, barriers.
-constexpr unsigned kAtX = kStages * kOperandBytes, kAtCodes = kAtX + kGroups * kOperandBytes, kAtBarriers = kAtCodes + kStages * kCodeBytes;
+constexpr unsigned kTurnBytes = 32 * 32 * 4;  // of an epilogue warp: 32 outputs of its 32 features
+// Shared memory, from a multiple of 1024 bytes on: dY of the stages, X^ of the groups, codes of the stages, what the epilogue turns, barriers.
+constexpr unsigned kAtX = kStages * kOperandBytes, kAtCodes = kAtX + kGroups * kOperandBytes, kAtTurn = kAtCodes + kStages * kCodeBytes,
+                   kAtBarriers = kAtTurn + 4 * kTurnBytes;
 constexpr unsigned kShared = kAtBarriers + 512 + 1024;
 static_assert(kShared <= 227 * 1024);
 
@@ -72,6 +74,7 @@ struct alignas(64) WeightGradArgs {
     float* bias;       // [tiles + pairs][256], or null
     unsigned* status;  // host memory
     u64 pitch;         // bytes of a token's codes
+    bool wide;         // rows of `out` start at multiples of 16 bytes
     unsigned tokens, inputs, outputs;
     unsigned feature_tiles, parts, steps_of_part, steps_of_tile;
     unsigned pairs, waves;  // of whole tiles
@@ -186,6 +189,48 @@ __device__ __forceinline__ Spot spot_of(const WeightGradArgs& a, unsigned k) {
     const unsigned chunk = k / (a.parts * kChunkSteps), in_chunk = k - chunk * (a.parts * kChunkSteps);
     const unsigned length = min(kChunkSteps, a.steps_of_part - chunk * kChunkSteps), part = in_chunk / length;
     return {part, chunk * kChunkSteps + in_chunk - part * length};
+}
+
+// Writes 32 outputs of a warp's 32 features, f[j] being output j of feature `lane`, to rows of `stride` elements at `to` (its feature 0): turned in
+// shared memory so that every lane stores 16 bytes of a row (a row per store and lane made an epilogue of 8 us for a tile). Only the first `rows` rows and
+// `columns` elements are there. later: added to what is there (32 bits).
+template <typename T>
+__device__ __forceinline__ void put(const float (&f)[32], unsigned turn, T* to, u64 stride, unsigned rows, unsigned columns, bool later) {
+    constexpr unsigned kWide = 16 / sizeof(T), kLanes = 32 / kWide, kRows = 32 / kLanes;  // lanes of a row, rows of a store
+    const unsigned lane = threadIdx.x & 31u, row = lane / kLanes, column = lane % kLanes * kWide;
+    const bool mine = column < columns;  // (columns are whole 16 bytes)
+    to += (u64)row * stride + column;
+    float4 old[sizeof(T) == 4 ? 32 / kRows : 1];
+    if constexpr (sizeof(T) == 4) {
+        if (later) {
+#pragma unroll
+            for (unsigned i = 0; i < 32 / kRows; ++i)
+                old[i] = mine && row + i * kRows < rows ? *reinterpret_cast<const float4*>(to + i * kRows * stride) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+#pragma unroll
+    for (unsigned j = 0; j < 32; ++j) {
+        if constexpr (sizeof(T) == 4) {
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(turn + j * 128u + lane * 4u), "r"(__float_as_uint(f[j])) : "memory");
+        } else {
+            const T v = Elem<T>::from_f(f[j]);
+            asm volatile("st.shared.b16 [%0], %1;" ::"r"(turn + j * 64u + lane * 2u), "h"(*reinterpret_cast<const unsigned short*>(&v)) : "memory");
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (unsigned i = 0; i < 32 / kRows; ++i) {
+        if (mine && row + i * kRows < rows) {
+            uint4 v = load_shared16(turn + i * 512u + lane * 16u);
+            if constexpr (sizeof(T) == 4) {
+                if (later)
+                    v = make_uint4(__float_as_uint(__uint_as_float(v.x) + old[i].x), __float_as_uint(__uint_as_float(v.y) + old[i].y),
+                                   __float_as_uint(__uint_as_float(v.z) + old[i].z), __float_as_uint(__uint_as_float(v.w) + old[i].w));
+            }
+            *reinterpret_cast<uint4*>(to + i * kRows * stride) = v;
+        }
+    }
+    __syncwarp();
 }
 
 // T: type of dY and the gradients. kBias: also columns of dY.
@@ -382,7 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         if (n >= share.all && n != group) wait_phase(bar(bars.x_empty[group]), (n / kGroups - 1u) & 1u, failed);
     } else {
         const unsigned quarter = warp & 3u;  // lanes of tensor memory that this warp reaches
-        const unsigned in_tile = rank * kHalf + quarter * 32u + lane;
+        const unsigned in_tile = rank * kHalf + quarter * 32u;
+        const unsigned turn = base + kAtTurn + quarter * kTurnBytes;
         unsigned pieces = 0, n = 0;
         for (; n < share.all; ++pieces) {
             const Piece p = segment_at(a, share, n);
@@ -396,30 +442,20 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                 float f[32];
                 __syncwarp();
                 tmem_load32(tmem + buffer * kTile + c + (quarter * 32u << 16), f);
-                if (p.whole) {
-                    if (feature < a.inputs) {
-                        T* out = static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature;
-                        const unsigned there = output0 + c < a.outputs ? min(32u, a.outputs - (output0 + c)) : 0u;
-                        if constexpr (sizeof(T) == 4) {
-                            if (p.later) {
+                const unsigned there = output0 + c < a.outputs ? min(32u, a.outputs - (output0 + c)) : 0u;
+                if (!p.whole) {
+                    put<float>(f, turn, piece + (u64)c * kTile, kTile, 32u, kTile, p.later);
+                } else if (a.wide) {
+                    put<T>(f, turn, static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature, a.inputs, there, a.inputs > feature ? a.inputs - feature : 0u, p.later);
+                } else if (feature + lane < a.inputs) {
+                    T* out = static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature + lane;
 #pragma unroll
-                                for (unsigned j = 0; j < 32; ++j)
-                                    if (j < there) f[j] += out[(u64)j * a.inputs];
-                            }
-                        }
-#pragma unroll
-                        for (unsigned j = 0; j < 32; ++j)
-                            if (j < there) out[(u64)j * a.inputs] = Elem<T>::from_f(f[j]);
-                    }
-                } else {
-                    if constexpr (sizeof(T) == 4) {
-                        if (p.later) {
-#pragma unroll
-                            for (unsigned j = 0; j < 32; ++j) f[j] += piece[(u64)(c + j) * kTile];
+                    for (unsigned j = 0; j < 32; ++j) {
+                        if (j < there) {
+                            if constexpr (sizeof(T) == 4) f[j] += p.later ? out[(u64)j * a.inputs] : 0.0f;
+                            out[(u64)j * a.inputs] = Elem<T>::from_f(f[j]);
                         }
                     }
-#pragma unroll
-                    for (unsigned j = 0; j < 32; ++j) piece[(u64)(c + j) * kTile] = f[j];
                 }
             }
             tcgen05_fence_before();
@@ -629,8 +665,8 @@ Plan plan_of(const WeightGradCall& c) {
     p.steps_of_tile = p.steps_of_part * p.parts;
     const int device = current_device();
     prepare_device(device);
-    // Four steps of a pair at least: less, and the pieces cost more than the sums (a piece is 256 KiB to write and read again).
-    p.pairs = (unsigned)std::max<u64>(1, std::min<u64>(pairs_of_device(device), tiles * p.steps_of_tile / 4));
+    // A pair for each tile, or for every four steps: with less each, the pieces cost more than the sums (one is 256 KiB to write and read again).
+    p.pairs = (unsigned)std::min<u64>(pairs_of_device(device), std::max(tiles, tiles * p.steps_of_tile / 4));
     p.waves = (unsigned)tiles / p.pairs;
     p.steps = ((unsigned)tiles - p.waves * p.pairs) * p.steps_of_tile;
     const std::size_t copy = p.copied ? (std::size_t)p.parts * c.tokens * p.pitch * 2 : 0;
@@ -697,6 +733,7 @@ void launch(const WeightGradCall& c, const Plan& p) {
     a.tokens = (unsigned)c.tokens;
     a.inputs = (unsigned)c.inputs;
     a.outputs = (unsigned)c.outputs;
+    a.wide = c.inputs * sizeof(T) % 16 == 0 && reinterpret_cast<std::uintptr_t>(c.weight_grad) % 16 == 0;
     a.feature_tiles = p.feature_tiles;
     a.parts = p.parts;
     a.steps_of_part = p.steps_of_part;

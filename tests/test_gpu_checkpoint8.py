@@ -31,7 +31,7 @@ def test_codec(dtype, shape):
 def test_codec_of_views(dtype):
     base = values((40, 200), dtype).cuda()
     for x in (base[:, :64], base[:, 3:131], base[::3, ::2], base.t(), base[1:].view(-1)[1:97], base.unsqueeze(1).expand(40, 3, 200), base[:, 32:96],
-              base[:1, :96], base.view(4, 10, 200)[:, 2:7]):
+              base[:1, :96], base.view(4, 10, 200)[:, 2:7], base[:, 1:98], base[1::2, 7:40], base.view(-1)[3:3 + 61 * 128].view(61, 128)):
         assert torch.equal(ops.unpack8(ops.pack8(x)).double().cpu(), plain8.kept(x))
 
 
@@ -85,6 +85,31 @@ def test_codec_past_32_bits():
     x[-2:] = values((2, columns), torch.bfloat16).cuda()
     got = ops.unpack8(ops.pack8(x))
     assert torch.equal(got[-2:].double().cpu(), plain8.kept(x[-2:])) and not got[:-2].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (9, 33), (5, 64), (70, 1003), (2000, 3)])
+def test_outputs_at_any_address(dtype, shape):
+    """The C interface takes outputs that start between multiples of 16 bytes: every element is written, and none beside them."""
+    import ctypes
+    import nano_nccl_b200 as nn
+    lib, code = nn.load(), {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    P, S, LL = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_longlong
+    stream = P(torch.cuda.current_stream().cuda_stream)
+    x, dy = values(shape, dtype).cuda(), values(shape, dtype, seed=1).cuda()
+    p = ops.pack8(x)
+    n, codes = x.numel(), p.data.data_ptr()
+    scales = codes + p.nbytes // 33 * 32
+    leaf = x.clone().requires_grad_()
+    y = ops.gelu8(leaf)
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    for shift in range(1, 16 // x.element_size()):
+        for want, call in ((ops.unpack8(p), lambda o: lib.b2_unpack8(P(codes), P(scales), S(shape[0]), S(shape[1]), code, P(o), stream)),
+                           (y, lambda o: lib.b2_gelu8_forward(P(x.data_ptr()), LL(shape[1]), S(shape[0]), S(shape[1]), code, 0, P(o), None, None, stream)),
+                           (dx, lambda o: lib.b2_gelu8_backward(P(dy.data_ptr()), LL(shape[1]), P(codes), P(scales), S(shape[0]), S(shape[1]), code, 0, P(o), stream))):
+            room = torch.full((n + 32,), 5.0, dtype=dtype, device="cuda")
+            assert call(room.data_ptr() + shift * x.element_size()) == 0
+            assert torch.equal(room[shift:shift + n], want.detach().reshape(-1)) and (room[:shift] == 5).all() and (room[shift + n:] == 5).all()
 
 
 # exp(-x^2/2): the argument is rounded once, x^2/2 * 1.44 * 2^-24 <= 6.2e-6 up to |x| = 12; the polynomial and what follows are below 1e-6.
