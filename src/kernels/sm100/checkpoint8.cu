@@ -354,23 +354,39 @@ __device__ __forceinline__ Spot spot_at(const Kept8Args& a, const Spot& from, un
     return {from.row + rows, in - rows * a.columns};
 }
 
-// One element of x^, or of dx.
-template <typename T, Activation kAct>
-__device__ __forceinline__ float read_one(const Kept8Args& a, const Spot& s) {
+// One element of the input, and of x^.
+template <typename T>
+__device__ __forceinline__ float input_at(const Kept8Args& a, const Spot& s) {
+    return Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)s.row * a.stride) + s.column));
+}
+__device__ __forceinline__ float kept_at(const Kept8Args& a, const Spot& s) {
     const u64 half = (u64)s.row * a.halves.d;
-    const float v = decode8<0>(a.codes[half * 16u + s.column], step8(a.scales[half / 2u + s.column / kBlock8]));
+    return decode8<0>(a.codes[half * 16u + s.column], step8(a.scales[half / 2u + s.column / kBlock8]));
+}
+// Two elements of the output.
+template <typename T, Activation kAct, bool kRead>
+__device__ __forceinline__ float2 two_at(const Kept8Args& a, const Spot& s, const Spot& t) {
+    if constexpr (!kRead) return activate<kAct>(make_float2(input_at<T>(a, s), input_at<T>(a, t)));
+    const float2 v = make_float2(kept_at(a, s), kept_at(a, t));
     if constexpr (kAct == Activation::None) return v;
-    const float dy = Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)s.row * a.stride) + s.column));
-    return through<kAct>(make_float2(v, 0.0f), make_float2(dy, 0.0f)).x;
+    else return through<kAct>(v, make_float2(input_at<T>(a, s), input_at<T>(a, t)));
 }
-template <typename T, Activation kAct>
-__device__ __forceinline__ float activate_one(const Kept8Args& a, const Spot& s) {
-    return activate<kAct>(make_float2(Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)s.row * a.stride) + s.column)), 0.0f)).x;
-}
-// The elements of a granule that lies across rows, or not wholly in the output.
-template <typename T, typename F>
-__device__ __forceinline__ void one_by_one(const Kept8Args& a, u64 begin, u64 end, const Spot& from, u64 origin, F&& f) {
-    for (u64 e = begin; e < end; ++e) reinterpret_cast<T*>(a.out)[e] = Elem<T>::from_f(f(spot_at(a, from, (unsigned)(e - origin))));
+// A granule of the output that lies across rows, or not wholly in it: elements [begin, end) of the E from `origin` + `offset` on, `origin` being (row, column).
+template <typename T, Activation kAct, bool kRead>
+__device__ __forceinline__ void gather_granule(const Kept8Args& a, u64 begin, u64 end, const Spot& from, u64 origin) {
+    constexpr unsigned E = kGranule<T>;
+    if (end - begin == E) {
+        float2 f[E / 2];
+#pragma unroll
+        for (unsigned i = 0; i < E / 2; ++i)
+            f[i] = two_at<T, kAct, kRead>(a, spot_at(a, from, (unsigned)(begin - origin) + 2u * i), spot_at(a, from, (unsigned)(begin - origin) + 2u * i + 1u));
+        store_granule<T>(a.out + begin * sizeof(T), f);
+    } else {
+        for (u64 e = begin; e < end; ++e) {
+            const Spot s = spot_at(a, from, (unsigned)(e - origin));
+            reinterpret_cast<T*>(a.out)[e] = Elem<T>::from_f(two_at<T, kAct, kRead>(a, s, s).x);
+        }
+    }
 }
 
 // Elements by which the output lies behind a multiple of 16 bytes.
@@ -428,7 +444,7 @@ __global__ void __launch_bounds__(kThreads) keep8_any_kernel(const Kept8Args a) 
                 for (unsigned i = 0; i < E / 2; ++i) f[i] = activate<kAct>(pair_in<T>(w, i));
                 store_granule<T>(a.out + e * sizeof(T), f);
             } else {
-                one_by_one<T>(a, k * E < m ? 0 : e, min(a.elements, e + E), from, origin, [&](const Spot& t) { return activate_one<T, kAct>(a, t); });
+                gather_granule<T, kAct, false>(a, k * E < m ? 0 : e, min(a.elements, e + E), from, origin);
             }
         }
     }
@@ -459,7 +475,7 @@ __global__ void __launch_bounds__(kThreads) read8_any_kernel(const Kept8Args a) 
         if (!before && e >= a.elements) continue;
         const Spot s = spot_at(a, from, before ? 0u : (unsigned)(e - origin));
         if (before || e + E > a.elements || s.column + E > a.columns) {
-            one_by_one<T>(a, before ? 0 : e, min(a.elements, e + E), from, origin, [&](const Spot& t) { return read_one<T, kAct>(a, t); });
+            gather_granule<T, kAct, true>(a, before ? 0 : e, min(a.elements, e + E), from, origin);
             continue;
         }
         // E codes, at any address, and the steps of the one or two blocks that they belong to.
