@@ -17,9 +17,9 @@
 // (All tiles in one row: pairs are at different tokens, and 16384 x 4096 x 4096 draws 3.2 GB from HBM.)
 //
 // fp32: X^ is a bf16 number in any case, and dY is the exact sum of three (its 24 bits cut into eights), so three products of bf16 numbers
-// with 32-bit accumulators give it in full. The tensor cores cut what an addition leaves below 24 bits, so their sums are added to those in
-// memory, rounded, after every 512 tokens: the error does not grow with the number of tokens as it would (8192 tokens: 7.5e-6 of the
-// result's norm without).
+// with 32-bit accumulators give it in full. The tensor cores cut what an addition leaves below 24 bits, so the small parts are summed first, and the
+// sums are added to those in memory, rounded, after every 1024 tokens: the error does not grow with the number of tokens as it would (8192 tokens:
+// 7.5e-6 of the result's norm without either, 2.4e-6 with the leading part first).
 //
 // dY that TMA cannot read (rows or address not at a multiple of 16 bytes) is copied first.
 #include "kernels/sm100/weight_grad.h"
@@ -55,7 +55,7 @@ constexpr unsigned kCodeBytes = kStep * kHalf;
 constexpr unsigned kThreads = 512;
 constexpr unsigned kFirstTransformWarp = 4, kFirstEpilogueWarp = 12;
 constexpr unsigned kGroups = 4, kGroupWarps = 2;  // of transform warps: a group widens every fourth step, into an operand of its own
-constexpr unsigned kChunkSteps = 8;   // fp32: steps of each part between two additions to the sums in memory
+constexpr unsigned kChunkSteps = 16;  // fp32: steps of each part between two additions to the sums in memory
 constexpr unsigned kMaxPairs = 74;    // 148 SMs
 constexpr unsigned kFinishRows = 16;  // outputs of a tile that a CTA of finish_kernel adds up
 constexpr unsigned kTurnBytes = 32 * 32 * 4;  // of an epilogue warp: 32 outputs of its 32 features
@@ -174,13 +174,14 @@ __device__ __forceinline__ Piece piece_at(const WeightGradArgs& a, const Share& 
     }
     return p;
 }
-// The part of a piece that is summed on the tensor cores alone: all of it, or (fp32) eight steps of each part of dY.
+// The part of a piece that is summed on the tensor cores alone: all of it, or (fp32) sixteen steps of each part of dY.
 __device__ __forceinline__ Piece segment_at(const WeightGradArgs& a, const Share& s, unsigned n) {
     Piece p = piece_at(a, s, n);
     if (a.parts > 1) p.to = min(p.to, (p.from / (a.parts * kChunkSteps) + 1u) * (a.parts * kChunkSteps));
     return p;
 }
-// Which part of dY, and which 64 tokens, step k of a tile takes: eight steps of one part, the same eight of the next, and so on.
+// Which part of dY, and which 64 tokens, step k of a tile takes: sixteen steps of the last part, whose sums are smallest, the same ones of the one before,
+// then of the leading one.
 struct Spot {
     unsigned part, step;
 };
@@ -188,7 +189,7 @@ __device__ __forceinline__ Spot spot_of(const WeightGradArgs& a, unsigned k) {
     if (a.parts == 1) return {0u, k};
     const unsigned chunk = k / (a.parts * kChunkSteps), in_chunk = k - chunk * (a.parts * kChunkSteps);
     const unsigned length = min(kChunkSteps, a.steps_of_part - chunk * kChunkSteps), part = in_chunk / length;
-    return {part, chunk * kChunkSteps + in_chunk - part * length};
+    return {a.parts - 1u - part, chunk * kChunkSteps + in_chunk - part * length};
 }
 
 // Writes 32 outputs of a warp's 32 features, f[j] being output j of feature `lane`, to rows of `stride` elements at `to` (its feature 0): turned in
