@@ -14,7 +14,8 @@
 // P pairs take P whole tiles at a time, as long as there are so many: they are at the same tokens then, and read them from L2 once one of them has.
 // What is left is cut evenly, not by tiles: its steps stand in one row, and pair i takes steps [i S / P, (i+1) S / P). A tile that is
 // cut is summed in pieces, in 32 bits in the workspace, and finish_kernel adds them in the order of tokens: the result does not depend on timing.
-// (All tiles in one row: pairs are at different tokens, and 16384 x 4096 x 4096 draws 3.2 GB from HBM.)
+// (All tiles in one row: pairs are at different tokens, and 16384 x 4096 x 4096 draws 3.2 GB from HBM.) For the same reason, where there are fewer tiles than
+// pairs, the pairs of all feature tiles go side by side through the outputs and tokens, as one group: dY is read once and not once for each.
 //
 // fp32: X^ is a bf16 number in any case, and dY is the exact sum of three (its 24 bits cut into eights), so three products of bf16 numbers
 // with 32-bit accumulators give it in full. The tensor cores cut what an addition leaves below 24 bits, so the small parts are summed first, and the
@@ -78,7 +79,8 @@ struct alignas(64) WeightGradArgs {
     unsigned tokens, inputs, outputs;
     unsigned feature_tiles, parts, steps_of_part, steps_of_tile;
     unsigned pairs, waves;  // of whole tiles
-    unsigned steps;         // of the tiles that are left
+    unsigned group;         // pairs side by side in the tiles that are left, each with a tile of its own
+    unsigned steps;         // of one such row of tiles that are left
 };
 
 struct FinishArgs {
@@ -86,7 +88,7 @@ struct FinishArgs {
     void* bias_out;
     const float* pieces;
     const float* bias;
-    unsigned inputs, outputs, feature_tiles, steps_of_tile, steps, pairs;
+    unsigned inputs, outputs, feature_tiles, steps_of_tile, steps, pairs, group;
     unsigned whole_tiles;  // that come before those that are cut
     unsigned piece_ctas;  // CTAs that add pieces; the others make the bias's gradient
 };
@@ -128,14 +130,15 @@ __device__ __forceinline__ unsigned load_shared4(unsigned at) {
 
 // What a pair does, in order: `waves` whole tiles, then its steps of the tiles that are left.
 struct Share {
-    unsigned pair, begin, end;  // in the row of steps that are left
+    unsigned pair, group, begin, end;  // in the row of steps that are left
     unsigned whole, all;        // steps of its whole tiles, of everything
 };
 __device__ __forceinline__ Share share_of(const WeightGradArgs& a, unsigned pair) {
     Share s;
     s.pair = pair;
-    s.begin = first_step(pair, a.steps, a.pairs);
-    s.end = first_step(pair + 1, a.steps, a.pairs);
+    s.group = pair / a.group;
+    s.begin = first_step(s.group, a.steps, a.pairs / a.group);
+    s.end = first_step(s.group + 1, a.steps, a.pairs / a.group);
     s.whole = a.waves * a.steps_of_tile;
     s.all = s.whole + (s.end - s.begin);
     return s;
@@ -147,7 +150,7 @@ struct Where {
 __device__ __forceinline__ Where where_is(const WeightGradArgs& a, const Share& s, unsigned n) {
     const bool whole = n < s.whole;
     const unsigned at = whole ? n : s.begin + (n - s.whole), row = at / a.steps_of_tile;
-    return {whole ? row * a.pairs + s.pair : a.waves * a.pairs + row, at - row * a.steps_of_tile};
+    return {whole ? row * a.pairs + s.pair : a.waves * a.pairs + row * a.group + (s.pair - s.group * a.group), at - row * a.steps_of_tile};
 }
 // A run of steps of one tile, from its n-th step on.
 struct Piece {
@@ -483,20 +486,21 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     if (blockIdx.x < a.piece_ctas) {
         // One tile for each border between pairs that is the first inside its tile.
         constexpr unsigned kParts = kTile / kFinishRows;
-        const unsigned border = blockIdx.x / kParts + 1u, part = blockIdx.x % kParts;
-        const unsigned at = first_step(border, a.steps, a.pairs);
-        const unsigned row = at / a.steps_of_tile, from = row * a.steps_of_tile, tile = a.whole_tiles + row;
-        const unsigned before = first_step(border - 1u, a.steps, a.pairs);
+        const unsigned index = blockIdx.x / kParts, part = blockIdx.x % kParts, groups = a.pairs / a.group;
+        const unsigned border = index / a.group + 1u, member = index % a.group;
+        const unsigned at = first_step(border, a.steps, groups);
+        const unsigned row = at / a.steps_of_tile, from = row * a.steps_of_tile, tile = a.whole_tiles + row * a.group + member;
+        const unsigned before = first_step(border - 1u, a.steps, groups);
         if (at == from || before > from) return;
         __shared__ unsigned slots[kMaxPairs];
         __shared__ unsigned count;
         if (threadIdx.x == 0) {
             unsigned n = 0;
-            slots[n++] = 2u * (border - 1u) + (before == from ? 0u : 1u);
+            slots[n++] = 2u * ((border - 1u) * a.group + member) + (before == from ? 0u : 1u);
             unsigned begin = at;
-            for (unsigned p = border; p < a.pairs && begin < from + a.steps_of_tile; ++p) {
-                const unsigned end = first_step(p + 1u, a.steps, a.pairs);
-                if (end != begin) slots[n++] = 2u * p;  // (else it has no step)
+            for (unsigned p = border; p < groups && begin < from + a.steps_of_tile; ++p) {
+                const unsigned end = first_step(p + 1u, a.steps, groups);
+                if (end != begin) slots[n++] = 2u * (p * a.group + member);  // (else it has no step)
                 begin = end;
             }
             count = n;
@@ -541,11 +545,12 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         const unsigned tile = output_tile * a.feature_tiles + m;
         sum += a.bias[(u64)tile * kTile + column];
         if (tile < a.whole_tiles) continue;
-        const unsigned from = (tile - a.whole_tiles) * a.steps_of_tile, to = from + a.steps_of_tile;
-        unsigned p = (unsigned)((u64)from * a.pairs / a.steps), begin = first_step(p, a.steps, a.pairs);
-        for (; p < a.pairs && begin < to; ++p) {
-            const unsigned end = first_step(p + 1u, a.steps, a.pairs);
-            if (begin > from && end != begin) sum += a.bias[(u64)(tiles + p) * kTile + column];
+        const unsigned groups = a.pairs / a.group, row = (tile - a.whole_tiles) / a.group, member = (tile - a.whole_tiles) % a.group;
+        const unsigned from = row * a.steps_of_tile, to = from + a.steps_of_tile;
+        unsigned p = (unsigned)((u64)from * groups / a.steps), begin = first_step(p, a.steps, groups);
+        for (; p < groups && begin < to; ++p) {
+            const unsigned end = first_step(p + 1u, a.steps, groups);
+            if (begin > from && end != begin) sum += a.bias[(u64)(tiles + p * a.group + member) * kTile + column];
             begin = end;
         }
     }
@@ -605,7 +610,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ La
 }
 
 struct Plan {
-    unsigned parts = 1, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0;
+    unsigned parts = 1, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0, group = 1;
     bool copied = false;
     std::size_t pieces_at = 0, bias_at = 0, bytes = 0;
 };
@@ -668,8 +673,16 @@ Plan plan_of(const WeightGradCall& c) {
     prepare_device(device);
     // A pair for each tile, or for every four steps: with less each, the pieces cost more than the sums (one is 256 KiB to write and read again).
     p.pairs = (unsigned)std::min<u64>(pairs_of_device(device), std::max(tiles, tiles * p.steps_of_tile / 4));
+    if (tiles < p.pairs) {
+        // All feature tiles side by side, unless that leaves more than a tenth of the pairs idle.
+        const unsigned side = p.pairs / p.feature_tiles * p.feature_tiles;
+        if (side * 10 >= p.pairs * 9) {
+            p.group = p.feature_tiles;
+            p.pairs = side;
+        }
+    }
     p.waves = (unsigned)tiles / p.pairs;
-    p.steps = ((unsigned)tiles - p.waves * p.pairs) * p.steps_of_tile;
+    p.steps = ((unsigned)tiles - p.waves * p.pairs) / p.group * p.steps_of_tile;
     const std::size_t copy = p.copied ? (std::size_t)p.parts * c.tokens * p.pitch * 2 : 0;
     p.pieces_at = (copy + 255) / 256 * 256;
     p.bias_at = p.pieces_at + (std::size_t)2 * p.pairs * kTile * kTile * sizeof(float);
@@ -742,6 +755,7 @@ void launch(const WeightGradCall& c, const Plan& p) {
     a.steps = p.steps;
     a.pairs = p.pairs;
     a.waves = p.waves;
+    a.group = p.group;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(2 * p.pairs);
     config.blockDim = dim3(kThreads);
@@ -757,7 +771,7 @@ void launch(const WeightGradCall& c, const Plan& p) {
     config.numAttrs = 2;
     B2_CUDA(cudaLaunchKernelEx(&config, c.bias_grad != nullptr ? weight_grad_kernel<T, true> : weight_grad_kernel<T, false>, a));
     bool cut = false;
-    for (unsigned i = 1; i < p.pairs; ++i) cut |= first_step(i, p.steps, p.pairs) % p.steps_of_tile != 0;
+    for (unsigned i = 1; i < p.pairs / p.group; ++i) cut |= first_step(i, p.steps, p.pairs / p.group) % p.steps_of_tile != 0;
     if (!cut && c.bias_grad == nullptr) return;
     FinishArgs f;
     f.out = c.weight_grad;
@@ -770,8 +784,9 @@ void launch(const WeightGradCall& c, const Plan& p) {
     f.steps_of_tile = p.steps_of_tile;
     f.steps = p.steps;
     f.pairs = p.pairs;
+    f.group = p.group;
     f.whole_tiles = p.waves * p.pairs;
-    f.piece_ctas = cut ? (p.pairs - 1) * (kTile / kFinishRows) : 0;
+    f.piece_ctas = cut ? (p.pairs - p.group) * (kTile / kFinishRows) : 0;
     const unsigned grid = f.piece_ctas + (c.bias_grad != nullptr ? p.output_tiles * (kTile / 32) : 0);
     B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<T>, dim3(grid), 256, 0, c.stream, f));
 }
