@@ -34,7 +34,7 @@ int b2_gelu8_backward(const void* dy, long long stride, const void* codes, const
 
 /* weight_grad[n][k] = sum over tokens t of dy[t][n] * x^[t][k]; bias_grad[n] = sum of dy[t][n]. The pointers other than dy and the 8-bit form are
  * without gaps; bias_grad may be null. `workspace` has the bytes that b2_weight_grad8_workspace gives for the same arguments (it reads no
- * memory), at a multiple of 256; it belongs to one call until that call is done. */
+ * memory; may be 0), at a multiple of 256; it belongs to one call until that call is done. */
 typedef struct b2_weight_grad {
     const void* dy;
     long long stride;

@@ -197,7 +197,7 @@ int b2_weight_grad8(const b2_weight_grad* call, void* stream) {
             if (c.tokens != 0) {
                 check_kept(c.codes, c.scales, c.tokens, c.inputs);
                 B2_REQUIRE(c.dy != nullptr, "dy must be non-null");
-                B2_REQUIRE(c.workspace != nullptr && aligned(c.workspace, 256), "the workspace must be non-null, at a multiple of 256 bytes");
+                B2_REQUIRE(aligned(c.workspace, 256), "the workspace must start at a multiple of 256 bytes");
             }
         }
         kernels::launch_weight_grad(c);

@@ -11,6 +11,10 @@
 // two masks, two byte permutes and four two-wide products); four warps write finished tiles; two sum columns of dY
 // for the bias out of shared memory, each tile of features for its own share of the steps, so that every step of dY is summed once.
 //
+// What bounds it is shared memory, and power: a step reads 32 KiB of operands, writes 16 KiB of dY, 8 KiB of codes and 16 KiB of widened X^, and reads the
+// codes again; the products alone take three quarters of its time. So a long product has tiles of 256 x 512, for which a widened step of X^ serves twice
+// (16384 x 4096 x 4096: 466 -> 395 us). They fill tensor memory, so that their epilogue stands alone: short products stay with 256 x 256.
+//
 // P pairs take P whole tiles at a time, as long as there are so many: they are at the same tokens then, and read them from L2 once one of them has.
 // What is left is cut evenly, not by tiles: its steps stand in one row, and pair i takes steps [i S / P, (i+1) S / P). A tile that is
 // cut is summed in pieces, in 32 bits in the workspace, and finish_kernel adds them in the order of tokens: the result does not depend on timing.
@@ -49,19 +53,21 @@ using u64 = unsigned long long;
 constexpr unsigned kTile = 256;       // features and outputs of a pair's tile
 constexpr unsigned kHalf = 128;       // of one CTA
 constexpr unsigned kStep = 64;        // tokens
-constexpr unsigned kStages = 6;       // steps whose dY and codes are in shared memory or on the way
+constexpr unsigned kDepth = 6;        // steps whose dY is in shared memory or on the way; half as many of wide tiles
 constexpr unsigned kBlockBytes = kStep * 128;         // 64 elements of every token of a step
 constexpr unsigned kOperandBytes = 2 * kBlockBytes;   // a CTA's half of an operand
 constexpr unsigned kCodeBytes = kStep * kHalf;
 constexpr unsigned kThreads = 512;
 constexpr unsigned kFirstTransformWarp = 4, kFirstEpilogueWarp = 12;
-constexpr unsigned kGroups = 4, kGroupWarps = 2;  // of transform warps: a group widens every fourth step, into an operand of its own
+// Transform warps: a group widens every fourth step, from codes at a place of its own into an operand of its own. (Its own, because a wait tells a phase
+// from the one before it only: whoever waits on a barrier has to have seen every phase of it.)
+constexpr unsigned kGroups = 4, kGroupWarps = 2;
 constexpr unsigned kChunkSteps = 16;  // fp32: steps of each part between two additions to the sums in memory
 constexpr unsigned kMaxPairs = 74;    // 148 SMs
 constexpr unsigned kFinishRows = 16;  // outputs of a tile that a CTA of finish_kernel adds up
 constexpr unsigned kTurnBytes = 32 * 32 * 4;  // of an epilogue warp: 32 outputs of its 32 features
-// Shared memory, from a multiple of 1024 bytes on: dY of the stages, X^ of the groups, codes of the stages, what the epilogue turns, barriers.
-constexpr unsigned kAtX = kStages * kOperandBytes, kAtCodes = kAtX + kGroups * kOperandBytes, kAtTurn = kAtCodes + kStages * kCodeBytes,
+// Shared memory, from a multiple of 1024 bytes on: dY of the stages, X^ of the groups, their codes, what the epilogue turns, barriers.
+constexpr unsigned kAtX = kDepth * kOperandBytes, kAtCodes = kAtX + kGroups * kOperandBytes, kAtTurn = kAtCodes + kGroups * kCodeBytes,
                    kAtBarriers = kAtTurn + 4 * kTurnBytes;
 constexpr unsigned kShared = kAtBarriers + 512 + 1024;
 static_assert(kShared <= 227 * 1024);
@@ -71,8 +77,8 @@ struct alignas(64) WeightGradArgs {
     CUtensorMap codes;  // [1][tokens][pitch]
     const unsigned char* scales;
     void* out;
-    float* pieces;     // [2 * pairs][256 outputs][256 features]
-    float* bias;       // [tiles + pairs][256], or null
+    float* pieces;     // [2 * pairs][outputs of a tile][256 features]
+    float* bias;       // [tiles + pairs][outputs of a tile], or null
     unsigned* status;  // host memory
     u64 pitch;         // bytes of a token's codes
     bool wide;         // rows of `out` start at multiples of 16 bytes
@@ -88,7 +94,7 @@ struct FinishArgs {
     void* bias_out;
     const float* pieces;
     const float* bias;
-    unsigned inputs, outputs, feature_tiles, steps_of_tile, steps, pairs, group;
+    unsigned inputs, outputs, width, feature_tiles, steps_of_tile, steps, pairs, group;  // width: outputs of a tile
     unsigned whole_tiles;  // that come before those that are cut
     unsigned piece_ctas;  // CTAs that add pieces; the others make the bias's gradient
 };
@@ -101,10 +107,11 @@ __host__ __device__ inline unsigned first_step(unsigned pair, unsigned steps, un
 
 // Barriers of a CTA, in its shared memory.
 struct Barriers {
-    u64 dy[kStages];       // this CTA's dY of a stage has come
-    u64 dy_other[kStages]; // first CTA: the other's has
-    u64 codes[kStages];    // this CTA's codes of a stage have come
-    u64 empty[kStages];    // the stage has been read
+    u64 dy[kDepth];       // this CTA's dY of a stage has come
+    u64 dy_other[kDepth]; // first CTA: the other's has
+    u64 empty[kDepth];    // it has been read
+    u64 codes[kGroups];        // this CTA's codes of a group have come
+    u64 codes_empty[kGroups];  // they have been read
     u64 x[kGroups];        // first CTA: both CTAs' X^ of a group is written
     u64 x_empty[kGroups];  // it has been read
     u64 sums[2];           // accumulators are complete
@@ -237,9 +244,12 @@ __device__ __forceinline__ void put(const float (&f)[32], unsigned turn, T* to, 
     __syncwarp();
 }
 
-// T: type of dY and the gradients. kBias: also columns of dY.
-template <typename T, bool kBias>
+// T: type of dY and the gradients. kBias: also columns of dY. kWide: tiles of 512 outputs (16-bit types).
+template <typename T, bool kBias, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_constant__ WeightGradArgs a) {
+    constexpr unsigned kBlocks = kWide ? 2 : 1, kWidth = kBlocks * kTile;  // blocks of 256 outputs, outputs of a tile
+    constexpr unsigned kStages = kWide ? kDepth / 2 : kDepth, kDyBytes = kBlocks * kOperandBytes;
+    constexpr unsigned kBuffers = kWide ? 1 : 2;                           // sets of accumulators, in turn
     constexpr bool kBf16 = !std::is_same_v<T, __half>;
     using Operand = std::conditional_t<kBf16, __nv_bfloat16, __half>;
     extern __shared__ unsigned char raw[];
@@ -256,14 +266,15 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         for (unsigned s = 0; s < kStages; ++s) {
             mbar_init(&bars.dy[s], 1);
             mbar_init(&bars.dy_other[s], 1);
-            mbar_init(&bars.codes[s], 1);
-            mbar_init(&bars.empty[s], 1 + kGroupWarps + (kBias ? 2 : 0));
+            mbar_init(&bars.empty[s], 1 + (kBias ? 2 : 0));
         }
         for (unsigned i = 0; i < kGroups; ++i) {
+            mbar_init(&bars.codes[i], 1);
+            mbar_init(&bars.codes_empty[i], kGroupWarps);
             mbar_init(&bars.x[i], 2 * kGroupWarps);
             mbar_init(&bars.x_empty[i], 1);
         }
-        for (unsigned i = 0; i < 2; ++i) {
+        for (unsigned i = 0; i < kBuffers; ++i) {
             mbar_init(&bars.sums[i], 1);
             mbar_init(&bars.sums_free[i], 8);
         }
@@ -285,33 +296,36 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
     const auto bar = [](u64& b) { return smem_addr(&b); };
     if (warp == 0) {
         if (lane == 0) {
-            unsigned n = 0;  // steps so far
+            unsigned n = 0, asked = 0;  // steps whose dY, and whose codes, have been asked for
             bool ok = true;
             while (n < share.all && ok) {
                 const Piece p = piece_at(a, share, n);
-                const int output = (int)((p.tile / a.feature_tiles) * kTile + rank * kHalf);
+                const int output = (int)((p.tile / a.feature_tiles) * kWidth + rank * kHalf);
                 const int feature = (int)((p.tile % a.feature_tiles) * kTile + rank * kHalf);
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
-                    const unsigned s = n % kStages;
+                    const unsigned s = n % kStages, group = n % kGroups;
                     const Spot spot = spot_of(a, k);
+                    ok = wait_phase(bar(bars.codes_empty[group]), ((n / kGroups) & 1u) ^ 1u, failed);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&bars.codes[group], kCodeBytes);
+                    tma_load_box(base + kAtCodes + group * kCodeBytes, &a.codes, feature, (int)(spot.step * kStep), 0, bar(bars.codes[group]));
+                    ++asked;
                     ok = wait_phase(bar(bars.empty[s]), ((n / kStages) & 1u) ^ 1u, failed);
                     if (!ok) break;
-                    mbar_arrive_expect_tx(&bars.codes[s], kCodeBytes);
-                    tma_load_box(base + kAtCodes + s * kCodeBytes, &a.codes, feature, (int)(spot.step * kStep), 0, bar(bars.codes[s]));
-                    mbar_arrive_expect_tx(&bars.dy[s], kOperandBytes);
-                    const unsigned dst = base + s * kOperandBytes;
-                    tma_load_box(dst, &a.dy, output, (int)(spot.step * kStep), (int)spot.part, bar(bars.dy[s]));
-                    tma_load_box(dst + kBlockBytes, &a.dy, output + 64, (int)(spot.step * kStep), (int)spot.part, bar(bars.dy[s]));
+                    mbar_arrive_expect_tx(&bars.dy[s], kDyBytes);
+#pragma unroll
+                    for (unsigned b = 0; b < 2 * kBlocks; ++b)  // 64 outputs each
+                        tma_load_box(base + s * kDyBytes + b * kBlockBytes, &a.dy, output + (int)(b / 2 * kTile + b % 2 * 64), (int)(spot.step * kStep),
+                                     (int)spot.part, bar(bars.dy[s]));
                 }
             }
-            // Copies have landed and stages been given back before the CTA ends, after a failure too.
-            if (ok) {
-                for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i) wait_phase(bar(bars.empty[i % kStages]), (i / kStages) & 1u, failed);
-            } else {
-                for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i)
-                    for (unsigned polls = 0; polls < 1000u && !(phase_over<false>(bar(bars.dy[i % kStages]), (i / kStages) & 1u) &&
-                                                                 phase_over<false>(bar(bars.codes[i % kStages]), (i / kStages) & 1u)); ++polls) {}
+            // Stages have been given back, and after a failure copies have landed, before the CTA ends.
+            for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i) {
+                if (ok) wait_phase(bar(bars.empty[i % kStages]), (i / kStages) & 1u, failed);
+                for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.dy[i % kStages]), (i / kStages) & 1u); ++polls) {}
             }
+            for (unsigned i = asked > kGroups ? asked - kGroups : 0; i < asked; ++i)
+                for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.codes[i % kGroups]), (i / kGroups) & 1u); ++polls) {}
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
@@ -320,8 +334,8 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             bool ok = true;
             for (; n < share.all && ok; ++pieces) {
                 const Piece p = segment_at(a, share, n);
-                const unsigned buffer = pieces & 1u;
-                ok = wait_phase<true>(bar(bars.sums_free[buffer]), ((pieces >> 1) & 1u) ^ 1u, failed);
+                const unsigned buffer = pieces % kBuffers;
+                ok = wait_phase<true>(bar(bars.sums_free[buffer]), ((pieces / kBuffers) & 1u) ^ 1u, failed);
                 if (!ok) break;
                 tcgen05_fence_after();
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
@@ -331,10 +345,13 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                     if (!ok) break;
                     tcgen05_fence_after();
                     const std::uint64_t x = operand_by_rows(base + kAtX + group * kOperandBytes, kBlockBytes);
-                    const std::uint64_t dy = operand_by_rows(base + s * kOperandBytes, kBlockBytes);
 #pragma unroll
-                    for (unsigned i = 0; i < kStep / 16; ++i)  // 16 tokens are 2048 bytes
-                        mma_pair(tmem + buffer * kTile, x + i * (2048 >> 4), dy + i * (2048 >> 4), shape, k > p.from || i > 0);
+                    for (unsigned b = 0; b < kBlocks; ++b) {
+                        const std::uint64_t dy = operand_by_rows(base + s * kDyBytes + b * kOperandBytes, kBlockBytes);
+#pragma unroll
+                        for (unsigned i = 0; i < kStep / 16; ++i)  // 16 tokens are 2048 bytes
+                            mma_pair(tmem + (buffer + b) * kTile, x + i * (2048 >> 4), dy + i * (2048 >> 4), shape, k > p.from || i > 0);
+                    }
                     commit_pair(bar(bars.x_empty[group]));
                     commit_pair(bar(bars.empty[s]));
                 }
@@ -359,27 +376,33 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             while (n < share.all && ok) {
                 const Piece p = piece_at(a, share, n);
                 const unsigned turn = p.tile % a.feature_tiles;
-                float x = 0.0f, y = 0.0f;
+                float2 sum[kBlocks];
+#pragma unroll
+                for (unsigned b = 0; b < kBlocks; ++b) sum[b] = make_float2(0.0f, 0.0f);
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
                     const unsigned s = n % kStages;
                     ok = __all_sync(0xffffffffu, wait_phase(bar(bars.dy[s]), (n / kStages) & 1u, failed));
                     if (!ok) break;
                     if (k % a.feature_tiles == turn) {
-                        const unsigned from = base + s * kOperandBytes + (warp - 2u) * kBlockBytes;
+#pragma unroll
+                        for (unsigned b = 0; b < kBlocks; ++b) {
+                            const unsigned from = base + s * kDyBytes + b * kOperandBytes + (warp - 2u) * kBlockBytes;
 #pragma unroll 16
-                        for (unsigned t = 0; t < kStep; ++t) {
-                            const unsigned w = load_shared4(from + t * 128u + (((lane / 4u) ^ (t & 7u)) * 16u) + (lane & 3u) * 4u);
-                            const float2 f = kBf16 ? b2_to_f2(w) : h2_to_f2(w);
-                            x += f.x;
-                            y += f.y;
+                            for (unsigned t = 0; t < kStep; ++t) {
+                                const unsigned w = load_shared4(from + t * 128u + (((lane / 4u) ^ (t & 7u)) * 16u) + (lane & 3u) * 4u);
+                                const float2 f = kBf16 ? b2_to_f2(w) : h2_to_f2(w);
+                                sum[b].x += f.x;
+                                sum[b].y += f.y;
+                            }
                         }
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(bars.empty[s]));
                 }
                 if (!ok) break;
-                float* to = a.bias + (u64)(p.from == 0 ? p.tile : a.feature_tiles * ((a.outputs + kTile - 1) / kTile) + share.pair) * kTile;
-                *reinterpret_cast<float2*>(to + rank * kHalf + column) = make_float2(x, y);
+                float* to = a.bias + (u64)(p.from == 0 ? p.tile : a.feature_tiles * ((a.outputs + kWidth - 1) / kWidth) + share.pair) * kWidth;
+#pragma unroll
+                for (unsigned b = 0; b < kBlocks; ++b) *reinterpret_cast<float2*>(to + b * kTile + rank * kHalf + column) = sum[b];
             }
         }
     } else if (warp < kFirstEpilogueWarp) {
@@ -403,16 +426,15 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         const unsigned odd = chunk >> 2, column = (chunk & 3u) * 2u;
         const unsigned block = base + kAtX + group * kOperandBytes + odd * kBlockBytes + row * 128u;
         const unsigned first = block + (((column + odd) ^ row) * 16u), second = block + (((column + (odd ^ 1u)) ^ row) * 16u);
-        const unsigned codes = base + kAtCodes + row * kHalf + chunk * 16u;
+        const unsigned codes = base + kAtCodes + group * kCodeBytes + row * kHalf + chunk * 16u;
         unsigned n = group;
         for (; n < share.all; n += kGroups) {
-            const unsigned s = n % kStages;
-            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.codes[s]), (n / kStages) & 1u, failed) &&
-                                             wait_phase(bar(bars.x_empty[group]), ((n / kGroups) & 1u) ^ 1u, failed)))
+            const unsigned parity = (n / kGroups) & 1u;
+            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.codes[group]), parity, failed) && wait_phase(bar(bars.x_empty[group]), parity ^ 1u, failed)))
                 break;
 #pragma unroll
             for (unsigned u = 0; u < 8; ++u) {
-                const uint4 c = load_shared16(codes + s * kCodeBytes + u * (8u * kHalf));
+                const uint4 c = load_shared16(codes + u * (8u * kHalf));
                 const unsigned s2 = step16<Operand>(scale[u]);
                 const uint2 w0 = widen8x4<Operand>(odd ? c.z : c.x, s2), w1 = widen8x4<Operand>(odd ? c.w : c.y, s2);
                 const uint2 w2 = widen8x4<Operand>(odd ? c.x : c.z, s2), w3 = widen8x4<Operand>(odd ? c.y : c.w, s2);
@@ -423,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive_at(bar(bars.x[group]), 0);
-                mbar_arrive(bar(bars.empty[s]));
+                mbar_arrive(bar(bars.codes_empty[group]));
             }
             if (n + kGroups < share.all) load_scales(n + kGroups);  // (before the fence, the fence would wait for them)
         }
@@ -436,13 +458,13 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         unsigned pieces = 0, n = 0;
         for (; n < share.all; ++pieces) {
             const Piece p = segment_at(a, share, n);
-            const unsigned buffer = pieces & 1u;
-            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.sums[buffer]), (pieces >> 1) & 1u, failed))) break;
+            const unsigned buffer = pieces % kBuffers;
+            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.sums[buffer]), (pieces / kBuffers) & 1u, failed))) break;
             tcgen05_fence_after();
             const unsigned feature = (p.tile % a.feature_tiles) * kTile + in_tile;
-            const unsigned output0 = (p.tile / a.feature_tiles) * kTile;
-            float* piece = a.pieces + (u64)p.slot * (kTile * kTile) + in_tile;
-            for (unsigned c = 0; c < kTile; c += 32u) {
+            const unsigned output0 = (p.tile / a.feature_tiles) * kWidth;
+            float* piece = a.pieces + (u64)p.slot * (kWidth * kTile) + in_tile;
+            for (unsigned c = 0; c < kWidth; c += 32u) {
                 float f[32];
                 __syncwarp();
                 tmem_load32(tmem + buffer * kTile + c + (quarter * 32u << 16), f);
@@ -485,8 +507,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x < a.piece_ctas) {
         // One tile for each border between pairs that is the first inside its tile.
-        constexpr unsigned kParts = kTile / kFinishRows;
-        const unsigned index = blockIdx.x / kParts, part = blockIdx.x % kParts, groups = a.pairs / a.group;
+        const unsigned parts = a.width / kFinishRows, index = blockIdx.x / parts, part = blockIdx.x % parts, groups = a.pairs / a.group;
         const unsigned border = index / a.group + 1u, member = index % a.group;
         const unsigned at = first_step(border, a.steps, groups);
         const unsigned row = at / a.steps_of_tile, from = row * a.steps_of_tile, tile = a.whole_tiles + row * a.group + member;
@@ -512,7 +533,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
 #pragma unroll
         for (unsigned r = 0; r < kRows; ++r) sum[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (unsigned i = 0; i < count; ++i) {
-            const float* piece = a.pieces + (u64)slots[i] * (kTile * kTile) + row0 * kTile + column;
+            const float* piece = a.pieces + (u64)slots[i] * (a.width * kTile) + row0 * kTile + column;
             float4 v[kRows];
 #pragma unroll
             for (unsigned r = 0; r < kRows; ++r) v[r] = *reinterpret_cast<const float4*>(piece + r * kTile);
@@ -527,7 +548,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         const unsigned feature = (tile % a.feature_tiles) * kTile + column;
 #pragma unroll
         for (unsigned r = 0; r < kRows; ++r) {
-            const unsigned output = (tile / a.feature_tiles) * kTile + row0 + r;
+            const unsigned output = (tile / a.feature_tiles) * a.width + row0 + r;
             if (output >= a.outputs) continue;
             T* out = static_cast<T*>(a.out) + (u64)output * a.inputs + feature;
             const float f[4] = {sum[r].x, sum[r].y, sum[r].z, sum[r].w};
@@ -538,19 +559,19 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         return;
     }
     // 32 outputs of a tile per CTA, eight threads for each.
-    const unsigned index = blockIdx.x - a.piece_ctas, output_tile = index / (kTile / 32u), column = (index % (kTile / 32u)) * 32u + (threadIdx.x & 31u);
-    const unsigned tiles = a.feature_tiles * ((a.outputs + kTile - 1) / kTile);
+    const unsigned index = blockIdx.x - a.piece_ctas, output_tile = index / (a.width / 32u), column = (index % (a.width / 32u)) * 32u + (threadIdx.x & 31u);
+    const unsigned tiles = a.feature_tiles * ((a.outputs + a.width - 1) / a.width);
     float sum = 0.0f;
     for (unsigned m = threadIdx.x / 32u; m < a.feature_tiles; m += 8u) {
         const unsigned tile = output_tile * a.feature_tiles + m;
-        sum += a.bias[(u64)tile * kTile + column];
+        sum += a.bias[(u64)tile * a.width + column];
         if (tile < a.whole_tiles) continue;
         const unsigned groups = a.pairs / a.group, row = (tile - a.whole_tiles) / a.group, member = (tile - a.whole_tiles) % a.group;
         const unsigned from = row * a.steps_of_tile, to = from + a.steps_of_tile;
         unsigned p = (unsigned)((u64)from * groups / a.steps), begin = first_step(p, a.steps, groups);
         for (; p < groups && begin < to; ++p) {
             const unsigned end = first_step(p + 1u, a.steps, groups);
-            if (begin > from && end != begin) sum += a.bias[(u64)(tiles + p * a.group + member) * kTile + column];
+            if (begin > from && end != begin) sum += a.bias[(u64)(tiles + p * a.group + member) * a.width + column];
             begin = end;
         }
     }
@@ -559,7 +580,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     __syncthreads();
     if (threadIdx.x >= 32u) return;
     for (unsigned i = 1; i < 8; ++i) sum += sums[i][threadIdx.x];
-    const unsigned output = output_tile * kTile + column;
+    const unsigned output = output_tile * a.width + column;
     if (output < a.outputs) static_cast<T*>(a.bias_out)[output] = Elem<T>::from_f(sum);
 }
 
@@ -610,7 +631,8 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ La
 }
 
 struct Plan {
-    unsigned parts = 1, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0, group = 1;
+    bool wide = false;
+    unsigned parts = 1, width = kTile, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0, group = 1;
     bool copied = false;
     std::size_t pieces_at = 0, bias_at = 0, bytes = 0;
 };
@@ -630,7 +652,7 @@ unsigned pairs_of_device(int device) {
     config.attrs = attr;
     config.numAttrs = 1;
     int clusters = 0;
-    B2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, weight_grad_kernel<__nv_bfloat16, true>, &config));
+    B2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, weight_grad_kernel<__nv_bfloat16, true, false>, &config));
     const unsigned pairs = std::min(kMaxPairs, (unsigned)std::max(1, clusters));
     if (device >= 0 && device < 64) known[device].store(pairs);
     return pairs;
@@ -642,9 +664,11 @@ void prepare_device(int device) {
     static bool done[64] = {};
     std::lock_guard<std::mutex> lock(mutex);
     if (device >= 0 && device < 64 && done[device]) return;
-    const void* kernels[] = {(const void*)weight_grad_kernel<float, false>, (const void*)weight_grad_kernel<float, true>,
-                             (const void*)weight_grad_kernel<__half, false>, (const void*)weight_grad_kernel<__half, true>,
-                             (const void*)weight_grad_kernel<__nv_bfloat16, false>, (const void*)weight_grad_kernel<__nv_bfloat16, true>};
+    const void* kernels[] = {(const void*)weight_grad_kernel<float, false, false>,         (const void*)weight_grad_kernel<float, true, false>,
+                             (const void*)weight_grad_kernel<__half, false, false>,        (const void*)weight_grad_kernel<__half, true, false>,
+                             (const void*)weight_grad_kernel<__half, false, true>,         (const void*)weight_grad_kernel<__half, true, true>,
+                             (const void*)weight_grad_kernel<__nv_bfloat16, false, false>, (const void*)weight_grad_kernel<__nv_bfloat16, true, false>,
+                             (const void*)weight_grad_kernel<__nv_bfloat16, false, true>,  (const void*)weight_grad_kernel<__nv_bfloat16, true, true>};
     for (const void* k : kernels) B2_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared));
     if (device >= 0 && device < 64) done[device] = true;
 }
@@ -655,6 +679,16 @@ int current_device() {
     return device;
 }
 
+// Whether tiles of 512 outputs are faster: with long sums, whose epilogue counts for little, and many steps for each pair. Steps of a tile squared, times tiles, tells
+// them apart (us, 256 / 512 outputs; thousands): 8192 x 1024 x 1024 31 / 33 (131), 2048 x 4096 x 4096 84 / 87 (131), 8192 x 768 x 2304 47 / 60 (246),
+// 4096 x 2048 x 4096 72 / 80 (262), 4096 x 4096 x 4096 163 / 131 (524), 8192 x 2048 x 2048 73 / 69 (524), 16384 x 2048 x 1000 75 / 73 (1049),
+// 16384 x 4096 x 4096 466 / 395 (8389). Not where rounding the outputs up to 512 adds more than an eighth.
+bool wide_tiles(const WeightGradCall& c, u64 steps) {
+    const u64 tiles = (c.inputs + kTile - 1) / kTile * ((c.outputs + 2 * kTile - 1) / (2 * kTile));
+    const u64 narrow = (c.outputs + kTile - 1) / kTile, wide = (c.outputs + 2 * kTile - 1) / (2 * kTile) * 2;
+    return c.dtype != DType::Float && c.outputs > kTile && steps * steps * tiles >= 400000 && wide * 8 <= narrow * 9;
+}
+
 Plan plan_of(const WeightGradCall& c) {
     Plan p;
     const std::size_t bytes = c.dtype == DType::Float ? 4 : 2;
@@ -663,8 +697,11 @@ Plan plan_of(const WeightGradCall& c) {
                c.stride < (long long)c.outputs;
     p.pitch = (unsigned)((c.outputs + 7) / 8 * 8);
     p.feature_tiles = (unsigned)((c.inputs + kTile - 1) / kTile);
-    p.output_tiles = (unsigned)((c.outputs + kTile - 1) / kTile);
-    const u64 steps_of_part = (c.tokens + kStep - 1) / kStep, tiles = (u64)p.feature_tiles * p.output_tiles;
+    const u64 steps_of_part = (c.tokens + kStep - 1) / kStep;
+    p.wide = wide_tiles(c, steps_of_part);
+    p.width = p.wide ? 2 * kTile : kTile;
+    p.output_tiles = (unsigned)((c.outputs + p.width - 1) / p.width);
+    const u64 tiles = (u64)p.feature_tiles * p.output_tiles;
     B2_REQUIRE(steps_of_part * p.parts * tiles < (1ull << 31) && tiles < (1ull << 24) && c.tokens < (1ull << 31),
                "weight_grad8: too many tokens, inputs and outputs for one call");
     p.steps_of_part = (unsigned)steps_of_part;
@@ -685,8 +722,8 @@ Plan plan_of(const WeightGradCall& c) {
     p.steps = ((unsigned)tiles - p.waves * p.pairs) / p.group * p.steps_of_tile;
     const std::size_t copy = p.copied ? (std::size_t)p.parts * c.tokens * p.pitch * 2 : 0;
     p.pieces_at = (copy + 255) / 256 * 256;
-    p.bias_at = p.pieces_at + (std::size_t)2 * p.pairs * kTile * kTile * sizeof(float);
-    p.bytes = p.bias_at + (c.bias_grad != nullptr ? (tiles + p.pairs) * kTile * sizeof(float) : 0);
+    p.bias_at = p.pieces_at + (p.steps != 0 ? (std::size_t)2 * p.pairs * p.width * kTile * sizeof(float) : 0);
+    p.bytes = p.bias_at + (c.bias_grad != nullptr ? (tiles + p.pairs) * p.width * sizeof(float) : 0);
     return p;
 }
 
@@ -769,7 +806,11 @@ void launch(const WeightGradCall& c, const Plan& p) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     config.attrs = attr;
     config.numAttrs = 2;
-    B2_CUDA(cudaLaunchKernelEx(&config, c.bias_grad != nullptr ? weight_grad_kernel<T, true> : weight_grad_kernel<T, false>, a));
+    const bool bias = c.bias_grad != nullptr;
+    void (*kernel)(WeightGradArgs) = bias ? weight_grad_kernel<T, true, false> : weight_grad_kernel<T, false, false>;
+    if constexpr (sizeof(T) == 2)
+        if (p.wide) kernel = bias ? weight_grad_kernel<T, true, true> : weight_grad_kernel<T, false, true>;
+    B2_CUDA(cudaLaunchKernelEx(&config, kernel, a));
     bool cut = false;
     for (unsigned i = 1; i < p.pairs / p.group; ++i) cut |= first_step(i, p.steps, p.pairs / p.group) % p.steps_of_tile != 0;
     if (!cut && c.bias_grad == nullptr) return;
@@ -780,14 +821,15 @@ void launch(const WeightGradCall& c, const Plan& p) {
     f.bias = a.bias;
     f.inputs = a.inputs;
     f.outputs = a.outputs;
+    f.width = p.width;
     f.feature_tiles = p.feature_tiles;
     f.steps_of_tile = p.steps_of_tile;
     f.steps = p.steps;
     f.pairs = p.pairs;
     f.group = p.group;
     f.whole_tiles = p.waves * p.pairs;
-    f.piece_ctas = cut ? (p.pairs - p.group) * (kTile / kFinishRows) : 0;
-    const unsigned grid = f.piece_ctas + (c.bias_grad != nullptr ? p.output_tiles * (kTile / 32) : 0);
+    f.piece_ctas = cut ? (p.pairs - p.group) * (p.width / kFinishRows) : 0;
+    const unsigned grid = f.piece_ctas + (c.bias_grad != nullptr ? p.output_tiles * (p.width / 32) : 0);
     B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<T>, dim3(grid), 256, 0, c.stream, f));
 }
 
@@ -810,6 +852,7 @@ void launch_weight_grad(const WeightGradCall& c) {
     if (__atomic_exchange_n(status_word(), 0u, __ATOMIC_RELAXED) != 0u)
         throw std::runtime_error("weight_grad8: a wait inside an earlier call ran out; that call's gradients are not valid");
     const Plan p = plan_of(c);
+    B2_REQUIRE(p.bytes == 0 || c.workspace != nullptr, "the workspace must be non-null");
     switch (c.dtype) {
         case DType::Float: return launch<float>(c, p);
         case DType::Float16: return launch<__half>(c, p);

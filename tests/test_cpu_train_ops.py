@@ -82,7 +82,7 @@ def test_c_interface_refuses_what_would_leave_its_buffers(lib):
     refused(lib, lib.b2_gelu8_backward(P(4096), LL(64), None, P(4096), S(2), S(64), I(0), I(0), P(4096), None), "non-null")
     assert pack(None, 0, 64, 0, None, None) == 0  # nothing to do
 
-    w = WeightGrad(4096, 64, 32, 64, 64, 2, 4096, 4096, 4096, None, None)
+    w = WeightGrad(4096, 64, 32, 64, 64, 2, 4096, 4096, 4096, None, 4100)
     refused(lib, lib.b2_weight_grad8(ctypes.byref(w), None), "workspace")
     w.workspace, w.dtype = 4096, 7
     refused(lib, lib.b2_weight_grad8(ctypes.byref(w), None), "dtype")

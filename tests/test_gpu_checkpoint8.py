@@ -206,17 +206,26 @@ def test_weight_grad_of_views(dtype):
     check_weight_grad(wide.permute(1, 0, 2), x.permute(1, 0, 2))
 
 
-@pytest.mark.parametrize("tokens", [1, 3, 64, 1000])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,inputs,outputs", [(26001, 700, 500), (20000, 1100, 260), (9000, 513, 4700)])
+def test_weight_grad_of_many_tokens(dtype, tokens, inputs, outputs):
+    check_weight_grad(values((tokens, outputs), dtype, seed=5, scale=0.01).cuda(), values((tokens, inputs), dtype, seed=6).cuda())
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 64, 1000, 30000])
 def test_weight_grad_is_exact_where_sums_are(tokens):
     """Whole numbers: every product and sum is exact, in any order, so that a term lost or taken twice shows."""
     gen = torch.Generator().manual_seed(tokens)
     for dtype in TYPES:
         x = torch.randint(-3, 4, (tokens, 200), generator=gen).to(dtype).cuda()
         x[:, ::32] = 64
-        dy = torch.randint(-2, 3, (tokens, 264), generator=gen).to(dtype).cuda()
+        dy = torch.randint(-2, 3, (tokens, 500), generator=gen).to(dtype).cuda()
         dw, db = ops.weight_grad8(dy, ops.pack8(x), bias=True)
         want = dy.double().t() @ x.double()
         assert torch.equal(dw, want.to(dtype)) and torch.equal(db, dy.double().sum(0).to(dtype))
+        for _ in range(3):
+            again = ops.weight_grad8(dy, ops.pack8(x), bias=True)
+            assert torch.equal(again[0], dw) and torch.equal(again[1], db)
 
 
 def test_full_precision_of_float32():
