@@ -2,7 +2,7 @@
 capabilities of nano-nccl (AllReduce / ReduceScatter / AllGather over float, fp16, bf16 with
 sum/avg/max/min), driven from PyTorch.
 
-Layout: ``communicator`` (ctypes binding of the C++ communicator), ``ops`` (torch custom ops),
+Layout: ``communicator`` (ctypes binding of the C++ communicator), ``ops`` (torch custom ops, and operators of a training step on one GPU),
 ``parallel`` (bucketed gradient all-reduce, data-parallel wrapper), ``models`` (synthetic tensor
 stacks shaped like real models, for benchmarks), ``utils`` (timing, clocks, simulator binding).
 """

@@ -1,7 +1,7 @@
 // Bulk asynchronous copies (TMA, untiled form) and the mbarrier that tracks them.
 // Only the plain forms are used: global → shared::cta (completion on an mbarrier of the same CTA)
-// and shared::cta → global (bulk async-group), both on this GPU's own memory. No multicast
-// qualifier appears anywhere in this library.
+// and shared::cta → global (bulk async-group), both on this GPU's own memory. No copy of this
+// library has a multicast qualifier.
 // Both addresses must be 16-byte aligned and the size a multiple of 16 bytes.
 #pragma once
 
