@@ -43,9 +43,8 @@ def rotary_frequencies(rotated, base=10000.0, scaling=None, factor=1.0, context=
             raise ValueError("scaling 'yarn' needs the context of the training, and fast > slow > 0")
         # The pair index that makes n turns in `context` positions.
         pair_of = lambda n: rotated * math.log(context / (2.0 * math.pi * n)) / (2.0 * math.log(base))  # noqa: E731
-        low = max(math.floor(pair_of(fast)), 0)
-        high = min(math.ceil(pair_of(slow)), rotated // 2 - 1)
-        divided = ((pairs - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        low, high = math.floor(pair_of(fast)), math.ceil(pair_of(slow))
+        divided = ((pairs - low) / (high - low)).clamp(0.0, 1.0)
         frequencies = frequencies * (1.0 - divided) + frequencies / factor * divided
         magnitude = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "ntk"):
@@ -68,10 +67,13 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, layout="hal
     """(q, k) after the norm of each head, ``x * (mean(x^2) + eps)^(-1/2) * weight``, and the rotation of :func:`rotary`, in one pass.
 
     ``q_weight`` and ``k_weight``: [dim], of the same dtype. For the backward pass q and k are kept in 8 bits (``keep="int8"``: as in
-    :mod:`.checkpoint8`, a head of a token being one block), or as they are (``keep=None``)."""
+    :mod:`.checkpoint8`, a head of a token being one block), or as they are (``keep=None``). Under autocast, weights of another dtype are
+    cast to that of q and k."""
     interleaved = _interleaved(layout)
     if keep not in (None, "int8"):
         raise ValueError(f"unknown way to keep queries and keys '{keep}'")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
+    if torch.is_autocast_enabled("cuda"):
+        q_weight, k_weight = (w if x is None or w is None else w.to(x.dtype) for x, w in ((q, q_weight), (k, k_weight)))
     return load_native_calls().qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, interleaved, magnitude, eps, keep == "int8")

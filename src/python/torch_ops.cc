@@ -76,6 +76,7 @@ int dtype_code(const char* what, const at::Tensor& t) {
 
 const at::Tensor& on_gpu(const char* what, const at::Tensor& t) {
     if (!t.is_cuda() || t.layout() != at::kStrided) refuse(std::string(what) + " must be a dense CUDA tensor");
+    if (t.is_neg()) refuse(std::string(what) + " is a view that stands for its negative: resolve_neg() makes a tensor of it");
     return t;
 }
 const at::Tensor& tensor_of(const char* what, PyObject* obj) {
@@ -249,6 +250,11 @@ variable_list in_backward(const char* what, F&& f) {
     return grads;
 }
 
+// What a call has no gradient of would come out of a backward pass as if it had no influence.
+void no_gradient_of(const char* what, const at::Tensor& t) {
+    if (at::GradMode::is_enabled() && t.requires_grad()) refuse(std::string(what) + " require a gradient, and none is made for them");
+}
+
 bool wants_gradient(std::initializer_list<const at::Tensor*> tensors) {
     if (!at::GradMode::is_enabled()) return false;
     for (const at::Tensor* t : tensors)
@@ -356,8 +362,7 @@ PyObject* weight_grad8(PyObject* const* args, Py_ssize_t nargs) {
 
 struct Linear8 : torch::autograd::Function<Linear8> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias) {
-        const bool needs = weight.requires_grad() || (bias.has_value() && bias->defined() && bias->requires_grad());
-        ctx->save_for_backward({weight, needs ? pack(x) : at::Tensor()});
+        ctx->save_for_backward({weight, weight.requires_grad() ? pack(x) : at::Tensor()});
         ctx->saved_data["bias"] = bias.has_value();
         return at::linear(x, weight, bias);
     }
@@ -370,6 +375,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
             if (ctx->needs_input_grad(0)) dx = at::matmul(dy, weight);
             const bool bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
             if (kept.defined()) std::tie(dw, db) = weight_grad(on_gpu("dy", dy), kept, weight.size(1), bias);
+            else if (bias) db = dy.reshape({-1, weight.size(0)}).sum(0);  // of a frozen weight
             if (!ctx->needs_input_grad(1)) dw = at::Tensor();
             return {dx, dw, db};
         });
@@ -383,7 +389,8 @@ PyObject* linear8(PyObject* const* args, Py_ssize_t nargs) {
     const at::Tensor bias = maybe_tensor("bias", args[2]);
     same_place("weight", weight, x);
     same_dtype("weight", weight, x);
-    if (x.dim() < 2 || weight.dim() != 2 || x.size(-1) != weight.size(1)) refuse("the input does not go into the weight");
+    if (x.dim() < 1 || weight.dim() != 2 || x.size(-1) != weight.size(1)) refuse("the input does not go into the weight");
+    if (weight.numel() == 0) refuse("a projection has at least one input and one output");
     if (bias.defined()) {
         same_place("bias", bias, x);
         same_dtype("bias", bias, x);
@@ -578,6 +585,7 @@ PyObject* rotary(PyObject* const* args, Py_ssize_t nargs) {
     need_arguments(nargs, 6);
     const at::Tensor q = maybe_tensor("q", args[0]), k = maybe_tensor("k", args[1]);
     const Turn turn{tensor_of("positions", args[2]), tensor_of("frequencies", args[3]), truth(args[4]), number("magnitude", args[5]), 0.0};
+    no_gradient_of("frequencies", turn.frequencies);
     if (wants_gradient({&q, &k}))
         return pair_of(Rotary::apply(optional_of(q), optional_of(k), turn.positions, turn.frequencies, turn.interleaved, turn.magnitude), q.defined(), k.defined());
     auto [q_out, k_out] = rotate(both_of("q", "k", q, k), turn, false);
@@ -716,6 +724,7 @@ PyObject* qk_norm_rotary(PyObject* const* args, Py_ssize_t nargs) {
     const at::Tensor weights[2] = {maybe_tensor(kWeightNames[0], args[2]), maybe_tensor(kWeightNames[1], args[3])};
     const Turn turn{tensor_of("positions", args[4]), tensor_of("frequencies", args[5]), truth(args[6]), number("magnitude", args[7]), number("eps", args[8])};
     const bool keep8 = truth(args[9]);
+    no_gradient_of("frequencies", turn.frequencies);
     if (wants_gradient({&q, &k, &weights[0], &weights[1]}))
         return pair_of(NormRotary::apply(optional_of(q), optional_of(k), optional_of(weights[0]), optional_of(weights[1]), turn.positions, turn.frequencies,
                                          turn.interleaved, turn.magnitude, turn.eps, keep8),

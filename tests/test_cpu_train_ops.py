@@ -42,6 +42,12 @@ def test_frequencies():
     f, m = ops.rotary_frequencies(128, scaling="yarn", factor=16.0, context=2048, device="cpu")
     plain = 10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64)
     assert torch.equal(f[:10], plain[:10]) and torch.allclose(f[-5:], plain[-5:] / 16) and m == pytest.approx(0.1 * math.log(16.0) + 1)
+    # ... where no pair makes fewer than `slow` turns (none is divided in full), and where none makes as many (all are)
+    f, _ = ops.rotary_frequencies(64, scaling="yarn", factor=16.0, context=131072, device="cpu")
+    plain = 10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    assert (plain * 131072 / (2 * math.pi) > 1).all() and (f > plain / 16 * 1.01).all()
+    f, _ = ops.rotary_frequencies(64, scaling="yarn", factor=16.0, context=4, device="cpu")
+    assert torch.allclose(f, plain / 16, rtol=1e-14, atol=0)
 
 
 class Heads(ctypes.Structure):

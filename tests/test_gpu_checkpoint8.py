@@ -267,6 +267,15 @@ def test_linear(dtype):
     assert torch.autograd.grad(ops.linear8(x, w), (w,), dy)[0].equal(dw)
     frozen = ops.linear8(x, w.detach(), b.detach())
     assert torch.autograd.grad(frozen, (x,), dy)[0].equal(dx)
+    # A frozen weight: the bias's gradient needs no input. Two roundings of at most half a step each, sums of 63 terms in 32 bits beside them.
+    (only_b,) = torch.autograd.grad(ops.linear8(x.detach(), w.detach(), b), (b,), dy)
+    assert torch.allclose(only_b.double(), db.double(), rtol=torch.finfo(dtype).eps, atol=64 * 2.0**-24 * float(dy.abs().sum((0, 1)).max()))
+    # One token without leading axes.
+    dx1, dw1, db1 = torch.autograd.grad(ops.linear8(x[0, 0], w, b), (x, w, b), dy[0, 0])
+    want = ops.weight_grad8(dy[0, 0], ops.pack8(x[0, 0]), bias=True)
+    assert torch.equal(dx1[0, 0], dy[0, 0] @ w) and torch.equal(dw1, want[0]) and torch.equal(db1, dy[0, 0])
+    # One product: exact in 32 bits where dy has 16; three parts of it added in 24 bits, cut or rounded, where it has 32.
+    assert torch.allclose(dw1, torch.outer(dy[0, 0], ops.unpack8(ops.pack8(x[0, 0]))), rtol=0.0 if dtype != torch.float32 else 4 * 2.0**-23, atol=0.0)
 
 
 def test_linear_under_autocast():
@@ -328,6 +337,7 @@ def test_refusals():
                  lambda: ops.unpack8(ops.Packed8(p.data, (4, 64), torch.float64)), lambda: ops.unpack8(ops.Packed8(p.data[1:], (4, 64), torch.float32)),
                  lambda: ops.gelu8(x, "erf"), lambda: ops.gelu8(x.double()), lambda: ops.weight_grad8(x, half), lambda: ops.weight_grad8(x[:3], p),
                  lambda: ops.weight_grad8(x.cpu(), p), lambda: ops.weight_grad8(x, x), lambda: ops.linear8(x, x.half()),
-                 lambda: ops.linear8(x, torch.ones(8, 63, device="cuda"))):
+                 lambda: ops.linear8(x, torch.ones(8, 63, device="cuda")), lambda: ops.linear8(x[:, :0], torch.ones(8, 0, device="cuda")),
+                 lambda: ops.pack8(torch.ones(4, 64, dtype=torch.complex64, device="cuda").conj().imag)):
         with pytest.raises(ValueError):
             call()

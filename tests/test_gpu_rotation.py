@@ -227,9 +227,24 @@ def test_refusals():
                  lambda: ops.rotary(q[None], None, torch.stack([p, p]), f), lambda: ops.rotary(q[:, :0], None, p, f),
                  lambda: ops.qk_norm_rotary(q, None, None, None, p, f), lambda: ops.qk_norm_rotary(q, None, w[:32], None, p, f),
                  lambda: ops.qk_norm_rotary(q, None, w.half(), None, p, f), lambda: ops.qk_norm_rotary(q, None, w, None, p, f, keep="fp8"),
-                 lambda: ops.qk_norm_rotary(q, None, w, None, p, f, eps=-1.0), lambda: ops.qk_norm_rotary(q, q, w, None, p, f)):
+                 lambda: ops.qk_norm_rotary(q, None, w, None, p, f, eps=-1.0), lambda: ops.qk_norm_rotary(q, q, w, None, p, f),
+                 lambda: ops.rotary(q, None, p, f.clone().requires_grad_()), lambda: ops.qk_norm_rotary(q, None, w, None, p, f.clone().requires_grad_())):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("keep", [None, "int8"])
+def test_norm_under_autocast(keep):
+    q, k = (torch.randn(2, 9, h, 64, device="cuda", dtype=torch.bfloat16) for h in (4, 2))
+    w = [torch.linspace(0.5, 1.5, 64, device="cuda", requires_grad=True) for _ in range(2)]
+    p, f = torch.arange(9, device="cuda"), frequencies(64).cuda()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = ops.qk_norm_rotary(q, k, *w, p, f, keep=keep)
+    narrow = [v.detach().bfloat16().requires_grad_() for v in w]
+    want = ops.qk_norm_rotary(q, k, *narrow, p, f, keep=keep)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for grads in zip(torch.autograd.grad([v.float().square().sum() for v in got], w), torch.autograd.grad([v.float().square().sum() for v in want], narrow)):
+        assert grads[0].dtype == torch.float32 and torch.equal(grads[0], grads[1].float())
 
 
 def test_scaled_frequencies():

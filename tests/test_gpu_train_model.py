@@ -144,6 +144,17 @@ def test_a_captured_step_repeats_the_eager_one(options, dtype):
     assert torch.equal(captured, eager)
 
 
+def test_a_step_under_autocast():
+    torch.manual_seed(2)
+    model = TinyGPT2(vocab=64, context=16, hidden=64, layers=2, heads=2, positions="rotary", qk_norm=True, checkpoints="int8").cuda()
+    tokens = torch.randint(0, 64, (4, 16), device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = model(tokens).float().logsumexp(-1).mean()
+    loss.backward()
+    for name, p in model.named_parameters():
+        assert p.grad.dtype == torch.float32 and p.grad.isfinite().all() and p.grad.any(), name
+
+
 def test_what_a_step_keeps():
     """The point of it: 33 bytes for 32 elements instead of 64 or 128."""
     def kept(f, *leaves):
