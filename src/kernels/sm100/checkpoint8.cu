@@ -1,6 +1,8 @@
 // Activations kept in 8 bits for the backward pass: the codec, alone and in the same pass as GELU and its derivative.
 //
-// Bound by HBM: a 16-bit element is read once and its 1 + 1/32 bytes are written once (and y beside them), or the other way round.
+// Bound by HBM: a 16-bit element is read once and its 1 + 1/32 bytes are written once (and y beside them), or the other way round. bf16: 16384 x 4096 are kept in
+// 28 us and read back in 30 (7.3 and 6.7 TB/s, some of it from L2); GELU of 8192 x 8192 takes 60 us, its gradient 64 (5.6 and 5.3 TB/s, 0.8 of a copy's rate, with
+// 0.7 of the issue slots taken: codes two at a time and fp32 numbers by pairs took 95 and 87 to that).
 // Formulas of the 8-bit form: block8.cuh. GELU keeps its INPUT: y = x Phi(x) is made from x itself, dx = dy * (Phi + x phi)(x^) from what
 // was kept, so the forward result does not change and the backward needs neither x nor y.
 //

@@ -31,7 +31,10 @@ def angle_error(x, n, interleaved, magnitude):
 
 # dim, rotated, heads, kv_heads, batch, tokens
 SHAPES = [(64, 64, 12, 12, 1, 1), (128, 128, 8, 2, 2, 33), (80, 40, 7, 1, 3, 21), (2, 2, 1, 1, 1, 5), (256, 256, 3, 1, 1, 9), (96, 32, 4, 4, 2, 7), (62, 30, 5, 3, 1, 17),
-          (250, 6, 2, 1, 2, 3), (64, 0, 2, 2, 1, 4), (32, 16, 1, 1, 1, 300), (48, 48, 130, 1, 1, 3)]
+          (250, 6, 2, 1, 2, 3), (64, 0, 2, 2, 1, 4), (32, 16, 1, 1, 1, 300), (48, 48, 130, 1, 1, 3),
+          # Halves and ends of the turning part between multiples of 16, 8 and 4 bytes; many heads of few tokens, which several warps share.
+          (128, 102, 56, 8, 1, 40), (256, 190, 4, 4, 3, 20), (72, 22, 9, 3, 2, 50), (76, 76, 5, 1, 1, 130), (132, 130, 3, 2, 1, 7), (254, 254, 2, 1, 1, 6),
+          (30, 30, 56, 8, 1, 31), (16, 2, 3, 3, 1, 700), (96, 24, 3, 3, 2, 90)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -92,6 +95,22 @@ def test_views_layouts_and_three_axes():
     out, _ = ops.rotary(leaf, None, positions, f)
     out.sum().backward()  # a gradient without memory of its own
     assert torch.equal(leaf.grad, ops.rotary(torch.ones_like(q), None, -positions, f)[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,r", [(128, 102), (128, 72), (64, 22), (72, 22), (76, 38), (30, 14), (64, 0)])
+def test_what_does_not_turn_stays_as_it_is(dtype, interleaved, d, r):
+    """To the last bit, whatever stands beside it: infinities, NaN, zeros with signs."""
+    x = values((1, 40, 3, d), dtype).cuda()
+    x[0, :10] = float("inf")
+    x[0, 10:20, :, :r] = float("nan")
+    x[0, 20:30, :, ::2] = float("-inf")
+    x[0, 30:] = -0.0
+    y, _ = ops.rotary(x, None, torch.arange(40).cuda(), frequencies(r).cuda(), "interleaved" if interleaved else "half")
+    as_bits = torch.int32 if dtype == torch.float32 else torch.int16
+    assert torch.equal(y[..., r:].contiguous().view(as_bits), x[..., r:].contiguous().view(as_bits))
+    assert y[0, 10:20, :, :r].isnan().all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
