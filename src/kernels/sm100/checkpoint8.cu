@@ -396,6 +396,19 @@ template <typename T>
 __device__ __forceinline__ unsigned behind(const Kept8Args& a) {
     return (unsigned)(reinterpret_cast<std::uintptr_t>(a.out) & 15u) / (unsigned)sizeof(T);
 }
+// Of the granules k0 to k1 those that lie across two rows, one at the end of a row: all of a CTA's side by side, because a warp that meets one
+// among others goes the long way for it (GELU of 13760 x 185 bf16, there and back: 27.5 us with them among the others, 17.5 so).
+template <typename T, Activation kAct, bool kRead>
+__device__ __forceinline__ void across_rows(const Kept8Args& a, u64 k0, u64 k1, const Spot& from, u64 origin, unsigned m) {
+    constexpr unsigned E = kGranule<T>;
+    if (a.columns < E) return;
+    for (u64 row = (u64)from.row + threadIdx.x;; row += kThreads) {
+        const u64 end = (row + 1u) * a.columns, k = (end + m) / E;
+        if (k >= k1) break;
+        const u64 e = k * E - m;
+        if ((end + m) % E != 0u && k >= k0 && k * E >= m && e + E <= a.elements) gather_granule<T, kAct, kRead>(a, e, e + E, from, origin);
+    }
+}
 
 template <typename T, Activation kAct>
 __global__ void __launch_bounds__(kThreads) keep8_any_kernel(const Kept8Args a) {
@@ -438,17 +451,18 @@ __global__ void __launch_bounds__(kThreads) keep8_any_kernel(const Kept8Args a) 
         for (u64 k = k0 + threadIdx.x; k < k1; k += kThreads) {
             const u64 e = k * E - m;  // before 0 for the first granule of an output that is not aligned
             const Spot s = spot_at(a, from, k * E < m ? 0u : (unsigned)(e - origin));
-            if (k * E >= m && e + E <= a.elements && s.column + E <= a.columns) {
+            if (k * E < m || e + E > a.elements || a.columns < E) {
+                gather_granule<T, kAct, false>(a, k * E < m ? 0 : e, min(a.elements, e + E), from, origin);
+            } else if (s.column + E <= a.columns) {
                 unsigned w[4];
                 load_any<T, E>(a.in + (long long)s.row * a.stride + (long long)(s.column * (unsigned)sizeof(T)), E, w);
                 float2 f[E / 2];
 #pragma unroll
                 for (unsigned i = 0; i < E / 2; ++i) f[i] = activate<kAct>(pair_in<T>(w, i));
                 store_granule<T>(a.out + e * sizeof(T), f);
-            } else {
-                gather_granule<T, kAct, false>(a, k * E < m ? 0 : e, min(a.elements, e + E), from, origin);
             }
         }
+        across_rows<T, kAct, false>(a, k0, k1, from, origin, m);
     }
 }
 
@@ -476,10 +490,11 @@ __global__ void __launch_bounds__(kThreads) read8_any_kernel(const Kept8Args a) 
         const u64 e = k * E - m;
         if (!before && e >= a.elements) continue;
         const Spot s = spot_at(a, from, before ? 0u : (unsigned)(e - origin));
-        if (before || e + E > a.elements || s.column + E > a.columns) {
+        if (before || e + E > a.elements || a.columns < E) {
             gather_granule<T, kAct, true>(a, before ? 0 : e, min(a.elements, e + E), from, origin);
             continue;
         }
+        if (s.column + E > a.columns) continue;
         // E codes, at any address, and the steps of the one or two blocks that they belong to.
         const u64 half = (u64)s.row * a.halves.d;
         const unsigned char* codes = a.codes + half * 16u + s.column;
@@ -508,6 +523,7 @@ __global__ void __launch_bounds__(kThreads) read8_any_kernel(const Kept8Args a) 
         }
         store_granule<T>(a.out + e * sizeof(T), f);
     }
+    across_rows<T, kAct, true>(a, k0, k0 + kThreads * kGranules, from, origin, m);
 }
 
 template <typename T, Activation kAct>
