@@ -134,4 +134,40 @@ __device__ __forceinline__ uint2 widen8x4(unsigned word, unsigned step) {
 
 __device__ __forceinline__ unsigned magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// N neighbouring elements at p, of which `count` are there; the others are zeros. p is a multiple of an element: the aligned 16 bytes that hold a wanted one
+// are read, and shifted.
+template <typename T, int N>
+__device__ __forceinline__ void load_any(const char* p, unsigned count, unsigned (&w)[N * sizeof(T) / 4]) {
+    constexpr unsigned W = N * sizeof(T) / 4, G = W / 4 + 1;
+    const unsigned shift = (unsigned)(reinterpret_cast<std::uintptr_t>(p) & 15u);
+    const char* base = p - shift;
+    unsigned r[4 * G];
+#pragma unroll
+    for (unsigned g = 0; g < G; ++g) {
+        const uint4 v = 16u * g < shift + count * (unsigned)sizeof(T) && count != 0u ? *reinterpret_cast<const uint4*>(base + 16 * g) : make_uint4(0u, 0u, 0u, 0u);
+        r[4 * g] = v.x;
+        r[4 * g + 1] = v.y;
+        r[4 * g + 2] = v.z;
+        r[4 * g + 3] = v.w;
+    }
+#pragma unroll
+    for (unsigned i = 0; i < W + 2; ++i) r[i] = shift & 8u ? r[i + 2] : r[i];
+#pragma unroll
+    for (unsigned i = 0; i < W + 1; ++i) r[i] = shift & 4u ? r[i + 1] : r[i];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (unsigned i = 0; i < W; ++i) w[i] = shift & 2u ? __funnelshift_r(r[i], r[i + 1], 16) : r[i];
+    } else {
+#pragma unroll
+        for (unsigned i = 0; i < W; ++i) w[i] = r[i];
+    }
+    if (count < (unsigned)N) {
+#pragma unroll
+        for (unsigned i = 0; i < W; ++i) {
+            if constexpr (sizeof(T) == 2) w[i] = 2u * i + 1u < count ? w[i] : (2u * i < count ? w[i] & 0xffffu : 0u);
+            else w[i] = i < count ? w[i] : 0u;
+        }
+    }
+}
+
 }  // namespace b200ccl::dev

@@ -288,41 +288,6 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const Kept8Args a) {
 // Inputs are read as the aligned 16 bytes that they lie in, and shifted; only those that hold a wanted element are touched. What is written to rows without
 // gaps is cut where the memory is aligned, wherever rows and blocks begin: a thread makes 16 bytes of the output.
 
-// N neighbouring elements at p, of which `count` are there; the others are zeros.
-template <typename T, int N>
-__device__ __forceinline__ void load_any(const char* p, unsigned count, unsigned (&w)[N * sizeof(T) / 4]) {
-    constexpr unsigned W = N * sizeof(T) / 4, G = W / 4 + 1;
-    const unsigned shift = (unsigned)(reinterpret_cast<std::uintptr_t>(p) & 15u);
-    const char* base = p - shift;
-    unsigned r[4 * G];
-#pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-        const uint4 v = 16u * g < shift + count * (unsigned)sizeof(T) && count != 0u ? *reinterpret_cast<const uint4*>(base + 16 * g) : make_uint4(0u, 0u, 0u, 0u);
-        r[4 * g] = v.x;
-        r[4 * g + 1] = v.y;
-        r[4 * g + 2] = v.z;
-        r[4 * g + 3] = v.w;
-    }
-#pragma unroll
-    for (unsigned i = 0; i < W + 2; ++i) r[i] = shift & 8u ? r[i + 2] : r[i];
-#pragma unroll
-    for (unsigned i = 0; i < W + 1; ++i) r[i] = shift & 4u ? r[i + 1] : r[i];
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (unsigned i = 0; i < W; ++i) w[i] = shift & 2u ? __funnelshift_r(r[i], r[i + 1], 16) : r[i];
-    } else {
-#pragma unroll
-        for (unsigned i = 0; i < W; ++i) w[i] = r[i];
-    }
-    if (count < (unsigned)N) {
-#pragma unroll
-        for (unsigned i = 0; i < W; ++i) {
-            if constexpr (sizeof(T) == 2) w[i] = 2u * i + 1u < count ? w[i] : (2u * i < count ? w[i] & 0xffffu : 0u);
-            else w[i] = i < count ? w[i] : 0u;
-        }
-    }
-}
-
 template <typename T>
 constexpr int kGranule = 16 / sizeof(T);  // elements of 16 bytes
 
