@@ -14,6 +14,7 @@
 #include "kernels/sm100/block8.cuh"
 #include "kernels/sm100/launch.h"
 #include "kernels/sm100/pair32.cuh"
+#include "kernels/sm100/tma.cuh"
 
 #include <cstdint>
 #include <type_traits>
@@ -38,7 +39,6 @@ struct Kept8Args {
     unsigned columns;
     Divisor halves;   // half blocks of a row
     unsigned items;   // half blocks of all rows
-    Divisor by_columns;
 };
 
 // exp(-x^2/2) and 1 - Phi(|x|) of two numbers.
@@ -285,210 +285,131 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const Kept8Args a) {
 }
 
 // ---- any columns, strides and alignment ------------------------------------------------------------------
-// Inputs are read as the aligned 16 bytes that they lie in, and shifted; only those that hold a wanted element are touched. What is written to rows without
-// gaps is cut where the memory is aligned, wherever rows and blocks begin: a thread makes 16 bytes of the output.
+// A lane still has 16 elements of one row, or what is left of it. Inputs are read as the aligned 16 bytes that they lie in, and shifted. Outputs have no gaps
+// between rows, so a warp's are one run of memory: it goes through shared memory, from where every lane writes aligned 16 bytes. (16384 x 2047 bf16, GELU there
+// and back: 115 us when threads made 16 bytes of the output each from what they belong to, 88 so; 16384 x 2048: 62.)
+template <typename T>
+constexpr unsigned kStageBytes = (32 * 16 * sizeof(T) + 16) / 128 * 144 + 144;
 
-template <typename T>
-constexpr int kGranule = 16 / sizeof(T);  // elements of 16 bytes
+// Byte p of a run, with a gap after every 128, so that lanes 32 bytes apart write to different banks.
+__device__ __forceinline__ unsigned in_stage(unsigned stage, unsigned p) { return stage + p + (p >> 7 << 4); }
+__device__ __forceinline__ void stage4(unsigned at, unsigned v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void stage2(unsigned at, unsigned v) { asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"((unsigned short)v) : "memory"); }
 
+// Writes the warp's elements: `count` of a lane, from element `first` of all on, behind those of the lane before it. All lanes call it.
 template <typename T>
-__device__ __forceinline__ float2 pair_in(const unsigned* w, int i) {
-    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-    else if constexpr (std::is_same_v<T, __half>) return h2_to_f2(w[i]);
-    else return b2_to_f2(w[i]);
-}
-template <typename T>
-__device__ __forceinline__ void store_granule(char* p, const float2 (&f)[kGranule<T> / 2]) {
-    unsigned w[4];
+__device__ __forceinline__ void store_run(char* out, unsigned stage, u64 first, unsigned count, const unsigned (&w)[4 * sizeof(T)]) {
+    constexpr unsigned S = sizeof(T);
+    const unsigned lane = threadIdx.x & 31u;
+    const u64 begin = __shfl_sync(0xffffffffu, first, 0);
+    const unsigned before = (unsigned)(first - begin), total = __shfl_sync(0xffffffffu, before + count, 31);
+    char* to = out + begin * S;
+    const unsigned off = (unsigned)(reinterpret_cast<std::uintptr_t>(to) & 15u), end = off + total * S, p = off + before * S;
+    to -= off;
+    if constexpr (S == 4) {
 #pragma unroll
-    for (int i = 0; i < kGranule<T> / 2; ++i) {
-        if constexpr (sizeof(T) == 4) {
-            w[2 * i] = __float_as_uint(f[i].x);
-            w[2 * i + 1] = __float_as_uint(f[i].y);
-        } else {
-            w[i] = std::is_same_v<T, __half> ? f2_to_h2(f[i].x, f[i].y) : f2_to_b2(f[i].x, f[i].y);
-        }
-    }
-    store16_once(p, make_uint4(w[0], w[1], w[2], w[3]));
-}
-
-// Where element `from + offset` of all lies, `from` being element (row, column): offsets are small.
-struct Spot {
-    unsigned row, column;
-};
-__device__ __forceinline__ Spot spot_at(const Kept8Args& a, const Spot& from, unsigned offset) {
-    const unsigned in = from.column + offset, rows = a.by_columns.divide(in);
-    return {from.row + rows, in - rows * a.columns};
-}
-
-// One element of the input, and of x^.
-template <typename T>
-__device__ __forceinline__ float input_at(const Kept8Args& a, const Spot& s) {
-    return Elem<T>::to_f(*(reinterpret_cast<const T*>(a.in + (long long)s.row * a.stride) + s.column));
-}
-__device__ __forceinline__ float kept_at(const Kept8Args& a, const Spot& s) {
-    const u64 half = (u64)s.row * a.halves.d;
-    return decode8<0>(a.codes[half * 16u + s.column], step8(a.scales[half / 2u + s.column / kBlock8]));
-}
-// Two elements of the output.
-template <typename T, Activation kAct, bool kRead>
-__device__ __forceinline__ float2 two_at(const Kept8Args& a, const Spot& s, const Spot& t) {
-    if constexpr (!kRead) return activate<kAct>(make_float2(input_at<T>(a, s), input_at<T>(a, t)));
-    const float2 v = make_float2(kept_at(a, s), kept_at(a, t));
-    if constexpr (kAct == Activation::None) return v;
-    else return through<kAct>(v, make_float2(input_at<T>(a, s), input_at<T>(a, t)));
-}
-// A granule of the output that lies across rows, or not wholly in it: elements [begin, end) of the E from `origin` + `offset` on, `origin` being (row, column).
-template <typename T, Activation kAct, bool kRead>
-__device__ __forceinline__ void gather_granule(const Kept8Args& a, u64 begin, u64 end, const Spot& from, u64 origin) {
-    constexpr unsigned E = kGranule<T>;
-    if (end - begin == E) {
-        float2 f[E / 2];
+        for (unsigned i = 0; i < 16; ++i)
+            if (i < count) stage4(in_stage(stage, p + 4u * i), w[i]);
+    } else if (count < 16u) {
 #pragma unroll
-        for (unsigned i = 0; i < E / 2; ++i)
-            f[i] = two_at<T, kAct, kRead>(a, spot_at(a, from, (unsigned)(begin - origin) + 2u * i), spot_at(a, from, (unsigned)(begin - origin) + 2u * i + 1u));
-        store_granule<T>(a.out + begin * sizeof(T), f);
+        for (unsigned i = 0; i < 16; ++i)
+            if (i < count) stage2(in_stage(stage, p + 2u * i), w[i / 2] >> (i % 2 * 16));
+    } else if ((p & 2u) == 0u) {
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i) stage4(in_stage(stage, p + 4u * i), w[i]);
     } else {
-        for (u64 e = begin; e < end; ++e) {
-            const Spot s = spot_at(a, from, (unsigned)(e - origin));
-            reinterpret_cast<T*>(a.out)[e] = Elem<T>::from_f(two_at<T, kAct, kRead>(a, s, s).x);
+        stage2(in_stage(stage, p), w[0]);
+#pragma unroll
+        for (unsigned i = 1; i < 8; ++i) stage4(in_stage(stage, p + 4u * i - 2u), __funnelshift_r(w[i - 1], w[i], 16));
+        stage2(in_stage(stage, p + 30u), w[7] >> 16);
+    }
+    __syncwarp();
+    for (unsigned b = lane * 16u; b + 16u <= end; b += 512u) {
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(in_stage(stage, b)) : "memory");
+        if (b >= off) store16_once(to + b, v);
+    }
+    // The ends: what stands before the first whole 16 bytes, and behind the last.
+    const unsigned last = end & ~15u;
+    const unsigned b = lane < 16u ? off + lane * S : last + (lane - 16u) * S;
+    if (lane < 16u ? off != 0u && b < min(16u, end) : b < end && (last != 0u || off == 0u)) {
+        const unsigned at = in_stage(stage, b);
+        if constexpr (S == 4) {
+            unsigned v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+            *reinterpret_cast<unsigned*>(to + b) = v;
+        } else {
+            unsigned short v;
+            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+            *reinterpret_cast<unsigned short*>(to + b) = v;
         }
     }
+    __syncwarp();
 }
 
-// Elements by which the output lies behind a multiple of 16 bytes.
-template <typename T>
-__device__ __forceinline__ unsigned behind(const Kept8Args& a) {
-    return (unsigned)(reinterpret_cast<std::uintptr_t>(a.out) & 15u) / (unsigned)sizeof(T);
+// Where the 16 elements of a half block lie.
+struct Half {
+    unsigned row, column, count;
+};
+__device__ __forceinline__ Half half_at(const Kept8Args& a, unsigned i) {
+    const unsigned row = a.halves.divide(i), column = (i - row * a.halves.d) * 16u;
+    return {row, column, i < a.items && column < a.columns ? min(16u, a.columns - column) : 0u};
 }
-// Of the granules k0 to k1 those that lie across two rows, one at the end of a row: all of a CTA's side by side, because a warp that meets one
-// among others goes the long way for it (GELU of 13760 x 185 bf16, there and back: 27.5 us with them among the others, 17.5 so).
-template <typename T, Activation kAct, bool kRead>
-__device__ __forceinline__ void across_rows(const Kept8Args& a, u64 k0, u64 k1, const Spot& from, u64 origin, unsigned m) {
-    constexpr unsigned E = kGranule<T>;
-    if (a.columns < E) return;
-    for (u64 row = (u64)from.row + threadIdx.x;; row += kThreads) {
-        const u64 end = (row + 1u) * a.columns, k = (end + m) / E;
-        if (k >= k1) break;
-        const u64 e = k * E - m;
-        if ((end + m) % E != 0u && k >= k0 && k * E >= m && e + E <= a.elements) gather_granule<T, kAct, kRead>(a, e, e + E, from, origin);
-    }
+// Its first element, of all; that of the next one if it has none.
+__device__ __forceinline__ u64 first_of(const Kept8Args& a, const Half& h, unsigned i) {
+    return i < a.items ? (u64)h.row * a.columns + min(h.column, a.columns) : a.elements;
+}
+template <typename T>
+__device__ __forceinline__ void load_half(const Kept8Args& a, const Half& h, unsigned (&w)[4 * sizeof(T)]) {
+    load_any<T, 16>(a.in + (h.count == 0u ? 0ll : (long long)h.row * a.stride + (long long)(h.column * (unsigned)sizeof(T))), h.count, w);
 }
 
 template <typename T, Activation kAct>
 __global__ void __launch_bounds__(kThreads) keep8_any_kernel(const Kept8Args a) {
-    constexpr int U = kInFlight<T>;
+    __shared__ __align__(16) unsigned char stages[kAct == Activation::None ? 16 : kThreads / 32 * kStageBytes<T>];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned begin = blockIdx.x * (kThreads * U);
+    const unsigned i = blockIdx.x * kThreads + threadIdx.x;
+    const Half h = half_at(a, i);
+    Sixteen<T> x;
+    load_half<T>(a, h, x.w);
     if (kAct == Activation::None || a.codes != nullptr) {
-        Sixteen<T> x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const unsigned i = begin + threadIdx.x + u * kThreads;
-            const unsigned row = a.halves.divide(i), column = (i - row * a.halves.d) * 16u;
-            const unsigned count = i < a.items && column < a.columns ? min(16u, a.columns - column) : 0u;
-            load_any<T, 16>(a.in + (count == 0u ? 0ll : (long long)row * a.stride + (long long)(column * (unsigned)sizeof(T))), count, x[u].w);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const unsigned i = begin + threadIdx.x + u * kThreads;
-            unsigned amax = x[u].amax();
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            if (i < a.items) {
-                const unsigned scale = scale8<T>(amax);
-                store16_once(a.codes + (u64)i * 16u, x[u].codes(scale));
-                if ((i & 1u) == 0) a.scales[i >> 1] = (unsigned char)scale;
-            }
+        unsigned amax = x.amax();
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        if (i < a.items) {
+            const unsigned scale = scale8<T>(amax);
+            store16_once(a.codes + (u64)i * 16u, x.codes(scale));
+            if ((i & 1u) == 0) a.scales[i >> 1] = (unsigned char)scale;
         }
     }
     if constexpr (kAct != Activation::None) {
-        // The elements of the same half blocks, by granules of the output that begin among them; they are in L1.
-        constexpr unsigned E = kGranule<T>;
-        const unsigned end = min(a.items, begin + kThreads * U), m = behind<T>(a);
-        const auto first_of = [&](unsigned i) {
-            const unsigned row = a.halves.divide(i);
-            return Spot{row, min(a.columns, (i - row * a.halves.d) * 16u)};
-        };
-        const Spot from = first_of(begin), to = first_of(end);
-        const u64 origin = (u64)from.row * a.columns + from.column, stop = end == a.items ? a.elements : (u64)to.row * a.columns + to.column;
-        const u64 k0 = origin == 0 ? 0 : (origin + m + E - 1) / E, k1 = (stop + m + E - 1) / E;
-        for (u64 k = k0 + threadIdx.x; k < k1; k += kThreads) {
-            const u64 e = k * E - m;  // before 0 for the first granule of an output that is not aligned
-            const Spot s = spot_at(a, from, k * E < m ? 0u : (unsigned)(e - origin));
-            if (k * E < m || e + E > a.elements || a.columns < E) {
-                gather_granule<T, kAct, false>(a, k * E < m ? 0 : e, min(a.elements, e + E), from, origin);
-            } else if (s.column + E <= a.columns) {
-                unsigned w[4];
-                load_any<T, E>(a.in + (long long)s.row * a.stride + (long long)(s.column * (unsigned)sizeof(T)), E, w);
-                float2 f[E / 2];
 #pragma unroll
-                for (unsigned i = 0; i < E / 2; ++i) f[i] = activate<kAct>(pair_in<T>(w, i));
-                store_granule<T>(a.out + e * sizeof(T), f);
-            }
-        }
-        across_rows<T, kAct, false>(a, k0, k1, from, origin, m);
+        for (int e = 0; e < 8; ++e) x.set(e, activate<kAct>(x.pair(e)));
+        store_run<T>(a.out, smem_addr(stages) + threadIdx.x / 32u * kStageBytes<T>, first_of(a, h, i), h.count, x.w);
     }
 }
 
-constexpr unsigned kGranules = 2;  // of a thread
-
 template <typename T, Activation kAct>
 __global__ void __launch_bounds__(kThreads) read8_any_kernel(const Kept8Args a) {
-    constexpr unsigned E = kGranule<T>;
+    __shared__ __align__(16) unsigned char stages[kThreads / 32 * kStageBytes<T>];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned m = behind<T>(a);
-    const u64 k0 = (u64)blockIdx.x * (kThreads * kGranules);
-    const u64 origin = k0 * E < m ? 0 : k0 * E - m;
-    __shared__ Spot first;
-    if (threadIdx.x == 0) {  // a division of 64 bits, once
-        const u64 row = origin / a.columns;
-        first = {(unsigned)row, (unsigned)(origin - row * a.columns)};
+    const unsigned i = blockIdx.x * kThreads + threadIdx.x;
+    const Half h = half_at(a, i);
+    uint4 c = make_uint4(0u, 0u, 0u, 0u);
+    unsigned scale = 127u;
+    if (i < a.items) {
+        c = load16_once(reinterpret_cast<const uint4*>(a.codes) + i);
+        scale = a.scales[i >> 1];
     }
-    __syncthreads();
-    const Spot from = first;
+    Sixteen<T> x, dy;
+    if constexpr (kAct != Activation::None) load_half<T>(a, h, dy.w);
+    x.widen(c, scale);
+    if constexpr (kAct != Activation::None) {
 #pragma unroll
-    for (unsigned u = 0; u < kGranules; ++u) {
-        const u64 k = k0 + threadIdx.x + u * kThreads;
-        const bool before = k * E < m;
-        const u64 e = k * E - m;
-        if (!before && e >= a.elements) continue;
-        const Spot s = spot_at(a, from, before ? 0u : (unsigned)(e - origin));
-        if (before || e + E > a.elements || a.columns < E) {
-            gather_granule<T, kAct, true>(a, before ? 0 : e, min(a.elements, e + E), from, origin);
-            continue;
-        }
-        if (s.column + E > a.columns) continue;
-        // E codes, at any address, and the steps of the one or two blocks that they belong to.
-        const u64 half = (u64)s.row * a.halves.d;
-        const unsigned char* codes = a.codes + half * 16u + s.column;
-        const unsigned shift = (unsigned)(reinterpret_cast<std::uintptr_t>(codes) & 3u) * 8u;
-        const unsigned* words = reinterpret_cast<const unsigned*>(codes - shift / 8u);
-        unsigned c[E / 4 + 1];
-#pragma unroll
-        for (unsigned i = 0; i < E / 4; ++i) c[i] = words[i];
-        c[E / 4] = shift != 0u ? words[E / 4] : 0u;
-        const unsigned char* scale = a.scales + half / 2u + s.column / kBlock8;
-        const unsigned in_block = s.column % kBlock8;
-        const float near = step8(scale[0]), far = in_block + E > kBlock8 ? step8(scale[1]) : near;
-        unsigned dy[4];
-        if constexpr (kAct != Activation::None)
-            load_any<T, E>(a.in + (long long)s.row * a.stride + (long long)(s.column * (unsigned)sizeof(T)), E, dy);
-        float2 f[E / 2];
-#pragma unroll
-        for (unsigned i = 0; i < E / 4; ++i) {
-            const unsigned w = __funnelshift_r(c[i], c[i + 1], shift);
-            f[2 * i] = make_float2(decode8<0>(w, in_block + 4u * i < kBlock8 ? near : far), decode8<1>(w, in_block + 4u * i + 1u < kBlock8 ? near : far));
-            f[2 * i + 1] = make_float2(decode8<2>(w, in_block + 4u * i + 2u < kBlock8 ? near : far), decode8<3>(w, in_block + 4u * i + 3u < kBlock8 ? near : far));
-        }
-        if constexpr (kAct != Activation::None) {
-#pragma unroll
-            for (unsigned i = 0; i < E / 2; ++i) f[i] = through<kAct>(f[i], pair_in<T>(dy, i));
-        }
-        store_granule<T>(a.out + e * sizeof(T), f);
+        for (int e = 0; e < 8; ++e) x.set(e, through<kAct>(x.pair(e), dy.pair(e)));
     }
-    across_rows<T, kAct, true>(a, k0, k0 + kThreads * kGranules, from, origin, m);
+    store_run<T>(a.out, smem_addr(stages) + threadIdx.x / 32u * kStageBytes<T>, first_of(a, h, i), h.count, x.w);
 }
 
 template <typename T, Activation kAct>
@@ -502,20 +423,15 @@ cudaError_t start(const Kept8Call& c, bool keep) {
     a.scales = c.scales;
     const unsigned blocks = (unsigned)((c.columns + kBlock8 - 1) / kBlock8);
     a.columns = (unsigned)c.columns;
-    a.by_columns = Divisor(a.columns);
     a.halves = Divisor(2u * blocks);
     a.items = (unsigned)(c.rows * blocks * 2);
     a.elements = (u64)c.rows * c.columns;
     const std::uintptr_t addresses = reinterpret_cast<std::uintptr_t>(c.in) | reinterpret_cast<std::uintptr_t>(c.out) |
                                      reinterpret_cast<std::uintptr_t>(c.codes) | (std::uintptr_t)(c.rows > 1 ? a.stride : 0);
     constexpr unsigned kPerCta = kThreads * kInFlight<T>;
-    const unsigned ctas = (a.items + kPerCta - 1) / kPerCta;
     if (c.columns % kBlock8 == 0 && addresses % 32 == 0)
-        return launch_dependent<Kept8Args>(keep ? keep8_kernel<T, kAct> : read8_kernel<T, kAct>, ctas, kThreads, 0, c.stream, a);
-    if (keep) return launch_dependent<Kept8Args>(keep8_any_kernel<T, kAct>, ctas, kThreads, 0, c.stream, a);
-    constexpr unsigned kElements = kThreads * kGranules * kGranule<T>;
-    const u64 granules = (a.elements + kGranule<T> + kElements - 1) / kElements;  // one more for an output that is not aligned
-    return launch_dependent<Kept8Args>(read8_any_kernel<T, kAct>, (unsigned)granules, kThreads, 0, c.stream, a);
+        return launch_dependent<Kept8Args>(keep ? keep8_kernel<T, kAct> : read8_kernel<T, kAct>, (a.items + kPerCta - 1) / kPerCta, kThreads, 0, c.stream, a);
+    return launch_dependent<Kept8Args>(keep ? keep8_any_kernel<T, kAct> : read8_any_kernel<T, kAct>, (a.items + kThreads - 1) / kThreads, kThreads, 0, c.stream, a);
 }
 
 template <typename T>
