@@ -608,7 +608,8 @@ struct LayOutArgs {
     const char* dy;
     long long stride;  // bytes
     char* out;
-    unsigned tokens, outputs, pitch;
+    unsigned tokens, outputs;
+    Divisor eights;  // of a row
 };
 
 // A thread takes eight outputs of a token.
@@ -616,7 +617,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ LayOutArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned eights = a.pitch / 8u, i = blockIdx.x * 256u + threadIdx.x, token = i / eights, n = (i - token * eights) * 8u;
+    const unsigned eights = a.eights.d, i = blockIdx.x * 256u + threadIdx.x, token = a.eights.divide(i), n = (i - token * eights) * 8u;
     if (token >= a.tokens) return;
     const T* from = reinterpret_cast<const T*>(a.dy + (long long)token * a.stride) + n;
     unsigned words[2 * sizeof(T)];
@@ -775,7 +776,7 @@ void launch(const WeightGradCall& c, const Plan& p) {
         l.out = workspace;
         l.tokens = (unsigned)c.tokens;
         l.outputs = (unsigned)c.outputs;
-        l.pitch = p.pitch;
+        l.eights = Divisor(p.pitch / 8);
         const u64 eights = (u64)c.tokens * (p.pitch / 8), ctas = (eights + 255) / 256;
         B2_REQUIRE(eights < (1ull << 31), "weight_grad8: dy is too large for one call");
         B2_CUDA(launch_dependent<LayOutArgs>(lay_out_kernel<T>, dim3((unsigned)ctas), 256, 0, c.stream, l));
