@@ -78,6 +78,7 @@ struct alignas(64) WeightGradArgs {
     void* out;
     float* pieces;     // [2 * pairs][outputs of a tile][256 features]
     float* bias;       // [tiles + pairs][outputs of a tile], or null
+    void* bias_out;    // or its gradient itself, where no tile is cut: the first tile of features sums all steps
     unsigned* status;  // host memory
     u64 pitch;         // bytes of a token's codes
     bool wide;         // rows of `out` start at multiples of 16 bytes
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                     const unsigned s = n % kStages;
                     ok = __all_sync(0xffffffffu, wait_phase(bar(bars.dy[s]), (n / kStages) & 1u, failed));
                     if (!ok) break;
-                    if (k % a.feature_tiles == turn) {
+                    if (a.bias_out != nullptr ? turn == 0u : k % a.feature_tiles == turn) {
 #pragma unroll
                         for (unsigned b = 0; b < kBlocks; ++b) {
                             const unsigned from = base + s * kDyBytes + b * kOperandBytes + (warp - 2u) * kBlockBytes;
@@ -400,6 +401,17 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                     if (lane == 0) mbar_arrive(bar(bars.empty[s]));
                 }
                 if (!ok) break;
+                if (a.bias_out != nullptr) {
+                    if (turn != 0u) continue;
+                    const unsigned output = (p.tile / a.feature_tiles) * kWidth + rank * kHalf + column;
+#pragma unroll
+                    for (unsigned b = 0; b < kBlocks; ++b) {
+                        T* out = static_cast<T*>(a.bias_out) + output + b * kTile;
+                        if (output + b * kTile < a.outputs) out[0] = Elem<T>::from_f(sum[b].x);
+                        if (output + b * kTile + 1u < a.outputs) out[1] = Elem<T>::from_f(sum[b].y);
+                    }
+                    continue;
+                }
                 float* to = a.bias + (u64)(p.from == 0 ? p.tile : a.feature_tiles * ((a.outputs + kWidth - 1) / kWidth) + share.pair) * kWidth;
 #pragma unroll
                 for (unsigned b = 0; b < kBlocks; ++b) *reinterpret_cast<float2*>(to + b * kTile + rank * kHalf + column) = sum[b];
@@ -648,6 +660,7 @@ struct Plan {
     bool wide = false;
     unsigned parts = 1, width = kTile, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0, group = 1, groups = 1;
     bool copied = false, cut = false;
+    bool direct = false;  // the bias's gradient comes from weight_grad_kernel itself
     std::size_t pieces_at = 0, bias_at = 0, bytes = 0;
 };
 
@@ -741,10 +754,12 @@ Plan plan_of(const WeightGradCall& c) {
     if (left != 0 && p.steps_of_tile < 8 + p.steps / p.groups) p.groups = left;
     if (p.waves == 0) p.pairs = p.groups * p.group;
     for (unsigned i = 1; i < p.groups; ++i) p.cut |= first_step(i, p.steps, p.groups) % p.steps_of_tile != 0;
+    // (A warp sums a step's 64 columns about as fast as the step goes, but no faster: the first tile of features must not hold up a long sum.)
+    p.direct = c.bias_grad != nullptr && !p.cut && (p.feature_tiles == 1 || p.steps_of_tile <= 32);
     const std::size_t copy = p.copied ? (std::size_t)p.parts * c.tokens * p.pitch * 2 : 0;
     p.pieces_at = (copy + 255) / 256 * 256;
     p.bias_at = p.pieces_at + (p.cut ? (std::size_t)2 * p.pairs * p.width * kTile * sizeof(float) : 0);
-    p.bytes = p.bias_at + (c.bias_grad != nullptr ? (tiles + p.pairs) * p.width * sizeof(float) : 0);
+    p.bytes = p.bias_at + (c.bias_grad != nullptr && !p.direct ? (tiles + p.pairs) * p.width * sizeof(float) : 0);
     return p;
 }
 
@@ -800,7 +815,8 @@ void launch(const WeightGradCall& c, const Plan& p) {
     a.scales = c.scales;
     a.out = c.weight_grad;
     a.pieces = reinterpret_cast<float*>(workspace + p.pieces_at);
-    a.bias = c.bias_grad != nullptr ? reinterpret_cast<float*>(workspace + p.bias_at) : nullptr;
+    a.bias_out = p.direct ? c.bias_grad : nullptr;
+    a.bias = c.bias_grad != nullptr && !p.direct ? reinterpret_cast<float*>(workspace + p.bias_at) : nullptr;
     a.status = status_word();
     a.tokens = (unsigned)c.tokens;
     a.inputs = (unsigned)c.inputs;
@@ -833,7 +849,7 @@ void launch(const WeightGradCall& c, const Plan& p) {
     if constexpr (sizeof(T) == 2)
         if (p.wide) kernel = bias ? weight_grad_kernel<T, true, true> : weight_grad_kernel<T, false, true>;
     B2_CUDA(cudaLaunchKernelEx(&config, kernel, a));
-    if (!p.cut && c.bias_grad == nullptr) return;
+    if (!p.cut && (c.bias_grad == nullptr || p.direct)) return;
     FinishArgs f;
     f.out = c.weight_grad;
     f.bias_out = c.bias_grad;
