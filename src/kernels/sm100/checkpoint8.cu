@@ -324,10 +324,10 @@ __device__ __forceinline__ void store_run(char* out, unsigned stage, u64 first, 
         stage2(in_stage(stage, p + 30u), w[7] >> 16);
     }
     __syncwarp();
-    for (unsigned b = lane * 16u; b + 16u <= end; b += 512u) {
+    for (unsigned b = ((off + 15u) & ~15u) + lane * 16u; b + 16u <= end; b += 512u) {
         uint4 v;
         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(in_stage(stage, b)) : "memory");
-        if (b >= off) store16_once(to + b, v);
+        store16_once(to + b, v);
     }
     // The ends: what stands before the first whole 16 bytes, and behind the last.
     const unsigned last = end & ~15u;

@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(1024) sum_kernel(const __grid_constant__ Rotat
     const Side& s = a.side[blockIdx.y];
     const unsigned column = blockIdx.x * 32u + (threadIdx.x & 31u), part = threadIdx.x >> 5;
     if (s.weight_grad == nullptr) return;
-    // (All loads at once: one after another they took 5 of this kernel's 7 us.)
+    // (All loads at once: 295 x 128 sums, 5.6 us; one after another, 7.0.)
     constexpr unsigned kEach = (kHeadGradCtas + 31) / 32;
     float x[kEach], sum = 0.0f;
 #pragma unroll

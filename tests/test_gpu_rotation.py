@@ -99,7 +99,7 @@ def test_views_layouts_and_three_axes():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("d,r", [(128, 102), (128, 72), (64, 22), (72, 22), (76, 38), (30, 14), (64, 0)])
+@pytest.mark.parametrize("d,r", [(128, 102), (128, 72), (64, 22), (72, 22), (76, 38), (30, 14), (64, 0), (30, 0), (76, 0)])
 def test_what_does_not_turn_stays_as_it_is(dtype, interleaved, d, r):
     """To the last bit, whatever stands beside it: infinities, NaN, zeros with signs."""
     x = values((1, 40, 3, d), dtype).cuda()
