@@ -13,7 +13,7 @@
 // both elements of a pair are in one lane and no exchange is needed but the sums over a head. Elements that do not turn are
 // pairs with no angle. V = 8 (two 16-byte accesses of 16-bit types), 4, 2 or 1, as sizes and addresses allow. Halves that do not begin at a multiple of 4
 // would leave V = 1 for most of them; there a lane holds 2V neighbouring elements (Layout::Apart) and finds their partners in shared memory (norm, forward and
-// backward, of 27264 x (8 + 4) x 128 bf16: 102 elements turned 475 -> 179 us; all of them, in halves, 116).
+// backward, of 27264 x (8 + 4) x 128 bf16: 102 elements turned 475 -> 174 us; all of them, in halves, 116).
 //
 // 32768 x (32 + 8) x 128 bf16 turn in 104 us (6.4 TB/s, 0.98 of a copy's rate); with the norm, 16384 x (32 + 8) x 128 take 85 us, and 108 backward, each 0.6 of that
 // rate: there it is instructions, 380 for 16 elements of a lane, two thirds of the slots of 32 warps (64 registers), and 0.57 of 16 warps' (128).
@@ -461,9 +461,9 @@ __device__ __forceinline__ const char* head_in(const RotationArgs& a, const View
     return v.data + (i64)w.b * v.batch + (i64)(w.n - w.b * a.tokens.d) * v.token + (i64)w.h * v.head;
 }
 
-// K: items of a lane. U: rows of a group in flight.
+// K: items of a lane. U: rows of a group in flight. (Apart: 80 registers, because in 64 it spills 130 bytes; forward alone 66 -> 63 us.)
 template <typename T, int V, int K, Layout kLayout, bool kNorm, int U>
-__global__ void __launch_bounds__(kThreads, 4) rotate_kernel(const __grid_constant__ RotationArgs a) {
+__global__ void __launch_bounds__(kThreads, kLayout == Layout::Apart ? 3 : 4) rotate_kernel(const __grid_constant__ RotationArgs a) {
     constexpr int P = kPairs<V>;
     extern __shared__ __align__(16) unsigned char shared[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
