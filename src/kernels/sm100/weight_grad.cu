@@ -26,6 +26,11 @@
 // sums are added to those in memory, rounded, after every 1024 tokens: the error does not grow with the number of tokens as it would (8192 tokens:
 // 7.5e-6 of the result's norm without either, 2.4e-6 with the leading part first).
 //
+// 16-bit types: an instruction cuts each of its 16 products at a quarter, and their sum with the accumulator at the whole, of the last of 24 bits (seen: products of
+// 3/16 of it beside a 1 are lost, 16 of a quarter come through). Of a sum of one sign that takes 1.8e-4 in 65536 tokens and more than fp16's own rounding
+// (4.9e-4) in 200,000. So their sums too are added to those in memory, rounded, but after every 16384 tokens: 4.5e-5 is lost, and at most
+// 512 * 5 * 2^-23 = 3.1e-4, at any length. (65536 x 4096 x 4096 bf16: 1627 -> 1684 us; after every 8192 tokens 1786, and 16384 x 4096 x 4096 would go from 376 to 408.)
+//
 // dY that TMA cannot read (rows or address not at a multiple of 16 bytes) is copied first.
 //
 // 16384 x 4096 x 4096 bf16: 369 us and 18 for the pieces, 1.42 PFLOP/s, 0.87 of what a library product of 16-bit operands reaches in a burst; tensor pipe 0.79 busy.
@@ -66,6 +71,7 @@ constexpr unsigned kFirstTransformWarp = 4, kFirstEpilogueWarp = 12;
 // from the one before it only: whoever waits on a barrier has to have seen every phase of it.)
 constexpr unsigned kGroups = 4, kGroupWarps = 2;
 constexpr unsigned kChunkSteps = 16;  // fp32: steps of each part between two additions to the sums in memory
+constexpr unsigned kLongSteps = 256;  // 16-bit types: steps between two additions to the sums in memory, see below
 constexpr unsigned kMaxPairs = 74;    // 148 SMs
 constexpr unsigned kTurnBytes = 32 * 32 * 4;  // of an epilogue warp: 32 outputs of its 32 features
 // Shared memory, from a multiple of 1024 bytes on: dY of the stages, X^ of the groups, their codes, what the epilogue turns, barriers.
@@ -168,7 +174,7 @@ struct Piece {
     unsigned tile, from, to;  // steps of the tile
     bool whole;               // this pair sums all of the tile
     bool later;               // not the pair's first step of the tile
-    unsigned slot;            // of the sums in memory, where it is not whole
+    unsigned slot;            // of the sums in memory: of a piece, or of a whole tile that is not done (a pair's last piece comes after its whole tiles)
 };
 __device__ __forceinline__ Piece piece_at(const WeightGradArgs& a, const Share& s, unsigned n) {
     const Where w = where_is(a, s, n);
@@ -179,7 +185,7 @@ __device__ __forceinline__ Piece piece_at(const WeightGradArgs& a, const Share& 
     if (n < s.whole) {
         p.whole = true;
         p.later = w.k != 0;
-        p.slot = 0;
+        p.slot = 2u * s.pair + 1u;
     } else {
         const unsigned tile_at = s.begin + (n - s.whole) - w.k;  // in the row of steps
         p.whole = tile_at >= s.begin && tile_at + a.steps_of_tile <= s.end;
@@ -188,10 +194,11 @@ __device__ __forceinline__ Piece piece_at(const WeightGradArgs& a, const Share& 
     }
     return p;
 }
-// The part of a piece that is summed on the tensor cores alone: all of it, or (fp32) sixteen steps of each part of dY.
+// The part of a piece that is summed on the tensor cores alone: fp32: sixteen steps of each part of dY.
 __device__ __forceinline__ Piece segment_at(const WeightGradArgs& a, const Share& s, unsigned n) {
     Piece p = piece_at(a, s, n);
-    if (a.parts > 1) p.to = min(p.to, (p.from / (a.parts * kChunkSteps) + 1u) * (a.parts * kChunkSteps));
+    const unsigned chunk = a.parts > 1 ? a.parts * kChunkSteps : kLongSteps;
+    p.to = min(p.to, (p.from / chunk + 1u) * chunk);
     return p;
 }
 // Which part of dY, and which 64 tokens, step k of a tile takes: sixteen steps of the last part, whose sums are smallest, the same ones of the one before,
@@ -487,7 +494,25 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                 const unsigned there = min(32u, outputs - c);
                 if (!p.whole) {
                     put<float>(f, turn, piece + (u64)c * kTile, kTile, 32u, kTile, p.later);
-                } else if (a.wide) {
+                    continue;
+                }
+                if constexpr (sizeof(T) == 2) {
+                    // A long sum: each lane finds what it left, four outputs of its feature beside those of the next.
+                    float4* sums = reinterpret_cast<float4*>(a.pieces + (u64)p.slot * (kWidth * kTile)) + c / 4u * kTile + in_tile + lane;
+                    if (p.later) {
+                        float4 old[8];
+#pragma unroll
+                        for (unsigned j = 0; j < 8; ++j) old[j] = sums[j * kTile];
+#pragma unroll
+                        for (unsigned j = 0; j < 8; ++j) { f[4 * j] += old[j].x; f[4 * j + 1] += old[j].y; f[4 * j + 2] += old[j].z; f[4 * j + 3] += old[j].w; }
+                    }
+                    if (p.to != a.steps_of_tile) {
+#pragma unroll
+                        for (unsigned j = 0; j < 8; ++j) sums[j * kTile] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                        continue;
+                    }
+                }
+                if (a.wide) {
                     put<T>(f, turn, static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature, a.inputs, there, a.inputs - feature, p.later);
                 } else if (feature + lane < a.inputs) {
                     T* out = static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature + lane;
@@ -663,6 +688,7 @@ struct Plan {
     bool wide = false;
     unsigned parts = 1, width = kTile, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0, group = 1, groups = 1;
     bool copied = false, cut = false;
+    bool summed = false;  // sums in memory: pieces, or whole tiles of long sums
     bool direct = false;  // the bias's gradient comes from weight_grad_kernel itself
     std::size_t pieces_at = 0, bias_at = 0, bytes = 0;
 };
@@ -761,7 +787,8 @@ Plan plan_of(const WeightGradCall& c) {
     p.direct = c.bias_grad != nullptr && !p.cut && (p.feature_tiles == 1 || p.steps_of_tile <= 32);
     const std::size_t copy = p.copied ? (std::size_t)p.parts * c.tokens * p.pitch * 2 : 0;
     p.pieces_at = (copy + 255) / 256 * 256;
-    p.bias_at = p.pieces_at + (p.cut ? (std::size_t)2 * p.pairs * p.width * kTile * sizeof(float) : 0);
+    p.summed = p.cut || (p.parts == 1 && p.steps_of_tile > kLongSteps);
+    p.bias_at = p.pieces_at + (p.summed ? (std::size_t)2 * p.pairs * p.width * kTile * sizeof(float) : 0);
     p.bytes = p.bias_at + (c.bias_grad != nullptr && !p.direct ? (tiles + p.pairs) * p.width * sizeof(float) : 0);
     return p;
 }
