@@ -44,3 +44,19 @@ def test_long_sums_of_one_sign(dtype, tokens, inputs, outputs):
     assert (error.abs() <= half + sums).all()
     # What all results have in common: no more than that half, and what is left of the mean of so many roundings.
     assert error.mean().abs() <= sums / 2 + 5 * half / 3 ** 0.5 / outputs ** 0.5
+
+
+# Few features, so that one tile sums every step, and many; one tile, cut, and as many as stay whole; parts of a chunk and of a step at the end.
+@pytest.mark.parametrize("sign", ["one", "both"])
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1025, 32, 8), (8192, 768, 2304), (26001, 700, 500), (200003, 64, 64), (70000, 32, 9000), (500009, 300, 130)])
+def test_bias_of_full_precision(tokens, inputs, outputs, sign):
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    dy = torch.rand(tokens, outputs, device="cuda", generator=gen) + 0.5
+    if sign == "both":
+        dy *= torch.randint(0, 2, dy.shape, device="cuda", generator=gen) * 2 - 1
+    x = torch.ones(tokens, inputs, device="cuda")
+    _, db = ops.weight_grad8(dy, ops.pack8(x), bias=True)
+    want, most = (sum(t[i:i + (1 << 16)].double().sum(0) for i in range(0, tokens, 1 << 16)) for t in (dy, dy.abs()))
+    # Steps of 64 tokens: 20 roundings, of each of dY's three parts; what comes behind them is added exactly. Then shares of at most 36 tiles and
+    # pairs, eight of them in one row, and a rounding.
+    assert ((db.double() - want).abs() <= (20 + 20) * 2.0 ** -24 * most).all()
