@@ -48,6 +48,10 @@ typedef struct b2_weight_grad {
 } b2_weight_grad;
 int b2_weight_grad8_workspace(const b2_weight_grad* call, size_t* bytes);
 int b2_weight_grad8(const b2_weight_grad* call, void* stream);
+/* Every wait inside the kernel is bounded, by two seconds or `wait_ns`. Where one runs out, the gradients that depend on it are NaN (in a replayed graph
+ * too), no other call is touched, and the check below says so once: 1, for calls on `device` that are done. */
+int b2_weight_grad8_within(const b2_weight_grad* call, unsigned long long wait_ns, void* stream);
+int b2_train_check_async_error(int device);
 
 /* Queries and keys [batch][tokens][heads][dim], the last axis without gaps. The first `rotated` elements of a head turn in pairs, (i, i + rotated/2) or with
  * `interleaved` (2i, 2i+1), by position * frequencies[i] radians, and are multiplied with `magnitude`. dim and rotated are even, dim at most 256.

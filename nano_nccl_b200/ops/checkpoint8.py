@@ -16,7 +16,7 @@ been run and their graphs dropped, as for any torch module.
 """
 import torch
 
-from .._lib import load_native_calls
+from .._lib import check, load, load_native_calls
 
 _APPROXIMATIONS = {"none": False, "tanh": True}
 
@@ -84,3 +84,10 @@ def linear8(x, weight, bias=None):
         with torch.autocast("cuda", enabled=False):
             return linear8(x, weight, bias)
     return load_native_calls().linear8(x, weight, bias)
+
+
+def check_async_error(device=None):
+    """Raises B200CclError if a bounded wait inside a weight gradient on ``device`` (default: the current one) ran out since this was last called.
+    Such gradients are NaN, so a loss scaler sees them too. Synchronize first: only calls that are done are known."""
+    index = torch.cuda.current_device() if device is None else torch.device(device).index if not isinstance(device, int) else device
+    check(load().b2_train_check_async_error(torch.cuda.current_device() if index is None else index))

@@ -187,9 +187,12 @@ int b2_weight_grad8_workspace(const b2_weight_grad* call, size_t* bytes) {
     });
 }
 
-int b2_weight_grad8(const b2_weight_grad* call, void* stream) {
+int b2_weight_grad8(const b2_weight_grad* call, void* stream) { return b2_weight_grad8_within(call, kernels::WeightGradCall().wait_ns, stream); }
+
+int b2_weight_grad8_within(const b2_weight_grad* call, unsigned long long wait_ns, void* stream) {
     return guarded("weight_grad8", [&] {
-        const kernels::WeightGradCall c = weight_grad_of(call, stream);
+        kernels::WeightGradCall c = weight_grad_of(call, stream);
+        c.wait_ns = wait_ns;
         if (c.outputs != 0 && c.inputs != 0) {
             const std::size_t bytes = dtype_size(c.dtype);
             B2_REQUIRE(c.weight_grad != nullptr, "weight_grad must be non-null");
@@ -201,6 +204,13 @@ int b2_weight_grad8(const b2_weight_grad* call, void* stream) {
             }
         }
         kernels::launch_weight_grad(c);
+    });
+}
+
+int b2_train_check_async_error(int device) {
+    return guarded("weight_grad8", [&] {
+        if (kernels::weight_grad_failed(device))
+            throw std::runtime_error("a wait inside a call on device " + std::to_string(device) + " ran out; its gradients are NaN");
     });
 }
 

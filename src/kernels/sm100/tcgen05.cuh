@@ -49,18 +49,22 @@ __device__ __forceinline__ bool phase_over(unsigned bar, unsigned parity) {
     }
     return done != 0u;
 }
-// Waits for the phase of parity `parity`, for two seconds at most; false then, and in every later wait of the CTA (`failed`, shared).
+// A word at this place in CTA `rank` of the cluster.
+__device__ __forceinline__ void store_word_at(unsigned where, unsigned rank, unsigned v) {
+    asm volatile("{\n .reg .b32 remote;\n mapa.shared::cluster.u32 remote, %0, %1;\n st.shared::cluster.u32 [remote], %2;\n}\n" ::"r"(where), "r"(rank), "r"(v) : "memory");
+}
+// Waits for the phase of parity `parity`, for `limit` ns (and a few polls) at most; false then, and in every later wait of the CTA (`failed`, shared).
 template <bool kCluster = false>
-__device__ __forceinline__ bool wait_phase(unsigned bar, unsigned parity, volatile unsigned* failed) {
+__device__ __forceinline__ bool wait_phase(unsigned bar, unsigned parity, volatile unsigned* failed, unsigned long long limit) {
     if (phase_over<kCluster>(bar, parity)) return true;
     unsigned long long t0 = 0;
     for (unsigned polls = 1;; ++polls) {
         if (phase_over<kCluster>(bar, parity)) return true;
-        if ((polls & 63u) != 0u) continue;
+        if ((polls & 15u) != 0u) continue;
         const unsigned long long now = global_timer_ns();
         if (t0 == 0) t0 = now;
         if (*failed != 0u) return false;
-        if (now - t0 > 2000000000ull) {
+        if (now - t0 >= limit) {
             *failed = 1u;
             return false;
         }

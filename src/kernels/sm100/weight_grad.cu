@@ -90,6 +90,7 @@ struct alignas(64) WeightGradArgs {
     float* bias;       // [tiles + pairs][outputs of a tile], or null
     void* bias_out;    // or its gradient itself, where no tile is cut: the first tile of features sums all steps
     unsigned* status;  // host memory
+    u64 wait_ns;       // limit of a wait
     u64 pitch;         // bytes of a token's codes
     bool wide;         // rows of `out` start at multiples of 16 bytes
     unsigned tokens, inputs, outputs;
@@ -127,7 +128,7 @@ struct Barriers {
     u64 x_empty[kGroups];  // it has been read
     u64 sums[2];           // accumulators are complete
     u64 sums_free[2];      // first CTA: both CTAs have written theirs out
-    u64 drained;           // first CTA, after a failure
+    u64 drained;           // all products are done
     unsigned tmem;
     unsigned failed;
 };
@@ -265,6 +266,31 @@ __device__ __forceinline__ void put(const float (&f)[32], unsigned turn, T* to, 
     __syncwarp();
 }
 
+// After a wait that ran out: all that this CTA's pair was to write is NaN (its own half of the features and of the bias), so that whoever reads it sees it.
+template <typename T, bool kBias, unsigned kWidth>
+__device__ __noinline__ void spoil(const WeightGradArgs& a, const Share& share, unsigned rank) {
+    const float nan = __uint_as_float(0x7fffffffu);
+    const unsigned column = threadIdx.x % kHalf, row0 = threadIdx.x / kHalf;
+    constexpr unsigned kRows = kThreads / kHalf;
+    for (unsigned n = 0; n < share.all;) {
+        const Piece p = piece_at(a, share, n);
+        const unsigned feature = (p.tile % a.feature_tiles) * kTile + rank * kHalf + column, output0 = (p.tile / a.feature_tiles) * kWidth;
+        for (unsigned r = row0; r < kWidth; r += kRows) {
+            if (!p.whole) a.pieces[((u64)p.slot * kWidth + r) * kTile + rank * kHalf + column] = nan;
+            else if (feature < a.inputs && output0 + r < a.outputs) static_cast<T*>(a.out)[(u64)(output0 + r) * a.inputs + feature] = Elem<T>::from_f(nan);
+        }
+        if constexpr (kBias) {
+            for (unsigned b = row0; b < kWidth / kTile; b += kRows) {
+                const unsigned output = b * kTile + rank * kHalf + column;
+                if (a.bias_out == nullptr)
+                    a.bias[(u64)(p.from == 0 ? p.tile : a.feature_tiles * ((a.outputs + kWidth - 1) / kWidth) + share.pair) * kWidth + output] = nan;
+                else if (p.tile % a.feature_tiles == 0 && output0 + output < a.outputs) static_cast<T*>(a.bias_out)[output0 + output] = Elem<T>::from_f(nan);
+            }
+        }
+        n += p.to - p.from;
+    }
+}
+
 // T: type of dY and the gradients. kBias: also columns of dY. kWide: tiles of 512 outputs (16-bit types).
 template <typename T, bool kBias, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_constant__ WeightGradArgs a) {
@@ -326,12 +352,12 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
                     const unsigned s = n % kStages, group = n % kGroups;
                     const Spot spot = spot_of(a, k);
-                    ok = wait_phase(bar(bars.codes_empty[group]), ((n / kGroups) & 1u) ^ 1u, failed);
+                    ok = wait_phase(bar(bars.codes_empty[group]), ((n / kGroups) & 1u) ^ 1u, failed, a.wait_ns);
                     if (!ok) break;
                     mbar_arrive_expect_tx(&bars.codes[group], kCodeBytes);
                     tma_load_box(base + kAtCodes + group * kCodeBytes, &a.codes, feature, (int)(spot.step * kStep), 0, bar(bars.codes[group]));
                     ++asked;
-                    ok = wait_phase(bar(bars.empty[s]), ((n / kStages) & 1u) ^ 1u, failed);
+                    ok = wait_phase(bar(bars.empty[s]), ((n / kStages) & 1u) ^ 1u, failed, a.wait_ns);
                     if (!ok) break;
                     mbar_arrive_expect_tx(&bars.dy[s], kDyBytes);
 #pragma unroll
@@ -342,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             }
             // Stages have been given back, and after a failure copies have landed, before the CTA ends.
             for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i) {
-                if (ok) wait_phase(bar(bars.empty[i % kStages]), (i / kStages) & 1u, failed);
+                if (ok) wait_phase(bar(bars.empty[i % kStages]), (i / kStages) & 1u, failed, a.wait_ns);
                 for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.dy[i % kStages]), (i / kStages) & 1u); ++polls) {}
             }
             for (unsigned i = asked > kGroups ? asked - kGroups : 0; i < asked; ++i)
@@ -356,13 +382,13 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             for (; n < share.all && ok; ++pieces) {
                 const Piece p = segment_at(a, share, n);
                 const unsigned buffer = pieces % kBuffers;
-                ok = wait_phase<true>(bar(bars.sums_free[buffer]), ((pieces / kBuffers) & 1u) ^ 1u, failed);
+                ok = wait_phase<true>(bar(bars.sums_free[buffer]), ((pieces / kBuffers) & 1u) ^ 1u, failed, a.wait_ns);
                 if (!ok) break;
                 tcgen05_fence_after();
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
                     const unsigned s = n % kStages, parity = (n / kStages) & 1u, group = n % kGroups;
-                    ok = wait_phase(bar(bars.dy[s]), parity, failed) && wait_phase<true>(bar(bars.dy_other[s]), parity, failed) &&
-                         wait_phase<true>(bar(bars.x[group]), (n / kGroups) & 1u, failed);
+                    ok = wait_phase(bar(bars.dy[s]), parity, failed, a.wait_ns) && wait_phase<true>(bar(bars.dy_other[s]), parity, failed, a.wait_ns) &&
+                         wait_phase<true>(bar(bars.x[group]), (n / kGroups) & 1u, failed, a.wait_ns);
                     if (!ok) break;
                     tcgen05_fence_after();
                     const std::uint64_t x = operand_by_rows(base + kAtX + group * kOperandBytes, kBlockBytes);
@@ -379,15 +405,16 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                 if (!ok) break;
                 commit_pair(bar(bars.sums[buffer]));
             }
-            if (!ok) {  // products under way read shared memory of both CTAs
-                commit_pair(bar(bars.drained));
-                for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
-            }
+            // Products under way read shared memory and write tensor memory of both CTAs. Where a wait ran out, nobody else may be waiting for them.
+            commit_pair(bar(bars.drained));
+            for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
         } else if (lane == 0) {
             for (unsigned n = 0; n < share.all; ++n) {
-                if (!wait_phase(bar(bars.dy[n % kStages]), (n / kStages) & 1u, failed)) break;
+                if (!wait_phase(bar(bars.dy[n % kStages]), (n / kStages) & 1u, failed, a.wait_ns)) break;
                 mbar_arrive_at(bar(bars.dy_other[n % kStages]), 0);
             }
+            if (!wait_phase(bar(bars.drained), 0, failed, a.wait_ns))
+                for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
         }
     } else if (warp < kFirstTransformWarp) {
         if constexpr (kBias) {
@@ -402,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                 for (unsigned b = 0; b < kBlocks; ++b) sum[b] = low[b] = make_float2(0.0f, 0.0f);
                 for (unsigned k = p.from; k < p.to; ++k, ++n) {
                     const unsigned s = n % kStages;
-                    ok = __all_sync(0xffffffffu, wait_phase(bar(bars.dy[s]), (n / kStages) & 1u, failed));
+                    ok = __all_sync(0xffffffffu, wait_phase(bar(bars.dy[s]), (n / kStages) & 1u, failed, a.wait_ns));
                     if (!ok) break;
                     if (a.bias_out != nullptr ? turn == 0u : k % a.feature_tiles == turn) {
 #pragma unroll
@@ -474,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         unsigned n = group;
         for (; n < share.all; n += kGroups) {
             const unsigned parity = (n / kGroups) & 1u;
-            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.codes[group]), parity, failed) && wait_phase(bar(bars.x_empty[group]), parity ^ 1u, failed)))
+            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.codes[group]), parity, failed, a.wait_ns) && wait_phase(bar(bars.x_empty[group]), parity ^ 1u, failed, a.wait_ns)))
                 break;
 #pragma unroll
             for (unsigned u = 0; u < 8; ++u) {
@@ -494,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             if (n + kGroups < share.all) load_scales(n + kGroups);  // (before the fence, the fence would wait for them)
         }
         // The arrival that gives the operand back comes before the CTA ends.
-        if (n >= share.all && n != group) wait_phase(bar(bars.x_empty[group]), (n / kGroups - 1u) & 1u, failed);
+        if (n >= share.all && n != group) wait_phase(bar(bars.x_empty[group]), (n / kGroups - 1u) & 1u, failed, a.wait_ns);
     } else {
         const unsigned quarter = warp & 3u;  // lanes of tensor memory that this warp reaches
         const unsigned in_tile = rank * kHalf + quarter * 32u;
@@ -503,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         for (; n < share.all; ++pieces) {
             const Piece p = segment_at(a, share, n);
             const unsigned buffer = pieces % kBuffers;
-            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.sums[buffer]), (pieces / kBuffers) & 1u, failed))) break;
+            if (!__all_sync(0xffffffffu, wait_phase(bar(bars.sums[buffer]), (pieces / kBuffers) & 1u, failed, a.wait_ns))) break;
             tcgen05_fence_after();
             const unsigned feature = (p.tile % a.feature_tiles) * kTile + in_tile;
             const unsigned output0 = (p.tile / a.feature_tiles) * kWidth;
@@ -554,13 +581,21 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0 && *failed != 0u) *static_cast<volatile unsigned*>(a.status) = 1u;
+    if (threadIdx.x == 0 && *failed != 0u) {
+        *static_cast<volatile unsigned*>(a.status) = 1u;
+        store_word_at(smem_addr(&bars.failed), rank ^ 1u, 1u);
+    }
     __syncwarp();
     tcgen05_fence_before();
     cluster_sync();  // nothing of this CTA is read or arrived at by the other any more
     tcgen05_fence_after();
     __syncwarp();
     if (warp == 1) tmem_free_pair(tmem, 2 * kTile);
+    if (*failed != 0u) {
+        spoil<T, kBias, kWidth>(a, share, rank);
+        if (rank == 1 && threadIdx.x == 0)  // (the last arrival from the first CTA)
+            for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
+    }
 }
 
 // Adds the pieces of cut tiles, and the bias's. kRows: rows of a thread, four outputs of a CTA for each. One where there are few tiles, whose
@@ -815,20 +850,23 @@ Plan plan_of(const WeightGradCall& c) {
     return p;
 }
 
-// A word of host memory that a kernel whose wait ran out writes to.
-unsigned* status_word() {
-    static unsigned* word = [] {
+// A word of host memory for each device, that a kernel whose wait ran out writes to.
+constexpr int kDevices = 64;
+std::atomic<unsigned*> status_words{nullptr};
+unsigned* status_word(int device) {
+    static unsigned* words = [] {
         // (Allocating is allowed beside a capture: nothing of it belongs to the graph.)
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
         B2_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
         void* p = nullptr;
-        const cudaError_t st = cudaHostAlloc(&p, sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable);
+        const cudaError_t st = cudaHostAlloc(&p, kDevices * sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable);
         cudaThreadExchangeStreamCaptureMode(&mode);
         B2_CUDA(st);
-        *static_cast<unsigned*>(p) = 0;
+        std::fill_n(static_cast<unsigned*>(p), kDevices, 0u);
+        status_words.store(static_cast<unsigned*>(p));
         return static_cast<unsigned*>(p);
     }();
-    return word;
+    return words + device % kDevices;
 }
 
 template <typename T>
@@ -869,7 +907,8 @@ void launch(const WeightGradCall& c, const Plan& p) {
     a.pieces = reinterpret_cast<float*>(workspace + p.pieces_at);
     a.bias_out = p.direct ? c.bias_grad : nullptr;
     a.bias = c.bias_grad != nullptr && !p.direct ? reinterpret_cast<float*>(workspace + p.bias_at) : nullptr;
-    a.status = status_word();
+    a.status = status_word(current_device());
+    a.wait_ns = c.wait_ns;
     a.tokens = (unsigned)c.tokens;
     a.inputs = (unsigned)c.inputs;
     a.outputs = (unsigned)c.outputs;
@@ -938,8 +977,6 @@ void launch_weight_grad(const WeightGradCall& c) {
         if (c.bias_grad != nullptr) B2_CUDA(cudaMemsetAsync(c.bias_grad, 0, c.outputs * bytes, c.stream));
         return;
     }
-    if (__atomic_exchange_n(status_word(), 0u, __ATOMIC_RELAXED) != 0u)
-        throw std::runtime_error("weight_grad8: a wait inside an earlier call ran out; that call's gradients are not valid");
     const Plan p = plan_of(c);
     B2_REQUIRE(p.bytes == 0 || c.workspace != nullptr, "the workspace must be non-null");
     switch (c.dtype) {
@@ -947,6 +984,12 @@ void launch_weight_grad(const WeightGradCall& c) {
         case DType::Float16: return launch<__half>(c, p);
         case DType::BFloat16: return launch<__nv_bfloat16>(c, p);
     }
+}
+
+bool weight_grad_failed(int device) {
+    B2_REQUIRE(device >= 0, "no such device");
+    unsigned* words = status_words.load();  // (null before the first call of all)
+    return words != nullptr && __atomic_exchange_n(words + device % kDevices, 0u, __ATOMIC_RELAXED) != 0u;
 }
 
 }  // namespace b200ccl::kernels

@@ -19,13 +19,16 @@ struct WeightGradCall {
     void* weight_grad = nullptr;  // [outputs, inputs]
     void* bias_grad = nullptr;    // [outputs], or null
     void* workspace = nullptr;    // weight_grad_workspace() bytes, at a multiple of 256
+    unsigned long long wait_ns = 2000000000ull;  // limit of each wait inside the kernel
     cudaStream_t stream = nullptr;
 };
 
 // Scratch of one call, on the current device.
 std::size_t weight_grad_workspace(const WeightGradCall& call);
-// weight_grad[n][k] = sum over tokens of dy[t][n] * x^[t][k], bias_grad[n] = sum of dy[t][n]. Throws std::runtime_error on a failed launch, and where
-// a wait inside an earlier call ran out.
+// weight_grad[n][k] = sum over tokens of dy[t][n] * x^[t][k], bias_grad[n] = sum of dy[t][n]. Throws std::runtime_error on a failed launch. Where a wait
+// inside the kernel runs out, what depends on it is NaN.
 void launch_weight_grad(const WeightGradCall& call);
+// Whether that happened on `device` since this was last asked.
+bool weight_grad_failed(int device);
 
 }  // namespace b200ccl::kernels
