@@ -66,7 +66,7 @@ def weight_grad8(dy, packed, bias=False):
 
     ``dy``: [..., outputs], ``packed``: of [..., inputs] with the same leading axes and the same dtype. Sums over all leading axes are held in
     32 bits and rounded once to that dtype (float32: products of full 24-bit numbers); the tensor cores' additions cut instead of rounding, which in
-    16-bit types takes 5e-5 of a long sum of one sign, 3e-4 at most, however long it is. Results do not depend on timing."""
+    16-bit types takes 7e-5 of a long sum of one sign, 3e-4 at most, however long it is. Results do not depend on timing."""
     _packed("packed", packed)
     if isinstance(dy, torch.Tensor):
         if dy.dtype != packed.dtype:

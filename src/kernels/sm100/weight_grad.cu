@@ -29,7 +29,7 @@
 //
 // 16-bit types: an instruction cuts each of its 16 products at a quarter, and their sum with the accumulator at the whole, of the last of 24 bits (seen: products of
 // 3/16 of it beside a 1 are lost, 16 of a quarter come through). Of a sum of one sign that takes 1.8e-4 in 65536 tokens and more than fp16's own rounding
-// (4.9e-4) in 200,000. So their sums too are added to those in memory, rounded, but after every 16384 tokens: 4.5e-5 is lost, and at most
+// (4.9e-4) in 200,000. So their sums too are added to those in memory, rounded, but after every 16384 tokens: 7e-5 is lost, and at most
 // 512 * 5 * 2^-23 = 3.1e-4, at any length. (65536 x 4096 x 4096 bf16: 1627 -> 1684 us; after every 8192 tokens 1786, and 16384 x 4096 x 4096 would go from 376 to 408.)
 //
 // dY that TMA cannot read (rows or address not at a multiple of 16 bytes) is copied first.
