@@ -109,12 +109,28 @@ bool truth(PyObject* obj) {
     return v != 0;
 }
 
-// The C interface, without the GIL where this thread has it.
+// Gives the GIL away where this thread has it, until the end of the block, by an exception too: a tensor without memory throws when asked for it.
+class WithoutGil {
+public:
+    WithoutGil() : held_(PyGILState_Check() ? PyEval_SaveThread() : nullptr) {}
+    ~WithoutGil() {
+        if (held_ != nullptr) PyEval_RestoreThread(held_);
+    }
+    WithoutGil(const WithoutGil&) = delete;
+    WithoutGil& operator=(const WithoutGil&) = delete;
+
+private:
+    PyThreadState* held_;
+};
+
+// The C interface, without the GIL.
 template <typename F>
 void call(F&& f) {
-    PyThreadState* held = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
-    const int rc = f();
-    if (held != nullptr) PyEval_RestoreThread(held);
+    int rc;
+    {
+        const WithoutGil gil;
+        rc = f();
+    }
     if (rc == 2) throw Refused(g.last_error());
     if (rc != 0) throw Failed(g.last_error());
 }
