@@ -77,6 +77,7 @@ int dtype_code(const char* what, const at::Tensor& t) {
 const at::Tensor& on_gpu(const char* what, const at::Tensor& t) {
     if (!t.is_cuda() || t.layout() != at::kStrided) refuse(std::string(what) + " must be a dense CUDA tensor");
     if (t.is_neg()) refuse(std::string(what) + " is a view that stands for its negative: resolve_neg() makes a tensor of it");
+    if (t._fw_grad(/*level=*/0).defined()) refuse(std::string(what) + " has a tangent: these operators have no forward-mode derivative");
     return t;
 }
 const at::Tensor& tensor_of(const char* what, PyObject* obj) {
@@ -95,7 +96,14 @@ void same_dtype(const char* what, const at::Tensor& t, const at::Tensor& first) 
         refuse(std::string(what) + " has dtype " + c10::toString(t.scalar_type()) + ", expected " + c10::toString(first.scalar_type()));
 }
 
+// What a call has no gradient of would come out of a backward pass as if it had no influence.
+void no_gradient_of(const char* what, const at::Tensor& t) {
+    if ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined())
+        refuse(std::string("a gradient is wanted of ") + what + ", and none is made of it");
+}
+
 double number(const char* what, PyObject* obj) {
+    if (THPVariable_Check(obj)) no_gradient_of(what, THPVariable_Unpack(obj));
     const double v = PyFloat_AsDouble(obj);
     if (v == -1.0 && PyErr_Occurred()) {
         PyErr_Clear();
@@ -266,11 +274,6 @@ variable_list in_backward(const char* what, F&& f) {
     return grads;
 }
 
-// What a call has no gradient of would come out of a backward pass as if it had no influence.
-void no_gradient_of(const char* what, const at::Tensor& t) {
-    if (at::GradMode::is_enabled() && t.requires_grad()) refuse(std::string(what) + " require a gradient, and none is made for them");
-}
-
 bool wants_gradient(std::initializer_list<const at::Tensor*> tensors) {
     if (!at::GradMode::is_enabled()) return false;
     for (const at::Tensor* t : tensors)
@@ -372,7 +375,9 @@ PyObject* weight_grad8(PyObject* const* args, Py_ssize_t nargs) {
     need_arguments(nargs, 4);
     const long long inputs = PyLong_AsLongLong(args[2]);
     if (inputs == -1 && PyErr_Occurred()) throw Raised{};
-    auto [dw, db] = weight_grad(tensor_of("dy", args[0]), tensor_of("the 8-bit form", args[1]), inputs, truth(args[3]));
+    const at::Tensor& dy = tensor_of("dy", args[0]);
+    no_gradient_of("dy", dy);
+    auto [dw, db] = weight_grad(dy, tensor_of("the 8-bit form", args[1]), inputs, truth(args[3]));
     return two(std::move(dw), std::move(db));
 }
 

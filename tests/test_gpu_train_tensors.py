@@ -41,3 +41,40 @@ print("alive", float(ops.gelu8(torch.zeros(1, device="cuda"))))
 def test_tensors_without_memory_of_their_own():
     run = subprocess.run([sys.executable, "-c", WITHOUT_MEMORY], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "alive 0.0" in run.stdout, run.stderr[-2000:] + run.stdout
+
+
+def arguments():
+    x, w, f = torch.randn(6, 2, 64, device="cuda"), torch.ones(64, device="cuda"), ops.rotary_frequencies(64)[0]
+    return x, w, f, torch.arange(6, device="cuda")
+
+
+def test_forward_mode_is_refused():
+    """Not dropped: an output without a tangent is a constant to whoever differentiates further."""
+    x, w, f, p = arguments()
+    kept = ops.pack8(x)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.pack8(dual(x)), lambda: ops.gelu8(dual(x)), lambda: ops.weight_grad8(dual(x), kept), lambda: ops.linear8(dual(x), w[None]),
+                     lambda: ops.linear8(x, dual(w[None])), lambda: ops.linear8(x, w[None], dual(w[:1])), lambda: ops.rotary(dual(x), x, p, f),
+                     lambda: ops.rotary(x, dual(x), p, f), lambda: ops.rotary(x, None, p, dual(f)), lambda: ops.qk_norm_rotary(dual(x), None, w, None, p, f),
+                     lambda: ops.qk_norm_rotary(x, None, dual(w), None, p, f), lambda: ops.gelu8(dual(x).requires_grad_()),
+                     lambda: ops.rotary(x, None, p, f, magnitude=dual(torch.ones((), device="cuda")))):
+            with pytest.raises(ValueError, match="tangent|wanted"):
+                call()
+        # A backward pass of a gradient with a tangent (a product with the Hessian).
+        leaf, weight = x.clone().requires_grad_(), w.clone()[None].requires_grad_()
+        for y, by in ((ops.gelu8(leaf), leaf), (ops.rotary(leaf, None, p, f)[0], leaf), (ops.linear8(leaf, weight), weight)):
+            with pytest.raises(ValueError, match="tangent"):
+                torch.autograd.grad(y, by, dual(torch.ones_like(y)))
+
+
+def test_gradients_that_are_not_made_are_refused():
+    x, w, f, p = arguments()
+    kept = ops.pack8(x)
+    for call in (lambda: ops.weight_grad8(x.clone().requires_grad_(), kept), lambda: ops.rotary(x, None, p, f, magnitude=torch.ones((), requires_grad=True)),
+                 lambda: ops.qk_norm_rotary(x, None, w, None, p, f, eps=torch.ones((), requires_grad=True))):
+        with pytest.raises(ValueError, match="wanted"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(ops.weight_grad8(x.clone().requires_grad_(), kept)[0], ops.weight_grad8(x, kept)[0])
+    assert torch.equal(ops.rotary(x, None, p, f, magnitude=torch.tensor(2.0))[0], ops.rotary(x, None, p, f, magnitude=2.0)[0])
