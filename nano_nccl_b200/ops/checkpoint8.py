@@ -13,6 +13,9 @@ exactly those of the formula at ``x^``. A block that holds an infinity or NaN re
 The kernels are this library's own (CUDA tensors of float32, float16 or bfloat16); calls run on the current stream of the tensors' device.
 A step captured into a CUDA graph is captured with its backward pass and on one stream, after eager steps of the same parameters have
 been run and their graphs dropped, as for any torch module.
+
+Unlike the collectives these are functions and no registered torch operators: reverse-mode gradients are made once, and tracing, fake tensors,
+forward mode, ``torch.func`` and tensors that stand for others are refused. (``torch.compile`` leaves its graph for them.)
 """
 import torch
 

@@ -11,12 +11,14 @@
 #include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cstdint>
@@ -75,6 +77,10 @@ int dtype_code(const char* what, const at::Tensor& t) {
 }
 
 const at::Tensor& on_gpu(const char* what, const at::Tensor& t) {
+    // Fake tensors, subclasses that stand for other tensors, those inside torch.func's transformations.
+    constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
+    if (t.unsafeGetTensorImpl()->is_python_dispatch() || t.key_set().has_any(kWrapped) || !t.has_storage())
+        refuse(std::string(what) + " has no memory of its own: these operators know plain tensors only, and no transformations of them");
     if (!t.is_cuda() || t.layout() != at::kStrided) refuse(std::string(what) + " must be a dense CUDA tensor");
     if (t.is_neg()) refuse(std::string(what) + " is a view that stands for its negative: resolve_neg() makes a tensor of it");
     if (t._fw_grad(/*level=*/0).defined()) refuse(std::string(what) + " has a tangent: these operators have no forward-mode derivative");
@@ -762,6 +768,11 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         return nullptr;
     }
     try {
+        // Whoever records torch's operators would record the allocation of a result, and not the kernel that fills it.
+        using Mode = c10::impl::TorchDispatchModeKey;
+        if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(Mode::PROXY).has_value() ||
+            c10::impl::TorchDispatchModeTLS::get_mode(Mode::FAKE).has_value() || c10::impl::TorchDispatchModeTLS::get_mode(Mode::FUNCTIONAL).has_value())
+            refuse("these operators are no torch operators and cannot be traced");
         return kFunction(args, nargs);
     } catch (const Refused& e) {
         PyErr_SetString(PyExc_ValueError, e.what());

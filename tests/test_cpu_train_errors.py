@@ -18,3 +18,16 @@ def test_asking_for_waits_that_ran_out(lib):
     with pytest.raises(ValueError, match="no such device"):
         ops.check_async_error(-1)
     assert lib.b2_weight_grad8_within(None, ctypes.c_ulonglong(5), None) == 2 and b"null" in lib.b2_last_error()
+
+
+def test_fake_tensors_are_refused(lib):
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        x, f, p = torch.empty(5, 2, 64, device="cuda"), torch.empty(32, dtype=torch.float64, device="cuda"), torch.empty(5, dtype=torch.int64, device="cuda")
+    calls = [lambda: ops.pack8(x), lambda: ops.gelu8(x), lambda: ops.linear8(x, x[0]), lambda: ops.rotary(x, None, p, f), lambda: ops.qk_norm_rotary(x, x, x[0, 0], x[0, 0], p, f)]
+    for call in calls:
+        with pytest.raises(ValueError, match="memory of its own"):
+            call()
+        with mode, pytest.raises(ValueError, match="traced"):
+            call()

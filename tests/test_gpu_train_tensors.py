@@ -4,6 +4,7 @@ import sys
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from nano_nccl_b200 import ops
 
@@ -78,3 +79,56 @@ def test_gradients_that_are_not_made_are_refused():
     with torch.no_grad():
         assert torch.equal(ops.weight_grad8(x.clone().requires_grad_(), kept)[0], ops.weight_grad8(x, kept)[0])
     assert torch.equal(ops.rotary(x, None, p, f, magnitude=torch.tensor(2.0))[0], ops.rotary(x, None, p, f, magnitude=2.0)[0])
+
+
+def every_call(x, w, f, p):
+    kept = ops.pack8(torch.ones(6, 2, 64, device="cuda"))
+    return [lambda x: ops.pack8(x).data, lambda x: ops.unpack8(kept) * x.sum(), lambda x: ops.gelu8(x), lambda x: ops.weight_grad8(x, kept)[0],
+            lambda x: ops.linear8(x, w[None]), lambda x: ops.rotary(x, None, p, f)[0], lambda x: ops.qk_norm_rotary(x, None, w, None, p, f)[0]]
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_tracing_is_refused():
+    """A trace would hold the allocation of a result and not what fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, f, p = arguments()
+    calls = every_call(x, w, f, p)
+    for call in calls:
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, (x,), check_trace=False)
+        with pytest.raises(ValueError, match="traced"):
+            make_fx(call)(x)
+    del calls[1]  # (under a transformation a constant, and right)
+    for call in calls:
+        with pytest.raises(ValueError, match="traced|memory"):
+            torch.func.vmap(call)(torch.stack([x, x]))
+        with pytest.raises(ValueError, match="traced|memory"):
+            torch.func.grad(lambda t: call(t).sum())(x)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_compilation_leaves_its_graph_for_them():
+    x, w, f, p = arguments()
+    calls = every_call(x, w, f, p)
+    compiled = [torch.compile(call, backend="eager") for call in calls]
+    for call, other in zip(calls, compiled):
+        assert torch.equal(call(x), other(x))
+
+
+def test_saved_tensors_may_go_elsewhere_and_be_made_again():
+    """Hooks on what is saved: to the CPU and back, or made again in the backward pass."""
+    x, w, f, p = arguments()
+    x, w, m = x.requires_grad_(), w.requires_grad_(), torch.randn(8, 64, device="cuda", requires_grad=True)
+
+    def step(x, w, m):
+        q, _ = ops.qk_norm_rotary(x, None, w, None, p, f, keep="int8")
+        return ops.gelu8(ops.linear8(ops.rotary(q, None, p, f)[0], m)).square().sum()
+
+    want = torch.autograd.grad(step(x, w, m), (x, w, m))
+    with torch.autograd.graph.save_on_cpu():
+        loss = step(x, w, m)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(loss, (x, w, m))))
+    for reentrant in (False, True):
+        x.grad = w.grad = m.grad = None
+        torch.utils.checkpoint.checkpoint(step, x, w, m, use_reentrant=reentrant).backward()
+        assert all(torch.equal(a, b) for a, b in zip(want, (x.grad, w.grad, m.grad)))
