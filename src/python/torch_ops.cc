@@ -401,7 +401,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
             at::Tensor dx, dw, db;
             if (ctx->needs_input_grad(0)) dx = at::matmul(dy, weight);
             const bool bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
-            if (kept.defined()) std::tie(dw, db) = weight_grad(on_gpu("dy", dy), kept, weight.size(1), bias);
+            if (kept.defined() && (bias || ctx->needs_input_grad(1))) std::tie(dw, db) = weight_grad(on_gpu("dy", dy), kept, weight.size(1), bias);
             else if (bias) db = dy.reshape({-1, weight.size(0)}).sum(0);  // of a frozen weight
             if (!ctx->needs_input_grad(1)) dw = at::Tensor();
             return {dx, dw, db};

@@ -1,0 +1,47 @@
+"""linear8: what its backward pass makes, keeps and says, and autocast."""
+import contextlib
+import ctypes
+
+import pytest
+import torch
+
+import nano_nccl_b200 as nn
+from nano_nccl_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+
+@contextlib.contextmanager
+def replaced(name, prototype, f):
+    """Calls of the operators reach f(original, *arguments) instead of the C interface's `name`."""
+    lib, native = nn.load(), nn.load_native_calls()
+    address = {n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _lib._TRAIN}
+    original = prototype(address[name])
+    fake = prototype(lambda *arguments: f(original, *arguments))
+    native.bind_train(nn.B200CclError, tuple(ctypes.cast(fake, ctypes.c_void_p).value if n == name else address[n] for n in _lib._TRAIN))
+    try:
+        yield
+    finally:
+        native.bind_train(nn.B200CclError, tuple(address[n] for n in _lib._TRAIN))
+
+
+WEIGHT_GRAD = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
+
+
+def test_weight_gradients_are_made_for_who_asks():
+    calls = []
+
+    def count(original, *arguments):
+        calls.append(1)
+        return original(*arguments)
+
+    x, w, b = (torch.randn(s, device="cuda", requires_grad=True) for s in ((40, 64), (32, 64), (32,)))
+    dy = torch.randn(40, 32, device="cuda")
+    with replaced("b2_weight_grad8", WEIGHT_GRAD, count):
+        for wanted, expected in (((x,), 0), ((x, w), 1), ((w,), 1), ((x, w, b), 1)):
+            y = ops.linear8(x, w, b)
+            calls.clear()
+            grads = torch.autograd.grad(y, wanted, dy)
+            assert len(calls) == expected, wanted
+            if wanted[0] is x:
+                assert torch.equal(grads[0], dy @ w)
