@@ -389,8 +389,10 @@ PyObject* weight_grad8(PyObject* const* args, Py_ssize_t nargs) {
 
 struct Linear8 : torch::autograd::Function<Linear8> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias) {
-        ctx->save_for_backward({weight, weight.requires_grad() ? pack(x) : at::Tensor()});
+        // What no gradient asks for is not kept: the weight may change then, as behind torch's own.
+        ctx->save_for_backward({x.requires_grad() ? weight : at::Tensor(), weight.requires_grad() ? pack(x) : at::Tensor()});
         ctx->saved_data["bias"] = bias.has_value();
+        ctx->saved_data["inputs"] = weight.size(1);
         return at::linear(x, weight, bias);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -401,8 +403,8 @@ struct Linear8 : torch::autograd::Function<Linear8> {
             at::Tensor dx, dw, db;
             if (ctx->needs_input_grad(0)) dx = at::matmul(dy, weight);
             const bool bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
-            if (kept.defined() && (bias || ctx->needs_input_grad(1))) std::tie(dw, db) = weight_grad(on_gpu("dy", dy), kept, weight.size(1), bias);
-            else if (bias) db = dy.reshape({-1, weight.size(0)}).sum(0);  // of a frozen weight
+            if (kept.defined() && (bias || ctx->needs_input_grad(1))) std::tie(dw, db) = weight_grad(on_gpu("dy", dy), kept, ctx->saved_data["inputs"].toInt(), bias);
+            else if (bias) db = dy.reshape({-1, dy.size(-1)}).sum(0);  // of a frozen weight
             if (!ctx->needs_input_grad(1)) dw = at::Tensor();
             return {dx, dw, db};
         });

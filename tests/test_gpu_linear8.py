@@ -45,3 +45,19 @@ def test_weight_gradients_are_made_for_who_asks():
             assert len(calls) == expected, wanted
             if wanted[0] is x:
                 assert torch.equal(grads[0], dy @ w)
+
+
+def test_a_weight_that_no_gradient_reads_may_change():
+    """As behind torch's own projection: without a gradient of x, nothing reads the weight again."""
+    for linear in (torch.nn.functional.linear, ops.linear8):
+        x, w, dy = torch.randn(40, 64, device="cuda"), torch.randn(32, 64, device="cuda", requires_grad=True), torch.randn(40, 32, device="cuda")
+        y = linear(x, w)
+        with torch.no_grad():
+            w.mul_(2.0)
+        (dw,) = torch.autograd.grad(y, w, dy)
+        assert torch.allclose(dw, dy.t() @ ops.unpack8(ops.pack8(x)), rtol=0.05, atol=0.5)
+        y = linear(x.requires_grad_(), w)
+        with torch.no_grad():
+            w.mul_(2.0)
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(y, x, dy)
