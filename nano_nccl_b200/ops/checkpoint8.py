@@ -80,12 +80,8 @@ def weight_grad8(dy, packed, bias=False):
 
 
 def linear8(x, weight, bias=None):
-    """``torch.nn.functional.linear(x, weight, bias)``; the weight's gradient reads ``x`` in 8 bits (:func:`weight_grad8`)."""
-    if torch.is_autocast_enabled("cuda"):
-        dtype = torch.get_autocast_dtype("cuda")
-        x, weight, bias = x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype)
-        with torch.autocast("cuda", enabled=False):
-            return linear8(x, weight, bias)
+    """``torch.nn.functional.linear(x, weight, bias)``; the weight's gradient reads ``x`` in 8 bits (:func:`weight_grad8`).
+    Under autocast its arguments are cast as those of ``linear``."""
     return load_native_calls().linear8(x, weight, bias)
 
 

@@ -9,6 +9,7 @@
 #include "b200ccl/train_ops.h"
 
 #include <ATen/Functions.h>
+#include <ATen/autocast_mode.h>
 #include <ATen/core/Tensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -414,8 +415,16 @@ struct Linear8 : torch::autograd::Function<Linear8> {
 // linear8(x, weight, bias or None) -> y
 PyObject* linear8(PyObject* const* args, Py_ssize_t nargs) {
     need_arguments(nargs, 3);
-    const at::Tensor &x = tensor_of("x", args[0]), &weight = tensor_of("weight", args[1]);
-    const at::Tensor bias = maybe_tensor("bias", args[2]);
+    at::Tensor x = tensor_of("x", args[0]), weight = tensor_of("weight", args[1]), bias = maybe_tensor("bias", args[2]);
+    std::optional<c10::impl::ExcludeDispatchKeyGuard> without_autocast;
+    if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+        // By autocast's rules and through its cache: a weight is cast once, and 64-bit tensors are not.
+        const at::ScalarType type = at::autocast::get_autocast_dtype(at::kCUDA);
+        x = at::autocast::cached_cast(type, x, at::kCUDA);
+        weight = at::autocast::cached_cast(type, weight, at::kCUDA);
+        if (bias.defined()) bias = at::autocast::cached_cast(type, bias, at::kCUDA);
+        without_autocast.emplace(c10::DispatchKey::AutocastCUDA);
+    }
     same_place("weight", weight, x);
     same_dtype("weight", weight, x);
     if (x.dim() < 1 || weight.dim() != 2 || x.size(-1) != weight.size(1)) refuse("the input does not go into the weight");

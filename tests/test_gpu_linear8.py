@@ -61,3 +61,20 @@ def test_a_weight_that_no_gradient_reads_may_change():
             w.mul_(2.0)
         with pytest.raises(RuntimeError, match="inplace"):
             torch.autograd.grad(y, x, dy)
+
+
+def test_autocast_casts_as_torch_does():
+    """A weight once in a context; 64-bit tensors, which torch leaves alone, not at all."""
+    x, w, b = (torch.randn(s, device="cuda", requires_grad=True) for s in ((40, 64), (32, 64), (32,)))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        first, second = ops.linear8(x, w, b), ops.linear8(x, w, b)
+        assert first.grad_fn.next_functions[1][0] is second.grad_fn.next_functions[1][0]
+        assert torch.equal(first, torch.nn.functional.linear(x, w, b)) and first.dtype == torch.bfloat16
+        with pytest.raises(ValueError, match="Double"):
+            ops.linear8(x.double(), w.double(), b.double())
+        with torch.autocast("cuda", enabled=False):
+            assert ops.linear8(x, w, b).dtype == torch.float32
+    (first.float().sum() + second.float().sum()).backward()
+    assert torch.equal(b.grad, torch.full_like(b, 80.0)) and w.grad.dtype == x.grad.dtype == torch.float32
+    with torch.autocast("cuda", dtype=torch.float16), torch.no_grad():
+        assert torch.equal(ops.linear8(x, w, b), torch.nn.functional.linear(x, w, b))
