@@ -258,8 +258,8 @@ at::Tensor new_like(const at::Tensor& t) { return at::empty(t.sizes(), t.options
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Gradients, computed by `f`. What f refuses is a ValueError where the backward pass was called; its results have no graph, and say so to
-// whoever differentiates them again.
+// Gradients, computed by `f`. What f refuses is a ValueError where the backward pass was called, what fails a B200CclError, as in a forward pass; its
+// results have no graph, and say so to whoever differentiates them again.
 template <typename F>
 variable_list in_backward(const char* what, F&& f) {
     variable_list grads;
@@ -267,6 +267,12 @@ variable_list in_backward(const char* what, F&& f) {
         grads = f();
     } catch (const Refused& e) {
         TORCH_CHECK_VALUE(false, e.what());
+    } catch (const Failed& e) {
+        const pybind11::gil_scoped_acquire gil;
+        PyErr_SetString(g_error_class, e.what());
+        python_error error;
+        error.persist();
+        throw error;
     }
     if (!at::GradMode::is_enabled()) return grads;
     variable_list marked;

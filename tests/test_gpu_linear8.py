@@ -78,3 +78,21 @@ def test_autocast_casts_as_torch_does():
     assert torch.equal(b.grad, torch.full_like(b, 80.0)) and w.grad.dtype == x.grad.dtype == torch.float32
     with torch.autocast("cuda", dtype=torch.float16), torch.no_grad():
         assert torch.equal(ops.linear8(x, w, b), torch.nn.functional.linear(x, w, b))
+
+
+def test_a_failure_in_a_backward_pass_is_this_library_s_error():
+    """The failing call is a stand-in on the host."""
+    x, w = (torch.randn(s, device="cuda", requires_grad=True) for s in ((40, 64), (32, 64)))
+    dy = torch.randn(40, 32, device="cuda")
+    with replaced("b2_weight_grad8", WEIGHT_GRAD, lambda original, *arguments: 1):
+        with pytest.raises(nn.B200CclError):
+            ops.weight_grad8(dy, ops.pack8(x))
+        for _ in range(2):
+            y = ops.linear8(x, w)
+            with pytest.raises(nn.B200CclError):
+                y.backward(dy)
+    with replaced("b2_weight_grad8", WEIGHT_GRAD, lambda original, *arguments: 2):
+        with pytest.raises(ValueError):
+            ops.linear8(x, w).backward(dy)
+    ops.linear8(x, w).backward(dy)
+    assert torch.equal(w.grad, ops.weight_grad8(dy, ops.pack8(x))[0])
