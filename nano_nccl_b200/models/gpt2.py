@@ -19,6 +19,24 @@ def gpt2_small_shapes(hidden=768, layers=12, vocab=50257, context=1024):
     return shapes
 
 
+class _Linear8(torch.nn.Linear):
+    """A projection whose input is kept in 8 bits."""
+
+    def forward(self, x):
+        return ops.linear8(x, self.weight, self.bias)
+
+
+class _Gelu8(torch.nn.GELU):
+    """GELU whose input is kept in 8 bits."""
+
+    def forward(self, x):
+        return ops.gelu8(x, self.approximate)
+
+
+def _modules(checkpoints):
+    return (torch.nn.Linear, torch.nn.GELU) if checkpoints is None else (_Linear8, _Gelu8)
+
+
 class _Attention(torch.nn.Module):
     """Self-attention whose queries and keys are turned by their positions (``rotary``), after a norm of each head where ``qk_norm`` says so.
     Projections keep their inputs in 8 bits where ``checkpoints`` says so; so do the norms."""
@@ -26,8 +44,9 @@ class _Attention(torch.nn.Module):
     def __init__(self, hidden, heads, rotary, qk_norm, checkpoints):
         super().__init__()
         self.heads, self.rotary, self.checkpoints = heads, rotary, checkpoints
-        self.c_attn = torch.nn.Linear(hidden, 3 * hidden)
-        self.c_proj = torch.nn.Linear(hidden, hidden)
+        linear, _ = _modules(checkpoints)
+        self.c_attn = linear(hidden, 3 * hidden)
+        self.c_proj = linear(hidden, hidden)
         if qk_norm:
             self.q_norm = torch.nn.Parameter(torch.ones(hidden // heads))
             self.k_norm = torch.nn.Parameter(torch.ones(hidden // heads))
@@ -42,38 +61,31 @@ class _Attention(torch.nn.Module):
 
     def forward(self, x):
         b, t, hidden = x.shape
-        q, k, v = (p.view(b, t, self.heads, -1) for p in _linear(x, self.c_attn, self.checkpoints).split(hidden, -1))
+        q, k, v = (p.view(b, t, self.heads, -1) for p in self.c_attn(x).split(hidden, -1))
         positions = torch.arange(t, device=x.device)
         if self.qk_norm:
             q, k = ops.qk_norm_rotary(q, k, self.q_norm, self.k_norm, positions, self.frequencies(x.device), keep=self.checkpoints)
         elif self.rotary:
             q, k = ops.rotary(q, k, positions, self.frequencies(x.device))
         y = torch.nn.functional.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
-        return _linear(y.transpose(1, 2).reshape(b, t, hidden), self.c_proj, self.checkpoints)
-
-
-def _linear(x, layer, checkpoints):
-    return layer(x) if checkpoints is None else ops.linear8(x, layer.weight, layer.bias)
+        return self.c_proj(y.transpose(1, 2).reshape(b, t, hidden))
 
 
 class _Block(torch.nn.Module):
     def __init__(self, hidden, heads, rotary=False, qk_norm=False, checkpoints=None):
         super().__init__()
-        self.checkpoints = checkpoints
+        linear, gelu = _modules(checkpoints)
         self.plain_attention = not rotary and not qk_norm and checkpoints is None
         self.ln_1 = torch.nn.LayerNorm(hidden)
         self.attn = (torch.nn.MultiheadAttention(hidden, heads, batch_first=True) if self.plain_attention
                      else _Attention(hidden, heads, rotary, qk_norm, checkpoints))
         self.ln_2 = torch.nn.LayerNorm(hidden)
-        self.mlp = torch.nn.Sequential(torch.nn.Linear(hidden, 4 * hidden), torch.nn.GELU(), torch.nn.Linear(4 * hidden, hidden))
+        self.mlp = torch.nn.Sequential(linear(hidden, 4 * hidden), gelu(), linear(4 * hidden, hidden))
 
     def forward(self, x):
         h = self.ln_1(x)
         x = x + (self.attn(h, h, h, need_weights=False)[0] if self.plain_attention else self.attn(h))
-        h = self.ln_2(x)
-        if self.checkpoints is None:
-            return x + self.mlp(h)
-        return x + _linear(ops.gelu8(_linear(h, self.mlp[0], self.checkpoints)), self.mlp[2], self.checkpoints)
+        return x + self.mlp(self.ln_2(x))
 
 
 class TinyGPT2(torch.nn.Module):

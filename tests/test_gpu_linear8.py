@@ -4,9 +4,11 @@ import ctypes
 
 import pytest
 import torch
+import torch.nn.utils.parametrize
 
 import nano_nccl_b200 as nn
 from nano_nccl_b200 import _lib, ops
+from nano_nccl_b200.models import TinyGPT2
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +98,23 @@ def test_a_failure_in_a_backward_pass_is_this_library_s_error():
             ops.linear8(x, w).backward(dy)
     ops.linear8(x, w).backward(dy)
     assert torch.equal(w.grad, ops.weight_grad8(dy, ops.pack8(x))[0])
+
+
+def test_hooks_of_a_model_s_modules_are_called():
+    """What is kept for the backward pass does not change which modules a forward pass goes through."""
+    tokens = torch.zeros(1, 4, dtype=torch.long, device="cuda")
+    names = {}
+    for checkpoints in (None, "int8"):
+        model = TinyGPT2(vocab=32, context=8, hidden=32, layers=1, heads=2, positions="rotary", checkpoints=checkpoints).cuda()
+        seen = []
+        for name, module in model.named_modules():
+            module.register_forward_hook(lambda module, inputs, output, name=name: seen.append(name))
+        model(tokens)
+        names[checkpoints] = seen
+        # A hook's result is what goes on, and a weight that is computed is the one that is used.
+        model.blocks[0].mlp[2].register_forward_hook(lambda module, inputs, output: output * 0.0)
+        torch.nn.utils.parametrize.register_parametrization(model.blocks[0].attn.c_proj, "weight", torch.nn.Identity())
+        x = torch.randn(1, 4, 32, device="cuda")
+        block = model.blocks[0]
+        assert torch.equal(block(x), x + block.attn(block.ln_1(x)))
+    assert names[None] == names["int8"] and "blocks.0.mlp.1" in names["int8"]
