@@ -63,11 +63,11 @@ def rotary(q, k, positions, frequencies, layout="half", magnitude=1.0):
     return load_native_calls().rotary(q, k, positions, frequencies, _interleaved(layout), magnitude)
 
 
-def qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, layout="half", magnitude=1.0, eps=1e-6, keep="int8"):
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, layout="half", magnitude=1.0, eps=1e-6, keep=None):
     """(q, k) after the norm of each head, ``x * (mean(x^2) + eps)^(-1/2) * weight``, and the rotation of :func:`rotary`, in one pass.
 
-    ``q_weight`` and ``k_weight``: [dim], of the same dtype. For the backward pass q and k are kept in 8 bits (``keep="int8"``: as in
-    :mod:`.checkpoint8`, a head of a token being one block), or as they are (``keep=None``). Under autocast, weights of another dtype are
+    ``q_weight`` and ``k_weight``: [dim], of the same dtype. For the backward pass q and k are kept as they are, or, with ``keep="int8"``,
+    in 8 bits, as in :mod:`.checkpoint8`, a head of a token being one block: the gradients are then those of the formula at what was kept. Under autocast, weights of another dtype are
     cast to that of q and k."""
     interleaved = _interleaved(layout)
     if keep not in (None, "int8"):

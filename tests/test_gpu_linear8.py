@@ -118,3 +118,10 @@ def test_hooks_of_a_model_s_modules_are_called():
         block = model.blocks[0]
         assert torch.equal(block(x), x + block.attn(block.ln_1(x)))
     assert names[None] == names["int8"] and "blocks.0.mlp.1" in names["int8"]
+
+
+def test_head_norms_keep_8_bits_only_where_they_are_told_to():
+    q, w, dy = (torch.randn(s, device="cuda") for s in ((9, 4, 64), (64,), (9, 4, 64)))
+    q, w, p, f = q.requires_grad_(), w.requires_grad_(), torch.arange(9, device="cuda"), ops.rotary_frequencies(64)[0]
+    given, full, short = (torch.autograd.grad(ops.qk_norm_rotary(q, None, w, None, p, f, **keep)[0], (q, w), dy) for keep in ({}, {"keep": None}, {"keep": "int8"}))
+    assert all(torch.equal(a, b) for a, b in zip(given, full)) and not torch.equal(given[0], short[0])
