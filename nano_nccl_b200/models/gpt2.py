@@ -99,7 +99,9 @@ class TinyGPT2(torch.nn.Module):
             raise ValueError(f"unknown kind of positions '{positions}'")
         if checkpoints not in (None, "int8"):
             raise ValueError(f"unknown kind of checkpoints '{checkpoints}'")
-        if (positions == "rotary" or qk_norm) and (hidden % heads or (hidden // heads) % 2 or hidden // heads > 256):
+        if hidden % heads and (positions == "rotary" or qk_norm or checkpoints is not None):
+            raise ValueError(f"{heads} heads do not make {hidden}")
+        if (positions == "rotary" or qk_norm) and ((hidden // heads) % 2 or hidden // heads > 256):
             raise ValueError(f"{heads} heads of an even size up to 256 do not make {hidden}")
         self.wte = torch.nn.Embedding(vocab, hidden)
         self.wpe = torch.nn.Embedding(context, hidden) if positions == "learned" else None

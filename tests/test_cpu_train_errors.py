@@ -31,3 +31,11 @@ def test_fake_tensors_are_refused(lib):
             call()
         with mode, pytest.raises(ValueError, match="traced"):
             call()
+
+
+def test_a_model_of_heads_that_do_not_fit_is_refused_when_it_is_made():
+    from nano_nccl_b200.models import TinyGPT2
+    for options in ({}, {"checkpoints": "int8"}, {"positions": "rotary"}):
+        with pytest.raises((ValueError, AssertionError)):
+            TinyGPT2(hidden=32, heads=3, **options)
+    TinyGPT2(hidden=32, heads=4, checkpoints="int8")
