@@ -60,3 +60,53 @@ def test_bias_of_full_precision(tokens, inputs, outputs, sign):
     # Steps of 64 tokens: 20 roundings, of each of dY's three parts; what comes behind them is added exactly. Then shares of at most 36 tiles and
     # pairs, eight of them in one row, and a rounding.
     assert ((db.double() - want).abs() <= (20 + 20) * 2.0 ** -24 * most).all()
+
+
+# Tiles of 256 and 512 outputs, whole and cut, side by side and not, one and several waves, few and many tokens.
+PLANS = [(26001, 700, 500), (20000, 1100, 260), (9000, 513, 4700), (16000, 64, 64), (12007, 29, 2227), (15126, 320, 61), (20000, 4096, 5000), (8192, 2048, 2048),
+         (1025, 4096, 4700), (40961, 512, 1536)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens,inputs,outputs", PLANS)
+def test_every_plan_is_exact_where_sums_are(dtype, tokens, inputs, outputs):
+    """Whole numbers whose sums stay below 2^24: a step of tokens lost, taken twice or added to another tile shows, and so does a share of the bias."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    x = torch.randint(-3, 4, (tokens, inputs), device="cuda", generator=gen).to(dtype)
+    x[:, ::32] = 64
+    dy = torch.randint(-2, 3, (tokens, outputs), device="cuda", generator=gen).to(dtype)
+    assert 64 * 2 * tokens < 1 << 24
+    dw, db = ops.weight_grad8(dy, ops.pack8(x), bias=True)
+    assert torch.equal(dw, product(dy, x).to(dtype)) and torch.equal(db, dy.double().sum(0).to(dtype))
+    again, none = ops.weight_grad8(dy, ops.pack8(x))
+    assert torch.equal(again, dw) and none is None
+
+
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1, 40, 30), (1025, 300, 700), (2048, 64, 64), (8192, 768, 2304), (15126, 320, 611), (1025, 4096, 4700), (8200, 1100, 5000), (100003, 96, 2000)])
+def test_every_part_of_float32_reaches_its_token(tokens, inputs, outputs):
+    """One number of 24 bits, of its own size, for each output, at a token that no other has (as far as there are so many): every result is exact, and
+    any of the three parts that met another token's inputs would show."""
+    gen = torch.Generator(device="cuda").manual_seed(outputs)
+    token = (torch.arange(outputs, device="cuda") * max(1, tokens // outputs) + torch.randint(0, max(1, tokens // outputs), (outputs,), device="cuda", generator=gen)) % tokens
+    token[-1] = tokens - 1
+    number = (torch.randint(1 << 22, 1 << 23, (outputs,), device="cuda", generator=gen) * 2 + 1).float()
+    number *= 2.0 ** torch.randint(-40, 20, (outputs,), device="cuda", generator=gen) * (torch.randint(0, 2, (outputs,), device="cuda", generator=gen) * 2 - 1)
+    dy = torch.zeros(tokens, outputs, device="cuda")
+    dy[token, torch.arange(outputs, device="cuda")] = number
+    # Powers of two that tell tokens apart, and blocks of features.
+    power = torch.arange(tokens, device="cuda")[:, None] * 7 % 11 + torch.arange(inputs, device="cuda")[None, :] // 32 % 5
+    x = 2.0 ** power.float()
+    dw, db = ops.weight_grad8(dy, ops.pack8(x), bias=True)
+    assert torch.equal(dw, number[:, None] * x[token]) and torch.equal(db, number)
+
+
+@pytest.mark.parametrize("tokens,inputs,outputs", [(8192, 768, 2304), (26001, 700, 500), (20000, 1100, 260), (16000, 64, 64), (2048, 64, 64), (65536, 512, 512)])
+def test_full_precision_of_long_sums(tokens, inputs, outputs):
+    gen = torch.Generator(device="cuda").manual_seed(inputs)
+    dy, x = torch.randn(tokens, outputs, device="cuda", generator=gen), torch.randn(tokens, inputs, device="cuda", generator=gen)
+    p = ops.pack8(x)
+    dw, db = ops.weight_grad8(dy, p, bias=True)
+    # T additions of both signs in a row, rounded to 24 bits, are off by 2^-24 / sqrt(3) * sqrt(T / 2) of the norm: 1.1e-6 for 2048 terms, more for more.
+    # The kernel adds in chunks and may not be worse than that. (dY cut to 8 bits would be off by 2^-8, to 16 by 2^-16.)
+    for got, want in ((dw, product(dy, ops.unpack8(p))), (db, dy.double().sum(0))):
+        assert (got.double() - want).norm() <= 1e-6 * want.norm()
