@@ -132,3 +132,37 @@ def test_saved_tensors_may_go_elsewhere_and_be_made_again():
         x.grad = w.grad = m.grad = None
         torch.utils.checkpoint.checkpoint(step, x, w, m, use_reentrant=reentrant).backward()
         assert all(torch.equal(a, b) for a, b in zip(want, (x.grad, w.grad, m.grad)))
+
+
+def test_branches_of_a_captured_graph():
+    """Two branches of one graph, joined in front of calls that read both: the kernels start early, and wait for both."""
+    x, dy = (torch.randn(700, n, device="cuda").bfloat16() for n in (288, 320))
+    q, w = torch.randn(1, 300, 4, 64, device="cuda").bfloat16(), torch.ones(64, device="cuda").bfloat16()
+    f, p = ops.rotary_frequencies(64)[0], torch.arange(300, device="cuda")
+
+    def first():
+        return [ops.unpack8(ops.pack8(x)), ops.gelu8(x)]
+
+    def second():
+        return [*ops.weight_grad8(dy, ops.pack8(x * 2), bias=True), *ops.rotary(q, q, p, f), *ops.qk_norm_rotary(q, q, w, w, p, f)]
+
+    def joined(a, b):
+        return [ops.weight_grad8(dy, ops.pack8(a[1]))[0], ops.gelu8(b[0]), ops.gelu8(a[0]), *ops.qk_norm_rotary(b[2], b[5], w, w, p, f)]
+
+    want = joined(first(), second())
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b = second()
+        a = first()
+        main.wait_stream(side)
+        got = joined(a, b)
+    for _ in range(10):
+        for t in got:
+            t.fill_(3.0)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
