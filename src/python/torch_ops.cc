@@ -786,9 +786,11 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     try {
         // Whoever records torch's operators would record the allocation of a result, and not the kernel that fills it.
+        using Modes = c10::impl::TorchDispatchModeTLS;
         using Mode = c10::impl::TorchDispatchModeKey;
-        if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(Mode::PROXY).has_value() ||
-            c10::impl::TorchDispatchModeTLS::get_mode(Mode::FAKE).has_value() || c10::impl::TorchDispatchModeTLS::get_mode(Mode::FUNCTIONAL).has_value())
+        if (torch::jit::tracer::isTracing() ||
+            (Modes::any_modes_set() &&
+             (Modes::get_mode(Mode::PROXY).has_value() || Modes::get_mode(Mode::FAKE).has_value() || Modes::get_mode(Mode::FUNCTIONAL).has_value())))
             refuse("these operators are no torch operators and cannot be traced");
         return kFunction(args, nargs);
     } catch (const Refused& e) {
