@@ -30,7 +30,7 @@
 // 16-bit types: an instruction cuts each of its 16 products at a quarter, and their sum with the accumulator at the whole, of the last of 24 bits (seen: products of
 // 3/16 of it beside a 1 are lost, 16 of a quarter come through). Of a sum of one sign that takes 1.8e-4 in 65536 tokens and more than fp16's own rounding
 // (4.9e-4) in 200,000. So their sums too are added to those in memory, rounded, but after every 16384 tokens: 7e-5 is lost, and at most
-// 512 * 5 * 2^-23 = 3.1e-4, at any length. (65536 x 4096 x 4096 bf16: 1627 -> 1684 us; after every 8192 tokens 1786, and 16384 x 4096 x 4096 would go from 376 to 408.)
+// 512 * 5 * 2^-23 = 3.1e-4, at any length. (65536 x 4096 x 4096 bf16: 1632 -> 1704 us; after every 8192 tokens 1786, and 16384 x 4096 x 4096 would go from 376 to 408.)
 //
 // dY that TMA cannot read (rows or address not at a multiple of 16 bytes) is copied first.
 //
@@ -266,6 +266,51 @@ __device__ __forceinline__ void put(const float (&f)[32], unsigned turn, T* to, 
     __syncwarp();
 }
 
+// The same to the gradient: 32 outputs from `output` on, of which `there` are there, of the warp's features from `feature` on.
+template <typename T>
+__device__ __forceinline__ void put_out(const WeightGradArgs& a, float (&f)[32], unsigned turn, unsigned feature, unsigned output, unsigned there, bool later) {
+    const unsigned lane = threadIdx.x & 31u;
+    if (a.wide) {
+        put<T>(f, turn, static_cast<T*>(a.out) + (u64)output * a.inputs + feature, a.inputs, there, a.inputs - feature, later);
+    } else if (feature + lane < a.inputs) {
+        T* out = static_cast<T*>(a.out) + (u64)output * a.inputs + feature + lane;
+#pragma unroll
+        for (unsigned j = 0; j < 32; ++j) {
+            if (j < there) {
+                if constexpr (sizeof(T) == 4) f[j] += later ? out[(u64)j * a.inputs] : 0.0f;
+                out[(u64)j * a.inputs] = Elem<T>::from_f(f[j]);
+            }
+        }
+    }
+}
+
+// 16-bit types: what was summed of a whole tile of a long sum, to the sums in memory, where each lane finds what it left (four outputs of its feature, beside
+// those of the next), or with them to the gradient. (Apart, because in the loop below it costs a short call 0.3 us.)
+template <typename T, unsigned kWidth>
+__device__ __noinline__ void add_long_sum(const WeightGradArgs& a, const Piece& p, unsigned columns, unsigned turn, unsigned in_tile) {
+    const unsigned feature = (p.tile % a.feature_tiles) * kTile + in_tile, output0 = (p.tile / a.feature_tiles) * kWidth;
+    const unsigned outputs = feature < a.inputs ? min(kWidth, a.outputs - output0) : 0u;
+    for (unsigned c = 0; c < outputs; c += 32u) {
+        float f[32];
+        __syncwarp();
+        tmem_load32(columns + c, f);
+        float4* sums = reinterpret_cast<float4*>(a.pieces + (u64)p.slot * (kWidth * kTile)) + c / 4u * kTile + in_tile + (threadIdx.x & 31u);
+        if (p.later) {
+            float4 old[8];
+#pragma unroll
+            for (unsigned j = 0; j < 8; ++j) old[j] = sums[j * kTile];
+#pragma unroll
+            for (unsigned j = 0; j < 8; ++j) { f[4 * j] += old[j].x; f[4 * j + 1] += old[j].y; f[4 * j + 2] += old[j].z; f[4 * j + 3] += old[j].w; }
+        }
+        if (p.to != a.steps_of_tile) {
+#pragma unroll
+            for (unsigned j = 0; j < 8; ++j) sums[j * kTile] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+        } else {
+            put_out<T>(a, f, turn, feature, output0 + c, min(32u, outputs - c), false);
+        }
+    }
+}
+
 // After a wait that ran out: all that this CTA's pair was to write is NaN (its own half of the features and of the bias), so that whoever reads it sees it.
 template <typename T, bool kBias, unsigned kWidth>
 __device__ __noinline__ void spoil(const WeightGradArgs& a, const Share& share, unsigned rank) {
@@ -437,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
                             const unsigned from = base + s * kDyBytes + b * kOperandBytes + (warp - 2u) * kBlockBytes;
                             // Sixteen tokens, four times, then to the sum of all: an error of at most 20 roundings, however many tokens there are.
                             float2 step = make_float2(0.0f, 0.0f);
-#pragma unroll 1
+#pragma unroll
                             for (unsigned t0 = 0; t0 < kStep; t0 += 16) {
                                 float2 some = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -536,42 +581,15 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
             const unsigned output0 = (p.tile / a.feature_tiles) * kWidth;
             float* piece = a.pieces + (u64)p.slot * (kWidth * kTile) + in_tile;
             const unsigned outputs = feature < a.inputs ? min(kWidth, a.outputs - output0) : 0u;  // of the tile, that this warp has to write
-            for (unsigned c = 0; c < outputs; c += 32u) {
-                float f[32];
-                __syncwarp();
-                tmem_load32(tmem + buffer * kTile + c + (quarter * 32u << 16), f);
-                const unsigned there = min(32u, outputs - c);
-                if (!p.whole) {
-                    put<float>(f, turn, piece + (u64)c * kTile, kTile, 32u, kTile, p.later);
-                    continue;
-                }
-                if constexpr (sizeof(T) == 2) {
-                    // A long sum: each lane finds what it left, four outputs of its feature beside those of the next.
-                    float4* sums = reinterpret_cast<float4*>(a.pieces + (u64)p.slot * (kWidth * kTile)) + c / 4u * kTile + in_tile + lane;
-                    if (p.later) {
-                        float4 old[8];
-#pragma unroll
-                        for (unsigned j = 0; j < 8; ++j) old[j] = sums[j * kTile];
-#pragma unroll
-                        for (unsigned j = 0; j < 8; ++j) { f[4 * j] += old[j].x; f[4 * j + 1] += old[j].y; f[4 * j + 2] += old[j].z; f[4 * j + 3] += old[j].w; }
-                    }
-                    if (p.to != a.steps_of_tile) {
-#pragma unroll
-                        for (unsigned j = 0; j < 8; ++j) sums[j * kTile] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-                        continue;
-                    }
-                }
-                if (a.wide) {
-                    put<T>(f, turn, static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature, a.inputs, there, a.inputs - feature, p.later);
-                } else if (feature + lane < a.inputs) {
-                    T* out = static_cast<T*>(a.out) + (u64)(output0 + c) * a.inputs + feature + lane;
-#pragma unroll
-                    for (unsigned j = 0; j < 32; ++j) {
-                        if (j < there) {
-                            if constexpr (sizeof(T) == 4) f[j] += p.later ? out[(u64)j * a.inputs] : 0.0f;
-                            out[(u64)j * a.inputs] = Elem<T>::from_f(f[j]);
-                        }
-                    }
+            if (sizeof(T) == 2 && p.whole && (p.later || p.to != a.steps_of_tile)) {
+                add_long_sum<T, kWidth>(a, p, tmem + buffer * kTile + (quarter * 32u << 16), turn, in_tile);
+            } else {
+                for (unsigned c = 0; c < outputs; c += 32u) {
+                    float f[32];
+                    __syncwarp();
+                    tmem_load32(tmem + buffer * kTile + c + (quarter * 32u << 16), f);
+                    if (p.whole) put_out<T>(a, f, turn, feature, output0 + c, min(32u, outputs - c), p.later);
+                    else put<float>(f, turn, piece + (u64)c * kTile, kTile, 32u, kTile, p.later);
                 }
             }
             tcgen05_fence_before();
