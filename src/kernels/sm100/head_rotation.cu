@@ -5,8 +5,8 @@
 // gradient of a rotation is the rotation back: g = R^T dy; of the norm, dw = sum g x rstd, dx = rstd (g w - x rstd^2 mean(g w x)).
 //
 // Bound by HBM: every head is read once and written once. Angles are made where they are used: position * frequency as
-// turns in 64 bits, less its whole turns, then one sincospi in 32 bits (error 2e-7 at any position; in 32 bits the product alone is off by
-// 0.06 at a million). A warp makes them once for its tokens, in shared memory of its own, and all heads of a token, of queries and
+// turns in 64 bits, less its whole turns, then one sincospi in 32 bits (error 2e-7, and beyond 2^26 turns 2^-49 radians for each of them;
+// in 32 bits the product alone is off by 0.06 at a million). A warp makes them once for its tokens, in shared memory of its own, and all heads of a token, of queries and
 // keys, share them. Warps meet nowhere but at the end of the backward pass.
 //
 // A group of lanes holds a head: each lane V pairs at V neighbouring places of either half (interleaved: 2V neighbouring elements), so
@@ -15,8 +15,9 @@
 // would leave V = 1 for most of them; there a lane holds 2V neighbouring elements (Layout::Apart) and finds their partners in shared memory (norm, forward and
 // backward, of 27264 x (8 + 4) x 128 bf16: 102 elements turned 475 -> 174 us; all of them, in halves, 116).
 //
-// 32768 x (32 + 8) x 128 bf16 turn in 104 us (6.4 TB/s, 0.98 of a copy's rate); with the norm, 16384 x (32 + 8) x 128 take 85 us, and 108 backward, each 0.6 of that
-// rate: there it is instructions, 380 for 16 elements of a lane, two thirds of the slots of 32 warps (64 registers), and 0.57 of 16 warps' (128).
+// 32768 x (32 + 8) x 128 bf16 turn in 104 us (6.4 TB/s, 0.98 of a copy's rate); with the norm, 16384 x (32 + 8) x 128 take 85 us, and 108 backward, 0.75 and 0.6 of that
+// rate. Forward, 380 instructions for 16 elements of a lane take 0.68 of the issue slots, and the 64 registers that 32 warps leave are too few: 48 to 56 bytes spill, 84 to 108
+// where pairs are interleaved. Backward, 126 registers leave 16 warps, which take 0.57 of the slots: the rest of the time none of them has an instruction ready.
 //
 // The inputs of the norm are kept for the backward pass in 8 bits, a head being a block (block8.cuh): the largest magnitude comes from
 // the same exchange as the sum of squares.

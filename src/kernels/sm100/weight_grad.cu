@@ -34,8 +34,8 @@
 //
 // dY that TMA cannot read (rows or address not at a multiple of 16 bytes) is copied first.
 //
-// 16384 x 4096 x 4096 bf16: 369 us and 18 for the pieces, 1.42 PFLOP/s, 0.87 of what a library product of 16-bit operands reaches in a burst; tensor pipe 0.79 busy.
-// 8192 x 768 x 2304 fp32: 94 us, 0.45 busy (three products of every widened step, 28 us before them to lay dY out, 10 behind them). 1024 x 768 x 768: 14 + 7 us.
+// 16384 x 4096 x 4096 bf16: 377 us and 17 for the pieces, 1.40 PFLOP/s, 0.85 of what a library product of 16-bit operands reaches in a burst; tensor pipe 0.78 busy.
+// 8192 x 768 x 2304 fp32: 97 us, 0.44 busy (three products of every widened step, 27 us before them to lay dY out, 10 behind them). 1024 x 768 x 768: 12.5 + 6 us.
 #include "kernels/sm100/weight_grad.h"
 
 #include "core/check.h"
