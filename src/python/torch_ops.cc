@@ -11,6 +11,7 @@
 #include <ATen/Functions.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
@@ -424,11 +425,15 @@ PyObject* linear8(PyObject* const* args, Py_ssize_t nargs) {
     at::Tensor x = tensor_of("x", args[0]), weight = tensor_of("weight", args[1]), bias = maybe_tensor("bias", args[2]);
     std::optional<c10::impl::ExcludeDispatchKeyGuard> without_autocast;
     if (at::autocast::is_autocast_enabled(at::kCUDA)) {
-        // By autocast's rules and through its cache: a weight is cast once, and 64-bit tensors are not.
+        // By autocast's rules and through its cache: a weight is cast once, and 64-bit tensors are not. In a capture without the cache: a replay would not see
+        // the weights of its time, and the cache would hold memory of the graph's.
         const at::ScalarType type = at::autocast::get_autocast_dtype(at::kCUDA);
-        x = at::autocast::cached_cast(type, x, at::kCUDA);
-        weight = at::autocast::cached_cast(type, weight, at::kCUDA);
-        if (bias.defined()) bias = at::autocast::cached_cast(type, bias, at::kCUDA);
+        const c10::cuda::CUDAGuard guard(x.device());
+        const bool captured = c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+        for (at::Tensor* t : {&x, &weight, &bias}) {
+            if (!t->defined() || !at::autocast::is_eligible(*t, at::kCUDA)) continue;
+            *t = captured ? t->to(type) : at::autocast::cached_cast(type, *t, at::kCUDA);
+        }
         without_autocast.emplace(c10::DispatchKey::AutocastCUDA);
     }
     same_place("weight", weight, x);

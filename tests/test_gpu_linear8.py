@@ -125,3 +125,29 @@ def test_head_norms_keep_8_bits_only_where_they_are_told_to():
     q, w, p, f = q.requires_grad_(), w.requires_grad_(), torch.arange(9, device="cuda"), ops.rotary_frequencies(64)[0]
     given, full, short = (torch.autograd.grad(ops.qk_norm_rotary(q, None, w, None, p, f, **keep)[0], (q, w), dy) for keep in ({}, {"keep": None}, {"keep": "int8"}))
     assert all(torch.equal(a, b) for a, b in zip(given, full)) and not torch.equal(given[0], short[0])
+
+
+def test_a_capture_inside_one_autocast_context_sees_later_weights():
+    """Eager steps and the capture share the context, and so its cache of cast weights, which is not for a graph."""
+    x, w = torch.randn(40, 64, device="cuda"), torch.randn(32, 64, device="cuda", requires_grad=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side), torch.no_grad():
+            ops.linear8(x, w)
+            eager = ops.linear8(x, w)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(graph):
+            captured = ops.linear8(x, w)
+        graph.replay()
+        assert torch.equal(captured, eager)
+        with torch.no_grad():
+            w.mul_(2.0)
+        graph.replay()
+        assert torch.equal(captured, eager * 2)
+    with torch.autocast("cuda", dtype=torch.bfloat16):  # a weight that was cast without a gradient has one all the same
+        with torch.no_grad():
+            ops.linear8(x, w)
+        (dw,) = torch.autograd.grad(ops.linear8(x, w).float().sum(), w)
+    assert dw.dtype == torch.float32 and dw.any()
