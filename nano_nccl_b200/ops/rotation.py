@@ -4,7 +4,8 @@
 joint projection costs no copy); their heads may differ in number, and either may be None. ``positions`` is [tokens] or
 [batch, tokens], int64 or int32. ``frequencies`` is a float64 vector, radians per position of each pair; it turns the first
 ``2 * len(frequencies)`` elements of a head and leaves the others as they are. The pairs are ``(i, i + len(frequencies))``
-(layout ``"half"``) or ``(2i, 2i + 1)`` (``"interleaved"``). Angles are made in 64 bits, so positions may be far.
+(layout ``"half"``) or ``(2i, 2i + 1)`` (``"interleaved"``). Angles are made in 64 bits, so positions may be far
+(an error of 2e-7, and beyond 2^26 turns of 2^-49 radians for each turn).
 """
 import math
 
