@@ -72,7 +72,7 @@ constexpr unsigned kFirstTransformWarp = 4, kFirstEpilogueWarp = 12;
 // from the one before it only: whoever waits on a barrier has to have seen every phase of it.)
 constexpr unsigned kGroups = 4, kGroupWarps = 2;
 constexpr unsigned kChunkSteps = 16;  // fp32: steps of each part between two additions to the sums in memory
-constexpr unsigned kLongSteps = 256;  // 16-bit types: steps between two additions to the sums in memory, see below
+constexpr unsigned kLongSteps = 256;  // 16-bit types: steps between two additions to the sums in memory, see above
 constexpr unsigned kMaxPairs = 74;    // 148 SMs
 constexpr unsigned kTurnBytes = 32 * 32 * 4;  // of an epilogue warp: 32 outputs of its 32 features
 // Shared memory, from a multiple of 1024 bytes on: dY of the stages, X^ of the groups, their codes, what the epilogue turns, barriers.
@@ -196,7 +196,7 @@ __device__ __forceinline__ Piece piece_at(const WeightGradArgs& a, const Share& 
     }
     return p;
 }
-// The part of a piece that is summed on the tensor cores alone: fp32: sixteen steps of each part of dY.
+// The part of a piece that is summed on the tensor cores alone: 256 steps, fp32 sixteen of each part of dY.
 __device__ __forceinline__ Piece segment_at(const WeightGradArgs& a, const Share& s, unsigned n) {
     Piece p = piece_at(a, s, n);
     const unsigned chunk = a.parts > 1 ? a.parts * kChunkSteps : kLongSteps;
