@@ -14,7 +14,8 @@ _NATIVE = None
 
 # What the training operators call, in the order that the native module expects.
 _TRAIN = ("b2_last_error", "b2_pack8", "b2_unpack8", "b2_gelu8_forward", "b2_gelu8_backward", "b2_weight_grad8_workspace", "b2_weight_grad8",
-          "b2_rotate_heads", "b2_rotate_heads_backward")
+          "b2_rotate_heads", "b2_rotate_heads_backward", "b2_embed", "b2_embed_backward_workspace", "b2_embed_backward", "b2_vocabulary_loss_sizes",
+          "b2_vocabulary_loss_forward", "b2_vocabulary_loss_backward")
 
 
 class B2Config(ctypes.Structure):
@@ -104,7 +105,7 @@ def check(code):
 
 
 def load_native_calls():
-    """The module with the collective calls and the training operators (src/python/torch_binding.cc, torch_ops.cc), bound to the library that
+    """The module with the collective calls and the training operators (src/python/torch_binding.cc, torch_ops.cc, vocabulary_ops.cc), bound to the library that
     load() returns. Like the library it is built in-tree, and nothing stands in for it."""
     global _NATIVE
     if _NATIVE is None:

@@ -33,6 +33,13 @@ class _Gelu8(torch.nn.GELU):
         return ops.gelu8(x, self.approximate)
 
 
+class _Embedding(torch.nn.Embedding):
+    """Tokens looked up by :func:`nano_nccl_b200.ops.embedding`."""
+
+    def forward(self, tokens):
+        return ops.embedding(tokens, self.weight)
+
+
 def _modules(checkpoints):
     return (torch.nn.Linear, torch.nn.GELU) if checkpoints is None else (_Linear8, _Gelu8)
 
@@ -91,27 +98,46 @@ class _Block(torch.nn.Module):
 class TinyGPT2(torch.nn.Module):
     """``positions``: "learned" (an embedding) or "rotary" (queries and keys are turned). ``qk_norm``: a norm of each head of queries and keys.
     ``checkpoints``: "int8" keeps the inputs of projections, activations and head norms in 8 bits for the backward pass, None keeps them as they
-    are. All but the defaults run on CUDA only (:mod:`nano_nccl_b200.ops`)."""
+    are. ``vocabulary``: "fused" looks tokens up, and makes losses, without logits in memory (:mod:`nano_nccl_b200.ops.vocabulary`; negative tokens are padding),
+    "plain" by torch's own. All but the defaults run on CUDA only (:mod:`nano_nccl_b200.ops`)."""
 
-    def __init__(self, vocab=512, context=64, hidden=64, layers=2, heads=4, positions="learned", qk_norm=False, checkpoints=None):
+    def __init__(self, vocab=512, context=64, hidden=64, layers=2, heads=4, positions="learned", qk_norm=False, checkpoints=None, vocabulary="plain"):
         super().__init__()
         if positions not in ("learned", "rotary"):
             raise ValueError(f"unknown kind of positions '{positions}'")
         if checkpoints not in (None, "int8"):
             raise ValueError(f"unknown kind of checkpoints '{checkpoints}'")
+        if vocabulary not in ("plain", "fused"):
+            raise ValueError(f"unknown kind of vocabulary '{vocabulary}'")
         if hidden % heads and (positions == "rotary" or qk_norm or checkpoints is not None):
             raise ValueError(f"{heads} heads do not make {hidden}")
         if (positions == "rotary" or qk_norm) and ((hidden // heads) % 2 or hidden // heads > 256):
             raise ValueError(f"{heads} heads of an even size up to 256 do not make {hidden}")
-        self.wte = torch.nn.Embedding(vocab, hidden)
+        self.vocabulary = vocabulary
+        self.wte = (_Embedding if vocabulary == "fused" else torch.nn.Embedding)(vocab, hidden)
         self.wpe = torch.nn.Embedding(context, hidden) if positions == "learned" else None
         self.blocks = torch.nn.ModuleList([_Block(hidden, heads, positions == "rotary", qk_norm, checkpoints) for _ in range(layers)])
         self.ln_f = torch.nn.LayerNorm(hidden)
 
-    def forward(self, tokens):
+    def forward(self, tokens, targets=None, teacher=None, temperature=1.0):
+        """Logits; with ``targets`` [batch, tokens] their mean cross entropy (negative targets do not count), with ``teacher``, a pair of the largest
+        logits of a teacher and their tokens ([batch, tokens, entries] each), the mean divergence from it (:func:`nano_nccl_b200.ops.linear_distillation`)."""
+        if targets is not None and teacher is not None:
+            raise ValueError("targets or a teacher, not both")
+        if teacher is not None and self.vocabulary != "fused":
+            raise ValueError("a teacher needs vocabulary='fused'")
         x = self.wte(tokens)
         if self.wpe is not None:
             x = x + self.wpe(torch.arange(tokens.shape[1], device=tokens.device))
         for b in self.blocks:
             x = b(x)
-        return self.ln_f(x) @ self.wte.weight.t()
+        x = self.ln_f(x)
+        if teacher is not None:
+            return ops.linear_distillation(x, self.wte.weight, *teacher, temperature=temperature)
+        if targets is not None and self.vocabulary == "fused":
+            return ops.linear_cross_entropy(x, self.wte.weight, targets)
+        logits = x @ self.wte.weight.t()
+        if targets is None:
+            return logits
+        losses = torch.nn.functional.cross_entropy(logits.flatten(0, -2).float(), targets.flatten().long().clamp(min=-1), ignore_index=-1, reduction="sum")
+        return losses / (targets >= 0).sum().clamp(min=1)

@@ -20,7 +20,7 @@ forward mode, ``torch.func`` and tensors that stand for others are refused. (``t
 """
 import torch
 
-from .._lib import check, load, load_native_calls
+from .._lib import B200CclError, load, load_native_calls
 
 _APPROXIMATIONS = {"none": False, "tanh": True}
 
@@ -90,7 +90,14 @@ def linear8(x, weight, bias=None):
 
 
 def check_async_error(device=None):
-    """Raises B200CclError if a bounded wait inside a weight gradient on ``device`` (default: the current one) ran out since this was last called.
-    Such gradients are NaN, so a loss scaler sees them too. Synchronize first: only calls that are done are known."""
+    """Raises B200CclError if a bounded wait inside a weight gradient, or a loss over a vocabulary or its gradients (:mod:`.vocabulary`), on ``device`` (default: the
+    current one) ran out since this was last called. Such results are NaN, so a loss scaler sees them too. Synchronize first: only calls that are done are known."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index if not isinstance(device, int) else device
-    check(load().b2_train_check_async_error(torch.cuda.current_device() if index is None else index))
+    index = torch.cuda.current_device() if index is None else index
+    codes = []
+    for what in (load().b2_train_check_async_error, load().b2_vocabulary_loss_check_async_error):
+        codes.append(what(index))  # (both are asked, and forget, whatever the first says)
+        if codes[-1] != 0:
+            failure = load().b2_last_error()
+    if any(codes):
+        raise (ValueError if 2 in codes else B200CclError)(failure.decode("utf-8", "replace"))

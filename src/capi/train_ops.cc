@@ -1,46 +1,17 @@
 #include "b200ccl/train_ops.h"
 
-#include "core/check.h"
+#include "capi/guarded.h"
 #include "kernels/sm100/checkpoint8.h"
 #include "kernels/sm100/head_rotation.h"
+#include "kernels/sm100/wait_status.h"
 #include "kernels/sm100/weight_grad.h"
 
-#include <cstdint>
-#include <exception>
-#include <stdexcept>
-#include <string>
-
 using namespace b200ccl;
-
-namespace b200ccl::kernels {
-void set_last_error_message(const std::string& message);  // b2_last_error() of the calling thread
-}
+using capi::aligned;
+using capi::dtype_of;
+using capi::guarded;
 
 namespace {
-
-template <typename F>
-int guarded(const char* what, F&& f) {
-    try {
-        f();
-        return 0;
-    } catch (const std::invalid_argument& e) {
-        kernels::set_last_error_message(std::string(what) + ": " + e.what());
-        return 2;
-    } catch (const std::exception& e) {
-        kernels::set_last_error_message(std::string(what) + ": " + e.what());
-        return 1;
-    } catch (...) {
-        kernels::set_last_error_message(std::string(what) + ": unknown failure");
-        return 1;
-    }
-}
-
-DType dtype_of(int code) {
-    B2_REQUIRE(code >= 0 && code <= 2, "unsupported dtype");
-    return static_cast<DType>(code);
-}
-
-bool aligned(const void* p, std::size_t n) { return reinterpret_cast<std::uintptr_t>(p) % n == 0; }
 
 void check_kept(const void* codes, const void* scales, std::size_t rows, std::size_t columns, bool needed = true) {
     B2_REQUIRE(columns <= (1ull << 30) && rows < (1ull << 31), "more than 2^31 rows or 2^30 columns");
@@ -209,7 +180,7 @@ int b2_weight_grad8_within(const b2_weight_grad* call, unsigned long long wait_n
 
 int b2_train_check_async_error(int device) {
     return guarded("weight_grad8", [&] {
-        if (kernels::weight_grad_failed(device))
+        if (kernels::waits_failed(kernels::WaitsOf::WeightGrad, device))
             throw std::runtime_error("a wait inside a call on device " + std::to_string(device) + " ran out; its gradients are NaN");
     });
 }

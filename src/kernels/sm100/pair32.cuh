@@ -28,6 +28,12 @@ __device__ __forceinline__ Pair32 mul2(Pair32 a, Pair32 b) {
     return r;
 }
 
+__device__ __forceinline__ Pair32 add2(Pair32 a, Pair32 b) {
+    Pair32 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
 // Wide accesses to what a kernel reads and writes once. They name no memory that they change, so that the compiler keeps a kernel's arguments in
 // registers across them: nothing is read here that was written in the same kernel.
 __device__ __forceinline__ uint4 load16_once(const void* p) {

@@ -79,6 +79,10 @@ __device__ __forceinline__ void tma_load_box(unsigned dst, const CUtensorMap* ma
         "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
+// A box of shared memory to a three-dimensional tensor map of this GPU's own memory, in the thread's bulk async-group; no coordinate is negative.
+__device__ __forceinline__ void tma_store_box(const CUtensorMap* map, unsigned src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -121,10 +125,21 @@ __device__ __forceinline__ std::uint64_t operand_by_rows(unsigned address, unsig
     d |= 2ull << 61;                                           // 128-byte swizzle
     return d;
 }
-// 16-bit operands by rows (both), 32-bit accumulators.
-__host__ __device__ constexpr unsigned product_by_rows(unsigned m, unsigned n, bool bf16) {
-    return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | 1u << 15 | 1u << 16 | n / 8u << 17 | m / 16u << 24;
+// An operand whose rows lie along m or n and hold 64 neighbouring elements of the summed axis (128 bytes, swizzled): eight rows are 1024 bytes.
+// The next 16 elements of the summed axis are 32 bytes further.
+__device__ __forceinline__ std::uint64_t operand_by_columns(unsigned address) {
+    std::uint64_t d = (address >> 4) & 0x3fffu;
+    d |= 1ull << 16;                          // not looked at: a row of the tile is one swizzled row
+    d |= (std::uint64_t)(1024u >> 4) << 32;   // from eight rows to the next eight
+    d |= 1ull << 46;                          // version of sm_100
+    d |= 2ull << 61;                          // 128-byte swizzle
+    return d;
 }
+// 16-bit operands, each by rows or not, 32-bit accumulators.
+__host__ __device__ constexpr unsigned product_shape(unsigned m, unsigned n, bool bf16, bool a_by_rows, bool b_by_rows) {
+    return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (a_by_rows ? 1u : 0u) << 15 | (b_by_rows ? 1u : 0u) << 16 | n / 8u << 17 | m / 16u << 24;
+}
+__host__ __device__ constexpr unsigned product_by_rows(unsigned m, unsigned n, bool bf16) { return product_shape(m, n, bf16, true, true); }
 // 16 rows of both operands, in both CTAs of the pair; one thread of the first CTA.
 __device__ __forceinline__ void mma_pair(unsigned accumulators, std::uint64_t a, std::uint64_t b, unsigned shape, bool add) {
     asm volatile(

@@ -1,0 +1,1471 @@
+// Losses over a vocabulary, cross entropy and distillation from a teacher's top logits, without the logits in memory, and their gradients.
+//
+//   z = x w^T / tau,   q = softmax(z) over the vocabulary,   y: the target, or the teacher's distribution over its few entries
+//   loss_t = sum_v y (log y - log q) tau^2,   dz = c_t (q - y),   c_t = tau * what comes back to loss_t (over the rows that count, for a mean)
+//   dx = dz w,   dw = dz^T x
+//
+// Four products on the tensor cores, one kernel for all of them (product_kernel): a pair of CTAs works on a tile of 256 x 256 (a gradient of a narrow
+// matrix: 256 x 128), 64 elements of the summed axis at a time, the accumulators in tensor memory, twice, so that one tile is worked off while the next is summed.
+//   Stats   x w^T  -> the maximum of each row of a tile and the sum of e^(z - maximum), joined by join_kernel; the target's logit by the way
+//   Probs   x w^T  -> P = r_t (q - y) for a piece of the vocabulary, in 16 bits, to memory
+//   WeightGrad  P^T x,   InputGrad  P w   of that piece
+// So the backward pass makes the logits a second time, a third more than the products that it cannot do without; keeping them would take 2 to 4 bytes for every token
+// and word of the vocabulary, from the forward pass on. Pieces of the vocabulary and not of the tokens, because a piece of dw is then
+// complete; dx, which is small, is added up in 32 bits. P is the operand of two products and therefore of their type: its rounding (2^-8 of each
+// element in bf16) is what the gradients lose beside their own. r_t = c_t / max |c| is 1 in a mean or a sum, so that the target's element
+// stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there.
+//
+// fp32: x, w and P are exact sums of three bf16 matrices each, and six products of those give the 24-bit product (the three smallest are below 2^-24 of it).
+// The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and sums are added up in memory, rounded, after every 1024
+// elements of the summed axis; in 16-bit types after 16384.
+//
+// Tiles of the gradients that do not go evenly into the pairs are cut along the summed axis, evenly: pair i takes steps [i S / P, (i+1) S / P) of those that are
+// left, and finish_kernel adds the pieces in order. Nothing depends on timing.
+#include "kernels/sm100/vocabulary_loss.h"
+
+#include "core/check.h"
+#include "kernels/sm100/lay_out.cuh"
+#include "kernels/sm100/pair32.cuh"
+#include "kernels/sm100/tcgen05.cuh"
+#include "kernels/sm100/vec.cuh"
+#include "kernels/sm100/wait_status.h"
+#include "mem/cu_driver.h"
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+#include <mutex>
+#include <stdexcept>
+#include <type_traits>
+
+namespace b200ccl::kernels {
+
+using namespace b200ccl::dev;
+
+namespace {
+
+using u64 = unsigned long long;
+
+enum class Kind { Stats, Probs, WeightGrad, InputGrad };
+
+constexpr unsigned kTile = 256;  // of both axes of a pair's tile
+constexpr unsigned kHalf = 128;  // of one CTA
+constexpr unsigned kStep = 64;   // elements of the summed axis
+constexpr unsigned kStages = 6;
+constexpr unsigned kBlockBytes = kStep * 128;
+constexpr unsigned kOperandBytes = 2 * kBlockBytes;  // a CTA's half of an operand
+constexpr unsigned kFirstEpilogueWarp = 4, kEpilogueWarps = 8, kThreads = (kFirstEpilogueWarp + kEpilogueWarps) * 32;
+constexpr unsigned kMaxPairs = 74;     // 148 SMs
+constexpr unsigned kStagingBytes = 32 * 128;  // of an epilogue warp: 128 bytes of each of its rows
+constexpr unsigned kAtStaging = kStages * 2 * kOperandBytes, kAtBarriers = kAtStaging + kEpilogueWarps * kStagingBytes;
+constexpr unsigned kShared = kAtBarriers + 256 + 1024;
+static_assert(kShared <= 227 * 1024);
+constexpr unsigned kTileFloats = kTile * kTile;
+constexpr unsigned kLongSteps = 256, kChunkSteps = 16;  // steps between two additions to sums in memory: 16-bit types; fp32, of each of its six products
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kHalfScale = 16384.0f;  // of P in fp16
+
+template <typename T>
+using OperandOf = std::conditional_t<std::is_same_v<T, __half>, __half, __nv_bfloat16>;
+
+struct alignas(64) ProductArgs {
+    CUtensorMap a, b;  // [parts][rows][columns]
+    CUtensorMap out;   // P, or a gradient whose rows TMA can write
+    unsigned m, n;     // extents of the result that are there
+    unsigned m_tiles, n_tiles, n_tile;  // n_tile: extent of a tile along n, 256 or 128
+    unsigned parts, steps_of_part, steps_of_tile;
+    unsigned b_offset;  // added to b's row
+    unsigned pairs, waves, steps, groups;  // whole tiles of a pair; the steps of the tiles that are left, and the pairs that share them
+    bool n_first;       // neighbouring tiles lie along n
+    float* slots;       // [2 * pairs][tile]: pieces, and sums of long tiles
+    float* sums;        // [tiles][tile]: sums of all pieces of the vocabulary, or null
+    bool prior, last;   // there are sums of earlier pieces; this is the last one
+    unsigned* status;   // host memory
+    u64 wait_ns;
+    // Stats and Probs
+    float factor;  // log2(e) / temperature
+    float2* stats; // [2 * tiles along n][m]
+    float* picked; // [m]
+    const void* targets;
+    long long target_stride;
+    bool targets64, hard;
+    const float* top;    // [m]: the largest logit, and the sum of e^(z - top): apart, because of a row that is sure of its target the logarithm of all
+    const float* sum;    // would round off what it is not sure of
+    const float* valid;  // whether the row counts: 1, 0, or NaN
+    const float* loss_grad;  // [m], or null: the same for all rows
+    long long loss_grad_stride;
+    float temperature;
+    // Gradients
+    float* header;         // of the workspace: max |c|, and NaN once a product went wrong
+    void* gradient;        // rows of n elements
+    bool wide;             // TMA can write them
+};
+
+struct Barriers {
+    u64 full[kStages];        // this CTA's operands of a stage have come
+    u64 full_other[kStages];  // first CTA: the other's have
+    u64 empty[kStages];       // they have been read
+    u64 sums[2];              // accumulators are complete
+    u64 sums_free[2];         // first CTA: both CTAs have worked theirs off
+    u64 drained;              // all products are done
+    unsigned tmem;
+    unsigned failed;
+};
+static_assert(sizeof(Barriers) <= 256);
+
+// pair * steps / pairs, in 32 bits: pairs are few.
+__host__ __device__ inline unsigned first_step(unsigned pair, unsigned steps, unsigned pairs) {
+    const unsigned each = steps / pairs;
+    return pair * each + pair * (steps - each * pairs) / pairs;
+}
+
+// What a pair does, in order: `waves` whole tiles, then its steps of the tiles that are left. A run of steps of one tile:
+struct Run {
+    unsigned tile, from, to;
+    bool whole;     // this pair sums all of the tile
+    unsigned slot;  // of a piece, or of a long sum (a pair's last piece comes after its whole tiles)
+};
+struct Share {
+    unsigned pair, begin, end, whole, all;
+    __device__ __forceinline__ Share(const ProductArgs& a, unsigned p) : pair(p) {
+        begin = first_step(min(p, a.groups), a.steps, a.groups);
+        end = first_step(min(p + 1u, a.groups), a.steps, a.groups);
+        whole = a.waves * a.steps_of_tile;
+        all = whole + (end - begin);
+    }
+    __device__ __forceinline__ Run at(const ProductArgs& a, unsigned n) const {
+        Run r;
+        if (n < whole) {
+            const unsigned wave = n / a.steps_of_tile;
+            r.tile = wave * a.pairs + pair;
+            r.from = n - wave * a.steps_of_tile;
+            r.to = a.steps_of_tile;
+            r.whole = true;
+            r.slot = 2u * pair + 1u;
+        } else {
+            const unsigned at = begin + (n - whole), row = at / a.steps_of_tile, tile_at = row * a.steps_of_tile;
+            r.tile = a.waves * a.pairs + row;
+            r.from = at - tile_at;
+            r.to = min(a.steps_of_tile, end - tile_at);
+            r.whole = tile_at >= begin && tile_at + a.steps_of_tile <= end;
+            r.slot = 2u * pair + (tile_at <= begin ? 0u : 1u);
+        }
+        return r;
+    }
+};
+// The end of the part of a run, from step k on, that is summed on the tensor cores alone.
+__device__ __forceinline__ unsigned segment_end(const ProductArgs& a, unsigned k, unsigned to) {
+    const unsigned chunk = a.parts > 1 ? 6u * kChunkSteps : kLongSteps;
+    return min(to, (k / chunk + 1u) * chunk);
+}
+// Which parts of the operands, and which 64 elements, step k of a tile takes: of sixteen steps the products with the smallest sums first.
+struct Spot {
+    unsigned part_a, part_b, step;
+};
+__device__ __forceinline__ Spot spot_of(const ProductArgs& a, unsigned k) {
+    if (a.parts == 1) return {0u, 0u, k};
+    const unsigned chunk = k / (6u * kChunkSteps), in_chunk = k - chunk * (6u * kChunkSteps);
+    const unsigned length = min(kChunkSteps, a.steps_of_part - chunk * kChunkSteps), product = in_chunk / length;
+    // (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)
+    return {(0x001102u >> (4u * product)) & 15u, (0x010120u >> (4u * product)) & 15u, chunk * kChunkSteps + in_chunk - product * length};
+}
+
+struct Tile {
+    unsigned m, n;  // first element
+};
+__device__ __forceinline__ Tile tile_at(const ProductArgs& a, unsigned tile) {
+    const unsigned along = a.n_first ? a.n_tiles : a.m_tiles, row = tile / along, column = tile - row * along;
+    return {(a.n_first ? row : column) * kTile, (a.n_first ? column : row) * a.n_tile};
+}
+
+__device__ __forceinline__ void store_shared16(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float nan32() { return __uint_as_float(0x7fffffffu); }
+
+// Target `row` of a matrix; -1 where it is negative.
+__device__ __forceinline__ long long target_at(const void* targets, bool wide, long long at) {
+    const long long v = wide ? static_cast<const long long*>(targets)[at] : static_cast<const int*>(targets)[at];
+    return v < 0 ? -1 : v;
+}
+
+// 32 columns of a warp's rows to columns 32 * part.. of its 128 bytes of each row (swizzled).
+template <typename T>
+__device__ __forceinline__ void stage(unsigned staging, unsigned part, const float (&f)[32]) {
+    const unsigned lane = threadIdx.x & 31u, row = staging + lane * 128u, turn = lane & 7u;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (unsigned j = 0; j < 8; ++j)
+            store_shared16(row + ((j ^ turn) << 4), __float_as_uint(f[4 * j]), __float_as_uint(f[4 * j + 1]), __float_as_uint(f[4 * j + 2]), __float_as_uint(f[4 * j + 3]));
+    } else {
+#pragma unroll
+        for (unsigned j = 0; j < 4; ++j) {
+            unsigned w[4];
+#pragma unroll
+            for (unsigned i = 0; i < 4; ++i)
+                w[i] = std::is_same_v<T, __half> ? f2_to_h2(f[8 * j + 2 * i], f[8 * j + 2 * i + 1]) : f2_to_b2(f[8 * j + 2 * i], f[8 * j + 2 * i + 1]);
+            store_shared16(row + (((4u * part + j) ^ turn) << 4), w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+// The staged rows have been read by the copy before.
+__device__ __forceinline__ void staging_free() {
+    if ((threadIdx.x & 31u) == 0) tma_wait_group_read<0>();
+    __syncwarp();
+}
+// What was staged, to rows of a tensor map.
+__device__ __forceinline__ void staging_out(const CUtensorMap* map, unsigned staging, unsigned column, unsigned row, unsigned part, unsigned rows) {
+    fence_shared_async();
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0 && row < rows) {
+        tma_store_box(map, staging, (int)column, (int)row, (int)part);
+        tma_commit_group();
+    }
+}
+
+// max |c| and whether anything went wrong, in the first words of a gradient's workspace.
+__device__ __forceinline__ float gradient_scale(const float* header, bool half) { return header[0] * (half ? 1.0f / kHalfScale : 1.0f) + header[1]; }
+
+// c_t / max |c|; 0 of rows that do not count.
+__device__ __forceinline__ float row_weight(float valid, const float* loss_grad, long long stride, float temperature, float largest, unsigned row) {
+    if (loss_grad == nullptr || valid == 0.0f) return valid;
+    return largest == 0.0f ? 0.0f * valid : loss_grad[(long long)row * stride] * temperature * valid / largest;
+}
+
+// After a wait that ran out: all that this CTA was to make is NaN.
+template <Kind kKind, typename T>
+__device__ __noinline__ void spoil(const ProductArgs& a, const Share& share, unsigned rank) {
+    if (kKind == Kind::Probs && threadIdx.x == 0) a.header[1] = nan32();
+    for (unsigned n = kKind == Kind::Probs ? share.all : 0; n < share.all;) {
+        const Run r = share.at(a, n);
+        const Tile t = tile_at(a, r.tile);
+        if constexpr (kKind == Kind::Stats) {
+            const unsigned row = t.m + rank * kHalf + threadIdx.x % kHalf;
+            if (threadIdx.x < kHalf && row < a.m)
+                for (unsigned group = 0; group < 2; ++group) a.stats[(u64)(2u * (t.n / kTile) + group) * a.m + row] = make_float2(nan32(), nan32());
+        } else {
+            float* sums = r.whole ? a.sums + (u64)r.tile * kTileFloats : a.slots + (u64)r.slot * kTileFloats;
+            const bool gradient = r.whole && a.last;
+            for (unsigned i = threadIdx.x; i < kHalf * a.n_tile; i += kThreads) {
+                const unsigned row = rank * kHalf + i % kHalf, column = i / kHalf;
+                if (!gradient) sums[((column / 4u) * kTile + row) * 4u + column % 4u] = nan32();
+                else if (t.m + row < a.m && t.n + column < a.n) static_cast<T*>(a.gradient)[(u64)(t.m + row) * a.n + t.n + column] = Elem<T>::from_f(nan32());
+            }
+        }
+        n += r.to - r.from;
+    }
+}
+
+// T: type of x, w and their gradients.
+template <Kind kKind, typename T>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
+    constexpr bool kLogits = kKind == Kind::Stats || kKind == Kind::Probs;
+    constexpr bool kAByRows = kKind == Kind::WeightGrad, kBByRows = !kLogits;
+    constexpr bool kHalfType = std::is_same_v<T, __half>;
+    extern __shared__ unsigned char raw[];
+    // Swizzled operands start at multiples of 1024 bytes; the same place in both CTAs.
+    unsigned char* shared = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+    Barriers& bars = *reinterpret_cast<Barriers*>(shared + kAtBarriers);
+    volatile unsigned* failed = &bars.failed;
+    const unsigned base = smem_addr(shared);
+    const unsigned warp = threadIdx.x / 32u, lane = threadIdx.x & 31u;
+    const unsigned rank = cluster_rank();
+    const Share share(a, blockIdx.x / 2u);
+    const unsigned b_rows = a.n_tile / 2u;  // of a CTA
+
+    if (warp == 0 && lane == 0) {
+        for (unsigned s = 0; s < kStages; ++s) {
+            mbar_init(&bars.full[s], 1);
+            mbar_init(&bars.full_other[s], 1);
+            mbar_init(&bars.empty[s], 1);
+        }
+        for (unsigned i = 0; i < 2; ++i) {
+            mbar_init(&bars.sums[i], 1);
+            mbar_init(&bars.sums_free[i], 2 * kEpilogueWarps);
+        }
+        mbar_init(&bars.drained, 1);
+        bars.failed = 0;
+        mbar_fence_init();
+        tma_prefetch_map(&a.a);
+        tma_prefetch_map(&a.b);
+    }
+    __syncwarp();
+    if (warp == 1) tmem_alloc_pair(smem_addr(&bars.tmem), 2 * kTile);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tcgen05_fence_before();
+    cluster_sync();
+    tcgen05_fence_after();
+    const unsigned tmem = bars.tmem;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const auto bar = [](u64& b) { return smem_addr(&b); };
+    const auto operand_a = [&](unsigned stage) { return base + stage * (2u * kOperandBytes); };
+    const auto operand_b = [&](unsigned stage) { return base + stage * (2u * kOperandBytes) + kOperandBytes; };
+    if (warp == 0) {
+        if (lane == 0) {
+            const unsigned bytes = kOperandBytes + b_rows * 128u;
+            unsigned n = 0;
+            bool ok = true;
+            while (n < share.all && ok) {
+                const Run r = share.at(a, n);
+                const Tile t = tile_at(a, r.tile);
+                const int m = (int)(t.m + rank * kHalf), at = (int)(t.n + rank * b_rows);
+                for (unsigned k = r.from; k < r.to; ++k, ++n) {
+                    const unsigned s = n % kStages;
+                    const Spot spot = spot_of(a, k);
+                    const int step = (int)(spot.step * kStep);
+                    ok = wait_phase(bar(bars.empty[s]), ((n / kStages) & 1u) ^ 1u, failed, a.wait_ns);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&bars.full[s], bytes);
+                    if constexpr (kAByRows) {
+                        tma_load_box(operand_a(s), &a.a, m, step, (int)spot.part_a, bar(bars.full[s]));
+                        tma_load_box(operand_a(s) + kBlockBytes, &a.a, m + 64, step, (int)spot.part_a, bar(bars.full[s]));
+                    } else {
+                        tma_load_box(operand_a(s), &a.a, step, m, (int)spot.part_a, bar(bars.full[s]));
+                    }
+                    if constexpr (kBByRows) {
+                        for (unsigned b = 0; b < b_rows / 64u; ++b)
+                            tma_load_box(operand_b(s) + b * kBlockBytes, &a.b, at + (int)(b * 64u), step + (int)a.b_offset, (int)spot.part_b, bar(bars.full[s]));
+                    } else {
+                        tma_load_box(operand_b(s), &a.b, step, at + (int)a.b_offset, (int)spot.part_b, bar(bars.full[s]));
+                    }
+                }
+            }
+            // Stages have been given back, and after a failure copies have landed, before the CTA ends.
+            for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i) {
+                if (ok) wait_phase(bar(bars.empty[i % kStages]), (i / kStages) & 1u, failed, a.wait_ns);
+                for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.full[i % kStages]), (i / kStages) & 1u); ++polls) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const unsigned shape = product_shape(kTile, a.n_tile, !kHalfType, kAByRows, kBByRows);
+            unsigned n = 0, segments = 0;
+            bool ok = true;
+            while (n < share.all && ok) {
+                const Run r = share.at(a, n);
+                for (unsigned k = r.from; k < r.to && ok; ++segments) {
+                    const unsigned end = segment_end(a, k, r.to), buffer = segments & 1u;
+                    ok = wait_phase<true>(bar(bars.sums_free[buffer]), ((segments >> 1) & 1u) ^ 1u, failed, a.wait_ns);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    for (bool add = false; k < end; ++k, ++n) {
+                        const unsigned s = n % kStages, parity = (n / kStages) & 1u;
+                        ok = wait_phase(bar(bars.full[s]), parity, failed, a.wait_ns) && wait_phase<true>(bar(bars.full_other[s]), parity, failed, a.wait_ns);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+                        // 16 elements of the summed axis: 2048 bytes of rows, 32 bytes of columns
+                        const std::uint64_t x = kAByRows ? operand_by_rows(operand_a(s), kBlockBytes) : operand_by_columns(operand_a(s));
+                        const std::uint64_t y = kBByRows ? operand_by_rows(operand_b(s), kBlockBytes) : operand_by_columns(operand_b(s));
+#pragma unroll
+                        for (unsigned i = 0; i < kStep / 16; ++i) {
+                            mma_pair(tmem + buffer * kTile, x + i * (kAByRows ? 2048 >> 4 : 32 >> 4), y + i * (kBByRows ? 2048 >> 4 : 32 >> 4), shape, add);
+                            add = true;
+                        }
+                        commit_pair(bar(bars.empty[s]));
+                    }
+                    if (!ok) break;
+                    commit_pair(bar(bars.sums[buffer]));
+                }
+            }
+            // Products under way read shared memory and write tensor memory of both CTAs. Where a wait ran out, nobody else may be waiting for them.
+            commit_pair(bar(bars.drained));
+            for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
+        } else if (lane == 0) {
+            for (unsigned n = 0; n < share.all; ++n) {
+                if (!wait_phase(bar(bars.full[n % kStages]), (n / kStages) & 1u, failed, a.wait_ns)) break;
+                mbar_arrive_at(bar(bars.full_other[n % kStages]), 0);
+            }
+            if (!wait_phase(bar(bars.drained), 0, failed, a.wait_ns))
+                for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
+        }
+    } else if (warp >= kFirstEpilogueWarp) {
+        const unsigned quarter = warp & 3u, group = (warp - kFirstEpilogueWarp) / 4u;  // lanes of tensor memory that this warp reaches; its half of the columns
+        const unsigned in_tile = rank * kHalf + quarter * 32u, column0 = group * b_rows;
+        const unsigned staging = base + kAtStaging + (warp - kFirstEpilogueWarp) * kStagingBytes;
+        const float scale = kLogits ? 1.0f : gradient_scale(a.header, kHalfType);
+        unsigned n = 0, segments = 0;
+        bool ok = true;
+        while (n < share.all && ok) {
+            const Run r = share.at(a, n);
+            const Tile t = tile_at(a, r.tile);
+            const unsigned first = t.n + column0, row = t.m + in_tile + lane;
+            const unsigned columns = first < a.n ? min(b_rows, a.n - first) : 0u;  // of this warp
+            float* sums = (r.whole && a.sums != nullptr ? a.sums + (u64)r.tile * kTileFloats : a.slots + (u64)r.slot * kTileFloats);
+            // What a row of logits needs beside them.
+            long long target = -1;
+            float weight = 0.0f, row_top = 0.0f, share_of_sum = 0.0f;
+            if constexpr (kLogits) {
+                if (row < a.m) {
+                    if (a.hard) target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
+                    if constexpr (kKind == Kind::Probs) {
+                        weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (kHalfType ? kHalfScale : 1.0f);
+                        row_top = a.top[row];
+                        share_of_sum = weight / a.sum[row];
+                    }
+                }
+                target = target < 0 ? -1 : target - (long long)(first + a.b_offset);
+            }
+            const unsigned own_target = target >= 0 && target < (long long)columns ? (unsigned)target : 0xffffffffu;  // its column of this warp's
+            for (unsigned k = r.from; k < r.to; ++segments) {
+                const unsigned end = segment_end(a, k, r.to), buffer = segments & 1u;
+                const bool prior = k != r.from || (!kLogits && r.whole && a.prior), done = end == r.to && (kLogits || (r.whole && a.last));
+                ok = __all_sync(0xffffffffu, wait_phase(bar(bars.sums[buffer]), (segments >> 1) & 1u, failed, a.wait_ns));
+                if (!ok) break;
+                tcgen05_fence_after();
+                const unsigned from = tmem + buffer * kTile + column0 + (quarter * 32u << 16);
+                float4* kept = reinterpret_cast<float4*>(sums) + (column0 / 4u) * kTile + in_tile + lane;  // four columns of a row, beside those of the next
+                const auto take = [&](unsigned c, float (&f)[32]) {
+                    __syncwarp();
+                    tmem_load32(from + c, f);
+                    if (!prior) return;
+                    const float4* old = kept + (c / 4u) * kTile;
+#pragma unroll
+                    for (unsigned j = 0; j < 8; ++j) {
+                        const float4 v = old[j * kTile];
+                        f[4 * j] += v.x;
+                        f[4 * j + 1] += v.y;
+                        f[4 * j + 2] += v.z;
+                        f[4 * j + 3] += v.w;
+                    }
+                };
+                if (!done) {
+                    for (unsigned c = 0; c < columns; c += 32u) {
+                        float f[32];
+                        take(c, f);
+#pragma unroll
+                        for (unsigned j = 0; j < 8; ++j) kept[(c / 4u + j) * kTile] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                    }
+                } else if constexpr (kKind == Kind::Stats) {
+                    float top = -__int_as_float(0x7f800000), sum = 0.0f;
+                    const Pair32 factor = both32(a.factor);
+                    for (unsigned c = 0; c < columns; c += 32u) {
+                        float f[32];
+                        take(c, f);
+                        if (c + 32u > columns) {
+#pragma unroll
+                            for (unsigned j = 0; j < 32; ++j) f[j] = c + j < columns ? f[j] : -__int_as_float(0x7f800000);
+                        }
+                        const unsigned at = own_target - c;
+                        if (__any_sync(0xffffffffu, at < 32u)) {
+                            float z = 0.0f;
+#pragma unroll
+                            for (unsigned j = 0; j < 32; ++j) z = j == at ? f[j] : z;
+                            if (at < 32u) a.picked[row] = z;
+                        }
+                        float most[4] = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+                        for (unsigned j = 4; j < 32; ++j) most[j & 3u] = fmaxf(most[j & 3u], f[j]);
+                        const float now = fmaxf(top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+                        const float off = now == -__int_as_float(0x7f800000) ? 0.0f : -now;
+                        float some[4] = {sum * exp2_fast((top + off) * a.factor), 0.0f, 0.0f, 0.0f};
+                        const Pair32 offs = both32(off);
+#pragma unroll
+                        for (unsigned j = 0; j < 32; j += 2) {
+                            const float2 e = apart(mul2(add2(pair32(f[j], f[j + 1]), offs), factor));
+                            some[j & 2u] += exp2_fast(e.x);
+                            some[(j & 2u) + 1u] += exp2_fast(e.y);
+                        }
+                        sum = (some[0] + some[1]) + (some[2] + some[3]);
+                        top = now;
+                    }
+                    if (row < a.m) a.stats[(u64)(2u * (t.n / kTile) + group) * a.m + row] = make_float2(top, sum);
+                } else if constexpr (kKind == Kind::Probs) {
+                    const Pair32 factor = both32(a.factor), off = both32(-row_top);
+                    for (unsigned c = 0; c < columns; c += 64u) {
+                        float f[2][32];
+#pragma unroll
+                        for (unsigned h = 0; h < 2; ++h) {
+                            take(c + 32u * h, f[h]);
+                            const unsigned at = own_target - (c + 32u * h);
+#pragma unroll
+                            for (unsigned j = 0; j < 32; j += 2) {
+                                const float2 e = apart(mul2(add2(pair32(f[h][j], f[h][j + 1]), off), factor));
+                                f[h][j] = share_of_sum * exp2_fast(e.x);
+                                f[h][j + 1] = share_of_sum * exp2_fast(e.y);
+                            }
+                            if (__any_sync(0xffffffffu, at < 32u)) {
+#pragma unroll
+                                for (unsigned j = 0; j < 32; ++j) f[h][j] -= j == at ? weight : 0.0f;
+                            }
+                            if (c + 32u * h + 32u > columns) {
+#pragma unroll
+                                for (unsigned j = 0; j < 32; ++j) f[h][j] = c + 32u * h + j < columns ? f[h][j] : 0.0f;
+                            }
+                            if (weight == 0.0f) {
+#pragma unroll
+                                for (unsigned j = 0; j < 32; ++j) f[h][j] = 0.0f;
+                            }
+                        }
+                        constexpr unsigned kParts = sizeof(T) == 4 ? 3 : 1;
+#pragma unroll
+                        for (unsigned p = 0; p < kParts; ++p) {
+                            staging_free();
+#pragma unroll
+                            for (unsigned h = 0; h < 2; ++h) {
+                                if constexpr (kParts == 1) {
+                                    stage<T>(staging, h, f[h]);
+                                } else {
+                                    float part[32];  // the leading eight bits of what is left
+#pragma unroll
+                                    for (unsigned j = 0; j < 32; ++j) {
+                                        part[j] = __uint_as_float(__float_as_uint(f[h][j]) & 0xffff0000u);
+                                        f[h][j] -= part[j];
+                                    }
+                                    stage<__nv_bfloat16>(staging, h, part);
+                                }
+                            }
+                            staging_out(&a.out, staging, first + c, t.m + in_tile, p, a.m);
+                        }
+                    }
+                } else {
+                    constexpr unsigned kBlock = 128u / sizeof(T);
+                    for (unsigned c = 0; c < columns; c += kBlock) {
+                        staging_free();
+#pragma unroll
+                        for (unsigned h = 0; h < kBlock / 32u; ++h) {
+                            float f[32];
+                            take(c + 32u * h, f);
+#pragma unroll
+                            for (unsigned j = 0; j < 32; ++j) f[j] *= scale;
+                            stage<T>(staging, h, f);
+                        }
+                        if (a.wide) {
+                            staging_out(&a.out, staging, first + c, t.m + in_tile, 0, a.m);
+                        } else {
+                            __syncwarp();
+                            const unsigned rows = t.m + in_tile < a.m ? min(32u, a.m - t.m - in_tile) : 0u;
+                            T* to = static_cast<T*>(a.gradient) + (u64)(t.m + in_tile) * a.n + first + c;
+                            for (unsigned i = 0; i < rows; ++i) {
+#pragma unroll
+                                for (unsigned h = 0; h < kBlock / 32u; ++h) {
+                                    const unsigned j = lane + 32u * h, at = j * (unsigned)sizeof(T);
+                                    if (c + j >= columns) continue;
+                                    to[(u64)i * a.n + j] = *reinterpret_cast<const T*>(shared + (staging - base) + i * 128u + (((at >> 4) ^ (i & 7u)) << 4) + (at & 15u));
+                                }
+                            }
+                            __syncwarp();
+                        }
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(bar(bars.sums_free[buffer]), 0);
+                n += end - k;
+                k = end;
+            }
+        }
+        if (lane == 0) tma_wait_group_all();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && *failed != 0u) {
+        *static_cast<volatile unsigned*>(a.status) = 1u;
+        store_word_at(smem_addr(&bars.failed), rank ^ 1u, 1u);
+    }
+    __syncwarp();
+    tcgen05_fence_before();
+    cluster_sync();  // nothing of this CTA is read or arrived at by the other any more
+    tcgen05_fence_after();
+    __syncwarp();
+    if (warp == 1) tmem_free_pair(tmem, 2 * kTile);
+    if (*failed != 0u) {
+        spoil<kKind, T>(a, share, rank);
+        if (rank == 1 && threadIdx.x == 0)  // (the last arrival from the first CTA)
+            for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
+    }
+}
+
+struct FinishArgs {
+    void* out;           // rows of n elements
+    const float* slots;
+    float* sums;         // see ProductArgs
+    bool prior, last;
+    const float* header;
+    bool half;
+    unsigned m, n, m_tiles, n_tiles, n_tile, whole_tiles, steps_of_tile, steps, groups;
+    bool n_first;
+};
+
+// Adds the pieces of cut tiles: 32 rows by 128 columns of a tile.
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ FinishArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned columns = a.n_tile / 128u, blocks = 8u * columns, index = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    const unsigned tile = a.whole_tiles + index, from = index * a.steps_of_tile, to = from + a.steps_of_tile;
+    // The pairs whose steps are of this tile, in order; a pair's last tile, if it began before it, is its second piece.
+    const unsigned pair = min(threadIdx.x, kMaxPairs);
+    const unsigned begin = first_step(min(pair, a.groups), a.steps, a.groups), end = first_step(min(pair + 1u, a.groups), a.steps, a.groups);
+    const unsigned before = __syncthreads_count(threadIdx.x < a.groups && end <= from);
+    const unsigned pieces = __syncthreads_count(threadIdx.x < a.groups && end > from && begin < to);
+    if (__syncthreads_or(threadIdx.x < a.groups && begin <= from && end >= to)) return;  // not cut
+    const unsigned row = (block / columns) * 32u + (threadIdx.x & 31u), column = (block % columns) * 128u;
+    __shared__ float turned[32][129];
+    float4 sum[4];
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const unsigned at = (column / 4u + threadIdx.x / 32u) * kTile + row;  // and eight fours of columns further, four times
+    const auto add = [&](const float* piece) {
+#pragma unroll
+        for (unsigned i = 0; i < 4; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(piece)[at + i * 8u * kTile];
+            sum[i].x += v.x;
+            sum[i].y += v.y;
+            sum[i].z += v.z;
+            sum[i].w += v.w;
+        }
+    };
+    if (a.prior) add(a.sums + (u64)tile * kTileFloats);
+#pragma unroll 2
+    for (unsigned p = 0; p < pieces; ++p) {
+        const unsigned pair = before + p, slot = 2u * pair + (from <= first_step(pair, a.steps, a.groups) ? 0u : 1u);
+        add(a.slots + (u64)slot * kTileFloats);
+    }
+    if (!a.last) {
+#pragma unroll
+        for (unsigned i = 0; i < 4; ++i) reinterpret_cast<float4*>(a.sums + (u64)tile * kTileFloats)[at + i * 8u * kTile] = sum[i];
+        return;
+    }
+    const float scale = gradient_scale(a.header, a.half);
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+        float* t = &turned[threadIdx.x & 31u][(threadIdx.x / 32u + 8u * i) * 4u];
+        t[0] = sum[i].x * scale;
+        t[1] = sum[i].y * scale;
+        t[2] = sum[i].z * scale;
+        t[3] = sum[i].w * scale;
+    }
+    __syncthreads();
+    const unsigned along = a.n_first ? a.n_tiles : a.m_tiles, tile_row = tile / along, tile_column = tile - tile_row * along;
+    const unsigned m0 = (a.n_first ? tile_row : tile_column) * kTile + (block / columns) * 32u, n0 = (a.n_first ? tile_column : tile_row) * a.n_tile + column;
+    for (unsigned i = threadIdx.x; i < 32u * 128u; i += 256u) {
+        const unsigned r = i / 128u, c = i % 128u;
+        if (m0 + r < a.m && n0 + c < a.n) static_cast<T*>(a.out)[(u64)(m0 + r) * a.n + n0 + c] = Elem<T>::from_f(turned[r][c]);
+    }
+}
+
+// ---- what stands around the products -----------------------------------------------------------------------
+
+struct JoinArgs {
+    const float2* stats;
+    unsigned rows, parts;
+    const float* picked;  // cross entropy
+    const void* targets;
+    long long target_stride;
+    bool targets64;
+    unsigned long long vocabulary;
+    const float* z;  // distillation: [rows][entries]
+    const float* p;
+    unsigned entries;
+    float temperature, factor;
+    float* top;
+    float* sum;
+    float* valid;
+    float* loss;
+};
+
+// Each row's maximum and sum, and its loss. A CTA takes 32 rows, each of its warps every eighth part of them.
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x / 32u, row = blockIdx.x * 32u + lane;
+    const float low = -__int_as_float(0x7f800000);
+    const float factor = a.factor;
+    const auto merge = [low, factor](float& top, float& sum, float2 v) {
+        const float now = fmaxf(top, v.x), off = now == low ? 0.0f : now;
+        sum = sum * exp2f((top - off) * factor) + v.y * exp2f((v.x - off) * factor);
+        top = now;
+    };
+    float top = low, sum = 0.0f;
+    if (row < a.rows) {
+        unsigned p = warp;
+        for (; p + 24u < a.parts; p += 32u) {
+            float2 v[4];
+#pragma unroll
+            for (unsigned i = 0; i < 4; ++i) v[i] = a.stats[(u64)(p + 8u * i) * a.rows + row];
+#pragma unroll
+            for (unsigned i = 0; i < 4; ++i) merge(top, sum, v[i]);
+        }
+        for (; p < a.parts; p += 8u) merge(top, sum, a.stats[(u64)p * a.rows + row]);
+    }
+    __shared__ float2 all[8][32];
+    __shared__ float2 of_row[32];
+    all[warp][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (warp == 0) {
+        for (unsigned w = 1; w < 8; ++w) merge(top, sum, all[w][lane]);
+        const float log_sum = log2f(sum);
+        of_row[lane] = make_float2(top, log_sum);
+        if (row < a.rows) {
+            a.top[row] = top;
+            a.sum[row] = sum;
+            if (a.entries == 0) {
+                const long long target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
+                const bool bad = target >= (long long)a.vocabulary;
+                a.valid[row] = bad ? nan32() : (target < 0 ? 0.0f : 1.0f);
+                a.loss[row] = bad ? nan32() : (target < 0 ? 0.0f : kLn2 * ((top - a.picked[row]) * factor + log_sum));
+            }
+        }
+    }
+    if (a.entries == 0) return;
+    __syncthreads();
+    for (unsigned r = warp; r < 32u && blockIdx.x * 32u + r < a.rows; r += 8u) {
+        const u64 at = (u64)(blockIdx.x * 32u + r);
+        float loss = 0.0f;
+        for (unsigned k = lane; k < a.entries; k += 32u) {
+            const float p = a.p[at * a.entries + k];
+            if (p != 0.0f) loss += p * (logf(p) + kLn2 * ((of_row[r].x - a.z[at * a.entries + k]) * factor + of_row[r].y));
+        }
+#pragma unroll
+        for (unsigned d = 16; d != 0; d /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, d);
+        const float valid = a.valid[at];
+        if (lane == 0) a.loss[at] = valid == 0.0f ? 0.0f : loss * a.temperature * a.temperature * valid;
+    }
+}
+
+struct SumArgs {
+    const float* losses;
+    const float* valid;
+    unsigned rows;
+    bool mean;
+    float* out;
+    float* count;
+};
+
+// The rows' losses in one, in an order that does not depend on timing.
+__global__ void __launch_bounds__(1024) sum_kernel(const __grid_constant__ SumArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float sum = 0.0f;
+    unsigned count = 0;
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) {
+        sum += a.losses[i];
+        count += a.valid[i] == 0.0f ? 0u : 1u;
+    }
+    __shared__ float sums[32];
+    __shared__ unsigned counts[32];
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if ((threadIdx.x & 31u) == 0) {
+        sums[threadIdx.x / 32u] = sum;
+        counts[threadIdx.x / 32u] = count;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 32u) return;
+    sum = sums[threadIdx.x];
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    count = __reduce_add_sync(0xffffffffu, counts[threadIdx.x]);
+    if (threadIdx.x == 0) {
+        *a.out = a.mean ? sum / fmaxf((float)count, 1.0f) : sum;
+        *a.count = (float)count;
+    }
+}
+
+struct EntriesArgs {
+    const void* x;  // rows at multiples of 16 bytes, but for fp32
+    long long x_stride;
+    const void* weight;
+    long long weight_stride;
+    unsigned rows, width, entries;
+    unsigned long long vocabulary;
+    const void* targets;
+    long long target_strides[2];
+    bool targets64;
+    const void* teacher;
+    int teacher_dtype;
+    long long teacher_strides[2];
+    float temperature;
+    float* z;
+    float* p;
+    float* valid;
+};
+
+__device__ __forceinline__ float load_as_float(const void* p, int dtype, long long at) {
+    if (dtype == 0) return static_cast<const float*>(p)[at];
+    return dtype == 1 ? __half2float(static_cast<const __half*>(p)[at]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
+}
+
+constexpr unsigned kEntryRounds = kMaxTeacherEntries / 32;
+
+// Distillation: the teacher's distribution over its entries, and the student's logits of them. A warp takes a row; reading the words' rows of the matrix
+// bounds it.
+template <typename T>
+__global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ EntriesArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned lane = threadIdx.x & 31u, row = blockIdx.x * 8u + threadIdx.x / 32u;
+    if (row >= a.rows) return;
+    const float low = -__int_as_float(0x7f800000);
+    long long token[kEntryRounds];
+    float p[kEntryRounds], top = low;
+    bool any = false, bad = false;
+#pragma unroll
+    for (unsigned i = 0; i < kEntryRounds; ++i) {
+        const unsigned k = lane + 32u * i;
+        token[i] = -1;
+        p[i] = low;
+        if (k < a.entries) {
+            token[i] = target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)k * a.target_strides[1]);
+            if (token[i] >= 0) p[i] = load_as_float(a.teacher, a.teacher_dtype, (long long)row * a.teacher_strides[0] + (long long)k * a.teacher_strides[1]);
+            if (p[i] == low) token[i] = -1;
+        }
+        any |= token[i] >= 0;
+        if (token[i] >= (long long)a.vocabulary) {
+            bad = true;
+            token[i] = -1;
+        }
+        top = fmaxf(top, p[i]);
+    }
+    any = __any_sync(0xffffffffu, any);
+    bad = __any_sync(0xffffffffu, bad);
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float sum = 0.0f;
+#pragma unroll
+    for (unsigned i = 0; i < kEntryRounds; ++i) {
+        p[i] = p[i] == low ? 0.0f : expf((p[i] - top) / a.temperature);
+        sum += p[i];
+    }
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) a.valid[row] = bad ? nan32() : (any ? 1.0f : 0.0f);
+    const u64 out = (u64)row * a.entries;
+    const T* x = static_cast<const T*>(a.x) + (long long)row * a.x_stride;
+#pragma unroll
+    for (unsigned i = 0; i < kEntryRounds; ++i) {
+        if (32u * i >= a.entries) break;
+        const unsigned k = lane + 32u * i;
+        if (k < a.entries) a.p[out + k] = any ? p[i] / sum : 0.0f;
+        float z = 0.0f;  // of this lane's entry
+        constexpr unsigned kAtOnce = 4;
+        const unsigned there = min(32u, a.entries - 32u * i);
+        for (unsigned e = 0; e < there; e += kAtOnce) {
+            const T* w[kAtOnce];
+            float dot[kAtOnce] = {};
+#pragma unroll
+            for (unsigned j = 0; j < kAtOnce; ++j) {
+                const long long t = __shfl_sync(0xffffffffu, token[i], e + j);
+                w[j] = t >= 0 ? static_cast<const T*>(a.weight) + t * a.weight_stride : nullptr;
+            }
+            if constexpr (sizeof(T) == 4) {
+                for (unsigned h = lane; h < a.width; h += 32u) {
+                    const float v = x[h];
+#pragma unroll
+                    for (unsigned j = 0; j < kAtOnce; ++j) dot[j] += w[j] != nullptr ? v * w[j][h] : 0.0f;
+                }
+            } else {
+                for (unsigned h = lane * 8u; h < a.width; h += 256u) {
+                    const unsigned n = min(8u, a.width - h);  // (what lies behind a row may be anything)
+                    const uint4 nothing = make_uint4(0u, 0u, 0u, 0u);
+                    uint4 xs = *reinterpret_cast<const uint4*>(x + h), ws[kAtOnce];
+#pragma unroll
+                    for (unsigned j = 0; j < kAtOnce; ++j) ws[j] = w[j] != nullptr ? *reinterpret_cast<const uint4*>(w[j] + h) : nothing;
+                    float v[8], u[8];
+                    Wide<T>::unpack(xs, v);
+#pragma unroll
+                    for (unsigned j = 0; j < kAtOnce; ++j) {
+                        Wide<T>::unpack(ws[j], u);
+                        if (n == 8u) {
+#pragma unroll
+                            for (unsigned q = 0; q < 8; ++q) dot[j] += v[q] * u[q];
+                        } else {
+#pragma unroll
+                            for (unsigned q = 0; q < 8; ++q) dot[j] += q < n ? v[q] * u[q] : 0.0f;
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (unsigned j = 0; j < kAtOnce; ++j) {
+#pragma unroll
+                for (unsigned d = 16; d != 0; d /= 2) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
+                if (lane == e + j) z = dot[j];
+            }
+        }
+        if (k < a.entries) a.z[out + k] = z;
+    }
+}
+
+struct HeaderArgs {
+    const float* loss_grad;
+    long long loss_grad_stride;
+    const float* valid;
+    const float* count;  // of a mean, or null
+    unsigned rows;       // 0: one loss for all rows
+    float temperature;
+    float* header;
+};
+
+// max |c| of the rows, c itself where they share it.
+__global__ void __launch_bounds__(1024) header_kernel(const __grid_constant__ HeaderArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.rows == 0) {
+        if (threadIdx.x == 0) {
+            a.header[0] = a.loss_grad[0] * a.temperature / (a.count != nullptr ? fmaxf(*a.count, 1.0f) : 1.0f);
+            a.header[1] = 0.0f;
+        }
+        return;
+    }
+    unsigned most = 0;  // (of magnitudes as whole numbers: NaN is above infinity)
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) {
+        const float valid = a.valid[i];
+        const unsigned bits = __float_as_uint(a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature) & 0x7fffffffu;
+        most = max(most, valid == 0.0f ? 0u : bits);
+    }
+    __shared__ unsigned all[32];
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = most;
+    __syncthreads();
+    if (threadIdx.x >= 32u) return;
+    most = __reduce_max_sync(0xffffffffu, all[threadIdx.x]);
+    if (threadIdx.x == 0) {
+        a.header[0] = __uint_as_float(most);
+        a.header[1] = 0.0f;
+    }
+}
+
+struct FixArgs {
+    void* probs;  // [parts][rows][pitch]
+    unsigned rows, pitch, entries;
+    long long first, columns;  // of the vocabulary
+    const void* targets;
+    long long target_strides[2];
+    bool targets64;
+    const float* z;
+    const float* p;
+    const float* top;
+    const float* sum;
+    const float* valid;
+    const float* loss_grad;
+    long long loss_grad_stride;
+    float temperature, factor;
+    const float* header;
+};
+
+// Distillation: the elements of P that the teacher has entries of. A warp takes a row; entries of the same word write the same.
+template <typename T>
+__global__ void __launch_bounds__(256) fix_kernel(const __grid_constant__ FixArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned lane = threadIdx.x & 31u, row = blockIdx.x * 8u + threadIdx.x / 32u;
+    if (row >= a.rows) return;
+    const float weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (std::is_same_v<T, __half> ? kHalfScale : 1.0f);
+    const float top = a.top[row], share_of_sum = weight / a.sum[row];
+    long long token[kEntryRounds];
+    float p[kEntryRounds];
+#pragma unroll
+    for (unsigned i = 0; i < kEntryRounds; ++i) {
+        const unsigned k = lane + 32u * i;
+        token[i] = k < a.entries ? target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)k * a.target_strides[1]) : -1;
+        p[i] = k < a.entries ? a.p[(u64)row * a.entries + k] : 0.0f;
+        if (p[i] == 0.0f) token[i] = -1;
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kEntryRounds; ++i) {
+        if (32u * i >= a.entries) break;
+        const long long column = token[i] - a.first;
+        const bool here = token[i] >= 0 && column >= 0 && column < a.columns;
+        if (!__any_sync(0xffffffffu, here)) continue;
+        float all = 0.0f;
+#pragma unroll
+        for (unsigned j = 0; j < kEntryRounds; ++j) {
+            if (32u * j >= a.entries) break;
+            for (unsigned e = 0; e < min(32u, a.entries - 32u * j); ++e) {
+                const long long other = __shfl_sync(0xffffffffu, token[j], e);
+                const float q = __shfl_sync(0xffffffffu, p[j], e);
+                all += other == token[i] ? q : 0.0f;
+            }
+        }
+        if (!here) continue;
+        float v = weight == 0.0f ? 0.0f : share_of_sum * exp2_fast((a.z[(u64)row * a.entries + lane + 32u * i] - top) * a.factor) - weight * all;
+        const u64 at = (u64)row * a.pitch + (u64)column;
+        if constexpr (sizeof(T) == 2) {
+            static_cast<T*>(a.probs)[at] = Elem<T>::from_f(v);
+        } else {
+#pragma unroll
+            for (unsigned part = 0; part < 3; ++part) {
+                const unsigned cut = __float_as_uint(v) >> 16;
+                v -= __uint_as_float(cut << 16);
+                static_cast<unsigned short*>(a.probs)[(u64)part * a.rows * a.pitch + at] = (unsigned short)cut;
+            }
+        }
+    }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------
+
+int current_device() {
+    int device = 0;
+    B2_CUDA(cudaGetDevice(&device));
+    return device;
+}
+
+template <Kind kKind>
+const void* kernel_of(DType dtype) {
+    switch (dtype) {
+        case DType::Float: return (const void*)product_kernel<kKind, float>;
+        case DType::Float16: return (const void*)product_kernel<kKind, __half>;
+        default: return (const void*)product_kernel<kKind, __nv_bfloat16>;
+    }
+}
+const void* kernel_of(Kind kind, DType dtype) {
+    switch (kind) {
+        case Kind::Stats: return kernel_of<Kind::Stats>(dtype);
+        case Kind::Probs: return kernel_of<Kind::Probs>(dtype);
+        case Kind::WeightGrad: return kernel_of<Kind::WeightGrad>(dtype);
+        default: return kernel_of<Kind::InputGrad>(dtype);
+    }
+}
+
+// Pairs of CTAs that run at once on `device` (where GPCs have odd numbers of SMs, fewer than half the SMs). The kernels' shared memory is asked for once.
+unsigned pairs_of_device(int device) {
+    static std::mutex mutex;
+    static unsigned known[64] = {};
+    std::lock_guard<std::mutex> lock(mutex);
+    if (device >= 0 && device < 64 && known[device] != 0) return known[device];
+    for (Kind kind : {Kind::Stats, Kind::Probs, Kind::WeightGrad, Kind::InputGrad})
+        for (DType dtype : {DType::Float, DType::Float16, DType::BFloat16})
+            B2_CUDA(cudaFuncSetAttribute(kernel_of(kind, dtype), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(2 * kMaxPairs);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kShared;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    int clusters = 0;
+    B2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel_of(Kind::Stats, DType::BFloat16), &config));
+    const unsigned pairs = std::min(kMaxPairs, (unsigned)std::max(1, clusters));
+    if (device >= 0 && device < 64) known[device] = pairs;
+    return pairs;
+}
+
+// How the pairs share the tiles of one product.
+struct Tiling {
+    unsigned m_tiles = 0, n_tiles = 0, n_tile = kTile, parts = 1, steps_of_part = 0, steps_of_tile = 0, pairs = 0, waves = 0, steps = 0, groups = 1;
+    bool cut = false, summed = false;  // pieces; sums in memory at all
+};
+
+Tiling tiling_of(u64 m, u64 n, u64 summed, unsigned parts, unsigned n_tile, bool may_cut, unsigned device_pairs) {
+    Tiling t;
+    t.parts = parts;
+    t.n_tile = n_tile;
+    const u64 m_tiles = (m + kTile - 1) / kTile, n_tiles = (n + n_tile - 1) / n_tile, steps = (summed + kStep - 1) / kStep;
+    const u64 tiles = m_tiles * n_tiles, steps_of_tile = steps * (parts > 1 ? 6 : 1);
+    B2_REQUIRE(steps_of_tile < (1ull << 31) && tiles < (1ull << 31) && tiles * steps_of_tile < (1ull << 31), "too many tokens, words and columns for one call");
+    t.m_tiles = (unsigned)m_tiles;
+    t.n_tiles = (unsigned)n_tiles;
+    t.steps_of_part = (unsigned)steps;
+    t.steps_of_tile = (unsigned)steps_of_tile;
+    // A pair for each tile; where they may be cut, for every eight steps of one.
+    t.pairs = (unsigned)std::min<u64>(device_pairs, may_cut ? std::max(tiles, tiles * steps_of_tile / 8) : tiles);
+    t.waves = (unsigned)tiles / t.pairs;
+    const unsigned left = (unsigned)tiles - t.waves * t.pairs;
+    t.steps = left * t.steps_of_tile;
+    // The tiles that are left are cut where that saves every pair more than eight steps, which is what writing and adding pieces costs.
+    t.groups = t.pairs;
+    if (!may_cut || t.steps_of_tile < 8 + t.steps / t.pairs) t.groups = std::max(1u, left);
+    if (t.waves == 0) t.pairs = t.groups;
+    for (unsigned i = 1; i < t.groups && left != 0; ++i) t.cut |= first_step(i, t.steps, t.groups) % t.steps_of_tile != 0;
+    t.summed = t.cut || t.steps_of_tile > (parts > 1 ? 6 * kChunkSteps : kLongSteps);
+    return t;
+}
+
+constexpr std::size_t kProbsBytes = 512ull << 20;  // of a piece of the vocabulary, unless that has fewer than kLeastPiece words
+constexpr u64 kLeastPiece = 4096;
+
+std::size_t padded(std::size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// What a call needs of its workspace, and where.
+struct Plan {
+    unsigned parts = 1;
+    bool copy_x = false, copy_weight = false;
+    std::size_t pitch = 0;  // elements of a row of the copies
+    unsigned device_pairs = 0;
+    u64 piece = 0, pieces = 1;  // words of the vocabulary
+    unsigned n_tile = kTile;
+    std::size_t x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
+};
+
+bool readable(const void* p, long long stride, std::size_t columns, std::size_t rows, std::size_t element) {
+    return reinterpret_cast<std::uintptr_t>(p) % 16 == 0 && (rows <= 1 || (stride * (long long)element % 16 == 0 && stride >= (long long)columns));
+}
+
+// 128 columns of a gradient to a tile instead of 256, where that leaves fewer of them empty.
+unsigned n_tile_of(std::size_t width) { return (width + 127) / 128 * 128 < (width + 255) / 256 * 256 && width <= 640 ? 128u : 256u; }
+
+Plan plan_of(const VocabularyLossCall& c, bool gradient) {
+    Plan p;
+    const std::size_t e = dtype_size(c.dtype), t = c.tokens, v = c.vocabulary;
+    p.parts = c.dtype == DType::Float ? 3 : 1;
+    p.device_pairs = pairs_of_device(current_device());
+    p.pitch = (c.width + 7) / 8 * 8;
+    p.copy_x = c.dtype == DType::Float || !readable(c.x, c.x_stride, c.width, t, e);
+    p.copy_weight = c.dtype == DType::Float || !readable(c.weight, c.weight_stride, c.width, v, e);
+    std::size_t at = 0;
+    const auto take = [&](std::size_t bytes) {
+        const std::size_t here = at;
+        at += padded(bytes);
+        return here;
+    };
+    p.x_at = take(p.copy_x ? p.parts * t * p.pitch * 2 : 0);
+    p.weight_at = take(p.copy_weight ? p.parts * v * p.pitch * 2 : 0);
+    bool summed = false;
+    const auto look = [&](u64 m, u64 n, u64 k, unsigned n_tile, bool may_cut) { summed |= tiling_of(m, n, k, p.parts, n_tile, may_cut, p.device_pairs).summed; };
+    if (!gradient) {
+        p.stats_at = take((v + kTile - 1) / kTile * 2 * t * sizeof(float2));
+        p.picked_at = take(t * sizeof(float));
+        p.losses_at = take(t * sizeof(float));
+        look(t, v, c.width, kTile, false);
+    } else {
+        const u64 tiles = (v + kTile - 1) / kTile, bytes = (u64)p.parts * t * 2;
+        const u64 most = std::max<u64>(std::max<u64>(kProbsBytes / bytes, kLeastPiece) / kTile, 1);
+        p.pieces = (tiles + most - 1) / most;
+        p.piece = (tiles + p.pieces - 1) / p.pieces * kTile;
+        p.pieces = (v + p.piece - 1) / p.piece;
+        p.n_tile = n_tile_of(c.width);
+        p.header_at = take(2 * sizeof(float));
+        p.probs_at = take(bytes * p.piece);
+        const u64 rest = v - (p.pieces - 1) * p.piece;
+        if (c.x_grad != nullptr && p.pieces > 1)
+            p.sums_at = take((t + kTile - 1) / kTile * ((c.width + p.n_tile - 1) / p.n_tile) * kTileFloats * sizeof(float));
+        for (const u64 words : {p.piece, rest}) {
+            look(t, words, c.width, kTile, false);
+            if (c.weight_grad != nullptr) look(words, c.width, t, p.n_tile, true);
+            if (c.x_grad != nullptr) look(t, c.width, words, p.n_tile, true);
+        }
+    }
+    p.slots_at = take(summed ? (std::size_t)2 * p.device_pairs * kTileFloats * sizeof(float) : 0);
+    p.bytes = at;
+    return p;
+}
+
+// A matrix as the tensor cores read it.
+struct Operand {
+    const void* data = nullptr;
+    u64 columns = 0, rows = 0, row_bytes = 0;
+};
+
+CUtensorMap map_of(DType dtype, const Operand& o, unsigned parts, unsigned box_columns, unsigned box_rows) {
+    CUtensorMap m;
+    const auto encode = cu::api().TensorMapEncodeTiled;
+    if (encode == nullptr) throw std::runtime_error("the driver does not export cuTensorMapEncodeTiled");
+    const CUtensorMapDataType type = dtype == DType::Float     ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : dtype == DType::Float16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t extent[3] = {o.columns, o.rows, parts}, strides[2] = {o.row_bytes, o.row_bytes * o.rows};
+    const cuuint32_t box[3] = {box_columns, box_rows, 1}, element_strides[3] = {1, 1, 1};
+    cu::check(encode(&m, type, 3, const_cast<void*>(o.data), extent, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+              "tensor map of an operand");
+    return m;
+}
+
+void launch_product(Kind kind, const VocabularyLossCall& c, const Tiling& t, ProductArgs& a, u64 m, u64 n) {
+    a.m = (unsigned)m;
+    a.n = (unsigned)n;
+    a.m_tiles = t.m_tiles;
+    a.n_tiles = t.n_tiles;
+    a.n_tile = t.n_tile;
+    a.parts = t.parts;
+    a.steps_of_part = t.steps_of_part;
+    a.steps_of_tile = t.steps_of_tile;
+    a.pairs = t.pairs;
+    a.waves = t.waves;
+    a.steps = t.steps;
+    a.groups = t.groups;
+    a.n_first = kind == Kind::WeightGrad || kind == Kind::InputGrad;
+    a.status = wait_status_word(WaitsOf::VocabularyLoss, current_device());
+    a.wait_ns = c.wait_ns;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(2 * t.pairs);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kShared;
+    config.stream = c.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 2;
+    void* arguments[1] = {&a};
+    B2_CUDA(cudaLaunchKernelExC(&config, kernel_of(kind, c.dtype), arguments));
+}
+
+// The pieces of a gradient's cut tiles.
+template <typename T>
+void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) {
+    if (!t.cut) return;
+    FinishArgs f;
+    f.out = a.gradient;
+    f.slots = a.slots;
+    f.sums = a.sums;
+    f.prior = a.prior;
+    f.last = a.last;
+    f.header = a.header;
+    f.half = std::is_same_v<T, __half>;
+    f.m = a.m;
+    f.n = a.n;
+    f.m_tiles = t.m_tiles;
+    f.n_tiles = t.n_tiles;
+    f.n_tile = t.n_tile;
+    f.whole_tiles = t.waves * t.pairs;
+    f.steps_of_tile = t.steps_of_tile;
+    f.steps = t.steps;
+    f.groups = t.groups;
+    f.n_first = a.n_first;
+    const unsigned left = t.steps / t.steps_of_tile;
+    B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<T>, dim3(left * 8 * (t.n_tile / 128)), 256, 0, c.stream, f));
+}
+
+struct Kept {
+    float *top, *sum, *valid, *count, *z, *p;
+};
+Kept kept_of(const VocabularyLossCall& c) {
+    Kept k;
+    k.top = c.kept;
+    k.sum = k.top + c.tokens;
+    k.valid = k.sum + c.tokens;
+    k.count = k.valid + c.tokens;
+    k.z = k.count + 1;
+    k.p = k.z + c.tokens * (std::size_t)c.entries;
+    return k;
+}
+
+constexpr const char* kTooLarge = "an operand is too large for one call";
+
+// x and the matrix as the tensor cores read them, copied where they have to be.
+template <typename T>
+void operands(const VocabularyLossCall& c, const Plan& p, Operand* x, Operand* w) {
+    char* workspace = static_cast<char*>(c.workspace);
+    // (The stride of a single row is not looked at, but must be a multiple of 16 bytes all the same.)
+    *x = {c.x, c.width, c.tokens, (c.tokens > 1 ? (u64)c.x_stride : (u64)p.pitch) * sizeof(T)};
+    *w = {c.weight, c.width, c.vocabulary, (c.vocabulary > 1 ? (u64)c.weight_stride : (u64)p.pitch) * sizeof(T)};
+    if (p.copy_x) {
+        lay_out<T>(c.x, c.x_stride, c.tokens, c.width, p.pitch, workspace + p.x_at, c.stream, kTooLarge);
+        *x = {workspace + p.x_at, c.width, c.tokens, p.pitch * 2};
+    }
+    if (p.copy_weight) {
+        lay_out<T>(c.weight, c.weight_stride, c.vocabulary, c.width, p.pitch, workspace + p.weight_at, c.stream, kTooLarge);
+        *w = {workspace + p.weight_at, c.width, c.vocabulary, p.pitch * 2};
+    }
+}
+
+template <typename T>
+constexpr DType operand_type() { return std::is_same_v<T, __half> ? DType::Float16 : DType::BFloat16; }
+
+void logits_arguments(const VocabularyLossCall& c, ProductArgs& a) {
+    a.factor = kLog2E / c.temperature;
+    a.hard = !c.distillation;
+    a.targets = c.targets;
+    a.target_stride = c.target_strides[0];
+    a.targets64 = c.targets64;
+    a.temperature = c.temperature;
+}
+
+template <typename T>
+void loss(const VocabularyLossCall& c, const Plan& p) {
+    char* workspace = static_cast<char*>(c.workspace);
+    const Kept kept = kept_of(c);
+    Operand x, w;
+    operands<T>(c, p, &x, &w);
+    if (c.distillation) {
+        EntriesArgs e;
+        const bool copied = sizeof(T) == 2;  // (fp32 reads the original)
+        e.x = copied ? x.data : c.x;
+        e.x_stride = copied && p.copy_x ? (long long)p.pitch : c.x_stride;
+        e.weight = copied ? w.data : c.weight;
+        e.weight_stride = copied && p.copy_weight ? (long long)p.pitch : c.weight_stride;
+        e.rows = (unsigned)c.tokens;
+        e.width = (unsigned)c.width;
+        e.entries = (unsigned)c.entries;
+        e.vocabulary = c.vocabulary;
+        e.targets = c.targets;
+        e.targets64 = c.targets64;
+        e.teacher = c.teacher;
+        e.teacher_dtype = static_cast<int>(c.teacher_dtype);
+        for (int i = 0; i < 2; ++i) {
+            e.target_strides[i] = c.target_strides[i];
+            e.teacher_strides[i] = c.teacher_strides[i];
+        }
+        e.temperature = c.temperature;
+        e.z = kept.z;
+        e.p = kept.p;
+        e.valid = kept.valid;
+        B2_CUDA(launch_dependent<EntriesArgs>(entries_kernel<T>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
+    }
+    ProductArgs a = {};
+    a.a = map_of(operand_type<T>(), x, p.parts, kStep, kHalf);
+    a.b = map_of(operand_type<T>(), w, p.parts, kStep, kHalf);
+    logits_arguments(c, a);
+    a.stats = reinterpret_cast<float2*>(workspace + p.stats_at);
+    a.picked = reinterpret_cast<float*>(workspace + p.picked_at);
+    a.slots = reinterpret_cast<float*>(workspace + p.slots_at);
+    const Tiling t = tiling_of(c.tokens, c.vocabulary, c.width, p.parts, kTile, false, p.device_pairs);
+    launch_product(Kind::Stats, c, t, a, c.tokens, c.vocabulary);
+    JoinArgs j;
+    j.stats = a.stats;
+    j.rows = (unsigned)c.tokens;
+    j.parts = 2 * t.n_tiles;
+    j.picked = a.picked;
+    j.targets = c.targets;
+    j.target_stride = c.target_strides[0];
+    j.targets64 = c.targets64;
+    j.vocabulary = c.vocabulary;
+    j.z = kept.z;
+    j.p = kept.p;
+    j.entries = (unsigned)c.entries;
+    j.temperature = c.temperature;
+    j.factor = a.factor;
+    j.top = kept.top;
+    j.sum = kept.sum;
+    j.valid = kept.valid;
+    j.loss = c.reduction == LossReduction::None ? c.loss : reinterpret_cast<float*>(workspace + p.losses_at);
+    B2_CUDA(launch_dependent<JoinArgs>(join_kernel, dim3((unsigned)((c.tokens + 31) / 32)), 256, 0, c.stream, j));
+    if (c.reduction == LossReduction::None) return;
+    SumArgs s;
+    s.losses = j.loss;
+    s.valid = kept.valid;
+    s.rows = (unsigned)c.tokens;
+    s.mean = c.reduction == LossReduction::Mean;
+    s.out = c.loss;
+    s.count = kept.count;
+    B2_CUDA(launch_dependent<SumArgs>(sum_kernel, dim3(1), 1024, 0, c.stream, s));
+}
+
+template <typename T>
+void gradient(const VocabularyLossCall& c, const Plan& p) {
+    char* workspace = static_cast<char*>(c.workspace);
+    const Kept kept = kept_of(c);
+    const bool each = c.reduction == LossReduction::None;
+    float* header = reinterpret_cast<float*>(workspace + p.header_at);
+    HeaderArgs h;
+    h.loss_grad = c.loss_grad;
+    h.loss_grad_stride = c.loss_grad_stride;
+    h.valid = kept.valid;
+    h.count = c.reduction == LossReduction::Mean ? kept.count : nullptr;
+    h.rows = each ? (unsigned)c.tokens : 0;
+    h.temperature = c.temperature;
+    h.header = header;
+    B2_CUDA(launch_dependent<HeaderArgs>(header_kernel, dim3(1), 1024, 0, c.stream, h));
+    Operand x, w;
+    operands<T>(c, p, &x, &w);
+    char* probs = workspace + p.probs_at;
+    for (u64 piece = 0; piece < p.pieces; ++piece) {
+        const u64 first = piece * p.piece, words = std::min<u64>(p.piece, c.vocabulary - first);
+        const Operand probs_of = {probs, p.piece, c.tokens, p.piece * 2};
+        ProductArgs a = {};
+        a.a = map_of(operand_type<T>(), x, p.parts, kStep, kHalf);
+        a.b = map_of(operand_type<T>(), w, p.parts, kStep, kHalf);
+        a.out = map_of(operand_type<T>(), probs_of, p.parts, 64, 32);
+        logits_arguments(c, a);
+        a.b_offset = (unsigned)first;
+        a.top = kept.top;
+        a.sum = kept.sum;
+        a.valid = kept.valid;
+        a.loss_grad = each ? c.loss_grad : nullptr;
+        a.loss_grad_stride = c.loss_grad_stride;
+        a.header = header;
+        a.slots = reinterpret_cast<float*>(workspace + p.slots_at);
+        launch_product(Kind::Probs, c, tiling_of(c.tokens, words, c.width, p.parts, kTile, false, p.device_pairs), a, c.tokens, words);
+        if (c.distillation) {
+            FixArgs f;
+            f.probs = probs;
+            f.rows = (unsigned)c.tokens;
+            f.pitch = (unsigned)p.piece;
+            f.entries = (unsigned)c.entries;
+            f.first = (long long)first;
+            f.columns = (long long)words;
+            f.targets = c.targets;
+            f.target_strides[0] = c.target_strides[0];
+            f.target_strides[1] = c.target_strides[1];
+            f.targets64 = c.targets64;
+            f.z = kept.z;
+            f.p = kept.p;
+            f.top = kept.top;
+            f.sum = kept.sum;
+            f.factor = a.factor;
+            f.valid = kept.valid;
+            f.loss_grad = a.loss_grad;
+            f.loss_grad_stride = a.loss_grad_stride;
+            f.temperature = c.temperature;
+            f.header = header;
+            B2_CUDA(launch_dependent<FixArgs>(fix_kernel<T>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, f));
+        }
+        const unsigned columns = 128 / sizeof(T);
+        const auto gradient_of = [&](void* out, u64 rows) {
+            a.gradient = out;
+            a.wide = c.width * sizeof(T) % 16 == 0 && reinterpret_cast<std::uintptr_t>(out) % 16 == 0;
+            if (a.wide) a.out = map_of(c.dtype, {out, c.width, rows, c.width * sizeof(T)}, 1, columns, 32);
+        };
+        if (c.weight_grad != nullptr) {
+            const Tiling t = tiling_of(words, c.width, c.tokens, p.parts, p.n_tile, true, p.device_pairs);
+            a.a = map_of(operand_type<T>(), probs_of, p.parts, 64, kStep);
+            a.b = map_of(operand_type<T>(), x, p.parts, 64, kStep);
+            a.b_offset = 0;
+            a.sums = nullptr;
+            a.prior = false;
+            a.last = true;
+            gradient_of(static_cast<T*>(c.weight_grad) + first * c.width, words);
+            launch_product(Kind::WeightGrad, c, t, a, words, c.width);
+            finish<T>(c, t, a);
+        }
+        if (c.x_grad != nullptr) {
+            const Tiling t = tiling_of(c.tokens, c.width, words, p.parts, p.n_tile, true, p.device_pairs);
+            a.a = map_of(operand_type<T>(), probs_of, p.parts, kStep, kHalf);
+            a.b = map_of(operand_type<T>(), w, p.parts, 64, kStep);
+            a.b_offset = (unsigned)first;
+            a.sums = p.pieces > 1 ? reinterpret_cast<float*>(workspace + p.sums_at) : nullptr;
+            a.prior = piece != 0;
+            a.last = piece + 1 == p.pieces;
+            gradient_of(c.x_grad, c.tokens);
+            launch_product(Kind::InputGrad, c, t, a, c.tokens, c.width);
+            finish<T>(c, t, a);
+        }
+    }
+}
+
+}  // namespace
+
+std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 3 + 1 + 2 * c.tokens * (std::size_t)c.entries; }
+
+std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient) { return call.tokens == 0 ? 0 : plan_of(call, gradient).bytes; }
+
+void launch_vocabulary_loss(const VocabularyLossCall& c) {
+    if (c.tokens == 0) {
+        if (c.reduction != LossReduction::None) B2_CUDA(cudaMemsetAsync(c.loss, 0, sizeof(float), c.stream));
+        return;
+    }
+    const Plan p = plan_of(c, false);
+    switch (c.dtype) {
+        case DType::Float: return loss<float>(c, p);
+        case DType::Float16: return loss<__half>(c, p);
+        case DType::BFloat16: return loss<__nv_bfloat16>(c, p);
+    }
+}
+
+void launch_vocabulary_loss_gradient(const VocabularyLossCall& c) {
+    if (c.x_grad == nullptr && c.weight_grad == nullptr) return;
+    if (c.tokens == 0) {
+        if (c.weight_grad != nullptr) B2_CUDA(cudaMemsetAsync(c.weight_grad, 0, c.vocabulary * c.width * dtype_size(c.dtype), c.stream));
+        return;
+    }
+    const Plan p = plan_of(c, true);
+    switch (c.dtype) {
+        case DType::Float: return gradient<float>(c, p);
+        case DType::Float16: return gradient<__half>(c, p);
+        case DType::BFloat16: return gradient<__nv_bfloat16>(c, p);
+    }
+}
+
+}  // namespace b200ccl::kernels

@@ -41,6 +41,8 @@
 #include "core/check.h"
 #include "kernels/sm100/block8.cuh"
 #include "kernels/sm100/launch.h"
+#include "kernels/sm100/lay_out.cuh"
+#include "kernels/sm100/wait_status.h"
 #include "kernels/sm100/tcgen05.cuh"
 #include "mem/cu_driver.h"
 
@@ -718,47 +720,6 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     if (output < a.outputs) static_cast<T*>(a.bias_out)[output] = Elem<T>::from_f(sum);
 }
 
-// dY as TMA reads it: rows of `pitch` elements; fp32 in three parts.
-struct LayOutArgs {
-    const char* dy;
-    long long stride;  // bytes
-    char* out;
-    unsigned tokens, outputs;
-    Divisor eights;  // of a row
-};
-
-// A thread takes eight outputs of a token.
-template <typename T>
-__global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ LayOutArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned eights = a.eights.d, i = blockIdx.x * 256u + threadIdx.x, token = a.eights.divide(i), n = (i - token * eights) * 8u;
-    if (token >= a.tokens) return;
-    const T* from = reinterpret_cast<const T*>(a.dy + (long long)token * a.stride) + n;
-    unsigned words[2 * sizeof(T)];
-    load_any<T, 8>(reinterpret_cast<const char*>(from), n < a.outputs ? min(8u, a.outputs - n) : 0u, words);
-    if constexpr (sizeof(T) == 2) {
-        *(reinterpret_cast<uint4*>(a.out) + i) = make_uint4(words[0], words[1], words[2], words[3]);
-    } else {
-        unsigned part[3][4] = {};
-#pragma unroll
-        for (unsigned e = 0; e < 8; ++e) {
-            float rest = __uint_as_float(words[e]);
-            const bool finite = (words[e] & 0x7f800000u) != 0x7f800000u;
-#pragma unroll
-            for (int p = 0; p < 3; ++p) {  // the leading eight bits of what is left, cut off and not rounded: the rest is exact, and nothing overflows
-                const unsigned cut = __float_as_uint(rest) >> 16;
-                rest -= __uint_as_float(cut << 16);
-                const unsigned put = finite ? cut : (p == 0 ? ((words[e] & 0x7fffffffu) > 0x7f800000u ? 0x7fc0u : cut) : 0u);
-                part[p][e / 2u] |= put << (16u * (e & 1u));
-            }
-        }
-        const u64 eight = (u64)a.tokens * eights;
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *(reinterpret_cast<uint4*>(a.out) + p * eight + i) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
-    }
-}
-
 struct Plan {
     bool wide = false;
     unsigned parts = 1, width = kTile, pitch = 0, feature_tiles = 0, output_tiles = 0, steps_of_part = 0, steps_of_tile = 0, steps = 0, pairs = 0, waves = 0, group = 1, groups = 1;
@@ -868,41 +829,13 @@ Plan plan_of(const WeightGradCall& c) {
     return p;
 }
 
-// A word of host memory for each device, that a kernel whose wait ran out writes to.
-constexpr int kDevices = 64;
-std::atomic<unsigned*> status_words{nullptr};
-unsigned* status_word(int device) {
-    static unsigned* words = [] {
-        // (Allocating is allowed beside a capture: nothing of it belongs to the graph.)
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        B2_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-        void* p = nullptr;
-        const cudaError_t st = cudaHostAlloc(&p, kDevices * sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable);
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        B2_CUDA(st);
-        std::fill_n(static_cast<unsigned*>(p), kDevices, 0u);
-        status_words.store(static_cast<unsigned*>(p));
-        return static_cast<unsigned*>(p);
-    }();
-    return words + device % kDevices;
-}
-
 template <typename T>
 void launch(const WeightGradCall& c, const Plan& p) {
     char* workspace = static_cast<char*>(c.workspace);
     const void* dy = c.dy;
     u64 row_bytes = (u64)c.stride * sizeof(T);
     if (p.copied) {
-        LayOutArgs l;
-        l.dy = static_cast<const char*>(c.dy);
-        l.stride = c.stride * (long long)sizeof(T);
-        l.out = workspace;
-        l.tokens = (unsigned)c.tokens;
-        l.outputs = (unsigned)c.outputs;
-        l.eights = Divisor(p.pitch / 8);
-        const u64 eights = (u64)c.tokens * (p.pitch / 8), ctas = (eights + 255) / 256;
-        B2_REQUIRE(eights < (1ull << 31), "weight_grad8: dy is too large for one call");
-        B2_CUDA(launch_dependent<LayOutArgs>(lay_out_kernel<T>, dim3((unsigned)ctas), 256, 0, c.stream, l));
+        lay_out<T>(c.dy, c.stride, c.tokens, c.outputs, p.pitch, workspace, c.stream, "weight_grad8: dy is too large for one call");
         dy = workspace;
         row_bytes = (u64)p.pitch * 2;
     }
@@ -925,7 +858,7 @@ void launch(const WeightGradCall& c, const Plan& p) {
     a.pieces = reinterpret_cast<float*>(workspace + p.pieces_at);
     a.bias_out = p.direct ? c.bias_grad : nullptr;
     a.bias = c.bias_grad != nullptr && !p.direct ? reinterpret_cast<float*>(workspace + p.bias_at) : nullptr;
-    a.status = status_word(current_device());
+    a.status = wait_status_word(WaitsOf::WeightGrad, current_device());
     a.wait_ns = c.wait_ns;
     a.tokens = (unsigned)c.tokens;
     a.inputs = (unsigned)c.inputs;
@@ -1002,12 +935,6 @@ void launch_weight_grad(const WeightGradCall& c) {
         case DType::Float16: return launch<__half>(c, p);
         case DType::BFloat16: return launch<__nv_bfloat16>(c, p);
     }
-}
-
-bool weight_grad_failed(int device) {
-    B2_REQUIRE(device >= 0, "no such device");
-    unsigned* words = status_words.load();  // (null before the first call of all)
-    return words != nullptr && __atomic_exchange_n(words + device % kDevices, 0u, __ATOMIC_RELAXED) != 0u;
 }
 
 }  // namespace b200ccl::kernels

@@ -28,7 +28,5 @@ std::size_t weight_grad_workspace(const WeightGradCall& call);
 // weight_grad[n][k] = sum over tokens of dy[t][n] * x^[t][k], bias_grad[n] = sum of dy[t][n]. Throws std::runtime_error on a failed launch. Where a wait
 // inside the kernel runs out, what depends on it is NaN.
 void launch_weight_grad(const WeightGradCall& call);
-// Whether that happened on `device` since this was last asked.
-bool weight_grad_failed(int device);
 
 }  // namespace b200ccl::kernels

@@ -309,7 +309,7 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_b200ccl_torch", nullptr, -1, 
 PyMODINIT_FUNC PyInit__b200ccl_torch() {
     PyObject* m = PyModule_Create(&module_def);
     if (m == nullptr) return nullptr;
-    if (PyModule_AddFunctions(m, b200ccl::python::train_methods) < 0) {
+    if (PyModule_AddFunctions(m, b200ccl::python::train_methods) < 0 || PyModule_AddFunctions(m, b200ccl::python::vocabulary_methods) < 0) {
         Py_DECREF(m);
         return nullptr;
     }
