@@ -586,12 +586,12 @@ struct FinishArgs {
     bool n_first;
 };
 
-// Adds the pieces of cut tiles: 32 rows by 128 columns of a tile.
+// Adds the pieces of cut tiles: 32 rows by 32 columns of a tile for a CTA (a tile that all pairs share has 74 pieces, and few CTAs took 51 us for two of them).
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ FinishArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned columns = a.n_tile / 128u, blocks = 8u * columns, index = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    const unsigned columns = a.n_tile / 32u, blocks = 8u * columns, index = blockIdx.x / blocks, block = blockIdx.x % blocks;
     const unsigned tile = a.whole_tiles + index, from = index * a.steps_of_tile, to = from + a.steps_of_tile;
     // The pairs whose steps are of this tile, in order; a pair's last tile, if it began before it, is its second piece.
     const unsigned pair = min(threadIdx.x, kMaxPairs);
@@ -599,49 +599,44 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     const unsigned before = __syncthreads_count(threadIdx.x < a.groups && end <= from);
     const unsigned pieces = __syncthreads_count(threadIdx.x < a.groups && end > from && begin < to);
     if (__syncthreads_or(threadIdx.x < a.groups && begin <= from && end >= to)) return;  // not cut
-    const unsigned row = (block / columns) * 32u + (threadIdx.x & 31u), column = (block % columns) * 128u;
-    __shared__ float turned[32][129];
-    float4 sum[4];
-#pragma unroll
-    for (unsigned i = 0; i < 4; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const unsigned at = (column / 4u + threadIdx.x / 32u) * kTile + row;  // and eight fours of columns further, four times
-    const auto add = [&](const float* piece) {
-#pragma unroll
-        for (unsigned i = 0; i < 4; ++i) {
-            const float4 v = reinterpret_cast<const float4*>(piece)[at + i * 8u * kTile];
-            sum[i].x += v.x;
-            sum[i].y += v.y;
-            sum[i].z += v.z;
-            sum[i].w += v.w;
-        }
+    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x / 32u, row0 = block / columns * 32u, column0 = block % columns * 32u;
+    const unsigned at = (column0 / 4u + warp) * kTile + row0 + lane;  // four columns of a row
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&sum](float4 v) {
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
     };
-    if (a.prior) add(a.sums + (u64)tile * kTileFloats);
-#pragma unroll 2
-    for (unsigned p = 0; p < pieces; ++p) {
-        const unsigned pair = before + p, slot = 2u * pair + (from <= first_step(pair, a.steps, a.groups) ? 0u : 1u);
-        add(a.slots + (u64)slot * kTileFloats);
+    if (a.prior) add(reinterpret_cast<const float4*>(a.sums + (u64)tile * kTileFloats)[at]);
+    constexpr unsigned kAtOnce = 8;
+    for (unsigned p = 0; p < pieces; p += kAtOnce) {
+        float4 v[kAtOnce];
+#pragma unroll
+        for (unsigned i = 0; i < kAtOnce; ++i) {
+            const unsigned piece = before + p + i, slot = 2u * piece + (i + p == 0 && from > first_step(piece, a.steps, a.groups) ? 1u : 0u);
+            v[i] = p + i < pieces ? reinterpret_cast<const float4*>(a.slots + (u64)slot * kTileFloats)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (unsigned i = 0; i < kAtOnce; ++i) add(v[i]);
     }
     if (!a.last) {
-#pragma unroll
-        for (unsigned i = 0; i < 4; ++i) reinterpret_cast<float4*>(a.sums + (u64)tile * kTileFloats)[at + i * 8u * kTile] = sum[i];
+        reinterpret_cast<float4*>(a.sums + (u64)tile * kTileFloats)[at] = sum;
         return;
     }
     const float scale = gradient_scale(a.header, a.half);
-#pragma unroll
-    for (unsigned i = 0; i < 4; ++i) {
-        float* t = &turned[threadIdx.x & 31u][(threadIdx.x / 32u + 8u * i) * 4u];
-        t[0] = sum[i].x * scale;
-        t[1] = sum[i].y * scale;
-        t[2] = sum[i].z * scale;
-        t[3] = sum[i].w * scale;
-    }
+    __shared__ float turned[32][33];
+    float* t = &turned[lane][warp * 4u];
+    t[0] = sum.x * scale;
+    t[1] = sum.y * scale;
+    t[2] = sum.z * scale;
+    t[3] = sum.w * scale;
     __syncthreads();
     const unsigned along = a.n_first ? a.n_tiles : a.m_tiles, tile_row = tile / along, tile_column = tile - tile_row * along;
-    const unsigned m0 = (a.n_first ? tile_row : tile_column) * kTile + (block / columns) * 32u, n0 = (a.n_first ? tile_column : tile_row) * a.n_tile + column;
-    for (unsigned i = threadIdx.x; i < 32u * 128u; i += 256u) {
-        const unsigned r = i / 128u, c = i % 128u;
-        if (m0 + r < a.m && n0 + c < a.n) static_cast<T*>(a.out)[(u64)(m0 + r) * a.n + n0 + c] = Elem<T>::from_f(turned[r][c]);
-    }
+    const unsigned m0 = (a.n_first ? tile_row : tile_column) * kTile + row0, n = (a.n_first ? tile_column : tile_row) * a.n_tile + column0 + lane;
+#pragma unroll
+    for (unsigned r = warp; r < 32u; r += 8u)
+        if (m0 + r < a.m && n < a.n) static_cast<T*>(a.out)[(u64)(m0 + r) * a.n + n] = Elem<T>::from_f(turned[r][lane]);
 }
 
 // ---- what stands around the products -----------------------------------------------------------------------
@@ -664,10 +659,12 @@ struct JoinArgs {
     float* loss;
 };
 
-// Each row's maximum and sum, and its loss. A CTA takes 32 rows, each of its warps every eighth part of them.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinArgs a) {
+// Each row's maximum and sum, and its loss. A CTA takes 32 rows, each of its warps every 32nd part of them (1024 rows of 394 parts: eight
+// warps took 12 us).
+__global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ JoinArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr unsigned kWarps = 32;
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x / 32u, row = blockIdx.x * 32u + lane;
     const float low = -__int_as_float(0x7f800000);
     const float factor = a.factor;
@@ -678,22 +675,20 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinA
     };
     float top = low, sum = 0.0f;
     if (row < a.rows) {
-        unsigned p = warp;
-        for (; p + 24u < a.parts; p += 32u) {
+        for (unsigned p = warp; p < a.parts; p += 4u * kWarps) {
             float2 v[4];
 #pragma unroll
-            for (unsigned i = 0; i < 4; ++i) v[i] = a.stats[(u64)(p + 8u * i) * a.rows + row];
+            for (unsigned i = 0; i < 4; ++i) v[i] = p + kWarps * i < a.parts ? a.stats[(u64)(p + kWarps * i) * a.rows + row] : make_float2(low, 0.0f);
 #pragma unroll
             for (unsigned i = 0; i < 4; ++i) merge(top, sum, v[i]);
         }
-        for (; p < a.parts; p += 8u) merge(top, sum, a.stats[(u64)p * a.rows + row]);
     }
-    __shared__ float2 all[8][32];
+    __shared__ float2 all[kWarps][33];
     __shared__ float2 of_row[32];
     all[warp][lane] = make_float2(top, sum);
     __syncthreads();
     if (warp == 0) {
-        for (unsigned w = 1; w < 8; ++w) merge(top, sum, all[w][lane]);
+        for (unsigned w = 1; w < kWarps; ++w) merge(top, sum, all[w][lane]);
         const float log_sum = log2f(sum);
         of_row[lane] = make_float2(top, log_sum);
         if (row < a.rows) {
@@ -709,12 +704,12 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinA
     }
     if (a.entries == 0) return;
     __syncthreads();
-    for (unsigned r = warp; r < 32u && blockIdx.x * 32u + r < a.rows; r += 8u) {
-        const u64 at = (u64)(blockIdx.x * 32u + r);
+    const u64 at = (u64)blockIdx.x * 32u + warp;  // a warp for each row
+    if (at < a.rows) {
         float loss = 0.0f;
         for (unsigned k = lane; k < a.entries; k += 32u) {
             const float p = a.p[at * a.entries + k];
-            if (p != 0.0f) loss += p * (logf(p) + kLn2 * ((of_row[r].x - a.z[at * a.entries + k]) * factor + of_row[r].y));
+            if (p != 0.0f) loss += p * (logf(p) + kLn2 * ((of_row[warp].x - a.z[at * a.entries + k]) * factor + of_row[warp].y));
         }
 #pragma unroll
         for (unsigned d = 16; d != 0; d /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, d);
@@ -840,7 +835,7 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
         const unsigned k = lane + 32u * i;
         if (k < a.entries) a.p[out + k] = any ? p[i] / sum : 0.0f;
         float z = 0.0f;  // of this lane's entry
-        constexpr unsigned kAtOnce = 4;
+        constexpr unsigned kAtOnce = 8;
         const unsigned there = min(32u, a.entries - 32u * i);
         for (unsigned e = 0; e < there; e += kAtOnce) {
             const T* w[kAtOnce];
@@ -1225,7 +1220,7 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
     f.groups = t.groups;
     f.n_first = a.n_first;
     const unsigned left = t.steps / t.steps_of_tile;
-    B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<T>, dim3(left * 8 * (t.n_tile / 128)), 256, 0, c.stream, f));
+    B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<T>, dim3(left * 8 * (t.n_tile / 32)), 256, 0, c.stream, f));
 }
 
 struct Kept {
@@ -1331,7 +1326,7 @@ void loss(const VocabularyLossCall& c, const Plan& p) {
     j.sum = kept.sum;
     j.valid = kept.valid;
     j.loss = c.reduction == LossReduction::None ? c.loss : reinterpret_cast<float*>(workspace + p.losses_at);
-    B2_CUDA(launch_dependent<JoinArgs>(join_kernel, dim3((unsigned)((c.tokens + 31) / 32)), 256, 0, c.stream, j));
+    B2_CUDA(launch_dependent<JoinArgs>(join_kernel, dim3((unsigned)((c.tokens + 31) / 32)), 1024, 0, c.stream, j));
     if (c.reduction == LossReduction::None) return;
     SumArgs s;
     s.losses = j.loss;
