@@ -5,7 +5,7 @@ stands for no token (the padding of a sequence): it is looked up as zeros, has n
 the vocabulary makes NaN, so that a loss scaler sees it. (Rows that do not count still go through the products: their hidden states must be numbers.)
 
 The logits of 8192 tokens over 50257 words take 1.6 GB in 32 bits, and their gradient as much again. The losses here make them tile by tile on the tensor cores
-and keep one number for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: three of them) of the two products that
+and keep one number for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: two of them) of the two products that
 make the gradients. It needs 512 MB at most for that, or 4096 words of the vocabulary.
 
 CUDA tensors of float32, float16 or bfloat16; calls run on the current stream of the tensors' device. As with the other operators of this package (:mod:`.checkpoint8`)
@@ -36,7 +36,8 @@ def linear_cross_entropy(x, weight, targets, reduction="mean"):
     one of all of them (a mean over the rows that have a target; 0 where none has). ``x``: [..., width], ``targets``: [...]. The loss is float32, gradients have the types of ``x``
     and ``weight``, which are the same. Under autocast both are cast as those of ``linear``.
 
-    What the logits lose is what 32-bit sums lose; the gradient of the logits is rounded to the type of ``x`` before it is multiplied (float32: it is not)."""
+    What the logits lose is what 32-bit sums lose; the gradient of the logits is rounded to the type of ``x`` before it is multiplied. float32: operands have 22 bits, or 2^-39 of
+    the largest element of ``x``, of ``weight`` and of the rows' weights in the loss, where that is more."""
     return load_native_calls().linear_cross_entropy(x, weight, targets, _reduction(reduction))
 
 

@@ -5,8 +5,8 @@
 // atomic additions would.
 //
 // Sorting (sort_kernel) is a matter of latency: a cluster of eight CTAs sorts by eight bits at a time, counts and places of its 256 warps in shared memory and
-// between the CTAs through distributed shared memory. Meanwhile the other clusters of the launch fill the gradient with zeros, which takes longer where the
-// vocabulary is large, so that sorting is free.
+// between the CTAs through distributed shared memory. Meanwhile the rest of the GPU fills the gradient with zeros (fill_kernel), which takes longer where the
+// matrix is large, so that sorting is free. (A CTA of few stores for each 64 KiB: 1.07 GB in 145 us, a loop in as many CTAs as run at once 170 us.)
 // Adding (sum_kernel): the list is cut into chunks, and a group of threads goes through one, 16 bytes of a row for each thread. A token whose rows lie in one chunk is
 // written at once. What crosses a chunk's ends is written as sums of 32 bits, and join_kernel adds them: a token may have any share of the rows.
 #include "kernels/sm100/embedding.h"
@@ -117,8 +117,6 @@ struct SortArgs {
     unsigned count, vocabulary, passes;
     unsigned* keys[2];    // [count]: the last pass writes to the first
     unsigned* places[2];
-    char* gradient;       // to be filled with zeros
-    u64 gradient_bytes;
 };
 
 // Tokens that are none are sorted behind all others.
@@ -133,17 +131,11 @@ __device__ __forceinline__ unsigned load_at_rank(const unsigned* p, unsigned ran
 }
 
 __global__ void __launch_bounds__(kSortThreads) __cluster_dims__(kSortCtas, 1, 1) sort_kernel(const __grid_constant__ SortArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (blockIdx.x >= kSortCtas) {
-        const u64 vectors = a.gradient_bytes / 16u, step = (u64)(gridDim.x - kSortCtas) * kSortThreads;
-        const u64 first = (u64)(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x;
-        for (u64 i = first; i < vectors; i += step) store16_once(a.gradient + i * 16u, make_uint4(0u, 0u, 0u, 0u));
-        if (first < a.gradient_bytes % 16u) a.gradient[vectors * 16u + first] = 0;
-        return;
-    }
-    __shared__ unsigned counts[kSortWarps][kBins];  // of each warp's part of the list, then where its next element of a bin goes
-    __shared__ unsigned totals[kBins];              // of this CTA
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (after the wait: fill_kernel starts then, and what came before the sort is over)
+    __shared__ unsigned counts[kSortWarps][kBins + 1];  // of each warp's part of the list, then where its next element of a bin goes in the CTA's
+    __shared__ unsigned totals[kBins];                  // of this CTA
+    __shared__ unsigned bases[kBins];                   // where its elements of a bin go
     __shared__ unsigned sums[kBins / 32];
     const unsigned rank = cluster_rank(), warp = threadIdx.x / 32u, lane = threadIdx.x & 31u;
     const unsigned each = ((a.count + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31u) / 32u * 32u;
@@ -161,17 +153,26 @@ __global__ void __launch_bounds__(kSortThreads) __cluster_dims__(kSortCtas, 1, 1
             __syncwarp();
         }
         __syncthreads();
+        // Four threads for a bin, each with eight warps.
+        const unsigned bin = threadIdx.x / 4u, part = threadIdx.x & 3u;
         unsigned total = 0;
-        if (threadIdx.x < kBins) {
-            for (unsigned w = 0; w < kSortWarps; ++w) {
-                const unsigned n = counts[w][threadIdx.x];
-                counts[w][threadIdx.x] = total;
-                total += n;
-            }
-            totals[threadIdx.x] = total;
+#pragma unroll
+        for (unsigned w = 0; w < kSortWarps / 4; ++w) {
+            const unsigned n = counts[part * (kSortWarps / 4) + w][bin];
+            counts[part * (kSortWarps / 4) + w][bin] = total;
+            total += n;
         }
+        unsigned scan = total;  // of this thread's and the parts before
+#pragma unroll
+        for (unsigned d = 1; d < 4u; d *= 2u) {
+            const unsigned v = __shfl_up_sync(0xffffffffu, scan, d, 4);
+            scan += part >= d ? v : 0u;
+        }
+#pragma unroll
+        for (unsigned w = 0; w < kSortWarps / 4; ++w) counts[part * (kSortWarps / 4) + w][bin] += scan - total;
+        if (part == 3u) totals[bin] = scan;
         cluster_sync();
-        unsigned before = 0, all = 0, scan = 0;
+        unsigned before = 0, all = 0;
         if (threadIdx.x < kBins) {
 #pragma unroll
             for (unsigned r = 0; r < kSortCtas; ++r) {
@@ -189,28 +190,49 @@ __global__ void __launch_bounds__(kSortThreads) __cluster_dims__(kSortCtas, 1, 1
         }
         __syncthreads();
         if (threadIdx.x < kBins) {
-            for (unsigned w = 0; w < warp; ++w) before += sums[w];
-            before += scan - all;
-            for (unsigned w = 0; w < kSortWarps; ++w) counts[w][threadIdx.x] += before;
+#pragma unroll
+            for (unsigned w = 0; w < kBins / 32; ++w) before += w < warp ? sums[w] : 0u;
+            bases[threadIdx.x] = before + scan - all;
         }
         __syncthreads();
         for (unsigned i = begin + lane; i - lane < end; i += 32u) {
             const bool there = i < end;
-            const unsigned key = there ? (pass == 0 ? key_of(a, i) : keys[i]) : 0u;
-            const unsigned bin = there ? key >> shift & (kBins - 1u) : kBins;
-            const unsigned same = __match_any_sync(0xffffffffu, bin);
+            const unsigned key = there ? (pass == 0 ? key_of(a, i) : keys[i]) : 0u, place = there && pass != 0 ? places[i] : i;
+            const unsigned to = there ? key >> shift & (kBins - 1u) : kBins;
+            const unsigned same = __match_any_sync(0xffffffffu, to);
             unsigned at = 0;
-            if (there) at = counts[warp][bin] + __popc(same & ((1u << lane) - 1u));
+            if (there) at = bases[to] + counts[warp][to] + __popc(same & ((1u << lane) - 1u));
             __syncwarp();
-            if (there && (int)lane == __ffs((int)same) - 1) counts[warp][bin] += __popc(same);
+            if (there && (int)lane == __ffs((int)same) - 1) counts[warp][to] += __popc(same);
             __syncwarp();
             if (there) {
                 a.keys[target][at] = key;
-                a.places[target][at] = pass == 0 ? i : places[i];
+                a.places[target][at] = place;
             }
         }
         cluster_sync();  // the list is whole, and the totals have been read
     }
+}
+
+struct FillArgs {
+    char* gradient;
+    u64 bytes;
+};
+
+constexpr unsigned kFillThreads = 512, kFillBytes = 65536;  // of a CTA
+
+// Zeros. It runs beside the sort, on which it does not depend; the first CTA stays until that is done, so that both are over for what comes next.
+__global__ void __launch_bounds__(kFillThreads) fill_kernel(const __grid_constant__ FillArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const u64 first = (u64)blockIdx.x * kFillBytes + threadIdx.x * 16u;
+#pragma unroll
+    for (unsigned i = 0; i < kFillBytes / (16u * kFillThreads); ++i) {
+        const u64 at = first + i * (16u * kFillThreads);
+        if (at + 16u <= a.bytes) store16_once(a.gradient + at, make_uint4(0u, 0u, 0u, 0u));
+        else
+            for (u64 b = at; b < a.bytes; ++b) a.gradient[b] = 0;
+    }
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 struct SumArgs {
@@ -419,18 +441,21 @@ cudaError_t launch_embedding_gradient(const EmbeddingCall& c) {
         s.keys[i] = reinterpret_cast<unsigned*>(workspace + w.keys[i]);
         s.places[i] = reinterpret_cast<unsigned*>(workspace + w.places[i]);
     }
-    s.gradient = static_cast<char*>(c.out);
-    s.gradient_bytes = bytes;
-    // A CTA that fills for every 32 KiB, up to what an SM has room for.
-    const unsigned fill = (unsigned)std::min<std::size_t>(17, (bytes + kSortCtas * 32768 - 1) / (kSortCtas * 32768));
-    cudaError_t st = launch_dependent<SortArgs>(sort_kernel, dim3((1 + std::max(1u, fill)) * kSortCtas), kSortThreads, 0, c.stream, s);
+    cudaError_t st = launch_dependent<SortArgs>(sort_kernel, dim3(kSortCtas), kSortThreads, 0, c.stream, s);
+    if (st != cudaSuccess) return st;
+    FillArgs f;
+    f.gradient = static_cast<char*>(c.out);
+    f.bytes = bytes;
+    const std::size_t ctas = (bytes + kFillBytes - 1) / kFillBytes;
+    B2_REQUIRE(ctas < (1ull << 31), "the gradient is too large for one call");
+    st = launch_dependent<FillArgs>(fill_kernel, dim3((unsigned)ctas), kFillThreads, 0, c.stream, f);
     if (st != cudaSuccess) return st;
     SumArgs a;
     a.keys = s.keys[0];
     a.places = s.places[0];
     a.dy = static_cast<const char*>(c.rows);
     a.stride = c.stride * (long long)e;
-    a.gradient = s.gradient;
+    a.gradient = f.gradient;
     a.partial = reinterpret_cast<float*>(workspace + w.partial);
     a.count = s.count;
     a.vocabulary = s.vocabulary;
@@ -451,7 +476,7 @@ cudaError_t launch_embedding_gradient(const EmbeddingCall& c) {
     JoinArgs j;
     j.keys = a.keys;
     j.partial = a.partial;
-    j.gradient = s.gradient;
+    j.gradient = f.gradient;
     j.count = s.count;
     j.vocabulary = s.vocabulary;
     j.chunk = w.chunk;

@@ -15,7 +15,9 @@
 // element in bf16) is what the gradients lose beside their own. r_t = c_t / max |c| is 1 in a mean or a sum, so that the target's element
 // stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there.
 //
-// fp32: x, w and P are exact sums of three bf16 matrices each, and six products of those give the 24-bit product (the three smallest are below 2^-24 of it).
+// fp32: x, w and P are sums of two fp16 matrices each, what fp16 makes of an element and what it makes of the rest, after a power of two that brings the largest
+// element of x and of w to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
+// it. (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 2055.)
 // The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and sums are added up in memory, rounded, after every 1024
 // elements of the summed axis; in 16-bit types after 16384.
 //
@@ -61,12 +63,13 @@ constexpr unsigned kAtStaging = kStages * 2 * kOperandBytes, kAtBarriers = kAtSt
 constexpr unsigned kShared = kAtBarriers + 256 + 1024;
 static_assert(kShared <= 227 * 1024);
 constexpr unsigned kTileFloats = kTile * kTile;
-constexpr unsigned kLongSteps = 256, kChunkSteps = 16;  // steps between two additions to sums in memory: 16-bit types; fp32, of each of its six products
+constexpr unsigned kLongSteps = 256, kChunkSteps = 16;  // steps between two additions to sums in memory: 16-bit types; fp32, of each of its products
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr unsigned kProducts = 3;        // of fp32
 constexpr float kHalfScale = 16384.0f;  // of P in fp16
 
 template <typename T>
-using OperandOf = std::conditional_t<std::is_same_v<T, __half>, __half, __nv_bfloat16>;
+using OperandOf = std::conditional_t<std::is_same_v<T, __nv_bfloat16>, __nv_bfloat16, __half>;
 
 struct alignas(64) ProductArgs {
     CUtensorMap a, b;  // [parts][rows][columns]
@@ -83,7 +86,8 @@ struct alignas(64) ProductArgs {
     unsigned* status;   // host memory
     u64 wait_ns;
     // Stats and Probs
-    float factor;  // log2(e) / temperature
+    const unsigned* magnitudes;  // fp32: the largest of x and of w, see scale_of()
+    float factor;                // log2(e) / temperature
     float2* stats; // [2 * tiles along n][m]
     float* picked; // [m]
     const void* targets;
@@ -155,7 +159,7 @@ struct Share {
 };
 // The end of the part of a run, from step k on, that is summed on the tensor cores alone.
 __device__ __forceinline__ unsigned segment_end(const ProductArgs& a, unsigned k, unsigned to) {
-    const unsigned chunk = a.parts > 1 ? 6u * kChunkSteps : kLongSteps;
+    const unsigned chunk = a.parts > 1 ? kProducts * kChunkSteps : kLongSteps;
     return min(to, (k / chunk + 1u) * chunk);
 }
 // Which parts of the operands, and which 64 elements, step k of a tile takes: of sixteen steps the products with the smallest sums first.
@@ -164,10 +168,9 @@ struct Spot {
 };
 __device__ __forceinline__ Spot spot_of(const ProductArgs& a, unsigned k) {
     if (a.parts == 1) return {0u, 0u, k};
-    const unsigned chunk = k / (6u * kChunkSteps), in_chunk = k - chunk * (6u * kChunkSteps);
+    const unsigned chunk = k / (kProducts * kChunkSteps), in_chunk = k - chunk * (kProducts * kChunkSteps);
     const unsigned length = min(kChunkSteps, a.steps_of_part - chunk * kChunkSteps), product = in_chunk / length;
-    // (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)
-    return {(0x001102u >> (4u * product)) & 15u, (0x010120u >> (4u * product)) & 15u, chunk * kChunkSteps + in_chunk - product * length};
+    return {product == 0u ? 1u : 0u, product == 1u ? 1u : 0u, chunk * kChunkSteps + in_chunk - product * length};
 }
 
 struct Tile {
@@ -223,8 +226,20 @@ __device__ __forceinline__ void staging_out(const CUtensorMap* map, unsigned sta
     }
 }
 
-// max |c| and whether anything went wrong, in the first words of a gradient's workspace.
-__device__ __forceinline__ float gradient_scale(const float* header, bool half) { return header[0] * (half ? 1.0f / kHalfScale : 1.0f) + header[1]; }
+// fp32: the power of two that brings a matrix whose largest magnitude has these bits to 2^14 and on, and back. (Below 2^-112 the largest stays smaller.)
+__device__ __forceinline__ float scale_of(unsigned magnitude, bool back) {
+    const int e = min(14 - ((int)(magnitude >> 23) - 127), 126);
+    return __uint_as_float((unsigned)((back ? -e : e) + 127) << 23);
+}
+
+// max |c| and whether anything went wrong, in the first words of a gradient's workspace, and what P and the other operand were scaled with.
+template <Kind kKind, typename T>
+__device__ __forceinline__ float gradient_scale(const float* header, const unsigned* magnitudes) {
+    float scale = header[0] + header[1];
+    if constexpr (!std::is_same_v<T, __nv_bfloat16>) scale *= 1.0f / kHalfScale;
+    if constexpr (sizeof(T) == 4) scale *= scale_of(magnitudes[kKind == Kind::WeightGrad ? 0 : 1], true);
+    return scale;
+}
 
 // c_t / max |c|; 0 of rows that do not count.
 __device__ __forceinline__ float row_weight(float valid, const float* loss_grad, long long stride, float temperature, float largest, unsigned row) {
@@ -261,7 +276,7 @@ template <Kind kKind, typename T>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
     constexpr bool kLogits = kKind == Kind::Stats || kKind == Kind::Probs;
     constexpr bool kAByRows = kKind == Kind::WeightGrad, kBByRows = !kLogits;
-    constexpr bool kHalfType = std::is_same_v<T, __half>;
+    constexpr bool kHalfType = !std::is_same_v<T, __nv_bfloat16>;
     extern __shared__ unsigned char raw[];
     // Swizzled operands start at multiples of 1024 bytes; the same place in both CTAs.
     unsigned char* shared = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
@@ -383,7 +398,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const unsigned quarter = warp & 3u, group = (warp - kFirstEpilogueWarp) / 4u;  // lanes of tensor memory that this warp reaches; its half of the columns
         const unsigned in_tile = rank * kHalf + quarter * 32u, column0 = group * b_rows;
         const unsigned staging = base + kAtStaging + (warp - kFirstEpilogueWarp) * kStagingBytes;
-        const float scale = kLogits ? 1.0f : gradient_scale(a.header, kHalfType);
+        float scale = 1.0f;
+        if constexpr (!kLogits) scale = gradient_scale<kKind, T>(a.header, a.magnitudes);
+        Pair32 back_x = both32(1.0f), back_w = both32(1.0f);
+        if constexpr (kLogits && sizeof(T) == 4) {
+            back_x = both32(scale_of(a.magnitudes[0], true));
+            back_w = both32(scale_of(a.magnitudes[1], true));
+        }
         unsigned n = 0, segments = 0;
         bool ok = true;
         while (n < share.all && ok) {
@@ -429,6 +450,18 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         f[4 * j + 3] += v.w;
                     }
                 };
+                // Logits, of sums that were scaled.
+                const auto take_logits = [&](unsigned c, float (&f)[32]) {
+                    take(c, f);
+                    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                        for (unsigned j = 0; j < 32; j += 2) {
+                            const float2 z = apart(mul2(mul2(pair32(f[j], f[j + 1]), back_x), back_w));
+                            f[j] = z.x;
+                            f[j + 1] = z.y;
+                        }
+                    }
+                };
                 if (!done) {
                     for (unsigned c = 0; c < columns; c += 32u) {
                         float f[32];
@@ -441,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                     const Pair32 factor = both32(a.factor);
                     for (unsigned c = 0; c < columns; c += 32u) {
                         float f[32];
-                        take(c, f);
+                        take_logits(c, f);
                         if (c + 32u > columns) {
 #pragma unroll
                             for (unsigned j = 0; j < 32; ++j) f[j] = c + j < columns ? f[j] : -__int_as_float(0x7f800000);
@@ -476,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         float f[2][32];
 #pragma unroll
                         for (unsigned h = 0; h < 2; ++h) {
-                            take(c + 32u * h, f[h]);
+                            take_logits(c + 32u * h, f[h]);
                             const unsigned at = own_target - (c + 32u * h);
 #pragma unroll
                             for (unsigned j = 0; j < 32; j += 2) {
@@ -497,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                                 for (unsigned j = 0; j < 32; ++j) f[h][j] = 0.0f;
                             }
                         }
-                        constexpr unsigned kParts = sizeof(T) == 4 ? 3 : 1;
+                        constexpr unsigned kParts = sizeof(T) == 4 ? 2 : 1;
 #pragma unroll
                         for (unsigned p = 0; p < kParts; ++p) {
                             staging_free();
@@ -506,13 +539,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                                 if constexpr (kParts == 1) {
                                     stage<T>(staging, h, f[h]);
                                 } else {
-                                    float part[32];  // the leading eight bits of what is left
+                                    stage<__half>(staging, h, f[h]);
+                                    if (p != 0) continue;
 #pragma unroll
-                                    for (unsigned j = 0; j < 32; ++j) {
-                                        part[j] = __uint_as_float(__float_as_uint(f[h][j]) & 0xffff0000u);
-                                        f[h][j] -= part[j];
-                                    }
-                                    stage<__nv_bfloat16>(staging, h, part);
+                                    for (unsigned j = 0; j < 32; ++j) f[h][j] -= __half2float(__float2half_rn(f[h][j]));
                                 }
                             }
                             staging_out(&a.out, staging, first + c, t.m + in_tile, p, a.m);
@@ -581,13 +611,13 @@ struct FinishArgs {
     float* sums;         // see ProductArgs
     bool prior, last;
     const float* header;
-    bool half;
+    const unsigned* magnitudes;
     unsigned m, n, m_tiles, n_tiles, n_tile, whole_tiles, steps_of_tile, steps, groups;
     bool n_first;
 };
 
 // Adds the pieces of cut tiles: 32 rows by 32 columns of a tile for a CTA (a tile that all pairs share has 74 pieces, and few CTAs took 51 us for two of them).
-template <typename T>
+template <Kind kKind, typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ FinishArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -624,7 +654,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         reinterpret_cast<float4*>(a.sums + (u64)tile * kTileFloats)[at] = sum;
         return;
     }
-    const float scale = gradient_scale(a.header, a.half);
+    const float scale = gradient_scale<kKind, T>(a.header, a.magnitudes);
     __shared__ float turned[32][33];
     float* t = &turned[lane][warp * 4u];
     t[0] = sum.x * scale;
@@ -949,7 +979,7 @@ __global__ void __launch_bounds__(256) fix_kernel(const __grid_constant__ FixArg
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned lane = threadIdx.x & 31u, row = blockIdx.x * 8u + threadIdx.x / 32u;
     if (row >= a.rows) return;
-    const float weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (std::is_same_v<T, __half> ? kHalfScale : 1.0f);
+    const float weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (std::is_same_v<T, __nv_bfloat16> ? 1.0f : kHalfScale);
     const float top = a.top[row], share_of_sum = weight / a.sum[row];
     long long token[kEntryRounds];
     float p[kEntryRounds];
@@ -982,14 +1012,78 @@ __global__ void __launch_bounds__(256) fix_kernel(const __grid_constant__ FixArg
         if constexpr (sizeof(T) == 2) {
             static_cast<T*>(a.probs)[at] = Elem<T>::from_f(v);
         } else {
-#pragma unroll
-            for (unsigned part = 0; part < 3; ++part) {
-                const unsigned cut = __float_as_uint(v) >> 16;
-                v -= __uint_as_float(cut << 16);
-                static_cast<unsigned short*>(a.probs)[(u64)part * a.rows * a.pitch + at] = (unsigned short)cut;
-            }
+            const __half part = __float2half_rn(v);
+            static_cast<__half*>(a.probs)[at] = part;
+            static_cast<__half*>(a.probs)[(u64)a.rows * a.pitch + at] = __float2half_rn(v - __half2float(part));
         }
     }
+}
+
+// fp32: the largest magnitudes of x and of the matrix, as whole numbers, without infinities and NaN.
+struct MagnitudeArgs {
+    const char* from[2];
+    long long stride[2];  // bytes
+    unsigned rows[2], columns, ctas_of_x;
+    Divisor eights;  // of a row
+    unsigned* magnitudes;
+};
+
+// A thread takes eight elements of a row, four times.
+__global__ void __launch_bounds__(256) magnitude_kernel(const __grid_constant__ MagnitudeArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned which = blockIdx.x >= a.ctas_of_x ? 1u : 0u, first = (blockIdx.x - which * a.ctas_of_x) * 1024u + threadIdx.x;
+    unsigned most = 0;
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+        const unsigned at = first + 256u * i, row = a.eights.divide(at), n = (at - row * a.eights.d) * 8u;
+        if (row >= a.rows[which]) continue;
+        unsigned w[8];
+        load_any<float, 8>(a.from[which] + (long long)row * a.stride[which] + (u64)n * 4u, n < a.columns ? min(8u, a.columns - n) : 0u, w);
+#pragma unroll
+        for (unsigned e = 0; e < 8; ++e) {
+            const unsigned magnitude = w[e] & 0x7fffffffu;
+            most = max(most, magnitude < 0x7f800000u ? magnitude : 0u);
+        }
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    __shared__ unsigned all[8];
+    if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = most;
+    __syncthreads();
+    if (threadIdx.x >= 32u) return;
+    most = __reduce_max_sync(0xffffffffu, threadIdx.x < 8u ? all[threadIdx.x] : 0u);
+    if (threadIdx.x == 0) atomicMax(a.magnitudes + which, most);  // (in any order)
+}
+
+// fp32 as two fp16 matrices [2][rows][pitch], scaled.
+struct SplitArgs {
+    const char* from;
+    long long stride;  // bytes
+    char* out;
+    unsigned rows, columns;
+    Divisor eights;  // of a row
+    const unsigned* magnitude;
+};
+
+// A thread takes eight elements of a row.
+__global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ SplitArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned i = blockIdx.x * 256u + threadIdx.x, row = a.eights.divide(i), n = (i - row * a.eights.d) * 8u;
+    if (row >= a.rows) return;
+    const float scale = scale_of(*a.magnitude, false);
+    unsigned words[8], first[4], second[4];
+    load_any<float, 8>(a.from + (long long)row * a.stride + (u64)n * 4u, n < a.columns ? min(8u, a.columns - n) : 0u, words);
+#pragma unroll
+    for (unsigned e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(words[2 * e]) * scale, y = __uint_as_float(words[2 * e + 1]) * scale;
+        first[e] = f2_to_h2(x, y);
+        const float2 f = h2_to_f2(first[e]);
+        // (Infinities and NaN have no rest.)
+        second[e] = f2_to_h2(fabsf(x) < 65536.0f ? x - f.x : 0.0f, fabsf(y) < 65536.0f ? y - f.y : 0.0f);
+    }
+    *(reinterpret_cast<uint4*>(a.out) + i) = make_uint4(first[0], first[1], first[2], first[3]);
+    *(reinterpret_cast<uint4*>(a.out) + (u64)a.rows * a.eights.d + i) = make_uint4(second[0], second[1], second[2], second[3]);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
@@ -1054,7 +1148,7 @@ Tiling tiling_of(u64 m, u64 n, u64 summed, unsigned parts, unsigned n_tile, bool
     t.parts = parts;
     t.n_tile = n_tile;
     const u64 m_tiles = (m + kTile - 1) / kTile, n_tiles = (n + n_tile - 1) / n_tile, steps = (summed + kStep - 1) / kStep;
-    const u64 tiles = m_tiles * n_tiles, steps_of_tile = steps * (parts > 1 ? 6 : 1);
+    const u64 tiles = m_tiles * n_tiles, steps_of_tile = steps * (parts > 1 ? kProducts : 1);
     B2_REQUIRE(steps_of_tile < (1ull << 31) && tiles < (1ull << 31) && tiles * steps_of_tile < (1ull << 31), "too many tokens, words and columns for one call");
     t.m_tiles = (unsigned)m_tiles;
     t.n_tiles = (unsigned)n_tiles;
@@ -1070,7 +1164,7 @@ Tiling tiling_of(u64 m, u64 n, u64 summed, unsigned parts, unsigned n_tile, bool
     if (!may_cut || t.steps_of_tile < 8 + t.steps / t.pairs) t.groups = std::max(1u, left);
     if (t.waves == 0) t.pairs = t.groups;
     for (unsigned i = 1; i < t.groups && left != 0; ++i) t.cut |= first_step(i, t.steps, t.groups) % t.steps_of_tile != 0;
-    t.summed = t.cut || t.steps_of_tile > (parts > 1 ? 6 * kChunkSteps : kLongSteps);
+    t.summed = t.cut || t.steps_of_tile > (parts > 1 ? kProducts * kChunkSteps : kLongSteps);
     return t;
 }
 
@@ -1100,7 +1194,7 @@ unsigned n_tile_of(std::size_t width) { return (width + 127) / 128 * 128 < (widt
 Plan plan_of(const VocabularyLossCall& c, bool gradient) {
     Plan p;
     const std::size_t e = dtype_size(c.dtype), t = c.tokens, v = c.vocabulary;
-    p.parts = c.dtype == DType::Float ? 3 : 1;
+    p.parts = c.dtype == DType::Float ? 2 : 1;
     p.device_pairs = pairs_of_device(current_device());
     p.pitch = (c.width + 7) / 8 * 8;
     p.copy_x = c.dtype == DType::Float || !readable(c.x, c.x_stride, c.width, t, e);
@@ -1198,7 +1292,7 @@ void launch_product(Kind kind, const VocabularyLossCall& c, const Tiling& t, Pro
 }
 
 // The pieces of a gradient's cut tiles.
-template <typename T>
+template <Kind kKind, typename T>
 void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) {
     if (!t.cut) return;
     FinishArgs f;
@@ -1208,7 +1302,7 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
     f.prior = a.prior;
     f.last = a.last;
     f.header = a.header;
-    f.half = std::is_same_v<T, __half>;
+    f.magnitudes = a.magnitudes;
     f.m = a.m;
     f.n = a.n;
     f.m_tiles = t.m_tiles;
@@ -1220,11 +1314,12 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
     f.groups = t.groups;
     f.n_first = a.n_first;
     const unsigned left = t.steps / t.steps_of_tile;
-    B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<T>, dim3(left * 8 * (t.n_tile / 32)), 256, 0, c.stream, f));
+    B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<kKind, T>, dim3(left * 8 * (t.n_tile / 32)), 256, 0, c.stream, f));
 }
 
 struct Kept {
     float *top, *sum, *valid, *count, *z, *p;
+    unsigned* magnitudes;
 };
 Kept kept_of(const VocabularyLossCall& c) {
     Kept k;
@@ -1232,7 +1327,8 @@ Kept kept_of(const VocabularyLossCall& c) {
     k.sum = k.top + c.tokens;
     k.valid = k.sum + c.tokens;
     k.count = k.valid + c.tokens;
-    k.z = k.count + 1;
+    k.magnitudes = reinterpret_cast<unsigned*>(k.count + 1);
+    k.z = k.count + 3;
     k.p = k.z + c.tokens * (std::size_t)c.entries;
     return k;
 }
@@ -1246,20 +1342,53 @@ void operands(const VocabularyLossCall& c, const Plan& p, Operand* x, Operand* w
     // (The stride of a single row is not looked at, but must be a multiple of 16 bytes all the same.)
     *x = {c.x, c.width, c.tokens, (c.tokens > 1 ? (u64)c.x_stride : (u64)p.pitch) * sizeof(T)};
     *w = {c.weight, c.width, c.vocabulary, (c.vocabulary > 1 ? (u64)c.weight_stride : (u64)p.pitch) * sizeof(T)};
-    if (p.copy_x) {
-        lay_out<T>(c.x, c.x_stride, c.tokens, c.width, p.pitch, workspace + p.x_at, c.stream, kTooLarge);
-        *x = {workspace + p.x_at, c.width, c.tokens, p.pitch * 2};
-    }
-    if (p.copy_weight) {
-        lay_out<T>(c.weight, c.weight_stride, c.vocabulary, c.width, p.pitch, workspace + p.weight_at, c.stream, kTooLarge);
-        *w = {workspace + p.weight_at, c.width, c.vocabulary, p.pitch * 2};
-    }
+    const auto copy = [&](const void* from, long long stride, std::size_t rows, std::size_t at, const unsigned* magnitude) -> Operand {
+        if constexpr (sizeof(T) == 2) {
+            lay_out<T>(from, stride, rows, c.width, p.pitch, workspace + at, c.stream, kTooLarge);
+        } else {
+            SplitArgs s;
+            s.from = static_cast<const char*>(from);
+            s.stride = stride * 4;
+            s.out = workspace + at;
+            s.rows = (unsigned)rows;
+            s.columns = (unsigned)c.width;
+            s.eights = Divisor((unsigned)(p.pitch / 8));
+            s.magnitude = magnitude;
+            const u64 eights = (u64)rows * (p.pitch / 8);
+            B2_REQUIRE(eights < (1ull << 31), kTooLarge);
+            B2_CUDA(launch_dependent<SplitArgs>(split_kernel, dim3((unsigned)((eights + 255) / 256)), 256, 0, c.stream, s));
+        }
+        return {workspace + at, c.width, rows, p.pitch * 2};
+    };
+    const unsigned* magnitudes = kept_of(c).magnitudes;
+    if (p.copy_x) *x = copy(c.x, c.x_stride, c.tokens, p.x_at, magnitudes);
+    if (p.copy_weight) *w = copy(c.weight, c.weight_stride, c.vocabulary, p.weight_at, magnitudes + 1);
+}
+
+// fp32: what x and the matrix are scaled with.
+void measure(const VocabularyLossCall& c, const Plan& p) {
+    MagnitudeArgs m;
+    m.magnitudes = kept_of(c).magnitudes;
+    m.from[0] = static_cast<const char*>(c.x);
+    m.from[1] = static_cast<const char*>(c.weight);
+    m.stride[0] = c.x_stride * 4;
+    m.stride[1] = c.weight_stride * 4;
+    m.rows[0] = (unsigned)c.tokens;
+    m.rows[1] = (unsigned)c.vocabulary;
+    m.columns = (unsigned)c.width;
+    m.eights = Divisor((unsigned)(p.pitch / 8));
+    const u64 x = (u64)c.tokens * (p.pitch / 8), w = (u64)c.vocabulary * (p.pitch / 8);
+    B2_REQUIRE(x < (1ull << 31) - 1024 && w < (1ull << 31) - 1024, kTooLarge);
+    m.ctas_of_x = (unsigned)((x + 1023) / 1024);
+    B2_CUDA(cudaMemsetAsync(m.magnitudes, 0, 2 * sizeof(unsigned), c.stream));
+    B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel, dim3(m.ctas_of_x + (unsigned)((w + 1023) / 1024)), 256, 0, c.stream, m));
 }
 
 template <typename T>
-constexpr DType operand_type() { return std::is_same_v<T, __half> ? DType::Float16 : DType::BFloat16; }
+constexpr DType operand_type() { return std::is_same_v<T, __nv_bfloat16> ? DType::BFloat16 : DType::Float16; }
 
 void logits_arguments(const VocabularyLossCall& c, ProductArgs& a) {
+    a.magnitudes = kept_of(c).magnitudes;
     a.factor = kLog2E / c.temperature;
     a.hard = !c.distillation;
     a.targets = c.targets;
@@ -1273,6 +1402,7 @@ void loss(const VocabularyLossCall& c, const Plan& p) {
     char* workspace = static_cast<char*>(c.workspace);
     const Kept kept = kept_of(c);
     Operand x, w;
+    if constexpr (sizeof(T) == 4) measure(c, p);
     operands<T>(c, p, &x, &w);
     if (c.distillation) {
         EntriesArgs e;
@@ -1413,7 +1543,7 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
             a.last = true;
             gradient_of(static_cast<T*>(c.weight_grad) + first * c.width, words);
             launch_product(Kind::WeightGrad, c, t, a, words, c.width);
-            finish<T>(c, t, a);
+            finish<Kind::WeightGrad, T>(c, t, a);
         }
         if (c.x_grad != nullptr) {
             const Tiling t = tiling_of(c.tokens, c.width, words, p.parts, p.n_tile, true, p.device_pairs);
@@ -1425,14 +1555,14 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
             a.last = piece + 1 == p.pieces;
             gradient_of(c.x_grad, c.tokens);
             launch_product(Kind::InputGrad, c, t, a, c.tokens, c.width);
-            finish<T>(c, t, a);
+            finish<Kind::InputGrad, T>(c, t, a);
         }
     }
 }
 
 }  // namespace
 
-std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 3 + 1 + 2 * c.tokens * (std::size_t)c.entries; }
+std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 3 + 3 + 2 * c.tokens * (std::size_t)c.entries; }
 
 std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient) { return call.tokens == 0 ? 0 : plan_of(call, gradient).bytes; }
 

@@ -29,10 +29,16 @@ def embedding_gradient(tokens, dy, vocabulary, scale):
 
 def _sums(dtype, summed):
     """Relative error (of the sum of the magnitudes) of a product's sum on the tensor cores: an instruction adds 16 products and may cut a step of 24 bits of the sum so far, at most 1024 of
-    them in 16-bit types and 6 * 64 in float32 before sums are added up in memory, rounded; float32 leaves out products of 2^-24."""
+    them in 16-bit types and 3 * 64 in float32 before sums are added up in memory, rounded. float32: both operands are two fp16 numbers, within 2^-22, and the product of the
+    second ones, 2^-22, is left out."""
     if dtype == torch.float32:
-        return (6 * (min(summed, 1024) / 16 + 1) + summed / 1024 + 4) * 2.0 ** -23
+        return (3 * (min(summed, 1024) / 16 + 1) + summed / 1024 + 4) * 2.0 ** -23 + 3 * 2.0 ** -22
     return (min(summed, 16384) / 16 + summed / 16384 + 3) * 2.0 ** -23
+
+
+def _floor(dtype, t):
+    """What the second fp16 number of a float32 one may be off by at least: half of 2^-24, scaled by a power of two that brings the largest element to 2^14 at least."""
+    return 2.0 ** -39 * t.abs().max() if dtype == torch.float32 else 0.0
 
 
 def losses(x, weight, targets, teacher_logits=None, temperature=1.0, reduction="mean", dloss=None):
@@ -41,6 +47,7 @@ def losses(x, weight, targets, teacher_logits=None, temperature=1.0, reduction="
     a, w, h = x.detach().double(), weight.detach().double(), half_step(x.dtype)
     z = a @ w.t() / temperature
     off = _sums(dtype, width) * (a.abs() @ w.abs().t()) / temperature  # of each logit
+    off = off + (_floor(dtype, a) * w.abs().sum(-1)[None] + _floor(dtype, w) * a.abs().sum(-1)[:, None]) / temperature
     off = off.max(-1, keepdim=True).values
     lse = torch.logsumexp(z, -1, keepdim=True)
     q = torch.exp(z - lse)
@@ -70,16 +77,16 @@ def losses(x, weight, targets, teacher_logits=None, temperature=1.0, reduction="
         return out
     c = temperature * counted[:, None] * (dloss.double() / count if reduction != "none" else dloss.double()[:, None])
     dz = q.scatter_add(1, entries, -y) * c
-    # Of an element of P: its own rounding (float32: three parts of 8 bits), and what the softmax is off by; in fp16 it is held as 2^14 times its share of the largest row's.
+    # Of an element of P: its own rounding (float32: two fp16 numbers), and what the softmax is off by; in fp16 it is held as 2^14 times its share of the largest row's.
     element = dz.abs() * (h if dtype != torch.float32 else 2.0 ** -22) + c.abs() * q * relative[:, None]
     element = element.scatter_add(1, entries, y * c.abs() * (0.0 if teacher_logits is None else 1.0) * relative[:, None])
-    if dtype == torch.float16:
-        element = element + c.abs().max() * 2.0 ** -14 * smallest(dtype)
+    if dtype != torch.bfloat16:
+        element = element + c.abs().max() * 2.0 ** -14 * smallest(torch.float16)
     element = element + 2.0 ** -126
     for name, p, e, m, summed in (("dx", dz, element, w, vocabulary), ("dw", dz.t(), element.t(), a, rows)):
         exact = p @ m
         sums = p.abs() @ m.abs()
-        out[name] = (exact, e @ m.abs() + (_sums(dtype, summed) + 16 * 2.0 ** -24) * sums + h * (exact.abs() + e @ m.abs()) + smallest(dtype))
+        out[name] = (exact, e @ m.abs() + _floor(dtype, m) * p.abs().sum(-1, keepdim=True) + (_sums(dtype, summed) + 16 * 2.0 ** -24) * sums + h * (exact.abs() + e @ m.abs()) + smallest(dtype))
     return out
 
 
