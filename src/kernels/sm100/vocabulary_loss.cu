@@ -566,12 +566,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             __syncwarp();
                             const unsigned rows = t.m + in_tile < a.m ? min(32u, a.m - t.m - in_tile) : 0u;
                             T* to = static_cast<T*>(a.gradient) + (u64)(t.m + in_tile) * a.n + first + c;
-                            for (unsigned i = 0; i < rows; ++i) {
+#pragma unroll 8
+                            for (unsigned i = 0; i < 32u; ++i) {
 #pragma unroll
                                 for (unsigned h = 0; h < kBlock / 32u; ++h) {
                                     const unsigned j = lane + 32u * h, at = j * (unsigned)sizeof(T);
-                                    if (c + j >= columns) continue;
-                                    to[(u64)i * a.n + j] = *reinterpret_cast<const T*>(shared + (staging - base) + i * 128u + (((at >> 4) ^ (i & 7u)) << 4) + (at & 15u));
+                                    const T v = *reinterpret_cast<const T*>(shared + (staging - base) + i * 128u + (((at >> 4) ^ (i & 7u)) << 4) + (at & 15u));
+                                    if (i < rows && c + j < columns) to[(u64)i * a.n + j] = v;
                                 }
                             }
                             __syncwarp();
@@ -1019,27 +1020,32 @@ __global__ void __launch_bounds__(256) fix_kernel(const __grid_constant__ FixArg
     }
 }
 
-// fp32: the largest magnitudes of x and of the matrix, as whole numbers, without infinities and NaN.
-struct MagnitudeArgs {
+// fp32: x and the matrix.
+struct Pair32Matrices {
     const char* from[2];
     long long stride[2];  // bytes
-    unsigned rows[2], columns, ctas_of_x;
+    unsigned rows[2], columns;
     Divisor eights;  // of a row
-    unsigned* magnitudes;
 };
 
-// A thread takes eight elements of a row, four times.
-__global__ void __launch_bounds__(256) magnitude_kernel(const __grid_constant__ MagnitudeArgs a) {
+constexpr unsigned kMagnitudeCtas = 256;  // for each of the two
+
+struct MagnitudeArgs {
+    Pair32Matrices m;
+    unsigned* partial;  // [2][kMagnitudeCtas]
+};
+
+// Their largest magnitudes, as whole numbers, without infinities and NaN: one of each CTA. A thread takes eight elements of a row at a time.
+__global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ MagnitudeArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned which = blockIdx.x >= a.ctas_of_x ? 1u : 0u, first = (blockIdx.x - which * a.ctas_of_x) * 1024u + threadIdx.x;
+    const unsigned which = blockIdx.x / kMagnitudeCtas, eights = a.m.rows[which] * a.m.eights.d;
     unsigned most = 0;
-#pragma unroll
-    for (unsigned i = 0; i < 4; ++i) {
-        const unsigned at = first + 256u * i, row = a.eights.divide(at), n = (at - row * a.eights.d) * 8u;
-        if (row >= a.rows[which]) continue;
+#pragma unroll 4
+    for (unsigned at = blockIdx.x % kMagnitudeCtas * 512u + threadIdx.x; at < eights; at += kMagnitudeCtas * 512u) {
+        const unsigned row = a.m.eights.divide(at), n = (at - row * a.m.eights.d) * 8u;
         unsigned w[8];
-        load_any<float, 8>(a.from[which] + (long long)row * a.stride[which] + (u64)n * 4u, n < a.columns ? min(8u, a.columns - n) : 0u, w);
+        load_any<float, 8>(a.m.from[which] + (long long)row * a.m.stride[which] + (u64)n * 4u, n < a.m.columns ? min(8u, a.m.columns - n) : 0u, w);
 #pragma unroll
         for (unsigned e = 0; e < 8; ++e) {
             const unsigned magnitude = w[e] & 0x7fffffffu;
@@ -1047,33 +1053,46 @@ __global__ void __launch_bounds__(256) magnitude_kernel(const __grid_constant__ 
         }
     }
     most = __reduce_max_sync(0xffffffffu, most);
-    __shared__ unsigned all[8];
+    __shared__ unsigned all[16];
     if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = most;
     __syncthreads();
     if (threadIdx.x >= 32u) return;
-    most = __reduce_max_sync(0xffffffffu, threadIdx.x < 8u ? all[threadIdx.x] : 0u);
-    if (threadIdx.x == 0) atomicMax(a.magnitudes + which, most);  // (in any order)
+    most = __reduce_max_sync(0xffffffffu, threadIdx.x < 16u ? all[threadIdx.x] : 0u);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = most;
 }
 
-// fp32 as two fp16 matrices [2][rows][pitch], scaled.
 struct SplitArgs {
-    const char* from;
-    long long stride;  // bytes
-    char* out;
-    unsigned rows, columns;
-    Divisor eights;  // of a row
-    const unsigned* magnitude;
+    Pair32Matrices m;
+    char* out[2];             // two fp16 matrices [2][rows][pitch] each, scaled
+    unsigned ctas_of_x;
+    const unsigned* partial;  // of magnitude_kernel; null: the magnitudes are known
+    unsigned* magnitudes;
 };
 
 // A thread takes eight elements of a row.
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ SplitArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned i = blockIdx.x * 256u + threadIdx.x, row = a.eights.divide(i), n = (i - row * a.eights.d) * 8u;
-    if (row >= a.rows) return;
-    const float scale = scale_of(*a.magnitude, false);
+    static_assert(kMagnitudeCtas == 256);
+    const unsigned which = blockIdx.x >= a.ctas_of_x ? 1u : 0u, block = blockIdx.x - which * a.ctas_of_x;
+    const unsigned i = block * 256u + threadIdx.x, row = a.m.eights.divide(i), n = (i - row * a.m.eights.d) * 8u;
     unsigned words[8], first[4], second[4];
-    load_any<float, 8>(a.from + (long long)row * a.stride + (u64)n * 4u, n < a.columns ? min(8u, a.columns - n) : 0u, words);
+    const bool there = row < a.m.rows[which];
+    if (there) load_any<float, 8>(a.m.from[which] + (long long)row * a.m.stride[which] + (u64)n * 4u, n < a.m.columns ? min(8u, a.m.columns - n) : 0u, words);
+    unsigned magnitude;
+    if (a.partial != nullptr) {
+        __shared__ unsigned all[8];
+        magnitude = __reduce_max_sync(0xffffffffu, a.partial[which * kMagnitudeCtas + threadIdx.x]);
+        if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = magnitude;
+        __syncthreads();
+#pragma unroll
+        for (unsigned w = 0; w < 8; ++w) magnitude = max(magnitude, all[w]);
+        if (block == 0 && threadIdx.x == 0) a.magnitudes[which] = magnitude;
+    } else {
+        magnitude = a.magnitudes[which];
+    }
+    if (!there) return;
+    const float scale = scale_of(magnitude, false);
 #pragma unroll
     for (unsigned e = 0; e < 4; ++e) {
         const float x = __uint_as_float(words[2 * e]) * scale, y = __uint_as_float(words[2 * e + 1]) * scale;
@@ -1082,8 +1101,8 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Spli
         // (Infinities and NaN have no rest.)
         second[e] = f2_to_h2(fabsf(x) < 65536.0f ? x - f.x : 0.0f, fabsf(y) < 65536.0f ? y - f.y : 0.0f);
     }
-    *(reinterpret_cast<uint4*>(a.out) + i) = make_uint4(first[0], first[1], first[2], first[3]);
-    *(reinterpret_cast<uint4*>(a.out) + (u64)a.rows * a.eights.d + i) = make_uint4(second[0], second[1], second[2], second[3]);
+    *(reinterpret_cast<uint4*>(a.out[which]) + i) = make_uint4(first[0], first[1], first[2], first[3]);
+    *(reinterpret_cast<uint4*>(a.out[which]) + (u64)a.m.rows[which] * a.m.eights.d + i) = make_uint4(second[0], second[1], second[2], second[3]);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
@@ -1168,7 +1187,10 @@ Tiling tiling_of(u64 m, u64 n, u64 summed, unsigned parts, unsigned n_tile, bool
     return t;
 }
 
-constexpr std::size_t kProbsBytes = 512ull << 20;  // of a piece of the vocabulary, unless that has fewer than kLeastPiece words
+// A piece of the vocabulary: so many bytes of P, unless that is fewer than kLeastPiece words, and of the matrix, which the gradient of x reads again for every few rows of tiles, out
+// of L2 in part. (8192 x 50257 x 768, loss and gradients: 2073 us in two pieces of P, 2112 in four, 2195 in seven; 4096 x 131072 x 4096: 13.7 ms in two
+// pieces, 13.2 in four of 256 MiB of the matrix, 13.3 in eight.)
+constexpr std::size_t kProbsBytes = 512ull << 20, kMatrixBytes = 256ull << 20;
 constexpr u64 kLeastPiece = 4096;
 
 std::size_t padded(std::size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -1181,7 +1203,7 @@ struct Plan {
     unsigned device_pairs = 0;
     u64 piece = 0, pieces = 1;  // words of the vocabulary
     unsigned n_tile = kTile;
-    std::size_t x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
+    std::size_t x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
 };
 
 bool readable(const void* p, long long stride, std::size_t columns, std::size_t rows, std::size_t element) {
@@ -1213,10 +1235,11 @@ Plan plan_of(const VocabularyLossCall& c, bool gradient) {
         p.stats_at = take((v + kTile - 1) / kTile * 2 * t * sizeof(float2));
         p.picked_at = take(t * sizeof(float));
         p.losses_at = take(t * sizeof(float));
+        p.partial_at = take(c.dtype == DType::Float ? 2 * kMagnitudeCtas * sizeof(unsigned) : 0);
         look(t, v, c.width, kTile, false);
     } else {
         const u64 tiles = (v + kTile - 1) / kTile, bytes = (u64)p.parts * t * 2;
-        const u64 most = std::max<u64>(std::max<u64>(kProbsBytes / bytes, kLeastPiece) / kTile, 1);
+        const u64 most = std::max<u64>(std::min<u64>(kProbsBytes / bytes, kMatrixBytes / (p.parts * c.width * 2)), kLeastPiece) / kTile;
         p.pieces = (tiles + most - 1) / most;
         p.piece = (tiles + p.pieces - 1) / p.pieces * kTile;
         p.pieces = (v + p.piece - 1) / p.piece;
@@ -1335,53 +1358,41 @@ Kept kept_of(const VocabularyLossCall& c) {
 
 constexpr const char* kTooLarge = "an operand is too large for one call";
 
-// x and the matrix as the tensor cores read them, copied where they have to be.
+// x and the matrix as the tensor cores read them, copied where they have to be. known: fp32's magnitudes are, from the forward pass.
 template <typename T>
-void operands(const VocabularyLossCall& c, const Plan& p, Operand* x, Operand* w) {
+void operands(const VocabularyLossCall& c, const Plan& p, bool known, Operand* x, Operand* w) {
     char* workspace = static_cast<char*>(c.workspace);
     // (The stride of a single row is not looked at, but must be a multiple of 16 bytes all the same.)
     *x = {c.x, c.width, c.tokens, (c.tokens > 1 ? (u64)c.x_stride : (u64)p.pitch) * sizeof(T)};
     *w = {c.weight, c.width, c.vocabulary, (c.vocabulary > 1 ? (u64)c.weight_stride : (u64)p.pitch) * sizeof(T)};
-    const auto copy = [&](const void* from, long long stride, std::size_t rows, std::size_t at, const unsigned* magnitude) -> Operand {
-        if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
+        const auto copy = [&](const void* from, long long stride, std::size_t rows, std::size_t at) -> Operand {
             lay_out<T>(from, stride, rows, c.width, p.pitch, workspace + at, c.stream, kTooLarge);
-        } else {
-            SplitArgs s;
-            s.from = static_cast<const char*>(from);
-            s.stride = stride * 4;
-            s.out = workspace + at;
-            s.rows = (unsigned)rows;
-            s.columns = (unsigned)c.width;
-            s.eights = Divisor((unsigned)(p.pitch / 8));
-            s.magnitude = magnitude;
-            const u64 eights = (u64)rows * (p.pitch / 8);
-            B2_REQUIRE(eights < (1ull << 31), kTooLarge);
-            B2_CUDA(launch_dependent<SplitArgs>(split_kernel, dim3((unsigned)((eights + 255) / 256)), 256, 0, c.stream, s));
+            return {workspace + at, c.width, rows, p.pitch * 2};
+        };
+        if (p.copy_x) *x = copy(c.x, c.x_stride, c.tokens, p.x_at);
+        if (p.copy_weight) *w = copy(c.weight, c.weight_stride, c.vocabulary, p.weight_at);
+    } else {
+        const u64 x_eights = (u64)c.tokens * (p.pitch / 8), w_eights = (u64)c.vocabulary * (p.pitch / 8);
+        B2_REQUIRE(x_eights < (1ull << 30) && w_eights < (1ull << 30), kTooLarge);
+        const Pair32Matrices m = {{static_cast<const char*>(c.x), static_cast<const char*>(c.weight)}, {c.x_stride * 4, c.weight_stride * 4},
+                                  {(unsigned)c.tokens, (unsigned)c.vocabulary}, (unsigned)c.width, Divisor((unsigned)(p.pitch / 8))};
+        SplitArgs s;
+        s.m = m;
+        s.out[0] = workspace + p.x_at;
+        s.out[1] = workspace + p.weight_at;
+        s.ctas_of_x = (unsigned)((x_eights + 255) / 256);
+        s.partial = nullptr;
+        s.magnitudes = kept_of(c).magnitudes;
+        if (!known) {
+            const MagnitudeArgs a = {m, reinterpret_cast<unsigned*>(workspace + p.partial_at)};
+            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel, dim3(2 * kMagnitudeCtas), 512, 0, c.stream, a));
+            s.partial = a.partial;
         }
-        return {workspace + at, c.width, rows, p.pitch * 2};
-    };
-    const unsigned* magnitudes = kept_of(c).magnitudes;
-    if (p.copy_x) *x = copy(c.x, c.x_stride, c.tokens, p.x_at, magnitudes);
-    if (p.copy_weight) *w = copy(c.weight, c.weight_stride, c.vocabulary, p.weight_at, magnitudes + 1);
-}
-
-// fp32: what x and the matrix are scaled with.
-void measure(const VocabularyLossCall& c, const Plan& p) {
-    MagnitudeArgs m;
-    m.magnitudes = kept_of(c).magnitudes;
-    m.from[0] = static_cast<const char*>(c.x);
-    m.from[1] = static_cast<const char*>(c.weight);
-    m.stride[0] = c.x_stride * 4;
-    m.stride[1] = c.weight_stride * 4;
-    m.rows[0] = (unsigned)c.tokens;
-    m.rows[1] = (unsigned)c.vocabulary;
-    m.columns = (unsigned)c.width;
-    m.eights = Divisor((unsigned)(p.pitch / 8));
-    const u64 x = (u64)c.tokens * (p.pitch / 8), w = (u64)c.vocabulary * (p.pitch / 8);
-    B2_REQUIRE(x < (1ull << 31) - 1024 && w < (1ull << 31) - 1024, kTooLarge);
-    m.ctas_of_x = (unsigned)((x + 1023) / 1024);
-    B2_CUDA(cudaMemsetAsync(m.magnitudes, 0, 2 * sizeof(unsigned), c.stream));
-    B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel, dim3(m.ctas_of_x + (unsigned)((w + 1023) / 1024)), 256, 0, c.stream, m));
+        B2_CUDA(launch_dependent<SplitArgs>(split_kernel, dim3(s.ctas_of_x + (unsigned)((w_eights + 255) / 256)), 256, 0, c.stream, s));
+        *x = {s.out[0], c.width, c.tokens, p.pitch * 2};
+        *w = {s.out[1], c.width, c.vocabulary, p.pitch * 2};
+    }
 }
 
 template <typename T>
@@ -1402,8 +1413,7 @@ void loss(const VocabularyLossCall& c, const Plan& p) {
     char* workspace = static_cast<char*>(c.workspace);
     const Kept kept = kept_of(c);
     Operand x, w;
-    if constexpr (sizeof(T) == 4) measure(c, p);
-    operands<T>(c, p, &x, &w);
+    operands<T>(c, p, false, &x, &w);
     if (c.distillation) {
         EntriesArgs e;
         const bool copied = sizeof(T) == 2;  // (fp32 reads the original)
@@ -1484,7 +1494,7 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
     h.header = header;
     B2_CUDA(launch_dependent<HeaderArgs>(header_kernel, dim3(1), 1024, 0, c.stream, h));
     Operand x, w;
-    operands<T>(c, p, &x, &w);
+    operands<T>(c, p, true, &x, &w);
     char* probs = workspace + p.probs_at;
     for (u64 piece = 0; piece < p.pieces; ++piece) {
         const u64 first = piece * p.piece, words = std::min<u64>(p.piece, c.vocabulary - first);

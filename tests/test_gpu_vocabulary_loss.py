@@ -345,26 +345,41 @@ def called(x, w, t, dloss, wait_ns, kept=None):
 
 
 def test_a_wait_that_runs_out_leaves_nan():
-    """Every pair of CTAs sums 512 steps before it writes a tile of logits: far longer than the few polls that a wait always makes."""
+    """Without any time a wait makes a few polls all the same, and may be over by then (it is for 256 steps at most, 70 us): a call's results are the right ones or NaN, its status says which, and
+    of many calls some run out."""
     x, w, t = inputs(4096, 1024, 32768, torch.bfloat16)
     t, dloss = t.clamp(min=0), torch.ones(4096, device="cuda")
-    torch.cuda.synchronize()
     ops.check_async_error()
     want, kept = called(x, w, t, dloss, 2 * 10 ** 9)
     grads, _ = called(x, w, t, dloss, 2 * 10 ** 9, kept)
-    spoilt, _ = called(x, w, t, dloss, 0)
-    assert spoilt.isnan().all()
-    # Nobody else is told: the next call works, and asking says it once.
-    assert torch.equal(called(x, w, t, dloss, 2 * 10 ** 9)[0], want) and want.isfinite().all()
-    with pytest.raises(nn.B200CclError, match="ran out"):
-        ops.check_async_error()
-    ops.check_async_error()
-    spoilt, _ = called(x, w, t, dloss, 0, kept)
-    assert spoilt[0].isnan().all() and spoilt[1].isnan().all()
-    again, _ = called(x, w, t, dloss, 2 * 10 ** 9, kept)
-    assert all(torch.equal(a, b) for a, b in zip(again, grads))
-    with pytest.raises(nn.B200CclError, match="ran out"):
-        ops.check_async_error(0)
+    assert want.isfinite().all() and all(g.isfinite().all() for g in grads)
+
+    def ran_out():
+        try:
+            ops.check_async_error()
+        except nn.B200CclError as e:
+            assert "ran out" in str(e)
+            ops.check_async_error()  # (it is said once)
+            return True
+        return False
+
+    seen = [0, 0]
+    for _ in range(60):
+        loss, _ = called(x, w, t, dloss, 0)
+        nan = loss.isnan()
+        assert torch.equal(loss[~nan], want[~nan]) and bool(nan.any()) == ran_out()
+        seen[0] += bool(nan.any())
+        got, _ = called(x, w, t, dloss, 0, kept)
+        if ran_out():
+            assert all(g.isnan().all() for g in got)
+            seen[1] += 1
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(got, grads))
+    assert min(seen) > 0
+    # Nobody else is told.
+    assert torch.equal(called(x, w, t, dloss, 2 * 10 ** 9)[0], want)
+    assert all(torch.equal(a, b) for a, b in zip(called(x, w, t, dloss, 2 * 10 ** 9, kept)[0], grads))
+    assert not ran_out()
 
 
 def test_a_failure_in_a_backward_pass_is_this_library_s_error():
