@@ -66,9 +66,15 @@ typedef struct b2_vocabulary_loss {
 int b2_vocabulary_loss_sizes(const b2_vocabulary_loss* call, int backward, size_t* kept_floats, size_t* workspace_bytes);
 int b2_vocabulary_loss_forward(const b2_vocabulary_loss* call, void* stream);
 int b2_vocabulary_loss_backward(const b2_vocabulary_loss* call, void* stream);
+/* bf16, one loss for all tokens (reduction 1 or 2): the loss together with the gradients whose pointers are given, for a loss_grad of 1, which saves making the logits
+ * a second time; loss_grad is not looked at. The first call gives the bytes of its workspace, 0 where a call is not of this kind or would need too much: the second refuses it then. The
+ * third multiplies gradients (null: not there) by *loss_grad, in place. */
+int b2_vocabulary_loss_both_workspace(const b2_vocabulary_loss* call, size_t* bytes);
+int b2_vocabulary_loss_both(const b2_vocabulary_loss* call, void* stream);
+int b2_vocabulary_loss_times(const b2_vocabulary_loss* call, void* stream);
 /* Every wait inside the kernels is bounded, by two seconds or `wait_ns`. Where one runs out, what depends on it is NaN, and the check below says so
  * once: 1, for calls on `device` that are done. */
-int b2_vocabulary_loss_within(const b2_vocabulary_loss* call, int backward, unsigned long long wait_ns, void* stream);
+int b2_vocabulary_loss_within(const b2_vocabulary_loss* call, int backward, unsigned long long wait_ns, void* stream); /* backward: 2 for both at once */
 int b2_vocabulary_loss_check_async_error(int device);
 
 #ifdef __cplusplus

@@ -15,7 +15,7 @@ _NATIVE = None
 # What the training operators call, in the order that the native module expects.
 _TRAIN = ("b2_last_error", "b2_pack8", "b2_unpack8", "b2_gelu8_forward", "b2_gelu8_backward", "b2_weight_grad8_workspace", "b2_weight_grad8",
           "b2_rotate_heads", "b2_rotate_heads_backward", "b2_embed", "b2_embed_backward_workspace", "b2_embed_backward", "b2_vocabulary_loss_sizes",
-          "b2_vocabulary_loss_forward", "b2_vocabulary_loss_backward")
+          "b2_vocabulary_loss_forward", "b2_vocabulary_loss_backward", "b2_vocabulary_loss_both_workspace", "b2_vocabulary_loss_both", "b2_vocabulary_loss_times")
 
 
 class B2Config(ctypes.Structure):

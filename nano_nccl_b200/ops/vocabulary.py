@@ -5,8 +5,12 @@ stands for no token (the padding of a sequence): it is looked up as zeros, has n
 the vocabulary makes NaN, so that a loss scaler sees it. (Rows that do not count still go through the products: their hidden states must be numbers.)
 
 The logits of 8192 tokens over 50257 words take 1.6 GB in 32 bits, and their gradient as much again. The losses here make them tile by tile on the tensor cores
-and keep one number for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: two of them) of the two products that
+and keep two numbers for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: two of them) of the two products that
 make the gradients. It needs 512 MB at most for that, or 4096 words of the vocabulary.
+
+bfloat16, with one loss for all rows: the logits are made once. A call whose inputs want gradients makes them with the loss, by pieces of the rows (512 MB of workspace, or as much as ``weight``
+has, and as much again for sums where there are several), and keeps them; the backward pass multiplies them by what comes back, which rounds once more unless that is a power of two.
+Asked for a second time (``retain_graph``) they are made from the logits.
 
 CUDA tensors of float32, float16 or bfloat16; calls run on the current stream of the tensors' device. As with the other operators of this package (:mod:`.checkpoint8`)
 reverse-mode gradients are made once, and tracing, forward mode and ``torch.func`` are refused; a step captured into a CUDA graph is captured with

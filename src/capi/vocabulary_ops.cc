@@ -48,7 +48,9 @@ kernels::EmbeddingCall embedding_of(const b2_embedding* e, bool backward, bool s
     return c;
 }
 
-kernels::VocabularyLossCall loss_of(const b2_vocabulary_loss* l, bool backward, bool sizes_only, void* stream) {
+// backward: 0 the loss, 1 its gradient, 2 both at once.
+kernels::VocabularyLossCall loss_of(const b2_vocabulary_loss* l, int backward, bool sizes_only, void* stream) {
+    B2_REQUIRE(backward >= 0 && backward <= 2, "unknown pass");
     B2_REQUIRE(l != nullptr, "null call");
     kernels::VocabularyLossCall c;
     c.dtype = dtype_of(l->dtype);
@@ -72,7 +74,7 @@ kernels::VocabularyLossCall loss_of(const b2_vocabulary_loss* l, bool backward, 
     c.distillation = l->entries != 0;
     c.entries = l->entries;
     c.teacher = l->teacher;
-    if (c.distillation && !backward) c.teacher_dtype = dtype_of(l->teacher_dtype);
+    if (c.distillation && backward != 1) c.teacher_dtype = dtype_of(l->teacher_dtype);
     for (int i = 0; i < 2; ++i) {
         c.target_strides[i] = l->target_strides[i];
         c.teacher_strides[i] = l->teacher_strides[i];
@@ -83,8 +85,8 @@ kernels::VocabularyLossCall loss_of(const b2_vocabulary_loss* l, bool backward, 
     c.kept = l->kept;
     c.loss_grad = l->loss_grad;
     c.loss_grad_stride = l->loss_grad_stride;
-    c.x_grad = backward ? l->x_grad : nullptr;
-    c.weight_grad = backward ? l->weight_grad : nullptr;
+    c.x_grad = backward != 0 ? l->x_grad : nullptr;
+    c.weight_grad = backward != 0 ? l->weight_grad : nullptr;
     c.workspace = l->workspace;
     c.stream = static_cast<cudaStream_t>(stream);
     // (The sizes depend on where x and the matrix lie: what TMA cannot read is copied.)
@@ -98,14 +100,15 @@ kernels::VocabularyLossCall loss_of(const b2_vocabulary_loss* l, bool backward, 
     if (c.tokens != 0) {
         B2_REQUIRE(c.targets != nullptr && c.kept != nullptr, "targets and what is kept must be non-null");
         B2_REQUIRE(aligned(c.targets, (std::size_t)l->target_bytes) && aligned(c.kept, 4), "a buffer is not aligned to its elements");
-        B2_REQUIRE(backward || !c.distillation || (c.teacher != nullptr && aligned(c.teacher, dtype_size(c.teacher_dtype))), "the teacher must be non-null and aligned to its elements");
+        B2_REQUIRE(backward == 1 || !c.distillation || (c.teacher != nullptr && aligned(c.teacher, dtype_size(c.teacher_dtype))), "the teacher must be non-null and aligned to its elements");
         B2_REQUIRE(c.workspace != nullptr && aligned(c.workspace, 256), "the workspace must start at a multiple of 256 bytes");
     }
-    if (!backward) {
+    if (backward != 1) {
         B2_REQUIRE(c.loss != nullptr || (c.tokens == 0 && c.reduction == kernels::LossReduction::None), "loss must be non-null");
         B2_REQUIRE(aligned(c.loss, 4), "a buffer is not aligned to its elements");
-    } else {
-        B2_REQUIRE(c.tokens == 0 || (c.loss_grad != nullptr && aligned(c.loss_grad, 4)), "loss_grad must be non-null and aligned to its elements");
+    }
+    if (backward == 1) B2_REQUIRE(c.tokens == 0 || (c.loss_grad != nullptr && aligned(c.loss_grad, 4)), "loss_grad must be non-null and aligned to its elements");
+    if (backward != 0) {
         B2_REQUIRE(aligned(c.x_grad, bytes) && aligned(c.weight_grad, bytes), "a buffer is not aligned to its elements");
     }
     return c;
@@ -132,7 +135,7 @@ int b2_embed_backward(const b2_embedding* call, void* stream) {
 
 int b2_vocabulary_loss_sizes(const b2_vocabulary_loss* call, int backward, size_t* kept_floats, size_t* workspace_bytes) {
     return guarded("vocabulary_loss", [&] {
-        const kernels::VocabularyLossCall c = loss_of(call, backward != 0, true, nullptr);
+        const kernels::VocabularyLossCall c = loss_of(call, backward != 0 ? 1 : 0, true, nullptr);
         if (kept_floats != nullptr) *kept_floats = kernels::vocabulary_loss_kept(c);
         if (workspace_bytes != nullptr) *workspace_bytes = kernels::vocabulary_loss_workspace(c, backward != 0);
     });
@@ -146,11 +149,32 @@ int b2_vocabulary_loss_backward(const b2_vocabulary_loss* call, void* stream) {
     return b2_vocabulary_loss_within(call, 1, kernels::VocabularyLossCall().wait_ns, stream);
 }
 
+int b2_vocabulary_loss_both_workspace(const b2_vocabulary_loss* call, size_t* bytes) {
+    return guarded("vocabulary_loss", [&] {
+        B2_REQUIRE(bytes != nullptr, "bytes must be non-null");
+        *bytes = kernels::vocabulary_loss_both_workspace(loss_of(call, 2, true, nullptr));
+    });
+}
+
+int b2_vocabulary_loss_both(const b2_vocabulary_loss* call, void* stream) {
+    return b2_vocabulary_loss_within(call, 2, kernels::VocabularyLossCall().wait_ns, stream);
+}
+
+int b2_vocabulary_loss_times(const b2_vocabulary_loss* call, void* stream) {
+    return guarded("vocabulary_loss", [&] {
+        kernels::VocabularyLossCall c = loss_of(call, 1, true, stream);
+        B2_REQUIRE(c.loss_grad != nullptr && aligned(c.loss_grad, 4), "loss_grad must be non-null and aligned to its elements");
+        B2_REQUIRE(aligned(c.x_grad, dtype_size(c.dtype)) && aligned(c.weight_grad, dtype_size(c.dtype)), "a buffer is not aligned to its elements");
+        kernels::launch_vocabulary_loss_times(c);
+    });
+}
+
 int b2_vocabulary_loss_within(const b2_vocabulary_loss* call, int backward, unsigned long long wait_ns, void* stream) {
     return guarded("vocabulary_loss", [&] {
-        kernels::VocabularyLossCall c = loss_of(call, backward != 0, false, stream);
+        kernels::VocabularyLossCall c = loss_of(call, backward, false, stream);
         c.wait_ns = wait_ns;
-        if (backward != 0) kernels::launch_vocabulary_loss_gradient(c);
+        if (backward == 2) kernels::launch_vocabulary_loss_both(c);
+        else if (backward == 1) kernels::launch_vocabulary_loss_gradient(c);
         else kernels::launch_vocabulary_loss(c);
     });
 }

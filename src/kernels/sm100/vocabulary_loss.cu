@@ -11,7 +11,14 @@
 //   WeightGrad  P^T x,   InputGrad  P w   of that piece
 // So the backward pass makes the logits a second time, a third more than the products that it cannot do without; keeping them would take 2 to 4 bytes for every token
 // and word of the vocabulary, from the forward pass on. Pieces of the vocabulary and not of the tokens, because a piece of dw is then
-// complete; dx, which is small, is added up in 32 bits. P is the operand of two products and therefore of their type: its rounding (2^-8 of each
+// complete; dx, which is small, is added up in 32 bits.
+//
+// bf16, one loss for all rows (both()): its gradient is known but for a factor when the loss is made, and bf16 has the exponents to do without a second product of
+// logits. What is stored of a piece of the rows is E = 2^((z - r_t) log2(e) / tau), r_t being the target's logit (the largest of the entries'), which a small kernel makes first:
+//   Exps  x w^T -> E in 16 bits, and its sums S_t over the words of a tile; close_kernel joins them and sets E of the targets to E - y S
+//   WeightGrad  E^T (x / S),   InputGrad  (E w) / S      and the backward pass multiplies by what comes back, if that is not 1
+// Where S_t passes 2^100 (a logit is 69 above the target's) a word in memory says so, and Stats, join_kernel and Probs, which look at it and end otherwise, make P instead.
+// 8192 x 50257 x 768, loss and gradients: 2030 -> 1694 us; 4096 x 131072 x 4096: 13.1 -> 9.7 ms. P is the operand of two products and therefore of their type: its rounding (2^-8 of each
 // element in bf16) is what the gradients lose beside their own. r_t = c_t / max |c| is 1 in a mean or a sum, so that the target's element
 // stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there.
 //
@@ -48,7 +55,7 @@ namespace {
 
 using u64 = unsigned long long;
 
-enum class Kind { Stats, Probs, WeightGrad, InputGrad };
+enum class Kind { Stats, Probs, Exps, WeightGrad, InputGrad };
 
 constexpr unsigned kTile = 256;  // of both axes of a pair's tile
 constexpr unsigned kHalf = 128;  // of one CTA
@@ -85,10 +92,12 @@ struct alignas(64) ProductArgs {
     bool prior, last;   // there are sums of earlier pieces; this is the last one
     unsigned* status;   // host memory
     u64 wait_ns;
-    // Stats and Probs
+    const unsigned* condition;  // nothing is done while this word is 0, or null
+    // Logits
     const unsigned* magnitudes;  // fp32: the largest of x and of w, see scale_of()
     float factor;                // log2(e) / temperature
     float2* stats; // [2 * tiles along n][m]
+    float* exp_sums;  // the same, of Exps
     float* picked; // [m]
     const void* targets;
     long long target_stride;
@@ -102,6 +111,7 @@ struct alignas(64) ProductArgs {
     // Gradients
     float* header;         // of the workspace: max |c|, and NaN once a product went wrong
     void* gradient;        // rows of n elements
+    const float* row_scale;  // [m], or null
     bool wide;             // TMA can write them
 };
 
@@ -254,10 +264,15 @@ __device__ __noinline__ void spoil(const ProductArgs& a, const Share& share, uns
     for (unsigned n = kKind == Kind::Probs ? share.all : 0; n < share.all;) {
         const Run r = share.at(a, n);
         const Tile t = tile_at(a, r.tile);
-        if constexpr (kKind == Kind::Stats) {
+        if constexpr (kKind == Kind::Stats || kKind == Kind::Exps) {
             const unsigned row = t.m + rank * kHalf + threadIdx.x % kHalf;
-            if (threadIdx.x < kHalf && row < a.m)
-                for (unsigned group = 0; group < 2; ++group) a.stats[(u64)(2u * (t.n / kTile) + group) * a.m + row] = make_float2(nan32(), nan32());
+            if (threadIdx.x < kHalf && row < a.m) {
+                for (unsigned group = 0; group < 2; ++group) {
+                    const u64 at = (u64)(2u * (t.n / kTile) + group) * a.m + row;
+                    if constexpr (kKind == Kind::Stats) a.stats[at] = make_float2(nan32(), nan32());
+                    else a.exp_sums[at] = nan32();
+                }
+            }
         } else {
             float* sums = r.whole ? a.sums + (u64)r.tile * kTileFloats : a.slots + (u64)r.slot * kTileFloats;
             const bool gradient = r.whole && a.last;
@@ -274,7 +289,7 @@ __device__ __noinline__ void spoil(const ProductArgs& a, const Share& share, uns
 // T: type of x, w and their gradients.
 template <Kind kKind, typename T>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
-    constexpr bool kLogits = kKind == Kind::Stats || kKind == Kind::Probs;
+    constexpr bool kLogits = kKind == Kind::Stats || kKind == Kind::Probs || kKind == Kind::Exps;
     constexpr bool kAByRows = kKind == Kind::WeightGrad, kBByRows = !kLogits;
     constexpr bool kHalfType = !std::is_same_v<T, __nv_bfloat16>;
     extern __shared__ unsigned char raw[];
@@ -288,6 +303,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     const Share share(a, blockIdx.x / 2u);
     const unsigned b_rows = a.n_tile / 2u;  // of a CTA
 
+    if ((kKind == Kind::Stats || kKind == Kind::Probs) && a.condition != nullptr) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (*a.condition == 0u) return;  // (both CTAs of a pair read the same)
+    }
     if (warp == 0 && lane == 0) {
         for (unsigned s = 0; s < kStages; ++s) {
             mbar_init(&bars.full[s], 1);
@@ -423,6 +442,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (kHalfType ? kHalfScale : 1.0f);
                         row_top = a.top[row];
                         share_of_sum = weight / a.sum[row];
+                    } else if constexpr (kKind == Kind::Exps) {
+                        weight = a.valid[row];
+                        row_top = a.top[row];
                     }
                 }
                 target = target < 0 ? -1 : target - (long long)(first + a.b_offset);
@@ -503,8 +525,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         top = now;
                     }
                     if (row < a.m) a.stats[(u64)(2u * (t.n / kTile) + group) * a.m + row] = make_float2(top, sum);
-                } else if constexpr (kKind == Kind::Probs) {
+                } else if constexpr (kLogits) {
                     const Pair32 factor = both32(a.factor), off = both32(-row_top);
+                    float some[4] = {};
                     for (unsigned c = 0; c < columns; c += 64u) {
                         float f[2][32];
 #pragma unroll
@@ -514,12 +537,17 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 #pragma unroll
                             for (unsigned j = 0; j < 32; j += 2) {
                                 const float2 e = apart(mul2(add2(pair32(f[h][j], f[h][j + 1]), off), factor));
-                                f[h][j] = share_of_sum * exp2_fast(e.x);
-                                f[h][j + 1] = share_of_sum * exp2_fast(e.y);
+                                f[h][j] = exp2_fast(e.x);
+                                f[h][j + 1] = exp2_fast(e.y);
+                                if constexpr (kKind == Kind::Probs) {
+                                    f[h][j] *= share_of_sum;
+                                    f[h][j + 1] *= share_of_sum;
+                                }
                             }
                             if (__any_sync(0xffffffffu, at < 32u)) {
+                                // (Exps: the target's is 1 by definition; its logit was made by another kernel, whose roundings differ.)
 #pragma unroll
-                                for (unsigned j = 0; j < 32; ++j) f[h][j] -= j == at ? weight : 0.0f;
+                                for (unsigned j = 0; j < 32; ++j) f[h][j] = j != at ? f[h][j] : (kKind == Kind::Probs ? f[h][j] - weight : 1.0f);
                             }
                             if (c + 32u * h + 32u > columns) {
 #pragma unroll
@@ -528,6 +556,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             if (weight == 0.0f) {
 #pragma unroll
                                 for (unsigned j = 0; j < 32; ++j) f[h][j] = 0.0f;
+                            }
+                            if constexpr (kKind == Kind::Exps) {
+#pragma unroll
+                                for (unsigned j = 0; j < 32; ++j) some[j & 3u] += f[h][j];
                             }
                         }
                         constexpr unsigned kParts = sizeof(T) == 4 ? 2 : 1;
@@ -548,8 +580,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             staging_out(&a.out, staging, first + c, t.m + in_tile, p, a.m);
                         }
                     }
+                    if constexpr (kKind == Kind::Exps) {
+                        if (row < a.m) a.exp_sums[(u64)(2u * (t.n / kTile) + group) * a.m + row] = (some[0] + some[1]) + (some[2] + some[3]);
+                    }
                 } else {
                     constexpr unsigned kBlock = 128u / sizeof(T);
+                    const float of_row = kKind == Kind::InputGrad && a.row_scale != nullptr && row < a.m ? scale * a.row_scale[row] : scale;
                     for (unsigned c = 0; c < columns; c += kBlock) {
                         staging_free();
 #pragma unroll
@@ -557,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             float f[32];
                             take(c + 32u * h, f);
 #pragma unroll
-                            for (unsigned j = 0; j < 32; ++j) f[j] *= scale;
+                            for (unsigned j = 0; j < 32; ++j) f[j] *= of_row;
                             stage<T>(staging, h, f);
                         }
                         if (a.wide) {
@@ -612,6 +648,7 @@ struct FinishArgs {
     float* sums;         // see ProductArgs
     bool prior, last;
     const float* header;
+    const float* row_scale;
     const unsigned* magnitudes;
     unsigned m, n, m_tiles, n_tiles, n_tile, whole_tiles, steps_of_tile, steps, groups;
     bool n_first;
@@ -667,7 +704,8 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     const unsigned m0 = (a.n_first ? tile_row : tile_column) * kTile + row0, n = (a.n_first ? tile_column : tile_row) * a.n_tile + column0 + lane;
 #pragma unroll
     for (unsigned r = warp; r < 32u; r += 8u)
-        if (m0 + r < a.m && n < a.n) static_cast<T*>(a.out)[(u64)(m0 + r) * a.n + n] = Elem<T>::from_f(turned[r][lane]);
+        if (m0 + r < a.m && n < a.n)
+            static_cast<T*>(a.out)[(u64)(m0 + r) * a.n + n] = Elem<T>::from_f(a.row_scale != nullptr ? turned[r][lane] * a.row_scale[m0 + r] : turned[r][lane]);
 }
 
 // ---- what stands around the products -----------------------------------------------------------------------
@@ -688,6 +726,8 @@ struct JoinArgs {
     float* sum;
     float* valid;
     float* loss;
+    const unsigned* condition;  // see ProductArgs
+    float* row_scale;           // 1 of rows that count, or null
 };
 
 // Each row's maximum and sum, and its loss. A CTA takes 32 rows, each of its warps every 32nd part of them (1024 rows of 394 parts: eight
@@ -695,6 +735,7 @@ struct JoinArgs {
 __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ JoinArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.condition != nullptr && *a.condition == 0u) return;
     constexpr unsigned kWarps = 32;
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x / 32u, row = blockIdx.x * 32u + lane;
     const float low = -__int_as_float(0x7f800000);
@@ -725,6 +766,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
         if (row < a.rows) {
             a.top[row] = top;
             a.sum[row] = sum;
+            if (a.row_scale != nullptr) a.row_scale[row] = 1.0f;  // (P has the rows' weights in it)
             if (a.entries == 0) {
                 const long long target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
                 const bool bad = target >= (long long)a.vocabulary;
@@ -800,13 +842,14 @@ struct EntriesArgs {
     const void* targets;
     long long target_strides[2];
     bool targets64;
-    const void* teacher;
+    const void* teacher;  // null: one entry of probability 1
     int teacher_dtype;
     long long teacher_strides[2];
     float temperature;
     float* z;
     float* p;
     float* valid;
+    float* top;  // the largest z, 0 of rows without entries; or null
 };
 
 __device__ __forceinline__ float load_as_float(const void* p, int dtype, long long at) {
@@ -816,7 +859,7 @@ __device__ __forceinline__ float load_as_float(const void* p, int dtype, long lo
 
 constexpr unsigned kEntryRounds = kMaxTeacherEntries / 32;
 
-// Distillation: the teacher's distribution over its entries, and the student's logits of them. A warp takes a row; reading the words' rows of the matrix
+// The teacher's distribution over its entries (cross entropy: the target), and the student's logits of them. A warp takes a row; reading the words' rows of the matrix
 // bounds it.
 template <typename T>
 __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ EntriesArgs a) {
@@ -835,7 +878,7 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
         p[i] = low;
         if (k < a.entries) {
             token[i] = target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)k * a.target_strides[1]);
-            if (token[i] >= 0) p[i] = load_as_float(a.teacher, a.teacher_dtype, (long long)row * a.teacher_strides[0] + (long long)k * a.teacher_strides[1]);
+            if (token[i] >= 0) p[i] = a.teacher == nullptr ? 0.0f : load_as_float(a.teacher, a.teacher_dtype, (long long)row * a.teacher_strides[0] + (long long)k * a.teacher_strides[1]);
             if (p[i] == low) token[i] = -1;
         }
         any |= token[i] >= 0;
@@ -858,6 +901,7 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
 #pragma unroll
     for (unsigned d = 16; d != 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) a.valid[row] = bad ? nan32() : (any ? 1.0f : 0.0f);
+    float most = low;
     const u64 out = (u64)row * a.entries;
     const T* x = static_cast<const T*>(a.x) + (long long)row * a.x_stride;
 #pragma unroll
@@ -912,7 +956,12 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
             }
         }
         if (k < a.entries) a.z[out + k] = z;
+        if (token[i] >= 0) most = fmaxf(most, z);
     }
+    if (a.top == nullptr) return;
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    if (lane == 0) a.top[row] = most == low ? 0.0f : most;
 }
 
 struct HeaderArgs {
@@ -971,6 +1020,7 @@ struct FixArgs {
     long long loss_grad_stride;
     float temperature, factor;
     const float* header;
+    const unsigned* condition;
 };
 
 // Distillation: the elements of P that the teacher has entries of. A warp takes a row; entries of the same word write the same.
@@ -979,7 +1029,7 @@ __global__ void __launch_bounds__(256) fix_kernel(const __grid_constant__ FixArg
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned lane = threadIdx.x & 31u, row = blockIdx.x * 8u + threadIdx.x / 32u;
-    if (row >= a.rows) return;
+    if (row >= a.rows || (a.condition != nullptr && *a.condition == 0u)) return;
     const float weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (std::is_same_v<T, __nv_bfloat16> ? 1.0f : kHalfScale);
     const float top = a.top[row], share_of_sum = weight / a.sum[row];
     long long token[kEntryRounds];
@@ -1017,6 +1067,165 @@ __global__ void __launch_bounds__(256) fix_kernel(const __grid_constant__ FixArg
             static_cast<__half*>(a.probs)[at] = part;
             static_cast<__half*>(a.probs)[(u64)a.rows * a.pitch + at] = __float2half_rn(v - __half2float(part));
         }
+    }
+}
+
+// Both at once: the rows' sums, their losses, what their gradients are divided by, and E of the targets.
+struct CloseArgs {
+    const float* exp_sums;  // [parts][rows]
+    unsigned rows, parts, entries;
+    long long vocabulary;
+    const void* targets;
+    long long target_strides[2];
+    bool targets64;
+    const float* z;  // [rows][entries]
+    const float* p;
+    const float* valid;
+    const float* top;
+    float temperature, factor;
+    float* sum;
+    float* loss;
+    float* row_scale;
+    unsigned* condition;  // set where a sum is too large for E
+    __nv_bfloat16* exps;  // [rows][pitch]
+    u64 pitch;
+};
+
+constexpr float kLargestSum = 1.2676506e30f;  // 2^100
+
+// A CTA takes 32 rows: each of its warps every 32nd part of them, then one row.
+__global__ void __launch_bounds__(1024) close_kernel(const __grid_constant__ CloseArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr unsigned kWarps = 32;
+    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x / 32u, first = blockIdx.x * 32u;
+    float sum = 0.0f;
+    if (first + lane < a.rows) {
+        for (unsigned p = warp; p < a.parts; p += 4u * kWarps) {
+            float v[4];
+#pragma unroll
+            for (unsigned i = 0; i < 4; ++i) v[i] = p + kWarps * i < a.parts ? a.exp_sums[(u64)(p + kWarps * i) * a.rows + first + lane] : 0.0f;
+            sum += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+    }
+    __shared__ float all[kWarps][33];
+    all[warp][lane] = sum;
+    __syncthreads();
+    const unsigned row = first + warp;
+    if (row >= a.rows) return;
+    sum = all[lane][warp];
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float valid = a.valid[row], top = a.top[row], log_sum = log2f(sum);
+    float loss = 0.0f;
+    for (unsigned k = lane; k - lane < a.entries; k += 32u) {
+        const u64 at = (u64)row * a.entries + k;
+        const long long token = k < a.entries ? target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)k * a.target_strides[1]) : -1;
+        const float p = k < a.entries ? a.p[at] : 0.0f, over = k < a.entries ? (a.z[at] - top) * a.factor : 0.0f;
+        if (p != 0.0f) loss += p * (logf(p) + kLn2 * (log_sum - over));
+        // Entries of the same word add up, and write the same.
+        float together = 0.0f;
+        for (unsigned e = 0; e < a.entries; ++e) {
+            const long long other = target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)e * a.target_strides[1]);
+            together += other == token ? a.p[(u64)row * a.entries + e] : 0.0f;
+        }
+        if (p != 0.0f && token >= 0 && token < a.vocabulary) a.exps[(u64)row * a.pitch + (u64)token] = __float2bfloat16_rn(exp2_fast(over) - together * sum);
+    }
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, d);
+    if (lane != 0) return;
+    a.sum[row] = sum;
+    a.loss[row] = valid == 0.0f ? 0.0f : loss * a.temperature * a.temperature * valid;
+    a.row_scale[row] = valid == 0.0f ? 0.0f : valid / sum;
+    if (valid != 0.0f && !(sum <= kLargestSum)) *a.condition = 1u;
+}
+
+struct CountArgs {
+    const float* valid;
+    unsigned rows;
+    bool mean;
+    float temperature;
+    float* count;
+    float* header;
+    unsigned* condition;
+    unsigned conditions;
+};
+
+// What all rows' gradients are multiplied with, before the backward pass.
+__global__ void __launch_bounds__(1024) count_kernel(const __grid_constant__ CountArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    unsigned count = 0;
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) count += a.valid[i] == 0.0f ? 0u : 1u;
+    for (unsigned i = threadIdx.x; i < a.conditions; i += 1024u) a.condition[i] = 0u;
+    __shared__ unsigned counts[32];
+    count = __reduce_add_sync(0xffffffffu, count);
+    if ((threadIdx.x & 31u) == 0) counts[threadIdx.x / 32u] = count;
+    __syncthreads();
+    if (threadIdx.x >= 32u) return;
+    count = __reduce_add_sync(0xffffffffu, counts[threadIdx.x]);
+    if (threadIdx.x == 0) {
+        *a.count = (float)count;
+        a.header[0] = a.mean ? a.temperature / fmaxf((float)count, 1.0f) : a.temperature;
+        a.header[1] = 0.0f;
+    }
+}
+
+struct DivideArgs {
+    const char* x;
+    long long stride;  // bytes
+    uint4* out;        // [rows][pitch]
+    unsigned rows, columns;
+    Divisor eights;  // of a row
+    const float* row_scale;
+};
+
+// Rows of x over their sums, rounded. A thread takes eight elements.
+__global__ void __launch_bounds__(256) divide_kernel(const __grid_constant__ DivideArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    using T = __nv_bfloat16;
+    const unsigned i = blockIdx.x * 256u + threadIdx.x, row = a.eights.divide(i), n = (i - row * a.eights.d) * 8u;
+    if (row >= a.rows) return;
+    unsigned w[4];
+    load_any<T, 8>(a.x + (long long)row * a.stride + (u64)n * 2u, n < a.columns ? min(8u, a.columns - n) : 0u, w);
+    const float scale = a.row_scale[row];
+    float f[8];
+    Wide<T>::unpack(make_uint4(w[0], w[1], w[2], w[3]), f);
+#pragma unroll
+    for (unsigned e = 0; e < 8; ++e) f[e] = scale == 0.0f ? 0.0f : f[e] * scale;
+    a.out[i] = Wide<T>::pack(f);
+}
+
+struct ScaleArgs {
+    __nv_bfloat16* gradients[2];
+    u64 elements[2];
+    const float* loss_grad;
+};
+
+// Gradients times what comes back to the loss. Most often that is 1, and there is nothing to do.
+__global__ void __launch_bounds__(512) times_kernel(const __grid_constant__ ScaleArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    using T = __nv_bfloat16;
+    const float scale = *a.loss_grad;
+    if (scale == 1.0f) return;
+    for (unsigned which = 0; which < 2; ++which) {
+        T* at = a.gradients[which];
+        if (at == nullptr) continue;
+        const u64 n = a.elements[which], step = (u64)gridDim.x * 512u, first = (u64)blockIdx.x * 512u + threadIdx.x;
+        const bool wide = reinterpret_cast<std::uintptr_t>(at) % 16u == 0;
+        const u64 eights = wide ? n / 8u : 0u;
+#pragma unroll 4
+        for (u64 i = first; i < eights; i += step) {
+            float f[8];
+            Wide<T>::unpack(reinterpret_cast<const uint4*>(at)[i], f);
+#pragma unroll
+            for (unsigned e = 0; e < 8; ++e) f[e] *= scale;
+            reinterpret_cast<uint4*>(at)[i] = Wide<T>::pack(f);
+        }
+        for (u64 i = eights * 8u + first; i < n; i += step) at[i] = __float2bfloat16_rn(__bfloat162float(at[i]) * scale);
     }
 }
 
@@ -1115,7 +1324,8 @@ int current_device() {
 
 template <Kind kKind>
 const void* kernel_of(DType dtype) {
-    switch (dtype) {
+    if constexpr (kKind == Kind::Exps) return (const void*)product_kernel<kKind, __nv_bfloat16>;
+    else switch (dtype) {
         case DType::Float: return (const void*)product_kernel<kKind, float>;
         case DType::Float16: return (const void*)product_kernel<kKind, __half>;
         default: return (const void*)product_kernel<kKind, __nv_bfloat16>;
@@ -1125,6 +1335,7 @@ const void* kernel_of(Kind kind, DType dtype) {
     switch (kind) {
         case Kind::Stats: return kernel_of<Kind::Stats>(dtype);
         case Kind::Probs: return kernel_of<Kind::Probs>(dtype);
+        case Kind::Exps: return kernel_of<Kind::Exps>(dtype);
         case Kind::WeightGrad: return kernel_of<Kind::WeightGrad>(dtype);
         default: return kernel_of<Kind::InputGrad>(dtype);
     }
@@ -1136,7 +1347,7 @@ unsigned pairs_of_device(int device) {
     static unsigned known[64] = {};
     std::lock_guard<std::mutex> lock(mutex);
     if (device >= 0 && device < 64 && known[device] != 0) return known[device];
-    for (Kind kind : {Kind::Stats, Kind::Probs, Kind::WeightGrad, Kind::InputGrad})
+    for (Kind kind : {Kind::Stats, Kind::Probs, Kind::Exps, Kind::WeightGrad, Kind::InputGrad})
         for (DType dtype : {DType::Float, DType::Float16, DType::BFloat16})
             B2_CUDA(cudaFuncSetAttribute(kernel_of(kind, dtype), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared));
     cudaLaunchConfig_t config = {};
@@ -1202,9 +1413,14 @@ struct Plan {
     std::size_t pitch = 0;  // elements of a row of the copies
     unsigned device_pairs = 0;
     u64 piece = 0, pieces = 1;  // words of the vocabulary
+    u64 rows = 0;                // both at once: of a piece
+    std::size_t exps_pitch = 0;
     unsigned n_tile = kTile;
-    std::size_t x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
+    std::size_t entries_at = 0, scale_at = 0, divided_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
 };
+
+// Both at once: bytes of E in a piece of the rows, or as many as the matrix has, and of the sums of dw where there are several.
+constexpr std::size_t kExpsBytes = 512ull << 20, kSumsBytes = 512ull << 20;
 
 bool readable(const void* p, long long stride, std::size_t columns, std::size_t rows, std::size_t element) {
     return reinterpret_cast<std::uintptr_t>(p) % 16 == 0 && (rows <= 1 || (stride * (long long)element % 16 == 0 && stride >= (long long)columns));
@@ -1213,7 +1429,9 @@ bool readable(const void* p, long long stride, std::size_t columns, std::size_t 
 // 128 columns of a gradient to a tile instead of 256, where that leaves fewer of them empty.
 unsigned n_tile_of(std::size_t width) { return (width + 127) / 128 * 128 < (width + 255) / 256 * 256 && width <= 640 ? 128u : 256u; }
 
-Plan plan_of(const VocabularyLossCall& c, bool gradient) {
+enum class Pass { Loss, Gradient, Both };
+
+Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     Plan p;
     const std::size_t e = dtype_size(c.dtype), t = c.tokens, v = c.vocabulary;
     p.parts = c.dtype == DType::Float ? 2 : 1;
@@ -1231,12 +1449,38 @@ Plan plan_of(const VocabularyLossCall& c, bool gradient) {
     p.weight_at = take(p.copy_weight ? p.parts * v * p.pitch * 2 : 0);
     bool summed = false;
     const auto look = [&](u64 m, u64 n, u64 k, unsigned n_tile, bool may_cut) { summed |= tiling_of(m, n, k, p.parts, n_tile, may_cut, p.device_pairs).summed; };
-    if (!gradient) {
+    if (pass == Pass::Loss) {
         p.stats_at = take((v + kTile - 1) / kTile * 2 * t * sizeof(float2));
         p.picked_at = take(t * sizeof(float));
         p.losses_at = take(t * sizeof(float));
         p.partial_at = take(c.dtype == DType::Float ? 2 * kMagnitudeCtas * sizeof(unsigned) : 0);
         look(t, v, c.width, kTile, false);
+    } else if (pass == Pass::Both) {
+        p.n_tile = n_tile_of(c.width);
+        p.exps_pitch = (v + kTile - 1) / kTile * kTile;
+        const std::size_t most = std::max(kExpsBytes, v * c.width * e) / (p.exps_pitch * 2) / kTile * kTile;
+        p.rows = std::min<u64>(t, std::max<std::size_t>(most, kTile));
+        p.pieces = (t + p.rows - 1) / p.rows;
+        p.rows = std::min<u64>(t, ((t + p.pieces - 1) / p.pieces + kTile - 1) / kTile * kTile);
+        p.pieces = (t + p.rows - 1) / p.rows;
+        p.stats_at = take(p.exps_pitch / kTile * 2 * p.rows * sizeof(float2));
+        p.picked_at = take(p.rows * sizeof(float));
+        p.losses_at = take(t * sizeof(float));
+        p.header_at = take((2 + p.pieces) * sizeof(float));
+        p.entries_at = take(c.distillation ? 0 : 2 * t * sizeof(float));
+        p.scale_at = take(p.rows * sizeof(float));
+        p.probs_at = take(p.rows * p.exps_pitch * 2);
+        if (c.weight_grad != nullptr) {
+            p.divided_at = take(p.rows * p.pitch * 2);
+            const std::size_t sums = p.exps_pitch / kTile * ((c.width + p.n_tile - 1) / p.n_tile) * kTileFloats * sizeof(float);
+            if (p.pieces > 1 && sums > kSumsBytes) return Plan();
+            if (p.pieces > 1) p.sums_at = take(sums);
+        }
+        for (const u64 rows : {p.rows, t - (p.pieces - 1) * p.rows}) {
+            look(rows, v, c.width, kTile, false);
+            if (c.weight_grad != nullptr) look(v, c.width, rows, p.n_tile, true);
+            if (c.x_grad != nullptr) look(rows, c.width, v, p.n_tile, true);
+        }
     } else {
         const u64 tiles = (v + kTile - 1) / kTile, bytes = (u64)p.parts * t * 2;
         const u64 most = std::max<u64>(std::min<u64>(kProbsBytes / bytes, kMatrixBytes / (p.parts * c.width * 2)), kLeastPiece) / kTile;
@@ -1325,6 +1569,7 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
     f.prior = a.prior;
     f.last = a.last;
     f.header = a.header;
+    f.row_scale = a.row_scale;
     f.magnitudes = a.magnitudes;
     f.m = a.m;
     f.n = a.n;
@@ -1409,36 +1654,40 @@ void logits_arguments(const VocabularyLossCall& c, ProductArgs& a) {
 }
 
 template <typename T>
+void launch_entries(const VocabularyLossCall& c, const Plan& p, const Operand& x, const Operand& w, float* z, float* prob, float* top) {
+    EntriesArgs e;
+    const bool copied = sizeof(T) == 2;  // (fp32 reads the original)
+    e.x = copied ? x.data : c.x;
+    e.x_stride = copied && p.copy_x ? (long long)p.pitch : c.x_stride;
+    e.weight = copied ? w.data : c.weight;
+    e.weight_stride = copied && p.copy_weight ? (long long)p.pitch : c.weight_stride;
+    e.rows = (unsigned)c.tokens;
+    e.width = (unsigned)c.width;
+    e.entries = c.distillation ? (unsigned)c.entries : 1u;
+    e.vocabulary = c.vocabulary;
+    e.targets = c.targets;
+    e.targets64 = c.targets64;
+    e.teacher = c.distillation ? c.teacher : nullptr;
+    e.teacher_dtype = static_cast<int>(c.teacher_dtype);
+    for (int i = 0; i < 2; ++i) {
+        e.target_strides[i] = c.target_strides[i];
+        e.teacher_strides[i] = c.teacher_strides[i];
+    }
+    e.temperature = c.temperature;
+    e.z = z;
+    e.p = prob;
+    e.valid = kept_of(c).valid;
+    e.top = top;
+    B2_CUDA(launch_dependent<EntriesArgs>(entries_kernel<T>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
+}
+
+template <typename T>
 void loss(const VocabularyLossCall& c, const Plan& p) {
     char* workspace = static_cast<char*>(c.workspace);
     const Kept kept = kept_of(c);
     Operand x, w;
     operands<T>(c, p, false, &x, &w);
-    if (c.distillation) {
-        EntriesArgs e;
-        const bool copied = sizeof(T) == 2;  // (fp32 reads the original)
-        e.x = copied ? x.data : c.x;
-        e.x_stride = copied && p.copy_x ? (long long)p.pitch : c.x_stride;
-        e.weight = copied ? w.data : c.weight;
-        e.weight_stride = copied && p.copy_weight ? (long long)p.pitch : c.weight_stride;
-        e.rows = (unsigned)c.tokens;
-        e.width = (unsigned)c.width;
-        e.entries = (unsigned)c.entries;
-        e.vocabulary = c.vocabulary;
-        e.targets = c.targets;
-        e.targets64 = c.targets64;
-        e.teacher = c.teacher;
-        e.teacher_dtype = static_cast<int>(c.teacher_dtype);
-        for (int i = 0; i < 2; ++i) {
-            e.target_strides[i] = c.target_strides[i];
-            e.teacher_strides[i] = c.teacher_strides[i];
-        }
-        e.temperature = c.temperature;
-        e.z = kept.z;
-        e.p = kept.p;
-        e.valid = kept.valid;
-        B2_CUDA(launch_dependent<EntriesArgs>(entries_kernel<T>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
-    }
+    if (c.distillation) launch_entries<T>(c, p, x, w, kept.z, kept.p, nullptr);
     ProductArgs a = {};
     a.a = map_of(operand_type<T>(), x, p.parts, kStep, kHalf);
     a.b = map_of(operand_type<T>(), w, p.parts, kStep, kHalf);
@@ -1465,6 +1714,8 @@ void loss(const VocabularyLossCall& c, const Plan& p) {
     j.top = kept.top;
     j.sum = kept.sum;
     j.valid = kept.valid;
+    j.condition = nullptr;
+    j.row_scale = nullptr;
     j.loss = c.reduction == LossReduction::None ? c.loss : reinterpret_cast<float*>(workspace + p.losses_at);
     B2_CUDA(launch_dependent<JoinArgs>(join_kernel, dim3((unsigned)((c.tokens + 31) / 32)), 1024, 0, c.stream, j));
     if (c.reduction == LossReduction::None) return;
@@ -1535,6 +1786,7 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
             f.loss_grad_stride = a.loss_grad_stride;
             f.temperature = c.temperature;
             f.header = header;
+            f.condition = nullptr;
             B2_CUDA(launch_dependent<FixArgs>(fix_kernel<T>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, f));
         }
         const unsigned columns = 128 / sizeof(T);
@@ -1570,18 +1822,219 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
     }
 }
 
+// bf16, one loss for all rows: the loss and, but for what comes back to it, its gradients.
+void both(const VocabularyLossCall& c, const Plan& p) {
+    using T = __nv_bfloat16;
+    char* workspace = static_cast<char*>(c.workspace);
+    const Kept kept = kept_of(c);
+    float* header = reinterpret_cast<float*>(workspace + p.header_at);
+    unsigned* conditions = reinterpret_cast<unsigned*>(header + 2);
+    float* losses = reinterpret_cast<float*>(workspace + p.losses_at);
+    float* row_scale = reinterpret_cast<float*>(workspace + p.scale_at);
+    const unsigned entries = c.distillation ? (unsigned)c.entries : 1u;
+    float* z = c.distillation ? kept.z : reinterpret_cast<float*>(workspace + p.entries_at);
+    float* prob = c.distillation ? kept.p : z + c.tokens;
+    Operand all_x, w;
+    operands<T>(c, p, false, &all_x, &w);
+    launch_entries<T>(c, p, all_x, w, z, prob, kept.top);
+    CountArgs n;
+    n.valid = kept.valid;
+    n.rows = (unsigned)c.tokens;
+    n.mean = c.reduction == LossReduction::Mean;
+    n.temperature = c.temperature;
+    n.count = kept.count;
+    n.header = header;
+    n.condition = conditions;
+    n.conditions = (unsigned)p.pieces;
+    B2_CUDA(launch_dependent<CountArgs>(count_kernel, dim3(1), 1024, 0, c.stream, n));
+    for (u64 piece = 0; piece < p.pieces; ++piece) {
+        const u64 first = piece * p.rows, rows = std::min<u64>(p.rows, c.tokens - first);
+        const long long element = c.targets64 ? 8 : 4;
+        const void* targets = static_cast<const char*>(c.targets) + (long long)first * c.target_strides[0] * element;
+        const Operand x = {static_cast<const char*>(all_x.data) + first * all_x.row_bytes, c.width, rows, all_x.row_bytes};
+        const Operand exps = {workspace + p.probs_at, p.exps_pitch, rows, p.exps_pitch * 2};
+        unsigned* condition = conditions + piece;
+        ProductArgs a = {};
+        a.a = map_of(DType::BFloat16, x, 1, kStep, kHalf);
+        a.b = map_of(DType::BFloat16, w, 1, kStep, kHalf);
+        a.out = map_of(DType::BFloat16, exps, 1, 64, 32);
+        logits_arguments(c, a);
+        a.targets = targets;
+        a.exp_sums = reinterpret_cast<float*>(workspace + p.stats_at);
+        a.stats = reinterpret_cast<float2*>(workspace + p.stats_at);
+        a.picked = reinterpret_cast<float*>(workspace + p.picked_at);
+        a.top = kept.top + first;
+        a.sum = kept.sum + first;
+        a.valid = kept.valid + first;
+        a.header = header;
+        a.slots = reinterpret_cast<float*>(workspace + p.slots_at);
+        const Tiling logits = tiling_of(rows, c.vocabulary, c.width, 1, kTile, false, p.device_pairs);
+        launch_product(Kind::Exps, c, logits, a, rows, c.vocabulary);
+        CloseArgs s;
+        s.exp_sums = a.exp_sums;
+        s.rows = (unsigned)rows;
+        s.parts = 2 * logits.n_tiles;
+        s.entries = entries;
+        s.vocabulary = (long long)c.vocabulary;
+        s.targets = targets;
+        s.target_strides[0] = c.target_strides[0];
+        s.target_strides[1] = c.target_strides[1];
+        s.targets64 = c.targets64;
+        s.z = z + first * entries;
+        s.p = prob + first * entries;
+        s.valid = a.valid;
+        s.top = a.top;
+        s.temperature = c.temperature;
+        s.factor = a.factor;
+        s.sum = kept.sum + first;
+        s.loss = losses + first;
+        s.row_scale = row_scale;
+        s.condition = condition;
+        s.exps = reinterpret_cast<T*>(workspace + p.probs_at);
+        s.pitch = p.exps_pitch;
+        const dim3 by_32((unsigned)((rows + 31) / 32));
+        B2_CUDA(launch_dependent<CloseArgs>(close_kernel, by_32, 1024, 0, c.stream, s));
+        // Where E has not the exponents: P, from the largest logits.
+        a.condition = condition;
+        launch_product(Kind::Stats, c, logits, a, rows, c.vocabulary);
+        JoinArgs j;
+        j.stats = a.stats;
+        j.rows = (unsigned)rows;
+        j.parts = 2 * logits.n_tiles;
+        j.picked = a.picked;
+        j.targets = targets;
+        j.target_stride = c.target_strides[0];
+        j.targets64 = c.targets64;
+        j.vocabulary = c.vocabulary;
+        j.z = s.z;
+        j.p = s.p;
+        j.entries = (unsigned)c.entries;
+        j.temperature = c.temperature;
+        j.factor = a.factor;
+        j.top = kept.top + first;
+        j.sum = kept.sum + first;
+        j.valid = kept.valid + first;
+        j.loss = losses + first;
+        j.condition = condition;
+        j.row_scale = row_scale;
+        B2_CUDA(launch_dependent<JoinArgs>(join_kernel, by_32, 1024, 0, c.stream, j));
+        launch_product(Kind::Probs, c, logits, a, rows, c.vocabulary);
+        if (c.distillation) {
+            FixArgs f;
+            f.probs = workspace + p.probs_at;
+            f.rows = (unsigned)rows;
+            f.pitch = (unsigned)p.exps_pitch;
+            f.entries = entries;
+            f.first = 0;
+            f.columns = (long long)c.vocabulary;
+            f.targets = targets;
+            f.target_strides[0] = c.target_strides[0];
+            f.target_strides[1] = c.target_strides[1];
+            f.targets64 = c.targets64;
+            f.z = s.z;
+            f.p = s.p;
+            f.top = a.top;
+            f.sum = a.sum;
+            f.valid = a.valid;
+            f.loss_grad = nullptr;
+            f.loss_grad_stride = 0;
+            f.temperature = c.temperature;
+            f.factor = a.factor;
+            f.header = header;
+            f.condition = condition;
+            B2_CUDA(launch_dependent<FixArgs>(fix_kernel<T>, dim3((unsigned)((rows + 7) / 8)), 256, 0, c.stream, f));
+        }
+        a.condition = nullptr;
+        const auto gradient_of = [&](void* out, u64 of_rows) {
+            a.gradient = out;
+            a.wide = c.width * sizeof(T) % 16 == 0 && reinterpret_cast<std::uintptr_t>(out) % 16 == 0;
+            if (a.wide) a.out = map_of(DType::BFloat16, {out, c.width, of_rows, c.width * sizeof(T)}, 1, 64, 32);
+        };
+        if (c.weight_grad != nullptr) {
+            DivideArgs d;
+            d.x = static_cast<const char*>(x.data);
+            d.stride = (long long)x.row_bytes;
+            d.out = reinterpret_cast<uint4*>(workspace + p.divided_at);
+            d.rows = (unsigned)rows;
+            d.columns = (unsigned)c.width;
+            d.eights = Divisor((unsigned)(p.pitch / 8));
+            d.row_scale = row_scale;
+            const u64 eights = rows * (p.pitch / 8);
+            B2_REQUIRE(eights < (1ull << 31), kTooLarge);
+            B2_CUDA(launch_dependent<DivideArgs>(divide_kernel, dim3((unsigned)((eights + 255) / 256)), 256, 0, c.stream, d));
+            const Tiling t = tiling_of(c.vocabulary, c.width, rows, 1, p.n_tile, true, p.device_pairs);
+            a.a = map_of(DType::BFloat16, exps, 1, 64, kStep);
+            a.b = map_of(DType::BFloat16, {d.out, c.width, rows, p.pitch * 2}, 1, 64, kStep);
+            a.sums = p.pieces > 1 ? reinterpret_cast<float*>(workspace + p.sums_at) : nullptr;
+            a.prior = piece != 0;
+            a.last = piece + 1 == p.pieces;
+            gradient_of(c.weight_grad, c.vocabulary);
+            launch_product(Kind::WeightGrad, c, t, a, c.vocabulary, c.width);
+            finish<Kind::WeightGrad, T>(c, t, a);
+        }
+        if (c.x_grad != nullptr) {
+            const Tiling t = tiling_of(rows, c.width, c.vocabulary, 1, p.n_tile, true, p.device_pairs);
+            a.a = map_of(DType::BFloat16, exps, 1, kStep, kHalf);
+            a.b = map_of(DType::BFloat16, w, 1, 64, kStep);
+            a.sums = nullptr;
+            a.prior = false;
+            a.last = true;
+            a.row_scale = row_scale;
+            gradient_of(static_cast<T*>(c.x_grad) + first * c.width, rows);
+            launch_product(Kind::InputGrad, c, t, a, rows, c.width);
+            finish<Kind::InputGrad, T>(c, t, a);
+        }
+    }
+    SumArgs s;
+    s.losses = losses;
+    s.valid = kept.valid;
+    s.rows = (unsigned)c.tokens;
+    s.mean = n.mean;
+    s.out = c.loss;
+    s.count = kept.count;
+    B2_CUDA(launch_dependent<SumArgs>(sum_kernel, dim3(1), 1024, 0, c.stream, s));
+}
+
+// Whether both() makes a call's gradients.
+bool at_once(const VocabularyLossCall& c) {
+    return c.dtype == DType::BFloat16 && c.reduction != LossReduction::None && c.tokens != 0 && (c.x_grad != nullptr || c.weight_grad != nullptr);
+}
+
 }  // namespace
 
 std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 3 + 3 + 2 * c.tokens * (std::size_t)c.entries; }
 
-std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient) { return call.tokens == 0 ? 0 : plan_of(call, gradient).bytes; }
+std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient) {
+    return call.tokens == 0 ? 0 : plan_of(call, gradient ? Pass::Gradient : Pass::Loss).bytes;
+}
+
+std::size_t vocabulary_loss_both_workspace(const VocabularyLossCall& call) { return at_once(call) ? plan_of(call, Pass::Both).bytes : 0; }
+
+void launch_vocabulary_loss_both(const VocabularyLossCall& c) {
+    const Plan p = at_once(c) ? plan_of(c, Pass::Both) : Plan();
+    B2_REQUIRE(p.bytes != 0, "the loss and its gradient are not made at once of such a call");
+    both(c, p);
+}
+
+void launch_vocabulary_loss_times(const VocabularyLossCall& c) {
+    B2_REQUIRE(c.dtype == DType::BFloat16, "gradients of bf16 only are made with the loss");
+    ScaleArgs a;
+    a.gradients[0] = static_cast<__nv_bfloat16*>(c.x_grad);
+    a.gradients[1] = static_cast<__nv_bfloat16*>(c.weight_grad);
+    a.elements[0] = (u64)c.tokens * c.width;
+    a.elements[1] = (u64)c.vocabulary * c.width;
+    a.loss_grad = c.loss_grad;
+    const u64 most = std::max(a.gradients[0] != nullptr ? a.elements[0] : 0, a.gradients[1] != nullptr ? a.elements[1] : 0);
+    if (most == 0) return;
+    B2_CUDA(launch_dependent<ScaleArgs>(times_kernel, dim3((unsigned)std::min<u64>(148 * 4, (most + 4095) / 4096)), 512, 0, c.stream, a));
+}
 
 void launch_vocabulary_loss(const VocabularyLossCall& c) {
     if (c.tokens == 0) {
         if (c.reduction != LossReduction::None) B2_CUDA(cudaMemsetAsync(c.loss, 0, sizeof(float), c.stream));
         return;
     }
-    const Plan p = plan_of(c, false);
+    const Plan p = plan_of(c, Pass::Loss);
     switch (c.dtype) {
         case DType::Float: return loss<float>(c, p);
         case DType::Float16: return loss<__half>(c, p);
@@ -1595,7 +2048,7 @@ void launch_vocabulary_loss_gradient(const VocabularyLossCall& c) {
         if (c.weight_grad != nullptr) B2_CUDA(cudaMemsetAsync(c.weight_grad, 0, c.vocabulary * c.width * dtype_size(c.dtype), c.stream));
         return;
     }
-    const Plan p = plan_of(c, true);
+    const Plan p = plan_of(c, Pass::Gradient);
     switch (c.dtype) {
         case DType::Float: return gradient<float>(c, p);
         case DType::Float16: return gradient<__half>(c, p);

@@ -48,5 +48,10 @@ std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradi
 // Both throw std::runtime_error on a failed launch. Where a wait inside a kernel runs out, what depends on it is NaN.
 void launch_vocabulary_loss(const VocabularyLossCall& call);
 void launch_vocabulary_loss_gradient(const VocabularyLossCall& call);
+// The loss together with the gradients that are wanted, for a loss_grad of 1: bf16, one loss for all rows. Its workspace; 0 where that is not so, or would take too much of it.
+std::size_t vocabulary_loss_both_workspace(const VocabularyLossCall& call);
+void launch_vocabulary_loss_both(const VocabularyLossCall& call);
+// x_grad and weight_grad, where they are, times loss_grad, in place.
+void launch_vocabulary_loss_times(const VocabularyLossCall& call);
 
 }  // namespace b200ccl::kernels

@@ -597,7 +597,7 @@ PyMethodDef train_methods[] = {
     {nullptr, nullptr, 0, nullptr}};
 
 bool bind_train(PyObject* error_class, PyObject* addresses) {
-    constexpr Py_ssize_t kAddresses = 15;
+    constexpr Py_ssize_t kAddresses = 18;
     unsigned long long a[kAddresses];
     if (!PyTuple_Check(addresses) || PyTuple_GET_SIZE(addresses) != kAddresses) {
         PyErr_Format(PyExc_TypeError, "expected a tuple of %zd addresses", kAddresses);

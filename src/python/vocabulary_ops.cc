@@ -18,6 +18,9 @@ struct Functions {
     decltype(&b2_vocabulary_loss_sizes) loss_sizes = nullptr;
     decltype(&b2_vocabulary_loss_forward) loss_forward = nullptr;
     decltype(&b2_vocabulary_loss_backward) loss_backward = nullptr;
+    decltype(&b2_vocabulary_loss_both_workspace) both_workspace = nullptr;
+    decltype(&b2_vocabulary_loss_both) both = nullptr;
+    decltype(&b2_vocabulary_loss_times) times = nullptr;
 } g;
 
 const at::Tensor& whole_numbers(const char* what, const at::Tensor& t) {
@@ -147,8 +150,13 @@ void prepare(Prepared* p, const at::Tensor& x, const at::Tensor& weight, const a
     c.reduction = static_cast<int>(asked.reduction);
 }
 
-// (loss, what its backward pass reads)
-std::pair<at::Tensor, at::Tensor> loss_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets, const at::Tensor& teacher, const Asked& asked) {
+struct Lost {
+    at::Tensor loss, kept;           // kept: what the backward pass reads
+    at::Tensor x_grad, weight_grad;  // made with the loss, but for what comes back to it
+};
+
+// wanted: gradients that will be asked for, and may be made with the loss.
+Lost loss_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets, const at::Tensor& teacher, const Asked& asked, bool x_wanted, bool weight_wanted) {
     const c10::cuda::CUDAGuard guard(x.device());
     Prepared p;
     prepare(&p, x, weight, targets, asked);
@@ -160,26 +168,43 @@ std::pair<at::Tensor, at::Tensor> loss_forward(const at::Tensor& x, const at::Te
         p.c.teacher_strides[1] = 1;
     }
     const auto options = x.options().dtype(at::kFloat).requires_grad(false);
-    at::Tensor loss = at::empty(asked.reduction == 0 ? x.sizes().slice(0, x.dim() - 1).vec() : std::vector<std::int64_t>(), options);
-    std::size_t floats = 0, bytes = 0;
+    Lost r;
+    r.loss = at::empty(asked.reduction == 0 ? x.sizes().slice(0, x.dim() - 1).vec() : std::vector<std::int64_t>(), options);
+    std::size_t floats = 0, bytes = 0, both = 0;
     call([&] { return g.loss_sizes(&p.c, 0, &floats, &bytes); });
-    at::Tensor kept = at::empty({static_cast<std::int64_t>(floats)}, options), workspace = new_bytes(x, static_cast<std::int64_t>(bytes));
-    p.c.loss = static_cast<float*>(loss.data_ptr());
-    p.c.kept = static_cast<float*>(kept.data_ptr());
+    r.kept = at::empty({static_cast<std::int64_t>(floats)}, options);
+    p.c.loss = static_cast<float*>(r.loss.data_ptr());
+    p.c.kept = static_cast<float*>(r.kept.data_ptr());
+    if ((x_wanted || weight_wanted) && x.scalar_type() == at::kBFloat16 && asked.reduction != 0) {
+        if (x_wanted) r.x_grad = new_like(x);
+        if (weight_wanted) r.weight_grad = new_like(weight);
+        p.c.x_grad = x_wanted ? r.x_grad.data_ptr() : nullptr;
+        p.c.weight_grad = weight_wanted ? r.weight_grad.data_ptr() : nullptr;
+        call([&] { return g.both_workspace(&p.c, &both); });
+    }
+    at::Tensor workspace = new_bytes(x, static_cast<std::int64_t>(both != 0 ? both : bytes));
     p.c.workspace = workspace.data_ptr();
     void* stream = stream_of(x);
-    call([&] { return g.loss_forward(&p.c, stream); });
-    return {std::move(loss), std::move(kept)};
+    if (both != 0) {
+        call([&] { return g.both(&p.c, stream); });
+    } else {
+        r.x_grad = r.weight_grad = at::Tensor();
+        call([&] { return g.loss_forward(&p.c, stream); });
+    }
+    return r;
 }
 
 struct VocabularyLoss : torch::autograd::Function<VocabularyLoss> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets, const std::optional<at::Tensor>& teacher,
                               std::int64_t entries, double temperature, std::int64_t reduction) {
-        auto [loss, kept] = loss_forward(x, weight, targets, teacher.has_value() ? *teacher : at::Tensor(), {entries, temperature, reduction});
-        ctx->save_for_backward({x, weight, targets, kept});
+        Lost r = loss_forward(x, weight, targets, teacher.has_value() ? *teacher : at::Tensor(), {entries, temperature, reduction}, x.requires_grad(), weight.requires_grad());
+        ctx->save_for_backward({x, weight, targets, r.kept});
+        // (Not among what is saved: whoever asks for them first takes them away.)
+        if (r.x_grad.defined()) ctx->saved_data["dx"] = std::move(r.x_grad);
+        if (r.weight_grad.defined()) ctx->saved_data["dw"] = std::move(r.weight_grad);
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["whole"] = std::vector<std::int64_t>{entries, reduction};
-        return loss;
+        return r.loss;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         return in_backward("the loss", [&]() -> variable_list {
@@ -195,18 +220,32 @@ struct VocabularyLoss : torch::autograd::Function<VocabularyLoss> {
             const Rows back = flat_of("dloss", dloss);
             if (dloss.numel() != (asked.reduction == 0 ? p.x.rows : 1)) refuse("dloss has another shape than the loss");
             variable_list result(7);
-            if (ctx->needs_input_grad(0)) result[0] = new_like(x);
-            if (ctx->needs_input_grad(1)) result[1] = new_like(weight);
             p.c.kept = static_cast<float*>(kept.data_ptr());
             p.c.loss_grad = static_cast<const float*>(back.t.data_ptr());
             p.c.loss_grad_stride = back.stride;
-            p.c.x_grad = result[0].defined() ? result[0].data_ptr() : nullptr;
-            p.c.weight_grad = result[1].defined() ? result[1].data_ptr() : nullptr;
+            void* stream = stream_of(x);
+            // What was made with the loss, once; asked for again, it is made from the logits, as if it had not been.
+            constexpr const char* kMade[2] = {"dx", "dw"};
+            void** const gradients[2] = {&p.c.x_grad, &p.c.weight_grad};
+            for (int i = 0; i < 2; ++i) {
+                const auto made = ctx->saved_data.find(kMade[i]);
+                if (!ctx->needs_input_grad(i) || made == ctx->saved_data.end()) continue;
+                result[i] = made->second.toTensor();
+                ctx->saved_data.erase(made);
+                *gradients[i] = result[i].data_ptr();
+            }
+            if (p.c.x_grad != nullptr || p.c.weight_grad != nullptr) call([&] { return g.times(&p.c, stream); });
+            p.c.x_grad = p.c.weight_grad = nullptr;
+            for (int i = 0; i < 2; ++i) {
+                if (!ctx->needs_input_grad(i) || result[i].defined()) continue;
+                result[i] = new_like(i == 0 ? x : weight);
+                *gradients[i] = result[i].data_ptr();
+            }
+            if (p.c.x_grad == nullptr && p.c.weight_grad == nullptr) return result;
             std::size_t bytes = 0;
             call([&] { return g.loss_sizes(&p.c, 1, nullptr, &bytes); });
             at::Tensor workspace = new_bytes(x, static_cast<std::int64_t>(bytes));
             p.c.workspace = workspace.data_ptr();
-            void* stream = stream_of(x);
             call([&] { return g.loss_backward(&p.c, stream); });
             return result;
         });
@@ -224,7 +263,7 @@ PyObject* loss_of(at::Tensor x, at::Tensor weight, const at::Tensor& targets, co
         const std::optional<at::Tensor> maybe = teacher.defined() ? std::optional<at::Tensor>(teacher) : std::nullopt;
         return THPVariable_Wrap(VocabularyLoss::apply(x, weight, targets, maybe, asked.entries, asked.temperature, asked.reduction));
     }
-    return THPVariable_Wrap(loss_forward(x, weight, targets, teacher, asked).first);
+    return THPVariable_Wrap(loss_forward(x, weight, targets, teacher, asked, false, false).loss);
 }
 
 std::int64_t reduction_of(PyObject* obj) {
@@ -274,6 +313,9 @@ void bind_vocabulary(const unsigned long long* a) {
     take(g.loss_sizes, a[3]);
     take(g.loss_forward, a[4]);
     take(g.loss_backward, a[5]);
+    take(g.both_workspace, a[6]);
+    take(g.both, a[7]);
+    take(g.times, a[8]);
 }
 
 }  // namespace b200ccl::python

@@ -86,7 +86,12 @@ def losses(x, weight, targets, teacher_logits=None, temperature=1.0, reduction="
     for name, p, e, m, summed in (("dx", dz, element, w, vocabulary), ("dw", dz.t(), element.t(), a, rows)):
         exact = p @ m
         sums = p.abs() @ m.abs()
-        out[name] = (exact, e @ m.abs() + _floor(dtype, m) * p.abs().sum(-1, keepdim=True) + (_sums(dtype, summed) + 16 * 2.0 ** -24) * sums + h * (exact.abs() + e @ m.abs()) + smallest(dtype))
+        # bf16, one loss for all rows: what is multiplied with x is 1 / S of P's row, S times P beside x / S, which is rounded as P is. Once in the sum of magnitudes, then.
+        # And what comes back to the loss is multiplied with a rounded gradient, and the product rounded.
+        made_with_the_loss = dtype == torch.bfloat16 and reduction != "none"
+        sums_of_rounded = h * (sums + e @ m.abs()) if name == "dw" and made_with_the_loss else 0.0
+        roundings = (2 + h) if made_with_the_loss else 1
+        out[name] = (exact, sums_of_rounded + e @ m.abs() + _floor(dtype, m) * p.abs().sum(-1, keepdim=True) + (_sums(dtype, summed) + 16 * 2.0 ** -24) * sums + roundings * h * (exact.abs() + sums_of_rounded + e @ m.abs()) + smallest(dtype))
     return out
 
 

@@ -55,8 +55,10 @@ def check(call, x, weight, targets, reduction, logits=None, temperature=1.0):
     want = plain.losses(x.reshape(rows, -1), weight, flat(targets, 0 if logits is None else 1), flat(logits, 1), temperature, reduction, dloss.reshape(-1) if reduction == "none" else dloss)
     for name, value in want.items():
         plain.within(out[name].reshape(value[0].shape), value, name)
-    with torch.no_grad():
-        assert torch.equal(call(x, weight), out["loss"])
+    with torch.no_grad():  # (bf16, one loss for all rows: by another way than with gradients)
+        loss = call(x, weight)
+        plain.within(loss.reshape(want["loss"][0].shape), want["loss"], "loss alone")
+        assert torch.equal(loss, out["loss"]) or (x.dtype == torch.bfloat16 and reduction != "none")
     again = run(call, x, weight, dloss)
     assert all(torch.equal(a, b) for a, b in zip(out.values(), again.values()))
     return out
@@ -199,6 +201,54 @@ def test_rows_that_are_sure(dtype):
     t = torch.where(torch.arange(rows, device="cuda") % 2 == 0, v - 1, 0)
     out = check(cross_entropy(t, "none"), x.to(dtype), w.to(dtype), t, "none")
     assert (out["loss"] >= 0).all() and out["loss"][-1] > 400 and out["loss"][-2] < 0.2
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_logits_too_far_above_the_target_s(wide):
+    """bf16, one loss for all rows: sums of exponentials over the target's that pass 2^100, in some pieces of the rows and not in others, and a few words over the edge."""
+    rows, v, h = (200, 300, 64) if not wide else (14000, 30000, 64)  # (in two pieces of the rows)
+    x, w, t = inputs(rows, v, h, torch.bfloat16)
+    logits, tokens = teacher(rows, 5, v, torch.bfloat16)
+    far = x.clone()
+    far[rows - 7] = w[5] * 40 * h ** 0.5  # (a logit of word 5 of a few hundred)
+    over = t.clone()
+    over[rows - 7] = 9
+    tokens[tokens == 5] = 6
+    calls = [(cross_entropy(over, "mean"), far, over, None, 1.0), (distillation(logits, tokens, 0.5, "sum"), far, tokens, logits, 0.5)]
+    if not wide:
+        calls += [(cross_entropy(over, "sum"), (far.float() * s).bfloat16(), over, None, 1.0) for s in (0.02, 0.04, 0.05, 0.06, 0.08, 0.5, 2.0)]
+    for call, given, targets, kind, tau in calls:
+        check(call, given, w, targets, "mean" if call is calls[0][0] else "sum", kind, tau)
+
+
+def test_gradients_made_with_the_loss():
+    """bf16, one loss for all rows: asked for twice, apart, multiplied with what comes back, of a loss whose inputs changed."""
+    x, w, t = inputs(300, 2000, 72, torch.bfloat16)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, t)
+    one = torch.ones((), device="cuda")
+    want = plain.losses(x, w, t, dloss=one)
+    (dx,) = torch.autograd.grad(loss, x, retain_graph=True)
+    kept = dx.clone()
+    (dw,) = torch.autograd.grad(loss, w, retain_graph=True)
+    again = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    assert torch.equal(dx, kept)
+    for name, value in (("dx", dx), ("dw", dw), ("dx", again[0]), ("dw", again[1])):
+        plain.within(value, want[name], name)
+    for scale in (0.0, 0.5, -3.0, 65536.0, float("nan")):
+        got = torch.autograd.grad(ops.linear_cross_entropy(x, w, t) * scale, (x, w))
+        for a, b in zip(got, (dx, dw)):
+            assert torch.equal(a.nan_to_num(7.0), (b.float() * scale).bfloat16().nan_to_num(7.0))
+    loss = ops.linear_cross_entropy(x, w, t)
+    with torch.no_grad():
+        x.mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    # Two losses of the same matrix in one backward pass.
+    first, second = ops.linear_cross_entropy(x, w, t), ops.linear_cross_entropy(x[:100], w, t[:100])
+    got = torch.autograd.grad(first + second, w)[0]
+    parts = [torch.autograd.grad(ops.linear_cross_entropy(x[:n], w, t[:n]), w)[0] for n in (300, 100)]
+    assert torch.equal(got, parts[0] + parts[1])
 
 
 def test_gradients_by_differences():
