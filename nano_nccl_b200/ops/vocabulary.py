@@ -8,8 +8,8 @@ The logits of 8192 tokens over 50257 words take 1.6 GB in 32 bits, and their gra
 and keep two numbers for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: two of them) of the two products that
 make the gradients. It needs 512 MB at most for that, or 4096 words of the vocabulary.
 
-bfloat16, with one loss for all rows: the logits are made once. A call whose inputs want gradients makes them with the loss, by pieces of the rows (512 MB of workspace, or as much as ``weight``
-has, and as much again for sums where there are several), and keeps them; the backward pass multiplies them by what comes back, which rounds once more unless that is a power of two.
+bfloat16, with one loss for all rows and a product large enough: the logits are made once. A call whose inputs want gradients makes them with the loss, by pieces of the rows (1 GB of workspace,
+and as much again at most for sums where there are several), and keeps them; the backward pass multiplies them by what comes back, which rounds once more unless that is a power of two.
 Asked for a second time (``retain_graph``) they are made from the logits.
 
 CUDA tensors of float32, float16 or bfloat16; calls run on the current stream of the tensors' device. As with the other operators of this package (:mod:`.checkpoint8`)

@@ -18,7 +18,7 @@
 //   Exps  x w^T -> E in 16 bits, and its sums S_t over the words of a tile; close_kernel joins them and sets E of the targets to E - y S
 //   WeightGrad  E^T (x / S),   InputGrad  (E w) / S      and the backward pass multiplies by what comes back, if that is not 1
 // Where S_t passes 2^100 (a logit is 69 above the target's) a word in memory says so, and Stats, join_kernel and Probs, which look at it and end otherwise, make P instead.
-// 8192 x 50257 x 768, loss and gradients: 2030 -> 1694 us; 4096 x 131072 x 4096: 13.1 -> 9.7 ms. P is the operand of two products and therefore of their type: its rounding (2^-8 of each
+// 8192 x 50257 x 768, loss and gradients: 2025 -> 1459 us; 4096 x 131072 x 4096: 13.2 -> 10.2 ms. P is the operand of two products and therefore of their type: its rounding (2^-8 of each
 // element in bf16) is what the gradients lose beside their own. r_t = c_t / max |c| is 1 in a mean or a sum, so that the target's element
 // stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there.
 //
@@ -28,8 +28,9 @@
 // The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and sums are added up in memory, rounded, after every 1024
 // elements of the summed axis; in 16-bit types after 16384.
 //
-// Tiles of the gradients that do not go evenly into the pairs are cut along the summed axis, evenly: pair i takes steps [i S / P, (i+1) S / P) of those that are
-// left, and finish_kernel adds the pieces in order. Nothing depends on timing.
+// P pairs take P whole tiles of a gradient at a time, as long as there are so many. Those that are left are cut along the summed axis, all into the same number of pieces, which go over the pairs
+// piece by piece and not tile by tile: pairs are at the same words, or tokens, then, and read them from L2 once one of them has. (Steps dealt out evenly, tile by
+// tile: 4096 x 50257 x 768, the gradient of x, 300 us instead of 205, at the rate of HBM.) finish_kernel adds the pieces in order. Nothing depends on timing.
 #include "kernels/sm100/vocabulary_loss.h"
 
 #include "core/check.h"
@@ -85,9 +86,10 @@ struct alignas(64) ProductArgs {
     unsigned m_tiles, n_tiles, n_tile;  // n_tile: extent of a tile along n, 256 or 128
     unsigned parts, steps_of_part, steps_of_tile;
     unsigned b_offset;  // added to b's row
-    unsigned pairs, waves, steps, groups;  // whole tiles of a pair; the steps of the tiles that are left, and the pairs that share them
+    unsigned pairs, waves;  // whole tiles of a pair
+    unsigned left, splits;  // tiles that are left, and the pieces of each
     bool n_first;       // neighbouring tiles lie along n
-    float* slots;       // [2 * pairs][tile]: pieces, and sums of long tiles
+    float* slots;       // [splits][left][tile], then [pairs][tile]: pieces, and sums of long tiles
     float* sums;        // [tiles][tile]: sums of all pieces of the vocabulary, or null
     bool prior, last;   // there are sums of earlier pieces; this is the last one
     unsigned* status;   // host memory
@@ -127,43 +129,33 @@ struct Barriers {
 };
 static_assert(sizeof(Barriers) <= 256);
 
-// pair * steps / pairs, in 32 bits: pairs are few.
-__host__ __device__ inline unsigned first_step(unsigned pair, unsigned steps, unsigned pairs) {
-    const unsigned each = steps / pairs;
-    return pair * each + pair * (steps - each * pairs) / pairs;
+// Where piece i of n of a tile's steps begins.
+__host__ __device__ inline unsigned piece_begin(unsigned i, unsigned steps, unsigned n) {
+    const unsigned each = steps / n;
+    return i * each + i * (steps - each * n) / n;
 }
 
-// What a pair does, in order: `waves` whole tiles, then its steps of the tiles that are left. A run of steps of one tile:
+// What a pair does, in order: `waves` whole tiles, then pieces of those that are left. A run of steps of one tile:
 struct Run {
     unsigned tile, from, to;
     bool whole;     // this pair sums all of the tile
-    unsigned slot;  // of a piece, or of a long sum (a pair's last piece comes after its whole tiles)
+    unsigned slot;  // of a piece, or of a long sum
 };
 struct Share {
-    unsigned pair, begin, end, whole, all;
+    unsigned pair, runs;
     __device__ __forceinline__ Share(const ProductArgs& a, unsigned p) : pair(p) {
-        begin = first_step(min(p, a.groups), a.steps, a.groups);
-        end = first_step(min(p + 1u, a.groups), a.steps, a.groups);
-        whole = a.waves * a.steps_of_tile;
-        all = whole + (end - begin);
+        const unsigned pieces = a.left * a.splits;
+        runs = a.waves + (pair < pieces ? (pieces - pair + a.pairs - 1u) / a.pairs : 0u);
     }
-    __device__ __forceinline__ Run at(const ProductArgs& a, unsigned n) const {
+    __device__ __forceinline__ Run at(const ProductArgs& a, unsigned i) const {
+        if (i < a.waves) return {i * a.pairs + pair, 0u, a.steps_of_tile, true, a.left * a.splits + pair};
+        const unsigned piece = pair + (i - a.waves) * a.pairs, part = piece / a.left;
         Run r;
-        if (n < whole) {
-            const unsigned wave = n / a.steps_of_tile;
-            r.tile = wave * a.pairs + pair;
-            r.from = n - wave * a.steps_of_tile;
-            r.to = a.steps_of_tile;
-            r.whole = true;
-            r.slot = 2u * pair + 1u;
-        } else {
-            const unsigned at = begin + (n - whole), row = at / a.steps_of_tile, tile_at = row * a.steps_of_tile;
-            r.tile = a.waves * a.pairs + row;
-            r.from = at - tile_at;
-            r.to = min(a.steps_of_tile, end - tile_at);
-            r.whole = tile_at >= begin && tile_at + a.steps_of_tile <= end;
-            r.slot = 2u * pair + (tile_at <= begin ? 0u : 1u);
-        }
+        r.tile = a.waves * a.pairs + (piece - part * a.left);
+        r.from = piece_begin(part, a.steps_of_tile, a.splits);
+        r.to = piece_begin(part + 1u, a.steps_of_tile, a.splits);
+        r.whole = a.splits == 1u;
+        r.slot = r.whole ? a.left * a.splits + pair : piece;
         return r;
     }
 };
@@ -261,8 +253,8 @@ __device__ __forceinline__ float row_weight(float valid, const float* loss_grad,
 template <Kind kKind, typename T>
 __device__ __noinline__ void spoil(const ProductArgs& a, const Share& share, unsigned rank) {
     if (kKind == Kind::Probs && threadIdx.x == 0) a.header[1] = nan32();
-    for (unsigned n = kKind == Kind::Probs ? share.all : 0; n < share.all;) {
-        const Run r = share.at(a, n);
+    for (unsigned i = kKind == Kind::Probs ? share.runs : 0; i < share.runs; ++i) {
+        const Run r = share.at(a, i);
         const Tile t = tile_at(a, r.tile);
         if constexpr (kKind == Kind::Stats || kKind == Kind::Exps) {
             const unsigned row = t.m + rank * kHalf + threadIdx.x % kHalf;
@@ -276,13 +268,12 @@ __device__ __noinline__ void spoil(const ProductArgs& a, const Share& share, uns
         } else {
             float* sums = r.whole ? a.sums + (u64)r.tile * kTileFloats : a.slots + (u64)r.slot * kTileFloats;
             const bool gradient = r.whole && a.last;
-            for (unsigned i = threadIdx.x; i < kHalf * a.n_tile; i += kThreads) {
-                const unsigned row = rank * kHalf + i % kHalf, column = i / kHalf;
+            for (unsigned e = threadIdx.x; e < kHalf * a.n_tile; e += kThreads) {
+                const unsigned row = rank * kHalf + e % kHalf, column = e / kHalf;
                 if (!gradient) sums[((column / 4u) * kTile + row) * 4u + column % 4u] = nan32();
                 else if (t.m + row < a.m && t.n + column < a.n) static_cast<T*>(a.gradient)[(u64)(t.m + row) * a.n + t.n + column] = Elem<T>::from_f(nan32());
             }
         }
-        n += r.to - r.from;
     }
 }
 
@@ -340,8 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             const unsigned bytes = kOperandBytes + b_rows * 128u;
             unsigned n = 0;
             bool ok = true;
-            while (n < share.all && ok) {
-                const Run r = share.at(a, n);
+            for (unsigned i = 0; i < share.runs && ok; ++i) {
+                const Run r = share.at(a, i);
                 const Tile t = tile_at(a, r.tile);
                 const int m = (int)(t.m + rank * kHalf), at = (int)(t.n + rank * b_rows);
                 for (unsigned k = r.from; k < r.to; ++k, ++n) {
@@ -376,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             const unsigned shape = product_shape(kTile, a.n_tile, !kHalfType, kAByRows, kBByRows);
             unsigned n = 0, segments = 0;
             bool ok = true;
-            while (n < share.all && ok) {
-                const Run r = share.at(a, n);
+            for (unsigned i = 0; i < share.runs && ok; ++i) {
+                const Run r = share.at(a, i);
                 for (unsigned k = r.from; k < r.to && ok; ++segments) {
                     const unsigned end = segment_end(a, k, r.to), buffer = segments & 1u;
                     ok = wait_phase<true>(bar(bars.sums_free[buffer]), ((segments >> 1) & 1u) ^ 1u, failed, a.wait_ns);
@@ -392,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         const std::uint64_t x = kAByRows ? operand_by_rows(operand_a(s), kBlockBytes) : operand_by_columns(operand_a(s));
                         const std::uint64_t y = kBByRows ? operand_by_rows(operand_b(s), kBlockBytes) : operand_by_columns(operand_b(s));
 #pragma unroll
-                        for (unsigned i = 0; i < kStep / 16; ++i) {
-                            mma_pair(tmem + buffer * kTile, x + i * (kAByRows ? 2048 >> 4 : 32 >> 4), y + i * (kBByRows ? 2048 >> 4 : 32 >> 4), shape, add);
+                        for (unsigned j = 0; j < kStep / 16; ++j) {
+                            mma_pair(tmem + buffer * kTile, x + j * (kAByRows ? 2048 >> 4 : 32 >> 4), y + j * (kBByRows ? 2048 >> 4 : 32 >> 4), shape, add);
                             add = true;
                         }
                         commit_pair(bar(bars.empty[s]));
@@ -406,7 +397,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             commit_pair(bar(bars.drained));
             for (unsigned polls = 0; polls < 1000u && !phase_over<false>(bar(bars.drained), 0); ++polls) {}
         } else if (lane == 0) {
-            for (unsigned n = 0; n < share.all; ++n) {
+            unsigned steps = 0;
+            for (unsigned i = 0; i < share.runs; ++i) {
+                const Run r = share.at(a, i);
+                steps += r.to - r.from;
+            }
+            for (unsigned n = 0; n < steps; ++n) {
                 if (!wait_phase(bar(bars.full[n % kStages]), (n / kStages) & 1u, failed, a.wait_ns)) break;
                 mbar_arrive_at(bar(bars.full_other[n % kStages]), 0);
             }
@@ -424,10 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             back_x = both32(scale_of(a.magnitudes[0], true));
             back_w = both32(scale_of(a.magnitudes[1], true));
         }
-        unsigned n = 0, segments = 0;
+        unsigned segments = 0;
         bool ok = true;
-        while (n < share.all && ok) {
-            const Run r = share.at(a, n);
+        for (unsigned i = 0; i < share.runs && ok; ++i) {
+            const Run r = share.at(a, i);
             const Tile t = tile_at(a, r.tile);
             const unsigned first = t.n + column0, row = t.m + in_tile + lane;
             const unsigned columns = first < a.n ? min(b_rows, a.n - first) : 0u;  // of this warp
@@ -603,12 +599,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             const unsigned rows = t.m + in_tile < a.m ? min(32u, a.m - t.m - in_tile) : 0u;
                             T* to = static_cast<T*>(a.gradient) + (u64)(t.m + in_tile) * a.n + first + c;
 #pragma unroll 8
-                            for (unsigned i = 0; i < 32u; ++i) {
+                            for (unsigned s = 0; s < 32u; ++s) {
 #pragma unroll
                                 for (unsigned h = 0; h < kBlock / 32u; ++h) {
                                     const unsigned j = lane + 32u * h, at = j * (unsigned)sizeof(T);
-                                    const T v = *reinterpret_cast<const T*>(shared + (staging - base) + i * 128u + (((at >> 4) ^ (i & 7u)) << 4) + (at & 15u));
-                                    if (i < rows && c + j < columns) to[(u64)i * a.n + j] = v;
+                                    const T v = *reinterpret_cast<const T*>(shared + (staging - base) + s * 128u + (((at >> 4) ^ (s & 7u)) << 4) + (at & 15u));
+                                    if (s < rows && c + j < columns) to[(u64)s * a.n + j] = v;
                                 }
                             }
                             __syncwarp();
@@ -618,7 +614,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at(bar(bars.sums_free[buffer]), 0);
-                n += end - k;
                 k = end;
             }
         }
@@ -650,7 +645,7 @@ struct FinishArgs {
     const float* header;
     const float* row_scale;
     const unsigned* magnitudes;
-    unsigned m, n, m_tiles, n_tiles, n_tile, whole_tiles, steps_of_tile, steps, groups;
+    unsigned m, n, m_tiles, n_tiles, n_tile, whole_tiles, left, splits;
     bool n_first;
 };
 
@@ -660,13 +655,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned columns = a.n_tile / 32u, blocks = 8u * columns, index = blockIdx.x / blocks, block = blockIdx.x % blocks;
-    const unsigned tile = a.whole_tiles + index, from = index * a.steps_of_tile, to = from + a.steps_of_tile;
-    // The pairs whose steps are of this tile, in order; a pair's last tile, if it began before it, is its second piece.
-    const unsigned pair = min(threadIdx.x, kMaxPairs);
-    const unsigned begin = first_step(min(pair, a.groups), a.steps, a.groups), end = first_step(min(pair + 1u, a.groups), a.steps, a.groups);
-    const unsigned before = __syncthreads_count(threadIdx.x < a.groups && end <= from);
-    const unsigned pieces = __syncthreads_count(threadIdx.x < a.groups && end > from && begin < to);
-    if (__syncthreads_or(threadIdx.x < a.groups && begin <= from && end >= to)) return;  // not cut
+    const unsigned tile = a.whole_tiles + index;
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x / 32u, row0 = block / columns * 32u, column0 = block % columns * 32u;
     const unsigned at = (column0 / 4u + warp) * kTile + row0 + lane;  // four columns of a row
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -678,12 +667,12 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     };
     if (a.prior) add(reinterpret_cast<const float4*>(a.sums + (u64)tile * kTileFloats)[at]);
     constexpr unsigned kAtOnce = 8;
-    for (unsigned p = 0; p < pieces; p += kAtOnce) {
+    for (unsigned p = 0; p < a.splits; p += kAtOnce) {
         float4 v[kAtOnce];
 #pragma unroll
         for (unsigned i = 0; i < kAtOnce; ++i) {
-            const unsigned piece = before + p + i, slot = 2u * piece + (i + p == 0 && from > first_step(piece, a.steps, a.groups) ? 1u : 0u);
-            v[i] = p + i < pieces ? reinterpret_cast<const float4*>(a.slots + (u64)slot * kTileFloats)[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4* piece = reinterpret_cast<const float4*>(a.slots + (u64)((p + i) * a.left + index) * kTileFloats);
+            v[i] = p + i < a.splits ? piece[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
         for (unsigned i = 0; i < kAtOnce; ++i) add(v[i]);
@@ -860,8 +849,8 @@ __device__ __forceinline__ float load_as_float(const void* p, int dtype, long lo
 constexpr unsigned kEntryRounds = kMaxTeacherEntries / 32;
 
 // The teacher's distribution over its entries (cross entropy: the target), and the student's logits of them. A warp takes a row; reading the words' rows of the matrix
-// bounds it.
-template <typename T>
+// bounds it: eight of them at a time, or one where there are no more (its loads are on the way together then).
+template <typename T, unsigned kAtOnce>
 __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ EntriesArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -910,7 +899,6 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
         const unsigned k = lane + 32u * i;
         if (k < a.entries) a.p[out + k] = any ? p[i] / sum : 0.0f;
         float z = 0.0f;  // of this lane's entry
-        constexpr unsigned kAtOnce = 8;
         const unsigned there = min(32u, a.entries - 32u * i);
         for (unsigned e = 0; e < there; e += kAtOnce) {
             const T* w[kAtOnce];
@@ -921,12 +909,14 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
                 w[j] = t >= 0 ? static_cast<const T*>(a.weight) + t * a.weight_stride : nullptr;
             }
             if constexpr (sizeof(T) == 4) {
+#pragma unroll(kAtOnce == 1 ? 8 : 1)
                 for (unsigned h = lane; h < a.width; h += 32u) {
                     const float v = x[h];
 #pragma unroll
                     for (unsigned j = 0; j < kAtOnce; ++j) dot[j] += w[j] != nullptr ? v * w[j][h] : 0.0f;
                 }
             } else {
+#pragma unroll(kAtOnce == 1 ? 4 : 1)
                 for (unsigned h = lane * 8u; h < a.width; h += 256u) {
                     const unsigned n = min(8u, a.width - h);  // (what lies behind a row may be anything)
                     const uint4 nothing = make_uint4(0u, 0u, 0u, 0u);
@@ -1369,8 +1359,8 @@ unsigned pairs_of_device(int device) {
 
 // How the pairs share the tiles of one product.
 struct Tiling {
-    unsigned m_tiles = 0, n_tiles = 0, n_tile = kTile, parts = 1, steps_of_part = 0, steps_of_tile = 0, pairs = 0, waves = 0, steps = 0, groups = 1;
-    bool cut = false, summed = false;  // pieces; sums in memory at all
+    unsigned m_tiles = 0, n_tiles = 0, n_tile = kTile, parts = 1, steps_of_part = 0, steps_of_tile = 0, pairs = 0, waves = 0, left = 0, splits = 1;
+    std::size_t slots = 0;  // sums in memory: pieces, and long sums
 };
 
 Tiling tiling_of(u64 m, u64 n, u64 summed, unsigned parts, unsigned n_tile, bool may_cut, unsigned device_pairs) {
@@ -1384,17 +1374,23 @@ Tiling tiling_of(u64 m, u64 n, u64 summed, unsigned parts, unsigned n_tile, bool
     t.n_tiles = (unsigned)n_tiles;
     t.steps_of_part = (unsigned)steps;
     t.steps_of_tile = (unsigned)steps_of_tile;
-    // A pair for each tile; where they may be cut, for every eight steps of one.
-    t.pairs = (unsigned)std::min<u64>(device_pairs, may_cut ? std::max(tiles, tiles * steps_of_tile / 8) : tiles);
+    t.pairs = device_pairs;
     t.waves = (unsigned)tiles / t.pairs;
-    const unsigned left = (unsigned)tiles - t.waves * t.pairs;
-    t.steps = left * t.steps_of_tile;
-    // The tiles that are left are cut where that saves every pair more than eight steps, which is what writing and adding pieces costs.
-    t.groups = t.pairs;
-    if (!may_cut || t.steps_of_tile < 8 + t.steps / t.pairs) t.groups = std::max(1u, left);
-    if (t.waves == 0) t.pairs = t.groups;
-    for (unsigned i = 1; i < t.groups && left != 0; ++i) t.cut |= first_step(i, t.steps, t.groups) % t.steps_of_tile != 0;
-    t.summed = t.cut || t.steps_of_tile > (parts > 1 ? kProducts * kChunkSteps : kLongSteps);
+    t.left = (unsigned)tiles - t.waves * t.pairs;
+    // The tiles that are left are cut where that saves more steps than writing the pieces and adding them costs: about sixteen, and half a step for each piece of a tile.
+    if (may_cut && t.left != 0) {
+        u64 least = t.steps_of_tile;
+        for (unsigned splits = 2; splits <= std::min(t.pairs, t.steps_of_tile / 8) && t.left * splits <= 4 * t.pairs; ++splits) {
+            const u64 cost = (u64)((t.left * splits + t.pairs - 1) / t.pairs) * ((t.steps_of_tile + splits - 1) / splits) + 16 + splits / 2;
+            if (cost >= least) continue;
+            least = cost;
+            t.splits = splits;
+        }
+    }
+    if (t.waves == 0) t.pairs = std::min(t.pairs, t.left * t.splits);
+    if (t.splits > 1) t.slots = (std::size_t)t.left * t.splits;
+    // (Pieces come first, whether they are cut or not: see Share.)
+    if (t.steps_of_tile > (parts > 1 ? kProducts * kChunkSteps : kLongSteps)) t.slots = (std::size_t)t.left * t.splits + t.pairs;
     return t;
 }
 
@@ -1419,8 +1415,9 @@ struct Plan {
     std::size_t entries_at = 0, scale_at = 0, divided_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
 };
 
-// Both at once: bytes of E in a piece of the rows, or as many as the matrix has, and of the sums of dw where there are several.
-constexpr std::size_t kExpsBytes = 512ull << 20, kSumsBytes = 512ull << 20;
+// Both at once: bytes of E in a piece of the rows, and of the sums of dw where there are several. (8192 x 50257 x 768, loss and gradients: 1459 us in one piece of 824 MB, 1565 in two,
+// 1684 in four; 4096 x 131072 x 4096: 10.2 ms in one, two or four.)
+constexpr std::size_t kExpsBytes = 1ull << 30, kSumsBytes = 1ull << 30;
 
 bool readable(const void* p, long long stride, std::size_t columns, std::size_t rows, std::size_t element) {
     return reinterpret_cast<std::uintptr_t>(p) % 16 == 0 && (rows <= 1 || (stride * (long long)element % 16 == 0 && stride >= (long long)columns));
@@ -1447,8 +1444,10 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     };
     p.x_at = take(p.copy_x ? p.parts * t * p.pitch * 2 : 0);
     p.weight_at = take(p.copy_weight ? p.parts * v * p.pitch * 2 : 0);
-    bool summed = false;
-    const auto look = [&](u64 m, u64 n, u64 k, unsigned n_tile, bool may_cut) { summed |= tiling_of(m, n, k, p.parts, n_tile, may_cut, p.device_pairs).summed; };
+    std::size_t slots = 0;
+    const auto look = [&](u64 m, u64 n, u64 k, unsigned n_tile, bool may_cut) {
+        slots = std::max(slots, tiling_of(m, n, k, p.parts, n_tile, may_cut, p.device_pairs).slots);
+    };
     if (pass == Pass::Loss) {
         p.stats_at = take((v + kTile - 1) / kTile * 2 * t * sizeof(float2));
         p.picked_at = take(t * sizeof(float));
@@ -1458,7 +1457,7 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     } else if (pass == Pass::Both) {
         p.n_tile = n_tile_of(c.width);
         p.exps_pitch = (v + kTile - 1) / kTile * kTile;
-        const std::size_t most = std::max(kExpsBytes, v * c.width * e) / (p.exps_pitch * 2) / kTile * kTile;
+        const std::size_t most = kExpsBytes / (p.exps_pitch * 2) / kTile * kTile;
         p.rows = std::min<u64>(t, std::max<std::size_t>(most, kTile));
         p.pieces = (t + p.rows - 1) / p.rows;
         p.rows = std::min<u64>(t, ((t + p.pieces - 1) / p.pieces + kTile - 1) / kTile * kTile);
@@ -1499,7 +1498,7 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
             if (c.x_grad != nullptr) look(t, c.width, words, p.n_tile, true);
         }
     }
-    p.slots_at = take(summed ? (std::size_t)2 * p.device_pairs * kTileFloats * sizeof(float) : 0);
+    p.slots_at = take(slots * kTileFloats * sizeof(float));
     p.bytes = at;
     return p;
 }
@@ -1536,8 +1535,8 @@ void launch_product(Kind kind, const VocabularyLossCall& c, const Tiling& t, Pro
     a.steps_of_tile = t.steps_of_tile;
     a.pairs = t.pairs;
     a.waves = t.waves;
-    a.steps = t.steps;
-    a.groups = t.groups;
+    a.left = t.left;
+    a.splits = t.splits;
     a.n_first = kind == Kind::WeightGrad || kind == Kind::InputGrad;
     a.status = wait_status_word(WaitsOf::VocabularyLoss, current_device());
     a.wait_ns = c.wait_ns;
@@ -1561,7 +1560,7 @@ void launch_product(Kind kind, const VocabularyLossCall& c, const Tiling& t, Pro
 // The pieces of a gradient's cut tiles.
 template <Kind kKind, typename T>
 void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) {
-    if (!t.cut) return;
+    if (t.splits == 1) return;
     FinishArgs f;
     f.out = a.gradient;
     f.slots = a.slots;
@@ -1577,12 +1576,10 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
     f.n_tiles = t.n_tiles;
     f.n_tile = t.n_tile;
     f.whole_tiles = t.waves * t.pairs;
-    f.steps_of_tile = t.steps_of_tile;
-    f.steps = t.steps;
-    f.groups = t.groups;
+    f.left = t.left;
+    f.splits = t.splits;
     f.n_first = a.n_first;
-    const unsigned left = t.steps / t.steps_of_tile;
-    B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<kKind, T>, dim3(left * 8 * (t.n_tile / 32)), 256, 0, c.stream, f));
+    B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<kKind, T>, dim3(t.left * 8 * (t.n_tile / 32)), 256, 0, c.stream, f));
 }
 
 struct Kept {
@@ -1678,7 +1675,7 @@ void launch_entries(const VocabularyLossCall& c, const Plan& p, const Operand& x
     e.p = prob;
     e.valid = kept_of(c).valid;
     e.top = top;
-    B2_CUDA(launch_dependent<EntriesArgs>(entries_kernel<T>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
+    B2_CUDA(launch_dependent<EntriesArgs>(e.entries == 1 ? entries_kernel<T, 1> : entries_kernel<T, 8>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
 }
 
 template <typename T>
@@ -1995,8 +1992,11 @@ void both(const VocabularyLossCall& c, const Plan& p) {
     B2_CUDA(launch_dependent<SumArgs>(sum_kernel, dim3(1), 1024, 0, c.stream, s));
 }
 
-// Whether both() makes a call's gradients.
+// Whether both() makes a call's gradients. Its kernels are more, which counts where the products are small, up to a whole tile of rows (us, apart / at once; rows x words x columns in thousand
+// millions): 512 x 512 x 64 90 / 93 (0.02), 512 x 5000 x 256 90 / 95 (0.7), 1024 x 5000 x 256 101 / 99 (1.3), 16 x 32000 x 768 91 / 96 (6.3), 16 x 50257 x 768 111 / 103 (9.9),
+// 512 x 32000 x 768 132 / 126 (12.6), 1024 x 50257 x 768 277 / 230 (40).
 bool at_once(const VocabularyLossCall& c) {
+    if (std::max<std::size_t>(c.tokens, kTile) * c.vocabulary < (1ull << 33) / std::max<std::size_t>(c.width, 1)) return false;
     return c.dtype == DType::BFloat16 && c.reduction != LossReduction::None && c.tokens != 0 && (c.x_grad != nullptr || c.weight_grad != nullptr);
 }
 

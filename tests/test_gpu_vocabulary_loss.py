@@ -8,6 +8,7 @@ import nano_nccl_b200 as nn
 import plain_vocabulary as plain
 from nano_nccl_b200 import ops
 from test_cpu_vocabulary_ops import LL, VocabularyLoss
+from test_gpu_linear8 import replaced
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -117,6 +118,59 @@ def test_pieces_of_the_vocabulary(dtype):
     check(distillation(logits, tokens, 2.0, "mean"), x, w, tokens, "mean", logits, 2.0)
 
 
+def made_with_the_loss(x, w, t):
+    """Whether the gradients of this call are made with the loss: its node has them."""
+    calls = []
+    prototype = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
+    with replaced("b2_vocabulary_loss_both", prototype, lambda original, *arguments: calls.append(1) or original(*arguments)):
+        ops.linear_cross_entropy(x.detach().requires_grad_(), w, t)
+    return bool(calls)
+
+
+# bf16, one loss for all rows, a matrix of 2^25 elements at least (256 rows of products are 2^33 then): the logits are made once.
+@pytest.mark.parametrize("rows,vocabulary,width", [(1, 50257, 768), (5, 9001, 3800), (257, 33000, 1030), (300, 470000, 72), (1000, 40000, 856), (700, 70001, 1003)])
+def test_gradients_made_with_the_loss(rows, vocabulary, width):
+    x, w, t = inputs(rows, vocabulary, width, torch.bfloat16)
+    assert made_with_the_loss(x, w, t)
+    for reduction in ("mean", "sum"):
+        check(cross_entropy(t, reduction), x, w, t, reduction)
+    logits, tokens = teacher(rows, 33, vocabulary, torch.bfloat16)
+    tokens = torch.where(torch.rand(tokens.shape, device="cuda", generator=gen(3)) < 0.1, -1, tokens)
+    logits = torch.where(torch.rand(tokens.shape, device="cuda", generator=gen(4)) < 0.1, -torch.inf, logits)
+    tokens[2::11], logits[5::11] = -7, -torch.inf
+    tokens[:, 3] = tokens[:, 4]  # the same word twice
+    check(distillation(logits, tokens, 1.5, "mean"), x, w, tokens, "mean", logits, 1.5)
+
+
+def test_gradients_made_with_the_loss_by_pieces_of_the_rows():
+    """More than 1 GB of exponentials, and a last piece of a few rows more than half."""
+    x, w, t = inputs(14001, 40000, 840, torch.bfloat16)
+    assert made_with_the_loss(x, w, t)
+    check(cross_entropy(t, "mean"), x, w, t, "mean")
+    logits, tokens = teacher(14001, 3, 40000, torch.float32)
+    check(distillation(logits, tokens, 2.0, "sum"), x, w, tokens, "sum", logits, 2.0)
+
+
+def test_rows_and_strides_of_gradients_made_with_the_loss():
+    b, s, v, h = 2, 60, 40000, 848
+    x, w, t = inputs(b * s, v, h + 8, torch.bfloat16)
+    x, t = x.view(b, s, h + 8), t.view(b, s)
+    check(cross_entropy(t.int(), "mean"), x[..., :h], w[:, :h], t, "mean")
+    check(cross_entropy(t, "sum"), x[..., 1:h + 1], w[:, 3:h + 3], t, "sum")
+    check(cross_entropy(t[:, ::2], "mean"), x[:, ::2, :h].transpose(0, 1).contiguous().transpose(0, 1), w[:, :h].t().contiguous().t(), t[:, ::2], "mean")
+    x, w = x[..., :h].detach(), w[:, :h].detach()
+    none = run(cross_entropy(torch.full_like(t, -3), "mean"), x, w, torch.ones((), device="cuda"))
+    assert not any(v.any() for v in none.values())
+    bad = t.clone()
+    bad[1, 7] = v
+    out = run(cross_entropy(bad, "mean"), x, w, torch.ones((), device="cuda"))
+    assert out["loss"].isnan() and out["dw"].isnan().all() and out["dx"][1, 7].isnan().all() and out["dx"][0].isfinite().all()
+    spoilt = x.clone()
+    spoilt[0, 3, 5] = float("inf")
+    out = run(cross_entropy(t.clamp(min=0), "mean"), spoilt, w, torch.ones((), device="cuda"))
+    assert not out["loss"].isfinite() and out["dx"][1].isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_strides_and_kinds(dtype):
     b, s, v, h = 3, 50, 300, 96
@@ -206,8 +260,9 @@ def test_rows_that_are_sure(dtype):
 @pytest.mark.parametrize("wide", [False, True])
 def test_logits_too_far_above_the_target_s(wide):
     """bf16, one loss for all rows: sums of exponentials over the target's that pass 2^100, in some pieces of the rows and not in others, and a few words over the edge."""
-    rows, v, h = (200, 300, 64) if not wide else (14000, 30000, 64)  # (in two pieces of the rows)
+    rows, v, h = (200, 530000, 64) if not wide else (14000, 40000, 840)  # (in two pieces of the rows)
     x, w, t = inputs(rows, v, h, torch.bfloat16)
+    assert made_with_the_loss(x, w, t)
     logits, tokens = teacher(rows, 5, v, torch.bfloat16)
     far = x.clone()
     far[rows - 7] = w[5] * 40 * h ** 0.5  # (a logit of word 5 of a few hundred)
@@ -221,9 +276,10 @@ def test_logits_too_far_above_the_target_s(wide):
         check(call, given, w, targets, "mean" if call is calls[0][0] else "sum", kind, tau)
 
 
-def test_gradients_made_with_the_loss():
-    """bf16, one loss for all rows: asked for twice, apart, multiplied with what comes back, of a loss whose inputs changed."""
-    x, w, t = inputs(300, 2000, 72, torch.bfloat16)
+def test_asking_for_gradients_made_with_the_loss():
+    """Twice, apart, multiplied with what comes back, of a loss whose inputs changed."""
+    x, w, t = inputs(300, 40000, 856, torch.bfloat16)
+    assert made_with_the_loss(x, w, t)
     x, w = x.requires_grad_(), w.requires_grad_()
     loss = ops.linear_cross_entropy(x, w, t)
     one = torch.ones((), device="cuda")
@@ -433,7 +489,6 @@ def test_a_wait_that_runs_out_leaves_nan():
 
 
 def test_a_failure_in_a_backward_pass_is_this_library_s_error():
-    from test_gpu_linear8 import replaced
     x, w, t = inputs(6, 30, 64, torch.float32)
     prototype = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
     with replaced("b2_vocabulary_loss_backward", prototype, lambda original, *arguments: 1):
@@ -442,3 +497,7 @@ def test_a_failure_in_a_backward_pass_is_this_library_s_error():
     with replaced("b2_vocabulary_loss_forward", prototype, lambda original, *arguments: 1):
         with pytest.raises(nn.B200CclError):
             ops.linear_cross_entropy(x, w, t)
+    x, w, t = inputs(6, 40000, 856, torch.bfloat16)
+    with replaced("b2_vocabulary_loss_times", prototype, lambda original, *arguments: 1):
+        with pytest.raises(nn.B200CclError):
+            ops.linear_cross_entropy(x.requires_grad_(), w, t).backward()
