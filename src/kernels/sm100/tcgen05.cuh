@@ -58,9 +58,10 @@ template <bool kCluster = false>
 __device__ __forceinline__ bool wait_phase(unsigned bar, unsigned parity, volatile unsigned* failed, unsigned long long limit) {
     if (phase_over<kCluster>(bar, parity)) return true;
     unsigned long long t0 = 0;
+    const unsigned between = limit != 0ull ? 15u : 0u;  // polls without a look at the clock
     for (unsigned polls = 1;; ++polls) {
         if (phase_over<kCluster>(bar, parity)) return true;
-        if ((polls & 15u) != 0u) continue;
+        if ((polls & between) != 0u) continue;
         const unsigned long long now = global_timer_ns();
         if (t0 == 0) t0 = now;
         if (*failed != 0u) return false;

@@ -451,8 +451,8 @@ def called(x, w, t, dloss, wait_ns, kept=None):
 
 
 def test_a_wait_that_runs_out_leaves_nan():
-    """Without any time a wait makes a few polls all the same, and may be over by then (it is for 256 steps at most, 70 us): a call's results are the right ones or NaN, its status says which, and
-    of many calls some run out."""
+    """Without any time a wait makes two polls all the same, of a microsecond or more, and may be over by then (it is for a few microseconds): a call's results are the right ones or NaN, its status
+    says which, and of many calls some run out."""
     x, w, t = inputs(4096, 1024, 32768, torch.bfloat16)
     t, dloss = t.clamp(min=0), torch.ones(4096, device="cuda")
     ops.check_async_error()
