@@ -25,8 +25,8 @@
 // fp32: x, w and P are sums of two fp16 matrices each, what fp16 makes of an element and what it makes of the rest, after a power of two that brings the largest
 // element of x and of w to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
 // it. (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 2055.)
-// The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and their sums are added up in registers, rounded, after every 1024
-// elements of the summed axis: a loss over columns of 4096 is 1.8e-6 off otherwise, all of it in one direction.
+// The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and their sums are added up in registers, rounded, after every 256 to 8192
+// elements of the summed axis: a loss over columns of 4096 in bf16 is 1.8e-6 off otherwise, all of it in one direction.
 //
 // P pairs take P whole tiles of a gradient at a time, as long as there are so many. Those that are left are cut along the summed axis, all into the same number of pieces, which go over the pairs
 // piece by piece and not tile by tile: pairs are at the same words, or tokens, then, and read them from L2 once one of them has. (Steps dealt out evenly, tile by
@@ -71,8 +71,10 @@ constexpr unsigned kAtStaging = kStages * 2 * kOperandBytes, kAtBarriers = kAtSt
 constexpr unsigned kShared = kAtBarriers + 256 + 1024;
 static_assert(kShared <= 227 * 1024);
 constexpr unsigned kTileFloats = kTile * kTile;
-// Steps that are summed on the tensor cores alone, of each product: of logits and fp32, where 3e-6 counts, and of gradients that are rounded to 16 bits.
-constexpr unsigned kChunkSteps = 16, kLongChunkSteps = 128;
+// Steps that are summed on the tensor cores alone, of each product: in fp32 and in small products; of logits; of gradients that are rounded to 16 bits. (fp32, 2048 x 50257 x 768, errors of dx and
+// dw in the norm: 1.32e-6 and 1.23e-6 with sixteen, 4.0e-7 and 3.6e-7 with four.)
+constexpr unsigned kShortChunkSteps = 4, kChunkSteps = 16, kLongChunkSteps = 128;
+constexpr unsigned kEntryRounds = kMaxTeacherEntries / 32;  // of a warp through a row's entries
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kHalfScale = 16384.0f;  // of P in fp16
 
@@ -103,9 +105,13 @@ struct alignas(64) ProductArgs {
     float2* stats; // [2 * tiles along n][m]
     float* exp_sums;  // the same, of Exps
     float* picked; // [m]
-    const void* targets;
+    const void* targets;  // cross entropy: [m]
     long long target_stride;
-    bool targets64, hard;
+    bool targets64;
+    const int* words;     // distillation: [entries][entry_stride] of each row, -1: none
+    const float* probs;   // the teacher's
+    float* entry_logits;  // made by Stats and Exps
+    unsigned entries, entry_stride;
     const float* top;    // [m]: the largest logit, and the sum of e^(z - top): apart, because of a row that is sure of its target the logarithm of all
     const float* sum;    // would round off what it is not sure of
     const float* valid;  // whether the row counts: 1, 0, or NaN
@@ -308,7 +314,8 @@ __device__ __noinline__ void spoil(const ProductArgs& a, const Share& share, uns
 }
 
 // T: type of x, w and their gradients. kLong: runs of several segments, whose sums are added up in registers: that unrolls what is made of them four times, which costs short runs a tenth.
-template <Kind kKind, typename T, bool kLong>
+// kTeacher: rows of logits have several words that count, and not one.
+template <Kind kKind, typename T, bool kLong, bool kTeacher>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
     constexpr bool kLogits = kKind == Kind::Stats || kKind == Kind::Probs || kKind == Kind::Exps;
     constexpr bool kAByRows = kKind == Kind::WeightGrad, kBByRows = !kLogits;
@@ -459,12 +466,25 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             const Tile t = tile_at(a, r.tile);
             const unsigned first = t.n + column0, row = t.m + in_tile + lane;
             const unsigned columns = first < a.n ? min(b_rows, a.n - first) : 0u;  // of this warp
-            // What a row of logits needs beside them.
+            // What a row of logits needs beside them: the columns of this warp's that count in it.
             long long target = -1;
+            unsigned hits[kTeacher ? kEntryRounds : 1] = {};  // kTeacher: entries that are here in some row of the warp
+            const long long first_word = (long long)(first + a.b_offset);
             float weight = 0.0f, row_top = 0.0f, share_of_sum = 1.0f;
             if constexpr (kLogits) {
+                if constexpr (kTeacher) {
+#pragma unroll
+                    for (unsigned b = 0; b < kEntryRounds; ++b) {
+                        if (32u * b >= a.entries) break;
+#pragma unroll 8
+                        for (unsigned e = 0; e < min(32u, a.entries - 32u * b); ++e) {
+                            const int word = row < a.m ? a.words[(u64)(32u * b + e) * a.entry_stride + row] : -1;
+                            hits[b] |= __any_sync(0xffffffffu, word >= 0 && (unsigned long long)(word - first_word) < columns) ? 1u << e : 0u;
+                        }
+                    }
+                }
                 if (row < a.m) {
-                    if (a.hard) target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
+                    if constexpr (!kTeacher) target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
                     if constexpr (kKind == Kind::Probs) {
                         weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (kHalfType ? kHalfScale : 1.0f);
                         row_top = a.top[row];
@@ -474,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         row_top = a.top[row];
                     }
                 }
-                target = target < 0 ? -1 : target - (long long)(first + a.b_offset);
+                target = target < 0 ? -1 : target - first_word;
             }
             const unsigned own_target = target >= 0 && target < (long long)columns ? (unsigned)target : 0xffffffffu;  // its column of this warp's
             // What is made of `kUnit` times 32 columns of sums, from the warp's column c on.
@@ -485,6 +505,20 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                 sums = r.whole ? a.sums + (u64)r.tile * kTileFloats : a.slots + (u64)r.slot * kTileFloats;
                 of_row = kKind == Kind::InputGrad && a.row_scale != nullptr && row < a.m ? scale * a.row_scale[row] : scale;
             }
+            // f(column of the 32 from c on, entry, its place) for every entry that is there in some row; in the others the column is above 31.
+            const auto each_entry = [&](unsigned c, auto&& f) {
+                if constexpr (kTeacher) {
+#pragma unroll
+                    for (unsigned b = 0; b < kEntryRounds; ++b) {
+                        for (unsigned left = hits[b]; left != 0u; left &= left - 1u) {
+                            const u64 place = (u64)(32u * b + (unsigned)__ffs((int)left) - 1u) * a.entry_stride + row;
+                            const long long at = row < a.m ? (long long)a.words[place] - first_word - (long long)c : -1;
+                            const unsigned column = at >= 0 && at < 32 && c + at < columns ? (unsigned)at : 0xffffffffu;
+                            if (__any_sync(0xffffffffu, column < 32u)) f(column, place);
+                        }
+                    }
+                }
+            };
             const auto work_off = [&](unsigned c, float (&f)[kUnit][32]) {
                 if constexpr (kLogits && sizeof(T) == 4) {
 #pragma unroll
@@ -505,12 +539,14 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             for (unsigned j = 0; j < 32; ++j) f[h][j] = c + 32u * h + j < columns ? f[h][j] : low;
                         }
                         const unsigned at = own_target - (c + 32u * h);
-                        if (__any_sync(0xffffffffu, at < 32u)) {
+                        const auto pick = [&](unsigned column, float* to) {
                             float z = 0.0f;
 #pragma unroll
-                            for (unsigned j = 0; j < 32; ++j) z = j == at ? f[h][j] : z;
-                            if (at < 32u) a.picked[row] = z;
-                        }
+                            for (unsigned j = 0; j < 32; ++j) z = j == column ? f[h][j] : z;
+                            if (column < 32u) *to = z;
+                        };
+                        if (!kTeacher && __any_sync(0xffffffffu, at < 32u)) pick(at, a.picked + row);
+                        each_entry(c + 32u * h, [&](unsigned column, u64 place) { pick(column, a.entry_logits + place); });
                         float most[4] = {f[h][0], f[h][1], f[h][2], f[h][3]};
 #pragma unroll
                         for (unsigned j = 4; j < 32; ++j) most[j & 3u] = fmaxf(most[j & 3u], f[h][j]);
@@ -530,13 +566,28 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 #pragma unroll
                     for (unsigned h = 0; h < 2; ++h) {
                         const unsigned at = own_target - (c + 32u * h);
+                        if constexpr (kKind == Kind::Exps) {
+                            each_entry(c + 32u * h, [&](unsigned column, u64 place) {
+                                float z = 0.0f;
+#pragma unroll
+                                for (unsigned j = 0; j < 32; ++j) z = j == column ? f[h][j] : z;
+                                if (column < 32u) a.entry_logits[place] = z;
+                            });
+                        }
 #pragma unroll
                         for (unsigned j = 0; j < 32; j += 2) {
                             const float2 e = exponentials<T>(f[h][j], f[h][j + 1], -row_top, a.factor, a.factor_rest);
                             f[h][j] = kKind == Kind::Probs ? share_of_sum * e.x : e.x;
                             f[h][j + 1] = kKind == Kind::Probs ? share_of_sum * e.y : e.y;
                         }
-                        if (__any_sync(0xffffffffu, at < 32u)) {
+                        if constexpr (kKind == Kind::Probs) {
+                            each_entry(c + 32u * h, [&](unsigned column, u64 place) {
+                                const float off = column < 32u ? weight * a.probs[place] : 0.0f;
+#pragma unroll
+                                for (unsigned j = 0; j < 32; ++j) f[h][j] -= j == column ? off : 0.0f;
+                            });
+                        }
+                        if (!kTeacher && __any_sync(0xffffffffu, at < 32u)) {
                             // (Exps: the target's is 1 by definition; its logit was made by another kernel, whose roundings differ.)
 #pragma unroll
                             for (unsigned j = 0; j < 32; ++j) f[h][j] = j != at ? f[h][j] : (kKind == Kind::Probs ? f[h][j] - weight : 1.0f);
@@ -757,9 +808,9 @@ struct JoinArgs {
     long long target_stride;
     bool targets64;
     unsigned long long vocabulary;
-    const float* z;  // distillation: [rows][entries]
+    const float* z;  // distillation: [entries][entry_stride]
     const float* p;
-    unsigned entries;
+    unsigned entries, entry_stride;
     float temperature, factor;
     float* top;
     float* sum;
@@ -820,8 +871,8 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
     if (at < a.rows) {
         float loss = 0.0f;
         for (unsigned k = lane; k < a.entries; k += 32u) {
-            const float p = a.p[at * a.entries + k];
-            if (p != 0.0f) loss += p * (logf(p) + kLn2 * ((of_row[warp].x - a.z[at * a.entries + k]) * factor + of_row[warp].y));
+            const float p = a.p[(u64)k * a.entry_stride + at];
+            if (p != 0.0f) loss += p * (logf(p) + kLn2 * ((of_row[warp].x - a.z[(u64)k * a.entry_stride + at]) * factor + of_row[warp].y));
         }
 #pragma unroll
         for (unsigned d = 16; d != 0; d /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, d);
@@ -872,7 +923,7 @@ __global__ void __launch_bounds__(1024) sum_kernel(const __grid_constant__ SumAr
 }
 
 struct EntriesArgs {
-    const void* x;  // rows at multiples of 16 bytes, but for fp32
+    const void* x;  // rows at multiples of 16 bytes
     long long x_stride;
     const void* weight;
     long long weight_stride;
@@ -881,14 +932,14 @@ struct EntriesArgs {
     const void* targets;
     long long target_strides[2];
     bool targets64;
-    const void* teacher;  // null: one entry of probability 1
+    const void* teacher;  // null: cross entropy, one entry
     int teacher_dtype;
     long long teacher_strides[2];
     float temperature;
-    float* z;
-    float* p;
+    int* words;    // [entries][rows], or null
+    float* probs;
     float* valid;
-    float* top;  // the largest z, 0 of rows without entries; or null
+    float* top;    // the logit of the entry that the teacher is surest of, 0 of rows without entries; or null
 };
 
 __device__ __forceinline__ float load_as_float(const void* p, int dtype, long long at) {
@@ -896,11 +947,7 @@ __device__ __forceinline__ float load_as_float(const void* p, int dtype, long lo
     return dtype == 1 ? __half2float(static_cast<const __half*>(p)[at]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
 }
 
-constexpr unsigned kEntryRounds = kMaxTeacherEntries / 32;
-
-// The teacher's distribution over its entries (cross entropy: the target), and the student's logits of them. A warp takes a row; reading the words' rows of the matrix
-// bounds it: eight of them at a time, or one where there are no more (its loads are on the way together then).
-template <typename T, unsigned kAtOnce>
+// The teacher's distribution over its entries (cross entropy: the target), and near which logit a row's sum will be. A warp takes a row.
 __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ EntriesArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -931,6 +978,11 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
     bad = __any_sync(0xffffffffu, bad);
 #pragma unroll
     for (unsigned d = 16; d != 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    // The place of the largest, if its word is one; the first of several.
+    unsigned surest = 0xffffffffu;
+#pragma unroll
+    for (unsigned i = kEntryRounds; i-- > 0;) surest = token[i] >= 0 && p[i] == top ? lane + 32u * i : surest;
+    surest = __reduce_min_sync(0xffffffffu, surest);
     float sum = 0.0f;
 #pragma unroll
     for (unsigned i = 0; i < kEntryRounds; ++i) {
@@ -940,68 +992,39 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
 #pragma unroll
     for (unsigned d = 16; d != 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) a.valid[row] = bad ? nan32() : (any ? 1.0f : 0.0f);
-    float most = low;
-    const u64 out = (u64)row * a.entries;
-    const T* x = static_cast<const T*>(a.x) + (long long)row * a.x_stride;
+    if (a.words != nullptr) {
 #pragma unroll
-    for (unsigned i = 0; i < kEntryRounds; ++i) {
-        if (32u * i >= a.entries) break;
-        const unsigned k = lane + 32u * i;
-        if (k < a.entries) a.p[out + k] = any ? p[i] / sum : 0.0f;
-        float z = 0.0f;  // of this lane's entry
-        const unsigned there = min(32u, a.entries - 32u * i);
-        for (unsigned e = 0; e < there; e += kAtOnce) {
-            const T* w[kAtOnce];
-            float dot[kAtOnce] = {};
-#pragma unroll
-            for (unsigned j = 0; j < kAtOnce; ++j) {
-                const long long t = __shfl_sync(0xffffffffu, token[i], e + j);
-                w[j] = t >= 0 ? static_cast<const T*>(a.weight) + t * a.weight_stride : nullptr;
-            }
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll(kAtOnce == 1 ? 8 : 1)
-                for (unsigned h = lane; h < a.width; h += 32u) {
-                    const float v = x[h];
-#pragma unroll
-                    for (unsigned j = 0; j < kAtOnce; ++j) dot[j] += w[j] != nullptr ? v * w[j][h] : 0.0f;
-                }
-            } else {
-#pragma unroll(kAtOnce == 1 ? 4 : 1)
-                for (unsigned h = lane * 8u; h < a.width; h += 256u) {
-                    const unsigned n = min(8u, a.width - h);  // (what lies behind a row may be anything)
-                    const uint4 nothing = make_uint4(0u, 0u, 0u, 0u);
-                    uint4 xs = *reinterpret_cast<const uint4*>(x + h), ws[kAtOnce];
-#pragma unroll
-                    for (unsigned j = 0; j < kAtOnce; ++j) ws[j] = w[j] != nullptr ? *reinterpret_cast<const uint4*>(w[j] + h) : nothing;
-                    float v[8], u[8];
-                    Wide<T>::unpack(xs, v);
-#pragma unroll
-                    for (unsigned j = 0; j < kAtOnce; ++j) {
-                        Wide<T>::unpack(ws[j], u);
-                        if (n == 8u) {
-#pragma unroll
-                            for (unsigned q = 0; q < 8; ++q) dot[j] += v[q] * u[q];
-                        } else {
-#pragma unroll
-                            for (unsigned q = 0; q < 8; ++q) dot[j] += q < n ? v[q] * u[q] : 0.0f;
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (unsigned j = 0; j < kAtOnce; ++j) {
-#pragma unroll
-                for (unsigned d = 16; d != 0; d /= 2) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
-                if (lane == e + j) z = dot[j];
-            }
+        for (unsigned i = 0; i < kEntryRounds; ++i) {
+            const unsigned k = lane + 32u * i;
+            if (k >= a.entries) break;
+            a.words[(u64)k * a.rows + row] = (int)token[i];
+            a.probs[(u64)k * a.rows + row] = any ? p[i] / sum : 0.0f;
         }
-        if (k < a.entries) a.z[out + k] = z;
-        if (token[i] >= 0) most = fmaxf(most, z);
     }
     if (a.top == nullptr) return;
+    long long word = -1;
 #pragma unroll
-    for (unsigned d = 16; d != 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    if (lane == 0) a.top[row] = most == low ? 0.0f : most;
+    for (unsigned i = 0; i < kEntryRounds; ++i) {
+        const long long other = __shfl_sync(0xffffffffu, token[i], surest & 31u);
+        word = surest / 32u == i ? other : word;
+    }
+    using T = __nv_bfloat16;
+    float z = 0.0f;
+    if (word >= 0) {
+        const T *x = static_cast<const T*>(a.x) + (long long)row * a.x_stride, *w = static_cast<const T*>(a.weight) + word * a.weight_stride;
+#pragma unroll 4
+        for (unsigned h = lane * 8u; h < a.width; h += 256u) {
+            const unsigned n = min(8u, a.width - h);  // (what lies behind a row may be anything)
+            float v[8], u[8];
+            Wide<T>::unpack(*reinterpret_cast<const uint4*>(x + h), v);
+            Wide<T>::unpack(*reinterpret_cast<const uint4*>(w + h), u);
+#pragma unroll
+            for (unsigned q = 0; q < 8; ++q) z += q < n ? v[q] * u[q] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (unsigned d = 16; d != 0; d /= 2) z += __shfl_xor_sync(0xffffffffu, z, d);
+    if (lane == 0) a.top[row] = z;
 }
 
 struct HeaderArgs {
@@ -1044,79 +1067,17 @@ __global__ void __launch_bounds__(1024) header_kernel(const __grid_constant__ He
     }
 }
 
-struct FixArgs {
-    void* probs;  // [parts][rows][pitch]
-    unsigned parts, rows, pitch, entries;
-    long long first, columns;  // of the vocabulary
-    const void* targets;
-    long long target_strides[2];
-    bool targets64;
-    const float* z;
-    const float* p;
-    const float* top;
-    const float* sum;
-    const float* valid;
-    const float* loss_grad;
-    long long loss_grad_stride;
-    float temperature, factor;
-    const float* header;
-    const unsigned* condition;
-};
-
-// Distillation: the elements of P that the teacher has entries of. A warp takes a row; entries of the same word write the same.
-template <typename T>
-__global__ void __launch_bounds__(256) fix_kernel(const __grid_constant__ FixArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned lane = threadIdx.x & 31u, row = blockIdx.x * 8u + threadIdx.x / 32u;
-    if (row >= a.rows || (a.condition != nullptr && *a.condition == 0u)) return;
-    const float weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (std::is_same_v<T, __nv_bfloat16> ? 1.0f : kHalfScale);
-    const float top = a.top[row], share_of_sum = weight / a.sum[row];
-    long long token[kEntryRounds];
-    float p[kEntryRounds];
-#pragma unroll
-    for (unsigned i = 0; i < kEntryRounds; ++i) {
-        const unsigned k = lane + 32u * i;
-        token[i] = k < a.entries ? target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)k * a.target_strides[1]) : -1;
-        p[i] = k < a.entries ? a.p[(u64)row * a.entries + k] : 0.0f;
-        if (p[i] == 0.0f) token[i] = -1;
-    }
-#pragma unroll
-    for (unsigned i = 0; i < kEntryRounds; ++i) {
-        if (32u * i >= a.entries) break;
-        const long long column = token[i] - a.first;
-        const bool here = token[i] >= 0 && column >= 0 && column < a.columns;
-        if (!__any_sync(0xffffffffu, here)) continue;
-        float all = 0.0f;
-#pragma unroll
-        for (unsigned j = 0; j < kEntryRounds; ++j) {
-            if (32u * j >= a.entries) break;
-            for (unsigned e = 0; e < min(32u, a.entries - 32u * j); ++e) {
-                const long long other = __shfl_sync(0xffffffffu, token[j], e);
-                const float q = __shfl_sync(0xffffffffu, p[j], e);
-                all += other == token[i] ? q : 0.0f;
-            }
-        }
-        if (!here) continue;
-        float v = weight == 0.0f ? 0.0f : share_of_sum * exp2_fast((a.z[(u64)row * a.entries + lane + 32u * i] - top) * a.factor) - weight * all;
-        const u64 at = (u64)row * a.pitch + (u64)column;
-        for (unsigned part = 0; part < a.parts; ++part) {
-            const OperandOf<T> rounded = Elem<OperandOf<T>>::from_f(v);
-            static_cast<OperandOf<T>*>(a.probs)[(u64)part * a.rows * a.pitch + at] = rounded;
-            v -= Elem<OperandOf<T>>::to_f(rounded);
-        }
-    }
-}
-
 // Both at once: the rows' sums, their losses, what their gradients are divided by, and E of the targets.
 struct CloseArgs {
     const float* exp_sums;  // [parts][rows]
-    unsigned rows, parts, entries;
+    unsigned rows, parts;
+    unsigned entries, entry_stride;  // 0: cross entropy
     long long vocabulary;
     const void* targets;
-    long long target_strides[2];
+    long long target_stride;
     bool targets64;
-    const float* z;  // [rows][entries]
+    const int* words;  // [entries][entry_stride]
+    const float* z;
     const float* p;
     const float* valid;
     const float* top;
@@ -1132,11 +1093,20 @@ struct CloseArgs {
 constexpr float kLargestSum = 1.2676506e30f;  // 2^100
 
 // A CTA takes 32 rows: each of its warps every 32nd part of them, then one row.
+//
+// Most of a row's gradient is that of its entries, and E of each is rounded on its own; but the row has a factor, in 32 bits, that may be a little off what it should be for all other
+// words. Cross entropy: it is what makes the target's exact. Distillation: of 33 factors within 2^-9 the one that rounds the entries best. (8192 x 50257 x 768, errors in the
+// norm of dx and dw: 2.35e-3 and 2.56e-3 otherwise, 1.67e-3 and 2.15e-3 so; with a teacher of 32 entries TODO.)
 __global__ void __launch_bounds__(1024) close_kernel(const __grid_constant__ CloseArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr unsigned kWarps = 32;
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x / 32u, first = blockIdx.x * 32u;
+    const auto all_lanes = [](float v) {
+#pragma unroll
+        for (unsigned d = 16; d != 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+        return v;
+    };
     float sum = 0.0f;
     if (first + lane < a.rows) {
         for (unsigned p = warp; p < a.parts; p += 4u * kWarps) {
@@ -1151,47 +1121,67 @@ __global__ void __launch_bounds__(1024) close_kernel(const __grid_constant__ Clo
     __syncthreads();
     const unsigned row = first + warp;
     if (row >= a.rows) return;
-    sum = all[lane][warp];
-#pragma unroll
-    for (unsigned d = 16; d != 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const float valid = a.valid[row], top = a.top[row], log_sum = log2f(sum);
-    float loss = 0.0f, largest = 0.0f, exactly = 1.0f;
-    for (unsigned k = lane; k - lane < a.entries; k += 32u) {
-        const u64 at = (u64)row * a.entries + k;
-        const long long token = k < a.entries ? target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)k * a.target_strides[1]) : -1;
-        const float p = k < a.entries ? a.p[at] : 0.0f, over = k < a.entries ? (a.z[at] - top) * a.factor : 0.0f;
-        if (p != 0.0f) loss += p * (logf(p) + kLn2 * (log_sum - over));
-        // Entries of the same word add up, and write the same.
-        float together = 0.0f;
-        for (unsigned e = 0; e < a.entries; ++e) {
-            const long long other = target_at(a.targets, a.targets64, (long long)row * a.target_strides[0] + (long long)e * a.target_strides[1]);
-            together += other == token ? a.p[(u64)row * a.entries + e] : 0.0f;
-        }
-        if (p != 0.0f && token >= 0 && token < a.vocabulary) {
-            const float v = exp2_fast(over) - together * sum;
+    sum = all_lanes(all[lane][warp]);
+    const float valid = a.valid[row], log_sum = log2f(sum);
+    float loss = 0.0f, factor = 1.0f;
+    if (a.entries == 0) {
+        const long long target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
+        if (lane == 0 && target >= 0 && target < a.vocabulary) {
+            const float v = 1.0f - sum;
             const __nv_bfloat16 rounded = __float2bfloat16_rn(v);
-            a.exps[(u64)row * a.pitch + (u64)token] = rounded;
-            if (fabsf(v) > largest) {
-                largest = fabsf(v);
-                exactly = v / __bfloat162float(rounded);
+            a.exps[(u64)row * a.pitch + (u64)target] = rounded;
+            if (v != 0.0f) factor = v / __bfloat162float(rounded);
+        }
+        loss = kLn2 * log_sum;
+    } else {
+        const float top = a.top[row];
+        float value[kEntryRounds];
+        int word[kEntryRounds];
+#pragma unroll
+        for (unsigned i = 0; i < kEntryRounds; ++i) {
+            const unsigned k = lane + 32u * i;
+            value[i] = 0.0f;
+            word[i] = -1;
+            if (32u * i >= a.entries) break;
+            const u64 at = (u64)k * a.entry_stride + row;
+            const float p = k < a.entries ? a.p[at] : 0.0f;
+            word[i] = p != 0.0f ? a.words[at] : -1;
+            const float over = word[i] >= 0 ? (a.z[at] - top) * a.factor : 0.0f;
+            if (p != 0.0f) loss += p * (logf(p) + kLn2 * (log_sum - over));
+            // Entries of the same word add up, and write the same.
+            float together = 0.0f;
+            for (unsigned e = 0; e < a.entries; ++e) {
+                const u64 other = (u64)e * a.entry_stride + row;
+                together += a.words[other] == word[i] ? a.p[other] : 0.0f;
+            }
+            if (word[i] >= 0) value[i] = exp2_fast(over) - together * sum;
+        }
+        loss = all_lanes(loss);
+        float least = __int_as_float(0x7f800000);
+        for (int n = -16; n <= 16; ++n) {
+            const float by = 1.0f + (float)n * (1.0f / 8192.0f), back = 1.0f / by;
+            float off = 0.0f;
+#pragma unroll
+            for (unsigned i = 0; i < kEntryRounds; ++i) {
+                if (32u * i >= a.entries) break;
+                const float d = value[i] - by * __bfloat162float(__float2bfloat16_rn(value[i] * back));
+                off += d * d;
+            }
+            off = all_lanes(off);
+            if (off < least) {
+                least = off;
+                factor = by;
             }
         }
-    }
-    // Most of a row's gradient is its target's: what rounding that takes is given back by the factor of the row. (Errors of 8192 x 50257 x 768 in the norm, of dx 2.35e-3 otherwise, TODO so.)
+        const float back = 1.0f / factor;
 #pragma unroll
-    for (unsigned d = 16; d != 0; d /= 2) {
-        const float other = __shfl_xor_sync(0xffffffffu, largest, d), others = __shfl_xor_sync(0xffffffffu, exactly, d);
-        if (other > largest || (other == largest && others > exactly)) {
-            largest = other;
-            exactly = others;
-        }
+        for (unsigned i = 0; i < kEntryRounds; ++i)
+            if (32u * i < a.entries && word[i] >= 0) a.exps[(u64)row * a.pitch + (u64)word[i]] = __float2bfloat16_rn(value[i] * back);
     }
-#pragma unroll
-    for (unsigned d = 16; d != 0; d /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, d);
     if (lane != 0) return;
     a.sum[row] = sum;
     a.loss[row] = valid == 0.0f ? 0.0f : loss * a.temperature * a.temperature * valid;
-    a.row_scale[row] = valid == 0.0f ? 0.0f : valid / sum * exactly;
+    a.row_scale[row] = valid == 0.0f ? 0.0f : valid / sum * factor;
     if (valid != 0.0f && !(sum <= kLargestSum)) *a.condition = 1u;
 }
 
@@ -1377,22 +1367,27 @@ int current_device() {
     return device;
 }
 
-template <Kind kKind, bool kLong>
+template <Kind kKind, bool kLong, bool kTeacher>
 const void* kernel_of(DType dtype) {
-    if constexpr (kKind == Kind::Exps) return (const void*)product_kernel<kKind, __nv_bfloat16, kLong>;
+    if constexpr (kKind == Kind::Exps) return (const void*)product_kernel<kKind, __nv_bfloat16, kLong, kTeacher>;
     else switch (dtype) {
-        case DType::Float: return (const void*)product_kernel<kKind, float, kLong>;
-        case DType::Float16: return (const void*)product_kernel<kKind, __half, kLong>;
-        default: return (const void*)product_kernel<kKind, __nv_bfloat16, kLong>;
+        case DType::Float: return (const void*)product_kernel<kKind, float, kLong, kTeacher>;
+        case DType::Float16: return (const void*)product_kernel<kKind, __half, kLong, kTeacher>;
+        default: return (const void*)product_kernel<kKind, __nv_bfloat16, kLong, kTeacher>;
     }
 }
-const void* kernel_of(Kind kind, DType dtype, bool longer) {
+template <Kind kKind>
+const void* logits_kernel_of(DType dtype, bool longer, bool teacher) {
+    return longer ? (teacher ? kernel_of<kKind, true, true>(dtype) : kernel_of<kKind, true, false>(dtype))
+                  : (teacher ? kernel_of<kKind, false, true>(dtype) : kernel_of<kKind, false, false>(dtype));
+}
+const void* kernel_of(Kind kind, DType dtype, bool longer, bool teacher) {
     switch (kind) {
-        case Kind::Stats: return longer ? kernel_of<Kind::Stats, true>(dtype) : kernel_of<Kind::Stats, false>(dtype);
-        case Kind::Probs: return longer ? kernel_of<Kind::Probs, true>(dtype) : kernel_of<Kind::Probs, false>(dtype);
-        case Kind::Exps: return longer ? kernel_of<Kind::Exps, true>(dtype) : kernel_of<Kind::Exps, false>(dtype);
-        case Kind::WeightGrad: return longer ? kernel_of<Kind::WeightGrad, true>(dtype) : kernel_of<Kind::WeightGrad, false>(dtype);
-        default: return longer ? kernel_of<Kind::InputGrad, true>(dtype) : kernel_of<Kind::InputGrad, false>(dtype);
+        case Kind::Stats: return logits_kernel_of<Kind::Stats>(dtype, longer, teacher);
+        case Kind::Probs: return logits_kernel_of<Kind::Probs>(dtype, longer, teacher);
+        case Kind::Exps: return logits_kernel_of<Kind::Exps>(dtype, longer, teacher);
+        case Kind::WeightGrad: return longer ? kernel_of<Kind::WeightGrad, true, false>(dtype) : kernel_of<Kind::WeightGrad, false, false>(dtype);
+        default: return longer ? kernel_of<Kind::InputGrad, true, false>(dtype) : kernel_of<Kind::InputGrad, false, false>(dtype);
     }
 }
 
@@ -1404,7 +1399,7 @@ unsigned pairs_of_device(int device) {
     if (device >= 0 && device < 64 && known[device] != 0) return known[device];
     for (Kind kind : {Kind::Stats, Kind::Probs, Kind::Exps, Kind::WeightGrad, Kind::InputGrad})
         for (DType dtype : {DType::Float, DType::Float16, DType::BFloat16})
-            for (bool longer : {false, true}) B2_CUDA(cudaFuncSetAttribute(kernel_of(kind, dtype, longer), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared));
+            for (int n = 0; n < 4; ++n) B2_CUDA(cudaFuncSetAttribute(kernel_of(kind, dtype, n / 2 != 0, n % 2 != 0), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(2 * kMaxPairs);
     config.blockDim = dim3(kThreads);
@@ -1416,7 +1411,7 @@ unsigned pairs_of_device(int device) {
     config.attrs = attr;
     config.numAttrs = 1;
     int clusters = 0;
-    B2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel_of(Kind::Stats, DType::BFloat16, true), &config));
+    B2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel_of(Kind::Stats, DType::BFloat16, true, true), &config));
     const unsigned pairs = std::min(kMaxPairs, (unsigned)std::max(1, clusters));
     if (device >= 0 && device < 64) known[device] = pairs;
     return pairs;
@@ -1476,7 +1471,7 @@ struct Plan {
     u64 rows = 0;                // both at once: of a piece
     std::size_t exps_pitch = 0;
     unsigned n_tile = kTile;
-    std::size_t entries_at = 0, scale_at = 0, divided_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
+    std::size_t scale_at = 0, divided_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
 };
 
 // Both at once: bytes of E in a piece of the rows, and of the sums of dw where there are several. (8192 x 50257 x 768, loss and gradients: 1459 us in one piece of 824 MB, 1565 in two,
@@ -1520,7 +1515,7 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     const auto look = [&](u64 m, u64 n, u64 k) { slots = std::max(slots, tiling_of(m, n, k, p.grad_products, p.n_tile, true, p.device_pairs).slots); };
     if (pass == Pass::Loss) {
         p.stats_at = take((v + kTile - 1) / kTile * 2 * t * sizeof(float2));
-        p.picked_at = take(t * sizeof(float));
+        p.picked_at = take(t * std::max(c.entries, 1) * sizeof(float));
         p.losses_at = take(t * sizeof(float));
         p.partial_at = take(c.dtype == DType::Float ? 2 * kMagnitudeCtas * sizeof(unsigned) : 0);
     } else if (pass == Pass::Both) {
@@ -1532,10 +1527,9 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         p.rows = std::min<u64>(t, ((t + p.pieces - 1) / p.pieces + kTile - 1) / kTile * kTile);
         p.pieces = (t + p.rows - 1) / p.rows;
         p.stats_at = take(p.exps_pitch / kTile * 2 * p.rows * sizeof(float2));
-        p.picked_at = take(p.rows * sizeof(float));
+        p.picked_at = take(t * std::max(c.entries, 1) * sizeof(float));
         p.losses_at = take(t * sizeof(float));
         p.header_at = take((2 + p.pieces) * sizeof(float));
-        p.entries_at = take(c.distillation ? 0 : 2 * t * sizeof(float));
         p.scale_at = take(p.rows * sizeof(float));
         p.probs_at = take(p.rows * p.exps_pitch * 2);
         if (c.weight_grad != nullptr) {
@@ -1605,7 +1599,7 @@ void launch_product(Kind kind, const VocabularyLossCall& c, const Tiling& t, Pro
     a.left = t.left;
     a.splits = t.splits;
     a.n_first = kind == Kind::WeightGrad || kind == Kind::InputGrad;
-    a.chunk = a.n_first && c.dtype != DType::Float ? kLongChunkSteps : kChunkSteps;
+    a.chunk = c.dtype == DType::Float || (!a.n_first && small(c)) ? kShortChunkSteps : (a.n_first ? kLongChunkSteps : kChunkSteps);
     a.status = wait_status_word(WaitsOf::VocabularyLoss, current_device());
     a.wait_ns = c.wait_ns;
     cudaLaunchConfig_t config = {};
@@ -1622,7 +1616,7 @@ void launch_product(Kind kind, const VocabularyLossCall& c, const Tiling& t, Pro
     config.attrs = attr;
     config.numAttrs = 2;
     void* arguments[1] = {&a};
-    B2_CUDA(cudaLaunchKernelExC(&config, kernel_of(kind, c.dtype, t.steps_of_tile > t.products * a.chunk), arguments));
+    B2_CUDA(cudaLaunchKernelExC(&config, kernel_of(kind, c.dtype, t.steps_of_tile > t.products * a.chunk, c.distillation), arguments));
 }
 
 // The pieces of a gradient's cut tiles.
@@ -1651,8 +1645,9 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
 }
 
 struct Kept {
-    float *top, *sum, *valid, *count, *z, *p;
+    float *top, *sum, *valid, *count, *probs;
     unsigned* magnitudes;
+    int* words;  // of the teacher's entries, and their probabilities: [entries][tokens]
 };
 Kept kept_of(const VocabularyLossCall& c) {
     Kept k;
@@ -1661,8 +1656,8 @@ Kept kept_of(const VocabularyLossCall& c) {
     k.valid = k.sum + c.tokens;
     k.count = k.valid + c.tokens;
     k.magnitudes = reinterpret_cast<unsigned*>(k.count + 1);
-    k.z = k.count + 3;
-    k.p = k.z + c.tokens * (std::size_t)c.entries;
+    k.probs = k.count + 3;
+    k.words = reinterpret_cast<int*>(k.probs + c.tokens * (std::size_t)c.entries);
     return k;
 }
 
@@ -1713,21 +1708,24 @@ void logits_arguments(const VocabularyLossCall& c, ProductArgs& a) {
     const double factor = 1.4426950408889634 / (double)c.temperature;
     a.factor = (float)factor;
     a.factor_rest = (float)(factor - (double)a.factor);
-    a.hard = !c.distillation;
+    a.entries = (unsigned)c.entries;
+    a.entry_stride = (unsigned)c.tokens;
+    a.words = kept_of(c).words;
+    a.probs = kept_of(c).probs;
     a.targets = c.targets;
     a.target_stride = c.target_strides[0];
     a.targets64 = c.targets64;
     a.temperature = c.temperature;
 }
 
-template <typename T>
-void launch_entries(const VocabularyLossCall& c, const Plan& p, const Operand& x, const Operand& w, float* z, float* prob, float* top) {
+// x and w: where top is wanted, in bf16.
+void launch_entries(const VocabularyLossCall& c, const Operand& x, const Operand& w, float* top) {
+    const Kept kept = kept_of(c);
     EntriesArgs e;
-    const bool copied = sizeof(T) == 2;  // (fp32 reads the original)
-    e.x = copied ? x.data : c.x;
-    e.x_stride = copied && p.copy_x ? (long long)p.pitch : c.x_stride;
-    e.weight = copied ? w.data : c.weight;
-    e.weight_stride = copied && p.copy_weight ? (long long)p.pitch : c.weight_stride;
+    e.x = x.data;
+    e.x_stride = (long long)(x.row_bytes / 2);
+    e.weight = w.data;
+    e.weight_stride = (long long)(w.row_bytes / 2);
     e.rows = (unsigned)c.tokens;
     e.width = (unsigned)c.width;
     e.entries = c.distillation ? (unsigned)c.entries : 1u;
@@ -1741,11 +1739,11 @@ void launch_entries(const VocabularyLossCall& c, const Plan& p, const Operand& x
         e.teacher_strides[i] = c.teacher_strides[i];
     }
     e.temperature = c.temperature;
-    e.z = z;
-    e.p = prob;
-    e.valid = kept_of(c).valid;
+    e.words = c.distillation ? kept.words : nullptr;
+    e.probs = kept.probs;
+    e.valid = kept.valid;
     e.top = top;
-    B2_CUDA(launch_dependent<EntriesArgs>(e.entries == 1 ? entries_kernel<T, 1> : entries_kernel<T, 8>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
+    B2_CUDA(launch_dependent<EntriesArgs>(entries_kernel, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
 }
 
 template <typename T>
@@ -1754,13 +1752,13 @@ void loss(const VocabularyLossCall& c, const Plan& p) {
     const Kept kept = kept_of(c);
     Operand x, w;
     operands<T>(c, p, false, &x, &w);
-    if (c.distillation) launch_entries<T>(c, p, x, w, kept.z, kept.p, nullptr);
+    if (c.distillation) launch_entries(c, x, w, nullptr);
     ProductArgs a = {};
     a.a = map_of(operand_type<T>(), x, p.parts, kStep, kHalf);
     a.b = map_of(operand_type<T>(), w, p.parts, kStep, kHalf);
     logits_arguments(c, a);
     a.stats = reinterpret_cast<float2*>(workspace + p.stats_at);
-    a.picked = reinterpret_cast<float*>(workspace + p.picked_at);
+    a.picked = a.entry_logits = reinterpret_cast<float*>(workspace + p.picked_at);
     const Tiling t = tiling_of(c.tokens, c.vocabulary, c.width, p.products, kTile, false, p.device_pairs);
     launch_product(Kind::Stats, c, t, a, c.tokens, c.vocabulary);
     JoinArgs j;
@@ -1772,9 +1770,10 @@ void loss(const VocabularyLossCall& c, const Plan& p) {
     j.target_stride = c.target_strides[0];
     j.targets64 = c.targets64;
     j.vocabulary = c.vocabulary;
-    j.z = kept.z;
-    j.p = kept.p;
+    j.z = a.entry_logits;
+    j.p = kept.probs;
     j.entries = (unsigned)c.entries;
+    j.entry_stride = a.entry_stride;
     j.temperature = c.temperature;
     j.factor = a.factor;
     j.top = kept.top;
@@ -1831,32 +1830,6 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
         a.header = header;
         a.slots = reinterpret_cast<float*>(workspace + p.slots_at);
         launch_product(Kind::Probs, c, tiling_of(c.tokens, words, c.width, p.products, kTile, false, p.device_pairs), a, c.tokens, words);
-        if (c.distillation) {
-            FixArgs f;
-            f.probs = probs;
-            f.parts = p.prob_parts;
-            f.rows = (unsigned)c.tokens;
-            f.pitch = (unsigned)p.piece;
-            f.entries = (unsigned)c.entries;
-            f.first = (long long)first;
-            f.columns = (long long)words;
-            f.targets = c.targets;
-            f.target_strides[0] = c.target_strides[0];
-            f.target_strides[1] = c.target_strides[1];
-            f.targets64 = c.targets64;
-            f.z = kept.z;
-            f.p = kept.p;
-            f.top = kept.top;
-            f.sum = kept.sum;
-            f.factor = a.factor;
-            f.valid = kept.valid;
-            f.loss_grad = a.loss_grad;
-            f.loss_grad_stride = a.loss_grad_stride;
-            f.temperature = c.temperature;
-            f.header = header;
-            f.condition = nullptr;
-            B2_CUDA(launch_dependent<FixArgs>(fix_kernel<T>, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, f));
-        }
         const unsigned columns = 128 / sizeof(T);
         const auto gradient_of = [&](void* out, u64 rows) {
             a.gradient = out;
@@ -1899,12 +1872,9 @@ void both(const VocabularyLossCall& c, const Plan& p) {
     unsigned* conditions = reinterpret_cast<unsigned*>(header + 2);
     float* losses = reinterpret_cast<float*>(workspace + p.losses_at);
     float* row_scale = reinterpret_cast<float*>(workspace + p.scale_at);
-    const unsigned entries = c.distillation ? (unsigned)c.entries : 1u;
-    float* z = c.distillation ? kept.z : reinterpret_cast<float*>(workspace + p.entries_at);
-    float* prob = c.distillation ? kept.p : z + c.tokens;
     Operand all_x, w;
     operands<T>(c, p, false, &all_x, &w);
-    launch_entries<T>(c, p, all_x, w, z, prob, kept.top);
+    launch_entries(c, all_x, w, kept.top);
     CountArgs n;
     n.valid = kept.valid;
     n.rows = (unsigned)c.tokens;
@@ -1931,7 +1901,9 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         a.targets = targets;
         a.exp_sums = reinterpret_cast<float*>(workspace + p.stats_at);
         a.stats = reinterpret_cast<float2*>(workspace + p.stats_at);
-        a.picked = reinterpret_cast<float*>(workspace + p.picked_at);
+        a.picked = a.entry_logits = reinterpret_cast<float*>(workspace + p.picked_at);
+        a.words = kept.words + first;
+        a.probs = kept.probs + first;
         a.top = kept.top + first;
         a.sum = kept.sum + first;
         a.valid = kept.valid + first;
@@ -1943,14 +1915,15 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         s.exp_sums = a.exp_sums;
         s.rows = (unsigned)rows;
         s.parts = 2 * logits.n_tiles;
-        s.entries = entries;
+        s.entries = (unsigned)c.entries;
+        s.entry_stride = a.entry_stride;
         s.vocabulary = (long long)c.vocabulary;
         s.targets = targets;
-        s.target_strides[0] = c.target_strides[0];
-        s.target_strides[1] = c.target_strides[1];
+        s.target_stride = c.target_strides[0];
         s.targets64 = c.targets64;
-        s.z = z + first * entries;
-        s.p = prob + first * entries;
+        s.words = a.words;
+        s.z = a.entry_logits;
+        s.p = a.probs;
         s.valid = a.valid;
         s.top = a.top;
         s.temperature = c.temperature;
@@ -1978,6 +1951,7 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         j.z = s.z;
         j.p = s.p;
         j.entries = (unsigned)c.entries;
+        j.entry_stride = a.entry_stride;
         j.temperature = c.temperature;
         j.factor = a.factor;
         j.top = kept.top + first;
@@ -1988,32 +1962,6 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         j.row_scale = row_scale;
         B2_CUDA(launch_dependent<JoinArgs>(join_kernel, by_32, 1024, 0, c.stream, j));
         launch_product(Kind::Probs, c, logits, a, rows, c.vocabulary);
-        if (c.distillation) {
-            FixArgs f;
-            f.probs = workspace + p.probs_at;
-            f.parts = 1;
-            f.rows = (unsigned)rows;
-            f.pitch = (unsigned)p.exps_pitch;
-            f.entries = entries;
-            f.first = 0;
-            f.columns = (long long)c.vocabulary;
-            f.targets = targets;
-            f.target_strides[0] = c.target_strides[0];
-            f.target_strides[1] = c.target_strides[1];
-            f.targets64 = c.targets64;
-            f.z = s.z;
-            f.p = s.p;
-            f.top = a.top;
-            f.sum = a.sum;
-            f.valid = a.valid;
-            f.loss_grad = nullptr;
-            f.loss_grad_stride = 0;
-            f.temperature = c.temperature;
-            f.factor = a.factor;
-            f.header = header;
-            f.condition = condition;
-            B2_CUDA(launch_dependent<FixArgs>(fix_kernel<T>, dim3((unsigned)((rows + 7) / 8)), 256, 0, c.stream, f));
-        }
         a.condition = nullptr;
         const auto gradient_of = [&](void* out, u64 of_rows) {
             a.gradient = out;
