@@ -112,6 +112,8 @@ struct alignas(64) ProductArgs {
     const float* probs;   // the teacher's
     float* entry_logits;  // made by Stats and Exps
     unsigned entries, entry_stride;
+    const unsigned* hits;  // [words / 128][hit_rows][rounds]: entries whose word is of 128, in some of 32 rows
+    unsigned hit_rows;
     const float* top;    // [m]: the largest logit, and the sum of e^(z - top): apart, because of a row that is sure of its target the logarithm of all
     const float* sum;    // would round off what it is not sure of
     const float* valid;  // whether the row counts: 1, 0, or NaN
@@ -222,6 +224,15 @@ __device__ __forceinline__ float2 exponentials(float z0, float z1, float off, fl
         e.y = fabsf(p.y) < 200.0f ? e.y + e.y * (kLn2 * (rest.y + o.y * factor_rest)) : e.y;
     }
     return e;
+}
+
+// Element i of a few in registers.
+template <unsigned kN>
+__device__ __forceinline__ unsigned pick_of(const unsigned (&v)[kN], unsigned i) {
+    unsigned r = 0;
+#pragma unroll
+    for (unsigned n = 0; n < kN; ++n) r = n == i ? v[n] : r;
+    return r;
 }
 
 // Target `row` of a matrix; -1 where it is negative.
@@ -468,19 +479,31 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             const unsigned columns = first < a.n ? min(b_rows, a.n - first) : 0u;  // of this warp
             // What a row of logits needs beside them: the columns of this warp's that count in it.
             long long target = -1;
-            unsigned hits[kTeacher ? kEntryRounds : 1] = {};  // kTeacher: entries that are here in some row of the warp
+            constexpr unsigned kNear = kTeacher ? 6 : 1;
+            unsigned hits[kTeacher ? kEntryRounds : 1] = {};  // kTeacher: entries that are here in some row of the warp,
+            unsigned near_column[kNear] = {};                 // and the columns of the first few in this row
             const long long first_word = (long long)(first + a.b_offset);
             float weight = 0.0f, row_top = 0.0f, share_of_sum = 1.0f;
             if constexpr (kLogits) {
                 if constexpr (kTeacher) {
+                    const unsigned rounds = (a.entries + 31u) / 32u;
+                    const unsigned* here = a.hits + ((u64)((unsigned)first_word / kHalf) * a.hit_rows + (t.m + in_tile) / 32u) * rounds;
+                    const bool any = columns != 0u && t.m + in_tile < a.m;
 #pragma unroll
-                    for (unsigned b = 0; b < kEntryRounds; ++b) {
-                        if (32u * b >= a.entries) break;
-#pragma unroll 8
-                        for (unsigned e = 0; e < min(32u, a.entries - 32u * b); ++e) {
-                            const int word = row < a.m ? a.words[(u64)(32u * b + e) * a.entry_stride + row] : -1;
-                            hits[b] |= __any_sync(0xffffffffu, word >= 0 && (unsigned long long)(word - first_word) < columns) ? 1u << e : 0u;
-                        }
+                    for (unsigned b = 0; b < kEntryRounds; ++b) hits[b] = any && b < rounds ? here[b] : 0u;
+                    // The words of the first few are read all at once, while the products are made.
+                    unsigned round = 0, rest = hits[0];
+#pragma unroll
+                    for (unsigned i = 0; i < kNear; ++i) {
+                        while (rest == 0u && round + 1u < rounds) rest = pick_of(hits, ++round);
+                        const unsigned entry = rest != 0u ? 32u * round + (unsigned)__ffs((int)rest) - 1u : 0u;
+                        near_column[i] = (unsigned)a.words[(u64)entry * a.entry_stride + min(row, a.m - 1u)];
+                        rest &= rest - 1u;
+                    }
+#pragma unroll
+                    for (unsigned i = 0; i < kNear; ++i) {
+                        const long long column = (long long)(int)near_column[i] - first_word;
+                        near_column[i] = row < a.m && column >= 0 && column < (long long)columns ? (unsigned)column : 0xffffffffu;
                     }
                 }
                 if (row < a.m) {
@@ -508,12 +531,21 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             // f(column of the 32 from c on, entry, its place) for every entry that is there in some row; in the others the column is above 31.
             const auto each_entry = [&](unsigned c, auto&& f) {
                 if constexpr (kTeacher) {
-#pragma unroll
-                    for (unsigned b = 0; b < kEntryRounds; ++b) {
-                        for (unsigned left = hits[b]; left != 0u; left &= left - 1u) {
-                            const u64 place = (u64)(32u * b + (unsigned)__ffs((int)left) - 1u) * a.entry_stride + row;
-                            const long long at = row < a.m ? (long long)a.words[place] - first_word - (long long)c : -1;
-                            const unsigned column = at >= 0 && at < 32 && c + at < columns ? (unsigned)at : 0xffffffffu;
+                    // (One body for all of them: unrolled, the code is more than the instruction cache holds beside the products' own.)
+                    unsigned n = 0;
+#pragma unroll 1
+                    for (unsigned round = 0; 32u * round < a.entries; ++round) {
+#pragma unroll 1
+                        for (unsigned left = pick_of(hits, round); left != 0u; left &= left - 1u, ++n) {
+                            const u64 place = (u64)(32u * round + (unsigned)__ffs((int)left) - 1u) * a.entry_stride + row;
+                            unsigned column = 0xffffffffu;
+                            if (n < kNear) {
+                                column = pick_of(near_column, n);
+                            } else if (row < a.m) {
+                                const long long at = (long long)a.words[place] - first_word;
+                                column = at >= 0 && at < (long long)columns ? (unsigned)at : 0xffffffffu;
+                            }
+                            column -= c;
                             if (__any_sync(0xffffffffu, column < 32u)) f(column, place);
                         }
                     }
@@ -938,6 +970,8 @@ struct EntriesArgs {
     float temperature;
     int* words;    // [entries][rows], or null
     float* probs;
+    unsigned* hits;  // see ProductArgs; all zeros
+    unsigned hit_rows;
     float* valid;
     float* top;    // the logit of the entry that the teacher is surest of, 0 of rows without entries; or null
 };
@@ -998,6 +1032,7 @@ __global__ void __launch_bounds__(256) entries_kernel(const __grid_constant__ En
             const unsigned k = lane + 32u * i;
             if (k >= a.entries) break;
             a.words[(u64)k * a.rows + row] = (int)token[i];
+            if (token[i] >= 0) atomicOr(a.hits + ((u64)((unsigned)token[i] / kHalf) * a.hit_rows + row / 32u) * ((a.entries + 31u) / 32u) + i, 1u << lane);  // (in any order)
             a.probs[(u64)k * a.rows + row] = any ? p[i] / sum : 0.0f;
         }
     }
@@ -1095,8 +1130,8 @@ constexpr float kLargestSum = 1.2676506e30f;  // 2^100
 // A CTA takes 32 rows: each of its warps every 32nd part of them, then one row.
 //
 // Most of a row's gradient is that of its entries, and E of each is rounded on its own; but the row has a factor, in 32 bits, that may be a little off what it should be for all other
-// words. Cross entropy: it is what makes the target's exact. Distillation: of 33 factors within 2^-9 the one that rounds the entries best. (8192 x 50257 x 768, errors in the
-// norm of dx and dw: 2.35e-3 and 2.56e-3 otherwise, 1.67e-3 and 2.15e-3 so; with a teacher of 32 entries TODO.)
+// words. Cross entropy: it is what makes the target's exact. Distillation: of 32 factors within 2^-9 the one that rounds the entries best. (8192 x 50257 x 768, errors in the
+// norm of dx and dw: 2.35e-3 and 2.56e-3 otherwise, 1.67e-3 and 2.15e-3 so; with a teacher of 32 entries 1.89e-3 and 2.37e-3.)
 __global__ void __launch_bounds__(1024) close_kernel(const __grid_constant__ CloseArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1149,30 +1184,40 @@ __global__ void __launch_bounds__(1024) close_kernel(const __grid_constant__ Clo
             const float over = word[i] >= 0 ? (a.z[at] - top) * a.factor : 0.0f;
             if (p != 0.0f) loss += p * (logf(p) + kLn2 * (log_sum - over));
             // Entries of the same word add up, and write the same.
-            float together = 0.0f;
-            for (unsigned e = 0; e < a.entries; ++e) {
-                const u64 other = (u64)e * a.entry_stride + row;
-                together += a.words[other] == word[i] ? a.p[other] : 0.0f;
+            float together = p;
+            if (a.entries > 32u) {
+                together = 0.0f;
+                for (unsigned e = 0; e < a.entries; ++e) {
+                    const u64 other = (u64)e * a.entry_stride + row;
+                    together += a.words[other] == word[i] ? a.p[other] : 0.0f;
+                }
+            } else {
+                const unsigned same = __match_any_sync(0xffffffffu, word[i]);
+                if (__any_sync(0xffffffffu, word[i] >= 0 && (same & (same - 1u)) != 0u)) {
+                    together = 0.0f;
+                    for (unsigned e = 0; e < 32u; ++e) {
+                        const float q = __shfl_sync(0xffffffffu, p, e);
+                        together += same >> e & 1u ? q : 0.0f;
+                    }
+                }
             }
             if (word[i] >= 0) value[i] = exp2_fast(over) - together * sum;
         }
         loss = all_lanes(loss);
-        float least = __int_as_float(0x7f800000);
-        for (int n = -16; n <= 16; ++n) {
-            const float by = 1.0f + (float)n * (1.0f / 8192.0f), back = 1.0f / by;
-            float off = 0.0f;
+        // A factor for each lane.
+        const float by = 1.0f + (float)((int)lane - 16) * (1.0f / 8192.0f), over_by = 1.0f / by;
+        float off = 0.0f;
 #pragma unroll
-            for (unsigned i = 0; i < kEntryRounds; ++i) {
-                if (32u * i >= a.entries) break;
-                const float d = value[i] - by * __bfloat162float(__float2bfloat16_rn(value[i] * back));
+        for (unsigned i = 0; i < kEntryRounds; ++i) {
+            if (32u * i >= a.entries) break;
+            for (unsigned e = 0; e < min(32u, a.entries - 32u * i); ++e) {
+                const float v = __shfl_sync(0xffffffffu, value[i], e), d = v - by * __bfloat162float(__float2bfloat16_rn(v * over_by));
                 off += d * d;
             }
-            off = all_lanes(off);
-            if (off < least) {
-                least = off;
-                factor = by;
-            }
         }
+        // The best of them; of equal ones the first. (Squares are not negative: as whole numbers they are in the same order, and NaN is behind them.)
+        const unsigned least = __reduce_min_sync(0xffffffffu, __float_as_uint(off) & 0x7fffffffu), best = __ballot_sync(0xffffffffu, (__float_as_uint(off) & 0x7fffffffu) == least);
+        factor = __shfl_sync(0xffffffffu, by, __ffs((int)best) - 1);
         const float back = 1.0f / factor;
 #pragma unroll
         for (unsigned i = 0; i < kEntryRounds; ++i)
@@ -1644,10 +1689,14 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
     B2_CUDA(launch_dependent<FinishArgs>(finish_kernel<kKind, T>, dim3(t.left * 8 * (t.n_tile / 32)), 256, 0, c.stream, f));
 }
 
+// Words of ProductArgs::hits.
+std::size_t hit_words(const VocabularyLossCall& c) { return (c.vocabulary + kHalf - 1) / kHalf * ((c.tokens + 31) / 32) * (std::size_t)((c.entries + 31) / 32); }
+
 struct Kept {
     float *top, *sum, *valid, *count, *probs;
     unsigned* magnitudes;
     int* words;  // of the teacher's entries, and their probabilities: [entries][tokens]
+    unsigned* hits;
 };
 Kept kept_of(const VocabularyLossCall& c) {
     Kept k;
@@ -1658,6 +1707,7 @@ Kept kept_of(const VocabularyLossCall& c) {
     k.magnitudes = reinterpret_cast<unsigned*>(k.count + 1);
     k.probs = k.count + 3;
     k.words = reinterpret_cast<int*>(k.probs + c.tokens * (std::size_t)c.entries);
+    k.hits = reinterpret_cast<unsigned*>(k.words + c.tokens * (std::size_t)c.entries);
     return k;
 }
 
@@ -1712,6 +1762,8 @@ void logits_arguments(const VocabularyLossCall& c, ProductArgs& a) {
     a.entry_stride = (unsigned)c.tokens;
     a.words = kept_of(c).words;
     a.probs = kept_of(c).probs;
+    a.hits = kept_of(c).hits;
+    a.hit_rows = (unsigned)((c.tokens + 31) / 32);
     a.targets = c.targets;
     a.target_stride = c.target_strides[0];
     a.targets64 = c.targets64;
@@ -1741,6 +1793,9 @@ void launch_entries(const VocabularyLossCall& c, const Operand& x, const Operand
     e.temperature = c.temperature;
     e.words = c.distillation ? kept.words : nullptr;
     e.probs = kept.probs;
+    e.hits = kept.hits;
+    e.hit_rows = (unsigned)((c.tokens + 31) / 32);
+    if (c.distillation) B2_CUDA(cudaMemsetAsync(kept.hits, 0, hit_words(c) * sizeof(unsigned), c.stream));
     e.valid = kept.valid;
     e.top = top;
     B2_CUDA(launch_dependent<EntriesArgs>(entries_kernel, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, c.stream, e));
@@ -1904,6 +1959,7 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         a.picked = a.entry_logits = reinterpret_cast<float*>(workspace + p.picked_at);
         a.words = kept.words + first;
         a.probs = kept.probs + first;
+        a.hits = kept.hits + first / 32 * (unsigned)((c.entries + 31) / 32);  // (pieces of the rows are whole tiles)
         a.top = kept.top + first;
         a.sum = kept.sum + first;
         a.valid = kept.valid + first;
@@ -2020,7 +2076,7 @@ bool at_once(const VocabularyLossCall& c) {
 
 }  // namespace
 
-std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 3 + 3 + 2 * c.tokens * (std::size_t)c.entries; }
+std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 3 + 3 + 2 * c.tokens * (std::size_t)c.entries + hit_words(c); }
 
 std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient) {
     return call.tokens == 0 ? 0 : plan_of(call, gradient ? Pass::Gradient : Pass::Loss).bytes;
