@@ -6,7 +6,9 @@
 //
 // Four products on the tensor cores, one kernel for all of them (product_kernel): a pair of CTAs works on a tile of 256 x 256 (a gradient of a narrow
 // matrix: 256 x 128), 64 elements of the summed axis at a time, the accumulators in tensor memory, twice, so that one tile is worked off while the next is summed.
-//   Stats   x w^T  -> the maximum of each row of a tile and the sum of e^(z - maximum), joined by join_kernel; the target's logit by the way
+// Of a CTA's warps one copies by TMA, one issues products, eight work tiles off. The products bound it (8192 x 50257 x 768 bf16: tensor pipe 0.95 busy in the gradients, 1.6 PFLOP/s, 0.82 where
+// exponentials are made), and in the long run power.
+//   Stats   x w^T  -> the maximum of each row of a tile and the sum of e^(z - maximum), joined by join_kernel; the logits that count by the way
 //   Probs   x w^T  -> P = r_t (q - y) for a piece of the vocabulary, in 16 bits, to memory
 //   WeightGrad  P^T x,   InputGrad  P w   of that piece
 // So the backward pass makes the logits a second time, a third more than the products that it cannot do without; keeping them would take 2 to 4 bytes for every token
@@ -14,11 +16,13 @@
 // complete; dx, which is small, is added up in 32 bits.
 //
 // bf16, one loss for all rows (both()): its gradient is known but for a factor when the loss is made, and bf16 has the exponents to do without a second product of
-// logits. What is stored of a piece of the rows is E = 2^((z - r_t) log2(e) / tau), r_t being the target's logit (the largest of the entries'), which a small kernel makes first:
+// logits. What is stored of a piece of the rows is E = 2^((z - r_t) log2(e) / tau), r_t being the target's logit (that of the entry which the teacher is surest of), which a small kernel makes first:
 //   Exps  x w^T -> E in 16 bits, and its sums S_t over the words of a tile; close_kernel joins them and sets E of the targets to E - y S
 //   WeightGrad  E^T (x / S),   InputGrad  (E w) / S      and the backward pass multiplies by what comes back, if that is not 1
 // Where S_t passes 2^100 (a logit is 69 above the target's) a word in memory says so, and Stats, join_kernel and Probs, which look at it and end otherwise, make P instead.
-// 8192 x 50257 x 768, loss and gradients: 2025 -> 1459 us; 4096 x 131072 x 4096: 13.2 -> 10.2 ms. P is the operand of two products and therefore of their type: its rounding (2^-8 of each
+// 8192 x 50257 x 768, loss and gradients: 2025 -> 1450 us; 4096 x 131072 x 4096: 13.2 -> 10.2 ms.
+//
+// P is the operand of two products and therefore of their type: its rounding (2^-8 of each
 // element in bf16) is what the gradients lose beside their own. r_t = c_t / max |c| is 1 in a mean or a sum, so that the target's element
 // stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there.
 //
@@ -42,7 +46,6 @@
 #include "mem/cu_driver.h"
 
 #include <algorithm>
-#include <atomic>
 #include <cstdint>
 #include <mutex>
 #include <stdexcept>
@@ -1534,15 +1537,17 @@ enum class Pass { Loss, Gradient, Both };
 
 // A product so small, up to a whole tile of rows, that launches count for more than it does: both() is not used, which has more of them (us, apart / at once; rows x words x columns in thousand
 // millions: 512 x 512 x 64 90 / 93 (0.02), 512 x 5000 x 256 90 / 95 (0.7), 1024 x 5000 x 256 101 / 99 (1.3), 16 x 32000 x 768 91 / 96 (6.3), 16 x 50257 x 768 111 / 103 (9.9),
-// 512 x 32000 x 768 132 / 126 (12.6), 1024 x 50257 x 768 277 / 230 (40)), and P has two parts, which costs its gradients a second product and leaves them their own rounding alone.
+// 512 x 32000 x 768 132 / 126 (12.6), 1024 x 50257 x 768 277 / 230 (40)).
 bool small(const VocabularyLossCall& c) { return std::max<std::size_t>(c.tokens, kTile) * c.vocabulary < (1ull << 33) / std::max<std::size_t>(c.width, 1); }
+// Of those, P has two parts in 16-bit types too, which costs its gradients a second product and leaves them their own rounding alone; not where P itself is large and its matrix narrow.
+bool fine(const VocabularyLossCall& c) { return small(c) && std::max<std::size_t>(c.tokens, kTile) * c.vocabulary <= (1ull << 25); }
 
 Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     Plan p;
     const std::size_t e = dtype_size(c.dtype), t = c.tokens, v = c.vocabulary;
     p.parts = c.dtype == DType::Float ? 2 : 1;
     p.products = c.dtype == DType::Float ? 3 : 1;
-    p.prob_parts = c.dtype == DType::Float || (pass == Pass::Gradient && small(c)) ? 2 : 1;
+    p.prob_parts = c.dtype == DType::Float || (pass == Pass::Gradient && fine(c)) ? 2 : 1;
     p.grad_products = c.dtype == DType::Float ? 3 : p.prob_parts;
     p.device_pairs = pairs_of_device(current_device());
     p.pitch = (c.width + 7) / 8 * 8;
