@@ -194,12 +194,26 @@ Lost loss_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tenso
     return r;
 }
 
+// The capture that the current stream is part of; 0: none.
+std::int64_t capture_of(const at::Tensor& t) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream_of(t)), &status, &id) != cudaSuccess) {
+        (void)cudaGetLastError();
+        throw Failed("the stream's capture has failed");
+    }
+    return status == cudaStreamCaptureStatusNone ? 0 : static_cast<std::int64_t>(id);
+}
+
 struct VocabularyLoss : torch::autograd::Function<VocabularyLoss> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets, const std::optional<at::Tensor>& teacher,
                               std::int64_t entries, double temperature, std::int64_t reduction) {
+        const c10::cuda::CUDAGuard guard(x.device());
         Lost r = loss_forward(x, weight, targets, teacher.has_value() ? *teacher : at::Tensor(), {entries, temperature, reduction}, x.requires_grad(), weight.requires_grad());
         ctx->save_for_backward({x, weight, targets, r.kept});
-        // (Not among what is saved: whoever asks for them first takes them away.)
+        // (Not among what is saved: whoever asks for them first takes them away. Only in the capture that they were made in: a graph of the
+        // backward pass alone would multiply them at each replay.)
+        ctx->saved_data["capture"] = capture_of(x);
         if (r.x_grad.defined()) ctx->saved_data["dx"] = std::move(r.x_grad);
         if (r.weight_grad.defined()) ctx->saved_data["dw"] = std::move(r.weight_grad);
         ctx->saved_data["temperature"] = temperature;
@@ -229,7 +243,7 @@ struct VocabularyLoss : torch::autograd::Function<VocabularyLoss> {
             void** const gradients[2] = {&p.c.x_grad, &p.c.weight_grad};
             for (int i = 0; i < 2; ++i) {
                 const auto made = ctx->saved_data.find(kMade[i]);
-                if (!ctx->needs_input_grad(i) || made == ctx->saved_data.end()) continue;
+                if (!ctx->needs_input_grad(i) || made == ctx->saved_data.end() || ctx->saved_data["capture"].toInt() != capture_of(x)) continue;
                 result[i] = made->second.toTensor();
                 ctx->saved_data.erase(made);
                 *gradients[i] = result[i].data_ptr();

@@ -1,5 +1,8 @@
 """Losses over a vocabulary whose logits are never stored, and their gradients, against 64 bits."""
 import ctypes
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -501,3 +504,165 @@ def test_a_failure_in_a_backward_pass_is_this_library_s_error():
     with replaced("b2_vocabulary_loss_times", prototype, lambda original, *arguments: 1):
         with pytest.raises(nn.B200CclError):
             ops.linear_cross_entropy(x.requires_grad_(), w, t).backward()
+
+
+def test_only_one_gradient_made_with_the_loss():
+    x, w, t = inputs(300, 40000, 856, torch.bfloat16)
+    assert made_with_the_loss(x, w, t)
+    one = torch.ones((), device="cuda")
+    both = run(cross_entropy(t, "mean"), x, w, one)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(ops.linear_cross_entropy(xg, w, t), xg)
+    (dw,) = torch.autograd.grad(ops.linear_cross_entropy(x, wg, t), wg)
+    assert torch.equal(dx, both["dx"]) and torch.equal(dw, both["dw"])
+    # A gradient that nobody asks for is left where it is.
+    loss = ops.linear_cross_entropy(xg, wg, t)
+    (dx,) = torch.autograd.grad(loss * 2, xg)
+    assert torch.equal(dx, both["dx"] * 2)
+
+
+def test_graphs_of_gradients_made_with_the_loss():
+    """Two graphs at once, with what comes back in memory that changes; and a backward pass in a graph whose loss was made before it."""
+    graphs, states, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for i, s in enumerate(streams):
+        x, w, t = inputs(200, 40000, 856, torch.bfloat16, seed=10 * i)
+        back = torch.tensor(1.0, device="cuda")
+        logits, tokens = teacher(200, 9, 40000, torch.bfloat16, seed=i)
+        call = cross_entropy(t, "mean") if i == 0 else distillation(logits, tokens, 2.0, "sum")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            run(call, x, w, back)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = run(call, x, w, back)
+        graphs.append(graph)
+        states.append((call, x, w, back, out))
+    for turn in range(4):
+        for i, (call, x, w, back, out) in enumerate(states):
+            x.copy_(inputs(200, 40000, 856, torch.bfloat16, seed=100 * turn + i)[0])
+            back.fill_((1.0, 0.3, 1.0, -2.0)[turn])
+        want = [run(*state[:4]) for state in states]
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for state, expected in zip(states, want):
+            assert all(torch.equal(state[4][name], expected[name]) for name in expected)
+    call, x, w, back, _ = states[0]
+    x, w = x.clone().requires_grad_(), w.clone().requires_grad_()
+    s = streams[0]
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loss = call(x, w)
+    torch.cuda.synchronize()
+    back.fill_(0.5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        grads = torch.autograd.grad(loss, (x, w), back, retain_graph=True)
+    want = plain.losses(x, w, inputs(200, 40000, 856, torch.bfloat16, seed=0)[2], dloss=torch.tensor(0.5, device="cuda"))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for name, g in zip(("dx", "dw"), grads):
+            plain.within(g, want[name], name)
+
+
+def test_a_graph_of_the_loss_and_one_of_its_backward_pass():
+    """The second may be replayed more often than the first."""
+    x, w, t = inputs(200, 40000, 856, torch.bfloat16)
+    s = torch.cuda.Stream()
+    back = torch.tensor(0.3, device="cuda")
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        expected = run(cross_entropy(t, "mean"), x, w, back)
+    torch.cuda.synchronize()
+    want = plain.losses(x, w, t, dloss=back)
+    x.requires_grad_()
+    w.requires_grad_()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=s):
+        loss = ops.linear_cross_entropy(x, w, t)
+    with torch.cuda.graph(second, stream=s, pool=first.pool()):
+        grads = torch.autograd.grad(loss, (x, w), back)
+    for _ in range(2):
+        first.replay()
+        for _ in range(2):
+            second.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(loss, expected["loss"])
+            for name, g in zip(("dx", "dw"), grads):
+                plain.within(g, want[name], name)
+
+
+FIRST_INSIDE_A_CAPTURE = """
+import torch
+from nano_nccl_b200 import ops
+torch.cuda.init()
+w = torch.randn(300, 64, device="cuda").bfloat16().requires_grad_()
+t = torch.randint(0, 300, (50,), device="cuda")
+s = torch.cuda.Stream()
+s.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(s):  # (torch's own first calls)
+    torch.autograd.grad((w * 2).float().sum(), w)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def step():
+    loss = ops.linear_cross_entropy(ops.embedding(t, w, 8.0), w, t)
+    return loss, torch.autograd.grad(loss, w)[0]
+with torch.cuda.graph(graph, stream=s):
+    captured = step()
+graph.replay()
+torch.cuda.synchronize()
+want = step()
+assert torch.equal(captured[0], want[0]) and torch.equal(captured[1], want[1])
+print("the same")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    done = subprocess.run([sys.executable, "-c", FIRST_INSIDE_A_CAPTURE], capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr
+
+
+def test_calls_of_several_threads():
+    """Each on a stream of its own, at the same time, with gradients."""
+    results, wanted = [None] * 4, []
+    states = []
+    for i in range(4):
+        x, w, t = inputs(150 + i, 3000, 136, (torch.bfloat16, torch.float32)[i % 2], seed=i)
+        states.append((cross_entropy(t, "mean"), x, w, torch.ones((), device="cuda")))
+        wanted.append(run(*states[-1]))
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                out = run(*states[i])
+            torch.cuda.current_stream().synchronize()
+        results[i] = out
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    for got, want in zip(results, wanted):
+        assert got is not None and all(torch.equal(got[name], want[name]) for name in want)
+
+
+def test_transformations_are_refused():
+    x, w, t = inputs(4, 30, 64, torch.float32)
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.vmap(lambda a: ops.linear_cross_entropy(a, w, t))(x.expand(2, 4, 64))
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.vmap(lambda a: ops.embedding(t, a))(w.expand(2, 30, 64))
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.grad(lambda a: ops.linear_cross_entropy(a, w, t))(x)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(ValueError, match="tangent"):
+            ops.linear_cross_entropy(dual, w, t)
+        with pytest.raises(ValueError, match="tangent"):
+            ops.embedding(t, dual)
