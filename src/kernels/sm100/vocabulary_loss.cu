@@ -19,7 +19,7 @@
 // logits. What is stored of a piece of the rows is E = 2^((z - r_t) log2(e) / tau), r_t being the target's logit (that of the entry which the teacher is surest of), which a small kernel makes first:
 //   Exps  x w^T -> E in 16 bits, and its sums S_t over the words of a tile; close_kernel joins them and sets E of the targets to E - y S
 //   WeightGrad  E^T (x / S),   InputGrad  (E w) / S      and the backward pass multiplies by what comes back, if that is not 1
-// Where S_t passes 2^100 (a logit is 69 above the target's) a word in memory says so, and Stats, join_kernel and Probs, which look at it and end otherwise, make P instead.
+// Where S_t passes 2^64 (a logit is 44 above the target's: E w and x / S have 2^64 to spare, whatever x and w are scaled by) a word in memory says so, and Stats, join_kernel and Probs, which look at it and end otherwise, make P instead.
 // 8192 x 50257 x 768, loss and gradients: 2025 -> 1450 us; 4096 x 131072 x 4096: 13.2 -> 10.2 ms.
 //
 // P is the operand of two products and therefore of their type: its rounding (2^-8 of each
@@ -28,7 +28,7 @@
 //
 // fp32: x, w and P are sums of two fp16 matrices each, what fp16 makes of an element and what it makes of the rest, after a power of two that brings the largest
 // element of x and of w to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
-// it. (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 2055.)
+// it. (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 1760.)
 // The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and their sums are added up in registers, rounded, after every 256 to 8192
 // elements of the summed axis: a loss over columns of 4096 in bf16 is 1.8e-6 off otherwise, all of it in one direction.
 //
@@ -1128,7 +1128,7 @@ struct CloseArgs {
     u64 pitch;
 };
 
-constexpr float kLargestSum = 1.2676506e30f;  // 2^100
+constexpr float kLargestSum = 18446744073709551616.0f;  // 2^64
 
 // A CTA takes 32 rows: each of its warps every 32nd part of them, then one row.
 //

@@ -279,6 +279,19 @@ def test_logits_too_far_above_the_target_s(wide):
         check(call, given, w, targets, "mean" if call is calls[0][0] else "sum", kind, tau)
 
 
+@pytest.mark.parametrize("power", [-50, 50])
+def test_logits_far_above_the_target_s_of_inputs_that_are_small_or_large(power):
+    """Neither the rows over their sums nor the exponentials times the matrix leave the range of the type."""
+    rows, v, h = 200, 530000, 64
+    x, w, t = inputs(rows, v, h, torch.bfloat16)
+    assert made_with_the_loss(x, w, t)
+    t[rows - 7] = 9
+    for s in (0.02, 0.03, 0.035, 0.045, 0.055):  # (a logit of word 5 of 25 to 70)
+        far = x.clone()
+        far[rows - 7] = w[5] * 40 * h ** 0.5 * s
+        check(cross_entropy(t, "mean"), far * 2.0 ** power, w * 2.0 ** -power, t, "mean")
+
+
 def test_asking_for_gradients_made_with_the_loss():
     """Twice, apart, multiplied with what comes back, of a loss whose inputs changed."""
     x, w, t = inputs(300, 40000, 856, torch.bfloat16)
