@@ -292,6 +292,22 @@ def test_logits_far_above_the_target_s_of_inputs_that_are_small_or_large(power):
         check(cross_entropy(t, "mean"), far * 2.0 ** power, w * 2.0 ** -power, t, "mean")
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 12])
+def test_gradients_of_few_rows_lose_their_own_rounding_alone(dtype, rows):
+    x, w, t = inputs(rows, 9000, 4072, dtype)
+    logits, tokens = teacher(rows, 12, 9000, dtype)
+    for targets, kind, call in ((t, None, cross_entropy(t, "none")), (tokens, logits, distillation(logits, tokens, 1.0, "none"))):
+        out = check(call, x, w, targets, "none", kind)
+        want = plain.losses(x, w, targets, kind, reduction="none", dloss=back_of(rows, "none"))
+        for name in ("dx", "dw"):
+            exact = want[name][0]
+            rounded = (exact.to(dtype).double() - exact).norm()
+            # The softmax is off by what the logits are: sums of 4072 products of about 0.03 that may lose 2^-23 of themselves 64 times, 1e-5 at most beside roundings of at least 2^-13 in the mean,
+            # which it makes larger by a tenth at most.
+            assert (out[name].double() - exact).norm() <= 1.1 * rounded, name
+
+
 def test_asking_for_gradients_made_with_the_loss():
     """Twice, apart, multiplied with what comes back, of a loss whose inputs changed."""
     x, w, t = inputs(300, 40000, 856, torch.bfloat16)
