@@ -623,9 +623,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             });
                         }
                         if (!kTeacher && __any_sync(0xffffffffu, at < 32u)) {
-                            // (Exps: the target's is 1 by definition; its logit was made by another kernel, whose roundings differ.)
+                            // (Exps: the target's is 1 by definition, its logit was made by another kernel, whose roundings differ. Sums are of the others alone, so that nothing is
+                            // lost of a row that is sure of its target, and close_kernel makes the element itself.)
 #pragma unroll
-                            for (unsigned j = 0; j < 32; ++j) f[h][j] = j != at ? f[h][j] : (kKind == Kind::Probs ? f[h][j] - weight : 1.0f);
+                            for (unsigned j = 0; j < 32; ++j) f[h][j] = j != at ? f[h][j] : (kKind == Kind::Probs ? f[h][j] - weight : 0.0f);
                         }
                         if (c + 32u * h + 32u > columns) {
 #pragma unroll
@@ -1160,19 +1161,20 @@ __global__ void __launch_bounds__(1024) close_kernel(const __grid_constant__ Clo
     const unsigned row = first + warp;
     if (row >= a.rows) return;
     sum = all_lanes(all[lane][warp]);
-    const float valid = a.valid[row], log_sum = log2f(sum);
+    const float valid = a.valid[row];
     float loss = 0.0f, factor = 1.0f;
     if (a.entries == 0) {
         const long long target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
-        if (lane == 0 && target >= 0 && target < a.vocabulary) {
-            const float v = 1.0f - sum;
-            const __nv_bfloat16 rounded = __float2bfloat16_rn(v);
-            a.exps[(u64)row * a.pitch + (u64)target] = rounded;
-            if (v != 0.0f) factor = v / __bfloat162float(rounded);
+        if (target >= 0 && target < a.vocabulary) {
+            const float others = sum;  // (E of the target less S is that of the others)
+            const __nv_bfloat16 rounded = __float2bfloat16_rn(-others);
+            if (lane == 0) a.exps[(u64)row * a.pitch + (u64)target] = rounded;
+            if (others > 1e-30f) factor = -others / __bfloat162float(rounded);
+            loss = log1pf(others);
+            sum = 1.0f + others;
         }
-        loss = kLn2 * log_sum;
     } else {
-        const float top = a.top[row];
+        const float top = a.top[row], log_sum = log2f(sum);
         float value[kEntryRounds];
         int word[kEntryRounds];
 #pragma unroll

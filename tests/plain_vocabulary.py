@@ -83,12 +83,16 @@ def losses(x, weight, targets, teacher_logits=None, temperature=1.0, reduction="
     if dtype != torch.bfloat16:
         element = element + c.abs().max() * 2.0 ** -14 * smallest(torch.float16)
     element = element + 2.0 ** -126
+    # bf16, one loss for all rows: a row has a factor that makes its target's element, or those of its entries, the ones that are rounded least. It is v / bf16(v) for some v, within h of 1, and the
+    # other elements, rounded on their own (h, above), are multiplied by it: (1 + h) (1 + h) - 1 is h and h (1 + h).
+    made_with_the_loss = dtype == torch.bfloat16 and reduction != "none"
+    if made_with_the_loss:
+        element = element + h * (1 + h) * dz.abs()
     for name, p, e, m, summed in (("dx", dz, element, w, vocabulary), ("dw", dz.t(), element.t(), a, rows)):
         exact = p @ m
         sums = p.abs() @ m.abs()
         # bf16, one loss for all rows: what is multiplied with x is 1 / S of P's row, S times P beside x / S, which is rounded as P is. Once in the sum of magnitudes, then.
         # And what comes back to the loss is multiplied with a rounded gradient, and the product rounded.
-        made_with_the_loss = dtype == torch.bfloat16 and reduction != "none"
         sums_of_rounded = h * (sums + e @ m.abs()) if name == "dw" and made_with_the_loss else 0.0
         roundings = (2 + h) if made_with_the_loss else 1
         out[name] = (exact, sums_of_rounded + e @ m.abs() + _floor(dtype, m) * p.abs().sum(-1, keepdim=True) + (_sums(dtype, summed) + 16 * 2.0 ** -24) * sums + roundings * h * (exact.abs() + sums_of_rounded + e @ m.abs()) + smallest(dtype))

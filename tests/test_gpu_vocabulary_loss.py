@@ -260,9 +260,28 @@ def test_rows_that_are_sure(dtype):
     assert (out["loss"] >= 0).all() and out["loss"][-1] > 400 and out["loss"][-2] < 0.2
 
 
+@pytest.mark.parametrize("c", [4.0, 8.0, 16.0, 40.0])
+def test_small_losses_made_with_their_gradients(c):
+    """Of rows that are sure of their targets: nothing of what the others leave is lost beside the target's 1."""
+    rows, v, h = 200, 530000, 64
+    _, w, t = inputs(rows, v, h, torch.bfloat16)
+    t[0] = 7
+    x = (w[t.clamp(min=0)].float() * c).bfloat16()
+    assert made_with_the_loss(x, w, t)
+    out = check(cross_entropy(t, "sum"), x, w, t, "sum")
+    there = t >= 0
+    z = x[there].double() @ w.double().t()
+    z = z - z.gather(1, t[there, None])
+    others = torch.exp(z).scatter(1, t[there, None], 0.0).sum(-1)
+    want = torch.log1p(others).sum()
+    # Logits of at most 40 * |w|^2 = 40 * 12: sums of 64 products lose 2^-23 seven times, and their factor of log2(e) rounds once more, of the word's and of the target's. That is what an exponential is off by,
+    # relative to itself, and a loss; the rest, additions and roundings in 32 bits, is 64 * 2^-24 of it.
+    assert abs(float(out["loss"]) - float(want)) <= (2 * 9 * 2.0 ** -23 * float((x.float().abs() * w[t.clamp(min=0)].float().abs()).sum(-1).max()) * 2 + 64 * 2.0 ** -24) * float(want) + 1e-30
+
+
 @pytest.mark.parametrize("wide", [False, True])
 def test_logits_too_far_above_the_target_s(wide):
-    """bf16, one loss for all rows: sums of exponentials over the target's that pass 2^100, in some pieces of the rows and not in others, and a few words over the edge."""
+    """bf16, one loss for all rows: sums of exponentials over the target's that pass 2^64, in some pieces of the rows and not in others, and a few words over the edge."""
     rows, v, h = (200, 530000, 64) if not wide else (14000, 40000, 840)  # (in two pieces of the rows)
     x, w, t = inputs(rows, v, h, torch.bfloat16)
     assert made_with_the_loss(x, w, t)
