@@ -18,7 +18,7 @@
 // bf16, one loss for all rows (both()): its gradient is known but for a factor when the loss is made, and bf16 has the exponents to do without a second product of
 // logits. What is stored of a piece of the rows is E = 2^((z - r_t) log2(e) / tau), r_t being the target's logit (that of the entry which the teacher is surest of), which a small kernel makes first:
 //   Exps  x w^T -> E in 16 bits, and its sums S_t over the words of a tile; close_kernel joins them and sets E of the targets to E - y S
-//   WeightGrad  E^T (x / S),   InputGrad  (E w) / S      and the backward pass multiplies by what comes back, if that is not 1
+//   WeightGrad  E^T (x / S),   InputGrad  (E w) / S      (few rows: x / S in two parts)      and the backward pass multiplies by what comes back, if that is not 1
 // Where S_t passes 2^64 (a logit is 44 above the target's: E w and x / S have 2^64 to spare, whatever x and w are scaled by) a word in memory says so, and Stats, join_kernel and Probs, which look at it and end otherwise, make P instead.
 // 8192 x 50257 x 768, loss and gradients: 2025 -> 1450 us; 4096 x 131072 x 4096: 13.2 -> 10.2 ms.
 //
@@ -92,6 +92,7 @@ struct alignas(64) ProductArgs {
     unsigned products, steps_of_part, steps_of_tile;  // products of parts of the operands
     unsigned chunk;  // steps that are summed on the tensor cores alone, of each of them
     unsigned b_offset;  // added to b's row
+    bool b_in_parts;    // two products: b has two parts, and not a
     unsigned pairs, waves;  // whole tiles of a pair
     unsigned left, splits;  // tiles that are left, and the pieces of each
     bool n_first;       // neighbouring tiles lie along n
@@ -178,7 +179,7 @@ __device__ __forceinline__ unsigned segment_end(const ProductArgs& a, unsigned k
     return min(to, (k / chunk + 1u) * chunk);
 }
 // Which parts of the operands, and which 64 elements, the steps of a tile take, one after another: of a chunk of steps the products with the smallest sums first. Three products:
-// (1, 0), (0, 1), (0, 0); two, of a P of two parts with a matrix of one: (1, 0), (0, 0). (Divided out for each step, the copying thread would be slower than the products.)
+// (1, 0), (0, 1), (0, 0); two, of a P of two parts with a matrix of one: (1, 0), (0, 0), or the other way round. (Divided out for each step, the copying thread would be slower than the products.)
 struct Spot {
     unsigned product, step, from, to;  // of the chunk
     __device__ __forceinline__ Spot(const ProductArgs& a, unsigned k) {
@@ -196,8 +197,8 @@ struct Spot {
         step = from = to;
         to = min(from + a.chunk, a.steps_of_part);
     }
-    __device__ __forceinline__ int part_a(const ProductArgs& a) const { return product == 0u && a.products > 1u ? 1 : 0; }
-    __device__ __forceinline__ int part_b(const ProductArgs& a) const { return product == 1u && a.products == 3u ? 1 : 0; }
+    __device__ __forceinline__ int part_a(const ProductArgs& a) const { return product == 0u && a.products > 1u && !a.b_in_parts ? 1 : 0; }
+    __device__ __forceinline__ int part_b(const ProductArgs& a) const { return a.b_in_parts ? (product == 0u ? 1 : 0) : (product == 1u && a.products == 3u ? 1 : 0); }
 };
 
 struct Tile {
@@ -1270,13 +1271,13 @@ __global__ void __launch_bounds__(1024) count_kernel(const __grid_constant__ Cou
 struct DivideArgs {
     const char* x;
     long long stride;  // bytes
-    uint4* out;        // [rows][pitch]
-    unsigned rows, columns;
+    uint4* out;        // [parts][rows][pitch]
+    unsigned rows, columns, parts;
     Divisor eights;  // of a row
     const float* row_scale;
 };
 
-// Rows of x over their sums, rounded. A thread takes eight elements.
+// Rows of x over their sums, rounded, and what that leaves. A thread takes eight elements.
 __global__ void __launch_bounds__(256) divide_kernel(const __grid_constant__ DivideArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1290,7 +1291,14 @@ __global__ void __launch_bounds__(256) divide_kernel(const __grid_constant__ Div
     Wide<T>::unpack(make_uint4(w[0], w[1], w[2], w[3]), f);
 #pragma unroll
     for (unsigned e = 0; e < 8; ++e) f[e] = scale == 0.0f ? 0.0f : f[e] * scale;
-    a.out[i] = Wide<T>::pack(f);
+    const uint4 v = Wide<T>::pack(f);
+    a.out[i] = v;
+    if (a.parts == 1) return;
+    float rounded[8];
+    Wide<T>::unpack(v, rounded);
+#pragma unroll
+    for (unsigned e = 0; e < 8; ++e) f[e] = fabsf(rounded[e]) < __int_as_float(0x7f800000) ? f[e] - rounded[e] : 0.0f;  // (infinities and NaN have no rest)
+    a.out[(u64)a.rows * a.eights.d + i] = Wide<T>::pack(f);
 }
 
 struct ScaleArgs {
@@ -1514,6 +1522,7 @@ std::size_t padded(std::size_t bytes) { return (bytes + 255) / 256 * 256; }
 struct Plan {
     unsigned parts = 1, products = 1;            // of x and the matrix, and of those of logits
     unsigned prob_parts = 1, grad_products = 1;  // of P, and of the gradients
+    unsigned divided_parts = 1;                  // both at once: of x / S
     bool copy_x = false, copy_weight = false;
     std::size_t pitch = 0;  // elements of a row of the copies
     unsigned device_pairs = 0;
@@ -1543,7 +1552,9 @@ enum class Pass { Loss, Gradient, Both };
 bool small(const VocabularyLossCall& c) { return std::max<std::size_t>(c.tokens, kTile) * c.vocabulary < (1ull << 33) / std::max<std::size_t>(c.width, 1); }
 // Of those, and of any with few rows, P has two parts in 16-bit types too, which costs its gradients a second product and leaves them their own rounding alone; not where P itself is
 // large and its matrix narrow. (Few rows: what P's rounding makes of a row's entry with most of its weight is in all of the row's gradient, and few other rows make up for it: 12 x 23488 x 4072, a teacher
-// of 12 entries in fp16, errors in the norm 3.6e-4 instead of 2.1e-4, which is the gradient's own rounding; 292 us instead of 262, 64 x 131072 x 4096 1265 instead of 1055.)
+// of 12 entries in fp16, errors in the norm 3.6e-4 instead of 2.1e-4, which is the gradient's own rounding; 292 us instead of 262, 64 x 131072 x 4096 1265 instead of 1055.
+// x / S, of both(), has two parts for few rows, whose products' second step of 64 is mostly hidden behind what they write. (2 x 40065 x 2496: errors of dw in the
+// norm 1.4e-3 -> 2.0e-4, most of it is of the targets; 64 x 131072 x 4096 644 -> 680 us, 16 x 50257 x 768 103 -> 101.)
 constexpr u64 kFewRows = 64;
 bool fine(const VocabularyLossCall& c) { return (small(c) || c.tokens <= kFewRows) && std::max<std::size_t>(c.tokens, kTile) * c.vocabulary <= (1ull << 25); }
 
@@ -1567,7 +1578,7 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     p.x_at = take(p.copy_x ? p.parts * t * p.pitch * 2 : 0);
     p.weight_at = take(p.copy_weight ? p.parts * v * p.pitch * 2 : 0);
     std::size_t slots = 0;
-    const auto look = [&](u64 m, u64 n, u64 k) { slots = std::max(slots, tiling_of(m, n, k, p.grad_products, p.n_tile, true, p.device_pairs).slots); };
+    const auto look = [&](u64 m, u64 n, u64 k, unsigned products) { slots = std::max(slots, tiling_of(m, n, k, products, p.n_tile, true, p.device_pairs).slots); };
     if (pass == Pass::Loss) {
         p.stats_at = take((v + kTile - 1) / kTile * 2 * t * sizeof(float2));
         p.picked_at = take(t * std::max(c.entries, 1) * sizeof(float));
@@ -1588,14 +1599,15 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         p.scale_at = take(p.rows * sizeof(float));
         p.probs_at = take(p.rows * p.exps_pitch * 2);
         if (c.weight_grad != nullptr) {
-            p.divided_at = take(p.rows * p.pitch * 2);
+            p.divided_parts = t <= kFewRows ? 2 : 1;
+            p.divided_at = take(p.divided_parts * p.rows * p.pitch * 2);
             const std::size_t sums = p.exps_pitch / kTile * ((c.width + p.n_tile - 1) / p.n_tile) * kTileFloats * sizeof(float);
             if (p.pieces > 1 && sums > kSumsBytes) return Plan();
             if (p.pieces > 1) p.sums_at = take(sums);
         }
         for (const u64 rows : {p.rows, t - (p.pieces - 1) * p.rows}) {
-            if (c.weight_grad != nullptr) look(v, c.width, rows);
-            if (c.x_grad != nullptr) look(rows, c.width, v);
+            if (c.weight_grad != nullptr) look(v, c.width, rows, p.divided_parts);
+            if (c.x_grad != nullptr) look(rows, c.width, v, 1);
         }
     } else {
         const u64 tiles = (v + kTile - 1) / kTile, bytes = (u64)p.prob_parts * t * 2;
@@ -1610,8 +1622,8 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         if (c.x_grad != nullptr && p.pieces > 1)
             p.sums_at = take((t + kTile - 1) / kTile * ((c.width + p.n_tile - 1) / p.n_tile) * kTileFloats * sizeof(float));
         for (const u64 words : {p.piece, rest}) {
-            if (c.weight_grad != nullptr) look(words, c.width, t);
-            if (c.x_grad != nullptr) look(t, c.width, words);
+            if (c.weight_grad != nullptr) look(words, c.width, t, p.grad_products);
+            if (c.x_grad != nullptr) look(t, c.width, words, p.grad_products);
         }
     }
     p.slots_at = take(slots * kTileFloats * sizeof(float));
@@ -2041,20 +2053,23 @@ void both(const VocabularyLossCall& c, const Plan& p) {
             d.out = reinterpret_cast<uint4*>(workspace + p.divided_at);
             d.rows = (unsigned)rows;
             d.columns = (unsigned)c.width;
+            d.parts = p.divided_parts;
             d.eights = Divisor((unsigned)(p.pitch / 8));
             d.row_scale = row_scale;
             const u64 eights = rows * (p.pitch / 8);
             B2_REQUIRE(eights < (1ull << 31), kTooLarge);
             B2_CUDA(launch_dependent<DivideArgs>(divide_kernel, dim3((unsigned)((eights + 255) / 256)), 256, 0, c.stream, d));
-            const Tiling t = tiling_of(c.vocabulary, c.width, rows, 1, p.n_tile, true, p.device_pairs);
+            const Tiling t = tiling_of(c.vocabulary, c.width, rows, p.divided_parts, p.n_tile, true, p.device_pairs);
             a.a = map_of(DType::BFloat16, exps, 1, 64, kStep);
-            a.b = map_of(DType::BFloat16, {d.out, c.width, rows, p.pitch * 2}, 1, 64, kStep);
+            a.b = map_of(DType::BFloat16, {d.out, c.width, rows, p.pitch * 2}, p.divided_parts, 64, kStep);
+            a.b_in_parts = p.divided_parts == 2;
             a.sums = p.pieces > 1 ? reinterpret_cast<float*>(workspace + p.sums_at) : nullptr;
             a.prior = piece != 0;
             a.last = piece + 1 == p.pieces;
             gradient_of(c.weight_grad, c.vocabulary);
             launch_product(Kind::WeightGrad, c, t, a, c.vocabulary, c.width);
             finish<Kind::WeightGrad, T>(c, t, a);
+            a.b_in_parts = false;
         }
         if (c.x_grad != nullptr) {
             const Tiling t = tiling_of(rows, c.width, c.vocabulary, 1, p.n_tile, true, p.device_pairs);

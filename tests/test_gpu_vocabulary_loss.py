@@ -327,6 +327,24 @@ def test_gradients_of_few_rows_lose_their_own_rounding_alone(dtype, rows):
             assert (out[name].double() - exact).norm() <= 1.1 * rounded, name
 
 
+def test_targets_of_few_rows_made_with_the_loss():
+    """The gradient of a target's word loses its own rounding alone, but for what the other rows have of it."""
+    rows, v, h = 9, 40065, 2496
+    x, w, t = inputs(rows, v, h, torch.bfloat16)
+    assert made_with_the_loss(x, w, t)
+    out = check(cross_entropy(t, "mean"), x, w, t, "mean")
+    one = torch.ones((), device="cuda")
+    dw = run(cross_entropy(t, "mean"), x, w, one)["dw"]
+    there = t >= 0
+    words, a = t[there], x[there].double()
+    exact = plain.losses(x, w, t, dloss=one)["dw"][0][words]
+    others = torch.softmax(a @ w.double().t(), -1).scatter(1, words[:, None], 0.0)[:, words] / len(words)
+    rounded = (exact.bfloat16().double() - exact).norm()
+    # (1.1: the softmax, as of few rows above. An element of another row is off by its own rounding and its row's factor, 2^-8 each.)
+    assert (dw[words].double() - exact).norm() <= 1.1 * rounded + 2.1 * 2.0 ** -8 * (others.t() @ a.abs()).norm()
+    assert out["dw"].shape == w.shape
+
+
 def test_asking_for_gradients_made_with_the_loss():
     """Twice, apart, multiplied with what comes back, of a loss whose inputs changed."""
     x, w, t = inputs(300, 40000, 856, torch.bfloat16)
