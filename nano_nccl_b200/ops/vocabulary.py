@@ -5,7 +5,7 @@ stands for no token (the padding of a sequence): it is looked up as zeros, has n
 the vocabulary makes NaN, so that a loss scaler sees it. (Rows that do not count still go through the products: their hidden states must be numbers.)
 
 The logits of 8192 tokens over 50257 words take 1.6 GB in 32 bits, and their gradient as much again. The losses here make them tile by tile on the tensor cores
-and keep two numbers for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: two of them) of the two products that
+and keep a few numbers for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: two of them) of the two products that
 make the gradients. It needs 512 MB at most for that, or 4096 words of the vocabulary.
 
 bfloat16, with one loss for all rows and a product large enough: the logits are made once. A call whose inputs want gradients makes them with the loss, by pieces of the rows (1 GB of workspace,

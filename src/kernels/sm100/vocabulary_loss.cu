@@ -8,7 +8,7 @@
 // matrix: 256 x 128), 64 elements of the summed axis at a time, the accumulators in tensor memory, twice, so that one tile is worked off while the next is summed.
 // Of a CTA's warps one copies by TMA, one issues products, eight work tiles off. The products bound it (8192 x 50257 x 768 bf16: tensor pipe 0.95 busy in the gradients, 1.6 PFLOP/s, 0.82 where
 // exponentials are made), and in the long run power.
-//   Stats   x w^T  -> the maximum of each row of a tile and the sum of e^(z - maximum), joined by join_kernel; the logits that count by the way
+//   Stats   x w^T  -> the maximum of each row of a tile and the sum of e^(z - maximum) (cross entropy: of the words beside the target), joined by join_kernel; the logits that count by the way
 //   Probs   x w^T  -> P = r_t (q - y) for a piece of the vocabulary, in 16 bits, to memory
 //   WeightGrad  P^T x,   InputGrad  P w   of that piece
 // So the backward pass makes the logits a second time, a third more than the products that it cannot do without; keeping them would take 2 to 4 bytes for every token
@@ -120,6 +120,7 @@ struct alignas(64) ProductArgs {
     unsigned hit_rows;
     const float* top;    // [m]: the largest logit, and the sum of e^(z - top): apart, because of a row that is sure of its target the logarithm of all
     const float* sum;    // would round off what it is not sure of
+    const float* rest;   // cross entropy: 1 - q of the target, from the other words' sum
     const float* valid;  // whether the row counts: 1, 0, or NaN
     const float* loss_grad;  // [m], or null: the same for all rows
     long long loss_grad_stride;
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             unsigned hits[kTeacher ? kEntryRounds : 1] = {};  // kTeacher: entries that are here in some row of the warp,
             unsigned near_column[kNear] = {};                 // and the columns of the first few in this row
             const long long first_word = (long long)(first + a.b_offset);
-            float weight = 0.0f, row_top = 0.0f, share_of_sum = 1.0f;
+            float weight = 0.0f, row_top = 0.0f, share_of_sum = 1.0f, of_target = 0.0f;
             if constexpr (kLogits) {
                 if constexpr (kTeacher) {
                     const unsigned rounds = (a.entries + 31u) / 32u;
@@ -516,6 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                         weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (kHalfType ? kHalfScale : 1.0f);
                         row_top = a.top[row];
                         share_of_sum = weight / a.sum[row];
+                        if constexpr (!kTeacher) of_target = -weight * a.rest[row];
                     } else if constexpr (kKind == Kind::Exps) {
                         weight = a.valid[row];
                         row_top = a.top[row];
@@ -581,7 +583,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             for (unsigned j = 0; j < 32; ++j) z = j == column ? f[h][j] : z;
                             if (column < 32u) *to = z;
                         };
-                        if (!kTeacher && __any_sync(0xffffffffu, at < 32u)) pick(at, a.picked + row);
+                        if (!kTeacher && __any_sync(0xffffffffu, at < 32u)) {
+                            pick(at, a.picked + row);
+                            // (Sums are of the other words: beside the target's 1, what they leave of a sure row would be lost.)
+#pragma unroll
+                            for (unsigned j = 0; j < 32; ++j) f[h][j] = j == at ? low : f[h][j];
+                        }
                         each_entry(c + 32u * h, [&](unsigned column, u64 place) { pick(column, a.entry_logits + place); });
                         float most[4] = {f[h][0], f[h][1], f[h][2], f[h][3]};
 #pragma unroll
@@ -627,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                             // (Exps: the target's is 1 by definition, its logit was made by another kernel, whose roundings differ. Sums are of the others alone, so that nothing is
                             // lost of a row that is sure of its target, and close_kernel makes the element itself.)
 #pragma unroll
-                            for (unsigned j = 0; j < 32; ++j) f[h][j] = j != at ? f[h][j] : (kKind == Kind::Probs ? f[h][j] - weight : 0.0f);
+                            for (unsigned j = 0; j < 32; ++j) f[h][j] = j != at ? f[h][j] : (kKind == Kind::Probs ? of_target : 0.0f);
                         }
                         if (c + 32u * h + 32u > columns) {
 #pragma unroll
@@ -851,13 +858,14 @@ struct JoinArgs {
     float temperature, factor;
     float* top;
     float* sum;
+    float* rest;
     float* valid;
     float* loss;
     const unsigned* condition;  // see ProductArgs
     float* row_scale;           // 1 of rows that count, or null
 };
 
-// Each row's maximum and sum, and its loss. A CTA takes 32 rows, each of its warps every 32nd part of them (1024 rows of 394 parts: eight
+// Each row's maximum and sum, those of the words beside the target brought together with it, and its loss. A CTA takes 32 rows, each of its warps every 32nd part of them (1024 rows of 394 parts: eight
 // warps took 12 us).
 __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ JoinArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -891,15 +899,28 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
         const float log_sum = log2f(sum);
         of_row[lane] = make_float2(top, log_sum);
         if (row < a.rows) {
-            a.top[row] = top;
-            a.sum[row] = sum;
             if (a.row_scale != nullptr) a.row_scale[row] = 1.0f;  // (P has the rows' weights in it)
             if (a.entries == 0) {
                 const long long target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
                 const bool bad = target >= (long long)a.vocabulary;
+                float loss = 0.0f, rest = 0.0f;
+                if (target >= 0 && !bad) {
+                    // The other words' sum beside the target: the loss is log(1 + odds).
+                    const float picked = a.picked[row], over = (top - picked) * factor, odds = sum * exp2f(over);
+                    const bool odds_fit = over < 60.0f;
+                    loss = odds_fit ? log1pf(odds) : kLn2 * (over + log_sum);
+                    rest = odds_fit ? odds / (1.0f + odds) : 1.0f;
+                    const float largest = fmaxf(top, picked);
+                    sum = sum * exp2f((top - largest) * factor) + exp2f((picked - largest) * factor);
+                    top = largest;
+                    if (sum != sum) loss = rest = sum;  // (infinite logits, and NaN)
+                }
                 a.valid[row] = bad ? nan32() : (target < 0 ? 0.0f : 1.0f);
-                a.loss[row] = bad ? nan32() : (target < 0 ? 0.0f : kLn2 * ((top - a.picked[row]) * factor + log_sum));
+                a.loss[row] = bad ? nan32() : loss;
+                a.rest[row] = rest;
             }
+            a.top[row] = top;
+            a.sum[row] = sum;
         }
     }
     if (a.entries == 0) return;
@@ -1123,6 +1144,7 @@ struct CloseArgs {
     const float* top;
     float temperature, factor;
     float* sum;
+    float* rest;
     float* loss;
     float* row_scale;
     unsigned* condition;  // set where a sum is too large for E
@@ -1173,6 +1195,7 @@ __global__ void __launch_bounds__(1024) close_kernel(const __grid_constant__ Clo
             if (others > 1e-30f) factor = -others / __bfloat162float(rounded);
             loss = log1pf(others);
             sum = 1.0f + others;
+            if (lane == 0) a.rest[row] = others / sum;
         }
     } else {
         const float top = a.top[row], log_sum = log2f(sum);
@@ -1715,7 +1738,7 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
 std::size_t hit_words(const VocabularyLossCall& c) { return (c.vocabulary + kHalf - 1) / kHalf * ((c.tokens + 31) / 32) * (std::size_t)((c.entries + 31) / 32); }
 
 struct Kept {
-    float *top, *sum, *valid, *count, *probs;
+    float *top, *sum, *rest, *valid, *count, *probs;
     unsigned* magnitudes;
     int* words;  // of the teacher's entries, and their probabilities: [entries][tokens]
     unsigned* hits;
@@ -1724,7 +1747,8 @@ Kept kept_of(const VocabularyLossCall& c) {
     Kept k;
     k.top = c.kept;
     k.sum = k.top + c.tokens;
-    k.valid = k.sum + c.tokens;
+    k.rest = k.sum + c.tokens;
+    k.valid = k.rest + c.tokens;
     k.count = k.valid + c.tokens;
     k.magnitudes = reinterpret_cast<unsigned*>(k.count + 1);
     k.probs = k.count + 3;
@@ -1855,6 +1879,7 @@ void loss(const VocabularyLossCall& c, const Plan& p) {
     j.factor = a.factor;
     j.top = kept.top;
     j.sum = kept.sum;
+    j.rest = kept.rest;
     j.valid = kept.valid;
     j.condition = nullptr;
     j.row_scale = nullptr;
@@ -1901,6 +1926,7 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
         a.b_offset = (unsigned)first;
         a.top = kept.top;
         a.sum = kept.sum;
+        a.rest = kept.rest;
         a.valid = kept.valid;
         a.loss_grad = each ? c.loss_grad : nullptr;
         a.loss_grad_stride = c.loss_grad_stride;
@@ -1984,6 +2010,7 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         a.hits = kept.hits + first / 32 * (unsigned)((c.entries + 31) / 32);  // (pieces of the rows are whole tiles)
         a.top = kept.top + first;
         a.sum = kept.sum + first;
+        a.rest = kept.rest + first;
         a.valid = kept.valid + first;
         a.header = header;
         a.slots = reinterpret_cast<float*>(workspace + p.slots_at);
@@ -2007,6 +2034,7 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         s.temperature = c.temperature;
         s.factor = a.factor;
         s.sum = kept.sum + first;
+        s.rest = kept.rest + first;
         s.loss = losses + first;
         s.row_scale = row_scale;
         s.condition = condition;
@@ -2034,6 +2062,7 @@ void both(const VocabularyLossCall& c, const Plan& p) {
         j.factor = a.factor;
         j.top = kept.top + first;
         j.sum = kept.sum + first;
+        j.rest = kept.rest + first;
         j.valid = kept.valid + first;
         j.loss = losses + first;
         j.condition = condition;
@@ -2101,7 +2130,7 @@ bool at_once(const VocabularyLossCall& c) {
 
 }  // namespace
 
-std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 3 + 3 + 2 * c.tokens * (std::size_t)c.entries + hit_words(c); }
+std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 4 + 3 + 2 * c.tokens * (std::size_t)c.entries + hit_words(c); }
 
 std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient) {
     return call.tokens == 0 ? 0 : plan_of(call, gradient ? Pass::Gradient : Pass::Loss).bytes;

@@ -279,6 +279,23 @@ def test_small_losses_made_with_their_gradients(c):
     assert abs(float(out["loss"]) - float(want)) <= (2 * 9 * 2.0 ** -23 * float((x.float().abs() * w[t.clamp(min=0)].float().abs()).sum(-1).max()) * 2 + 64 * 2.0 ** -24) * float(want) + 1e-30
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [4.0, 16.0, 40.0])
+def test_small_losses_of_each_row(dtype, c):
+    rows, v, h = 70, 2001, 64
+    _, w, t = inputs(rows, v, h, dtype)
+    x = (w[t.clamp(min=0)].float() * c).to(dtype)
+    out = check(cross_entropy(t, "none"), x, w, t, "none")
+    there = t >= 0
+    z = x[there].double() @ w.double().t()
+    z = z - z.gather(1, t[there, None])
+    want = torch.log1p(torch.exp(z).scatter(1, t[there, None], 0.0).sum(-1))
+    # As above, of each row; float32 sums lose 2^-23 fifteen times and have operands of 22 bits: 24 * 2^-23 at most. Below the normal numbers exponentials are zeros.
+    off = 4 * 24 * 2.0 ** -23 * (x[there].float().abs() * w[t[there]].float().abs()).sum(-1).double() + 64 * 2.0 ** -24
+    assert ((out["loss"][there].double() - want).abs() <= off * want + v * 2.0 ** -126).all()
+    assert (want < 1e-6).any() or c == 4.0
+
+
 @pytest.mark.parametrize("wide", [False, True])
 def test_logits_too_far_above_the_target_s(wide):
     """bf16, one loss for all rows: sums of exponentials over the target's that pass 2^64, in some pieces of the rows and not in others, and a few words over the edge."""
