@@ -55,7 +55,7 @@ typedef struct b2_vocabulary_loss {
     float temperature;           /* 1 without a teacher */
     int reduction;               /* 0 none, 1 mean, 2 sum */
     float* loss;                 /* [tokens], or one */
-    float* kept;                 /* written by the loss, read by its backward pass: b2_vocabulary_loss_kept() floats */
+    float* kept;                 /* written by the loss, read by its backward pass: as many floats as the sizes below say */
     /* backward */
     const float* loss_grad;      /* [tokens], or one */
     long long loss_grad_stride;

@@ -94,6 +94,18 @@ def test_c_interface_refuses_what_would_leave_its_buffers(lib):
     for words, kw in (("loss_grad", dict(loss_grad=None)), ("loss_grad", dict(loss_grad=4098)), ("aligned", dict(x_grad=4097)), ("aligned", dict(weight_grad=4097))):
         refused(lib, lib.b2_vocabulary_loss_backward(loss(**kw), None), words)
     assert lib.b2_vocabulary_loss_forward(loss(tokens=0, x=None, targets=None, kept=None, loss=None, workspace=None), None) == 0  # nothing to do
+    # Gradients with the loss: of bf16, of one loss for all rows, of large products, and where they are wanted; otherwise no bytes are asked for, and the call is refused.
+    large = dict(tokens=4096, vocabulary=50000, width=768, x_stride=768, weight_stride=768, reduction=1)
+    for kw in (dict(reduction=1), {**large, "dtype": 0}, {**large, "dtype": 1}, {**large, "reduction": 0}, {**large, "x_grad": None, "weight_grad": None}):
+        assert lib.b2_vocabulary_loss_both_workspace(loss(**kw), ctypes.byref(size)) == 0 and size.value == 0
+        refused(lib, lib.b2_vocabulary_loss_both(loss(**kw), None), "at once")
+    refused(lib, lib.b2_vocabulary_loss_both_workspace(loss(**large), None), "non-null")
+    for words, kw in (("loss must be", dict(loss=None)), ("workspace", dict(workspace=None)), ("aligned", dict(x_grad=4097)), ("aligned", dict(loss=4098))):
+        refused(lib, lib.b2_vocabulary_loss_both(loss(**{**large, **kw}), None), words)
+    for words, kw in (("bf16", dict(dtype=0)), ("loss_grad", dict(loss_grad=None)), ("aligned", dict(weight_grad=4097))):
+        refused(lib, lib.b2_vocabulary_loss_times(loss(**kw), None), words)
+    assert lib.b2_vocabulary_loss_times(loss(x_grad=None, weight_grad=None), None) == 0  # nothing to do
+    refused(lib, lib.b2_vocabulary_loss_within(loss(), 3, ctypes.c_ulonglong(1), None), "pass")
     refused(lib, lib.b2_vocabulary_loss_check_async_error(-1), "device")
 
 
