@@ -95,6 +95,29 @@ class _Block(torch.nn.Module):
         return x + self.mlp(self.ln_2(x))
 
 
+# What a model is asked for beside its logits is looked at in functions of their own, which torch.fx keeps as calls: a traced model decides when it is called.
+@torch.fx.wrap
+def _check_ends(vocabulary, targets, teacher):
+    if targets is not None and teacher is not None:
+        raise ValueError("targets or a teacher, not both")
+    if teacher is not None and vocabulary != "fused":
+        raise ValueError("a teacher needs vocabulary='fused'")
+
+
+@torch.fx.wrap
+def _end(x, weight, vocabulary, targets, teacher, temperature):
+    _check_ends(vocabulary, targets, teacher)
+    if teacher is not None:
+        return ops.linear_distillation(x, weight, *teacher, temperature=temperature)
+    if targets is not None and vocabulary == "fused":
+        return ops.linear_cross_entropy(x, weight, targets)
+    logits = x @ weight.t()
+    if targets is None:
+        return logits
+    losses = torch.nn.functional.cross_entropy(logits.flatten(0, -2).float(), targets.flatten().long().clamp(min=-1), ignore_index=-1, reduction="sum")
+    return losses / (targets >= 0).sum().clamp(min=1)
+
+
 class TinyGPT2(torch.nn.Module):
     """``positions``: "learned" (an embedding) or "rotary" (queries and keys are turned). ``qk_norm``: a norm of each head of queries and keys.
     ``checkpoints``: "int8" keeps the inputs of projections, activations and head norms in 8 bits for the backward pass, None keeps them as they
@@ -122,22 +145,10 @@ class TinyGPT2(torch.nn.Module):
     def forward(self, tokens, targets=None, teacher=None, temperature=1.0):
         """Logits; with ``targets`` [batch, tokens] their mean cross entropy (negative targets do not count), with ``teacher``, a pair of the largest
         logits of a teacher and their tokens ([batch, tokens, entries] each), the mean divergence from it (:func:`nano_nccl_b200.ops.linear_distillation`)."""
-        if targets is not None and teacher is not None:
-            raise ValueError("targets or a teacher, not both")
-        if teacher is not None and self.vocabulary != "fused":
-            raise ValueError("a teacher needs vocabulary='fused'")
+        _check_ends(self.vocabulary, targets, teacher)
         x = self.wte(tokens)
         if self.wpe is not None:
             x = x + self.wpe(torch.arange(tokens.shape[1], device=tokens.device))
         for b in self.blocks:
             x = b(x)
-        x = self.ln_f(x)
-        if teacher is not None:
-            return ops.linear_distillation(x, self.wte.weight, *teacher, temperature=temperature)
-        if targets is not None and self.vocabulary == "fused":
-            return ops.linear_cross_entropy(x, self.wte.weight, targets)
-        logits = x @ self.wte.weight.t()
-        if targets is None:
-            return logits
-        losses = torch.nn.functional.cross_entropy(logits.flatten(0, -2).float(), targets.flatten().long().clamp(min=-1), ignore_index=-1, reduction="sum")
-        return losses / (targets >= 0).sum().clamp(min=1)
+        return _end(self.ln_f(x), self.wte.weight, self.vocabulary, targets, teacher, temperature)
