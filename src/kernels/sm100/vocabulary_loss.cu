@@ -1573,13 +1573,14 @@ enum class Pass { Loss, Gradient, Both };
 // millions: 512 x 512 x 64 90 / 93 (0.02), 512 x 5000 x 256 90 / 95 (0.7), 1024 x 5000 x 256 101 / 99 (1.3), 16 x 32000 x 768 91 / 96 (6.3), 16 x 50257 x 768 111 / 103 (9.9),
 // 512 x 32000 x 768 132 / 126 (12.6), 1024 x 50257 x 768 277 / 230 (40)).
 bool small(const VocabularyLossCall& c) { return std::max<std::size_t>(c.tokens, kTile) * c.vocabulary < (1ull << 33) / std::max<std::size_t>(c.width, 1); }
-// Of those, and of any with few rows, P has two parts in 16-bit types too, which costs its gradients a second product and leaves them their own rounding alone; not where P itself is
+// Of those, and of any with few rows, P has two parts in 16-bit types too, which costs its gradients a second product and leaves them their own rounding alone; not where the rows are many, P itself
 // large and its matrix narrow. (Few rows: what P's rounding makes of a row's entry with most of its weight is in all of the row's gradient, and few other rows make up for it: 12 x 23488 x 4072, a teacher
-// of 12 entries in fp16, errors in the norm 3.6e-4 instead of 2.1e-4, which is the gradient's own rounding; 292 us instead of 262, 64 x 131072 x 4096 1265 instead of 1055.
+// of 12 entries in fp16, errors in the norm 3.6e-4 instead of 2.1e-4, which is the gradient's own rounding; 292 us instead of 262, 64 x 131072 x 4096 1265 instead of 1055;
+// 64 x 262144 x 768 509 instead of 420, 64 x 1048576 x 16, the narrowest, 786 instead of 568.)
 // x / S, of both(), has two parts for few rows, whose products' second step of 64 is mostly hidden behind what they write. (2 x 40065 x 2496: errors of dw in the
 // norm 1.4e-3 -> 2.0e-4, most of it is of the targets; 64 x 131072 x 4096 644 -> 680 us, 16 x 50257 x 768 103 -> 101.)
 constexpr u64 kFewRows = 64;
-bool fine(const VocabularyLossCall& c) { return (small(c) || c.tokens <= kFewRows) && std::max<std::size_t>(c.tokens, kTile) * c.vocabulary <= (1ull << 25); }
+bool fine(const VocabularyLossCall& c) { return c.tokens <= kFewRows || (small(c) && std::max<std::size_t>(c.tokens, kTile) * c.vocabulary <= (1ull << 25)); }
 
 Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     Plan p;
