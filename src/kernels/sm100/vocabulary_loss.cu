@@ -295,10 +295,12 @@ __device__ __forceinline__ float gradient_scale(const float* header, const unsig
     return scale;
 }
 
-// c_t / max |c|; 0 of rows that do not count.
+// c_t / max |c|, of the c that are numbers; 0 of rows that do not count. An infinite c, or NaN, stays what it is, in its own row.
 __device__ __forceinline__ float row_weight(float valid, const float* loss_grad, long long stride, float temperature, float largest, unsigned row) {
     if (loss_grad == nullptr || valid == 0.0f) return valid;
-    return largest == 0.0f ? 0.0f * valid : loss_grad[(long long)row * stride] * temperature * valid / largest;
+    const float c = loss_grad[(long long)row * stride] * temperature;
+    if (!(fabsf(c) < __int_as_float(0x7f800000))) return c * valid;
+    return largest == 0.0f ? 0.0f * valid : c * valid / largest;
 }
 
 // After a wait that ran out: all that this CTA was to make is NaN.
@@ -1098,7 +1100,7 @@ struct HeaderArgs {
     float* header;
 };
 
-// max |c| of the rows, c itself where they share it.
+// max |c| of the rows, of those that are numbers; c itself where they share it.
 __global__ void __launch_bounds__(1024) header_kernel(const __grid_constant__ HeaderArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1109,12 +1111,12 @@ __global__ void __launch_bounds__(1024) header_kernel(const __grid_constant__ He
         }
         return;
     }
-    unsigned most = 0;  // (of magnitudes as whole numbers: NaN is above infinity)
+    unsigned most = 0;  // (of magnitudes as whole numbers: infinity and NaN are above all others)
 #pragma unroll 4
     for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) {
         const float valid = a.valid[i];
         const unsigned bits = __float_as_uint(a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature) & 0x7fffffffu;
-        most = max(most, valid == 0.0f ? 0u : bits);
+        most = max(most, valid == 0.0f || bits >= 0x7f800000u ? 0u : bits);
     }
     __shared__ unsigned all[32];
     most = __reduce_max_sync(0xffffffffu, most);

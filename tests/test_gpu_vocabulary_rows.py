@@ -4,9 +4,33 @@ import pytest
 import torch
 
 import plain_vocabulary as plain
-from test_gpu_vocabulary_loss import cross_entropy, gen, inputs, made_with_the_loss, run
+from test_gpu_vocabulary_loss import DTYPES, cross_entropy, distillation, gen, inputs, made_with_the_loss, run, teacher
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- what comes back to rows that are weighted one by one ------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("frozen", [False, True])
+def test_a_weight_that_is_no_number_stays_in_its_row(dtype, frozen):
+    x, w, t = inputs(80, 700, 72, dtype)
+    t = t.clamp(min=0)
+    dloss = torch.rand(80, device="cuda", generator=gen(5)) + 0.5
+    spoilt, without = dloss.clone(), dloss.clone()
+    spoilt[5], spoilt[9], spoilt[70] = float("inf"), float("nan"), -float("inf")
+    without[[5, 9, 70]] = 0.0
+    logits, tokens = teacher(80, 5, 700, dtype)
+    others = without != 0.0
+    for call in (cross_entropy(t, "none"), distillation(logits, tokens, 2.0, "none")):
+        def gradients(back):
+            a, b = x.clone().requires_grad_(), w.clone().requires_grad_(not frozen)
+            return torch.autograd.grad(call(a, b), (a,) if frozen else (a, b), back)
+        got, want = gradients(spoilt), gradients(without)
+        assert torch.equal(got[0][others], want[0][others]) and want[0].isfinite().all()
+        assert not got[0][~others].isfinite().any()
+        if not frozen:
+            assert not got[1].isfinite().any() and want[1].isfinite().all()
 
 
 # ---- which way a call takes, and what it may lose there --------------------------------------------------
