@@ -2,7 +2,7 @@
 
 ``weight`` is [vocabulary, width], the same matrix at both ends where a model ties them. Tokens and targets are int64 or int32, of any shape and strides. A negative one
 stands for no token (the padding of a sequence): it is looked up as zeros, has no loss and no gradient, and does not count in a mean. One that is not below
-the vocabulary makes NaN, so that a loss scaler sees it. (Rows that do not count still go through the products: their hidden states must be numbers.)
+the vocabulary makes NaN, so that a loss scaler sees it. (Rows that do not count still go through the products: their hidden states must be numbers, of any size.)
 
 The logits of 8192 tokens over 50257 words take 1.6 GB in 32 bits, and their gradient as much again. The losses here make them tile by tile on the tensor cores
 and keep a few numbers for each row; the backward pass makes them again, by pieces of the vocabulary, each of which is an operand of 16 bits (float32: two of them) of the two products that
@@ -41,7 +41,7 @@ def linear_cross_entropy(x, weight, targets, reduction="mean"):
     and ``weight``, which are the same. Under autocast both are cast as those of ``linear``.
 
     What the logits lose is what 32-bit sums lose; the gradient of the logits is rounded to the type of ``x`` before it is multiplied. float32: operands have 22 bits, or 2^-39 of
-    the largest element of ``x``, of ``weight`` and of the rows' weights in the loss, where that is more."""
+    the largest element of ``weight``, of the row of ``x`` (in the gradient of ``weight``: of the rows that count) and of the rows' weights in the loss, where that is more."""
     return load_native_calls().linear_cross_entropy(x, weight, targets, _reduction(reduction))
 
 

@@ -27,8 +27,9 @@
 // stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there.
 //
 // fp32: x, w and P are sums of two fp16 matrices each, what fp16 makes of an element and what it makes of the rest, after a power of two that brings the largest
-// element of x and of w to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
-// it. (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 1760.)
+// element to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
+// it. For logits each row of x has a power of its own, so that no row's loss or gradient depends on how large another is; the gradient of w, which is a sum over rows, takes x
+// with one power for all rows that count, laid out a second time (2048 x 768: 3 us). (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 1760.)
 // The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and their sums are added up in registers, rounded, after every 256 to 8192
 // elements of the summed axis: a loss over columns of 4096 in bf16 is 1.8e-6 off otherwise, all of it in one direction.
 //
@@ -103,7 +104,8 @@ struct alignas(64) ProductArgs {
     u64 wait_ns;
     const unsigned* condition;  // nothing is done while this word is 0, or null
     // Logits
-    const unsigned* magnitudes;  // fp32: the largest of x and of w, see scale_of()
+    const unsigned* magnitudes;  // fp32: the largest of each row of x, see scale_of()
+    const unsigned* w_magnitude; // fp32: that of w
     float factor, factor_rest;   // log2(e) / temperature, see exponentials()
     unsigned out_parts;          // matrices whose sum P is: fp32, and small products of 16 bits, two
     float2* stats; // [2 * tiles along n][m]
@@ -126,7 +128,7 @@ struct alignas(64) ProductArgs {
     long long loss_grad_stride;
     float temperature;
     // Gradients
-    float* header;         // of the workspace: max |c|, and NaN once a product went wrong
+    float* header;         // of the workspace: max |c|, NaN once a product went wrong, and fp32: the power of two that brings x, as the gradient of w takes it, back
     void* gradient;        // rows of n elements
     const float* row_scale;  // [m], or null
     bool wide;             // TMA can write them
@@ -288,10 +290,10 @@ __device__ __forceinline__ float scale_of(unsigned magnitude, bool back) {
 
 // max |c| and whether anything went wrong, in the first words of a gradient's workspace, and what P and the other operand were scaled with.
 template <Kind kKind, typename T>
-__device__ __forceinline__ float gradient_scale(const float* header, const unsigned* magnitudes) {
+__device__ __forceinline__ float gradient_scale(const float* header, const unsigned* w_magnitude) {
     float scale = header[0] + header[1];
     if constexpr (!std::is_same_v<T, __nv_bfloat16>) scale *= 1.0f / kHalfScale;
-    if constexpr (sizeof(T) == 4) scale *= scale_of(magnitudes[kKind == Kind::WeightGrad ? 0 : 1], true);
+    if constexpr (sizeof(T) == 4) scale *= kKind == Kind::WeightGrad ? header[2] : scale_of(*w_magnitude, true);
     return scale;
 }
 
@@ -471,12 +473,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const unsigned in_tile = rank * kHalf + quarter * 32u, column0 = group * b_rows;
         const unsigned staging = base + kAtStaging + (warp - kFirstEpilogueWarp) * kStagingBytes;
         float scale = 1.0f;
-        if constexpr (!kLogits) scale = gradient_scale<kKind, T>(a.header, a.magnitudes);
+        if constexpr (!kLogits) scale = gradient_scale<kKind, T>(a.header, a.w_magnitude);
         Pair32 back_x = both32(1.0f), back_w = both32(1.0f);
-        if constexpr (kLogits && sizeof(T) == 4) {
-            back_x = both32(scale_of(a.magnitudes[0], true));
-            back_w = both32(scale_of(a.magnitudes[1], true));
-        }
+        if constexpr (kLogits && sizeof(T) == 4) back_w = both32(scale_of(*a.w_magnitude, true));
         const float low = -__int_as_float(0x7f800000);
         unsigned segments = 0;
         for (unsigned i = 0; i < share.runs; ++i) {
@@ -514,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                     }
                 }
                 if (row < a.m) {
+                    if constexpr (sizeof(T) == 4) back_x = both32(scale_of(a.magnitudes[row], true));
                     if constexpr (!kTeacher) target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
                     if constexpr (kKind == Kind::Probs) {
                         weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (kHalfType ? kHalfScale : 1.0f);
@@ -791,7 +791,7 @@ struct FinishArgs {
     bool prior, last;
     const float* header;
     const float* row_scale;
-    const unsigned* magnitudes;
+    const unsigned* w_magnitude;
     unsigned m, n, m_tiles, n_tiles, n_tile, whole_tiles, left, splits;
     bool n_first;
 };
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
         reinterpret_cast<float4*>(a.sums + (u64)tile * kTileFloats)[at] = sum;
         return;
     }
-    const float scale = gradient_scale<kKind, T>(a.header, a.magnitudes);
+    const float scale = gradient_scale<kKind, T>(a.header, a.w_magnitude);
     __shared__ float turned[32][33];
     float* t = &turned[lane][warp * 4u];
     t[0] = sum.x * scale;
@@ -1095,38 +1095,42 @@ struct HeaderArgs {
     long long loss_grad_stride;
     const float* valid;
     const float* count;  // of a mean, or null
-    unsigned rows;       // 0: one loss for all rows
+    unsigned rows;
+    bool each;           // loss_grad has an element for each row
+    const unsigned* magnitudes;  // fp32: the largest of each row of x, or null
     float temperature;
     float* header;
 };
 
-// max |c| of the rows, of those that are numbers; c itself where they share it.
+// max |c| of the rows, of those that are numbers; c itself where they share it. fp32: the power of two for x in the gradient of w, of the rows that count.
 __global__ void __launch_bounds__(1024) header_kernel(const __grid_constant__ HeaderArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (a.rows == 0) {
-        if (threadIdx.x == 0) {
-            a.header[0] = a.loss_grad[0] * a.temperature / (a.count != nullptr ? fmaxf(*a.count, 1.0f) : 1.0f);
-            a.header[1] = 0.0f;
-        }
-        return;
-    }
-    unsigned most = 0;  // (of magnitudes as whole numbers: infinity and NaN are above all others)
+    unsigned most = 0, most_x = 0;  // (of magnitudes as whole numbers: infinity and NaN are above all others)
+    if (a.each || a.magnitudes != nullptr) {
 #pragma unroll 4
-    for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) {
-        const float valid = a.valid[i];
-        const unsigned bits = __float_as_uint(a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature) & 0x7fffffffu;
-        most = max(most, valid == 0.0f || bits >= 0x7f800000u ? 0u : bits);
+        for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) {
+            const float valid = a.valid[i];
+            const unsigned bits = a.each ? __float_as_uint(a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature) & 0x7fffffffu : 0u;
+            most = max(most, valid == 0.0f || bits >= 0x7f800000u ? 0u : bits);
+            if (a.magnitudes != nullptr) most_x = max(most_x, valid == 0.0f ? 0u : a.magnitudes[i]);
+        }
     }
-    __shared__ unsigned all[32];
+    __shared__ unsigned all[32], all_x[32];
     most = __reduce_max_sync(0xffffffffu, most);
-    if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = most;
+    most_x = __reduce_max_sync(0xffffffffu, most_x);
+    if ((threadIdx.x & 31u) == 0) {
+        all[threadIdx.x / 32u] = most;
+        all_x[threadIdx.x / 32u] = most_x;
+    }
     __syncthreads();
     if (threadIdx.x >= 32u) return;
     most = __reduce_max_sync(0xffffffffu, all[threadIdx.x]);
+    most_x = __reduce_max_sync(0xffffffffu, all_x[threadIdx.x]);
     if (threadIdx.x == 0) {
-        a.header[0] = __uint_as_float(most);
+        a.header[0] = a.each ? __uint_as_float(most) : a.loss_grad[0] * a.temperature / (a.count != nullptr ? fmaxf(*a.count, 1.0f) : 1.0f);
         a.header[1] = 0.0f;
+        a.header[2] = scale_of(most_x, true);
     }
 }
 
@@ -1357,37 +1361,74 @@ __global__ void __launch_bounds__(512) times_kernel(const __grid_constant__ Scal
     }
 }
 
-// fp32: x and the matrix.
-struct Pair32Matrices {
-    const char* from[2];
-    long long stride[2];  // bytes
-    unsigned rows[2], columns;
+// ---- fp32 --------------------------------------------------------------------------------------------------
+
+struct Matrix32 {
+    const char* from;
+    long long stride;  // bytes
+    unsigned rows, columns;
     Divisor eights;  // of a row
 };
+// Eight elements; zeros behind the row.
+__device__ __forceinline__ void load_eight(const Matrix32& m, unsigned row, unsigned n, unsigned (&w)[8]) {
+    load_any<float, 8>(m.from + (long long)row * m.stride + (u64)n * 4u, n < m.columns ? min(8u, m.columns - n) : 0u, w);
+}
+// The largest magnitude, as a whole number, without infinities and NaN.
+__device__ __forceinline__ unsigned largest_of(const unsigned (&w)[8]) {
+    unsigned most = 0;
+#pragma unroll
+    for (unsigned e = 0; e < 8; ++e) {
+        const unsigned magnitude = w[e] & 0x7fffffffu;
+        most = max(most, magnitude < 0x7f800000u ? magnitude : 0u);
+    }
+    return most;
+}
+// Eight elements as two times eight fp16 numbers, `apart` sixteens of bytes from each other.
+__device__ __forceinline__ void store_split(char* out, u64 i, u64 apart, const unsigned (&words)[8], float scale) {
+    unsigned first[4], second[4];
+#pragma unroll
+    for (unsigned e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(words[2 * e]) * scale, y = __uint_as_float(words[2 * e + 1]) * scale;
+        first[e] = f2_to_h2(x, y);
+        const float2 f = h2_to_f2(first[e]);
+        // (Infinities and NaN have no rest.)
+        second[e] = f2_to_h2(fabsf(x) < 65536.0f ? x - f.x : 0.0f, fabsf(y) < 65536.0f ? y - f.y : 0.0f);
+    }
+    *(reinterpret_cast<uint4*>(out) + i) = make_uint4(first[0], first[1], first[2], first[3]);
+    *(reinterpret_cast<uint4*>(out) + apart + i) = make_uint4(second[0], second[1], second[2], second[3]);
+}
 
-constexpr unsigned kMagnitudeCtas = 256;  // for each of the two
+constexpr unsigned kMagnitudeCtas = 256;  // for the matrix
 
 struct MagnitudeArgs {
-    Pair32Matrices m;
-    unsigned* partial;  // [2][kMagnitudeCtas]
+    Matrix32 x, w;
+    unsigned* rows;     // of each row of x
+    unsigned* partial;  // of each CTA's part of w
 };
 
-// Their largest magnitudes, as whole numbers, without infinities and NaN: one of each CTA. A thread takes eight elements of a row at a time.
+// The largest magnitudes. A warp takes a row of x; a thread eight elements of w at a time.
 __global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ MagnitudeArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const unsigned which = blockIdx.x / kMagnitudeCtas, eights = a.m.rows[which] * a.m.eights.d;
-    unsigned most = 0;
+    unsigned most = 0, w[8];
+    if (blockIdx.x >= kMagnitudeCtas) {
+        const unsigned row = (blockIdx.x - kMagnitudeCtas) * 16u + threadIdx.x / 32u;
+        if (row >= a.x.rows) return;
 #pragma unroll 4
-    for (unsigned at = blockIdx.x % kMagnitudeCtas * 512u + threadIdx.x; at < eights; at += kMagnitudeCtas * 512u) {
-        const unsigned row = a.m.eights.divide(at), n = (at - row * a.m.eights.d) * 8u;
-        unsigned w[8];
-        load_any<float, 8>(a.m.from[which] + (long long)row * a.m.stride[which] + (u64)n * 4u, n < a.m.columns ? min(8u, a.m.columns - n) : 0u, w);
-#pragma unroll
-        for (unsigned e = 0; e < 8; ++e) {
-            const unsigned magnitude = w[e] & 0x7fffffffu;
-            most = max(most, magnitude < 0x7f800000u ? magnitude : 0u);
+        for (unsigned n = threadIdx.x % 32u * 8u; n < a.x.columns; n += 256u) {
+            load_eight(a.x, row, n, w);
+            most = max(most, largest_of(w));
         }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (threadIdx.x % 32u == 0) a.rows[row] = most;
+        return;
+    }
+    const unsigned eights = a.w.rows * a.w.eights.d;
+#pragma unroll 4
+    for (unsigned at = blockIdx.x * 512u + threadIdx.x; at < eights; at += kMagnitudeCtas * 512u) {
+        const unsigned row = a.w.eights.divide(at);
+        load_eight(a.w, row, (at - row * a.w.eights.d) * 8u, w);
+        most = max(most, largest_of(w));
     }
     most = __reduce_max_sync(0xffffffffu, most);
     __shared__ unsigned all[16];
@@ -1399,11 +1440,12 @@ __global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ 
 }
 
 struct SplitArgs {
-    Pair32Matrices m;
-    char* out[2];             // two fp16 matrices [2][rows][pitch] each, scaled
+    Matrix32 x, w;
+    char *x_out, *w_out;      // two fp16 matrices [2][rows][pitch] each, scaled
     unsigned ctas_of_x;
-    const unsigned* partial;  // of magnitude_kernel; null: the magnitudes are known
-    unsigned* magnitudes;
+    const unsigned* rows;     // of magnitude_kernel
+    const unsigned* partial;  // the same; null: that of w is known
+    unsigned* w_magnitude;
 };
 
 // A thread takes eight elements of a row.
@@ -1411,35 +1453,44 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Spli
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     static_assert(kMagnitudeCtas == 256);
-    const unsigned which = blockIdx.x >= a.ctas_of_x ? 1u : 0u, block = blockIdx.x - which * a.ctas_of_x;
-    const unsigned i = block * 256u + threadIdx.x, row = a.m.eights.divide(i), n = (i - row * a.m.eights.d) * 8u;
-    unsigned words[8], first[4], second[4];
-    const bool there = row < a.m.rows[which];
-    if (there) load_any<float, 8>(a.m.from[which] + (long long)row * a.m.stride[which] + (u64)n * 4u, n < a.m.columns ? min(8u, a.m.columns - n) : 0u, words);
-    unsigned magnitude;
-    if (a.partial != nullptr) {
+    const bool of_x = blockIdx.x < a.ctas_of_x;
+    const Matrix32& m = of_x ? a.x : a.w;
+    const unsigned block = of_x ? blockIdx.x : blockIdx.x - a.ctas_of_x, i = block * 256u + threadIdx.x, row = m.eights.divide(i);
+    const bool there = row < m.rows;
+    unsigned words[8], magnitude = 0;
+    if (there) load_eight(m, row, (i - row * m.eights.d) * 8u, words);
+    if (of_x) {
+        if (there) magnitude = a.rows[row];
+    } else if (a.partial != nullptr) {
         __shared__ unsigned all[8];
-        magnitude = __reduce_max_sync(0xffffffffu, a.partial[which * kMagnitudeCtas + threadIdx.x]);
+        magnitude = __reduce_max_sync(0xffffffffu, a.partial[threadIdx.x]);
         if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = magnitude;
         __syncthreads();
 #pragma unroll
         for (unsigned w = 0; w < 8; ++w) magnitude = max(magnitude, all[w]);
-        if (block == 0 && threadIdx.x == 0) a.magnitudes[which] = magnitude;
+        if (block == 0 && threadIdx.x == 0) *a.w_magnitude = magnitude;
     } else {
-        magnitude = a.magnitudes[which];
+        magnitude = *a.w_magnitude;
     }
-    if (!there) return;
-    const float scale = scale_of(magnitude, false);
-#pragma unroll
-    for (unsigned e = 0; e < 4; ++e) {
-        const float x = __uint_as_float(words[2 * e]) * scale, y = __uint_as_float(words[2 * e + 1]) * scale;
-        first[e] = f2_to_h2(x, y);
-        const float2 f = h2_to_f2(first[e]);
-        // (Infinities and NaN have no rest.)
-        second[e] = f2_to_h2(fabsf(x) < 65536.0f ? x - f.x : 0.0f, fabsf(y) < 65536.0f ? y - f.y : 0.0f);
-    }
-    *(reinterpret_cast<uint4*>(a.out[which]) + i) = make_uint4(first[0], first[1], first[2], first[3]);
-    *(reinterpret_cast<uint4*>(a.out[which]) + (u64)a.m.rows[which] * a.m.eights.d + i) = make_uint4(second[0], second[1], second[2], second[3]);
+    if (there) store_split(of_x ? a.x_out : a.w_out, i, (u64)m.rows * m.eights.d, words, scale_of(magnitude, false));
+}
+
+struct WeighArgs {
+    Matrix32 x;
+    char* out;  // [2][rows][pitch]
+    const float* valid;
+    const float* header;
+};
+
+// x as the gradient of w takes it: one power of two for all rows, zeros for those that do not count.
+__global__ void __launch_bounds__(256) weigh_kernel(const __grid_constant__ WeighArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned i = blockIdx.x * 256u + threadIdx.x, row = a.x.eights.divide(i);
+    if (row >= a.x.rows) return;
+    unsigned words[8] = {};
+    if (a.valid[row] != 0.0f) load_eight(a.x, row, (i - row * a.x.eights.d) * 8u, words);
+    store_split(a.out, i, (u64)a.x.rows * a.x.eights.d, words, 1.0f / a.header[2]);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
@@ -1555,7 +1606,7 @@ struct Plan {
     u64 rows = 0;                // both at once: of a piece
     std::size_t exps_pitch = 0;
     unsigned n_tile = kTile;
-    std::size_t scale_at = 0, divided_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
+    std::size_t scale_at = 0, divided_at = 0, weighed_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
 };
 
 // Both at once: bytes of E in a piece of the rows, and of the sums of dw where there are several. (8192 x 50257 x 768, loss and gradients: 1459 us in one piece of 824 MB, 1565 in two,
@@ -1609,7 +1660,7 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         p.stats_at = take((v + kTile - 1) / kTile * 2 * t * sizeof(float2));
         p.picked_at = take(t * std::max(c.entries, 1) * sizeof(float));
         p.losses_at = take(t * sizeof(float));
-        p.partial_at = take(c.dtype == DType::Float ? 2 * kMagnitudeCtas * sizeof(unsigned) : 0);
+        p.partial_at = take(c.dtype == DType::Float ? kMagnitudeCtas * sizeof(unsigned) : 0);
     } else if (pass == Pass::Both) {
         p.n_tile = n_tile_of(c.width);
         p.exps_pitch = (v + kTile - 1) / kTile * kTile;
@@ -1642,7 +1693,8 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         p.piece = (tiles + p.pieces - 1) / p.pieces * kTile;
         p.pieces = (v + p.piece - 1) / p.piece;
         p.n_tile = n_tile_of(c.width);
-        p.header_at = take(2 * sizeof(float));
+        p.header_at = take(3 * sizeof(float));
+        p.weighed_at = take(c.dtype == DType::Float && c.weight_grad != nullptr ? p.parts * t * p.pitch * 2 : 0);
         p.probs_at = take(bytes * p.piece);
         const u64 rest = v - (p.pieces - 1) * p.piece;
         if (c.x_grad != nullptr && p.pieces > 1)
@@ -1724,7 +1776,7 @@ void finish(const VocabularyLossCall& c, const Tiling& t, const ProductArgs& a) 
     f.last = a.last;
     f.header = a.header;
     f.row_scale = a.row_scale;
-    f.magnitudes = a.magnitudes;
+    f.w_magnitude = a.w_magnitude;
     f.m = a.m;
     f.n = a.n;
     f.m_tiles = t.m_tiles;
@@ -1742,7 +1794,7 @@ std::size_t hit_words(const VocabularyLossCall& c) { return (c.vocabulary + kHal
 
 struct Kept {
     float *top, *sum, *rest, *valid, *count, *probs;
-    unsigned* magnitudes;
+    unsigned *w_magnitude, *magnitudes;  // fp32: of the matrix, of each row of x
     int* words;  // of the teacher's entries, and their probabilities: [entries][tokens]
     unsigned* hits;
 };
@@ -1753,14 +1805,19 @@ Kept kept_of(const VocabularyLossCall& c) {
     k.rest = k.sum + c.tokens;
     k.valid = k.rest + c.tokens;
     k.count = k.valid + c.tokens;
-    k.magnitudes = reinterpret_cast<unsigned*>(k.count + 1);
-    k.probs = k.count + 3;
+    k.w_magnitude = reinterpret_cast<unsigned*>(k.count + 1);
+    k.probs = k.count + 2;
     k.words = reinterpret_cast<int*>(k.probs + c.tokens * (std::size_t)c.entries);
     k.hits = reinterpret_cast<unsigned*>(k.words + c.tokens * (std::size_t)c.entries);
+    k.magnitudes = k.hits + hit_words(c);
     return k;
 }
 
 constexpr const char* kTooLarge = "an operand is too large for one call";
+
+Matrix32 x_of(const VocabularyLossCall& c, const Plan& p) {
+    return {static_cast<const char*>(c.x), c.x_stride * 4, (unsigned)c.tokens, (unsigned)c.width, Divisor((unsigned)(p.pitch / 8))};
+}
 
 // x and the matrix as the tensor cores read them, copied where they have to be. known: fp32's magnitudes are, from the forward pass.
 template <typename T>
@@ -1779,23 +1836,24 @@ void operands(const VocabularyLossCall& c, const Plan& p, bool known, Operand* x
     } else {
         const u64 x_eights = (u64)c.tokens * (p.pitch / 8), w_eights = (u64)c.vocabulary * (p.pitch / 8);
         B2_REQUIRE(x_eights < (1ull << 30) && w_eights < (1ull << 30), kTooLarge);
-        const Pair32Matrices m = {{static_cast<const char*>(c.x), static_cast<const char*>(c.weight)}, {c.x_stride * 4, c.weight_stride * 4},
-                                  {(unsigned)c.tokens, (unsigned)c.vocabulary}, (unsigned)c.width, Divisor((unsigned)(p.pitch / 8))};
+        const Kept kept = kept_of(c);
         SplitArgs s;
-        s.m = m;
-        s.out[0] = workspace + p.x_at;
-        s.out[1] = workspace + p.weight_at;
+        s.x = x_of(c, p);
+        s.w = {static_cast<const char*>(c.weight), c.weight_stride * 4, (unsigned)c.vocabulary, (unsigned)c.width, Divisor((unsigned)(p.pitch / 8))};
+        s.x_out = workspace + p.x_at;
+        s.w_out = workspace + p.weight_at;
         s.ctas_of_x = (unsigned)((x_eights + 255) / 256);
+        s.rows = kept.magnitudes;
         s.partial = nullptr;
-        s.magnitudes = kept_of(c).magnitudes;
+        s.w_magnitude = kept.w_magnitude;
         if (!known) {
-            const MagnitudeArgs a = {m, reinterpret_cast<unsigned*>(workspace + p.partial_at)};
-            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel, dim3(2 * kMagnitudeCtas), 512, 0, c.stream, a));
+            const MagnitudeArgs a = {s.x, s.w, kept.magnitudes, reinterpret_cast<unsigned*>(workspace + p.partial_at)};
+            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel, dim3(kMagnitudeCtas + (unsigned)((c.tokens + 15) / 16)), 512, 0, c.stream, a));
             s.partial = a.partial;
         }
         B2_CUDA(launch_dependent<SplitArgs>(split_kernel, dim3(s.ctas_of_x + (unsigned)((w_eights + 255) / 256)), 256, 0, c.stream, s));
-        *x = {s.out[0], c.width, c.tokens, p.pitch * 2};
-        *w = {s.out[1], c.width, c.vocabulary, p.pitch * 2};
+        *x = {s.x_out, c.width, c.tokens, p.pitch * 2};
+        *w = {s.w_out, c.width, c.vocabulary, p.pitch * 2};
     }
 }
 
@@ -1804,6 +1862,7 @@ constexpr DType operand_type() { return std::is_same_v<T, __nv_bfloat16> ? DType
 
 void logits_arguments(const VocabularyLossCall& c, ProductArgs& a) {
     a.magnitudes = kept_of(c).magnitudes;
+    a.w_magnitude = kept_of(c).w_magnitude;
     const double factor = 1.4426950408889634 / (double)c.temperature;
     a.factor = (float)factor;
     a.factor_rest = (float)(factor - (double)a.factor);
@@ -1910,12 +1969,22 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
     h.loss_grad_stride = c.loss_grad_stride;
     h.valid = kept.valid;
     h.count = c.reduction == LossReduction::Mean ? kept.count : nullptr;
-    h.rows = each ? (unsigned)c.tokens : 0;
+    h.rows = (unsigned)c.tokens;
+    h.each = each;
+    h.magnitudes = sizeof(T) == 4 && c.weight_grad != nullptr ? kept.magnitudes : nullptr;
     h.temperature = c.temperature;
     h.header = header;
     B2_CUDA(launch_dependent<HeaderArgs>(header_kernel, dim3(1), 1024, 0, c.stream, h));
     Operand x, w;
     operands<T>(c, p, true, &x, &w);
+    Operand weighed = x;
+    if constexpr (sizeof(T) == 4) {
+        if (c.weight_grad != nullptr) {
+            weighed.data = workspace + p.weighed_at;
+            const WeighArgs e = {x_of(c, p), workspace + p.weighed_at, kept.valid, header};
+            B2_CUDA(launch_dependent<WeighArgs>(weigh_kernel, dim3((unsigned)((c.tokens * (p.pitch / 8) + 255) / 256)), 256, 0, c.stream, e));
+        }
+    }
     char* probs = workspace + p.probs_at;
     for (u64 piece = 0; piece < p.pieces; ++piece) {
         const u64 first = piece * p.piece, words = std::min<u64>(p.piece, c.vocabulary - first);
@@ -1945,7 +2014,7 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
         if (c.weight_grad != nullptr) {
             const Tiling t = tiling_of(words, c.width, c.tokens, p.grad_products, p.n_tile, true, p.device_pairs);
             a.a = map_of(operand_type<T>(), probs_of, p.prob_parts, 64, kStep);
-            a.b = map_of(operand_type<T>(), x, p.parts, 64, kStep);
+            a.b = map_of(operand_type<T>(), weighed, p.parts, 64, kStep);
             a.b_offset = 0;
             a.sums = nullptr;
             a.prior = false;
@@ -2133,7 +2202,9 @@ bool at_once(const VocabularyLossCall& c) {
 
 }  // namespace
 
-std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) { return c.tokens * 4 + 3 + 2 * c.tokens * (std::size_t)c.entries + hit_words(c); }
+std::size_t vocabulary_loss_kept(const VocabularyLossCall& c) {
+    return c.tokens * 4 + 2 + 2 * c.tokens * (std::size_t)c.entries + hit_words(c) + (c.dtype == DType::Float ? c.tokens : 0);
+}
 
 std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient) {
     return call.tokens == 0 ? 0 : plan_of(call, gradient ? Pass::Gradient : Pass::Loss).bytes;

@@ -1,12 +1,75 @@
 """Losses over a vocabulary: what one row is must not reach another's loss or gradient, and the ways that a call may take are each held to what that way may lose."""
+import ctypes
 
 import pytest
 import torch
 
 import plain_vocabulary as plain
+from test_gpu_linear8 import replaced
 from test_gpu_vocabulary_loss import DTYPES, cross_entropy, distillation, gen, inputs, made_with_the_loss, run, teacher
 
 pytestmark = pytest.mark.gpu
+
+
+def each_row_alone(out, x, w, targets, dloss, rows, logits=None, temperature=1.0):
+    """The loss and the gradient of x of some rows, each against the formula of that row alone: its bound knows nothing of the others."""
+    for t in rows:
+        part = slice(t, t + 1)
+        want = plain.losses(x[part], w, targets[part], None if logits is None else logits[part], temperature, "none", dloss[part])
+        for name in ("loss", "dx"):
+            plain.within(out[name][part], want[name], f"{name} of row {t}")
+
+
+# ---- float32: rows of very different sizes ---------------------------------------------------------------
+
+@pytest.mark.parametrize("size", [1e10, 1e30])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_what_a_padded_row_holds_does_not_matter(size, reduction):
+    x, w, t = inputs(100, 700, 72, torch.float32)
+    padded = t < 0
+    dloss = torch.rand(100, device="cuda", generator=gen(5)) + 0.5 if reduction == "none" else torch.tensor(0.75, device="cuda")
+    want = run(cross_entropy(t, reduction), torch.where(padded[:, None], 0.0, x), w, dloss)
+    got = run(cross_entropy(t, reduction), torch.where(padded[:, None], size, x), w, dloss)
+    assert all(torch.equal(got[name], want[name]) for name in want)
+    counted = ~padded
+    exact = plain.losses(x[counted], w, t[counted], reduction=reduction, dloss=dloss[counted] if reduction == "none" else dloss)
+    plain.within(got["loss"][counted] if reduction == "none" else got["loss"], exact["loss"], "loss")
+    plain.within(got["dx"][counted], exact["dx"], "dx")
+    plain.within(got["dw"], exact["dw"], "dw")
+    logits, tokens = teacher(100, 5, 700, torch.float32)
+    tokens[padded] = -1
+    call = distillation(logits, tokens, 2.0, reduction)
+    want, got = run(call, torch.where(padded[:, None], 0.0, x), w, dloss), run(call, torch.where(padded[:, None], size, x), w, dloss)
+    assert all(torch.equal(got[name], want[name]) for name in want)
+
+
+def test_rows_of_any_size_have_their_own_loss_and_gradient():
+    """Rows of 1e-12 to 1e10, some of zeros: the logits and the gradient of each lose what its own elements lose."""
+    rows = 60
+    x, w, t = inputs(rows, 700, 72, torch.float32)
+    t = t.clamp(min=0)
+    x = x * 10.0 ** torch.linspace(-12, 10, rows, device="cuda")[:, None]
+    x[7] = 0.0
+    dloss = torch.rand(rows, device="cuda", generator=gen(5)) + 0.5
+    out = run(cross_entropy(t, "none"), x, w, dloss)
+    each_row_alone(out, x, w, t, dloss, range(rows))
+    plain.within(out["dw"], plain.losses(x, w, t, reduction="none", dloss=dloss)["dw"], "dw")
+    logits, tokens = teacher(rows, 5, 700, torch.float32)
+    out = run(distillation(logits, tokens, 2.0, "none"), x, w, dloss)
+    each_row_alone(out, x, w, tokens, dloss, range(rows), logits, 2.0)
+
+
+def test_a_row_s_own_infinities_stay_its_own():
+    x, w, t = inputs(60, 300, 64, torch.float32)
+    t = t.clamp(min=0)
+    spoilt = x.clone()
+    spoilt[3, 5], spoilt[9, 0] = float("inf"), float("nan")
+    dloss = torch.ones(60, device="cuda")
+    got, want = run(cross_entropy(t, "none"), spoilt, w, dloss), run(cross_entropy(t, "none"), x, w, dloss)
+    others = torch.ones(60, dtype=torch.bool, device="cuda")
+    others[[3, 9]] = False
+    assert torch.equal(got["loss"][others], want["loss"][others]) and torch.equal(got["dx"][others], want["dx"][others])
+    assert not got["loss"][~others].isfinite().any() and not got["dx"][~others].isfinite().any()
 
 
 # ---- what comes back to rows that are weighted one by one ------------------------------------------------
@@ -70,3 +133,11 @@ def test_gradients_of_few_rows_made_with_the_loss():
         # Each other word's exponential is off by half a step, 2^-8, and its row's factor by as much; as independent numbers, of which the norm is the root of the sum of squares.
         spread = ((p ** 2) @ (m.double() ** 2)).sum().sqrt()
         assert (out[name].double() - exact).norm() <= 1.1 * rounded + 2.1 * 2.0 ** -8 * spread + 2.0 ** -8 * (p @ m.double()).norm(), name
+
+
+# ---- the model, large enough for gradients that are made with the loss -----------------------------------
+
+
+def counted(calls):
+    prototype = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
+    return replaced("b2_vocabulary_loss_both", prototype, lambda original, *arguments: calls.append(1) or original(*arguments))
