@@ -40,8 +40,8 @@ def linear_cross_entropy(x, weight, targets, reduction="mean"):
     one of all of them (a mean over the rows that have a target; 0 where none has). ``x``: [..., width], ``targets``: [...]. The loss is float32, gradients have the types of ``x``
     and ``weight``, which are the same. Under autocast both are cast as those of ``linear``.
 
-    What the logits lose is what 32-bit sums lose; the gradient of the logits is rounded to the type of ``x`` before it is multiplied. float32: operands have 22 bits, or 2^-39 of
-    the largest element of ``weight``, of the row of ``x`` (in the gradient of ``weight``: of the rows that count) and of the rows' weights in the loss, where that is more."""
+    What the logits lose is what 32-bit sums lose; the gradient of the logits is rounded to the type of ``x`` before it is multiplied. float32: operands have 22 bits, or where that is
+    more 2^-39 of the largest element of ``weight``, of the row of ``x`` (in the gradient of ``weight``: of the rows of ``x`` that count, times their weights in the loss), and of 1 in the softmax."""
     return load_native_calls().linear_cross_entropy(x, weight, targets, _reduction(reduction))
 
 

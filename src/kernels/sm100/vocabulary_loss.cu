@@ -24,7 +24,9 @@
 //
 // P is the operand of two products and therefore of their type: its rounding (2^-8 of each
 // element in bf16) is what the gradients lose beside their own. r_t = c_t / max |c| is 1 in a mean or a sum, so that the target's element
-// stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there.
+// stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there. Nor has it any for rows whose c is far below the largest: where
+// rows have weights of their own, fp16 and fp32 leave the power of two of c out of P. The gradient of x takes it at the end, that of w with x, which is laid out once more (777 x 32003 x 1003 in fp16: 311 -> 322 us,
+// 128 x 512 x 64 78 -> 84).
 //
 // fp32: x, w and P are sums of two fp16 matrices each, what fp16 makes of an element and what it makes of the rest, after a power of two that brings the largest
 // element to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
@@ -128,7 +130,7 @@ struct alignas(64) ProductArgs {
     long long loss_grad_stride;
     float temperature;
     // Gradients
-    float* header;         // of the workspace: max |c|, NaN once a product went wrong, and fp32: the power of two that brings x, as the gradient of w takes it, back
+    float* header;         // of the workspace: max |c|, NaN once a product went wrong, and fp16 and fp32: the power of two that brings x, as the gradient of w takes it, back
     void* gradient;        // rows of n elements
     const float* row_scale;  // [m], or null
     bool wide;             // TMA can write them
@@ -292,16 +294,23 @@ __device__ __forceinline__ float scale_of(unsigned magnitude, bool back) {
 template <Kind kKind, typename T>
 __device__ __forceinline__ float gradient_scale(const float* header, const unsigned* w_magnitude) {
     float scale = header[0] + header[1];
-    if constexpr (!std::is_same_v<T, __nv_bfloat16>) scale *= 1.0f / kHalfScale;
-    if constexpr (sizeof(T) == 4) scale *= kKind == Kind::WeightGrad ? header[2] : scale_of(*w_magnitude, true);
+    if constexpr (!std::is_same_v<T, __nv_bfloat16>) scale *= 1.0f / kHalfScale * (kKind == Kind::WeightGrad ? header[2] : 1.0f);
+    if constexpr (sizeof(T) == 4 && kKind != Kind::WeightGrad) scale *= scale_of(*w_magnitude, true);
     return scale;
 }
 
-// c_t / max |c|, of the c that are numbers; 0 of rows that do not count. An infinite c, or NaN, stays what it is, in its own row.
+// The power of two of a row's c, which fp16 and fp32 leave out of P: the largest that is not above it, 1 of an infinite c and NaN.
+__device__ __forceinline__ float power_of(float c) {
+    const unsigned exponent = __float_as_uint(c) & 0x7f800000u;
+    return exponent == 0x7f800000u ? 1.0f : __uint_as_float(max(exponent, 0x00800000u));
+}
+// c_t over that power, in bf16 over max |c| of those that are numbers; 0 of rows that do not count. An infinite c, or NaN, stays what it is, in its own row.
+template <bool kHalfType>
 __device__ __forceinline__ float row_weight(float valid, const float* loss_grad, long long stride, float temperature, float largest, unsigned row) {
     if (loss_grad == nullptr || valid == 0.0f) return valid;
     const float c = loss_grad[(long long)row * stride] * temperature;
     if (!(fabsf(c) < __int_as_float(0x7f800000))) return c * valid;
+    if (kHalfType) return c / power_of(c) * valid;
     return largest == 0.0f ? 0.0f * valid : c * valid / largest;
 }
 
@@ -516,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                     if constexpr (sizeof(T) == 4) back_x = both32(scale_of(a.magnitudes[row], true));
                     if constexpr (!kTeacher) target = target_at(a.targets, a.targets64, (long long)row * a.target_stride);
                     if constexpr (kKind == Kind::Probs) {
-                        weight = row_weight(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (kHalfType ? kHalfScale : 1.0f);
+                        weight = row_weight<kHalfType>(a.valid[row], a.loss_grad, a.loss_grad_stride, a.temperature, a.header[0], row) * (kHalfType ? kHalfScale : 1.0f);
                         row_top = a.top[row];
                         share_of_sum = weight / a.sum[row];
                         if constexpr (!kTeacher) of_target = -weight * a.rest[row];
@@ -1097,40 +1106,48 @@ struct HeaderArgs {
     const float* count;  // of a mean, or null
     unsigned rows;
     bool each;           // loss_grad has an element for each row
-    const unsigned* magnitudes;  // fp32: the largest of each row of x, or null
+    float* powers;       // of each row's c, or null
+    const unsigned* magnitudes;  // the largest of each row of x, where the gradient of w takes it apart; or null
     float temperature;
     float* header;
 };
 
-// max |c| of the rows, of those that are numbers; c itself where they share it. fp32: the power of two for x in the gradient of w, of the rows that count.
+// max |c| of the rows, of those that are numbers; c itself where they share it, 1 where P has no powers of two of theirs. The power of two for x in the gradient of w, of the rows that count.
 __global__ void __launch_bounds__(1024) header_kernel(const __grid_constant__ HeaderArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    unsigned most = 0, most_x = 0;  // (of magnitudes as whole numbers: infinity and NaN are above all others)
+    constexpr int kNone = -1000;
+    unsigned most = 0;       // (of magnitudes as whole numbers: infinity and NaN are above all others)
+    int exponent_x = kNone;  // of the largest element of x times its row's power
     if (a.each || a.magnitudes != nullptr) {
 #pragma unroll 4
         for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) {
-            const float valid = a.valid[i];
-            const unsigned bits = a.each ? __float_as_uint(a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature) & 0x7fffffffu : 0u;
-            most = max(most, valid == 0.0f || bits >= 0x7f800000u ? 0u : bits);
-            if (a.magnitudes != nullptr) most_x = max(most_x, valid == 0.0f ? 0u : a.magnitudes[i]);
+            const float c = a.each ? a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature : 1.0f, power = a.powers != nullptr ? power_of(c) : 1.0f;
+            const unsigned bits = __float_as_uint(c) & 0x7fffffffu;
+            const bool counts = a.valid[i] != 0.0f && bits < 0x7f800000u && bits != 0u;
+            most = max(most, counts ? bits : 0u);
+            if (a.powers != nullptr) a.powers[i] = power;
+            const unsigned x = a.magnitudes != nullptr ? a.magnitudes[i] : 0u;
+            if (counts && x != 0u) exponent_x = max(exponent_x, (int)(x >> 23) + (int)(__float_as_uint(power) >> 23) - 254);
         }
     }
-    __shared__ unsigned all[32], all_x[32];
+    __shared__ unsigned all[32];
+    __shared__ int all_x[32];
     most = __reduce_max_sync(0xffffffffu, most);
-    most_x = __reduce_max_sync(0xffffffffu, most_x);
+    exponent_x = __reduce_max_sync(0xffffffffu, exponent_x);
     if ((threadIdx.x & 31u) == 0) {
         all[threadIdx.x / 32u] = most;
-        all_x[threadIdx.x / 32u] = most_x;
+        all_x[threadIdx.x / 32u] = exponent_x;
     }
     __syncthreads();
     if (threadIdx.x >= 32u) return;
     most = __reduce_max_sync(0xffffffffu, all[threadIdx.x]);
-    most_x = __reduce_max_sync(0xffffffffu, all_x[threadIdx.x]);
+    exponent_x = __reduce_max_sync(0xffffffffu, all_x[threadIdx.x]);
     if (threadIdx.x == 0) {
-        a.header[0] = a.each ? __uint_as_float(most) : a.loss_grad[0] * a.temperature / (a.count != nullptr ? fmaxf(*a.count, 1.0f) : 1.0f);
+        if (!a.each) a.header[0] = a.loss_grad[0] * a.temperature / (a.count != nullptr ? fmaxf(*a.count, 1.0f) : 1.0f);
+        else a.header[0] = a.powers != nullptr ? 1.0f : __uint_as_float(most);
         a.header[1] = 0.0f;
-        a.header[2] = scale_of(most_x, true);
+        a.header[2] = exponent_x == kNone ? 1.0f : ldexpf(1.0f, min(max(exponent_x - 14, -126), 127));
     }
 }
 
@@ -1361,63 +1378,75 @@ __global__ void __launch_bounds__(512) times_kernel(const __grid_constant__ Scal
     }
 }
 
-// ---- fp32 --------------------------------------------------------------------------------------------------
+// ---- fp32, and fp16 where rows have weights of their own ------------------------------------------------------
 
-struct Matrix32 {
+struct Matrix {
     const char* from;
     long long stride;  // bytes
     unsigned rows, columns;
     Divisor eights;  // of a row
 };
 // Eight elements; zeros behind the row.
-__device__ __forceinline__ void load_eight(const Matrix32& m, unsigned row, unsigned n, unsigned (&w)[8]) {
-    load_any<float, 8>(m.from + (long long)row * m.stride + (u64)n * 4u, n < m.columns ? min(8u, m.columns - n) : 0u, w);
+template <typename T>
+__device__ __forceinline__ void load_eight(const Matrix& m, unsigned row, unsigned n, float (&f)[8]) {
+    unsigned w[2 * sizeof(T)];
+    load_any<T, 8>(m.from + (long long)row * m.stride + (u64)n * sizeof(T), n < m.columns ? min(8u, m.columns - n) : 0u, w);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (unsigned e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
+    } else {
+        Wide<T>::unpack(make_uint4(w[0], w[1], w[2], w[3]), f);
+    }
 }
 // The largest magnitude, as a whole number, without infinities and NaN.
-__device__ __forceinline__ unsigned largest_of(const unsigned (&w)[8]) {
+__device__ __forceinline__ unsigned largest_of(const float (&f)[8]) {
     unsigned most = 0;
 #pragma unroll
     for (unsigned e = 0; e < 8; ++e) {
-        const unsigned magnitude = w[e] & 0x7fffffffu;
+        const unsigned magnitude = __float_as_uint(f[e]) & 0x7fffffffu;
         most = max(most, magnitude < 0x7f800000u ? magnitude : 0u);
     }
     return most;
 }
-// Eight elements as two times eight fp16 numbers, `apart` sixteens of bytes from each other.
-__device__ __forceinline__ void store_split(char* out, u64 i, u64 apart, const unsigned (&words)[8], float scale) {
+// Eight elements as fp16 numbers; fp32: as two times eight, `apart` sixteens of bytes from each other.
+template <typename T>
+__device__ __forceinline__ void store_split(char* out, u64 i, u64 apart, const float (&f)[8], float scale) {
     unsigned first[4], second[4];
 #pragma unroll
     for (unsigned e = 0; e < 4; ++e) {
-        const float x = __uint_as_float(words[2 * e]) * scale, y = __uint_as_float(words[2 * e + 1]) * scale;
+        const float x = f[2 * e] * scale, y = f[2 * e + 1] * scale;
         first[e] = f2_to_h2(x, y);
-        const float2 f = h2_to_f2(first[e]);
+        const float2 rounded = h2_to_f2(first[e]);
         // (Infinities and NaN have no rest.)
-        second[e] = f2_to_h2(fabsf(x) < 65536.0f ? x - f.x : 0.0f, fabsf(y) < 65536.0f ? y - f.y : 0.0f);
+        second[e] = f2_to_h2(fabsf(x) < 65536.0f ? x - rounded.x : 0.0f, fabsf(y) < 65536.0f ? y - rounded.y : 0.0f);
     }
     *(reinterpret_cast<uint4*>(out) + i) = make_uint4(first[0], first[1], first[2], first[3]);
-    *(reinterpret_cast<uint4*>(out) + apart + i) = make_uint4(second[0], second[1], second[2], second[3]);
+    if constexpr (sizeof(T) == 4) *(reinterpret_cast<uint4*>(out) + apart + i) = make_uint4(second[0], second[1], second[2], second[3]);
 }
 
 constexpr unsigned kMagnitudeCtas = 256;  // for the matrix
 
 struct MagnitudeArgs {
-    Matrix32 x, w;
+    Matrix x, w;
     unsigned* rows;     // of each row of x
     unsigned* partial;  // of each CTA's part of w
+    unsigned ctas_of_w;
 };
 
 // The largest magnitudes. A warp takes a row of x; a thread eight elements of w at a time.
+template <typename T>
 __global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ MagnitudeArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    unsigned most = 0, w[8];
-    if (blockIdx.x >= kMagnitudeCtas) {
-        const unsigned row = (blockIdx.x - kMagnitudeCtas) * 16u + threadIdx.x / 32u;
+    unsigned most = 0;
+    float f[8];
+    if (blockIdx.x >= a.ctas_of_w) {
+        const unsigned row = (blockIdx.x - a.ctas_of_w) * 16u + threadIdx.x / 32u;
         if (row >= a.x.rows) return;
 #pragma unroll 4
         for (unsigned n = threadIdx.x % 32u * 8u; n < a.x.columns; n += 256u) {
-            load_eight(a.x, row, n, w);
-            most = max(most, largest_of(w));
+            load_eight<T>(a.x, row, n, f);
+            most = max(most, largest_of(f));
         }
         most = __reduce_max_sync(0xffffffffu, most);
         if (threadIdx.x % 32u == 0) a.rows[row] = most;
@@ -1427,8 +1456,8 @@ __global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ 
 #pragma unroll 4
     for (unsigned at = blockIdx.x * 512u + threadIdx.x; at < eights; at += kMagnitudeCtas * 512u) {
         const unsigned row = a.w.eights.divide(at);
-        load_eight(a.w, row, (at - row * a.w.eights.d) * 8u, w);
-        most = max(most, largest_of(w));
+        load_eight<T>(a.w, row, (at - row * a.w.eights.d) * 8u, f);
+        most = max(most, largest_of(f));
     }
     most = __reduce_max_sync(0xffffffffu, most);
     __shared__ unsigned all[16];
@@ -1440,7 +1469,7 @@ __global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ 
 }
 
 struct SplitArgs {
-    Matrix32 x, w;
+    Matrix x, w;
     char *x_out, *w_out;      // two fp16 matrices [2][rows][pitch] each, scaled
     unsigned ctas_of_x;
     const unsigned* rows;     // of magnitude_kernel
@@ -1448,17 +1477,18 @@ struct SplitArgs {
     unsigned* w_magnitude;
 };
 
-// A thread takes eight elements of a row.
+// fp32. A thread takes eight elements of a row.
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ SplitArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     static_assert(kMagnitudeCtas == 256);
     const bool of_x = blockIdx.x < a.ctas_of_x;
-    const Matrix32& m = of_x ? a.x : a.w;
+    const Matrix& m = of_x ? a.x : a.w;
     const unsigned block = of_x ? blockIdx.x : blockIdx.x - a.ctas_of_x, i = block * 256u + threadIdx.x, row = m.eights.divide(i);
     const bool there = row < m.rows;
-    unsigned words[8], magnitude = 0;
-    if (there) load_eight(m, row, (i - row * m.eights.d) * 8u, words);
+    float f[8] = {};
+    unsigned magnitude = 0;
+    if (there) load_eight<float>(m, row, (i - row * m.eights.d) * 8u, f);
     if (of_x) {
         if (there) magnitude = a.rows[row];
     } else if (a.partial != nullptr) {
@@ -1472,25 +1502,29 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Spli
     } else {
         magnitude = *a.w_magnitude;
     }
-    if (there) store_split(of_x ? a.x_out : a.w_out, i, (u64)m.rows * m.eights.d, words, scale_of(magnitude, false));
+    if (there) store_split<float>(of_x ? a.x_out : a.w_out, i, (u64)m.rows * m.eights.d, f, scale_of(magnitude, false));
 }
 
 struct WeighArgs {
-    Matrix32 x;
-    char* out;  // [2][rows][pitch]
+    Matrix x;
+    char* out;  // [parts][rows][pitch]
     const float* valid;
+    const float* powers;  // of each row, or null
     const float* header;
 };
 
-// x as the gradient of w takes it: one power of two for all rows, zeros for those that do not count.
+// x as the gradient of w takes it: times the power of two of each row's c and one for all rows, zeros for rows that do not count.
+template <typename T>
 __global__ void __launch_bounds__(256) weigh_kernel(const __grid_constant__ WeighArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned i = blockIdx.x * 256u + threadIdx.x, row = a.x.eights.divide(i);
     if (row >= a.x.rows) return;
-    unsigned words[8] = {};
-    if (a.valid[row] != 0.0f) load_eight(a.x, row, (i - row * a.x.eights.d) * 8u, words);
-    store_split(a.out, i, (u64)a.x.rows * a.x.eights.d, words, 1.0f / a.header[2]);
+    float f[8] = {};
+    if (a.valid[row] != 0.0f) load_eight<T>(a.x, row, (i - row * a.x.eights.d) * 8u, f);
+    // (Powers may be further apart than floats reach: a row whose largest element is below 2^-112 stays smaller, and what is 2^-149 of another's is nothing beside it.)
+    const int power = a.powers != nullptr ? (int)(__float_as_uint(a.powers[row]) >> 23) : 127, back = ilogbf(a.header[2]);
+    store_split<T>(a.out, i, (u64)a.x.rows * a.x.eights.d, f, ldexpf(1.0f, min(power - 127 - back, 126)));
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
@@ -1606,7 +1640,7 @@ struct Plan {
     u64 rows = 0;                // both at once: of a piece
     std::size_t exps_pitch = 0;
     unsigned n_tile = kTile;
-    std::size_t scale_at = 0, divided_at = 0, weighed_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
+    std::size_t scale_at = 0, divided_at = 0, weighed_at = 0, powers_at = 0, magnitudes_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
 };
 
 // Both at once: bytes of E in a piece of the rows, and of the sums of dw where there are several. (8192 x 50257 x 768, loss and gradients: 1459 us in one piece of 824 MB, 1565 in two,
@@ -1634,6 +1668,10 @@ bool small(const VocabularyLossCall& c) { return std::max<std::size_t>(c.tokens,
 // norm 1.4e-3 -> 2.0e-4, most of it is of the targets; 64 x 131072 x 4096 644 -> 680 us, 16 x 50257 x 768 103 -> 101.)
 constexpr u64 kFewRows = 64;
 bool fine(const VocabularyLossCall& c) { return c.tokens <= kFewRows || (small(c) && std::max<std::size_t>(c.tokens, kTile) * c.vocabulary <= (1ull << 25)); }
+
+// Whether P is without the powers of two of the rows' weights, and whether the gradient of w has its own x.
+bool powers_apart(const VocabularyLossCall& c) { return c.dtype != DType::BFloat16 && c.reduction == LossReduction::None; }
+bool weighed(const VocabularyLossCall& c) { return c.weight_grad != nullptr && (c.dtype == DType::Float || powers_apart(c)); }
 
 Plan plan_of(const VocabularyLossCall& c, Pass pass) {
     Plan p;
@@ -1694,7 +1732,9 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         p.pieces = (v + p.piece - 1) / p.piece;
         p.n_tile = n_tile_of(c.width);
         p.header_at = take(3 * sizeof(float));
-        p.weighed_at = take(c.dtype == DType::Float && c.weight_grad != nullptr ? p.parts * t * p.pitch * 2 : 0);
+        p.weighed_at = take(weighed(c) ? p.parts * t * p.pitch * 2 : 0);
+        p.powers_at = take(powers_apart(c) ? t * sizeof(float) : 0);
+        p.magnitudes_at = take(weighed(c) && c.dtype == DType::Float16 ? t * sizeof(unsigned) : 0);
         p.probs_at = take(bytes * p.piece);
         const u64 rest = v - (p.pieces - 1) * p.piece;
         if (c.x_grad != nullptr && p.pieces > 1)
@@ -1815,9 +1855,10 @@ Kept kept_of(const VocabularyLossCall& c) {
 
 constexpr const char* kTooLarge = "an operand is too large for one call";
 
-Matrix32 x_of(const VocabularyLossCall& c, const Plan& p) {
-    return {static_cast<const char*>(c.x), c.x_stride * 4, (unsigned)c.tokens, (unsigned)c.width, Divisor((unsigned)(p.pitch / 8))};
+Matrix x_of(const VocabularyLossCall& c, const Plan& p) {
+    return {static_cast<const char*>(c.x), c.x_stride * (long long)dtype_size(c.dtype), (unsigned)c.tokens, (unsigned)c.width, Divisor((unsigned)(p.pitch / 8))};
 }
+unsigned magnitude_ctas(const VocabularyLossCall& c) { return (unsigned)((c.tokens + 15) / 16); }
 
 // x and the matrix as the tensor cores read them, copied where they have to be. known: fp32's magnitudes are, from the forward pass.
 template <typename T>
@@ -1847,8 +1888,8 @@ void operands(const VocabularyLossCall& c, const Plan& p, bool known, Operand* x
         s.partial = nullptr;
         s.w_magnitude = kept.w_magnitude;
         if (!known) {
-            const MagnitudeArgs a = {s.x, s.w, kept.magnitudes, reinterpret_cast<unsigned*>(workspace + p.partial_at)};
-            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel, dim3(kMagnitudeCtas + (unsigned)((c.tokens + 15) / 16)), 512, 0, c.stream, a));
+            const MagnitudeArgs a = {s.x, s.w, kept.magnitudes, reinterpret_cast<unsigned*>(workspace + p.partial_at), kMagnitudeCtas};
+            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel<float>, dim3(kMagnitudeCtas + magnitude_ctas(c)), 512, 0, c.stream, a));
             s.partial = a.partial;
         }
         B2_CUDA(launch_dependent<SplitArgs>(split_kernel, dim3(s.ctas_of_x + (unsigned)((w_eights + 255) / 256)), 256, 0, c.stream, s));
@@ -1962,8 +2003,17 @@ template <typename T>
 void gradient(const VocabularyLossCall& c, const Plan& p) {
     char* workspace = static_cast<char*>(c.workspace);
     const Kept kept = kept_of(c);
-    const bool each = c.reduction == LossReduction::None;
+    const bool each = c.reduction == LossReduction::None, apart = !std::is_same_v<T, __nv_bfloat16> && weighed(c);
     float* header = reinterpret_cast<float*>(workspace + p.header_at);
+    float* powers = powers_apart(c) ? reinterpret_cast<float*>(workspace + p.powers_at) : nullptr;
+    const unsigned* magnitudes = apart ? kept.magnitudes : nullptr;
+    if constexpr (std::is_same_v<T, __half>) {
+        if (apart) {
+            unsigned* rows = reinterpret_cast<unsigned*>(workspace + p.magnitudes_at);
+            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel<T>, dim3(magnitude_ctas(c)), 512, 0, c.stream, MagnitudeArgs{x_of(c, p), {}, rows, nullptr, 0}));
+            magnitudes = rows;
+        }
+    }
     HeaderArgs h;
     h.loss_grad = c.loss_grad;
     h.loss_grad_stride = c.loss_grad_stride;
@@ -1971,18 +2021,21 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
     h.count = c.reduction == LossReduction::Mean ? kept.count : nullptr;
     h.rows = (unsigned)c.tokens;
     h.each = each;
-    h.magnitudes = sizeof(T) == 4 && c.weight_grad != nullptr ? kept.magnitudes : nullptr;
+    h.powers = powers;
+    h.magnitudes = magnitudes;
     h.temperature = c.temperature;
     h.header = header;
     B2_CUDA(launch_dependent<HeaderArgs>(header_kernel, dim3(1), 1024, 0, c.stream, h));
     Operand x, w;
     operands<T>(c, p, true, &x, &w);
-    Operand weighed = x;
-    if constexpr (sizeof(T) == 4) {
-        if (c.weight_grad != nullptr) {
-            weighed.data = workspace + p.weighed_at;
-            const WeighArgs e = {x_of(c, p), workspace + p.weighed_at, kept.valid, header};
-            B2_CUDA(launch_dependent<WeighArgs>(weigh_kernel, dim3((unsigned)((c.tokens * (p.pitch / 8) + 255) / 256)), 256, 0, c.stream, e));
+    Operand weighed_x = x;
+    if constexpr (!std::is_same_v<T, __nv_bfloat16>) {
+        if (apart) {
+            const WeighArgs e = {x_of(c, p), workspace + p.weighed_at, kept.valid, powers, header};
+            const u64 eights = (u64)c.tokens * (p.pitch / 8);
+            B2_REQUIRE(eights < (1ull << 31), kTooLarge);
+            B2_CUDA(launch_dependent<WeighArgs>(weigh_kernel<T>, dim3((unsigned)((eights + 255) / 256)), 256, 0, c.stream, e));
+            weighed_x = {e.out, c.width, c.tokens, p.pitch * 2};
         }
     }
     char* probs = workspace + p.probs_at;
@@ -2014,7 +2067,7 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
         if (c.weight_grad != nullptr) {
             const Tiling t = tiling_of(words, c.width, c.tokens, p.grad_products, p.n_tile, true, p.device_pairs);
             a.a = map_of(operand_type<T>(), probs_of, p.prob_parts, 64, kStep);
-            a.b = map_of(operand_type<T>(), weighed, p.parts, 64, kStep);
+            a.b = map_of(operand_type<T>(), weighed_x, p.parts, 64, kStep);
             a.b_offset = 0;
             a.sums = nullptr;
             a.prior = false;
@@ -2031,6 +2084,7 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
             a.sums = p.pieces > 1 ? reinterpret_cast<float*>(workspace + p.sums_at) : nullptr;
             a.prior = piece != 0;
             a.last = piece + 1 == p.pieces;
+            a.row_scale = powers;
             gradient_of(c.x_grad, c.tokens);
             launch_product(Kind::InputGrad, c, t, a, c.tokens, c.width);
             finish<Kind::InputGrad, T>(c, t, a);

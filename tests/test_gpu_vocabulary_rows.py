@@ -96,6 +96,40 @@ def test_a_weight_that_is_no_number_stays_in_its_row(dtype, frozen):
             assert not got[1].isfinite().any() and want[1].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype,least", [(torch.float32, -30), (torch.float32, -12), (torch.float16, -5), (torch.bfloat16, -30)])
+def test_a_row_s_gradient_does_not_depend_on_the_weights_of_others(dtype, least):
+    """Weights over many powers of ten: each row's gradient loses what it would lose alone."""
+    rows = 60
+    x, w, t = inputs(rows, 3000, 72, dtype)
+    t = t.clamp(min=0)
+    dloss = 10.0 ** torch.linspace(least, 0, rows, device="cuda") * torch.where(torch.arange(rows, device="cuda") % 3 == 0, -1.0, 1.0)
+    if dtype == torch.float16:
+        dloss = dloss * 1024  # (what a loss scaler leaves room for: gradients that the type can hold)
+    for targets, logits, call in ((t, None, cross_entropy(t, "none")), (*reversed(teacher(rows, 5, 3000, dtype)), None)):
+        if call is None:
+            call = distillation(logits, targets, 2.0, "none")
+        out = run(call, x, w, dloss)
+        each_row_alone(out, x, w, targets, dloss, range(rows), logits, 1.0 if logits is None else 2.0)
+        want = plain.losses(x, w, targets, logits, 1.0 if logits is None else 2.0, "none", dloss)
+        plain.within(out["dw"], want["dw"], "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weights_at_the_ends_of_their_range(dtype):
+    """The largest and the smallest numbers that there are, and a matrix that is frozen or not."""
+    x, w, t = inputs(40, 300, 64, dtype)
+    t = t.clamp(min=0)
+    dloss = torch.full((40,), 1e-44, device="cuda")
+    dloss[3], dloss[4] = 1e-38, 0.0
+    if dtype != torch.float16:
+        dloss[5], dloss[6] = 2.9e38, -1.8e38
+        x[5:7], w = x[5:7] * 0.01, w * 0.01
+    out = run(cross_entropy(t, "none"), x, w, dloss)
+    assert out["dx"].isfinite().all() and out["dw"].isfinite().all() and not out["dx"][4].any()
+    if dtype != torch.float16:
+        each_row_alone(out, x, w, t, dloss, (5, 6))
+
+
 # ---- which way a call takes, and what it may lose there --------------------------------------------------
 
 def loses_its_own_rounding(out, want, dtype, what=""):
