@@ -72,8 +72,8 @@ int b2_vocabulary_loss_backward(const b2_vocabulary_loss* call, void* stream);
 int b2_vocabulary_loss_both_workspace(const b2_vocabulary_loss* call, size_t* bytes);
 int b2_vocabulary_loss_both(const b2_vocabulary_loss* call, void* stream);
 int b2_vocabulary_loss_times(const b2_vocabulary_loss* call, void* stream);
-/* Every wait inside the kernels is bounded, by two seconds or `wait_ns`. Where one runs out, what depends on it is NaN, and the check below says so
- * once: 1, for calls on `device` that are done. */
+/* Every wait inside the kernels is bounded, by two seconds or `wait_ns`. Where one runs out, what depends on it is NaN (of gradients made with the loss, what
+ * a wait for their first logits left out is made again, and may be right), and the check below says once that a wait ran out: 1, for calls on `device` that are done. */
 int b2_vocabulary_loss_within(const b2_vocabulary_loss* call, int backward, unsigned long long wait_ns, void* stream); /* backward: 2 for both at once */
 int b2_vocabulary_loss_check_async_error(int device);
 

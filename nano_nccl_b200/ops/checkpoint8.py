@@ -91,7 +91,8 @@ def linear8(x, weight, bias=None):
 
 def check_async_error(device=None):
     """Raises B200CclError if a bounded wait inside a weight gradient, or a loss over a vocabulary or its gradients (:mod:`.vocabulary`), on ``device`` (default: the
-    current one) ran out since this was last called. Such results are NaN, so a loss scaler sees them too. Synchronize first: only calls that are done are known."""
+    current one) ran out since this was last called. Such results are NaN, so a loss scaler
+    sees them too (gradients made with a loss may have been made again, and be right). Synchronize first: only calls that are done are known."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index if not isinstance(device, int) else device
     index = torch.cuda.current_device() if index is None else index
     codes = []

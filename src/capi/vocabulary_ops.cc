@@ -182,7 +182,7 @@ int b2_vocabulary_loss_within(const b2_vocabulary_loss* call, int backward, unsi
 int b2_vocabulary_loss_check_async_error(int device) {
     return guarded("vocabulary_loss", [&] {
         if (kernels::waits_failed(kernels::WaitsOf::VocabularyLoss, device))
-            throw std::runtime_error("a wait inside a call on device " + std::to_string(device) + " ran out; what depends on it is NaN");
+            throw std::runtime_error("a wait inside a call on device " + std::to_string(device) + " ran out; what depends on it is NaN, unless it was made again");
     });
 }
 

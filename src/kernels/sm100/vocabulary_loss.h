@@ -45,7 +45,7 @@ struct VocabularyLossCall {
 
 std::size_t vocabulary_loss_kept(const VocabularyLossCall& call);
 std::size_t vocabulary_loss_workspace(const VocabularyLossCall& call, bool gradient);
-// Both throw std::runtime_error on a failed launch. Where a wait inside a kernel runs out, what depends on it is NaN.
+// Both throw std::runtime_error on a failed launch. Where a wait inside a kernel runs out, what depends on it is NaN, or made again.
 void launch_vocabulary_loss(const VocabularyLossCall& call);
 void launch_vocabulary_loss_gradient(const VocabularyLossCall& call);
 // The loss together with the gradients that are wanted, for a loss_grad of 1: bf16, one loss for all rows. Its workspace; 0 where that is not so, or would take too much of it.

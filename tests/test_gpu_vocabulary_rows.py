@@ -4,7 +4,10 @@ import ctypes
 import pytest
 import torch
 
+import nano_nccl_b200 as nn
 import plain_vocabulary as plain
+from nano_nccl_b200 import ops
+from test_cpu_vocabulary_ops import LL, VocabularyLoss
 from test_gpu_linear8 import replaced
 from test_gpu_vocabulary_loss import DTYPES, cross_entropy, distillation, gen, inputs, made_with_the_loss, run, teacher
 
@@ -167,6 +170,53 @@ def test_gradients_of_few_rows_made_with_the_loss():
         # Each other word's exponential is off by half a step, 2^-8, and its row's factor by as much; as independent numbers, of which the norm is the root of the sum of squares.
         spread = ((p ** 2) @ (m.double() ** 2)).sum().sqrt()
         assert (out[name].double() - exact).norm() <= 1.1 * rounded + 2.1 * 2.0 ** -8 * spread + 2.0 ** -8 * (p @ m.double()).norm(), name
+
+
+# ---- waits of gradients made with the loss ---------------------------------------------------------------
+
+def both(x, w, t, wait_ns):
+    """The C interface: the mean loss with its gradients, with waits of `wait_ns`."""
+    lib, rows = nn.load(), x.shape[0]
+    loss, dx, dw = torch.zeros((), device="cuda"), torch.zeros_like(x), torch.zeros_like(w)
+    c = VocabularyLoss(dtype=2, x=x.data_ptr(), x_stride=x.stride(0), weight=w.data_ptr(), weight_stride=w.stride(0), tokens=rows, width=x.shape[1], vocabulary=w.shape[0], targets=t.data_ptr(),
+                       target_bytes=8, target_strides=(LL * 2)(1, 1), temperature=1.0, reduction=1, loss=loss.data_ptr(), x_grad=dx.data_ptr(), weight_grad=dw.data_ptr())
+    floats, size = ctypes.c_size_t(), ctypes.c_size_t()
+    assert lib.b2_vocabulary_loss_sizes(ctypes.byref(c), 0, ctypes.byref(floats), None) == 0
+    assert lib.b2_vocabulary_loss_both_workspace(ctypes.byref(c), ctypes.byref(size)) == 0 and size.value != 0
+    kept, workspace = torch.zeros(floats.value, device="cuda"), torch.zeros(size.value, dtype=torch.uint8, device="cuda")
+    c.kept, c.workspace = kept.data_ptr(), workspace.data_ptr()
+    assert lib.b2_vocabulary_loss_within(ctypes.byref(c), 2, ctypes.c_ulonglong(wait_ns), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    torch.cuda.synchronize()
+    return {"loss": loss, "dx": dx, "dw": dw}
+
+
+def test_a_wait_of_gradients_made_with_the_loss_that_runs_out():
+    """Without any time a wait may be over or not when it is looked at. Results are right or NaN; where the logits were not done in time they are made again, and may be right then; the status says that a wait
+    ran out whenever anything is NaN."""
+    x, w, t = inputs(4096, 1024, 32768, torch.bfloat16)
+    ops.check_async_error()
+    want = plain.losses(x, w, t, dloss=torch.ones((), device="cuda"))
+    for name, value in both(x, w, t, 2 * 10 ** 9).items():
+        plain.within(value, want[name], name)
+    ops.check_async_error()
+    ran_out = 0
+    for _ in range(40):
+        got = both(x, w, t, 0)
+        nan = False
+        for name, (value, bound) in want.items():
+            there = ~got[name].isnan()
+            assert ((got[name].double() - value).abs() <= bound)[there].all(), name
+            nan |= not bool(there.all())
+        try:
+            ops.check_async_error()
+            assert not nan
+        except nn.B200CclError as e:
+            assert "ran out" in str(e)
+            ran_out += 1
+    assert ran_out > 0
+    for name, value in both(x, w, t, 2 * 10 ** 9).items():
+        plain.within(value, want[name], name)
+    ops.check_async_error()
 
 
 # ---- the model, large enough for gradients that are made with the loss -----------------------------------
