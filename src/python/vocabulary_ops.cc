@@ -176,21 +176,20 @@ Lost loss_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tenso
     p.c.loss = static_cast<float*>(r.loss.data_ptr());
     p.c.kept = static_cast<float*>(r.kept.data_ptr());
     if ((x_wanted || weight_wanted) && x.scalar_type() == at::kBFloat16 && asked.reduction != 0) {
-        if (x_wanted) r.x_grad = new_like(x);
-        if (weight_wanted) r.weight_grad = new_like(weight);
-        p.c.x_grad = x_wanted ? r.x_grad.data_ptr() : nullptr;
-        p.c.weight_grad = weight_wanted ? r.weight_grad.data_ptr() : nullptr;
+        // (The size depends on which of them there are, and not on where: they are allocated if they are made.)
+        p.c.x_grad = x_wanted ? p.x.t.data_ptr() : nullptr;
+        p.c.weight_grad = weight_wanted ? p.weight.t.data_ptr() : nullptr;
         call([&] { return g.both_workspace(&p.c, &both); });
+        if (both != 0 && x_wanted) r.x_grad = new_like(x);
+        if (both != 0 && weight_wanted) r.weight_grad = new_like(weight);
+        p.c.x_grad = r.x_grad.defined() ? r.x_grad.data_ptr() : nullptr;
+        p.c.weight_grad = r.weight_grad.defined() ? r.weight_grad.data_ptr() : nullptr;
     }
     at::Tensor workspace = new_bytes(x, static_cast<std::int64_t>(both != 0 ? both : bytes));
     p.c.workspace = workspace.data_ptr();
     void* stream = stream_of(x);
-    if (both != 0) {
-        call([&] { return g.both(&p.c, stream); });
-    } else {
-        r.x_grad = r.weight_grad = at::Tensor();
-        call([&] { return g.loss_forward(&p.c, stream); });
-    }
+    if (both != 0) call([&] { return g.both(&p.c, stream); });
+    else call([&] { return g.loss_forward(&p.c, stream); });
     return r;
 }
 

@@ -219,6 +219,22 @@ def test_a_wait_of_gradients_made_with_the_loss_that_runs_out():
     ops.check_async_error()
 
 
+# ---- memory ----------------------------------------------------------------------------------------------
+
+def test_a_loss_that_makes_no_gradients_allocates_none():
+    """A small product's gradients are made in the backward pass: nothing of their size is asked for before."""
+    x, w, t = inputs(16, 30000, 1024, torch.bfloat16)
+    assert not made_with_the_loss(x, w, t)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    ops.linear_cross_entropy(x, w, t)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    loss = ops.linear_cross_entropy(x, w, t)
+    assert torch.cuda.max_memory_allocated() - before < w.numel() * 2 / 4
+    assert loss.isfinite()
+
+
 # ---- the model, large enough for gradients that are made with the loss -----------------------------------
 
 
