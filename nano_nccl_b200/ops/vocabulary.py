@@ -10,7 +10,8 @@ make the gradients. It needs 512 MB at most for that, or 4096 words of the vocab
 
 bfloat16, with one loss for all rows and a product large enough: the logits are made once. A call whose inputs want gradients makes them with the loss, by pieces of the rows (1 GB of workspace,
 and as much again at most for sums where there are several), and keeps them; the backward pass multiplies them by what comes back, which rounds once more unless that is a power of two.
-Asked for a second time (``retain_graph``) they are made from the logits.
+Asked for a second time (``retain_graph``) they are made from the logits. A loss whose gradient nobody will ask for is cheaper under
+``torch.no_grad()``; one of each row, added up by the caller, takes less memory, and makes its logits twice.
 
 CUDA tensors of float32, float16 or bfloat16; calls run on the current stream of the tensors' device. As with the other operators of this package (:mod:`.checkpoint8`)
 reverse-mode gradients are made once, and tracing, forward mode and ``torch.func`` are refused; a step captured into a CUDA graph is captured with

@@ -1707,6 +1707,7 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         p.pieces = (t + p.rows - 1) / p.rows;
         p.rows = std::min<u64>(t, ((t + p.pieces - 1) / p.pieces + kTile - 1) / kTile * kTile);
         p.pieces = (t + p.rows - 1) / p.rows;
+        if (p.rows * p.exps_pitch * 2 > kExpsBytes) return Plan();  // (a tile's rows alone, over more than two million words)
         p.stats_at = take(p.exps_pitch / kTile * 2 * p.rows * sizeof(float2));
         p.picked_at = take(t * std::max(c.entries, 1) * sizeof(float));
         p.losses_at = take(t * sizeof(float));

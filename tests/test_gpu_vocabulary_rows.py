@@ -9,7 +9,7 @@ import plain_vocabulary as plain
 from nano_nccl_b200 import ops
 from test_cpu_vocabulary_ops import LL, VocabularyLoss
 from test_gpu_linear8 import replaced
-from test_gpu_vocabulary_loss import DTYPES, cross_entropy, distillation, gen, inputs, made_with_the_loss, run, teacher
+from test_gpu_vocabulary_loss import DTYPES, cross_entropy, distillation, gen, inputs, made_with_the_loss, normal, run, teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -233,6 +233,36 @@ def test_a_loss_that_makes_no_gradients_allocates_none():
     loss = ops.linear_cross_entropy(x, w, t)
     assert torch.cuda.max_memory_allocated() - before < w.numel() * 2 / 4
     assert loss.isfinite()
+
+
+def test_exponentials_of_a_vocabulary_that_is_too_large_are_not_kept():
+    """256 rows of them would be 1.5 GB: such a loss makes its gradients by pieces of the vocabulary."""
+    rows, v, h = 256, 3_000_000, 16
+    w, x = normal((v, h), torch.bfloat16, 1, 0.5), normal((rows, h), torch.bfloat16, 2)
+    t = torch.randint(0, v, (rows,), device="cuda", generator=gen(3))
+    assert made_with_the_loss(x[:64], w, t[:64])
+    x, w = x.requires_grad_(), w.requires_grad_()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    loss = ops.linear_cross_entropy(x, w, t)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert torch.cuda.max_memory_allocated() - before < 1 << 30
+    want, exact = 0.0, torch.zeros(rows, h, dtype=torch.float64, device="cuda")
+    off = torch.zeros_like(exact)
+    m = w.detach().double()
+    for at in range(0, rows, 32):
+        z = x.detach()[at:at + 32].double() @ m.t()
+        lse = torch.logsumexp(z, -1, keepdim=True)
+        want += float((lse - z.gather(1, t[at:at + 32, None])).sum()) / rows
+        p = torch.exp(z - lse).scatter_add_(1, t[at:at + 32, None], -torch.ones(32, 1, dtype=torch.float64, device="cuda")) / rows
+        exact[at:at + 32] = p @ m
+        off[at:at + 32] = p.abs() @ m.abs()
+    assert abs(float(loss) - want) <= 2.0 ** -18 * want
+    # P's rounding, the result's, and what 32-bit sums of three million words lose.
+    assert ((dx.double() - exact).abs() <= 2.0 ** -8 * exact.abs() + (2.0 ** -8 + 2.0 ** -9) * off).all()
+    assert dw.isfinite().all()
 
 
 # ---- the model, large enough for gradients that are made with the loss -----------------------------------
