@@ -1,4 +1,5 @@
 """Losses over a vocabulary: what one row is must not reach another's loss or gradient, and the ways that a call may take are each held to what that way may lose."""
+import copy
 import ctypes
 
 import pytest
@@ -7,6 +8,8 @@ import torch
 import nano_nccl_b200 as nn
 import plain_vocabulary as plain
 from nano_nccl_b200 import ops
+from nano_nccl_b200.models import TinyGPT2
+from nano_nccl_b200.parallel import CclBackend, DistributedDataParallel
 from test_cpu_vocabulary_ops import LL, VocabularyLoss
 from test_gpu_linear8 import replaced
 from test_gpu_vocabulary_loss import DTYPES, cross_entropy, distillation, gen, inputs, made_with_the_loss, normal, run, teacher
@@ -153,6 +156,17 @@ def test_gradients_of_few_rows_over_a_large_vocabulary(dtype, rows, vocabulary, 
     loses_its_own_rounding(out, plain.losses(x, w, t, reduction="none", dloss=dloss), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocabulary,width", [(5, 257, 64), (129, 255, 65), (300, 5000, 72), (1000, 700, 1003), (33, 20011, 80), (513, 1025, 392)])
+def test_gradients_of_small_products_lose_their_own_rounding_alone(dtype, rows, vocabulary, width):
+    x, w, t = inputs(rows, vocabulary, width, dtype)
+    logits, tokens = teacher(rows, 4, vocabulary, dtype)
+    assert not made_with_the_loss(x, w, t)
+    one = torch.ones((), device="cuda")
+    for targets, kind, call in ((t, None, cross_entropy(t, "mean")), (tokens, logits, distillation(logits, tokens, 1.0, "sum"))):
+        loses_its_own_rounding(run(call, x, w, one), plain.losses(x, w, targets, kind, reduction="mean" if kind is None else "sum", dloss=one), dtype)
+
+
 def test_gradients_of_few_rows_made_with_the_loss():
     """One loss for all rows, few of them: the exponentials are rounded once, what is divided by their sums is not."""
     rows, v, h = 12, 152064, 1024
@@ -267,7 +281,60 @@ def test_exponentials_of_a_vocabulary_that_is_too_large_are_not_kept():
 
 # ---- the model, large enough for gradients that are made with the loss -----------------------------------
 
+def large_model():
+    torch.manual_seed(0)
+    model = TinyGPT2(vocab=50257, context=40, hidden=768, layers=1, heads=12, vocabulary="fused").cuda()
+    with torch.no_grad():
+        model.wte.weight.mul_(0.05)
+    g = torch.Generator().manual_seed(1)
+    tokens, targets = (torch.randint(0, 50257, (3, 40), generator=g).cuda() for _ in range(2))
+    targets[0, 30:] = -1
+    return model, tokens, targets
+
 
 def counted(calls):
     prototype = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
     return replaced("b2_vocabulary_loss_both", prototype, lambda original, *arguments: calls.append(1) or original(*arguments))
+
+
+def test_a_large_model_under_autocast():
+    model, tokens, targets = large_model()
+    seen, calls = [], []
+
+    def keep(module, arguments, output):
+        output.retain_grad()
+        seen.append(output)
+
+    model.ln_f.register_forward_hook(keep)
+    with counted(calls):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = model(tokens, targets)
+        loss.backward()
+    assert len(calls) == 1
+    x, w, one = seen[0].detach().bfloat16().view(120, 768), model.wte.weight.detach().bfloat16(), torch.ones((), device="cuda")
+    want = plain.losses(x, w, targets.view(-1), dloss=one)
+    plain.within(loss, want["loss"], "loss")
+    plain.within(seen[0].grad.bfloat16().view(120, 768), want["dx"], "dx")  # (a 16-bit gradient, cast to 32 bits)
+    untouched = torch.ones(50257, dtype=torch.bool, device="cuda")
+    untouched[tokens.view(-1)] = False  # rows of the tied matrix that were not looked up: the loss's gradient alone
+    value, bound = want["dw"]
+    plain.within(model.wte.weight.grad[untouched].bfloat16(), (value[untouched], bound[untouched]), "dw")
+    assert all(p.grad.isfinite().all() for p in model.parameters())
+
+
+def test_a_large_model_under_the_data_parallel_wrapper():
+    torch.cuda.set_device(0)
+    comm = nn.Communicator(devices=[0], wait_timeout_ms=2000)
+    model, tokens, targets = large_model()
+    alone, calls = copy.deepcopy(model), []
+    with counted(calls), torch.autocast("cuda", dtype=torch.bfloat16):
+        alone(tokens, targets).backward()
+        ddp = DistributedDataParallel(model, CclBackend(comm))
+        ddp.zero_grad()
+        ddp(tokens, targets).backward()
+        ddp.finish()
+    torch.cuda.synchronize()
+    assert len(calls) == 2
+    for p, q in zip(model.parameters(), alone.parameters()):
+        assert torch.equal(p.grad, q.grad)
+    comm.close()
