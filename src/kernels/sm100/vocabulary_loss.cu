@@ -25,8 +25,8 @@
 // P is the operand of two products and therefore of their type: its rounding (2^-8 of each
 // element in bf16) is what the gradients lose beside their own. r_t = c_t / max |c| is 1 in a mean or a sum, so that the target's element
 // stays -(1 - q); max |c| is multiplied in 32 bits at the end. fp16 has no exponents for a small q: P is 2^14 times as large there. Nor has it any for rows whose c is far below the largest: where
-// rows have weights of their own, fp16 and fp32 leave the power of two of c out of P. The gradient of x takes it at the end, that of w with x, which is laid out once more (777 x 32003 x 1003 in fp16: 311 -> 322 us,
-// 128 x 512 x 64 78 -> 84).
+// rows have weights of their own, fp16 and fp32 leave the power of two of c out of P. The gradient of x takes it at the end, that of w with x, which is laid out once more (777 x 32003 x 1003 in fp16: 311 -> 318 us,
+// 128 x 512 x 64 78 -> 81).
 //
 // fp32: x, w and P are sums of two fp16 matrices each, what fp16 makes of an element and what it makes of the rest, after a power of two that brings the largest
 // element to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
@@ -1107,48 +1107,38 @@ struct HeaderArgs {
     unsigned rows;
     bool each;           // loss_grad has an element for each row
     float* powers;       // of each row's c, or null
-    const unsigned* magnitudes;  // the largest of each row of x, where the gradient of w takes it apart; or null
     float temperature;
     float* header;
 };
 
-// max |c| of the rows, of those that are numbers; c itself where they share it, 1 where P has no powers of two of theirs. The power of two for x in the gradient of w, of the rows that count.
+// The first three numbers of a gradient's header: max |c| of the rows, of those that are numbers, c itself where they share it, 1 where P has no powers of two of theirs; nothing went wrong; x as it is.
+__device__ __forceinline__ void write_header(const HeaderArgs& a, unsigned most) {
+    if (!a.each) a.header[0] = a.loss_grad[0] * a.temperature / (a.count != nullptr ? fmaxf(*a.count, 1.0f) : 1.0f);
+    else a.header[0] = a.powers != nullptr ? 1.0f : __uint_as_float(most);
+    a.header[1] = 0.0f;
+    a.header[2] = 1.0f;
+}
+
 __global__ void __launch_bounds__(1024) header_kernel(const __grid_constant__ HeaderArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int kNone = -1000;
-    unsigned most = 0;       // (of magnitudes as whole numbers: infinity and NaN are above all others)
-    int exponent_x = kNone;  // of the largest element of x times its row's power
-    if (a.each || a.magnitudes != nullptr) {
+    unsigned most = 0;  // (of magnitudes as whole numbers: infinity and NaN are above all others)
+    if (a.each) {
 #pragma unroll 4
         for (unsigned i = threadIdx.x; i < a.rows; i += 1024u) {
-            const float c = a.each ? a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature : 1.0f, power = a.powers != nullptr ? power_of(c) : 1.0f;
+            const float c = a.loss_grad[(long long)i * a.loss_grad_stride] * a.temperature;
             const unsigned bits = __float_as_uint(c) & 0x7fffffffu;
-            const bool counts = a.valid[i] != 0.0f && bits < 0x7f800000u && bits != 0u;
-            most = max(most, counts ? bits : 0u);
-            if (a.powers != nullptr) a.powers[i] = power;
-            const unsigned x = a.magnitudes != nullptr ? a.magnitudes[i] : 0u;
-            if (counts && x != 0u) exponent_x = max(exponent_x, (int)(x >> 23) + (int)(__float_as_uint(power) >> 23) - 254);
+            most = max(most, a.valid[i] == 0.0f || bits >= 0x7f800000u ? 0u : bits);
+            if (a.powers != nullptr) a.powers[i] = power_of(c);
         }
     }
     __shared__ unsigned all[32];
-    __shared__ int all_x[32];
     most = __reduce_max_sync(0xffffffffu, most);
-    exponent_x = __reduce_max_sync(0xffffffffu, exponent_x);
-    if ((threadIdx.x & 31u) == 0) {
-        all[threadIdx.x / 32u] = most;
-        all_x[threadIdx.x / 32u] = exponent_x;
-    }
+    if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = most;
     __syncthreads();
     if (threadIdx.x >= 32u) return;
     most = __reduce_max_sync(0xffffffffu, all[threadIdx.x]);
-    exponent_x = __reduce_max_sync(0xffffffffu, all_x[threadIdx.x]);
-    if (threadIdx.x == 0) {
-        if (!a.each) a.header[0] = a.loss_grad[0] * a.temperature / (a.count != nullptr ? fmaxf(*a.count, 1.0f) : 1.0f);
-        else a.header[0] = a.powers != nullptr ? 1.0f : __uint_as_float(most);
-        a.header[1] = 0.0f;
-        a.header[2] = exponent_x == kNone ? 1.0f : ldexpf(1.0f, min(max(exponent_x - 14, -126), 127));
-    }
+    if (threadIdx.x == 0) write_header(a, most);
 }
 
 // Both at once: the rows' sums, their losses, what their gradients are divided by, and E of the targets.
@@ -1430,22 +1420,20 @@ struct MagnitudeArgs {
     Matrix x, w;
     unsigned* rows;     // of each row of x
     unsigned* partial;  // of each CTA's part of w
-    unsigned ctas_of_w;
 };
 
 // The largest magnitudes. A warp takes a row of x; a thread eight elements of w at a time.
-template <typename T>
 __global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ MagnitudeArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     unsigned most = 0;
     float f[8];
-    if (blockIdx.x >= a.ctas_of_w) {
-        const unsigned row = (blockIdx.x - a.ctas_of_w) * 16u + threadIdx.x / 32u;
+    if (blockIdx.x >= kMagnitudeCtas) {
+        const unsigned row = (blockIdx.x - kMagnitudeCtas) * 16u + threadIdx.x / 32u;
         if (row >= a.x.rows) return;
 #pragma unroll 4
         for (unsigned n = threadIdx.x % 32u * 8u; n < a.x.columns; n += 256u) {
-            load_eight<T>(a.x, row, n, f);
+            load_eight<float>(a.x, row, n, f);
             most = max(most, largest_of(f));
         }
         most = __reduce_max_sync(0xffffffffu, most);
@@ -1456,7 +1444,7 @@ __global__ void __launch_bounds__(512) magnitude_kernel(const __grid_constant__ 
 #pragma unroll 4
     for (unsigned at = blockIdx.x * 512u + threadIdx.x; at < eights; at += kMagnitudeCtas * 512u) {
         const unsigned row = a.w.eights.divide(at);
-        load_eight<T>(a.w, row, (at - row * a.w.eights.d) * 8u, f);
+        load_eight<float>(a.w, row, (at - row * a.w.eights.d) * 8u, f);
         most = max(most, largest_of(f));
     }
     most = __reduce_max_sync(0xffffffffu, most);
@@ -1505,26 +1493,83 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Spli
     if (there) store_split<float>(of_x ? a.x_out : a.w_out, i, (u64)m.rows * m.eights.d, f, scale_of(magnitude, false));
 }
 
+constexpr unsigned kPowersCtas = 256;
+constexpr int kNoExponent = -1000;
+
+struct PowersArgs {
+    HeaderArgs header;
+    Matrix x;
+    const unsigned* magnitudes;  // fp32: of each row of x
+    int* partial;                // of each CTA
+};
+
+// header_kernel's work where the gradient of w takes x apart, and the exponent of the largest element of x times its row's power, of the rows that count. A warp takes a row.
+template <typename T>
+__global__ void __launch_bounds__(512) powers_kernel(const __grid_constant__ PowersArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const HeaderArgs& h = a.header;
+    const unsigned lane = threadIdx.x % 32u;
+    int exponent = kNoExponent;
+    for (unsigned row = blockIdx.x * 16u + threadIdx.x / 32u; row < a.x.rows; row += gridDim.x * 16u) {
+        unsigned most = 0;
+        if constexpr (sizeof(T) == 4) {
+            most = a.magnitudes[row];
+        } else {
+            float f[8];
+#pragma unroll 4
+            for (unsigned n = lane * 8u; n < a.x.columns; n += 256u) {
+                load_eight<T>(a.x, row, n, f);
+                most = max(most, largest_of(f));
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+        }
+        const float c = h.each ? h.loss_grad[(long long)row * h.loss_grad_stride] * h.temperature : 1.0f, power = h.powers != nullptr ? power_of(c) : 1.0f;
+        if (h.powers != nullptr && lane == 0) h.powers[row] = power;
+        const bool counts = h.valid[row] != 0.0f && c != 0.0f && fabsf(c) < __int_as_float(0x7f800000) && most != 0u;
+        if (counts) exponent = max(exponent, (int)(most >> 23) + (int)(__float_as_uint(power) >> 23) - 254);
+    }
+    __shared__ int all[16];
+    if (lane == 0) all[threadIdx.x / 32u] = exponent;
+    __syncthreads();
+    if (threadIdx.x >= 32u) return;
+    exponent = __reduce_max_sync(0xffffffffu, all[lane % 16u]);
+    if (lane != 0) return;
+    a.partial[blockIdx.x] = exponent;
+    if (blockIdx.x == 0) write_header(h, 0u);
+}
+
 struct WeighArgs {
     Matrix x;
     char* out;  // [parts][rows][pitch]
     const float* valid;
     const float* powers;  // of each row, or null
-    const float* header;
+    const int* partial;   // of powers_kernel
+    unsigned partials;
+    float* header;
 };
 
-// x as the gradient of w takes it: times the power of two of each row's c and one for all rows, zeros for rows that do not count.
+// x as the gradient of w takes it: times the power of two of each row's c and one for all rows, zeros for rows that do not count. A thread takes eight elements.
 template <typename T>
 __global__ void __launch_bounds__(256) weigh_kernel(const __grid_constant__ WeighArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    static_assert(kPowersCtas == 256);
     const unsigned i = blockIdx.x * 256u + threadIdx.x, row = a.x.eights.divide(i);
-    if (row >= a.x.rows) return;
     float f[8] = {};
-    if (a.valid[row] != 0.0f) load_eight<T>(a.x, row, (i - row * a.x.eights.d) * 8u, f);
+    if (row < a.x.rows && a.valid[row] != 0.0f) load_eight<T>(a.x, row, (i - row * a.x.eights.d) * 8u, f);
+    __shared__ int all[8];
+    int exponent = __reduce_max_sync(0xffffffffu, threadIdx.x < a.partials ? a.partial[threadIdx.x] : kNoExponent);
+    if ((threadIdx.x & 31u) == 0) all[threadIdx.x / 32u] = exponent;
+    __syncthreads();
+#pragma unroll
+    for (unsigned w = 0; w < 8; ++w) exponent = max(exponent, all[w]);
+    const int back = exponent == kNoExponent ? 0 : min(max(exponent - 14, -126), 127);
+    if (i == 0) a.header[2] = ldexpf(1.0f, back);
+    if (row >= a.x.rows) return;
     // (Powers may be further apart than floats reach: a row whose largest element is below 2^-112 stays smaller, and what is 2^-149 of another's is nothing beside it.)
-    const int power = a.powers != nullptr ? (int)(__float_as_uint(a.powers[row]) >> 23) : 127, back = ilogbf(a.header[2]);
-    store_split<T>(a.out, i, (u64)a.x.rows * a.x.eights.d, f, ldexpf(1.0f, min(power - 127 - back, 126)));
+    const int power = a.powers != nullptr ? (int)(__float_as_uint(a.powers[row]) >> 23) - 127 : 0;
+    store_split<T>(a.out, i, (u64)a.x.rows * a.x.eights.d, f, ldexpf(1.0f, min(power - back, 126)));
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
@@ -1640,7 +1685,7 @@ struct Plan {
     u64 rows = 0;                // both at once: of a piece
     std::size_t exps_pitch = 0;
     unsigned n_tile = kTile;
-    std::size_t scale_at = 0, divided_at = 0, weighed_at = 0, powers_at = 0, magnitudes_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
+    std::size_t scale_at = 0, divided_at = 0, weighed_at = 0, powers_at = 0, x_at = 0, weight_at = 0, stats_at = 0, picked_at = 0, losses_at = 0, partial_at = 0, header_at = 0, probs_at = 0, sums_at = 0, slots_at = 0, bytes = 0;
 };
 
 // Both at once: bytes of E in a piece of the rows, and of the sums of dw where there are several. (8192 x 50257 x 768, loss and gradients: 1459 us in one piece of 824 MB, 1565 in two,
@@ -1735,7 +1780,7 @@ Plan plan_of(const VocabularyLossCall& c, Pass pass) {
         p.header_at = take(3 * sizeof(float));
         p.weighed_at = take(weighed(c) ? p.parts * t * p.pitch * 2 : 0);
         p.powers_at = take(powers_apart(c) ? t * sizeof(float) : 0);
-        p.magnitudes_at = take(weighed(c) && c.dtype == DType::Float16 ? t * sizeof(unsigned) : 0);
+        p.partial_at = take(weighed(c) ? kPowersCtas * sizeof(int) : 0);
         p.probs_at = take(bytes * p.piece);
         const u64 rest = v - (p.pieces - 1) * p.piece;
         if (c.x_grad != nullptr && p.pieces > 1)
@@ -1859,7 +1904,6 @@ constexpr const char* kTooLarge = "an operand is too large for one call";
 Matrix x_of(const VocabularyLossCall& c, const Plan& p) {
     return {static_cast<const char*>(c.x), c.x_stride * (long long)dtype_size(c.dtype), (unsigned)c.tokens, (unsigned)c.width, Divisor((unsigned)(p.pitch / 8))};
 }
-unsigned magnitude_ctas(const VocabularyLossCall& c) { return (unsigned)((c.tokens + 15) / 16); }
 
 // x and the matrix as the tensor cores read them, copied where they have to be. known: fp32's magnitudes are, from the forward pass.
 template <typename T>
@@ -1889,8 +1933,8 @@ void operands(const VocabularyLossCall& c, const Plan& p, bool known, Operand* x
         s.partial = nullptr;
         s.w_magnitude = kept.w_magnitude;
         if (!known) {
-            const MagnitudeArgs a = {s.x, s.w, kept.magnitudes, reinterpret_cast<unsigned*>(workspace + p.partial_at), kMagnitudeCtas};
-            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel<float>, dim3(kMagnitudeCtas + magnitude_ctas(c)), 512, 0, c.stream, a));
+            const MagnitudeArgs a = {s.x, s.w, kept.magnitudes, reinterpret_cast<unsigned*>(workspace + p.partial_at)};
+            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel, dim3(kMagnitudeCtas + (unsigned)((c.tokens + 15) / 16)), 512, 0, c.stream, a));
             s.partial = a.partial;
         }
         B2_CUDA(launch_dependent<SplitArgs>(split_kernel, dim3(s.ctas_of_x + (unsigned)((w_eights + 255) / 256)), 256, 0, c.stream, s));
@@ -2007,14 +2051,6 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
     const bool each = c.reduction == LossReduction::None, apart = !std::is_same_v<T, __nv_bfloat16> && weighed(c);
     float* header = reinterpret_cast<float*>(workspace + p.header_at);
     float* powers = powers_apart(c) ? reinterpret_cast<float*>(workspace + p.powers_at) : nullptr;
-    const unsigned* magnitudes = apart ? kept.magnitudes : nullptr;
-    if constexpr (std::is_same_v<T, __half>) {
-        if (apart) {
-            unsigned* rows = reinterpret_cast<unsigned*>(workspace + p.magnitudes_at);
-            B2_CUDA(launch_dependent<MagnitudeArgs>(magnitude_kernel<T>, dim3(magnitude_ctas(c)), 512, 0, c.stream, MagnitudeArgs{x_of(c, p), {}, rows, nullptr, 0}));
-            magnitudes = rows;
-        }
-    }
     HeaderArgs h;
     h.loss_grad = c.loss_grad;
     h.loss_grad_stride = c.loss_grad_stride;
@@ -2023,16 +2059,19 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
     h.rows = (unsigned)c.tokens;
     h.each = each;
     h.powers = powers;
-    h.magnitudes = magnitudes;
     h.temperature = c.temperature;
     h.header = header;
-    B2_CUDA(launch_dependent<HeaderArgs>(header_kernel, dim3(1), 1024, 0, c.stream, h));
+    int* partial = reinterpret_cast<int*>(workspace + p.partial_at);
+    const unsigned partials = (unsigned)std::min<std::size_t>(kPowersCtas, (c.tokens + 15) / 16);
+    if (!apart) B2_CUDA(launch_dependent<HeaderArgs>(header_kernel, dim3(1), 1024, 0, c.stream, h));
+    if constexpr (!std::is_same_v<T, __nv_bfloat16>)
+        if (apart) B2_CUDA(launch_dependent<PowersArgs>(powers_kernel<T>, dim3(partials), 512, 0, c.stream, PowersArgs{h, x_of(c, p), kept.magnitudes, partial}));
     Operand x, w;
     operands<T>(c, p, true, &x, &w);
     Operand weighed_x = x;
     if constexpr (!std::is_same_v<T, __nv_bfloat16>) {
         if (apart) {
-            const WeighArgs e = {x_of(c, p), workspace + p.weighed_at, kept.valid, powers, header};
+            const WeighArgs e = {x_of(c, p), workspace + p.weighed_at, kept.valid, powers, partial, partials, header};
             const u64 eights = (u64)c.tokens * (p.pitch / 8);
             B2_REQUIRE(eights < (1ull << 31), kTooLarge);
             B2_CUDA(launch_dependent<WeighArgs>(weigh_kernel<T>, dim3((unsigned)((eights + 255) / 256)), 256, 0, c.stream, e));

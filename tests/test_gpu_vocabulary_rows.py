@@ -136,6 +136,57 @@ def test_weights_at_the_ends_of_their_range(dtype):
         each_row_alone(out, x, w, t, dloss, (5, 6))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_with_weights_of_their_own(dtype):
+    """More rows than are looked at at once, the largest weight at their end; only one of the gradients."""
+    rows = 9001
+    x, w, t = inputs(rows, 300, 72, dtype)
+    dloss = 10.0 ** (-4 * torch.rand(rows, device="cuda", generator=gen(5)))
+    dloss[-1], t[-1] = 30.0, 7
+    out, want = run(cross_entropy(t, "none"), x, w, dloss), plain.losses(x, w, t, reduction="none", dloss=dloss)
+    for name in want:
+        plain.within(out[name], want[name], name)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(ops.linear_cross_entropy(a, w, t, reduction="none"), a, dloss)
+    (dw,) = torch.autograd.grad(ops.linear_cross_entropy(x, b, t, reduction="none"), b, dloss)
+    assert torch.equal(dx, out["dx"]) and torch.equal(dw, out["dw"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_graphs_of_losses_of_each_row(dtype):
+    """Two graphs at once, replayed with other rows, weights and targets than they were captured with, beside eager calls on a third stream."""
+    rows, v, h = 150, 2000, 136
+    states, streams = [], [torch.cuda.Stream() for _ in range(3)]
+    for i, s in enumerate(streams):
+        x, w, t = inputs(rows, v, h, dtype, seed=10 * i)
+        back = torch.ones(rows, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            run(cross_entropy(t, "none"), x, w, back)
+        torch.cuda.synchronize()
+        graph, out = torch.cuda.CUDAGraph(), None
+        if i < 2:
+            with torch.cuda.graph(graph, stream=s):
+                out = run(cross_entropy(t, "none"), x, w, back)
+        states.append((graph, x, w, t, back, out))
+    for turn in range(3):
+        for i, (_, x, w, t, back, _) in enumerate(states):
+            other, _, targets = inputs(rows, v, h, dtype, seed=100 * turn + i)
+            x.copy_(other * 10.0 ** turn)
+            t.copy_(targets)
+            back.copy_(10.0 ** (-3 * turn * torch.rand(rows, device="cuda", generator=gen(turn))))
+        want = [run(cross_entropy(t, "none"), x, w, back) for _, x, w, t, back, _ in states]
+        torch.cuda.synchronize()
+        for s, state in zip(streams[:2], states):
+            with torch.cuda.stream(s):
+                state[0].replay()
+        with torch.cuda.stream(streams[2]):
+            third = run(cross_entropy(states[2][3], "none"), *states[2][1:3], states[2][4])
+        torch.cuda.synchronize()
+        for got, expected in zip((states[0][5], states[1][5], third), want):
+            assert all(torch.equal(got[name], expected[name]) for name in expected)
+
+
 # ---- which way a call takes, and what it may lose there --------------------------------------------------
 
 def loses_its_own_rounding(out, want, dtype, what=""):
@@ -273,7 +324,7 @@ def test_exponentials_of_a_vocabulary_that_is_too_large_are_not_kept():
         p = torch.exp(z - lse).scatter_add_(1, t[at:at + 32, None], -torch.ones(32, 1, dtype=torch.float64, device="cuda")) / rows
         exact[at:at + 32] = p @ m
         off[at:at + 32] = p.abs() @ m.abs()
-    assert abs(float(loss) - want) <= 2.0 ** -18 * want
+    assert abs(float(loss.detach()) - want) <= 2.0 ** -18 * want
     # P's rounding, the result's, and what 32-bit sums of three million words lose.
     assert ((dx.double() - exact).abs() <= 2.0 ** -8 * exact.abs() + (2.0 ** -8 + 2.0 ** -9) * off).all()
     assert dw.isfinite().all()
