@@ -31,7 +31,8 @@
 // fp32: x, w and P are sums of two fp16 matrices each, what fp16 makes of an element and what it makes of the rest, after a power of two that brings the largest
 // element to 2^14: 22 bits, of elements down to 2^-28 of the largest (which stands for 2^-39 in those below). Three products of the four give theirs; the fourth is 2^-22 of
 // it. For logits each row of x has a power of its own, so that no row's loss or gradient depends on how large another is; the gradient of w, which is a sum over rows, takes x
-// with one power for all rows that count, laid out a second time (2048 x 768: 3 us). (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 1760.)
+// with one power for all rows that count, laid out a second time (2048 x 768: 6 us).
+// (Three bf16 matrices have 24 bits, of any element, and take six products: 2048 x 50257 x 768, loss and gradients, 3362 us, with these 1850.)
 // The tensor cores cut what an addition leaves below 24 bits, so the small products come first, and their sums are added up in registers, rounded, after every 256 to 8192
 // elements of the summed axis: a loss over columns of 4096 in bf16 is 1.8e-6 off otherwise, all of it in one direction.
 //
@@ -1541,7 +1542,8 @@ __global__ void __launch_bounds__(512) powers_kernel(const __grid_constant__ Pow
 
 struct WeighArgs {
     Matrix x;
-    char* out;  // [parts][rows][pitch]
+    char* out;   // [parts][rows][pitch], from the first of x's rows on
+    u64 apart;   // sixteens of bytes from part to part
     const float* valid;
     const float* powers;  // of each row, or null
     const int* partial;   // of powers_kernel
@@ -1569,7 +1571,7 @@ __global__ void __launch_bounds__(256) weigh_kernel(const __grid_constant__ Weig
     if (row >= a.x.rows) return;
     // (Powers may be further apart than floats reach: a row whose largest element is below 2^-112 stays smaller, and what is 2^-149 of another's is nothing beside it.)
     const int power = a.powers != nullptr ? (int)(__float_as_uint(a.powers[row]) >> 23) - 127 : 0;
-    store_split<T>(a.out, i, (u64)a.x.rows * a.x.eights.d, f, ldexpf(1.0f, min(power - back, 126)));
+    store_split<T>(a.out, i, a.apart, f, ldexpf(1.0f, min(power - back, 126)));
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
@@ -2071,11 +2073,15 @@ void gradient(const VocabularyLossCall& c, const Plan& p) {
     Operand weighed_x = x;
     if constexpr (!std::is_same_v<T, __nv_bfloat16>) {
         if (apart) {
-            const WeighArgs e = {x_of(c, p), workspace + p.weighed_at, kept.valid, powers, partial, partials, header};
-            const u64 eights = (u64)c.tokens * (p.pitch / 8);
-            B2_REQUIRE(eights < (1ull << 31), kTooLarge);
-            B2_CUDA(launch_dependent<WeighArgs>(weigh_kernel<T>, dim3((unsigned)((eights + 255) / 256)), 256, 0, c.stream, e));
-            weighed_x = {e.out, c.width, c.tokens, p.pitch * 2};
+            const u64 eights = p.pitch / 8, most = (1ull << 30) / eights;  // rows of a launch
+            for (u64 first = 0; first < c.tokens; first += most) {
+                WeighArgs e = {x_of(c, p), workspace + p.weighed_at + first * p.pitch * 2, c.tokens * eights, kept.valid + first, powers, partial, partials, header};
+                e.x.from += (long long)first * e.x.stride;
+                e.x.rows = (unsigned)std::min<u64>(most, c.tokens - first);
+                if (powers != nullptr) e.powers += first;
+                B2_CUDA(launch_dependent<WeighArgs>(weigh_kernel<T>, dim3((unsigned)((e.x.rows * eights + 255) / 256)), 256, 0, c.stream, e));
+            }
+            weighed_x = {workspace + p.weighed_at, c.width, c.tokens, p.pitch * 2};
         }
     }
     char* probs = workspace + p.probs_at;
