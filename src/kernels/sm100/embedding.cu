@@ -6,7 +6,7 @@
 //
 // Sorting (sort_kernel) is a matter of latency: a cluster of eight CTAs sorts by eight bits at a time, counts and places of its 256 warps in shared memory and
 // between the CTAs through distributed shared memory. Meanwhile the rest of the GPU fills the gradient with zeros (fill_kernel), which takes longer where the
-// matrix is large beside the tokens, so that sorting is free (50257 x 768 in bf16: up to 32768 tokens; 131072 take 197 us, 1048576 1130, most of it the sort). (A CTA of few stores for each 64 KiB: 1.07 GB in 145 us, a loop in as many CTAs as run at once 170 us.)
+// matrix is large beside the tokens, so that sorting is free (50257 x 768 in bf16: up to 32768 tokens; 131072 take 197 us, 1048576 1130, of which the sort is 600). (A CTA of few stores for each 64 KiB: 1.07 GB in 145 us, a loop in as many CTAs as run at once 170 us.)
 // Adding (sum_kernel): the list is cut into chunks, and a group of threads goes through one, 16 bytes of a row for each thread. A token whose rows lie in one chunk is
 // written at once. What crosses a chunk's ends is written as sums of 32 bits, and join_kernel adds them: a token may have any share of the rows.
 #include "kernels/sm100/embedding.h"
