@@ -124,6 +124,8 @@ class TinyGPT2(torch.nn.Module):
     are. ``vocabulary``: "fused" looks tokens up, and makes losses, without logits in memory (:mod:`nano_nccl_b200.ops.vocabulary`; negative tokens are padding),
     "plain" by torch's own. All but the defaults run on CUDA only (:mod:`nano_nccl_b200.ops`)."""
 
+    vocabulary = "plain"  # of modules that were pickled before there was a choice
+
     def __init__(self, vocab=512, context=64, hidden=64, layers=2, heads=4, positions="learned", qk_norm=False, checkpoints=None, vocabulary="plain"):
         super().__init__()
         if positions not in ("learned", "rotary"):
