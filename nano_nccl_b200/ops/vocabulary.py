@@ -42,7 +42,8 @@ def linear_cross_entropy(x, weight, targets, reduction="mean"):
     and ``weight``, which are the same. Under autocast both are cast as those of ``linear``.
 
     What the logits lose is what 32-bit sums lose; the gradient of the logits is rounded to the type of ``x`` before it is multiplied. float32: operands have 22 bits, or where that is
-    more 2^-39 of the largest element of ``weight``, of the row of ``x`` (in the gradient of ``weight``: of the rows of ``x`` that count, times their weights in the loss), and of 1 in the softmax."""
+    more 2^-39 of the largest element of ``weight``, of the row of ``x`` (in the gradient of ``weight``: of the rows of ``x`` that count, times their weights in the loss), and of 1 in the softmax.
+    float16, a loss of each row: the gradient of ``weight`` takes ``x`` times a power of two of its row's weight, exactly, down to 2^-28 of the largest such element."""
     return load_native_calls().linear_cross_entropy(x, weight, targets, _reduction(reduction))
 
 
